@@ -369,6 +369,120 @@ int skv_irap_importance(const float* scores, int B, int H, int Sq, int Sk, int i
                         void* scratch, size_t scratch_bytes, float* importance, float* ema, double* delta_parts,
                         void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Serving over a page pool: rotary positions, the append that quantises as it writes, the read
+ * back, and the attention of new tokens.  No counterpart in the reference, whose paged store
+ * (shadowinfer/shadowkv/paged_kv_store.py) holds equal-length batches and hands attention a
+ * dense gather; the page rows and scales are that store's, bit for bit.
+ *
+ * A pool holds the pages of many sequences of different lengths: payload [num_pages, heads,
+ * page_size, row] (row as for the paged store, by precision) and float scales [num_pages, heads,
+ * page_size] (int8) or [num_pages, heads, page_size, D/G] (int4); token t of sequence b is row
+ * t % page_size of page block_table[b][t / page_size].  Lengths and tables are DEVICE memory, so
+ * nothing here waits for the host and every call can be captured in a graph.  A page number
+ * outside [0, num_pages), a token past the table's width or a position past the rotary tables is
+ * never followed: the row is not written / not attended to / zero when read / NaN when rotated,
+ * and *error_flag (device int32, where not NULL) is set to 1.
+ * ------------------------------------------------------------------------------------- */
+typedef struct skv_pool {
+    void* k;                     /* K pages */
+    void* v;                     /* V pages */
+    float* scale_k;              /* NULL for fp32 / fp16 */
+    float* scale_v;
+    const int32_t* block_table;  /* [batch, table_width] */
+    int64_t table_stride;        /* int32 values from one sequence's row to the next */
+    int32_t table_width;
+    int32_t num_pages;
+    int32_t page_size;
+    int32_t heads;
+    int32_t head_dim;
+    int32_t int4_group;          /* values per int4 scale (divides head_dim) */
+    int32_t precision;           /* 0 fp32, 1 fp16, 2 int8, 3 int4 */
+    int32_t batch;
+} skv_pool;                      /* 80 bytes */
+
+/* Rows [batch, heads, tokens, D] with D contiguous values: strides in values. */
+typedef struct skv_rows {
+    void* ptr;
+    int64_t stride_b, stride_h, stride_s;
+    int32_t dtype;               /* 0 fp32, 1 fp16, 2 bf16 */
+    int32_t heads;               /* 0: absent */
+} skv_rows;                      /* 40 bytes */
+
+/* The rotary tables of a call: float cos, sin [max_positions, rot/2]; positions (device, int32
+ * or int64 by pos_bytes; NULL: the token's own index) at b * pos_stride_b + s * pos_stride_s. */
+typedef struct skv_rope {
+    const float* cos;
+    const float* sin;
+    const void* positions;
+    int64_t pos_stride_b, pos_stride_s;
+    int32_t pos_bytes;           /* 4 or 8 */
+    int32_t rot;                 /* leading values of a row that turn; 0: none */
+    int32_t max_positions;
+    int32_t interleaved;         /* pairs (2i, 2i+1) instead of (i, i + rot/2) */
+    int32_t inverse;             /* turn back: also the gradient with respect to the rows */
+    int32_t reserved;
+} skv_rope;                      /* 64 bytes */
+
+typedef struct skv_rotary_args {
+    skv_rows q, k, q_out, k_out; /* k.heads == 0: q only */
+    skv_rope rope;
+    int32_t B, S, D, reserved;
+} skv_rotary_args;
+
+/* out = rows with (a, b) -> (a cos - b sin, b cos + a sin) over the pairs of the first rot
+ * values; products and sums in fp32, each rounded, then one rounding to the rows' type. */
+int skv_rotary(const skv_rotary_args* args, void* stream);
+
+typedef struct skv_pool_append_args {
+    skv_pool pool;
+    skv_rows k, v;               /* new rows [B, heads, S, D] */
+    skv_rows q, q_out;           /* rotated queries; q.heads == 0: none */
+    skv_rope rope;               /* rot == 0: keys are stored as they are (and q must be absent) */
+    const int32_t* lengths;      /* tokens each sequence holds before the call */
+    const int32_t* new_lengths;  /* rows of each sequence that are tokens; NULL: all S */
+    int32_t* error_flag;
+    int32_t S, reserved;
+} skv_pool_append_args;
+
+/* Rows s < new_lengths[b] become tokens lengths[b] + s: the rotated key and the value, quantised
+ * per row (int8) or per group (int4) exactly like skv_paged_write.  The position of a token is
+ * its index unless rope.positions says otherwise.  All S rows of q are rotated. */
+int skv_pool_append(const skv_pool_append_args* args, void* stream);
+
+typedef struct skv_pool_read_args {
+    skv_pool pool;
+    skv_rows k_out, v_out;       /* [B, heads, S, D] */
+    const int32_t* start;        /* first token of each sequence; NULL: 0 */
+    const int32_t* lengths;      /* tokens at or past it are zero */
+    int32_t* error_flag;
+    int32_t S, reserved;
+} skv_pool_read_args;
+
+/* The values that tokens start[b] .. start[b] + S - 1 stand for. */
+int skv_pool_read(const skv_pool_read_args* args, void* stream);
+
+typedef struct skv_pool_attention_args {
+    skv_pool pool;
+    skv_rows q, out;             /* [B, H_q, S_q, D], one type; H_q a multiple of pool.heads */
+    const int32_t* lengths;      /* tokens of each sequence, the new ones included */
+    const int32_t* new_lengths;  /* queries of each sequence that are tokens; NULL: all S_q */
+    void* scratch;
+    int64_t scratch_bytes;
+    int32_t* error_flag;
+    int32_t S_q;
+    int32_t causal;              /* query i sees tokens <= lengths[b] - new_lengths[b] + i, else all */
+    float scale;
+    int32_t reserved;
+} skv_pool_attention_args;
+
+/* out = softmax(scale q k^T) v over each sequence's tokens; a query that sees no token gives 0, and so
+ * does a query i >= new_lengths[b] (the padding of a ragged batch).
+ * Query head h reads key head h / (H_q / heads).  scratch: skv_pool_attention_scratch_bytes
+ * bytes, 16-byte aligned, any contents. */
+size_t skv_pool_attention_scratch_bytes(int D);
+int skv_pool_attention(const skv_pool_attention_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -128,6 +128,12 @@ _SIGNATURES = {
     "skv_irap_importance": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, ctypes.c_double,
                                     ctypes.c_double, c_int, ctypes.c_double, c_void_p, c_size_t, c_void_p, c_void_p,
                                     c_void_p, c_void_p]),
+    # one packed argument struct each (skv_rotary_args and so on), passed as bytes
+    "skv_rotary": (c_int, [ctypes.c_char_p, c_void_p]),
+    "skv_pool_append": (c_int, [ctypes.c_char_p, c_void_p]),
+    "skv_pool_read": (c_int, [ctypes.c_char_p, c_void_p]),
+    "skv_pool_attention_scratch_bytes": (c_size_t, [c_int]),
+    "skv_pool_attention": (c_int, [ctypes.c_char_p, c_void_p]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES.keys())

@@ -1,0 +1,163 @@
+"""Rotary positions: the tables and the turn of queries and keys by their positions.
+
+The reference's models leave positions to the checkpoint's own attention module
+(shadowinfer/models/diffusion_llama.py:357-375 calls it before the cache); a serving step
+needs them next to the paged cache, which stores keys after the turn.
+"""
+
+from __future__ import annotations
+
+import math
+import struct
+from typing import Any, Optional, Tuple
+
+import torch
+
+from .. import _lib
+from .._device import as_device, back, compute_device, device_ctx
+
+_DTYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_ARGS = struct.Struct("<" + "Qqqqii" * 4 + "QQQqqiiiiii" + "iiii")   # skv_rotary_args
+assert _ARGS.size == 240
+_NO_ROWS = (0, 0, 0, 0, 0, 0)
+
+
+def rotary_tables(
+    rotary_dim: int,
+    max_positions: int,
+    base: float = 10000.0,
+    scaling: Optional[str] = None,
+    factor: float = 1.0,
+    original_positions: Optional[int] = None,
+    device: Any = "cuda",
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(cos, sin)`` float32 ``[max_positions, rotary_dim / 2]``: pair i turns by ``p * base**(-2 i / rotary_dim)``.
+
+    ``scaling`` stretches the positions a model was trained on by ``factor``:
+
+    * ``"linear"``: every frequency divided by ``factor``;
+    * ``"ntk"``: the base raised to ``base * factor ** (rotary_dim / (rotary_dim - 2))``, which leaves the
+      fastest pair as it is and divides the slowest one's frequency by ``factor``;
+    * ``"ntk_parts"``: pairs that turn over 32 times within ``original_positions`` keep their frequency, those
+      that turn less than once are divided by ``factor``, a linear ramp in between, and the
+      tables are multiplied by ``0.1 ln(factor) + 1``.
+
+    Angles are computed in 64 bits (a 32-bit angle is off by 4e-3 at position 65536).
+    """
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
+    if max_positions < 1:
+        raise ValueError(f"max_positions must be >= 1, got {max_positions}")
+    if scaling not in (None, "linear", "ntk", "ntk_parts"):
+        raise ValueError(f"unknown rotary scaling: {scaling}")
+    if factor <= 0 or (scaling == "ntk_parts" and (original_positions is None or original_positions < 1)):
+        raise ValueError("rotary scaling needs a positive factor (and original_positions for 'ntk_parts')")
+    gain = 1.0
+    if scaling == "ntk":
+        base = base * factor ** (rotary_dim / max(1, rotary_dim - 2))
+    inv = base ** (-torch.arange(rotary_dim // 2, dtype=torch.float64) * 2 / rotary_dim)
+    if scaling == "linear":
+        inv = inv / factor
+    elif scaling == "ntk_parts":
+        keep = ((original_positions * inv / (2 * math.pi) - 1.0) / (32.0 - 1.0)).clamp(0, 1)
+        inv = inv / factor * (1 - keep) + inv * keep
+        gain = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    dev = as_device(device)
+    angle = torch.arange(max_positions, dtype=torch.float64, device=dev)[:, None] * inv.to(dev)
+    return (angle.cos() * gain).float(), (angle.sin() * gain).float()
+
+
+def _as_rows(t: torch.Tensor, dev: torch.device, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``t`` [B, H, S, D] as the kernels read it: on ``dev``, fp32 / fp16 / bf16, the last dimension contiguous."""
+    if t.requires_grad:
+        t = t.detach()
+    if dtype is None:
+        dtype = t.dtype if t.dtype in _DTYPE_CODE else torch.float32
+    if t.dtype is not dtype or not t.is_cuda or t.get_device() != dev.index:
+        t = t.to(device=dev, dtype=dtype)
+    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
+
+
+def _rows_fields(t: torch.Tensor) -> Tuple[int, int, int, int, int, int]:
+    """The ``skv_rows`` fields of a tensor from ``_as_rows``."""
+    st = t.stride()
+    return (t.data_ptr(), st[0], st[1], st[2], _DTYPE_CODE[t.dtype], t.shape[1])
+
+
+def _table_checked(t: torch.Tensor, dev: torch.device, name: str) -> torch.Tensor:
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be [max_positions, rotary_dim / 2], got {tuple(t.shape)}")
+    if t.dtype is not torch.float32 or not t.is_cuda or t.get_device() != dev.index or not t.is_contiguous():
+        t = t.detach().to(device=dev, dtype=torch.float32).contiguous()
+    return t
+
+
+def _rope_fields(cos, sin, positions, B: int, S: int, D: int, interleaved: bool, inverse: bool, dev: torch.device):
+    """The ``skv_rope`` fields, and the tensors they point into (to be kept until the launch)."""
+    cos, sin = _table_checked(cos, dev, "cos"), _table_checked(sin, dev, "sin")
+    if cos.shape != sin.shape:
+        raise ValueError(f"cos/sin shapes disagree: {tuple(cos.shape)} vs {tuple(sin.shape)}")
+    rot = 2 * cos.shape[1]
+    if rot < 2 or rot > D:
+        raise ValueError(f"the tables rotate {rot} values of a head of {D}")
+    at = (0, 0, 0, 0)
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
+        if not positions.is_cuda or positions.get_device() != dev.index:
+            positions = positions.to(dev)
+        if positions.shape != (B, S):
+            try:
+                positions = positions.expand(B, S)
+            except RuntimeError:
+                raise ValueError(f"positions must broadcast to [{B}, {S}], got {tuple(positions.shape)}") from None
+        st = positions.stride()
+        at = (positions.data_ptr(), st[0], st[1], positions.element_size())
+    return ((cos.data_ptr(), sin.data_ptr(), *at, rot, cos.shape[0], bool(interleaved), bool(inverse), 0),
+            (cos, sin, positions))
+
+
+def apply_rotary(
+    q: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    k: Optional[torch.Tensor] = None,
+    positions: Optional[torch.Tensor] = None,
+    interleaved: bool = False,
+    inverse: bool = False,
+):
+    """``q`` (and ``k``) ``[B, heads, S, D]`` turned by their positions; returns ``q'``, or ``(q', k')`` with ``k``.
+
+    A pair ``(a, b)`` at position p becomes ``(a c - b s, b c + a s)`` with ``c, s = cos[p][i], sin[p][i]``.  Pairs
+    are ``(x[i], x[i + rot/2])``, or ``(x[2i], x[2i+1])`` with ``interleaved``, over the first
+    ``rot = 2 * cos.shape[1]`` values of a head; the others are copied.  ``positions``: int32 or int64, broadcast to
+    ``[B, S]`` (default: 0 .. S-1); rows whose position the tables do not hold become NaN.
+    ``inverse`` turns back, which is also the gradient with respect to the rows.
+
+    fp32, fp16 and bf16 rows are read in place with any strides over the first three dimensions
+    (slices of one projection's output, transposed views); products and sums are fp32, rounded once to the
+    rows' type.  One launch for both tensors.
+    """
+    if q.dim() != 4:
+        raise ValueError(f"q must be 4-D [batch, heads, seq, head_dim], got shape {tuple(q.shape)}")
+    B, _, S, D = q.shape
+    if k is not None and (k.dim() != 4 or (k.shape[0], k.shape[2], k.shape[3]) != (B, S, D)):
+        raise ValueError(f"q/k shapes disagree: {tuple(q.shape)} vs {tuple(k.shape)}")
+    dev = compute_device(q, k, cos)
+    qd = _as_rows(q, dev)
+    q_out = torch.empty(qd.shape, dtype=qd.dtype, device=dev)
+    if k is not None:
+        kd = _as_rows(k, dev, qd.dtype)
+        k_out = torch.empty(kd.shape, dtype=qd.dtype, device=dev)
+        k_rows, k_out_rows = _rows_fields(kd), _rows_fields(k_out)
+    else:
+        k_rows = k_out_rows = _NO_ROWS
+    rope, keep = _rope_fields(cos, sin, positions, B, S, D, interleaved, inverse, dev)
+    args = _ARGS.pack(*_rows_fields(qd), *k_rows, *_rows_fields(q_out), *k_out_rows, *rope, B, S, D, 0)
+    with device_ctx(dev):
+        st = _lib.load().skv_rotary(args, _lib.stream_of(dev))
+    _lib.check(st, "apply_rotary")
+    del keep
+    if k is None:
+        return back(q_out, q.device)
+    return back(q_out, q.device), back(k_out, k.device)
