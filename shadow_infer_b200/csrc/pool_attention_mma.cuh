@@ -1,0 +1,723 @@
+// Attention over the page pool on the tensor cores, pages read straight into MMA fragments.
+//
+// A decoding step is bound by the pages' bytes, but at 4 bits a value the FMA pipe cannot keep up with
+// HBM, and neither can one operand row a value where several query rows share a key head.  So
+// both products run as mma.m16n8k16 (fp16 operands, fp32 sums), transposed so that the few query rows
+// are the narrow side:
+//     S^T [16 tokens x 8 rows] = K [16 x D] Q^T,     O^T [16 values x 8 rows] += V^T [16 x 16 tokens] P^T.
+// (tcgen05 wants 128 rows of A in shared memory and its sums back through TMEM; with 8..32 query
+// rows the pages would pass through shared memory only to be read once.)
+//
+// The contraction order of an MMA is free as long as both operands agree, so a lane's 16-byte load of
+// a page row IS its share of the A operand: lane (g, c) = (lane / 4, lane % 4) takes chunks c, c+4, ...
+// of the rows of tokens g and g+8 (K), and the g-th chunks of tokens 2c, 2c+1, 2c+8, 2c+9 (V), whose
+// token pairs are interleaved with byte permutes.  No shared memory, no transposes of pages; the
+// queries are laid out once per segment to match.  P^T's operand is S^T's result transposed by
+// movmatrix.
+//
+// Exactness.  Page values enter the MMAs exactly: fp16 as it is, int8 and int4 as small integers.  An
+// int8 row's scale multiplies its score (K) or its weight (V) in fp32.  An int4 group's scale is split into an
+// 8-bit part r1 (times a 4-bit integer exact in fp16) and an 11-bit remainder r2, two MMAs, after a
+// power of two is taken out (per tile for K, per token for V), so range is no concern.  Queries are
+// scaled by a power of two a row; 16-bit ones fit one fp16 operand, fp32 ones take two (22 bits).  Weights are
+// 2^(z - ref) <= 2^15 with z the score plus the exponent of V's scale; one operand for bf16 outputs, whose
+// own rounding is 8 times coarser, else two.
+//
+// ref follows the running maximum lazily (only when a weight would pass 2^15 are sums rescaled), so
+// most tiles need one vote and no shuffles; row sums stay in the lanes until the segment ends.
+#pragma once
+
+#include "pool_attention.cuh"
+
+namespace skv {
+
+constexpr int kMmaWarps = 4, kMmaThreads = 32 * kMmaWarps, kMmaTile = 16 * kMmaWarps;
+constexpr float kRefDrop = 5.0f;    // a fresh maximum's weight is 2^5: small weights keep their bits in fp16
+constexpr float kRefRoom = 14.0f;   // weights may grow to 2^14 (times a mantissa < 2) before ref moves
+
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint2 b) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint4 load_page16(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint2 load_page8(const void* p) {
+    uint2 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t load_page4(const void* p) {
+    uint32_t v;
+    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t h2_sub(uint32_t a, uint32_t b) {
+    const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
+    const __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
+    const __half2 r = __hfma2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b), *reinterpret_cast<__half2*>(&c));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t h2_pack(float a, float b) {
+    const __half2 r = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+// Small integers as fp16: 1024 + n has n in its low bits.
+__device__ __forceinline__ uint32_t i8_pair(uint32_t biased, uint32_t sel) {        // bytes n + 128
+    return h2_sub(__byte_perm(biased, 0x64646464u, sel), 0x64806480u);              // - 1152
+}
+__device__ __forceinline__ uint32_t i4_low(uint32_t w) {                            // nibbles n + 8 in bits 0-3
+    return h2_sub((w & 0x000F000Fu) | 0x64006400u, 0x64086408u);                    // - 1032
+}
+__device__ __forceinline__ uint32_t i4_high(uint32_t w) {                           // in bits 4-7: 1024 + 16 (n + 8)
+    return h2_fma((w & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);       // / 16 - 72
+}
+// x as an 8-bit value and an 11-bit remainder, each twice in a register.
+__device__ __forceinline__ void split_scale(float x, float& r1, float& r2) {
+    r1 = __uint_as_float((__float_as_uint(x) + 0x8000u) & 0xFFFF0000u);
+    r2 = x - r1;
+}
+// 2^(127 + 10 - e) scales a float of exponent field e to [2^10, 2^11).
+__device__ __forceinline__ int clamp_exp(uint32_t bits) { return min(max((int)(bits >> 23), 11), 253); }
+__device__ __forceinline__ float exp_down(int e) { return __uint_as_float((uint32_t)(264 - e) << 23); }
+__device__ __forceinline__ float exp_up(int e) { return __uint_as_float((uint32_t)(e - 10) << 23); }
+
+// The page rows of a sequence's tokens for one key head.  A warp keeps the next 64 entries of the
+// block table in its lanes and asks them by shuffle: tiles need no dependent load.
+struct PageRows {
+    const int32_t* table;
+    int width, base, cur, next, lane;
+    __device__ __forceinline__ int entry(int i) const { return i < width ? __ldg(table + i) : -1; }
+    __device__ __forceinline__ void start(const skv_pool& p, int b, int first) {
+        table = p.block_table + b * p.table_stride;
+        width = p.table_width;
+        lane = threadIdx.x & 31;
+        base = first;
+        cur = entry(base + lane);
+        next = entry(base + 32 + lane);
+    }
+    __device__ __forceinline__ int page(int j) {   // j does not decrease
+        while (j >= base + 32) {
+            base += 32;
+            cur = next;
+            next = entry(base + 32 + lane);
+        }
+        return __shfl_sync(0xffffffffu, cur, j - base);
+    }
+};
+
+// One warp's tile of 16 tokens, as loaded.
+template <int PREC, int DP>
+struct KTile;
+template <int PREC, int DP>
+struct VTile;
+
+template <int DP>
+struct KTile<1, DP> {
+    uint4 x[2][DP / 32];
+    __device__ __forceinline__ void load(const skv_pool& p, const int64_t (&row)[2], int c) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int j = 0; j < DP / 32; ++j) {
+                const int chunk = c + 4 * j;
+                x[t][j] = make_uint4(0, 0, 0, 0);
+                if (row[t] >= 0 && chunk * 8 < p.head_dim)
+                    x[t][j] = load_page16(static_cast<const __half*>(p.k) + row[t] * p.head_dim + chunk * 8);
+            }
+    }
+};
+template <int DP>
+struct KTile<2, DP> {
+    uint4 x[2][DP / 64];
+    float s[2];
+    __device__ __forceinline__ void load(const skv_pool& p, const int64_t (&row)[2], int c) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int j = 0; j < DP / 64; ++j) {
+                const int chunk = c + 4 * j;
+                x[t][j] = make_uint4(0, 0, 0, 0);
+                if (row[t] >= 0 && chunk * 16 < p.head_dim)
+                    x[t][j] = load_page16(static_cast<const int8_t*>(p.k) + row[t] * p.head_dim + chunk * 16);
+            }
+            s[t] = row[t] >= 0 ? __ldg(p.scale_k + row[t]) : 0.0f;
+        }
+    }
+};
+template <int DP>
+struct KTile<3, DP> {
+    uint2 x[2][DP / 64];
+    float s[2][DP / 64];
+    __device__ __forceinline__ void load(const skv_pool& p, const int64_t (&row)[2], int c) {
+        const int ng = p.head_dim / p.int4_group;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int j = 0; j < DP / 64; ++j) {
+                const int chunk = c + 4 * j;
+                const bool on = row[t] >= 0 && chunk * 16 < p.head_dim;
+                x[t][j] = make_uint2(0x88888888u, 0x88888888u);
+                s[t][j] = 0.0f;
+                if (on) {
+                    x[t][j] = load_page8(static_cast<const uint8_t*>(p.k) + row[t] * (p.head_dim / 2) + chunk * 8);
+                    s[t][j] = __ldg(p.scale_k + row[t] * ng + chunk * 16 / p.int4_group);
+                }
+            }
+    }
+};
+
+template <int DP>
+struct VTile<1, DP> {
+    uint4 x[4][DP / 64];
+    __device__ __forceinline__ void load(const skv_pool& p, const int64_t (&row)[4], const int64_t (&)[2], int g, int) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int j = 0; j < DP / 64; ++j) {
+                const int chunk = g + 8 * j;
+                x[t][j] = make_uint4(0, 0, 0, 0);
+                if (row[t] >= 0 && chunk * 8 < p.head_dim)
+                    x[t][j] = load_page16(static_cast<const __half*>(p.v) + row[t] * p.head_dim + chunk * 8);
+            }
+    }
+};
+template <int DP>
+struct VTile<2, DP> {
+    uint32_t x[4][DP / 32];
+    float s[2];   // of tokens g and g + 8
+    __device__ __forceinline__ void load(const skv_pool& p, const int64_t (&row)[4], const int64_t (&own)[2], int g, int) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int w = 0; w < DP / 32; ++w) x[t][w] = 0;
+            if (row[t] >= 0 && g * (DP / 8) < p.head_dim) {
+                const int8_t* q = static_cast<const int8_t*>(p.v) + row[t] * p.head_dim + g * (DP / 8);
+                if constexpr (DP == 128) {
+                    const uint4 u = load_page16(q);
+                    x[t][0] = u.x; x[t][1] = u.y; x[t][2] = u.z; x[t][3] = u.w;
+                } else {
+                    const uint2 u = load_page8(q);
+                    x[t][0] = u.x; x[t][1] = u.y;
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) s[t] = own[t] >= 0 ? __ldg(p.scale_v + own[t]) : 1.0f;
+    }
+};
+template <int DP>
+struct VTile<3, DP> {
+    uint32_t x[4][DP / 64];
+    float s[4];              // of this lane's values, tokens 2c, 2c + 1, 2c + 8, 2c + 9
+    float own[2][DP / 64];   // this lane's quarter of the scales of tokens g and g + 8
+    __device__ __forceinline__ void load(const skv_pool& p, const int64_t (&row)[4], const int64_t (&mine)[2], int g, int c) {
+        const int ng = p.head_dim / p.int4_group;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+            for (int w = 0; w < DP / 64; ++w) x[t][w] = 0x88888888u;
+            s[t] = 0.0f;
+            if (row[t] >= 0 && g * (DP / 8) < p.head_dim) {
+                const uint8_t* q = static_cast<const uint8_t*>(p.v) + row[t] * (p.head_dim / 2) + g * (DP / 16);
+                if constexpr (DP == 128) {
+                    const uint2 u = load_page8(q);
+                    x[t][0] = u.x; x[t][1] = u.y;
+                } else {
+                    x[t][0] = load_page4(q);
+                }
+                s[t] = __ldg(p.scale_v + row[t] * ng + g * (DP / 8) / p.int4_group);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int j = 0; j < DP / 64; ++j) {
+                const int chunk = c + 4 * j;
+                own[t][j] = mine[t] >= 0 && chunk * 16 < p.head_dim ? __ldg(p.scale_v + mine[t] * ng + chunk * 16 / p.int4_group) : 0.0f;
+            }
+    }
+};
+
+// Where value d of a query row sits in the B operands: MMA, lane column c, register and half.
+template <int PREC>
+__device__ __forceinline__ void query_place(int d, int& mma, int& c, int& reg, int& half) {
+    if (PREC == 1) {
+        const int chunk = d / 8, h = d % 8;
+        mma = 2 * (chunk / 4) + h / 4; c = chunk % 4; reg = (h % 4) / 2; half = h % 2;
+    } else if (PREC == 2) {
+        const int chunk = d / 16, h = d % 16;
+        mma = 4 * (chunk / 4) + h / 4; c = chunk % 4; reg = (h % 4) / 2; half = h % 2;
+    } else {
+        const int chunk = d / 16, h = d % 8;
+        mma = 2 * (2 * (chunk / 4) + (d % 16) / 8) + (h % 4) / 2; c = chunk % 4; reg = h % 2; half = h / 4;
+    }
+}
+
+template <int DP, int NT, int NQ>
+__host__ __device__ constexpr size_t mma_smem() {
+    return (size_t)(DP / 16) * NT * NQ * 32 * 8 + (size_t)kMmaWarps * 8 * NT * (DP + 2) * 4 + (3 * kMmaWarps + 2) * 8 * NT * 4;
+}
+
+template <int PREC, int DP, int NT, int NQ, int NP, int CTAS>
+__global__ void __launch_bounds__(kMmaThreads, CTAS)
+pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int row_tiles) {
+    constexpr int M = DP / 16, ROWS = 8 * NT;
+    extern __shared__ __align__(16) char mma_sm[];
+    __shared__ Share s;
+    uint2* s_q = reinterpret_cast<uint2*>(mma_sm);                       // [M][NT][NQ][32]
+    float* s_o = reinterpret_cast<float*>(s_q + M * NT * NQ * 32);       // [warps][ROWS][DP + 2]
+    float* s_ref = s_o + kMmaWarps * ROWS * (DP + 2);                    // [warps][ROWS]
+    float* s_sum = s_ref + kMmaWarps * ROWS;                             // [warps][ROWS]
+    float* s_w = s_sum + kMmaWarps * ROWS;                               // [warps][ROWS]
+    float* s_c = s_w + kMmaWarps * ROWS;                                 // [ROWS] factor of a row's scores; later its max
+    float* s_l = s_c + ROWS;                                             // [ROWS]
+    const int D = a.pool.head_dim, P = a.pool.page_size;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, lg = lane >> 2, lc = lane & 3;
+    const int rep = a.q.heads / a.pool.heads, R = rep * a.S_q;
+    const bool p16 = P % 16 == 0;   // a tile lies in one page
+    take_share<kMmaThreads>(a, kMmaTile, a.pool.heads * row_tiles, 1, &s);
+    int b = s.b;
+    long long base = s.base;
+    for (long long at = s.lo; at < s.hi;) {
+        const Segment g = segment_at(a, s, at, kMmaTile, row_tiles, b, base);
+        at += g.t1 - g.t0;
+        const int n = (int)g.tokens, r0 = g.rt * ROWS;
+        // ---- queries: a power of two taken out of each row, laid out as B operands
+        __syncthreads();
+        for (int j = warp; j < ROWS; j += kMmaWarps) {
+            float x[DP / 32], top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) {
+                const int d = lane + 32 * i;
+                x[i] = 0.0f;
+                if (r0 + j < R && d < D) {
+                    if (a.q.dtype == kF32) x[i] = row_ptr<const float>(a.q, a.S_q, rep, g.b, g.hk, r0 + j)[d];
+                    else if (a.q.dtype == kF16) x[i] = __half2float(row_ptr<const __half>(a.q, a.S_q, rep, g.b, g.hk, r0 + j)[d]);
+                    else x[i] = __bfloat162float(row_ptr<const __nv_bfloat16>(a.q, a.S_q, rep, g.b, g.hk, r0 + j)[d]);
+                }
+                top = fmaxf(top, fabsf(x[i]));
+            }
+            const int e = clamp_exp(__float_as_uint(warp_max(top)));
+            const float down = exp_down(e);
+            if (lane == 0) s_c[j] = a.scale * 1.4426950408889634f * exp_up(e);
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) {
+                int mma, c, reg, half;
+                query_place<PREC>(lane + 32 * i, mma, c, reg, half);
+                const float y = x[i] * down;
+                const __half hi = __float2half_rn(y);
+                __half* q = reinterpret_cast<__half*>(s_q + ((mma * NT + j / 8) * NQ) * 32 + (j % 8) * 4 + c) + 2 * reg + half;
+                q[0] = hi;
+                if (NQ == 2) q[32 * 4] = __float2half_rn(y - __half2float(hi));
+            }
+        }
+        __syncthreads();
+        float cf[NT][2], ref[NT][2], sum[NT][2], o[NT][M][4];
+        int see[NT][2], see_all = n;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int j = 8 * t + 2 * lc + i;
+                cf[t][i] = s_c[j];
+                ref[t][i] = -INFINITY;
+                sum[t][i] = 0.0f;
+                see[t][i] = r0 + j < R ? (int)max(seen_by(a, g.b, g.tokens, (r0 + j) % a.S_q), (int64_t)0) : n;
+                see_all = min(see_all, see[t][i]);
+            }
+        see_all = min(see_all, __shfl_xor_sync(0xffffffffu, see_all, 1));
+        see_all = min(see_all, __shfl_xor_sync(0xffffffffu, see_all, 2));
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int m = 0; m < M; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[t][m][i] = 0.0f;
+
+        const int end = min((int)g.t1 * kMmaWarps, (n + 15) / 16);
+        int st = (int)g.t0 * kMmaWarps + warp;
+        PageRows pages;
+        if (p16) pages.start(a.pool, g.b, st * 16 / P);
+        // rows of a tile's tokens: `own` g, g + 8; `four` 2c, 2c + 1, 2c + 8, 2c + 9; -1 where there is none
+        auto rows_of = [&](int tile, int64_t (&own)[2], int64_t (&four)[4]) {
+            const int t0 = tile * 16;
+            if (p16) {
+                const int j = t0 / P, page = pages.page(j);
+                const bool ok = page >= 0 && page < a.pool.num_pages;
+                const int64_t row = ((int64_t)page * a.pool.heads + g.hk) * P + (t0 - j * P);
+                if (!ok && lane == 0 && a.error_flag) atomicExch(a.error_flag, 1);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) own[i] = ok && t0 + lg + 8 * i < n ? row + lg + 8 * i : -1;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int k = 2 * lc + (i & 1) + 8 * (i >> 1);
+                    four[i] = ok && t0 + k < n ? row + k : -1;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int t = t0 + lg + 8 * i;
+                    own[i] = t < n ? pool_row(a.pool, g.b, t) : -1;
+                    if (t < n && own[i] < 0 && a.error_flag) atomicExch(a.error_flag, 1);
+                    if (own[i] >= 0) own[i] += (int64_t)g.hk * P;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int t = t0 + 2 * lc + (i & 1) + 8 * (i >> 1);
+                    four[i] = t < n ? pool_row(a.pool, g.b, t) : -1;
+                    if (four[i] >= 0) four[i] += (int64_t)g.hk * P;
+                }
+            }
+        };
+        KTile<PREC, DP> kt;
+        VTile<PREC, DP> vt;
+        int64_t own[2], four[4];
+        bool here[2] = {false, false};
+        if (st < end) {
+            rows_of(st, own, four);
+            kt.load(a.pool, own, lc);
+            vt.load(a.pool, four, own, lg, lc);
+            here[0] = own[0] >= 0;
+            here[1] = own[1] >= 0;
+        }
+        for (; st < end; st += kMmaWarps) {
+            const bool more = st + kMmaWarps < end;
+            if (more) rows_of(st + kMmaWarps, own, four);
+            // ---- scores
+            float x[NT][4];
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[t][i] = 0.0f;
+            float k_factor[2] = {1.0f, 1.0f};
+            auto qk = [&](const uint32_t (&f)[4], int m, int terms) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int q = 0; q < NQ; ++q)
+                        if (q < terms) mma16816(x[t], f, s_q[((m * NT + t) * NQ + q) * 32 + lane]);
+            };
+            if constexpr (PREC == 1) {
+#pragma unroll
+                for (int j = 0; j < DP / 32; ++j) {
+                    const uint4 u = kt.x[0][j], v = kt.x[1][j];
+                    const uint32_t f0[4] = {u.x, v.x, u.y, v.y}, f1[4] = {u.z, v.z, u.w, v.w};
+                    qk(f0, 2 * j, NQ);
+                    qk(f1, 2 * j + 1, NQ);
+                }
+            } else if constexpr (PREC == 2) {
+#pragma unroll
+                for (int j = 0; j < DP / 64; ++j) {
+                    const uint32_t u[4] = {kt.x[0][j].x, kt.x[0][j].y, kt.x[0][j].z, kt.x[0][j].w};
+                    const uint32_t v[4] = {kt.x[1][j].x, kt.x[1][j].y, kt.x[1][j].z, kt.x[1][j].w};
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const uint32_t p = u[w] ^ 0x80808080u, q = v[w] ^ 0x80808080u;
+                        const uint32_t f[4] = {i8_pair(p, 0x4140), i8_pair(q, 0x4140), i8_pair(p, 0x4342), i8_pair(q, 0x4342)};
+                        qk(f, 4 * j + w, NQ);
+                    }
+                }
+                k_factor[0] = kt.s[0];
+                k_factor[1] = kt.s[1];
+            } else {
+                uint32_t top = 0;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int j = 0; j < DP / 64; ++j) top = max(top, __float_as_uint(kt.s[t][j]) & 0x7fffffffu);
+                const int e = clamp_exp(__reduce_max_sync(0xffffffffu, top));
+                const float down = exp_down(e);
+                k_factor[0] = k_factor[1] = exp_up(e);
+#pragma unroll
+                for (int j = 0; j < DP / 64; ++j) {
+                    uint32_t r1[2], r2[2];
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        float y1, y2;
+                        split_scale(kt.s[t][j] * down, y1, y2);
+                        r1[t] = h2_pack(y1, y1);
+                        r2[t] = h2_pack(y2, y2);
+                    }
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        uint32_t p = w ? kt.x[0][j].y : kt.x[0][j].x, q = w ? kt.x[1][j].y : kt.x[1][j].x;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t f[4] = {i4_high(p), i4_high(q), i4_low(p), i4_low(q)};
+                            const uint32_t f1[4] = {h2_mul(f[0], r1[0]), h2_mul(f[1], r1[1]), h2_mul(f[2], r1[0]), h2_mul(f[3], r1[1])};
+                            const uint32_t f2[4] = {h2_mul(f[0], r2[0]), h2_mul(f[1], r2[1]), h2_mul(f[2], r2[0]), h2_mul(f[3], r2[1])};
+                            qk(f1, 2 * (2 * j + w) + h, NQ);
+                            qk(f2, 2 * (2 * j + w) + h, 1);
+                            p >>= 8;
+                            q >>= 8;
+                        }
+                    }
+                }
+            }
+            if (more) kt.load(a.pool, own, lc);
+            // ---- weights
+            float v_add[2] = {0.0f, 0.0f}, v_mul[2] = {1.0f, 1.0f}, v_sum[2] = {1.0f, 1.0f};
+            int ve[2] = {0, 0};
+            if constexpr (PREC == 2) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    ve[i] = clamp_exp(__float_as_uint(vt.s[i]) & 0x7fffffffu);
+                    v_add[i] = (float)(ve[i] - 127);
+                    v_sum[i] = __uint_as_float((uint32_t)(254 - ve[i]) << 23);   // 2^-(ve - 127)
+                    v_mul[i] = vt.s[i] * v_sum[i];
+                }
+            } else if constexpr (PREC == 3) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int j = 0; j < DP / 64; ++j) top = max(top, __float_as_uint(vt.own[i][j]) & 0x7fffffffu);
+                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    ve[i] = clamp_exp(top);
+                    v_add[i] = (float)(ve[i] - 137);
+                    v_sum[i] = exp_down(ve[i]);                                 // 2^-(ve - 137)
+                }
+            }
+            const int t0 = st * 16;
+            const bool all = t0 + 16 <= see_all && p16 && __all_sync(0xffffffffu, here[0]);
+            bool grow = false;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int tok = i >> 1, col = i & 1;
+                    float z = x[t][i] * (cf[t][col] * k_factor[tok]);
+                    if (PREC >= 2) z += v_add[tok];
+                    if (!all && (!here[tok] || t0 + lg + 8 * tok >= see[t][col])) z = -INFINITY;
+                    x[t][i] = z;
+                    grow |= z > (ref[t][col] == -INFINITY ? -INFINITY : ref[t][col] + kRefRoom);
+                }
+            if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float top = fmaxf(x[t][i], x[t][i + 2]);
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                        const float now = fmaxf(ref[t][i], top - kRefDrop);
+                        const float f = now == -INFINITY ? 1.0f : fast_exp2(ref[t][i] - now);
+                        ref[t][i] = now;
+                        sum[t][i] *= f;
+#pragma unroll
+                        for (int m = 0; m < M; ++m) {
+                            o[t][m][i] *= f;
+                            o[t][m][i + 2] *= f;
+                        }
+                    }
+            }
+            uint2 p[NT][NP];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int tok = i >> 1, col = i & 1;
+                    const float y = fast_exp2(x[t][i] - (ref[t][col] == -INFINITY ? 0.0f : ref[t][col]));
+                    sum[t][col] = PREC >= 2 ? fmaf(y, v_sum[tok], sum[t][col]) : sum[t][col] + y;
+                    w[i] = PREC == 2 ? y * v_mul[tok] : y;
+                }
+                const uint32_t lo = h2_pack(w[0], w[1]), hi = h2_pack(w[2], w[3]);
+                p[t][0] = make_uint2(transpose8x8(lo), transpose8x8(hi));
+                if constexpr (NP == 2) {
+                    const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+                    const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                    p[t][1] = make_uint2(transpose8x8(h2_pack(w[0] - f0.x, w[1] - f0.y)),
+                                         transpose8x8(h2_pack(w[2] - f1.x, w[3] - f1.y)));
+                }
+            }
+            // ---- values
+            auto pv = [&](const uint32_t (&f)[4], int m, int terms) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int q = 0; q < NP; ++q)
+                        if (q < terms) mma16816(o[t][m], f, p[t][q]);
+            };
+            if constexpr (PREC == 1) {
+#pragma unroll
+                for (int j = 0; j < DP / 64; ++j) {
+                    const uint32_t u[4][4] = {{vt.x[0][j].x, vt.x[0][j].y, vt.x[0][j].z, vt.x[0][j].w},
+                                              {vt.x[1][j].x, vt.x[1][j].y, vt.x[1][j].z, vt.x[1][j].w},
+                                              {vt.x[2][j].x, vt.x[2][j].y, vt.x[2][j].z, vt.x[2][j].w},
+                                              {vt.x[3][j].x, vt.x[3][j].y, vt.x[3][j].z, vt.x[3][j].w}};
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const uint32_t f[4] = {__byte_perm(u[0][w], u[1][w], 0x5410), __byte_perm(u[0][w], u[1][w], 0x7632),
+                                               __byte_perm(u[2][w], u[3][w], 0x5410), __byte_perm(u[2][w], u[3][w], 0x7632)};
+                        pv(f, 4 * j + w, NP);
+                    }
+                }
+            } else if constexpr (PREC == 2) {
+#pragma unroll
+                for (int w = 0; w < DP / 32; ++w) {
+                    uint32_t y[2][2];   // [tokens low / high][values 0,1 / 2,3]
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t u = vt.x[2 * h][w] ^ 0x80808080u, v = vt.x[2 * h + 1][w] ^ 0x80808080u;
+                        y[h][0] = __byte_perm(u, v, 0x5140);
+                        y[h][1] = __byte_perm(u, v, 0x7362);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t f[4] = {i8_pair(y[0][i], 0x4140), i8_pair(y[0][i], 0x4342),
+                                               i8_pair(y[1][i], 0x4140), i8_pair(y[1][i], 0x4342)};
+                        pv(f, 2 * w + i, NP);
+                    }
+                }
+            } else {
+                // the exponents of tokens 2c, 2c + 1 (+ 8) sit in lanes 4 (2c), 4 (2c + 1)
+                uint32_t r1[2], r2[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float y1[2], y2[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int e = __shfl_sync(0xffffffffu, ve[h], 4 * (2 * lc + i));
+                        split_scale(vt.s[2 * h + i] * exp_down(e), y1[i], y2[i]);
+                    }
+                    r1[h] = h2_pack(y1[0], y1[1]);
+                    r2[h] = h2_pack(y2[0], y2[1]);
+                }
+#pragma unroll
+                for (int w = 0; w < DP / 64; ++w)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t u = __byte_perm(vt.x[0][w], vt.x[1][w], i ? 0x7632 : 0x5410);
+                        uint32_t v = __byte_perm(vt.x[2][w], vt.x[3][w], i ? 0x7632 : 0x5410);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t f[4] = {i4_high(u), i4_low(u), i4_high(v), i4_low(v)};
+                            const uint32_t f1[4] = {h2_mul(f[0], r1[0]), h2_mul(f[1], r1[0]), h2_mul(f[2], r1[1]), h2_mul(f[3], r1[1])};
+                            const uint32_t f2[4] = {h2_mul(f[0], r2[0]), h2_mul(f[1], r2[0]), h2_mul(f[2], r2[1]), h2_mul(f[3], r2[1])};
+                            pv(f1, 4 * w + 2 * i + h, NP);
+                            pv(f2, 4 * w + 2 * i + h, 1);
+                            u >>= 8;
+                            v >>= 8;
+                        }
+                    }
+            }
+            if (more) {
+                vt.load(a.pool, four, own, lg, lc);
+                here[0] = own[0] >= 0;
+                here[1] = own[1] >= 0;
+            }
+        }
+
+        // ---- the warps' parts joined
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float l = sum[t][i];
+                l += __shfl_xor_sync(0xffffffffu, l, 4);
+                l += __shfl_xor_sync(0xffffffffu, l, 8);
+                l += __shfl_xor_sync(0xffffffffu, l, 16);
+                const int j = 8 * t + 2 * lc + i;
+                if (lg == 0) {
+                    s_ref[warp * ROWS + j] = ref[t][i];
+                    s_sum[warp * ROWS + j] = l;
+                }
+                float* row = s_o + (warp * ROWS + j) * (DP + 2);
+#pragma unroll
+                for (int m = 0; m < M; ++m) {
+                    const int d = PREC == 1 ? 64 * (m / 4) + 8 * lg + 2 * (m % 4) : lg * (DP / 8) + 2 * m;
+                    *reinterpret_cast<float2*>(row + d) = make_float2(o[t][m][i], o[t][m][i + 2]);
+                }
+            }
+        __syncthreads();
+        if (tid < ROWS) {
+            float m = -INFINITY, l = 0.0f;
+            for (int w = 0; w < kMmaWarps; ++w) m = fmaxf(m, s_ref[w * ROWS + tid]);
+            const float r = m == -INFINITY ? 0.0f : m;
+            for (int w = 0; w < kMmaWarps; ++w) {
+                const float f = exp2f(s_ref[w * ROWS + tid] - r);
+                s_w[w * ROWS + tid] = f;
+                l += s_sum[w * ROWS + tid] * f;
+            }
+            s_c[tid] = m;
+            s_l[tid] = l;
+        }
+        __syncthreads();
+        float* part = slot_of(a, blockIdx.x, g.slot, ROWS);
+        for (int i = tid; i < ROWS * D; i += kMmaThreads) {
+            const int j = i / D, d = i - j * D;
+            if (r0 + j >= R) break;
+            float y = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kMmaWarps; ++w) y += s_o[(w * ROWS + j) * (DP + 2) + d] * s_w[w * ROWS + j];
+            if (g.whole) store_out(a, g.b, g.hk, r0 + j, d, s_l[j] == 0.0f ? 0.0f : y / s_l[j]);
+            else part[j * D + d] = y;
+        }
+        if (g.whole) continue;
+        if (tid < ROWS) {
+            part[ROWS * D + tid] = s_c[tid];
+            part[ROWS * D + ROWS + tid] = s_l[tid];
+        }
+        if (arrive(a, s, g)) join<ROWS>(a, s, g, R);
+    }
+}
+
+// CTAs an SM: what their registers allow.
+template <int PREC, int DP, int NT, int NQ, int NP>
+int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
+    constexpr int CTAS = NT >= 4 ? 2 : NT == 2 ? 3 : PREC == 1 ? 3 : 4;
+    static_assert(CTAS * 2 * 8 * NT <= kRowsPerSm, "the scratch holds every CTA's slots");
+    constexpr size_t smem = mma_smem<DP, NT, NQ>();
+    const auto kernel = pool_attention_mma_kernel<PREC, DP, NT, NQ, NP, CTAS>;
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return fail(SKV_ERR_CUDA, "pool_attention: %s", cudaGetErrorString(e));
+    }
+    const int R = a.q.heads / a.pool.heads * a.S_q;
+    kernel<<<sm_count() * CTAS, kMmaThreads, smem, st>>>(a, (R + 8 * NT - 1) / (8 * NT));
+    return check_launch("pool_attention");
+}
+
+template <int PREC, int DP, int NT>
+int launch_mma_type(const skv_pool_attention_args& a, cudaStream_t st) {
+    if (a.q.dtype == kF32) return launch_mma<PREC, DP, NT, 2, 2>(a, st);
+    if (a.q.dtype == kF16) return launch_mma<PREC, DP, NT, 1, 2>(a, st);
+    return launch_mma<PREC, DP, NT, 1, 1>(a, st);
+}
+
+// Row tiles of 8, 16 or 32 rows: the pages are read once for up to 32 rows of a key head.
+template <int PREC>
+int launch_mma_prec(const skv_pool_attention_args& a, cudaStream_t st) {
+    const int R = a.q.heads / a.pool.heads * a.S_q;
+    if (a.pool.head_dim <= 64) {
+        if (R <= 8) return launch_mma_type<PREC, 64, 1>(a, st);
+        return R <= 16 ? launch_mma_type<PREC, 64, 2>(a, st) : launch_mma_type<PREC, 64, 4>(a, st);
+    }
+    if (R <= 8) return launch_mma_type<PREC, 128, 1>(a, st);
+    return R <= 16 ? launch_mma_type<PREC, 128, 2>(a, st) : launch_mma_type<PREC, 128, 4>(a, st);
+}
+
+}  // namespace skv
