@@ -18,10 +18,11 @@ namespace skv {
 // --------------------------------------------------------------------------- any size and alignment
 // Products on the FMA pipe from fp32 tiles in shared memory: 8 rows, 32 tokens at a time.  Thread =
 // (token, rows w and w + 4) for the scores, value d for the sums.
-constexpr int kAnyRows = 8, kAnyTile = 32, kAnyThreads = 128, kAnyMaxD = 512;
+constexpr int kAnyRows = 8, kAnyTile = 32, kAnyThreads = 128, kAnyMaxD = 512, kAnyParts = 64;
 
 __host__ __device__ inline size_t any_smem(int D) {
-    return ((size_t)kAnyRows * D + (size_t)kAnyTile * (D + 1) + (size_t)kAnyTile * D + kAnyRows * kAnyTile + kAnyRows) * 4;
+    return ((size_t)kAnyRows * D + (size_t)kAnyTile * (D + 1) + (size_t)kAnyTile * D + kAnyRows * kAnyTile + kAnyRows +
+            join_floats<kAnyRows, kAnyThreads, kAnyParts>()) * 4;
 }
 
 template <class T>
@@ -35,11 +36,11 @@ __global__ void __launch_bounds__(kAnyThreads) pool_attention_any_kernel(const _
     float* sv = sk + kAnyTile * (D + 1);
     float* sp = sv + kAnyTile * D;
     float* sc = sp + kAnyRows * kAnyTile;
+    float* sj = sc + kAnyRows;
     const int rep = a.q.heads / a.pool.heads, R = rep * a.S_q;
     take_share<kAnyThreads>(a, kAnyTile, a.pool.heads * row_tiles, 2, &s);
-    int b = s.b;
-    long long base = s.base;
-    for (long long at = s.lo; at < s.hi;) {
+    int b = s.b, base = s.base;
+    for (int at = s.lo; at < s.hi;) {
         const Segment g = segment_at(a, s, at, kAnyTile, row_tiles, b, base);
         at += g.t1 - g.t0;
         const int r0 = g.rt * kAnyRows;
@@ -49,7 +50,7 @@ __global__ void __launch_bounds__(kAnyThreads) pool_attention_any_kernel(const _
             sq[i] = r < R ? to_float(row_ptr<const T>(a.q, a.S_q, rep, g.b, g.hk, r)[i % D]) * (a.scale * 1.4426950408889634f)
                           : 0.0f;
         }
-        int64_t see[2];   // tokens that each of this warp's two rows sees
+        int see[2];   // tokens that each of this warp's two rows sees
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
         float o[kAnyRows][kAnyMaxD / kAnyThreads];
 #pragma unroll
@@ -59,8 +60,8 @@ __global__ void __launch_bounds__(kAnyThreads) pool_attention_any_kernel(const _
         for (int j = 0; j < kAnyRows; ++j)
 #pragma unroll
             for (int i = 0; i < kAnyMaxD / kAnyThreads; ++i) o[j][i] = 0.0f;
-        for (long long t = g.t0; t < g.t1; ++t) {
-            const int64_t tok0 = t * kAnyTile;
+        for (int t = g.t0; t < g.t1; ++t) {
+            const int tok0 = t * kAnyTile;
             __syncthreads();
             for (int j = warp; j < kAnyTile; j += kAnyThreads / 32) {
                 int64_t row = tok0 + j < g.tokens ? pool_row(a.pool, g.b, tok0 + j) : -1;
@@ -144,7 +145,7 @@ __global__ void __launch_bounds__(kAnyThreads) pool_attention_any_kernel(const _
             part[kAnyRows * D + tid] = sp[kAnyRows + tid];
             part[kAnyRows * D + kAnyRows + tid] = sp[tid];
         }
-        if (arrive(a, s, g)) join<kAnyRows>(a, s, g, R);
+        if (arrive(a, s, g)) join<kAnyRows, kAnyThreads, 1, kAnyParts>(a, s, g, R, sj);
     }
 }
 
@@ -170,9 +171,10 @@ int attend_int8(const skv_pool_attention_args& a, cudaStream_t st);
 int attend_int4(const skv_pool_attention_args& a, cudaStream_t st);
 
 // They need heads of up to 128 values in chunks of 16 bytes (fp16) or 16 values (int8, int4), int4
-// groups of whole chunks, and payloads on 16-byte boundaries.
+// groups of whole chunks, payloads on 16-byte boundaries, and row numbers of 31 bits.
 bool fits_mma(const skv_pool& p) {
     const int D = p.head_dim;
+    if ((int64_t)p.num_pages * p.heads * p.page_size > 0x7fffffff) return false;
     if (p.precision == 0 || D > 128 || D % (p.precision == 1 ? 8 : 16) || (p.precision == 3 && p.int4_group % 16)) return false;
     return ((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v)) & 15) == 0;
 }
@@ -204,6 +206,9 @@ int skv_pool_attention(const skv_pool_attention_args* args, void* stream) {
         return fail(SKV_ERR_UNSUPPORTED, "pool_attention: head_dim %d above %d", a.pool.head_dim, kAnyMaxD);
     if ((int64_t)a.q.heads * a.S_q > (1 << 28) || a.pool.batch > (1 << 24))
         return fail(SKV_ERR_TOO_LARGE, "pool_attention: too many rows");
+    const int64_t tiles = ((int64_t)a.pool.table_width * a.pool.page_size + kAnyTile - 1) / kAnyTile + 1;
+    if (tiles * a.pool.batch > 0x7fffffff / ((int64_t)a.q.heads * a.S_q))   // row tiles hold one row at least
+        return fail(SKV_ERR_TOO_LARGE, "pool_attention: more than 2^31 tiles of work");
     if (a.scratch_bytes < (int64_t)skv_pool_attention_scratch_bytes(a.pool.head_dim))
         return fail(SKV_ERR_SCRATCH, "pool_attention: scratch of %lld bytes", (long long)a.scratch_bytes);
     cudaStream_t st = as_stream(stream);

@@ -10,101 +10,102 @@ constexpr int kMaxCtas = 4096;      // arrival counters in the scratch
 constexpr int kRowsPerSm = 128;     // rows of partial results in the scratch for each SM: CTAs x 2 slots x rows
 
 // ------------------------------------------------------------------------------ shares of the work
+// Tile numbers fit 31 bits (the launch checks the most that the table allows).
 struct Share {
-    long long lo, hi, total;   // this CTA's tiles [lo, hi) of all
-    long long base;            // tiles of the sequences before b
+    int lo, hi, total;         // this CTA's tiles [lo, hi) of all
+    int base;                  // tiles of the sequences before b
     int b;                     // the sequence that holds tile lo
-    int ctas;                  // CTAs that share the work
+    int each, more;            // a share is `each` tiles, one more for the first `more` CTAs
+    __device__ __forceinline__ int first_of(int cta) const { return cta * each + min(cta, more); }
+    __device__ __forceinline__ int owner_of(int tile) const {
+        const int head = more * (each + 1);
+        return tile < head ? tile / (each + 1) : more + (tile - head) / each;
+    }
 };
 
-__device__ __forceinline__ int64_t seq_tokens(const skv_pool_attention_args& a, int b) {
-    const int64_t n = a.lengths[b], cap = (int64_t)a.pool.table_width * a.pool.page_size;
-    return n < 0 ? 0 : n > cap ? cap : n;
+__device__ __forceinline__ int seq_tokens(const skv_pool_attention_args& a, int b) {
+    const int64_t n = __ldg(a.lengths + b), cap = (int64_t)a.pool.table_width * a.pool.page_size;
+    return (int)(n < 0 ? 0 : n > cap ? cap : n);
 }
 // Tiles of a sequence for one row tile of one head; an empty sequence keeps one, to write its zeros.
-__device__ __forceinline__ int64_t seq_tiles(int64_t tokens, int tile) {
-    return tokens == 0 ? 1 : (tokens + tile - 1) / tile;
-}
+__device__ __forceinline__ int seq_tiles(int tokens, int tile) { return max(1, (tokens + tile - 1) / tile); }
 
 // Every thread of the block calls this; *s is valid for all after it.  At least min_tiles a CTA.
 template <int THREADS>
 __device__ __forceinline__ void take_share(const skv_pool_attention_args& a, int tile, int units, int min_tiles,
                                            Share* s) {
-    __shared__ long long s_part[THREADS / 32];
+    __shared__ int s_part[THREADS / 32];
     const int tid = threadIdx.x, lane = tid & 31, B = a.pool.batch;
     const int per = (B + THREADS - 1) / THREADS, b0 = min(B, tid * per), b1 = min(B, b0 + per);
-    long long mine = 0;
+    int mine = 0;
     for (int b = b0; b < b1; ++b) mine += seq_tiles(seq_tokens(a, b), tile) * units;
-    long long incl = mine;
+    int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, incl, o);
+        const int x = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += x;
     }
     if (lane == 31) s_part[tid >> 5] = incl;
     __syncthreads();
-    long long before = 0, total = 0;
+    int before = 0, total = 0;
+#pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) {
         if (w < (tid >> 5)) before += s_part[w];
         total += s_part[w];
     }
     before += incl - mine;
-    const long long want = (total + min_tiles - 1) / min_tiles;
-    const int ctas = (int)min((long long)gridDim.x, max(want, 1ll)), c = blockIdx.x;
-    const long long lo = c < ctas ? c * total / ctas : total, hi = c < ctas ? (c + 1) * total / ctas : total;
-    if (tid == 0) {
-        s->lo = lo;
-        s->hi = hi;
-        s->total = total;
-        s->ctas = ctas;
-    }
-    if (lo >= before && lo < before + mine) {
-        long long base = before;
-        int b = b0;
-        for (;; ++b) {
-            const long long n = seq_tiles(seq_tokens(a, b), tile) * units;
-            if (lo < base + n) break;
-            base += n;
+    const int ctas = min((int)gridDim.x, max(1, (total + min_tiles - 1) / min_tiles));
+    Share t;
+    t.each = total / ctas;
+    t.more = total - t.each * ctas;
+    t.total = total;
+    const int c = blockIdx.x;
+    t.lo = c < ctas ? t.first_of(c) : total;
+    t.hi = c < ctas ? t.first_of(c + 1) : total;
+    t.b = 0;
+    t.base = 0;
+    if (t.lo >= before && t.lo < before + mine) {   // one thread
+        t.base = before;
+        for (t.b = b0;; ++t.b) {
+            const int n = seq_tiles(seq_tokens(a, t.b), tile) * units;
+            if (t.lo < t.base + n) break;
+            t.base += n;
         }
-        s->b = b;
-        s->base = base;
+        *s = t;
+    } else if (t.lo == total && tid == 0) {         // nothing for this CTA
+        *s = t;
     }
     __syncthreads();
 }
 
-// The CTA whose share holds tile i.
-__device__ __forceinline__ int owner_of(const Share& s, long long i) {
-    return (int)(((i + 1) * s.ctas - 1) / s.total);
-}
-
 // Tokens [0, n) of its sequence that query i of sequence b sees.
-__device__ __forceinline__ int64_t seen_by(const skv_pool_attention_args& a, int b, int64_t tokens, int i) {
-    const int n_new = a.new_lengths ? a.new_lengths[b] : a.S_q;
-    return i >= n_new ? 0 : a.causal ? tokens - n_new + 1 + i : tokens;
+__device__ __forceinline__ int seen_by(const skv_pool_attention_args& a, int b, int tokens, int i) {
+    const int n_new = a.new_lengths ? __ldg(a.new_lengths + b) : a.S_q;
+    return i >= n_new ? 0 : a.causal ? max(0, tokens - n_new + 1 + i) : tokens;
 }
 
 struct Segment {
     int b, hk, rt;             // unit
-    int64_t tokens;            // of the sequence
-    long long t0, t1;          // its tiles [t0, t1) are this CTA's
-    long long first, last;     // global numbers of the unit's first and last tile
+    int tokens;                // of the sequence
+    int t0, t1;                // its tiles [t0, t1) are this CTA's
+    int first, last;           // global numbers of the unit's first and last tile
     bool whole;
     int slot;                  // partial slot of this CTA (0 or 1) if not whole
 };
 
 // The segment that starts at tile `at` of the share.
-__device__ __forceinline__ Segment segment_at(const skv_pool_attention_args& a, const Share& s, long long at, int tile,
-                                              int row_tiles, int& b, long long& base) {
+__device__ __forceinline__ Segment segment_at(const skv_pool_attention_args& a, const Share& s, int at, int tile,
+                                              int row_tiles, int& b, int& base) {
     Segment g;
     const int units = a.pool.heads * row_tiles;
     for (;;) {
         g.tokens = seq_tokens(a, b);
-        const long long nt = seq_tiles(g.tokens, tile);
+        const int nt = seq_tiles(g.tokens, tile);
         if (at < base + nt * units) {
-            const long long u = (at - base) / nt;
+            const int u = (at - base) / nt;
             g.b = b;
-            g.hk = (int)(u / row_tiles);
-            g.rt = (int)(u % row_tiles);
+            g.hk = u / row_tiles;
+            g.rt = u - g.hk * row_tiles;
             g.first = base + u * nt;
             g.last = g.first + nt - 1;
             g.t0 = at - g.first;
@@ -121,25 +122,25 @@ __device__ __forceinline__ Segment segment_at(const skv_pool_attention_args& a, 
 
 // ------------------------------------------------------------------------------------- publishing
 // Scratch: kMaxCtas arrival counters (zeroed before the launch), then two slots a CTA of
-// rows * (D + 2) floats: O [rows][D], max [rows], sum [rows].
+// rows * (D + 2) floats (rounded up to 16 bytes): O [rows][D], max [rows], sum [rows].
 __device__ __forceinline__ float* slot_of(const skv_pool_attention_args& a, int cta, int slot, int rows) {
     return reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kMaxCtas * 4) +
            ((int64_t)2 * cta + slot) * rows * (a.pool.head_dim + 2);
 }
 
-// Called by all threads once the CTA's part is in its slot; true for the CTA that joins.
+// Called by all threads once the CTA's part is in its slot; true for the CTA that joins.  The barrier puts
+// every thread's stores before thread 0's fence, which puts them before its arrival.
 __device__ __forceinline__ bool arrive(const skv_pool_attention_args& a, const Share& s, const Segment& g) {
     __shared__ int s_last;
-    __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
-        const int c0 = owner_of(s, g.first), c1 = owner_of(s, g.last);
+        __threadfence();
+        const int c0 = s.owner_of(g.first), c1 = s.owner_of(g.last);
         s_last = atomicAdd(reinterpret_cast<int*>(a.scratch) + c0, 1) == c1 - c0;
+        __threadfence();
     }
     __syncthreads();
-    const bool last = s_last;
-    if (last) __threadfence();
-    return last;
+    return s_last;
 }
 
 // Where query row r of a unit lives (r counts head-major: H_q / heads heads of S_q tokens).
@@ -148,35 +149,184 @@ __device__ __forceinline__ T* row_ptr(const skv_rows& x, int S_q, int rep, int b
     return static_cast<T*>(x.ptr) + b * x.stride_b + (int64_t)(hk * rep + r / S_q) * x.stride_h + (r % S_q) * x.stride_s;
 }
 
-// Value d of output row r of a unit, rounded to the output's type.
-__device__ __forceinline__ void store_out(const skv_pool_attention_args& a, int b, int hk, int r, int d, float x) {
+// Values d .. d + VEC - 1 of output row r of a unit, rounded to the output's type (VEC 4: aligned rows).
+template <int VEC>
+__device__ __forceinline__ void store_out(const skv_pool_attention_args& a, int b, int hk, int r, int d, const float (&x)[VEC]) {
     const int rep = a.q.heads / a.pool.heads;
-    if (a.out.dtype == kF32) row_ptr<float>(a.out, a.S_q, rep, b, hk, r)[d] = x;
-    else if (a.out.dtype == kF16) row_ptr<__half>(a.out, a.S_q, rep, b, hk, r)[d] = __float2half_rn(x);
-    else row_ptr<__nv_bfloat16>(a.out, a.S_q, rep, b, hk, r)[d] = __float2bfloat16_rn(x);
+    if (a.out.dtype == kF32) {
+        float* p = row_ptr<float>(a.out, a.S_q, rep, b, hk, r) + d;
+        if constexpr (VEC == 4) *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+        else p[0] = x[0];
+    } else if (a.out.dtype == kF16) {
+        __half* p = row_ptr<__half>(a.out, a.S_q, rep, b, hk, r) + d;
+        if constexpr (VEC == 4) {
+            const __half2 u = __floats2half2_rn(x[0], x[1]), v = __floats2half2_rn(x[2], x[3]);
+            *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&v));
+        } else {
+            p[0] = __float2half_rn(x[0]);
+        }
+    } else {
+        __nv_bfloat16* p = row_ptr<__nv_bfloat16>(a.out, a.S_q, rep, b, hk, r) + d;
+        if constexpr (VEC == 4) {
+            const __nv_bfloat162 u = __floats2bfloat162_rn(x[0], x[1]), v = __floats2bfloat162_rn(x[2], x[3]);
+            *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&v));
+        } else {
+            p[0] = __float2bfloat16_rn(x[0]);
+        }
+    }
 }
 
-// Joins the parts of a unit in token order, a thread for each value of each row.
-template <int ROWS>
-__device__ __forceinline__ void join(const skv_pool_attention_args& a, const Share& s, const Segment& g, int R) {
-    const int D = a.pool.head_dim;
-    const int c0 = owner_of(s, g.first), c1 = owner_of(s, g.last);
-    const bool c0_starts = g.first == c0 * s.total / s.ctas;   // the unit starts at c0's first tile
-    for (int i = threadIdx.x; i < ROWS * D; i += blockDim.x) {
-        const int j = i / D, d = i - j * D, r = g.rt * ROWS + j;
-        if (r >= R) break;
-        float m = -INFINITY, l = 0.0f, o = 0.0f;
-        for (int c = c0; c <= c1; ++c) {
-            const float* p = slot_of(a, c, c == c0 && !c0_starts ? 1 : 0, ROWS);
-            const float mi = __ldcg(p + ROWS * D + j), li = __ldcg(p + ROWS * D + ROWS + j), oi = __ldcg(p + j * D + d);
-            const float mn = fmaxf(m, mi), ref = mn == -INFINITY ? 0.0f : mn;
-            const float wa = exp2f(m - ref), wb = exp2f(mi - ref);
-            l = l * wa + li * wb;
-            o = o * wa + oi * wb;
-            m = mn;
+__device__ __forceinline__ void store_row(const skv_pool_attention_args& a, const Segment& g, int r, int d, bool vec, const float (&y)[4]) {
+    if (vec) {
+        store_out<4>(a, g.b, g.hk, r, d, y);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float one[1] = {y[k]};
+            store_out<1>(a, g.b, g.hk, r, d + k, one);
         }
-        store_out(a, g.b, g.hk, r, d, l == 0.0f ? 0.0f : o / l);
     }
+}
+
+template <int VEC>
+__device__ __forceinline__ void load_part(const float* p, float (&x)[VEC]) {
+    if constexpr (VEC == 4) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(p));
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else {
+        x[0] = __ldcg(p);
+    }
+}
+
+// Joins the parts of a unit in token order.  A joining CTA's time is latency, one L2 round trip after the
+// other, so loads are issued in batches of 16 a thread: first the maxima and sums of all parts (THREADS / ROWS
+// threads a row), which leave the parts' factors in shared memory, then the values, VEC to a load.  Where
+// the rows have fewer loads than the block has threads, `ways` threads take every ways-th part of a value, and
+// their sums are added in order.  buf: join_floats of shared memory.
+constexpr int kJoinWays = 8;
+template <int ROWS, int THREADS, int PARTS>
+__host__ __device__ constexpr int join_floats() { return PARTS * ROWS + 2 * ROWS + THREADS * 4; }
+
+template <int ROWS, int THREADS, int VEC, int PARTS>
+__device__ __forceinline__ void join(const skv_pool_attention_args& a, const Share& s, const Segment& g, int R, float* buf, bool out_vec = false) {
+    const int D = a.pool.head_dim, tid = threadIdx.x, rows = min(ROWS, R - g.rt * ROWS), items = rows * D / VEC;
+    const int c0 = s.owner_of(g.first), parts = s.owner_of(g.last) - c0 + 1;
+    // part i lies at base + i * stride, the first one in its CTA's second slot unless it starts that CTA's share
+    const int64_t stride = (int64_t)2 * ROWS * (D + 2);
+    const float* base = slot_of(a, c0, 0, ROWS);
+    const float* part0 = slot_of(a, c0, g.first == s.first_of(c0) ? 0 : 1, ROWS);
+    auto part = [&](int i) { return i == 0 ? part0 : base + i * stride; };
+    float* s_f = buf;                  // [PARTS][ROWS] 2^(m_i - m) of a block of parts
+    float* s_m = s_f + PARTS * ROWS;   // [ROWS] max over all parts (0 if there is none)
+    float* s_l = s_m + ROWS;           // [ROWS] sum over all parts
+    float* s_add = s_l + ROWS;         // [THREADS][VEC]
+    __syncthreads();
+    {
+        constexpr int TPR = THREADS / ROWS;   // a power of two, at most 32
+        const int j = tid / TPR, sub = tid % TPR;
+        float m = -INFINITY, l = 0.0f;
+        for (int i0 = sub; i0 < parts; i0 += 8 * TPR) {
+            float mi[8], li[8], top = m;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int i = i0 + k * TPR;
+                const float* p = part(min(i, parts - 1)) + ROWS * D + min(j, rows - 1);
+                mi[k] = i < parts ? __ldcg(p) : -INFINITY;
+                li[k] = i < parts ? __ldcg(p + ROWS) : 0.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                top = fmaxf(top, mi[k]);
+                if (i0 + k * TPR < min(parts, PARTS)) s_f[(i0 + k * TPR) * ROWS + j] = mi[k];
+            }
+            const float r = top == -INFINITY ? 0.0f : top;
+            l *= exp2f(m - r);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) l += li[k] * exp2f(mi[k] - r);
+            m = top;
+        }
+#pragma unroll
+        for (int o = 1; o < TPR; o <<= 1) {
+            const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
+            const float top = fmaxf(m, m2), r = top == -INFINITY ? 0.0f : top;
+            l = l * exp2f(m - r) + l2 * exp2f(m2 - r);
+            m = top;
+        }
+        const float r = m == -INFINITY ? 0.0f : m;
+        for (int i = sub; i < min(parts, PARTS); i += TPR) s_f[i * ROWS + j] = exp2f(s_f[i * ROWS + j] - r);
+        if (sub == 0) {
+            s_m[j] = r;
+            s_l[j] = l;
+        }
+    }
+    __syncthreads();
+    const int ways = items >= THREADS ? 1 : min(THREADS / items, kJoinWays), wide = THREADS / ways;
+    const int way = tid / wide;
+    constexpr int I = ROWS >= 16 ? 4 : 2;   // values of a thread at a time
+    for (int v0 = 0; v0 < items; v0 += I * wide) {
+        float y[I][VEC];
+        int v[I], row[I];
+#pragma unroll
+        for (int n = 0; n < I; ++n) {
+            v[n] = v0 + n * wide + tid - way * wide;
+            row[n] = v[n] < items ? v[n] * VEC / D : 0;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) y[n][e] = 0.0f;
+        }
+        for (int i0 = 0; i0 < parts; i0 += PARTS) {
+            const int count = min(PARTS, parts - i0);
+            if (parts > PARTS) {   // more parts than factors fit: block by block
+                __syncthreads();
+                for (int i = tid; i < count * rows; i += THREADS) {
+                    const int k = i / rows, r = i - k * rows;
+                    s_f[k * ROWS + r] = exp2f(__ldcg(part(i0 + k) + ROWS * D + r) - s_m[r]);
+                }
+                __syncthreads();
+            }
+            if (way >= ways) continue;
+            for (int k0 = way; k0 < count; k0 += 16 / I * ways) {
+                float x[16 / I][I][VEC];
+#pragma unroll
+                for (int u = 0; u < 16 / I; ++u)
+#pragma unroll
+                    for (int n = 0; n < I; ++n) {
+                        const int k = k0 + u * ways;
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) x[u][n][e] = 0.0f;
+                        if (k < count && v[n] < items) load_part<VEC>(part(i0 + k) + v[n] * VEC, x[u][n]);
+                    }
+#pragma unroll
+                for (int u = 0; u < 16 / I; ++u)
+#pragma unroll
+                    for (int n = 0; n < I; ++n) {
+                        const int k = k0 + u * ways;
+                        const float f = k < count ? s_f[k * ROWS + row[n]] : 0.0f;
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) y[n][e] = fmaf(x[u][n][e], f, y[n][e]);
+                    }
+            }
+        }
+        if (ways > 1) {   // items < THREADS: one value a thread, n = 0
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) s_add[tid * VEC + e] = y[0][e];
+            __syncthreads();
+            if (way == 0)
+                for (int w = 1; w < ways; ++w)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) y[0][e] += s_add[(w * wide + tid) * VEC + e];
+        }
+        if (way == 0) {
+#pragma unroll
+            for (int n = 0; n < I; ++n)
+                if (v[n] < items && (ways == 1 || n == 0)) {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) y[n][e] = s_l[row[n]] == 0.0f ? 0.0f : y[n][e] / s_l[row[n]];
+                    if constexpr (VEC == 4) store_row(a, g, g.rt * ROWS + row[n], v[n] * VEC - row[n] * D, out_vec, y[n]);
+                    else store_out<1>(a, g.b, g.hk, g.rt * ROWS + row[n], v[n] - row[n] * D, y[n]);
+                }
+        }
+    }
+    __syncthreads();
 }
 
 }  // namespace skv

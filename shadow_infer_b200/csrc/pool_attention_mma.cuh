@@ -31,18 +31,18 @@
 
 namespace skv {
 
-constexpr int kMmaWarps = 4, kMmaThreads = 32 * kMmaWarps, kMmaTile = 16 * kMmaWarps;
+constexpr int kMmaWarps = 4, kMmaThreads = 32 * kMmaWarps, kMmaTile = 16 * kMmaWarps, kMmaParts = 128;
 constexpr float kRefDrop = 5.0f;    // a fresh maximum's weight is 2^5: small weights keep their bits in fp16
 constexpr float kRefRoom = 14.0f;   // weights may grow to 2^14 (times a mantissa < 2) before ref moves
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint2 b) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -134,7 +134,7 @@ struct VTile;
 template <int DP>
 struct KTile<1, DP> {
     uint4 x[2][DP / 32];
-    __device__ __forceinline__ void load(const skv_pool& p, const int64_t (&row)[2], int c) {
+    __device__ __forceinline__ void load(const skv_pool& p, const int (&row)[2], int c) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -142,7 +142,7 @@ struct KTile<1, DP> {
                 const int chunk = c + 4 * j;
                 x[t][j] = make_uint4(0, 0, 0, 0);
                 if (row[t] >= 0 && chunk * 8 < p.head_dim)
-                    x[t][j] = load_page16(static_cast<const __half*>(p.k) + row[t] * p.head_dim + chunk * 8);
+                    x[t][j] = load_page16(static_cast<const __half*>(p.k) + (int64_t)row[t] * p.head_dim + chunk * 8);
             }
     }
 };
@@ -150,7 +150,7 @@ template <int DP>
 struct KTile<2, DP> {
     uint4 x[2][DP / 64];
     float s[2];
-    __device__ __forceinline__ void load(const skv_pool& p, const int64_t (&row)[2], int c) {
+    __device__ __forceinline__ void load(const skv_pool& p, const int (&row)[2], int c) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
 #pragma unroll
@@ -158,7 +158,7 @@ struct KTile<2, DP> {
                 const int chunk = c + 4 * j;
                 x[t][j] = make_uint4(0, 0, 0, 0);
                 if (row[t] >= 0 && chunk * 16 < p.head_dim)
-                    x[t][j] = load_page16(static_cast<const int8_t*>(p.k) + row[t] * p.head_dim + chunk * 16);
+                    x[t][j] = load_page16(static_cast<const int8_t*>(p.k) + (int64_t)row[t] * p.head_dim + chunk * 16);
             }
             s[t] = row[t] >= 0 ? __ldg(p.scale_k + row[t]) : 0.0f;
         }
@@ -168,7 +168,7 @@ template <int DP>
 struct KTile<3, DP> {
     uint2 x[2][DP / 64];
     float s[2][DP / 64];
-    __device__ __forceinline__ void load(const skv_pool& p, const int64_t (&row)[2], int c) {
+    __device__ __forceinline__ void load(const skv_pool& p, const int (&row)[2], int c) {
         const int ng = p.head_dim / p.int4_group;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -179,8 +179,8 @@ struct KTile<3, DP> {
                 x[t][j] = make_uint2(0x88888888u, 0x88888888u);
                 s[t][j] = 0.0f;
                 if (on) {
-                    x[t][j] = load_page8(static_cast<const uint8_t*>(p.k) + row[t] * (p.head_dim / 2) + chunk * 8);
-                    s[t][j] = __ldg(p.scale_k + row[t] * ng + chunk * 16 / p.int4_group);
+                    x[t][j] = load_page8(static_cast<const uint8_t*>(p.k) + (int64_t)row[t] * (p.head_dim / 2) + chunk * 8);
+                    s[t][j] = __ldg(p.scale_k + (int64_t)row[t] * ng + chunk * 16 / p.int4_group);
                 }
             }
     }
@@ -189,7 +189,7 @@ struct KTile<3, DP> {
 template <int DP>
 struct VTile<1, DP> {
     uint4 x[4][DP / 64];
-    __device__ __forceinline__ void load(const skv_pool& p, const int64_t (&row)[4], const int64_t (&)[2], int g, int) {
+    __device__ __forceinline__ void load(const skv_pool& p, const int (&row)[4], const int (&)[2], int g, int) {
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -197,7 +197,7 @@ struct VTile<1, DP> {
                 const int chunk = g + 8 * j;
                 x[t][j] = make_uint4(0, 0, 0, 0);
                 if (row[t] >= 0 && chunk * 8 < p.head_dim)
-                    x[t][j] = load_page16(static_cast<const __half*>(p.v) + row[t] * p.head_dim + chunk * 8);
+                    x[t][j] = load_page16(static_cast<const __half*>(p.v) + (int64_t)row[t] * p.head_dim + chunk * 8);
             }
     }
 };
@@ -205,13 +205,13 @@ template <int DP>
 struct VTile<2, DP> {
     uint32_t x[4][DP / 32];
     float s[2];   // of tokens g and g + 8
-    __device__ __forceinline__ void load(const skv_pool& p, const int64_t (&row)[4], const int64_t (&own)[2], int g, int) {
+    __device__ __forceinline__ void load(const skv_pool& p, const int (&row)[4], const int (&own)[2], int g, int) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
 #pragma unroll
             for (int w = 0; w < DP / 32; ++w) x[t][w] = 0;
             if (row[t] >= 0 && g * (DP / 8) < p.head_dim) {
-                const int8_t* q = static_cast<const int8_t*>(p.v) + row[t] * p.head_dim + g * (DP / 8);
+                const int8_t* q = static_cast<const int8_t*>(p.v) + (int64_t)row[t] * p.head_dim + g * (DP / 8);
                 if constexpr (DP == 128) {
                     const uint4 u = load_page16(q);
                     x[t][0] = u.x; x[t][1] = u.y; x[t][2] = u.z; x[t][3] = u.w;
@@ -230,7 +230,7 @@ struct VTile<3, DP> {
     uint32_t x[4][DP / 64];
     float s[4];              // of this lane's values, tokens 2c, 2c + 1, 2c + 8, 2c + 9
     float own[2][DP / 64];   // this lane's quarter of the scales of tokens g and g + 8
-    __device__ __forceinline__ void load(const skv_pool& p, const int64_t (&row)[4], const int64_t (&mine)[2], int g, int c) {
+    __device__ __forceinline__ void load(const skv_pool& p, const int (&row)[4], const int (&mine)[2], int g, int c) {
         const int ng = p.head_dim / p.int4_group;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -238,14 +238,14 @@ struct VTile<3, DP> {
             for (int w = 0; w < DP / 64; ++w) x[t][w] = 0x88888888u;
             s[t] = 0.0f;
             if (row[t] >= 0 && g * (DP / 8) < p.head_dim) {
-                const uint8_t* q = static_cast<const uint8_t*>(p.v) + row[t] * (p.head_dim / 2) + g * (DP / 16);
+                const uint8_t* q = static_cast<const uint8_t*>(p.v) + (int64_t)row[t] * (p.head_dim / 2) + g * (DP / 16);
                 if constexpr (DP == 128) {
                     const uint2 u = load_page8(q);
                     x[t][0] = u.x; x[t][1] = u.y;
                 } else {
                     x[t][0] = load_page4(q);
                 }
-                s[t] = __ldg(p.scale_v + row[t] * ng + g * (DP / 8) / p.int4_group);
+                s[t] = __ldg(p.scale_v + (int64_t)row[t] * ng + g * (DP / 8) / p.int4_group);
             }
         }
 #pragma unroll
@@ -253,10 +253,45 @@ struct VTile<3, DP> {
 #pragma unroll
             for (int j = 0; j < DP / 64; ++j) {
                 const int chunk = c + 4 * j;
-                own[t][j] = mine[t] >= 0 && chunk * 16 < p.head_dim ? __ldg(p.scale_v + mine[t] * ng + chunk * 16 / p.int4_group) : 0.0f;
+                own[t][j] = mine[t] >= 0 && chunk * 16 < p.head_dim ? __ldg(p.scale_v + (int64_t)mine[t] * ng + chunk * 16 / p.int4_group) : 0.0f;
             }
     }
 };
+
+// E values of a row of which `left` exist, with one load where rows are aligned to them (their count is a
+// multiple of E then, as head sizes here are multiples of 8).
+template <int E, class T>
+__device__ __forceinline__ void load_row(const T* p, int left, bool vec, float (&x)[E]) {
+    if (vec) {
+        if constexpr (sizeof(T) == 4) {
+            if constexpr (E == 4) {
+                const float4 v = *reinterpret_cast<const float4*>(p);
+                x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+            } else {
+                const float2 v = *reinterpret_cast<const float2*>(p);
+                x[0] = v.x; x[1] = v.y;
+            }
+        } else {
+            uint32_t w[E / 2];
+            if constexpr (E == 4) {
+                const uint2 v = *reinterpret_cast<const uint2*>(p);
+                w[0] = v.x; w[1] = v.y;
+            } else {
+                w[0] = *reinterpret_cast<const uint32_t*>(p);
+            }
+#pragma unroll
+            for (int i = 0; i < E / 2; ++i) {
+                const T* h = reinterpret_cast<const T*>(&w[i]);
+                x[2 * i] = to_float(h[0]);
+                x[2 * i + 1] = to_float(h[1]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (i < left) x[i] = to_float(p[i]);
+    }
+}
 
 // Where value d of a query row sits in the B operands: MMA, lane column c, register and half.
 template <int PREC>
@@ -275,18 +310,19 @@ __device__ __forceinline__ void query_place(int d, int& mma, int& c, int& reg, i
 
 template <int DP, int NT, int NQ>
 __host__ __device__ constexpr size_t mma_smem() {
-    return (size_t)(DP / 16) * NT * NQ * 32 * 8 + (size_t)kMmaWarps * 8 * NT * (DP + 2) * 4 + (3 * kMmaWarps + 2) * 8 * NT * 4;
+    static_assert(join_floats<8 * NT, kMmaThreads, kMmaParts>() <= kMmaWarps * 8 * NT * (DP + 4), "the join works in the warps' sums");
+    return (size_t)(DP / 16) * NT * NQ * 32 * 8 + (size_t)kMmaWarps * 8 * NT * (DP + 4) * 4 + (3 * kMmaWarps + 2) * 8 * NT * 4;
 }
 
 template <int PREC, int DP, int NT, int NQ, int NP, int CTAS>
 __global__ void __launch_bounds__(kMmaThreads, CTAS)
-pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int row_tiles) {
+pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int row_tiles, bool q_vec, bool out_vec) {
     constexpr int M = DP / 16, ROWS = 8 * NT;
     extern __shared__ __align__(16) char mma_sm[];
     __shared__ Share s;
     uint2* s_q = reinterpret_cast<uint2*>(mma_sm);                       // [M][NT][NQ][32]
-    float* s_o = reinterpret_cast<float*>(s_q + M * NT * NQ * 32);       // [warps][ROWS][DP + 2]
-    float* s_ref = s_o + kMmaWarps * ROWS * (DP + 2);                    // [warps][ROWS]
+    float* s_o = reinterpret_cast<float*>(s_q + M * NT * NQ * 32);       // [warps][ROWS][DP + 4]
+    float* s_ref = s_o + kMmaWarps * ROWS * (DP + 4);                    // [warps][ROWS]
     float* s_sum = s_ref + kMmaWarps * ROWS;                             // [warps][ROWS]
     float* s_w = s_sum + kMmaWarps * ROWS;                               // [warps][ROWS]
     float* s_c = s_w + kMmaWarps * ROWS;                                 // [ROWS] factor of a row's scores; later its max
@@ -296,39 +332,84 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
     const int rep = a.q.heads / a.pool.heads, R = rep * a.S_q;
     const bool p16 = P % 16 == 0;   // a tile lies in one page
     take_share<kMmaThreads>(a, kMmaTile, a.pool.heads * row_tiles, 1, &s);
-    int b = s.b;
-    long long base = s.base;
-    for (long long at = s.lo; at < s.hi;) {
+    int b = s.b, base = s.base;
+    for (int at = s.lo; at < s.hi;) {
         const Segment g = segment_at(a, s, at, kMmaTile, row_tiles, b, base);
         at += g.t1 - g.t0;
-        const int n = (int)g.tokens, r0 = g.rt * ROWS;
+        const int n = g.tokens, r0 = g.rt * ROWS;
+        const int end = min(g.t1 * kMmaWarps, (n + 15) / 16);
+        int st = g.t0 * kMmaWarps + warp;
+        PageRows pages;
+        if (p16) pages.start(a.pool, g.b, st * 16 / P);
+        // the pool row of token lane % 16 of a tile, -1 where there is none
+        auto row_of = [&](int tile) {
+            const int t0 = tile * 16, t = t0 + (lane & 15);
+            int row = -1;
+            if (p16) {
+                const int j = t0 / P, page = pages.page(j);
+                if (t < n && page >= 0 && page < a.pool.num_pages) row = (page * a.pool.heads + g.hk) * P + (t - j * P);
+            } else if (t < n) {
+                const int64_t r = pool_row(a.pool, g.b, t);
+                if (r >= 0) row = (int)r + g.hk * P;
+            }
+            if (t < n && row < 0 && a.error_flag) atomicExch(a.error_flag, 1);
+            return row;
+        };
+        // the rows of the tokens whose K (g, g + 8) and V (2c, 2c + 1, 2c + 8, 2c + 9) this lane loads
+        auto k_rows = [&](int row, int (&own)[2]) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) own[i] = __shfl_sync(0xffffffffu, row, lg + 8 * i);
+        };
+        auto v_rows = [&](int row, int (&four)[4]) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) four[i] = __shfl_sync(0xffffffffu, row, 2 * lc + (i & 1) + 8 * (i >> 1));
+        };
+        KTile<PREC, DP> kt;
+        VTile<PREC, DP> vt;
+        int row = -1, next = -1;   // of this tile's tokens, of the next one's
+        if (st < end) {
+            int own[2], four[4];
+            row = row_of(st);
+            k_rows(row, own);
+            v_rows(row, four);
+            kt.load(a.pool, own, lc);
+            vt.load(a.pool, four, own, lg, lc);
+        }
         // ---- queries: a power of two taken out of each row, laid out as B operands
         __syncthreads();
-        for (int j = warp; j < ROWS; j += kMmaWarps) {
-            float x[DP / 32], top = 0.0f;
+        {
+            constexpr int RW = ROWS / kMmaWarps, E = DP / 32;   // a warp's rows, a lane's values of each
+            float x[RW][E];
 #pragma unroll
-            for (int i = 0; i < DP / 32; ++i) {
-                const int d = lane + 32 * i;
-                x[i] = 0.0f;
-                if (r0 + j < R && d < D) {
-                    if (a.q.dtype == kF32) x[i] = row_ptr<const float>(a.q, a.S_q, rep, g.b, g.hk, r0 + j)[d];
-                    else if (a.q.dtype == kF16) x[i] = __half2float(row_ptr<const __half>(a.q, a.S_q, rep, g.b, g.hk, r0 + j)[d]);
-                    else x[i] = __bfloat162float(row_ptr<const __nv_bfloat16>(a.q, a.S_q, rep, g.b, g.hk, r0 + j)[d]);
+            for (int i = 0; i < RW; ++i) {   // every load before the first use
+                const int r = r0 + warp * RW + i, d = lane * E;
+#pragma unroll
+                for (int k = 0; k < E; ++k) x[i][k] = 0.0f;
+                if (r < R && d < D) {
+                    if (a.q.dtype == kF32) load_row<E>(row_ptr<const float>(a.q, a.S_q, rep, g.b, g.hk, r) + d, D - d, q_vec, x[i]);
+                    else if (a.q.dtype == kF16) load_row<E>(row_ptr<const __half>(a.q, a.S_q, rep, g.b, g.hk, r) + d, D - d, q_vec, x[i]);
+                    else load_row<E>(row_ptr<const __nv_bfloat16>(a.q, a.S_q, rep, g.b, g.hk, r) + d, D - d, q_vec, x[i]);
                 }
-                top = fmaxf(top, fabsf(x[i]));
             }
-            const int e = clamp_exp(__float_as_uint(warp_max(top)));
-            const float down = exp_down(e);
-            if (lane == 0) s_c[j] = a.scale * 1.4426950408889634f * exp_up(e);
 #pragma unroll
-            for (int i = 0; i < DP / 32; ++i) {
-                int mma, c, reg, half;
-                query_place<PREC>(lane + 32 * i, mma, c, reg, half);
-                const float y = x[i] * down;
-                const __half hi = __float2half_rn(y);
-                __half* q = reinterpret_cast<__half*>(s_q + ((mma * NT + j / 8) * NQ) * 32 + (j % 8) * 4 + c) + 2 * reg + half;
-                q[0] = hi;
-                if (NQ == 2) q[32 * 4] = __float2half_rn(y - __half2float(hi));
+            for (int i = 0; i < RW; ++i) {
+                const int j = warp * RW + i;
+                float top = 0.0f;
+#pragma unroll
+                for (int k = 0; k < E; ++k) top = fmaxf(top, fabsf(x[i][k]));
+                const int e = clamp_exp(__float_as_uint(warp_max(top)));
+                const float down = exp_down(e);
+                if (lane == 0) s_c[j] = a.scale * 1.4426950408889634f * exp_up(e);
+#pragma unroll
+                for (int k = 0; k < E; ++k) {
+                    int mma, c, reg, half;
+                    query_place<PREC>(lane * E + k, mma, c, reg, half);
+                    const float y = x[i][k] * down;
+                    const __half hi = __float2half_rn(y);
+                    __half* q = reinterpret_cast<__half*>(s_q + ((mma * NT + j / 8) * NQ) * 32 + (j % 8) * 4 + c) + 2 * reg + half;
+                    q[0] = hi;
+                    if (NQ == 2) q[32 * 4] = __float2half_rn(y - __half2float(hi));
+                }
             }
         }
         __syncthreads();
@@ -342,7 +423,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                 cf[t][i] = s_c[j];
                 ref[t][i] = -INFINITY;
                 sum[t][i] = 0.0f;
-                see[t][i] = r0 + j < R ? (int)max(seen_by(a, g.b, g.tokens, (r0 + j) % a.S_q), (int64_t)0) : n;
+                see[t][i] = r0 + j < R ? seen_by(a, g.b, n, (r0 + j) % a.S_q) : n;
                 see_all = min(see_all, see[t][i]);
             }
         see_all = min(see_all, __shfl_xor_sync(0xffffffffu, see_all, 1));
@@ -354,55 +435,9 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[t][m][i] = 0.0f;
 
-        const int end = min((int)g.t1 * kMmaWarps, (n + 15) / 16);
-        int st = (int)g.t0 * kMmaWarps + warp;
-        PageRows pages;
-        if (p16) pages.start(a.pool, g.b, st * 16 / P);
-        // rows of a tile's tokens: `own` g, g + 8; `four` 2c, 2c + 1, 2c + 8, 2c + 9; -1 where there is none
-        auto rows_of = [&](int tile, int64_t (&own)[2], int64_t (&four)[4]) {
-            const int t0 = tile * 16;
-            if (p16) {
-                const int j = t0 / P, page = pages.page(j);
-                const bool ok = page >= 0 && page < a.pool.num_pages;
-                const int64_t row = ((int64_t)page * a.pool.heads + g.hk) * P + (t0 - j * P);
-                if (!ok && lane == 0 && a.error_flag) atomicExch(a.error_flag, 1);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) own[i] = ok && t0 + lg + 8 * i < n ? row + lg + 8 * i : -1;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int k = 2 * lc + (i & 1) + 8 * (i >> 1);
-                    four[i] = ok && t0 + k < n ? row + k : -1;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int t = t0 + lg + 8 * i;
-                    own[i] = t < n ? pool_row(a.pool, g.b, t) : -1;
-                    if (t < n && own[i] < 0 && a.error_flag) atomicExch(a.error_flag, 1);
-                    if (own[i] >= 0) own[i] += (int64_t)g.hk * P;
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int t = t0 + 2 * lc + (i & 1) + 8 * (i >> 1);
-                    four[i] = t < n ? pool_row(a.pool, g.b, t) : -1;
-                    if (four[i] >= 0) four[i] += (int64_t)g.hk * P;
-                }
-            }
-        };
-        KTile<PREC, DP> kt;
-        VTile<PREC, DP> vt;
-        int64_t own[2], four[4];
-        bool here[2] = {false, false};
-        if (st < end) {
-            rows_of(st, own, four);
-            kt.load(a.pool, own, lc);
-            vt.load(a.pool, four, own, lg, lc);
-            here[0] = own[0] >= 0;
-            here[1] = own[1] >= 0;
-        }
         for (; st < end; st += kMmaWarps) {
             const bool more = st + kMmaWarps < end;
-            if (more) rows_of(st + kMmaWarps, own, four);
+            next = more ? row_of(st + kMmaWarps) : -1;
             // ---- scores
             float x[NT][4];
 #pragma unroll
@@ -474,7 +509,11 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                     }
                 }
             }
-            if (more) kt.load(a.pool, own, lc);
+            int own[2];
+            if (more) {
+                k_rows(next, own);
+                kt.load(a.pool, own, lc);
+            }
             // ---- weights
             float v_add[2] = {0.0f, 0.0f}, v_mul[2] = {1.0f, 1.0f}, v_sum[2] = {1.0f, 1.0f};
             int ve[2] = {0, 0};
@@ -500,7 +539,12 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                 }
             }
             const int t0 = st * 16;
-            const bool all = t0 + 16 <= see_all && p16 && __all_sync(0xffffffffu, here[0]);
+            const bool all = t0 + 16 <= see_all && __all_sync(0xffffffffu, row >= 0);
+            bool here[2] = {true, true};
+            if (!all) {
+                here[0] = __shfl_sync(0xffffffffu, row, lg) >= 0;
+                here[1] = __shfl_sync(0xffffffffu, row, lg + 8) >= 0;
+            }
             bool grow = false;
 #pragma unroll
             for (int t = 0; t < NT; ++t)
@@ -625,10 +669,11 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                     }
             }
             if (more) {
+                int four[4];
+                v_rows(next, four);
                 vt.load(a.pool, four, own, lg, lc);
-                here[0] = own[0] >= 0;
-                here[1] = own[1] >= 0;
             }
+            row = next;
         }
 
         // ---- the warps' parts joined
@@ -645,7 +690,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                     s_ref[warp * ROWS + j] = ref[t][i];
                     s_sum[warp * ROWS + j] = l;
                 }
-                float* row = s_o + (warp * ROWS + j) * (DP + 2);
+                float* row = s_o + (warp * ROWS + j) * (DP + 4);
 #pragma unroll
                 for (int m = 0; m < M; ++m) {
                     const int d = PREC == 1 ? 64 * (m / 4) + 8 * lg + 2 * (m % 4) : lg * (DP / 8) + 2 * m;
@@ -667,21 +712,32 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
         }
         __syncthreads();
         float* part = slot_of(a, blockIdx.x, g.slot, ROWS);
-        for (int i = tid; i < ROWS * D; i += kMmaThreads) {
-            const int j = i / D, d = i - j * D;
-            if (r0 + j >= R) break;
-            float y = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kMmaWarps; ++w) y += s_o[(w * ROWS + j) * (DP + 2) + d] * s_w[w * ROWS + j];
-            if (g.whole) store_out(a, g.b, g.hk, r0 + j, d, s_l[j] == 0.0f ? 0.0f : y / s_l[j]);
-            else part[j * D + d] = y;
+        for (int i = tid; i < ROWS * DP / 4; i += kMmaThreads) {
+            const int j = i / (DP / 4), d = i % (DP / 4) * 4;
+            if (r0 + j >= R || d >= D) continue;
+            float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < kMmaWarps; ++w) {
+                const float4 v = *reinterpret_cast<const float4*>(s_o + (w * ROWS + j) * (DP + 4) + d);
+                const float f = s_w[w * ROWS + j];
+                y[0] = fmaf(v.x, f, y[0]); y[1] = fmaf(v.y, f, y[1]); y[2] = fmaf(v.z, f, y[2]); y[3] = fmaf(v.w, f, y[3]);
+            }
+            if (!g.whole) {
+                *reinterpret_cast<float4*>(part + j * D + d) = make_float4(y[0], y[1], y[2], y[3]);
+                continue;
+            }
+            const float l = s_l[j];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] = l == 0.0f ? 0.0f : y[k] / l;
+            store_row(a, g, r0 + j, d, out_vec, y);
         }
         if (g.whole) continue;
         if (tid < ROWS) {
             part[ROWS * D + tid] = s_c[tid];
             part[ROWS * D + ROWS + tid] = s_l[tid];
         }
-        if (arrive(a, s, g)) join<ROWS>(a, s, g, R);
+        if (arrive(a, s, g)) join<ROWS, kMmaThreads, 4, kMmaParts>(a, s, g, R, s_o, out_vec);
     }
 }
 
@@ -697,7 +753,7 @@ int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
         if (e != cudaSuccess) return fail(SKV_ERR_CUDA, "pool_attention: %s", cudaGetErrorString(e));
     }
     const int R = a.q.heads / a.pool.heads * a.S_q;
-    kernel<<<sm_count() * CTAS, kMmaThreads, smem, st>>>(a, (R + 8 * NT - 1) / (8 * NT));
+    kernel<<<sm_count() * CTAS, kMmaThreads, smem, st>>>(a, (R + 8 * NT - 1) / (8 * NT), rows_aligned(a.q), rows_aligned(a.out));
     return check_launch("pool_attention");
 }
 
