@@ -467,7 +467,7 @@ typedef struct skv_pool_attention_args {
     skv_rows q, out;             /* [B, H_q, S_q, D], one type; H_q a multiple of pool.heads */
     const int32_t* lengths;      /* tokens of each sequence, the new ones included */
     const int32_t* new_lengths;  /* queries of each sequence that are tokens; NULL: all S_q */
-    void* scratch;
+    void* scratch;               /* zero before its first use; every call leaves it ready for the next */
     int64_t scratch_bytes;
     int32_t* error_flag;
     int32_t S_q;
@@ -479,8 +479,11 @@ typedef struct skv_pool_attention_args {
 /* out = softmax(scale q k^T) v over each sequence's tokens; a query that sees no token gives 0, and so
  * does a query i >= new_lengths[b] (the padding of a ragged batch).
  * Query head h reads key head h / (H_q / heads).  scratch: skv_pool_attention_scratch_bytes
- * bytes, 16-byte aligned, any contents. */
+ * bytes, 16-byte aligned, with the first skv_pool_attention_scratch_zeros bytes zero before the
+ * first call that uses it (arrival counters, which every call leaves zero).  Calls that may overlap
+ * on the GPU use scratch of their own. */
 size_t skv_pool_attention_scratch_bytes(int D);
+size_t skv_pool_attention_scratch_zeros(void);
 int skv_pool_attention(const skv_pool_attention_args* args, void* stream);
 
 #ifdef __cplusplus

@@ -133,6 +133,7 @@ _SIGNATURES = {
     "skv_pool_append": (c_int, [ctypes.c_char_p, c_void_p]),
     "skv_pool_read": (c_int, [ctypes.c_char_p, c_void_p]),
     "skv_pool_attention_scratch_bytes": (c_size_t, [c_int]),
+    "skv_pool_attention_scratch_zeros": (c_size_t, []),
     "skv_pool_attention": (c_int, [ctypes.c_char_p, c_void_p]),
 }
 

@@ -189,6 +189,8 @@ size_t skv_pool_attention_scratch_bytes(int D) {
     return D <= 0 ? 0 : (size_t)kMaxCtas * 4 + (size_t)sm_count() * kRowsPerSm * (D + 2) * 4;
 }
 
+size_t skv_pool_attention_scratch_zeros(void) { return (size_t)kMaxCtas * 4; }
+
 int skv_pool_attention(const skv_pool_attention_args* args, void* stream) {
     if (!args) return fail(SKV_ERR_INVALID_ARGUMENT, "pool_attention: null pointer");
     const skv_pool_attention_args& a = *args;
@@ -212,8 +214,6 @@ int skv_pool_attention(const skv_pool_attention_args* args, void* stream) {
     if (a.scratch_bytes < (int64_t)skv_pool_attention_scratch_bytes(a.pool.head_dim))
         return fail(SKV_ERR_SCRATCH, "pool_attention: scratch of %lld bytes", (long long)a.scratch_bytes);
     cudaStream_t st = as_stream(stream);
-    const cudaError_t e = cudaMemsetAsync(a.scratch, 0, kMaxCtas * 4, st);
-    if (e != cudaSuccess) return fail(SKV_ERR_CUDA, "pool_attention: %s", cudaGetErrorString(e));
     if (fits_mma(a.pool))
         return a.pool.precision == 1 ? attend_fp16(a, st) : a.pool.precision == 2 ? attend_int8(a, st) : attend_int4(a, st);
     if (a.q.dtype == kF32) return launch_any<float>(a, st);

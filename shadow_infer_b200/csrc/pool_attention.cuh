@@ -121,7 +121,8 @@ __device__ __forceinline__ Segment segment_at(const skv_pool_attention_args& a, 
 }
 
 // ------------------------------------------------------------------------------------- publishing
-// Scratch: kMaxCtas arrival counters (zeroed before the launch), then two slots a CTA of
+// Scratch: kMaxCtas arrival counters (zero between launches: the last to arrive resets its counter), then two
+// slots a CTA of
 // rows * (D + 2) floats (rounded up to 16 bytes): O [rows][D], max [rows], sum [rows].
 __device__ __forceinline__ float* slot_of(const skv_pool_attention_args& a, int cta, int slot, int rows) {
     return reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kMaxCtas * 4) +
@@ -136,7 +137,9 @@ __device__ __forceinline__ bool arrive(const skv_pool_attention_args& a, const S
     if (threadIdx.x == 0) {
         __threadfence();
         const int c0 = s.owner_of(g.first), c1 = s.owner_of(g.last);
-        s_last = atomicAdd(reinterpret_cast<int*>(a.scratch) + c0, 1) == c1 - c0;
+        int* count = reinterpret_cast<int*>(a.scratch) + c0;
+        s_last = atomicAdd(count, 1) == c1 - c0;
+        if (s_last) *count = 0;
         __threadfence();
     }
     __syncthreads();

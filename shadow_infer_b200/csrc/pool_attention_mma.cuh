@@ -31,7 +31,7 @@
 
 namespace skv {
 
-constexpr int kMmaWarps = 4, kMmaThreads = 32 * kMmaWarps, kMmaTile = 16 * kMmaWarps, kMmaParts = 128;
+constexpr int kMmaParts = 128;      // parts whose factors a joining CTA holds at a time
 constexpr float kRefDrop = 5.0f;    // a fresh maximum's weight is 2^5: small weights keep their bits in fp16
 constexpr float kRefRoom = 14.0f;   // weights may grow to 2^14 (times a mantissa < 2) before ref moves
 
@@ -308,77 +308,84 @@ __device__ __forceinline__ void query_place(int d, int& mma, int& c, int& reg, i
     }
 }
 
-template <int DP, int NT, int NQ>
+template <int DP, int NT, int NQ, int W>
 __host__ __device__ constexpr size_t mma_smem() {
-    static_assert(join_floats<8 * NT, kMmaThreads, kMmaParts>() <= kMmaWarps * 8 * NT * (DP + 4), "the join works in the warps' sums");
-    return (size_t)(DP / 16) * NT * NQ * 32 * 8 + (size_t)kMmaWarps * 8 * NT * (DP + 4) * 4 + (3 * kMmaWarps + 2) * 8 * NT * 4;
+    static_assert(join_floats<8 * NT, 32 * W, kMmaParts>() <= W * 8 * NT * (DP + 4), "the join works in the warps' sums");
+    return (size_t)(DP / 16) * NT * NQ * 32 * 8 + (size_t)W * 8 * NT * (DP + 4) * 4 + (3 * W + 2) * 8 * NT * 4;
 }
 
-template <int PREC, int DP, int NT, int NQ, int NP, int CTAS>
-__global__ void __launch_bounds__(kMmaThreads, CTAS)
+template <int PREC, int DP, int NT, int NQ, int NP, int W, int CTAS>
+__global__ void __launch_bounds__(32 * W, CTAS)
 pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int row_tiles, bool q_vec, bool out_vec) {
-    constexpr int M = DP / 16, ROWS = 8 * NT;
+    constexpr int M = DP / 16, ROWS = 8 * NT, THREADS = 32 * W, TILE = 16 * W;
     extern __shared__ __align__(16) char mma_sm[];
     __shared__ Share s;
     uint2* s_q = reinterpret_cast<uint2*>(mma_sm);                       // [M][NT][NQ][32]
     float* s_o = reinterpret_cast<float*>(s_q + M * NT * NQ * 32);       // [warps][ROWS][DP + 4]
-    float* s_ref = s_o + kMmaWarps * ROWS * (DP + 4);                    // [warps][ROWS]
-    float* s_sum = s_ref + kMmaWarps * ROWS;                             // [warps][ROWS]
-    float* s_w = s_sum + kMmaWarps * ROWS;                               // [warps][ROWS]
-    float* s_c = s_w + kMmaWarps * ROWS;                                 // [ROWS] factor of a row's scores; later its max
+    float* s_ref = s_o + W * ROWS * (DP + 4);                    // [warps][ROWS]
+    float* s_sum = s_ref + W * ROWS;                             // [warps][ROWS]
+    float* s_w = s_sum + W * ROWS;                               // [warps][ROWS]
+    float* s_c = s_w + W * ROWS;                                 // [ROWS] factor of a row's scores; later its max
     float* s_l = s_c + ROWS;                                             // [ROWS]
     const int D = a.pool.head_dim, P = a.pool.page_size;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, lg = lane >> 2, lc = lane & 3;
     const int rep = a.q.heads / a.pool.heads, R = rep * a.S_q;
     const bool p16 = P % 16 == 0;   // a tile lies in one page
-    take_share<kMmaThreads>(a, kMmaTile, a.pool.heads * row_tiles, 1, &s);
-    int b = s.b, base = s.base;
-    for (int at = s.lo; at < s.hi;) {
-        const Segment g = segment_at(a, s, at, kMmaTile, row_tiles, b, base);
+    take_share<THREADS>(a, TILE, a.pool.heads * row_tiles, 2, &s);
+    if (s.lo >= s.hi) return;
+    int b = s.b, base = s.base, at = s.lo;
+    PageRows pages;
+    // the pool row of token lane % 16 of a tile, -1 where there is none
+    auto row_of = [&](const Segment& g, int tile) {
+        const int t0 = tile * 16, t = t0 + (lane & 15), n = g.tokens;
+        int row = -1;
+        if (p16) {
+            const int j = t0 / P, page = pages.page(j);
+            if (t < n && page >= 0 && page < a.pool.num_pages) row = (page * a.pool.heads + g.hk) * P + (t - j * P);
+        } else if (t < n) {
+            const int64_t r = pool_row(a.pool, g.b, t);
+            if (r >= 0) row = (int)r + g.hk * P;
+        }
+        if (t < n && row < 0 && a.error_flag) atomicExch(a.error_flag, 1);
+        return row;
+    };
+    // the rows of the tokens whose K (g, g + 8) and V (2c, 2c + 1, 2c + 8, 2c + 9) this lane loads
+    auto k_rows = [&](int row, int (&own)[2]) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) own[i] = __shfl_sync(0xffffffffu, row, lg + 8 * i);
+    };
+    auto v_rows = [&](int row, int (&four)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) four[i] = __shfl_sync(0xffffffffu, row, 2 * lc + (i & 1) + 8 * (i >> 1));
+    };
+    KTile<PREC, DP> kt;
+    VTile<PREC, DP> vt;
+    int st = 0, end = 0, row = -1;   // this warp's tile, the end of its tiles, the rows of the tile's tokens
+    // The next segment, its first tile on the way.
+    auto open = [&]() {
+        const Segment g = segment_at(a, s, at, TILE, row_tiles, b, base);
         at += g.t1 - g.t0;
-        const int n = g.tokens, r0 = g.rt * ROWS;
-        const int end = min(g.t1 * kMmaWarps, (n + 15) / 16);
-        int st = g.t0 * kMmaWarps + warp;
-        PageRows pages;
+        end = min(g.t1 * W, (g.tokens + 15) / 16);
+        st = g.t0 * W + warp;
         if (p16) pages.start(a.pool, g.b, st * 16 / P);
-        // the pool row of token lane % 16 of a tile, -1 where there is none
-        auto row_of = [&](int tile) {
-            const int t0 = tile * 16, t = t0 + (lane & 15);
-            int row = -1;
-            if (p16) {
-                const int j = t0 / P, page = pages.page(j);
-                if (t < n && page >= 0 && page < a.pool.num_pages) row = (page * a.pool.heads + g.hk) * P + (t - j * P);
-            } else if (t < n) {
-                const int64_t r = pool_row(a.pool, g.b, t);
-                if (r >= 0) row = (int)r + g.hk * P;
-            }
-            if (t < n && row < 0 && a.error_flag) atomicExch(a.error_flag, 1);
-            return row;
-        };
-        // the rows of the tokens whose K (g, g + 8) and V (2c, 2c + 1, 2c + 8, 2c + 9) this lane loads
-        auto k_rows = [&](int row, int (&own)[2]) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) own[i] = __shfl_sync(0xffffffffu, row, lg + 8 * i);
-        };
-        auto v_rows = [&](int row, int (&four)[4]) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) four[i] = __shfl_sync(0xffffffffu, row, 2 * lc + (i & 1) + 8 * (i >> 1));
-        };
-        KTile<PREC, DP> kt;
-        VTile<PREC, DP> vt;
-        int row = -1, next = -1;   // of this tile's tokens, of the next one's
+        row = -1;
         if (st < end) {
             int own[2], four[4];
-            row = row_of(st);
+            row = row_of(g, st);
             k_rows(row, own);
             v_rows(row, four);
             kt.load(a.pool, own, lc);
             vt.load(a.pool, four, own, lg, lc);
         }
+        return g;
+    };
+    Segment g = open();
+    for (;;) {
+        const int n = g.tokens, r0 = g.rt * ROWS;
         // ---- queries: a power of two taken out of each row, laid out as B operands
         __syncthreads();
         {
-            constexpr int RW = ROWS / kMmaWarps, E = DP / 32;   // a warp's rows, a lane's values of each
+            constexpr int RW = ROWS / W, E = DP / 32;   // a warp's rows, a lane's values of each
             float x[RW][E];
 #pragma unroll
             for (int i = 0; i < RW; ++i) {   // every load before the first use
@@ -435,9 +442,9 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[t][m][i] = 0.0f;
 
-        for (; st < end; st += kMmaWarps) {
-            const bool more = st + kMmaWarps < end;
-            next = more ? row_of(st + kMmaWarps) : -1;
+        for (; st < end; st += W) {
+            const bool more = st + W < end;
+            const int next = more ? row_of(g, st + W) : -1;
             // ---- scores
             float x[NT][4];
 #pragma unroll
@@ -676,7 +683,9 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
             row = next;
         }
 
-        // ---- the warps' parts joined
+        // ---- the warps' parts joined, while the next segment's first tiles load
+        const bool another = at < s.hi;
+        Segment following;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -697,12 +706,13 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                     *reinterpret_cast<float2*>(row + d) = make_float2(o[t][m][i], o[t][m][i + 2]);
                 }
             }
+        if (another) following = open();
         __syncthreads();
         if (tid < ROWS) {
             float m = -INFINITY, l = 0.0f;
-            for (int w = 0; w < kMmaWarps; ++w) m = fmaxf(m, s_ref[w * ROWS + tid]);
+            for (int w = 0; w < W; ++w) m = fmaxf(m, s_ref[w * ROWS + tid]);
             const float r = m == -INFINITY ? 0.0f : m;
-            for (int w = 0; w < kMmaWarps; ++w) {
+            for (int w = 0; w < W; ++w) {
                 const float f = exp2f(s_ref[w * ROWS + tid] - r);
                 s_w[w * ROWS + tid] = f;
                 l += s_sum[w * ROWS + tid] * f;
@@ -713,12 +723,12 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
         __syncthreads();
         float* part = slot_of(a, blockIdx.x, g.slot, ROWS);
 #pragma unroll
-        for (int i = tid; i < ROWS * DP / 4; i += kMmaThreads) {
+        for (int i = tid; i < ROWS * DP / 4; i += THREADS) {
             const int j = i / (DP / 4), d = i % (DP / 4) * 4;
             if (r0 + j >= R || d >= D) continue;
             float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int w = 0; w < kMmaWarps; ++w) {
+            for (int w = 0; w < W; ++w) {
                 const float4 v = *reinterpret_cast<const float4*>(s_o + (w * ROWS + j) * (DP + 4) + d);
                 const float f = s_w[w * ROWS + j];
                 y[0] = fmaf(v.x, f, y[0]); y[1] = fmaf(v.y, f, y[1]); y[2] = fmaf(v.z, f, y[2]); y[3] = fmaf(v.w, f, y[3]);
@@ -732,28 +742,32 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
             for (int k = 0; k < 4; ++k) y[k] = l == 0.0f ? 0.0f : y[k] / l;
             store_row(a, g, r0 + j, d, out_vec, y);
         }
-        if (g.whole) continue;
-        if (tid < ROWS) {
-            part[ROWS * D + tid] = s_c[tid];
-            part[ROWS * D + ROWS + tid] = s_l[tid];
+        if (!g.whole) {
+            if (tid < ROWS) {
+                part[ROWS * D + tid] = s_c[tid];
+                part[ROWS * D + ROWS + tid] = s_l[tid];
+            }
+            if (arrive(a, s, g)) join<ROWS, THREADS, 4, kMmaParts>(a, s, g, R, s_o, out_vec);
         }
-        if (arrive(a, s, g)) join<ROWS, kMmaThreads, 4, kMmaParts>(a, s, g, R, s_o, out_vec);
+        if (!another) break;
+        g = following;
     }
 }
 
 // CTAs an SM: what their registers allow.
 template <int PREC, int DP, int NT, int NQ, int NP>
 int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
-    constexpr int CTAS = NT >= 4 ? 2 : NT == 2 ? 3 : PREC == 1 ? 3 : 4;
+    constexpr int W = NT == 1 && PREC >= 2 ? 8 : 4;
+    constexpr int CTAS = NT >= 4 ? 2 : NT == 2 ? 3 : PREC == 1 ? 3 : 2;
     static_assert(CTAS * 2 * 8 * NT <= kRowsPerSm, "the scratch holds every CTA's slots");
-    constexpr size_t smem = mma_smem<DP, NT, NQ>();
-    const auto kernel = pool_attention_mma_kernel<PREC, DP, NT, NQ, NP, CTAS>;
+    constexpr size_t smem = mma_smem<DP, NT, NQ, W>();
+    const auto kernel = pool_attention_mma_kernel<PREC, DP, NT, NQ, NP, W, CTAS>;
     if (smem > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (e != cudaSuccess) return fail(SKV_ERR_CUDA, "pool_attention: %s", cudaGetErrorString(e));
     }
     const int R = a.q.heads / a.pool.heads * a.S_q;
-    kernel<<<sm_count() * CTAS, kMmaThreads, smem, st>>>(a, (R + 8 * NT - 1) / (8 * NT), rows_aligned(a.q), rows_aligned(a.out));
+    kernel<<<sm_count() * CTAS, 32 * W, smem, st>>>(a, (R + 8 * NT - 1) / (8 * NT), rows_aligned(a.q), rows_aligned(a.out));
     return check_launch("pool_attention");
 }
 

@@ -39,7 +39,22 @@ _READ = struct.Struct("<" + _POOL + _ROWS * 2 + "QQQii")
 _ATTENTION = struct.Struct("<" + _POOL + _ROWS * 2 + "QQQqQiifi")
 assert (_APPEND.size, _READ.size, _ATTENTION.size) == (336, 192, 216)
 _NO_ROPE = (0,) * 11
-_SCRATCH_BYTES = {}
+_SCRATCH = {}   # (device, stream) -> attention scratch
+
+
+def _scratch(dev: torch.device, stream: int, D: int) -> torch.Tensor:
+    """The attention's scratch on a stream: partial results and arrival counters that every call leaves zero.  Calls
+    of one stream follow each other, so they share one; a graph being captured gets its own."""
+    t = _SCRATCH.get((dev.index, stream))
+    capturing = torch.cuda.is_current_stream_capturing()
+    if t is None or capturing:
+        lib = _lib.load()
+        # sized for any head the kernels take, so that it is made once
+        t = torch.empty(lib.skv_pool_attention_scratch_bytes(max(D, 512)), dtype=torch.uint8, device=dev)
+        t[:lib.skv_pool_attention_scratch_zeros()].zero_()
+        if not capturing:
+            _SCRATCH[dev.index, stream] = t
+    return t
 
 
 def _index(t: torch.Tensor, shape: Tuple[int, ...], dev: torch.device, name: str) -> torch.Tensor:
@@ -247,16 +262,14 @@ def paged_attention(
     out = torch.empty((B, Hq, S_q, D), dtype=qd.dtype, device=dev)
     lib = _lib.load()
     with device_ctx(dev):
-        need = _SCRATCH_BYTES.get((dev.index, D))
-        if need is None:
-            need = _SCRATCH_BYTES[dev.index, D] = max(256, lib.skv_pool_attention_scratch_bytes(D))
-        scratch = torch.empty(need, dtype=torch.uint8, device=dev)
+        stream = _lib.stream_of(dev)
+        scratch = _scratch(dev, stream, D)
         flag = _flag(check, dev)
         args = _ATTENTION.pack(*pool, *_rows_fields(qd), *_rows_fields(out), lens.data_ptr(),
-                               0 if new is None else new.data_ptr(), scratch.data_ptr(), need,
+                               0 if new is None else new.data_ptr(), scratch.data_ptr(), scratch.numel(),
                                0 if flag is None else flag.data_ptr(), S_q, bool(causal),
                                1.0 / math.sqrt(D) if scale is None else scale, 0)
-        st = lib.skv_pool_attention(args, _lib.stream_of(dev))
+        st = lib.skv_pool_attention(args, stream)
     _lib.check(st, "paged_attention")
     del table
     _raise_flag(flag, "paged_attention")
