@@ -50,20 +50,21 @@ __device__ __forceinline__ float fast_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ uint4 load_page16(const void* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
+// Page loads that keep the register's value where `on` is 0 (predicated: no branch in the loop).
+__device__ __forceinline__ void load_page(uint4& v, const void* p, int on) {
+    asm volatile("{ .reg .pred t; setp.ne.s32 t, %5, 0; @t ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4]; }"
+                 : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w) : "l"(p), "r"(on));
 }
-__device__ __forceinline__ uint2 load_page8(const void* p) {
-    uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
+__device__ __forceinline__ void load_page(uint2& v, const void* p, int on) {
+    asm volatile("{ .reg .pred t; setp.ne.s32 t, %3, 0; @t ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2]; }"
+                 : "+r"(v.x), "+r"(v.y) : "l"(p), "r"(on));
 }
-__device__ __forceinline__ uint32_t load_page4(const void* p) {
-    uint32_t v;
-    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
-    return v;
+__device__ __forceinline__ void load_page(uint32_t& v, const void* p, int on) {
+    asm volatile("{ .reg .pred t; setp.ne.s32 t, %2, 0; @t ld.global.nc.L1::no_allocate.u32 %0, [%1]; }"
+                 : "+r"(v) : "l"(p), "r"(on));
+}
+__device__ __forceinline__ void load_scale(float& v, const float* p, int on) {
+    asm volatile("{ .reg .pred t; setp.ne.s32 t, %2, 0; @t ld.global.nc.f32 %0, [%1]; }" : "+f"(v) : "l"(p), "r"(on));
 }
 __device__ __forceinline__ uint32_t h2_sub(uint32_t a, uint32_t b) {
     const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
@@ -101,6 +102,12 @@ __device__ __forceinline__ int clamp_exp(uint32_t bits) { return min(max((int)(b
 __device__ __forceinline__ float exp_down(int e) { return __uint_as_float((uint32_t)(264 - e) << 23); }
 __device__ __forceinline__ float exp_up(int e) { return __uint_as_float((uint32_t)(e - 10) << 23); }
 
+// t / page_size for t < 2^31 as a product: mul = ceil(2^shift / page_size), shift = 31 + ceil(log2 page_size).
+struct PageDivide {
+    uint32_t mul;
+    int shift;
+};
+
 // The page rows of a sequence's tokens for one key head.  A warp keeps the next 64 entries of the
 // block table in its lanes and asks them by shuffle: tiles need no dependent load.
 struct PageRows {
@@ -125,136 +132,210 @@ struct PageRows {
     }
 };
 
-// One warp's tile of 16 tokens, as loaded.
+// A lane's place in the pages: addresses of its chunk in row 0, and which of its chunks the head has.
+template <int PREC, int DP>
+struct LanePlace {
+    static constexpr int KC = PREC == 1 ? DP / 32 : DP / 64;   // chunks of a K row
+    static constexpr int VC = PREC == 1 ? DP / 64 : 1;         // of a V row
+    const char *k, *v;
+    const float *sk[PREC == 3 ? KC : 1], *sv, *sv_own[PREC == 3 ? KC : 1];
+    int row_bytes, groups;
+    int k_on[KC], v_on[VC];
+    __device__ __forceinline__ void set(const skv_pool& p, int g, int c) {
+        const int D = p.head_dim;
+        row_bytes = PREC == 1 ? 2 * D : PREC == 2 ? D : D / 2;
+        groups = PREC == 3 ? D / p.int4_group : 1;
+        const int kb = PREC == 3 ? 8 : 16, vb = PREC == 1 ? 16 : PREC == 2 ? DP / 8 : DP / 16;
+        k = static_cast<const char*>(p.k) + c * kb;
+        v = static_cast<const char*>(p.v) + g * vb;
+#pragma unroll
+        for (int j = 0; j < KC; ++j) k_on[j] = (c + 4 * j) * kb < row_bytes;
+#pragma unroll
+        for (int j = 0; j < VC; ++j) v_on[j] = (g + 8 * j) * vb < row_bytes;
+        sk[0] = p.scale_k;
+        sv = p.scale_v;
+        sv_own[0] = p.scale_v;
+        if constexpr (PREC == 3) {
+            sv += g * (DP / 8) / p.int4_group;
+#pragma unroll
+            for (int j = 0; j < KC; ++j) {
+                sk[j] = p.scale_k + (c + 4 * j) * 16 / p.int4_group;
+                sv_own[j] = p.scale_v + (c + 4 * j) * 16 / p.int4_group;
+            }
+        }
+    }
+};
+
+// One warp's tile of 16 tokens, as loaded.  Chunks that the head does not have stay zero from clear().
 template <int PREC, int DP>
 struct KTile;
 template <int PREC, int DP>
 struct VTile;
 
+template <int BYTES> struct PageChunk;
+template <> struct PageChunk<16> { using type = uint4; };
+template <> struct PageChunk<8> { using type = uint2; };
+template <> struct PageChunk<4> { using type = uint32_t; };
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ uint32_t word_of(const uint2& v, int i) { return i == 0 ? v.x : v.y; }
+__device__ __forceinline__ uint32_t word_of(uint32_t v, int) { return v; }
+
 template <int DP>
 struct KTile<1, DP> {
     uint4 x[2][DP / 32];
-    __device__ __forceinline__ void load(const skv_pool& p, const int (&row)[2], int c) {
+    __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int j = 0; j < DP / 32; ++j) {
-                const int chunk = c + 4 * j;
-                x[t][j] = make_uint4(0, 0, 0, 0);
-                if (row[t] >= 0 && chunk * 8 < p.head_dim)
-                    x[t][j] = load_page16(static_cast<const __half*>(p.k) + (int64_t)row[t] * p.head_dim + chunk * 8);
-            }
+            for (int j = 0; j < DP / 32; ++j) x[t][j] = make_uint4(0, 0, 0, 0);
     }
+    __device__ __forceinline__ void load(const LanePlace<1, DP>& at, const int (&row)[2]) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const char* q = at.k + (int64_t)row[t] * at.row_bytes;
+#pragma unroll
+            for (int j = 0; j < DP / 32; ++j)
+                load_page(x[t][j], q + 64 * j, at.k_on[j]);
+        }
+    }
+    __device__ __forceinline__ void only(const bool (&)[2]) {}   // scores of absent tokens are overwritten
 };
 template <int DP>
 struct KTile<2, DP> {
     uint4 x[2][DP / 64];
     float s[2];
-    __device__ __forceinline__ void load(const skv_pool& p, const int (&row)[2], int c) {
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int j = 0; j < DP / 64; ++j) x[t][j] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void load(const LanePlace<2, DP>& at, const int (&row)[2]) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
+            const char* q = at.k + (int64_t)row[t] * at.row_bytes;
 #pragma unroll
-            for (int j = 0; j < DP / 64; ++j) {
-                const int chunk = c + 4 * j;
-                x[t][j] = make_uint4(0, 0, 0, 0);
-                if (row[t] >= 0 && chunk * 16 < p.head_dim)
-                    x[t][j] = load_page16(static_cast<const int8_t*>(p.k) + (int64_t)row[t] * p.head_dim + chunk * 16);
-            }
-            s[t] = row[t] >= 0 ? __ldg(p.scale_k + row[t]) : 0.0f;
+            for (int j = 0; j < DP / 64; ++j)
+                load_page(x[t][j], q + 64 * j, at.k_on[j]);
+            s[t] = __ldg(at.sk[0] + row[t]);
         }
     }
+    __device__ __forceinline__ void only(const bool (&)[2]) {}
 };
 template <int DP>
 struct KTile<3, DP> {
     uint2 x[2][DP / 64];
     float s[2][DP / 64];
-    __device__ __forceinline__ void load(const skv_pool& p, const int (&row)[2], int c) {
-        const int ng = p.head_dim / p.int4_group;
+    __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int j = 0; j < DP / 64; ++j) {
-                const int chunk = c + 4 * j;
-                const bool on = row[t] >= 0 && chunk * 16 < p.head_dim;
-                x[t][j] = make_uint2(0x88888888u, 0x88888888u);
+                x[t][j] = make_uint2(0, 0);
                 s[t][j] = 0.0f;
-                if (on) {
-                    x[t][j] = load_page8(static_cast<const uint8_t*>(p.k) + (int64_t)row[t] * (p.head_dim / 2) + chunk * 8);
-                    s[t][j] = __ldg(p.scale_k + (int64_t)row[t] * ng + chunk * 16 / p.int4_group);
-                }
             }
+    }
+    __device__ __forceinline__ void load(const LanePlace<3, DP>& at, const int (&row)[2]) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const char* q = at.k + (int64_t)row[t] * at.row_bytes;
+#pragma unroll
+            for (int j = 0; j < DP / 64; ++j) {
+                load_page(x[t][j], q + 32 * j, at.k_on[j]);
+                load_scale(s[t][j], at.sk[j] + (int64_t)row[t] * at.groups, at.k_on[j]);
+            }
+        }
+    }
+    __device__ __forceinline__ void only(const bool (&own)[2]) {   // the tile's exponent is that of its tokens
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int j = 0; j < DP / 64; ++j) s[t][j] = own[t] ? s[t][j] : 0.0f;
     }
 };
 
 template <int DP>
 struct VTile<1, DP> {
     uint4 x[4][DP / 64];
-    __device__ __forceinline__ void load(const skv_pool& p, const int (&row)[4], const int (&)[2], int g, int) {
+    __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-            for (int j = 0; j < DP / 64; ++j) {
-                const int chunk = g + 8 * j;
-                x[t][j] = make_uint4(0, 0, 0, 0);
-                if (row[t] >= 0 && chunk * 8 < p.head_dim)
-                    x[t][j] = load_page16(static_cast<const __half*>(p.v) + (int64_t)row[t] * p.head_dim + chunk * 8);
-            }
+            for (int j = 0; j < DP / 64; ++j) x[t][j] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void load(const LanePlace<1, DP>& at, const int (&row)[4], const int (&)[2]) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const char* q = at.v + (int64_t)row[t] * at.row_bytes;
+#pragma unroll
+            for (int j = 0; j < DP / 64; ++j)
+                load_page(x[t][j], q + 128 * j, at.v_on[j]);
+        }
+    }
+    // a weight of zero does not hide a NaN or an infinity in a row that holds no token
+    __device__ __forceinline__ void only(const bool (&four)[4], const bool (&)[2]) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+            if (!four[t])
+#pragma unroll
+                for (int j = 0; j < DP / 64; ++j) x[t][j] = make_uint4(0, 0, 0, 0);
     }
 };
 template <int DP>
 struct VTile<2, DP> {
-    uint32_t x[4][DP / 32];
+    using Chunk = typename PageChunk<DP / 8>::type;
+    Chunk x[4];
     float s[2];   // of tokens g and g + 8
-    __device__ __forceinline__ void load(const skv_pool& p, const int (&row)[4], const int (&own)[2], int g, int) {
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < 4; ++t) x[t] = Chunk{};
+    }
+    __device__ __forceinline__ void load(const LanePlace<2, DP>& at, const int (&row)[4], const int (&own)[2]) {
 #pragma unroll
-            for (int w = 0; w < DP / 32; ++w) x[t][w] = 0;
-            if (row[t] >= 0 && g * (DP / 8) < p.head_dim) {
-                const int8_t* q = static_cast<const int8_t*>(p.v) + (int64_t)row[t] * p.head_dim + g * (DP / 8);
-                if constexpr (DP == 128) {
-                    const uint4 u = load_page16(q);
-                    x[t][0] = u.x; x[t][1] = u.y; x[t][2] = u.z; x[t][3] = u.w;
-                } else {
-                    const uint2 u = load_page8(q);
-                    x[t][0] = u.x; x[t][1] = u.y;
-                }
-            }
-        }
+        for (int t = 0; t < 4; ++t) load_page(x[t], at.v + (int64_t)row[t] * at.row_bytes, at.v_on[0]);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) s[t] = own[t] >= 0 ? __ldg(p.scale_v + own[t]) : 1.0f;
+        for (int t = 0; t < 2; ++t) s[t] = __ldg(at.sv + own[t]);
+    }
+    __device__ __forceinline__ void only(const bool (&)[4], const bool (&own)[2]) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) s[t] = own[t] ? s[t] : 1.0f;
     }
 };
 template <int DP>
 struct VTile<3, DP> {
-    uint32_t x[4][DP / 64];
+    using Chunk = typename PageChunk<DP / 16>::type;
+    Chunk x[4];
     float s[4];              // of this lane's values, tokens 2c, 2c + 1, 2c + 8, 2c + 9
     float own[2][DP / 64];   // this lane's quarter of the scales of tokens g and g + 8
-    __device__ __forceinline__ void load(const skv_pool& p, const int (&row)[4], const int (&mine)[2], int g, int c) {
-        const int ng = p.head_dim / p.int4_group;
+    __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-#pragma unroll
-            for (int w = 0; w < DP / 64; ++w) x[t][w] = 0x88888888u;
             s[t] = 0.0f;
-            if (row[t] >= 0 && g * (DP / 8) < p.head_dim) {
-                const uint8_t* q = static_cast<const uint8_t*>(p.v) + (int64_t)row[t] * (p.head_dim / 2) + g * (DP / 16);
-                if constexpr (DP == 128) {
-                    const uint2 u = load_page8(q);
-                    x[t][0] = u.x; x[t][1] = u.y;
-                } else {
-                    x[t][0] = load_page4(q);
-                }
-                s[t] = __ldg(p.scale_v + (int64_t)row[t] * ng + g * (DP / 8) / p.int4_group);
-            }
+            x[t] = Chunk{};
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int j = 0; j < DP / 64; ++j) {
-                const int chunk = c + 4 * j;
-                own[t][j] = mine[t] >= 0 && chunk * 16 < p.head_dim ? __ldg(p.scale_v + (int64_t)mine[t] * ng + chunk * 16 / p.int4_group) : 0.0f;
-            }
+            for (int j = 0; j < DP / 64; ++j) own[t][j] = 0.0f;
+    }
+    __device__ __forceinline__ void load(const LanePlace<3, DP>& at, const int (&row)[4], const int (&mine)[2]) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            load_page(x[t], at.v + (int64_t)row[t] * at.row_bytes, at.v_on[0]);
+            load_scale(s[t], at.sv + (int64_t)row[t] * at.groups, at.v_on[0]);
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int j = 0; j < DP / 64; ++j) load_scale(own[t][j], at.sv_own[j] + (int64_t)mine[t] * at.groups, at.k_on[j]);
+    }
+    __device__ __forceinline__ void only(const bool (&four)[4], const bool (&mine)[2]) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) s[t] = four[t] ? s[t] : 0.0f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int j = 0; j < DP / 64; ++j) own[t][j] = mine[t] ? own[t][j] : 0.0f;
     }
 };
 
@@ -316,7 +397,7 @@ __host__ __device__ constexpr size_t mma_smem() {
 
 template <int PREC, int DP, int NT, int NQ, int NP, int W, int CTAS>
 __global__ void __launch_bounds__(32 * W, CTAS)
-pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int row_tiles, bool q_vec, bool out_vec) {
+pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int row_tiles, PageDivide magic, bool q_vec, bool out_vec) {
     constexpr int M = DP / 16, ROWS = 8 * NT, THREADS = 32 * W, TILE = 16 * W;
     extern __shared__ __align__(16) char mma_sm[];
     __shared__ Share s;
@@ -331,35 +412,48 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, lg = lane >> 2, lc = lane & 3;
     const int rep = a.q.heads / a.pool.heads, R = rep * a.S_q;
     const bool p16 = P % 16 == 0;   // a tile lies in one page
+    auto page_of = [&](int t) { return (int)(((uint64_t)(uint32_t)t * magic.mul) >> magic.shift); };
     take_share<THREADS>(a, TILE, a.pool.heads * row_tiles, 2, &s);
     if (s.lo >= s.hi) return;
     int b = s.b, base = s.base, at = s.lo;
     PageRows pages;
-    // the pool row of token lane % 16 of a tile, -1 where there is none
+    // Where a tile's tokens are: the pool row of its first token where a tile lies in one page, else the row of
+    // token lane % 16; -1 where there is none (past the end, or no page).
     auto row_of = [&](const Segment& g, int tile) {
-        const int t0 = tile * 16, t = t0 + (lane & 15), n = g.tokens;
+        const int t0 = tile * 16;
         int row = -1;
+        bool lost = false;
         if (p16) {
-            const int j = t0 / P, page = pages.page(j);
-            if (t < n && page >= 0 && page < a.pool.num_pages) row = (page * a.pool.heads + g.hk) * P + (t - j * P);
-        } else if (t < n) {
-            const int64_t r = pool_row(a.pool, g.b, t);
-            if (r >= 0) row = (int)r + g.hk * P;
+            const int j = page_of(t0), page = pages.page(j);
+            if (page >= 0 && page < a.pool.num_pages) row = (page * a.pool.heads + g.hk) * P + (t0 - j * P);
+            else lost = true;
+        } else if (t0 + (lane & 15) < g.tokens) {
+            const int t = t0 + (lane & 15), j = page_of(t), page = __ldg(pages.table + j);   // t is below the table's width
+            if (page >= 0 && page < a.pool.num_pages) row = (page * a.pool.heads + g.hk) * P + (t - j * P);
+            else lost = true;
         }
-        if (t < n && row < 0 && a.error_flag) atomicExch(a.error_flag, 1);
+        if (lost && a.error_flag) atomicExch(a.error_flag, 1);
         return row;
     };
-    // the rows of the tokens whose K (g, g + 8) and V (2c, 2c + 1, 2c + 8, 2c + 9) this lane loads
+    // The rows of the tokens whose K (g, g + 8) and V (2c, 2c + 1, 2c + 8, 2c + 9) this lane loads.  What has no row
+    // reads row 0, and what it reads is not used.
     auto k_rows = [&](int row, int (&own)[2]) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) own[i] = __shfl_sync(0xffffffffu, row, lg + 8 * i);
+        for (int i = 0; i < 2; ++i) own[i] = max(p16 ? row : __shfl_sync(0xffffffffu, row, lg + 8 * i), 0) + (p16 ? lg + 8 * i : 0);
     };
     auto v_rows = [&](int row, int (&four)[4]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) four[i] = __shfl_sync(0xffffffffu, row, 2 * lc + (i & 1) + 8 * (i >> 1));
+        for (int i = 0; i < 4; ++i) {
+            const int k = 2 * lc + (i & 1) + 8 * (i >> 1);
+            four[i] = max(p16 ? row : __shfl_sync(0xffffffffu, row, k), 0) + (p16 ? k : 0);
+        }
     };
+    LanePlace<PREC, DP> place;
+    place.set(a.pool, lg, lc);
     KTile<PREC, DP> kt;
     VTile<PREC, DP> vt;
+    kt.clear();
+    vt.clear();
     int st = 0, end = 0, row = -1;   // this warp's tile, the end of its tiles, the rows of the tile's tokens
     // The next segment, its first tile on the way.
     auto open = [&]() {
@@ -367,15 +461,15 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
         at += g.t1 - g.t0;
         end = min(g.t1 * W, (g.tokens + 15) / 16);
         st = g.t0 * W + warp;
-        if (p16) pages.start(a.pool, g.b, st * 16 / P);
+        pages.start(a.pool, g.b, p16 ? page_of(st * 16) : 0);
         row = -1;
         if (st < end) {
             int own[2], four[4];
             row = row_of(g, st);
             k_rows(row, own);
             v_rows(row, four);
-            kt.load(a.pool, own, lc);
-            vt.load(a.pool, four, own, lg, lc);
+            kt.load(place, own);
+            vt.load(place, four, own);
         }
         return g;
     };
@@ -420,7 +514,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
             }
         }
         __syncthreads();
-        float cf[NT][2], ref[NT][2], sum[NT][2], o[NT][M][4];
+        float cf[NT][2], ref[NT][2], base_of[NT][2], sum[NT][2], o[NT][M][4];   // base_of: ref, or 0 before there is one
         int see[NT][2], see_all = n;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -429,6 +523,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                 const int j = 8 * t + 2 * lc + i;
                 cf[t][i] = s_c[j];
                 ref[t][i] = -INFINITY;
+                base_of[t][i] = 0.0f;
                 sum[t][i] = 0.0f;
                 see[t][i] = r0 + j < R ? seen_by(a, g.b, n, (r0 + j) % a.S_q) : n;
                 see_all = min(see_all, see[t][i]);
@@ -445,19 +540,40 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
         for (; st < end; st += W) {
             const bool more = st + W < end;
             const int next = more ? row_of(g, st + W) : -1;
+            // ---- tokens that are there
+            const int t0 = st * 16;
+            const bool all = t0 + 16 <= see_all && (p16 ? row >= 0 : __all_sync(0xffffffffu, row >= 0));
+            bool here[2] = {true, true};
+            if (!all) {
+                bool four[4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    here[i] = (p16 ? row : __shfl_sync(0xffffffffu, row, lg + 8 * i)) >= 0 && t0 + lg + 8 * i < n;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int k = 2 * lc + (i & 1) + 8 * (i >> 1);
+                    four[i] = (p16 ? row : __shfl_sync(0xffffffffu, row, k)) >= 0 && t0 + k < n;
+                }
+                kt.only(here);
+                vt.only(four, here);
+            }
             // ---- scores
-            float x[NT][4];
+            // CH chains of dependent MMAs at a time: one would be as long as their latencies added up
+            constexpr int CH = NT == 1 ? 4 : NT == 2 ? 2 : 1;
+            float x[NT][4], acc[CH][NT][4];
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int h = 0; h < CH; ++h)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[t][i] = 0.0f;
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[h][t][i] = 0.0f;
             float k_factor[2] = {1.0f, 1.0f};
             auto qk = [&](const uint32_t (&f)[4], int m, int terms) {
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int q = 0; q < NQ; ++q)
-                        if (q < terms) mma16816(x[t], f, s_q[((m * NT + t) * NQ + q) * 32 + lane]);
+                        if (q < terms) mma16816(acc[(m * NQ + q) % CH][t], f, s_q[((m * NT + t) * NQ + q) * 32 + lane]);
             };
             if constexpr (PREC == 1) {
 #pragma unroll
@@ -516,10 +632,18 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                     }
                 }
             }
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[t][i] = acc[0][t][i];
+#pragma unroll
+                    for (int h = 1; h < CH; ++h) x[t][i] += acc[h][t][i];
+                }
             int own[2];
             if (more) {
                 k_rows(next, own);
-                kt.load(a.pool, own, lc);
+                kt.load(place, own);
             }
             // ---- weights
             float v_add[2] = {0.0f, 0.0f}, v_mul[2] = {1.0f, 1.0f}, v_sum[2] = {1.0f, 1.0f};
@@ -545,13 +669,6 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                     v_sum[i] = exp_down(ve[i]);                                 // 2^-(ve - 137)
                 }
             }
-            const int t0 = st * 16;
-            const bool all = t0 + 16 <= see_all && __all_sync(0xffffffffu, row >= 0);
-            bool here[2] = {true, true};
-            if (!all) {
-                here[0] = __shfl_sync(0xffffffffu, row, lg) >= 0;
-                here[1] = __shfl_sync(0xffffffffu, row, lg + 8) >= 0;
-            }
             bool grow = false;
 #pragma unroll
             for (int t = 0; t < NT; ++t)
@@ -562,7 +679,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                     if (PREC >= 2) z += v_add[tok];
                     if (!all && (!here[tok] || t0 + lg + 8 * tok >= see[t][col])) z = -INFINITY;
                     x[t][i] = z;
-                    grow |= z > (ref[t][col] == -INFINITY ? -INFINITY : ref[t][col] + kRefRoom);
+                    grow |= z > ref[t][col] + kRefRoom;
                 }
             if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -576,6 +693,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                         const float now = fmaxf(ref[t][i], top - kRefDrop);
                         const float f = now == -INFINITY ? 1.0f : fast_exp2(ref[t][i] - now);
                         ref[t][i] = now;
+                        base_of[t][i] = now == -INFINITY ? 0.0f : now;
                         sum[t][i] *= f;
 #pragma unroll
                         for (int m = 0; m < M; ++m) {
@@ -591,7 +709,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int tok = i >> 1, col = i & 1;
-                    const float y = fast_exp2(x[t][i] - (ref[t][col] == -INFINITY ? 0.0f : ref[t][col]));
+                    const float y = fast_exp2(x[t][i] - base_of[t][col]);
                     sum[t][col] = PREC >= 2 ? fmaf(y, v_sum[tok], sum[t][col]) : sum[t][col] + y;
                     w[i] = PREC == 2 ? y * v_mul[tok] : y;
                 }
@@ -632,7 +750,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                     uint32_t y[2][2];   // [tokens low / high][values 0,1 / 2,3]
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const uint32_t u = vt.x[2 * h][w] ^ 0x80808080u, v = vt.x[2 * h + 1][w] ^ 0x80808080u;
+                        const uint32_t u = word_of(vt.x[2 * h], w) ^ 0x80808080u, v = word_of(vt.x[2 * h + 1], w) ^ 0x80808080u;
                         y[h][0] = __byte_perm(u, v, 0x5140);
                         y[h][1] = __byte_perm(u, v, 0x7362);
                     }
@@ -661,8 +779,8 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                 for (int w = 0; w < DP / 64; ++w)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        uint32_t u = __byte_perm(vt.x[0][w], vt.x[1][w], i ? 0x7632 : 0x5410);
-                        uint32_t v = __byte_perm(vt.x[2][w], vt.x[3][w], i ? 0x7632 : 0x5410);
+                        uint32_t u = __byte_perm(word_of(vt.x[0], w), word_of(vt.x[1], w), i ? 0x7632 : 0x5410);
+                        uint32_t v = __byte_perm(word_of(vt.x[2], w), word_of(vt.x[3], w), i ? 0x7632 : 0x5410);
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const uint32_t f[4] = {i4_high(u), i4_low(u), i4_high(v), i4_low(v)};
@@ -678,7 +796,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
             if (more) {
                 int four[4];
                 v_rows(next, four);
-                vt.load(a.pool, four, own, lg, lc);
+                vt.load(place, four, own);
             }
             row = next;
         }
@@ -767,7 +885,11 @@ int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
         if (e != cudaSuccess) return fail(SKV_ERR_CUDA, "pool_attention: %s", cudaGetErrorString(e));
     }
     const int R = a.q.heads / a.pool.heads * a.S_q;
-    kernel<<<sm_count() * CTAS, 32 * W, smem, st>>>(a, (R + 8 * NT - 1) / (8 * NT), rows_aligned(a.q), rows_aligned(a.out));
+    PageDivide magic;
+    magic.shift = 31;
+    while ((1ll << (magic.shift - 31)) < a.pool.page_size) ++magic.shift;
+    magic.mul = (uint32_t)(((1ull << magic.shift) + a.pool.page_size - 1) / a.pool.page_size);
+    kernel<<<sm_count() * CTAS, 32 * W, smem, st>>>(a, (R + 8 * NT - 1) / (8 * NT), magic, rows_aligned(a.q), rows_aligned(a.out));
     return check_launch("pool_attention");
 }
 
