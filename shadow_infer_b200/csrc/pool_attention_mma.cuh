@@ -1,37 +1,36 @@
-// Attention over the page pool on the tensor cores, pages read straight into MMA fragments.
+// Attention over the page pool on the tensor cores.
 //
-// A decoding step is bound by the pages' bytes, but at 4 bits a value the FMA pipe cannot keep up with
-// HBM, and neither can one operand row a value where several query rows share a key head.  So
-// both products run as mma.m16n8k16 (fp16 operands, fp32 sums), transposed so that the few query rows
-// are the narrow side:
+// A decoding step is bound by the pages' bytes, but at 4 or 8 bits a value the FMA pipe cannot keep up with
+// HBM, nor can it where several query rows share a key head.  So both products run as mma.m16n8k16 (fp16 operands, fp32
+// sums), transposed so that the few query rows are the narrow side:
 //     S^T [16 tokens x 8 rows] = K [16 x D] Q^T,     O^T [16 values x 8 rows] += V^T [16 x 16 tokens] P^T.
-// (tcgen05 wants 128 rows of A in shared memory and its sums back through TMEM; with 8..32 query
-// rows the pages would pass through shared memory only to be read once.)
+// (tcgen05 wants 128 rows of A and brings its sums back through TMEM; 8 to 32 query rows would leave it idle.)
 //
-// The contraction order of an MMA is free as long as both operands agree, so a lane's 16-byte load of
-// a page row IS its share of the A operand: lane (g, c) = (lane / 4, lane % 4) takes chunks c, c+4, ...
-// of the rows of tokens g and g+8 (K), and the g-th chunks of tokens 2c, 2c+1, 2c+8, 2c+9 (V), whose
-// token pairs are interleaved with byte permutes.  No shared memory, no transposes of pages; the
-// queries are laid out once per segment to match.  P^T's operand is S^T's result transposed by
-// movmatrix.
+// Feeding.  A warp owns every W-th tile of 16 tokens of its CTA's share and a ring of slots in shared memory; it
+// copies its next tiles' rows and scales with cp.async while it multiplies this one's, across segments, and waits for no
+// other warp.  Slots are swizzled in 16-byte chunks, so the fragments are read without bank conflicts: fp16 by ldmatrix
+// (transposed for V), int8 and int4 as words whose integers become fp16 in registers.  The contraction order of an MMA is
+// free as long as both operands agree: the queries are laid out, once a segment, in the order the words come in.  P^T's
+// operand is S^T's result transposed by movmatrix.
 //
-// Exactness.  Page values enter the MMAs exactly: fp16 as it is, int8 and int4 as small integers.  An
-// int8 row's scale multiplies its score (K) or its weight (V) in fp32.  An int4 group's scale is split into an
-// 8-bit part r1 (times a 4-bit integer exact in fp16) and an 11-bit remainder r2, two MMAs, after a
-// power of two is taken out (per tile for K, per token for V), so range is no concern.  Queries are
-// scaled by a power of two a row; 16-bit ones fit one fp16 operand, fp32 ones take two (22 bits).  Weights are
-// 2^(z - ref) <= 2^15 with z the score plus the exponent of V's scale; one operand for bf16 outputs, whose
-// own rounding is 8 times coarser, else two.
+// Exactness.  Page values enter the MMAs exactly: fp16 as it is, int8 and int4 as small integers.  For the scores they stay
+// biased, as fp16 subnormals (their bits are the operand), and the sums start at minus the bias times the query's sum;
+// the values' sums would cancel too much that way, so V's integers are made signed.  An int8 row's scale multiplies its
+// score (K) or its weight (V) in fp32.  An int4 group's scale multiplies the group's own MMA result (K), or is split into
+// parts of 7 bits, an MMA each, that times a 4-bit integer are exact in fp16 (V), after a power of two a token is taken out
+// into its weight.  Queries are scaled by a power of two a row; 16-bit ones fit one fp16 operand, fp32 ones take two
+// (22 bits).  Weights are 2^(z - ref) <= 2^15 with z the score plus the exponent of V's scale; one operand for bf16
+// outputs, whose own rounding is 8 times coarser, else two.
 //
-// ref follows the running maximum lazily (only when a weight would pass 2^15 are sums rescaled), so
-// most tiles need one vote and no shuffles; row sums stay in the lanes until the segment ends.
+// ref follows the running maximum lazily (sums are rescaled only when a weight would pass 2^15), so most tiles need one
+// vote and no shuffles; row sums stay in the lanes until the segment ends.
 #pragma once
 
 #include "pool_attention.cuh"
 
 namespace skv {
 
-constexpr int kMmaParts = 128;      // parts whose factors a joining CTA holds at a time
+constexpr int kMmaParts = 64;       // parts whose factors a joining CTA holds at a time
 constexpr float kRefDrop = 5.0f;    // a fresh maximum's weight is 2^5: small weights keep their bits in fp16
 constexpr float kRefRoom = 14.0f;   // weights may grow to 2^14 (times a mantissa < 2) before ref moves
 
@@ -39,6 +38,12 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
+}
+// The same with new sums: c = a b + (c0, c1 for every row of A).
+__device__ __forceinline__ void mma16816_from(float (&c)[4], const uint32_t (&a)[4], uint2 b, float c0, float c1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "f"(c0), "f"(c1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
@@ -50,28 +55,25 @@ __device__ __forceinline__ float fast_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Page loads that keep the register's value where `on` is 0 (predicated: no branch in the loop).
-__device__ __forceinline__ void load_page(uint4& v, const void* p, int on) {
-    asm volatile("{ .reg .pred t; setp.ne.s32 t, %5, 0; @t ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4]; }"
-                 : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w) : "l"(p), "r"(on));
+__device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
-__device__ __forceinline__ void load_page(uint2& v, const void* p, int on) {
-    asm volatile("{ .reg .pred t; setp.ne.s32 t, %3, 0; @t ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2]; }"
-                 : "+r"(v.x), "+r"(v.y) : "l"(p), "r"(on));
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
+__device__ __forceinline__ void load_matrix(uint32_t (&f)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3]) : "r"(at) : "memory");
 }
-__device__ __forceinline__ void load_page(uint32_t& v, const void* p, int on) {
-    asm volatile("{ .reg .pred t; setp.ne.s32 t, %2, 0; @t ld.global.nc.L1::no_allocate.u32 %0, [%1]; }"
-                 : "+r"(v) : "l"(p), "r"(on));
-}
-__device__ __forceinline__ void load_scale(float& v, const float* p, int on) {
-    asm volatile("{ .reg .pred t; setp.ne.s32 t, %2, 0; @t ld.global.nc.f32 %0, [%1]; }" : "+f"(v) : "l"(p), "r"(on));
+__device__ __forceinline__ void load_matrix_trans(uint32_t (&f)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(f[0]), "=r"(f[1]), "=r"(f[2]), "=r"(f[3]) : "r"(at) : "memory");
 }
 __device__ __forceinline__ uint32_t h2_sub(uint32_t a, uint32_t b) {
     const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
-    const __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
@@ -82,25 +84,24 @@ __device__ __forceinline__ uint32_t h2_pack(float a, float b) {
     const __half2 r = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&r);
 }
-// Small integers as fp16: 1024 + n has n in its low bits.
-__device__ __forceinline__ uint32_t i8_pair(uint32_t biased, uint32_t sel) {        // bytes n + 128
-    return h2_sub(__byte_perm(biased, 0x64646464u, sel), 0x64806480u);              // - 1152
+// Bytes n + 128 as fp16: 1024 + b has b in its low bits; less 1152 it is n.
+__device__ __forceinline__ uint32_t i8_pair(uint32_t biased, uint32_t sel) {
+    return h2_sub(__byte_perm(biased, 0x64646464u, sel), 0x64806480u);
 }
-__device__ __forceinline__ uint32_t i4_low(uint32_t w) {                            // nibbles n + 8 in bits 0-3
-    return h2_sub((w & 0x000F000Fu) | 0x64006400u, 0x64086408u);                    // - 1032
+// Nibbles n + 8 in bits 4-7 of each half as 64 + (n + 8).
+__device__ __forceinline__ uint32_t i4_pair(uint32_t w) { return (w & 0x00F000F0u) | 0x54005400u; }
+// The first 7 significant bits of x, rounded; x becomes what is left.
+__device__ __forceinline__ float take7(float& x) {
+    const float r = __uint_as_float((__float_as_uint(x) + 0x10000u) & 0xFFFE0000u);
+    x -= r;
+    return r;
 }
-__device__ __forceinline__ uint32_t i4_high(uint32_t w) {                           // in bits 4-7: 1024 + 16 (n + 8)
-    return h2_fma((w & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);       // / 16 - 72
-}
-// x as an 8-bit value and an 11-bit remainder, each twice in a register.
-__device__ __forceinline__ void split_scale(float x, float& r1, float& r2) {
-    r1 = __uint_as_float((__float_as_uint(x) + 0x8000u) & 0xFFFF0000u);
-    r2 = x - r1;
-}
-// 2^(127 + 10 - e) scales a float of exponent field e to [2^10, 2^11).
-__device__ __forceinline__ int clamp_exp(uint32_t bits) { return min(max((int)(bits >> 23), 11), 253); }
-__device__ __forceinline__ float exp_down(int e) { return __uint_as_float((uint32_t)(264 - e) << 23); }
-__device__ __forceinline__ float exp_up(int e) { return __uint_as_float((uint32_t)(e - 10) << 23); }
+// The exponent field of a float, kept where the powers of two below stay normal.
+__device__ __forceinline__ int clamp_exp(uint32_t bits) { return min(max((int)(bits >> 23), 35), 219); }
+// 2^(127 + to - e) scales a float of exponent field e to [2^to, 2^(to + 1)).
+__device__ __forceinline__ float exp_down(int e, int to) { return __uint_as_float((uint32_t)(254 + to - e) << 23); }
+__device__ __forceinline__ float exp_up(int e, int to) { return __uint_as_float((uint32_t)(e - to) << 23); }
+constexpr int kQueryExp = 10, kValueExp = 8;   // where a query row's and a token's int4 scales' maxima are put
 
 // t / page_size for t < 2^31 as a product: mul = ceil(2^shift / page_size), shift = 31 + ceil(log2 page_size).
 struct PageDivide {
@@ -129,213 +130,6 @@ struct PageRows {
             next = entry(base + 32 + lane);
         }
         return __shfl_sync(0xffffffffu, cur, j - base);
-    }
-};
-
-// A lane's place in the pages: addresses of its chunk in row 0, and which of its chunks the head has.
-template <int PREC, int DP>
-struct LanePlace {
-    static constexpr int KC = PREC == 1 ? DP / 32 : DP / 64;   // chunks of a K row
-    static constexpr int VC = PREC == 1 ? DP / 64 : 1;         // of a V row
-    const char *k, *v;
-    const float *sk[PREC == 3 ? KC : 1], *sv, *sv_own[PREC == 3 ? KC : 1];
-    int row_bytes, groups;
-    int k_on[KC], v_on[VC];
-    __device__ __forceinline__ void set(const skv_pool& p, int g, int c) {
-        const int D = p.head_dim;
-        row_bytes = PREC == 1 ? 2 * D : PREC == 2 ? D : D / 2;
-        groups = PREC == 3 ? D / p.int4_group : 1;
-        const int kb = PREC == 3 ? 8 : 16, vb = PREC == 1 ? 16 : PREC == 2 ? DP / 8 : DP / 16;
-        k = static_cast<const char*>(p.k) + c * kb;
-        v = static_cast<const char*>(p.v) + g * vb;
-#pragma unroll
-        for (int j = 0; j < KC; ++j) k_on[j] = (c + 4 * j) * kb < row_bytes;
-#pragma unroll
-        for (int j = 0; j < VC; ++j) v_on[j] = (g + 8 * j) * vb < row_bytes;
-        sk[0] = p.scale_k;
-        sv = p.scale_v;
-        sv_own[0] = p.scale_v;
-        if constexpr (PREC == 3) {
-            sv += g * (DP / 8) / p.int4_group;
-#pragma unroll
-            for (int j = 0; j < KC; ++j) {
-                sk[j] = p.scale_k + (c + 4 * j) * 16 / p.int4_group;
-                sv_own[j] = p.scale_v + (c + 4 * j) * 16 / p.int4_group;
-            }
-        }
-    }
-};
-
-// One warp's tile of 16 tokens, as loaded.  Chunks that the head does not have stay zero from clear().
-template <int PREC, int DP>
-struct KTile;
-template <int PREC, int DP>
-struct VTile;
-
-template <int BYTES> struct PageChunk;
-template <> struct PageChunk<16> { using type = uint4; };
-template <> struct PageChunk<8> { using type = uint2; };
-template <> struct PageChunk<4> { using type = uint32_t; };
-__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
-__device__ __forceinline__ uint32_t word_of(const uint2& v, int i) { return i == 0 ? v.x : v.y; }
-__device__ __forceinline__ uint32_t word_of(uint32_t v, int) { return v; }
-
-template <int DP>
-struct KTile<1, DP> {
-    uint4 x[2][DP / 32];
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int j = 0; j < DP / 32; ++j) x[t][j] = make_uint4(0, 0, 0, 0);
-    }
-    __device__ __forceinline__ void load(const LanePlace<1, DP>& at, const int (&row)[2]) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const char* q = at.k + (int64_t)row[t] * at.row_bytes;
-#pragma unroll
-            for (int j = 0; j < DP / 32; ++j)
-                load_page(x[t][j], q + 64 * j, at.k_on[j]);
-        }
-    }
-    __device__ __forceinline__ void only(const bool (&)[2]) {}   // scores of absent tokens are overwritten
-};
-template <int DP>
-struct KTile<2, DP> {
-    uint4 x[2][DP / 64];
-    float s[2];
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int j = 0; j < DP / 64; ++j) x[t][j] = make_uint4(0, 0, 0, 0);
-    }
-    __device__ __forceinline__ void load(const LanePlace<2, DP>& at, const int (&row)[2]) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const char* q = at.k + (int64_t)row[t] * at.row_bytes;
-#pragma unroll
-            for (int j = 0; j < DP / 64; ++j)
-                load_page(x[t][j], q + 64 * j, at.k_on[j]);
-            s[t] = __ldg(at.sk[0] + row[t]);
-        }
-    }
-    __device__ __forceinline__ void only(const bool (&)[2]) {}
-};
-template <int DP>
-struct KTile<3, DP> {
-    uint2 x[2][DP / 64];
-    float s[2][DP / 64];
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int j = 0; j < DP / 64; ++j) {
-                x[t][j] = make_uint2(0, 0);
-                s[t][j] = 0.0f;
-            }
-    }
-    __device__ __forceinline__ void load(const LanePlace<3, DP>& at, const int (&row)[2]) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const char* q = at.k + (int64_t)row[t] * at.row_bytes;
-#pragma unroll
-            for (int j = 0; j < DP / 64; ++j) {
-                load_page(x[t][j], q + 32 * j, at.k_on[j]);
-                load_scale(s[t][j], at.sk[j] + (int64_t)row[t] * at.groups, at.k_on[j]);
-            }
-        }
-    }
-    __device__ __forceinline__ void only(const bool (&own)[2]) {   // the tile's exponent is that of its tokens
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int j = 0; j < DP / 64; ++j) s[t][j] = own[t] ? s[t][j] : 0.0f;
-    }
-};
-
-template <int DP>
-struct VTile<1, DP> {
-    uint4 x[4][DP / 64];
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int j = 0; j < DP / 64; ++j) x[t][j] = make_uint4(0, 0, 0, 0);
-    }
-    __device__ __forceinline__ void load(const LanePlace<1, DP>& at, const int (&row)[4], const int (&)[2]) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const char* q = at.v + (int64_t)row[t] * at.row_bytes;
-#pragma unroll
-            for (int j = 0; j < DP / 64; ++j)
-                load_page(x[t][j], q + 128 * j, at.v_on[j]);
-        }
-    }
-    // a weight of zero does not hide a NaN or an infinity in a row that holds no token
-    __device__ __forceinline__ void only(const bool (&four)[4], const bool (&)[2]) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-            if (!four[t])
-#pragma unroll
-                for (int j = 0; j < DP / 64; ++j) x[t][j] = make_uint4(0, 0, 0, 0);
-    }
-};
-template <int DP>
-struct VTile<2, DP> {
-    using Chunk = typename PageChunk<DP / 8>::type;
-    Chunk x[4];
-    float s[2];   // of tokens g and g + 8
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int t = 0; t < 4; ++t) x[t] = Chunk{};
-    }
-    __device__ __forceinline__ void load(const LanePlace<2, DP>& at, const int (&row)[4], const int (&own)[2]) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t) load_page(x[t], at.v + (int64_t)row[t] * at.row_bytes, at.v_on[0]);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) s[t] = __ldg(at.sv + own[t]);
-    }
-    __device__ __forceinline__ void only(const bool (&)[4], const bool (&own)[2]) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) s[t] = own[t] ? s[t] : 1.0f;
-    }
-};
-template <int DP>
-struct VTile<3, DP> {
-    using Chunk = typename PageChunk<DP / 16>::type;
-    Chunk x[4];
-    float s[4];              // of this lane's values, tokens 2c, 2c + 1, 2c + 8, 2c + 9
-    float own[2][DP / 64];   // this lane's quarter of the scales of tokens g and g + 8
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            s[t] = 0.0f;
-            x[t] = Chunk{};
-        }
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int j = 0; j < DP / 64; ++j) own[t][j] = 0.0f;
-    }
-    __device__ __forceinline__ void load(const LanePlace<3, DP>& at, const int (&row)[4], const int (&mine)[2]) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            load_page(x[t], at.v + (int64_t)row[t] * at.row_bytes, at.v_on[0]);
-            load_scale(s[t], at.sv + (int64_t)row[t] * at.groups, at.v_on[0]);
-        }
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int j = 0; j < DP / 64; ++j) load_scale(own[t][j], at.sv_own[j] + (int64_t)mine[t] * at.groups, at.k_on[j]);
-    }
-    __device__ __forceinline__ void only(const bool (&four)[4], const bool (&mine)[2]) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t) s[t] = four[t] ? s[t] : 0.0f;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int j = 0; j < DP / 64; ++j) own[t][j] = mine[t] ? own[t][j] : 0.0f;
     }
 };
 
@@ -374,40 +168,82 @@ __device__ __forceinline__ void load_row(const T* p, int left, bool vec, float (
     }
 }
 
-// Where value d of a query row sits in the B operands: MMA, lane column c, register and half.
-template <int PREC>
-__device__ __forceinline__ void query_place(int d, int& mma, int& c, int& reg, int& half) {
-    if (PREC == 1) {
-        const int chunk = d / 8, h = d % 8;
-        mma = 2 * (chunk / 4) + h / 4; c = chunk % 4; reg = (h % 4) / 2; half = h % 2;
-    } else if (PREC == 2) {
-        const int chunk = d / 16, h = d % 16;
-        mma = 4 * (chunk / 4) + h / 4; c = chunk % 4; reg = (h % 4) / 2; half = h % 2;
-    } else {
-        const int chunk = d / 16, h = d % 8;
-        mma = 2 * (2 * (chunk / 4) + (d % 16) / 8) + (h % 4) / 2; c = chunk % 4; reg = h % 2; half = h / 4;
+// Where value d of a query row sits in the B operands (MMA, lane column c, register and half), and what it is
+// multiplied by there: the high nibbles of int4 bytes are read as 16 (n + 8).
+template <int PREC, int DP>
+__device__ __forceinline__ float query_place(int d, int& mma, int& c, int& reg, int& half) {
+    if (PREC == 1) {   // ldmatrix order
+        mma = d / 16; c = (d % 8) / 2; reg = (d % 16) / 8; half = d % 2;
+        return 1.0f;
     }
+    const int r = d % 4;   // of a word's or a byte pair's values: 0 and 2 in one register, 1 and 3 in the other
+    reg = r % 2; half = r / 2;
+    if (PREC == 2) {       // lane column c reads chunks 2c, 2c + 1 (the row's only four: chunk c)
+        const int chunk = d / 16, per = DP / 64;
+        mma = 4 * (chunk % per) + (d % 16) / 4; c = chunk / per;
+        return 1.0f;
+    }
+    mma = d / 16; c = (d % 16) / 4;
+    return r % 2 ? 1.0f : 0.0625f;
 }
+constexpr float kSubnormal = 5.9604644775390625e-08f;   // 2^-24: an fp16 whose bits are m has the value m 2^-24
+template <int PREC, int DP>
+__host__ __device__ constexpr int bias_blocks() { return PREC == 3 ? DP / 16 : 1; }
 
-template <int DP, int NT, int NQ, int W>
+// A slot: 16 rows of K and of V, their scales (int4: one for each 16 values), and the tokens' pool rows.
+template <int PREC, int DP>
+struct Slot {
+    static constexpr int ROW = PREC == 1 ? 2 * DP : PREC == 2 ? DP : DP / 2, CHUNKS = ROW / 16, BLOCKS = DP / 16;
+    static constexpr int SCALES = PREC == 1 ? 0 : PREC == 2 ? 1 : BLOCKS;   // a token
+    static constexpr int K = 0, V = 16 * ROW, SK = 2 * V, SV = SK + 64 * SCALES, ID = SV + 64 * SCALES, USED = ID + 64;
+    static constexpr int MERGE = 8 * (DP + 4) * 4;   // the warp's sums of 8 rows pass through a free slot
+    static constexpr int BYTES = (USED > MERGE ? USED : MERGE) + 15 & ~15;
+    // Byte of chunk ch of a row: chunks are exchanged within lines of 128 bytes so that the same chunk of 8 rows, and
+    // neighbouring chunks of the rows a fragment takes, fall into different banks.
+    __device__ static __forceinline__ int at(int row, int ch) {
+        if (CHUNKS >= 8) return row * ROW + ((ch & ~7) | ((ch ^ row) & 7)) * 16;
+        constexpr int PER = 8 / (CHUNKS < 8 ? CHUNKS : 8);   // rows in a line
+        const int line = row / PER;
+        return line * 128 + ((row % PER) * CHUNKS + (ch ^ (line % CHUNKS))) * 16;
+    }
+};
+
+template <int PREC, int DP, int NT>
+struct MmaShape {
+    // Warps a CTA, CTAs an SM, slots a warp: what 64 K registers and 227 KB of shared memory hold, with at least 60 KB of
+    // rows on their way (HBM's latency times its rate is about 43 KB an SM).
+    static constexpr int W = NT == 1 && PREC >= 2 ? 8 : 4;
+    static constexpr int CTAS = NT == 4 ? 2 : NT == 2 ? (PREC == 1 ? 2 : 3) : PREC == 1 ? 3 : 2;
+    static constexpr int SLOTS = PREC == 1 ? 2 : 3;
+};
+
+template <int PREC, int DP, int NT, int NQ>
 __host__ __device__ constexpr size_t mma_smem() {
-    static_assert(join_floats<8 * NT, 32 * W, kMmaParts>() <= W * 8 * NT * (DP + 4), "the join works in the warps' sums");
-    return (size_t)(DP / 16) * NT * NQ * 32 * 8 + (size_t)W * 8 * NT * (DP + 4) * 4 + (3 * W + 2) * 8 * NT * 4;
+    constexpr int W = MmaShape<PREC, DP, NT>::W, ROWS = 8 * NT;
+    return (size_t)W * MmaShape<PREC, DP, NT>::SLOTS * Slot<PREC, DP>::BYTES + (size_t)(DP / 16) * NT * NQ * 32 * 8 +
+           (join_floats<ROWS, 32 * W, kMmaParts>() + (3 * W + 2 + bias_blocks<PREC, DP>()) * ROWS) * 4;
 }
 
-template <int PREC, int DP, int NT, int NQ, int NP, int W, int CTAS>
-__global__ void __launch_bounds__(32 * W, CTAS)
-pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int row_tiles, PageDivide magic, bool q_vec, bool out_vec) {
-    constexpr int M = DP / 16, ROWS = 8 * NT, THREADS = 32 * W, TILE = 16 * W;
-    extern __shared__ __align__(16) char mma_sm[];
+// exact: the head has DP values (and, for int4, groups of 16): rows and scales are copied whole, in steps known here.
+template <int PREC, int DP, int NT, int NQ, int NP>
+__global__ void __launch_bounds__(32 * MmaShape<PREC, DP, NT>::W, MmaShape<PREC, DP, NT>::CTAS)
+pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int row_tiles, PageDivide magic, bool exact, bool q_vec,
+                          bool out_vec) {
+    using L = Slot<PREC, DP>;
+    constexpr int M = DP / 16, ROWS = 8 * NT, W = MmaShape<PREC, DP, NT>::W, S = MmaShape<PREC, DP, NT>::SLOTS;
+    constexpr int THREADS = 32 * W, TILE = 16 * W;
+    extern __shared__ __align__(128) char mma_sm[];
     __shared__ Share s;
-    uint2* s_q = reinterpret_cast<uint2*>(mma_sm);                       // [M][NT][NQ][32]
-    float* s_o = reinterpret_cast<float*>(s_q + M * NT * NQ * 32);       // [warps][ROWS][DP + 4]
-    float* s_ref = s_o + W * ROWS * (DP + 4);                    // [warps][ROWS]
-    float* s_sum = s_ref + W * ROWS;                             // [warps][ROWS]
-    float* s_w = s_sum + W * ROWS;                               // [warps][ROWS]
-    float* s_c = s_w + W * ROWS;                                 // [ROWS] factor of a row's scores; later its max
-    float* s_l = s_c + ROWS;                                             // [ROWS]
+    __shared__ int s_free[W];
+    char* s_ring = mma_sm;                                                       // [W][S] slots
+    uint2* s_q = reinterpret_cast<uint2*>(s_ring + W * S * L::BYTES);            // [M][NT][NQ][32]
+    float* s_join = reinterpret_cast<float*>(s_q + M * NT * NQ * 32);
+    float* s_ref = s_join + join_floats<ROWS, THREADS, kMmaParts>();             // [W][ROWS]
+    float* s_sum = s_ref + W * ROWS;                                             // [W][ROWS]
+    float* s_w = s_sum + W * ROWS;                                               // [W][ROWS]
+    float* s_c = s_w + W * ROWS;                                                 // [ROWS] factor of a row's scores; later its max
+    float* s_l = s_c + ROWS;                                                     // [ROWS]
+    float* s_bias = s_l + ROWS;                                                  // [blocks][ROWS] where the score sums start
     const int D = a.pool.head_dim, P = a.pool.page_size;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, lg = lane >> 2, lc = lane & 3;
     const int rep = a.q.heads / a.pool.heads, R = rep * a.S_q;
@@ -415,66 +251,119 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
     auto page_of = [&](int t) { return (int)(((uint64_t)(uint32_t)t * magic.mul) >> magic.shift); };
     take_share<THREADS>(a, TILE, a.pool.heads * row_tiles, 2, &s);
     if (s.lo >= s.hi) return;
-    int b = s.b, base = s.base, at = s.lo;
+    char* ring = s_ring + warp * S * L::BYTES;
+    if (!exact) {   // chunks that the head does not have are never copied: they count as zero
+        for (int i = lane; i < S * L::BYTES / 16; i += 32) reinterpret_cast<uint4*>(ring)[i] = make_uint4(0, 0, 0, 0);
+        __syncwarp();
+    }
+
+    // ---- copying ahead: this warp's tiles in order, over all segments of the share
+    struct {
+        int at, b, base;             // the next segment to open
+        int hk, tokens, st, end;     // the open one: tiles [st, end), every W-th is this warp's
+    } f;
+    f.at = s.lo;
+    f.b = s.b;
+    f.base = s.base;
+    f.st = f.end = f.hk = f.tokens = 0;
     PageRows pages;
-    // Where a tile's tokens are: the pool row of its first token where a tile lies in one page, else the row of
-    // token lane % 16; -1 where there is none (past the end, or no page).
-    auto row_of = [&](const Segment& g, int tile) {
-        const int t0 = tile * 16;
-        int row = -1;
-        bool lost = false;
+    const int row_bytes = PREC == 1 ? 2 * D : PREC == 2 ? D : D / 2;
+    constexpr int STEP = 32 / L::CHUNKS, COPIES = 16 / STEP;   // rows a warp's copy takes, copies a tile takes
+    const int my_row = lane / L::CHUNKS, my_chunk = lane % L::CHUNKS;
+    const char* k_lane = static_cast<const char*>(a.pool.k) + my_chunk * 16;
+    const char* v_lane = static_cast<const char*>(a.pool.v) + my_chunk * 16;
+    auto copy_next = [&](char* slot) {
+        while (f.st >= f.end) {
+            if (f.at >= s.hi) {
+                copy_commit();   // an empty group keeps the count
+                return;
+            }
+            const Segment g = segment_at(a, s, f.at, TILE, row_tiles, f.b, f.base);
+            f.at += g.t1 - g.t0;
+            f.hk = g.hk;
+            f.tokens = g.tokens;
+            f.end = min(g.t1 * W, (g.tokens + 15) / 16);
+            f.st = g.t0 * W + warp;
+            pages.start(a.pool, g.b, p16 ? page_of(f.st * 16) : 0);
+        }
+        // the pool row of token lane % 16 of the tile, -1 where there is none; absent rows copy row 0, unused
+        const int t0 = f.st * 16, t = t0 + (lane & 15);
+        int row = -1, first = 0;
         if (p16) {
             const int j = page_of(t0), page = pages.page(j);
-            if (page >= 0 && page < a.pool.num_pages) row = (page * a.pool.heads + g.hk) * P + (t0 - j * P);
-            else lost = true;
-        } else if (t0 + (lane & 15) < g.tokens) {
-            const int t = t0 + (lane & 15), j = page_of(t), page = __ldg(pages.table + j);   // t is below the table's width
-            if (page >= 0 && page < a.pool.num_pages) row = (page * a.pool.heads + g.hk) * P + (t - j * P);
-            else lost = true;
+            if (page >= 0 && page < a.pool.num_pages) {
+                first = (page * a.pool.heads + f.hk) * P + (t0 - j * P);
+                row = t < f.tokens ? first + (lane & 15) : -1;
+            } else if (a.error_flag) {
+                atomicExch(a.error_flag, 1);
+            }
+        } else if (t < f.tokens) {
+            const int j = page_of(t), page = __ldg(pages.table + j);   // t is below the table's width
+            if (page >= 0 && page < a.pool.num_pages) row = (page * a.pool.heads + f.hk) * P + (t - j * P);
+            else if (a.error_flag) atomicExch(a.error_flag, 1);
         }
-        if (lost && a.error_flag) atomicExch(a.error_flag, 1);
-        return row;
-    };
-    // The rows of the tokens whose K (g, g + 8) and V (2c, 2c + 1, 2c + 8, 2c + 9) this lane loads.  What has no row
-    // reads row 0, and what it reads is not used.
-    auto k_rows = [&](int row, int (&own)[2]) {
+        const uint32_t to = shared_address(slot);
+        if (lane < 16) *reinterpret_cast<int*>(slot + L::ID + 4 * lane) = row;
+        if (p16 && exact) {
+            const char* k = k_lane + (int64_t)(first + my_row) * L::ROW;
+            const char* v = v_lane + (int64_t)(first + my_row) * L::ROW;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) own[i] = max(p16 ? row : __shfl_sync(0xffffffffu, row, lg + 8 * i), 0) + (p16 ? lg + 8 * i : 0);
-    };
-    auto v_rows = [&](int row, int (&four)[4]) {
+            for (int i = 0; i < COPIES; ++i) {
+                const uint32_t y = to + L::K + L::at(my_row + i * STEP, my_chunk);
+                copy_async<16>(y, k + i * STEP * L::ROW);
+                copy_async<16>(y + L::V, v + i * STEP * L::ROW);
+            }
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int k = 2 * lc + (i & 1) + 8 * (i >> 1);
-            four[i] = max(p16 ? row : __shfl_sync(0xffffffffu, row, k), 0) + (p16 ? k : 0);
+            for (int i = 0; i < COPIES; ++i) {
+                const int r = p16 ? first + my_row + i * STEP : max(__shfl_sync(0xffffffffu, row, my_row + i * STEP), 0);
+                const uint32_t y = to + L::K + L::at(my_row + i * STEP, my_chunk);
+                if (my_chunk * 16 < row_bytes) {
+                    copy_async<16>(y, k_lane + (int64_t)r * row_bytes);
+                    copy_async<16>(y + L::V, v_lane + (int64_t)r * row_bytes);
+                }
+            }
         }
+        if constexpr (PREC == 2) {
+            copy_async<4>(to + (lane < 16 ? L::SK : L::SV) + 4 * (lane & 15),
+                          (lane < 16 ? a.pool.scale_k : a.pool.scale_v) + (p16 ? first + (lane & 15) : max(row, 0)));
+        } else if constexpr (PREC == 3) {
+            constexpr int PARTS = L::BLOCKS / 4;   // 16-byte pieces of a token's scales
+            if (exact) {
+                const int tok = DP == 128 ? lane / 2 : lane % 16;
+                const int r = p16 ? first + tok : max(__shfl_sync(0xffffffffu, row, tok), 0);
+                if constexpr (PARTS == 2) {
+                    copy_async<16>(to + L::SK + lane * 16, a.pool.scale_k + (int64_t)r * L::BLOCKS + (lane & 1) * 4);
+                    copy_async<16>(to + L::SV + lane * 16, a.pool.scale_v + (int64_t)r * L::BLOCKS + (lane & 1) * 4);
+                } else {
+                    copy_async<16>(to + (lane < 16 ? L::SK : L::SV) + tok * 16,
+                                   (lane < 16 ? a.pool.scale_k : a.pool.scale_v) + (int64_t)r * L::BLOCKS);
+                }
+            } else {
+                const int groups = D / a.pool.int4_group;
+#pragma unroll
+                for (int i = 0; i < L::BLOCKS / 2; ++i) {
+                    const int tok = (lane + 32 * i) / L::BLOCKS, block = (lane + 32 * i) % L::BLOCKS;
+                    const int r = p16 ? first + tok : max(__shfl_sync(0xffffffffu, row, tok), 0);
+                    if (block * 16 < D) {
+                        const int64_t x = (int64_t)r * groups + block * 16 / a.pool.int4_group;
+                        copy_async<4>(to + L::SK + (lane + 32 * i) * 4, a.pool.scale_k + x);
+                        copy_async<4>(to + L::SV + (lane + 32 * i) * 4, a.pool.scale_v + x);
+                    }
+                }
+            }
+        }
+        copy_commit();
+        f.st += W;
     };
-    LanePlace<PREC, DP> place;
-    place.set(a.pool, lg, lc);
-    KTile<PREC, DP> kt;
-    VTile<PREC, DP> vt;
-    kt.clear();
-    vt.clear();
-    int st = 0, end = 0, row = -1;   // this warp's tile, the end of its tiles, the rows of the tile's tokens
-    // The next segment, its first tile on the way.
-    auto open = [&]() {
+    int head = 0;   // slot of the tile to multiply; the one before it is free
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) copy_next(ring + i * L::BYTES);
+
+    int at = s.lo, b = s.b, base = s.base;
+    while (at < s.hi) {
         const Segment g = segment_at(a, s, at, TILE, row_tiles, b, base);
         at += g.t1 - g.t0;
-        end = min(g.t1 * W, (g.tokens + 15) / 16);
-        st = g.t0 * W + warp;
-        pages.start(a.pool, g.b, p16 ? page_of(st * 16) : 0);
-        row = -1;
-        if (st < end) {
-            int own[2], four[4];
-            row = row_of(g, st);
-            k_rows(row, own);
-            v_rows(row, four);
-            kt.load(place, own);
-            vt.load(place, four, own);
-        }
-        return g;
-    };
-    Segment g = open();
-    for (;;) {
         const int n = g.tokens, r0 = g.rt * ROWS;
         // ---- queries: a power of two taken out of each row, laid out as B operands
         __syncthreads();
@@ -499,21 +388,35 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
 #pragma unroll
                 for (int k = 0; k < E; ++k) top = fmaxf(top, fabsf(x[i][k]));
                 const int e = clamp_exp(__float_as_uint(warp_max(top)));
-                const float down = exp_down(e);
-                if (lane == 0) s_c[j] = a.scale * 1.4426950408889634f * exp_up(e);
+                const float down = exp_down(e, kQueryExp);
+                if (lane == 0) s_c[j] = a.scale * 1.4426950408889634f * exp_up(e, kQueryExp) * (PREC == 1 ? 1.0f : 1.0f / kSubnormal);
+                float total = 0.0f;
 #pragma unroll
                 for (int k = 0; k < E; ++k) {
                     int mma, c, reg, half;
-                    query_place<PREC>(lane * E + k, mma, c, reg, half);
-                    const float y = x[i][k] * down;
+                    const float part = query_place<PREC, DP>(lane * E + k, mma, c, reg, half);
+                    const float y = x[i][k] * down * part;
                     const __half hi = __float2half_rn(y);
                     __half* q = reinterpret_cast<__half*>(s_q + ((mma * NT + j / 8) * NQ) * 32 + (j % 8) * 4 + c) + 2 * reg + half;
                     q[0] = hi;
-                    if (NQ == 2) q[32 * 4] = __float2half_rn(y - __half2float(hi));
+                    float used = __half2float(hi);
+                    if (NQ == 2) {
+                        const __half lo = __float2half_rn(y - used);
+                        q[32 * 4] = lo;
+                        used += __half2float(lo);
+                    }
+                    total += used / part;
+                }
+                if constexpr (PREC >= 2) {
+                    constexpr int LANES = PREC == 2 ? 32 : 16 / E;   // that share a bias
+#pragma unroll
+                    for (int w = 1; w < LANES; w <<= 1) total += __shfl_xor_sync(0xffffffffu, total, w);
+                    if (lane % LANES == 0) s_bias[lane / LANES * ROWS + j] = total * ((PREC == 2 ? -128.0f : -8.0f) * kSubnormal);
                 }
             }
         }
         __syncthreads();
+        float start_at[NT][2];   // of the score sums
         float cf[NT][2], ref[NT][2], base_of[NT][2], sum[NT][2], o[NT][M][4];   // base_of: ref, or 0 before there is one
         int see[NT][2], see_all = n;
 #pragma unroll
@@ -522,6 +425,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
             for (int i = 0; i < 2; ++i) {
                 const int j = 8 * t + 2 * lc + i;
                 cf[t][i] = s_c[j];
+                start_at[t][i] = PREC == 2 ? s_bias[j] : 0.0f;
                 ref[t][i] = -INFINITY;
                 base_of[t][i] = 0.0f;
                 sum[t][i] = 0.0f;
@@ -537,136 +441,147 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[t][m][i] = 0.0f;
 
-        for (; st < end; st += W) {
-            const bool more = st + W < end;
-            const int next = more ? row_of(g, st + W) : -1;
+        const int end = min(g.t1 * W, (n + 15) / 16);
+        for (int st = g.t0 * W + warp; st < end; st += W) {
+            copy_wait<S - 2>();
+            __syncwarp();
+            copy_next(ring + (head == 0 ? S - 1 : head - 1) * L::BYTES);
+            char* slot = ring + head * L::BYTES;
+            head = head + 1 == S ? 0 : head + 1;
             // ---- tokens that are there
             const int t0 = st * 16;
-            const bool all = t0 + 16 <= see_all && (p16 ? row >= 0 : __all_sync(0xffffffffu, row >= 0));
+            const bool held = *reinterpret_cast<const int*>(slot + L::ID + 4 * (lane & 15)) >= 0;   // token lane % 16
+            const bool all = __all_sync(0xffffffffu, held) && t0 + 16 <= see_all;
             bool here[2] = {true, true};
             if (!all) {
-                bool four[4];
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    here[i] = (p16 ? row : __shfl_sync(0xffffffffu, row, lg + 8 * i)) >= 0 && t0 + lg + 8 * i < n;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int k = 2 * lc + (i & 1) + 8 * (i >> 1);
-                    four[i] = (p16 ? row : __shfl_sync(0xffffffffu, row, k)) >= 0 && t0 + k < n;
+                for (int i = 0; i < 2; ++i) here[i] = __shfl_sync(0xffffffffu, (int)held, lg + 8 * i);
+                // a weight of zero would not hide a NaN in what an absent token's row or scale happens to hold
+                if (!held && lane < 16) {
+                    if constexpr (PREC == 1)
+                        for (int i = 0; i < L::CHUNKS; ++i) *reinterpret_cast<uint4*>(slot + L::V + lane * L::ROW + i * 16) = make_uint4(0, 0, 0, 0);
+                    else
+                        for (int i = 0; i < L::SCALES; ++i) reinterpret_cast<float*>(slot + L::SV)[lane * L::SCALES + i] = 1.0f;
                 }
-                kt.only(here);
-                vt.only(four, here);
+                __syncwarp();
             }
             // ---- scores
-            // CH chains of dependent MMAs at a time: one would be as long as their latencies added up
-            constexpr int CH = NT == 1 ? 4 : NT == 2 ? 2 : 1;
-            float x[NT][4], acc[CH][NT][4];
+            float x[NT][4], k_factor[2] = {1.0f, 1.0f};
+            if constexpr (PREC < 3) {
+                // CH chains of dependent MMAs at a time: one would be as long as their latencies added up
+                constexpr int CH = NT == 1 ? 4 : NT == 2 ? 2 : 1;
+                float acc[CH][NT][4];
+                auto qk = [&](const uint32_t (&f)[4], int m) {
 #pragma unroll
-            for (int h = 0; h < CH; ++h)
+                    for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
+                        for (int q = 0; q < NQ; ++q) {
+                            const int h = (m * NQ + q) % CH;
+                            const uint2 bq = s_q[((m * NT + t) * NQ + q) * 32 + lane];
+                            if (m * NQ + q == 0) mma16816_from(acc[h][t], f, bq, start_at[t][0], start_at[t][1]);
+                            else if (m * NQ + q < CH) mma16816_from(acc[h][t], f, bq, 0.0f, 0.0f);
+                            else mma16816(acc[h][t], f, bq);
+                        }
+                };
+                if constexpr (PREC == 1) {
+                    const uint32_t k = shared_address(slot + L::K);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[h][t][i] = 0.0f;
-            float k_factor[2] = {1.0f, 1.0f};
-            auto qk = [&](const uint32_t (&f)[4], int m, int terms) {
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int q = 0; q < NQ; ++q)
-                        if (q < terms) mma16816(acc[(m * NQ + q) % CH][t], f, s_q[((m * NT + t) * NQ + q) * 32 + lane]);
-            };
-            if constexpr (PREC == 1) {
-#pragma unroll
-                for (int j = 0; j < DP / 32; ++j) {
-                    const uint4 u = kt.x[0][j], v = kt.x[1][j];
-                    const uint32_t f0[4] = {u.x, v.x, u.y, v.y}, f1[4] = {u.z, v.z, u.w, v.w};
-                    qk(f0, 2 * j, NQ);
-                    qk(f1, 2 * j + 1, NQ);
-                }
-            } else if constexpr (PREC == 2) {
-#pragma unroll
-                for (int j = 0; j < DP / 64; ++j) {
-                    const uint32_t u[4] = {kt.x[0][j].x, kt.x[0][j].y, kt.x[0][j].z, kt.x[0][j].w};
-                    const uint32_t v[4] = {kt.x[1][j].x, kt.x[1][j].y, kt.x[1][j].z, kt.x[1][j].w};
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const uint32_t p = u[w] ^ 0x80808080u, q = v[w] ^ 0x80808080u;
-                        const uint32_t f[4] = {i8_pair(p, 0x4140), i8_pair(q, 0x4140), i8_pair(p, 0x4342), i8_pair(q, 0x4342)};
-                        qk(f, 4 * j + w, NQ);
+                    for (int m = 0; m < M; ++m) {
+                        uint32_t f[4];
+                        load_matrix(f, k + L::at(lane & 15, 2 * m + (lane >> 4)));
+                        qk(f, m);
                     }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < DP / 64; ++j) {
+                        const int ch = DP == 128 ? 2 * lc + j : lc;
+                        const uint4 u4 = *reinterpret_cast<const uint4*>(slot + L::K + L::at(lg, ch));
+                        const uint4 v4 = *reinterpret_cast<const uint4*>(slot + L::K + L::at(lg + 8, ch));
+                        const uint32_t u[4] = {u4.x, u4.y, u4.z, u4.w}, v[4] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const uint32_t f[4] = {(u[w] & 0x00FF00FFu) ^ 0x00800080u, (v[w] & 0x00FF00FFu) ^ 0x00800080u,
+                                                   ((u[w] >> 8) & 0x00FF00FFu) ^ 0x00800080u, ((v[w] >> 8) & 0x00FF00FFu) ^ 0x00800080u};
+                            qk(f, 4 * j + w);
+                        }
+                    }
+                    k_factor[0] = reinterpret_cast<const float*>(slot + L::SK)[lg];
+                    k_factor[1] = reinterpret_cast<const float*>(slot + L::SK)[lg + 8];
                 }
-                k_factor[0] = kt.s[0];
-                k_factor[1] = kt.s[1];
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        x[t][i] = acc[0][t][i];
+#pragma unroll
+                        for (int h = 1; h < CH; ++h) x[t][i] += acc[h][t][i];
+                    }
             } else {
-                uint32_t top = 0;
+                // A group of 16 values is one MMA, so that its scale can multiply the result: lane column c takes bytes
+                // 2c, 2c + 1 of each group, of two groups at a time (blocks k and k + M / 2) in one register.
+                const uint32_t pick = lc & 1 ? 0x7362 : 0x5140;
+                float sc[2][M];
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int j = 0; j < DP / 64; ++j) top = max(top, __float_as_uint(kt.s[t][j]) & 0x7fffffffu);
-                const int e = clamp_exp(__reduce_max_sync(0xffffffffu, top));
-                const float down = exp_down(e);
-                k_factor[0] = k_factor[1] = exp_up(e);
-#pragma unroll
-                for (int j = 0; j < DP / 64; ++j) {
-                    uint32_t r1[2], r2[2];
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        float y1, y2;
-                        split_scale(kt.s[t][j] * down, y1, y2);
-                        r1[t] = h2_pack(y1, y1);
-                        r2[t] = h2_pack(y2, y2);
+                    for (int k = 0; k < M / 4; ++k) {
+                        const float4 y = *reinterpret_cast<const float4*>(slot + L::SK + ((lg + 8 * t) * M + 4 * k) * 4);
+                        sc[t][4 * k] = y.x; sc[t][4 * k + 1] = y.y; sc[t][4 * k + 2] = y.z; sc[t][4 * k + 3] = y.w;
                     }
+                auto word = [&](int row, int block) {
+                    return *reinterpret_cast<const uint32_t*>(slot + L::K + L::at(row, block / 2) + 8 * (block % 2) + 4 * (lc >> 1));
+                };
 #pragma unroll
-                    for (int w = 0; w < 2; ++w) {
-                        uint32_t p = w ? kt.x[0][j].y : kt.x[0][j].x, q = w ? kt.x[1][j].y : kt.x[1][j].x;
+                for (int k = 0; k < M / 2; ++k) {
+                    const uint32_t u = __byte_perm(word(lg, k), word(lg, k + M / 2), pick);
+                    const uint32_t v = __byte_perm(word(lg + 8, k), word(lg + 8, k + M / 2), pick);
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const uint32_t f[4] = {i4_high(p), i4_high(q), i4_low(p), i4_low(q)};
-                            const uint32_t f1[4] = {h2_mul(f[0], r1[0]), h2_mul(f[1], r1[1]), h2_mul(f[2], r1[0]), h2_mul(f[3], r1[1])};
-                            const uint32_t f2[4] = {h2_mul(f[0], r2[0]), h2_mul(f[1], r2[1]), h2_mul(f[2], r2[0]), h2_mul(f[3], r2[1])};
-                            qk(f1, 2 * (2 * j + w) + h, NQ);
-                            qk(f2, 2 * (2 * j + w) + h, 1);
-                            p >>= 8;
-                            q >>= 8;
+                    for (int h = 0; h < 2; ++h) {
+                        const int m = k + M / 2 * h;
+                        const uint32_t uh = u >> (8 * h), vh = v >> (8 * h);
+                        const uint32_t f[4] = {uh & 0x00F000F0u, vh & 0x00F000F0u, uh & 0x000F000Fu, vh & 0x000F000Fu};
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) {
+                            float acc[4];
+                            const float2 start = *reinterpret_cast<const float2*>(s_bias + m * ROWS + 8 * t + 2 * lc);
+#pragma unroll
+                            for (int q = 0; q < NQ; ++q) {
+                                const uint2 bq = s_q[((m * NT + t) * NQ + q) * 32 + lane];
+                                if (q == 0) mma16816_from(acc, f, bq, start.x, start.y);
+                                else mma16816(acc, f, bq);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                x[t][i] = k + h == 0 ? acc[i] * sc[i >> 1][m] : fmaf(acc[i], sc[i >> 1][m], x[t][i]);
                         }
                     }
                 }
             }
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[t][i] = acc[0][t][i];
-#pragma unroll
-                    for (int h = 1; h < CH; ++h) x[t][i] += acc[h][t][i];
-                }
-            int own[2];
-            if (more) {
-                k_rows(next, own);
-                kt.load(place, own);
-            }
             // ---- weights
             float v_add[2] = {0.0f, 0.0f}, v_mul[2] = {1.0f, 1.0f}, v_sum[2] = {1.0f, 1.0f};
-            int ve[2] = {0, 0};
+            int token_exp = 0;   // int4: of token lane % 16
             if constexpr (PREC == 2) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    ve[i] = clamp_exp(__float_as_uint(vt.s[i]) & 0x7fffffffu);
-                    v_add[i] = (float)(ve[i] - 127);
-                    v_sum[i] = __uint_as_float((uint32_t)(254 - ve[i]) << 23);   // 2^-(ve - 127)
-                    v_mul[i] = vt.s[i] * v_sum[i];
+                    const float sv = reinterpret_cast<const float*>(slot + L::SV)[lg + 8 * i];
+                    const int e = clamp_exp(__float_as_uint(sv) & 0x7fffffffu);
+                    v_add[i] = (float)(e - 127);
+                    v_sum[i] = __uint_as_float((uint32_t)(254 - e) << 23);   // 2^-(e - 127)
+                    v_mul[i] = sv * v_sum[i];
                 }
             } else if constexpr (PREC == 3) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int k = 0; k < M / 4; ++k) {
+                    const uint4 y = *reinterpret_cast<const uint4*>(slot + L::SV + ((lane & 15) * M + 4 * k) * 4);
+                    top = max(max(top, y.x & 0x7fffffffu), max(y.y & 0x7fffffffu, max(y.z & 0x7fffffffu, y.w & 0x7fffffffu)));
+                }
+                token_exp = clamp_exp(top);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    uint32_t top = 0;
-#pragma unroll
-                    for (int j = 0; j < DP / 64; ++j) top = max(top, __float_as_uint(vt.own[i][j]) & 0x7fffffffu);
-                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    ve[i] = clamp_exp(top);
-                    v_add[i] = (float)(ve[i] - 137);
-                    v_sum[i] = exp_down(ve[i]);                                 // 2^-(ve - 137)
+                    const int e = __shfl_sync(0xffffffffu, token_exp, lg + 8 * i);
+                    v_add[i] = (float)(e - 127 - kValueExp);
+                    v_sum[i] = exp_down(e, kValueExp);                      // 2^-(e - 127 - kValueExp)
                 }
             }
             bool grow = false;
@@ -731,26 +646,32 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                         if (q < terms) mma16816(o[t][m], f, p[t][q]);
             };
             if constexpr (PREC == 1) {
+                const uint32_t v = shared_address(slot + L::V);
 #pragma unroll
-                for (int j = 0; j < DP / 64; ++j) {
-                    const uint32_t u[4][4] = {{vt.x[0][j].x, vt.x[0][j].y, vt.x[0][j].z, vt.x[0][j].w},
-                                              {vt.x[1][j].x, vt.x[1][j].y, vt.x[1][j].z, vt.x[1][j].w},
-                                              {vt.x[2][j].x, vt.x[2][j].y, vt.x[2][j].z, vt.x[2][j].w},
-                                              {vt.x[3][j].x, vt.x[3][j].y, vt.x[3][j].z, vt.x[3][j].w}};
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const uint32_t f[4] = {__byte_perm(u[0][w], u[1][w], 0x5410), __byte_perm(u[0][w], u[1][w], 0x7632),
-                                               __byte_perm(u[2][w], u[3][w], 0x5410), __byte_perm(u[2][w], u[3][w], 0x7632)};
-                        pv(f, 4 * j + w, NP);
-                    }
+                for (int m = 0; m < M; ++m) {
+                    uint32_t f[4];
+                    load_matrix_trans(f, v + L::at((lane & 7) + (lane >> 4) * 8, 2 * m + ((lane >> 3) & 1)));
+                    pv(f, m, NP);
                 }
             } else if constexpr (PREC == 2) {
+                uint32_t vx[4][DP / 32];   // values DP/8 g .. of tokens 2c, 2c + 1, 2c + 8, 2c + 9
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int tok = 2 * lc + (i & 1) + 8 * (i >> 1);
+                    if constexpr (DP == 128) {
+                        const uint4 y = *reinterpret_cast<const uint4*>(slot + L::V + L::at(tok, lg));
+                        vx[i][0] = y.x; vx[i][1] = y.y; vx[i][2] = y.z; vx[i][3] = y.w;
+                    } else {
+                        const uint2 y = *reinterpret_cast<const uint2*>(slot + L::V + L::at(tok, lg / 2) + 8 * (lg & 1));
+                        vx[i][0] = y.x; vx[i][1] = y.y;
+                    }
+                }
 #pragma unroll
                 for (int w = 0; w < DP / 32; ++w) {
                     uint32_t y[2][2];   // [tokens low / high][values 0,1 / 2,3]
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const uint32_t u = word_of(vt.x[2 * h], w) ^ 0x80808080u, v = word_of(vt.x[2 * h + 1], w) ^ 0x80808080u;
+                        const uint32_t u = vx[2 * h][w] ^ 0x80808080u, v = vx[2 * h + 1][w] ^ 0x80808080u;
                         y[h][0] = __byte_perm(u, v, 0x5140);
                         y[h][1] = __byte_perm(u, v, 0x7362);
                     }
@@ -762,48 +683,54 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                     }
                 }
             } else {
-                // the exponents of tokens 2c, 2c + 1 (+ 8) sit in lanes 4 (2c), 4 (2c + 1)
-                uint32_t r1[2], r2[2];
+                // A group's scale in parts of 7 bits (two, or three for 32-bit outputs): x = 64 + (n + 8) times a part
+                // less 72 times it is exact in one fp16 fma.
+                constexpr int PARTS = NQ == 2 ? 3 : 2;
+                uint32_t vx[4][DP / 64], r[PARTS][2], r72[PARTS][2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    float y1[2], y2[2];
+                    float y[2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const int e = __shfl_sync(0xffffffffu, ve[h], 4 * (2 * lc + i));
-                        split_scale(vt.s[2 * h + i] * exp_down(e), y1[i], y2[i]);
+                        const int tok = 2 * lc + i + 8 * h;
+                        if constexpr (DP == 128) {
+                            const uint2 z = *reinterpret_cast<const uint2*>(slot + L::V + L::at(tok, lg / 2) + 8 * (lg & 1));
+                            vx[2 * h + i][0] = z.x; vx[2 * h + i][1] = z.y;
+                        } else {
+                            vx[2 * h + i][0] = *reinterpret_cast<const uint32_t*>(slot + L::V + L::at(tok, lg / 4) + 4 * (lg & 3));
+                        }
+                        y[i] = reinterpret_cast<const float*>(slot + L::SV)[tok * M + lg * M / 8] *
+                               exp_down(__shfl_sync(0xffffffffu, token_exp, tok), kValueExp);
                     }
-                    r1[h] = h2_pack(y1[0], y1[1]);
-                    r2[h] = h2_pack(y2[0], y2[1]);
+#pragma unroll
+                    for (int k = 0; k < PARTS; ++k) {
+                        const float y0 = take7(y[0]), y1 = take7(y[1]);
+                        r[k][h] = h2_pack(y0, y1);
+                        r72[k][h] = h2_pack(-72.0f * y0, -72.0f * y1);
+                    }
                 }
 #pragma unroll
                 for (int w = 0; w < DP / 64; ++w)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        uint32_t u = __byte_perm(word_of(vt.x[0], w), word_of(vt.x[1], w), i ? 0x7632 : 0x5410);
-                        uint32_t v = __byte_perm(word_of(vt.x[2], w), word_of(vt.x[3], w), i ? 0x7632 : 0x5410);
+                        const uint32_t u = __byte_perm(vx[0][w], vx[1][w], i ? 0x7632 : 0x5410);
+                        const uint32_t v = __byte_perm(vx[2][w], vx[3][w], i ? 0x7632 : 0x5410);
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const uint32_t f[4] = {i4_high(u), i4_low(u), i4_high(v), i4_low(v)};
-                            const uint32_t f1[4] = {h2_mul(f[0], r1[0]), h2_mul(f[1], r1[0]), h2_mul(f[2], r1[1]), h2_mul(f[3], r1[1])};
-                            const uint32_t f2[4] = {h2_mul(f[0], r2[0]), h2_mul(f[1], r2[0]), h2_mul(f[2], r2[1]), h2_mul(f[3], r2[1])};
-                            pv(f1, 4 * w + 2 * i + h, NP);
-                            pv(f2, 4 * w + 2 * i + h, 1);
-                            u >>= 8;
-                            v >>= 8;
+                        for (int h = 0; h < 2; ++h) {   // values 0, 1 and 2, 3 of the two bytes
+                            const uint32_t f[4] = {i4_pair(h ? u >> 8 : u), i4_pair(h ? u >> 4 : u << 4),
+                                                   i4_pair(h ? v >> 8 : v), i4_pair(h ? v >> 4 : v << 4)};
+#pragma unroll
+                            for (int k = 0; k < PARTS; ++k) {
+                                const uint32_t y[4] = {h2_fma(f[0], r[k][0], r72[k][0]), h2_fma(f[1], r[k][0], r72[k][0]),
+                                                       h2_fma(f[2], r[k][1], r72[k][1]), h2_fma(f[3], r[k][1], r72[k][1])};
+                                pv(y, 4 * w + 2 * i + h, k == 0 ? NP : 1);
+                            }
                         }
                     }
             }
-            if (more) {
-                int four[4];
-                v_rows(next, four);
-                vt.load(place, four, own);
-            }
-            row = next;
         }
 
-        // ---- the warps' parts joined, while the next segment's first tiles load
-        const bool another = at < s.hi;
-        Segment following;
+        // ---- the warps' parts joined, 8 rows at a time through their free slots
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -812,84 +739,98 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                 l += __shfl_xor_sync(0xffffffffu, l, 4);
                 l += __shfl_xor_sync(0xffffffffu, l, 8);
                 l += __shfl_xor_sync(0xffffffffu, l, 16);
-                const int j = 8 * t + 2 * lc + i;
                 if (lg == 0) {
-                    s_ref[warp * ROWS + j] = ref[t][i];
-                    s_sum[warp * ROWS + j] = l;
-                }
-                float* row = s_o + (warp * ROWS + j) * (DP + 4);
-#pragma unroll
-                for (int m = 0; m < M; ++m) {
-                    const int d = PREC == 1 ? 64 * (m / 4) + 8 * lg + 2 * (m % 4) : lg * (DP / 8) + 2 * m;
-                    *reinterpret_cast<float2*>(row + d) = make_float2(o[t][m][i], o[t][m][i + 2]);
+                    s_ref[warp * ROWS + 8 * t + 2 * lc + i] = ref[t][i];
+                    s_sum[warp * ROWS + 8 * t + 2 * lc + i] = l;
                 }
             }
-        if (another) following = open();
-        __syncthreads();
-        if (tid < ROWS) {
-            float m = -INFINITY, l = 0.0f;
-            for (int w = 0; w < W; ++w) m = fmaxf(m, s_ref[w * ROWS + tid]);
-            const float r = m == -INFINITY ? 0.0f : m;
-            for (int w = 0; w < W; ++w) {
-                const float f = exp2f(s_ref[w * ROWS + tid] - r);
-                s_w[w * ROWS + tid] = f;
-                l += s_sum[w * ROWS + tid] * f;
-            }
-            s_c[tid] = m;
-            s_l[tid] = l;
-        }
-        __syncthreads();
+        const int free_at = (warp * S + (head == 0 ? S - 1 : head - 1)) * L::BYTES;
+        if (lane == 0) s_free[warp] = free_at;
         float* part = slot_of(a, blockIdx.x, g.slot, ROWS);
 #pragma unroll
-        for (int i = tid; i < ROWS * DP / 4; i += THREADS) {
-            const int j = i / (DP / 4), d = i % (DP / 4) * 4;
-            if (r0 + j >= R || d >= D) continue;
-            float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int t = 0; t < NT; ++t) {
+            float* mine = reinterpret_cast<float*>(s_ring + free_at);
+            __syncwarp();
 #pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const float4 v = *reinterpret_cast<const float4*>(s_o + (w * ROWS + j) * (DP + 4) + d);
-                const float f = s_w[w * ROWS + j];
-                y[0] = fmaf(v.x, f, y[0]); y[1] = fmaf(v.y, f, y[1]); y[2] = fmaf(v.z, f, y[2]); y[3] = fmaf(v.w, f, y[3]);
-            }
-            if (!g.whole) {
-                *reinterpret_cast<float4*>(part + j * D + d) = make_float4(y[0], y[1], y[2], y[3]);
-                continue;
-            }
-            const float l = s_l[j];
+            for (int i = 0; i < 2; ++i) {
+                float* row = mine + (2 * lc + i) * (DP + 4);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) y[k] = l == 0.0f ? 0.0f : y[k] / l;
-            store_row(a, g, r0 + j, d, out_vec, y);
+                for (int m = 0; m < M; ++m) {
+                    if constexpr (PREC == 1) {
+                        row[16 * m + lg] = o[t][m][i];
+                        row[16 * m + 8 + lg] = o[t][m][i + 2];
+                    } else {
+                        *reinterpret_cast<float2*>(row + lg * (DP / 8) + 2 * m) = make_float2(o[t][m][i], o[t][m][i + 2]);
+                    }
+                }
+            }
+            __syncthreads();
+            if (t == 0) {
+                if (tid < ROWS) {
+                    float m = -INFINITY, l = 0.0f;
+                    for (int w = 0; w < W; ++w) m = fmaxf(m, s_ref[w * ROWS + tid]);
+                    const float r = m == -INFINITY ? 0.0f : m;
+                    for (int w = 0; w < W; ++w) {
+                        const float y = exp2f(s_ref[w * ROWS + tid] - r);
+                        s_w[w * ROWS + tid] = y;
+                        l += s_sum[w * ROWS + tid] * y;
+                    }
+                    s_c[tid] = m;
+                    s_l[tid] = l;
+                }
+                __syncthreads();
+            }
+#pragma unroll
+            for (int i = tid; i < 8 * DP / 4; i += THREADS) {
+                const int j = 8 * t + i / (DP / 4), d = i % (DP / 4) * 4;
+                if (r0 + j >= R || d >= D) continue;
+                float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    const float4 v = *reinterpret_cast<const float4*>(s_ring + s_free[w] + ((j - 8 * t) * (DP + 4) + d) * 4);
+                    const float z = s_w[w * ROWS + j];
+                    y[0] = fmaf(v.x, z, y[0]); y[1] = fmaf(v.y, z, y[1]); y[2] = fmaf(v.z, z, y[2]); y[3] = fmaf(v.w, z, y[3]);
+                }
+                if (!g.whole) {
+                    *reinterpret_cast<float4*>(part + j * D + d) = make_float4(y[0], y[1], y[2], y[3]);
+                    continue;
+                }
+                const float l = s_l[j];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) y[k] = l == 0.0f ? 0.0f : y[k] / l;
+                store_row(a, g, r0 + j, d, out_vec, y);
+            }
+            if (t + 1 < NT) __syncthreads();
         }
         if (!g.whole) {
             if (tid < ROWS) {
                 part[ROWS * D + tid] = s_c[tid];
                 part[ROWS * D + ROWS + tid] = s_l[tid];
             }
-            if (arrive(a, s, g)) join<ROWS, THREADS, 4, kMmaParts>(a, s, g, R, s_o, out_vec);
+            if (arrive(a, s, g)) join<ROWS, THREADS, 4, kMmaParts>(a, s, g, R, s_join, out_vec);
         }
-        if (!another) break;
-        g = following;
     }
 }
 
-// CTAs an SM: what their registers allow.
 template <int PREC, int DP, int NT, int NQ, int NP>
 int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
-    constexpr int W = NT == 1 && PREC >= 2 ? 8 : 4;
-    constexpr int CTAS = NT >= 4 ? 2 : NT == 2 ? 3 : PREC == 1 ? 3 : 2;
-    static_assert(CTAS * 2 * 8 * NT <= kRowsPerSm, "the scratch holds every CTA's slots");
-    constexpr size_t smem = mma_smem<DP, NT, NQ, W>();
-    const auto kernel = pool_attention_mma_kernel<PREC, DP, NT, NQ, NP, W, CTAS>;
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return fail(SKV_ERR_CUDA, "pool_attention: %s", cudaGetErrorString(e));
-    }
+    using Shape = MmaShape<PREC, DP, NT>;
+    static_assert(Shape::CTAS * 2 * 8 * NT <= kRowsPerSm, "the scratch holds every CTA's slots");
+    constexpr size_t smem = mma_smem<PREC, DP, NT, NQ>();
+    static_assert(Shape::CTAS * (smem + 2048) <= 228 * 1024, "an SM holds the CTAs");
+    const auto kernel = pool_attention_mma_kernel<PREC, DP, NT, NQ, NP>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return fail(SKV_ERR_CUDA, "pool_attention: %s", cudaGetErrorString(e));
     const int R = a.q.heads / a.pool.heads * a.S_q;
     PageDivide magic;
     magic.shift = 31;
     while ((1ll << (magic.shift - 31)) < a.pool.page_size) ++magic.shift;
     magic.mul = (uint32_t)(((1ull << magic.shift) + a.pool.page_size - 1) / a.pool.page_size);
-    kernel<<<sm_count() * CTAS, 32 * W, smem, st>>>(a, (R + 8 * NT - 1) / (8 * NT), magic, rows_aligned(a.q), rows_aligned(a.out));
+    const bool exact = a.pool.head_dim == DP &&
+                       (PREC != 3 || (a.pool.int4_group == 16 && ((reinterpret_cast<uintptr_t>(a.pool.scale_k) |
+                                                                   reinterpret_cast<uintptr_t>(a.pool.scale_v)) & 15) == 0));
+    kernel<<<sm_count() * Shape::CTAS, 32 * Shape::W, smem, st>>>(a, (R + 8 * NT - 1) / (8 * NT), magic, exact, rows_aligned(a.q),
+                                                                  rows_aligned(a.out));
     return check_launch("pool_attention");
 }
 
