@@ -208,7 +208,7 @@ __device__ __forceinline__ void load_part(const float* p, float (&x)[VEC]) {
 // their sums are added in order.  buf: join_floats of shared memory.
 constexpr int kJoinWays = 8;
 template <int ROWS, int THREADS, int PARTS>
-__host__ __device__ constexpr int join_floats() { return PARTS * ROWS + 2 * ROWS + THREADS * 4; }
+__host__ __device__ constexpr int join_floats() { return (PARTS * ROWS > THREADS * 4 ? PARTS * ROWS : THREADS * 4) + 2 * ROWS; }
 
 template <int ROWS, int THREADS, int VEC, int PARTS>
 __device__ __forceinline__ void join(const skv_pool_attention_args& a, const Share& s, const Segment& g, int R, float* buf, bool out_vec = false) {
@@ -219,10 +219,10 @@ __device__ __forceinline__ void join(const skv_pool_attention_args& a, const Sha
     const float* base = slot_of(a, c0, 0, ROWS);
     const float* part0 = slot_of(a, c0, g.first == s.first_of(c0) ? 0 : 1, ROWS);
     auto part = [&](int i) { return i == 0 ? part0 : base + i * stride; };
-    float* s_f = buf;                  // [PARTS][ROWS] 2^(m_i - m) of a block of parts
-    float* s_m = s_f + PARTS * ROWS;   // [ROWS] max over all parts (0 if there is none)
+    float* s_m = buf;                  // [ROWS] max over all parts (0 if there is none)
     float* s_l = s_m + ROWS;           // [ROWS] sum over all parts
-    float* s_add = s_l + ROWS;         // [THREADS][VEC]
+    float* s_f = s_l + ROWS;           // [PARTS][ROWS] 2^(m_i - m) of a block of parts
+    float* s_add = s_f;                // [THREADS][VEC] once the factors are used
     __syncthreads();
     {
         constexpr int TPR = THREADS / ROWS;   // a power of two, at most 32
@@ -310,6 +310,7 @@ __device__ __forceinline__ void join(const skv_pool_attention_args& a, const Sha
             }
         }
         if (ways > 1) {   // items < THREADS: one value a thread, n = 0
+            __syncthreads();
 #pragma unroll
             for (int e = 0; e < VEC; ++e) s_add[tid * VEC + e] = y[0][e];
             __syncthreads();

@@ -197,7 +197,11 @@ struct Slot {
     static constexpr int SCALES = PREC == 1 ? 0 : PREC == 2 ? 1 : BLOCKS;   // a token
     static constexpr int K = 0, V = 16 * ROW, SK = 2 * V, SV = SK + 64 * SCALES, ID = SV + 64 * SCALES, USED = ID + 64;
     static constexpr int MERGE = 8 * (DP + 4) * 4;   // the warp's sums of 8 rows pass through a free slot
-    static constexpr int BYTES = (USED > MERGE ? USED : MERGE) + 15 & ~15;
+    static constexpr int BYTES = ((USED > MERGE ? USED : MERGE) + 127) & ~127;   // lines stay on 128-byte boundaries
+    // The same for row my_row + i STEP, from the address of row my_row (STEP rows: what a warp copies at a time).
+    __device__ static __forceinline__ uint32_t step(uint32_t to, int i, int rows) {
+        return (CHUNKS >= 8 ? to ^ (((i * rows) & 7) << 4) : to) + i * rows * ROW;
+    }
     // Byte of chunk ch of a row: chunks are exchanged within lines of 128 bytes so that the same chunk of 8 rows, and
     // neighbouring chunks of the rows a fragment takes, fall into different banks.
     __device__ static __forceinline__ int at(int row, int ch) {
@@ -272,6 +276,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
     const int my_row = lane / L::CHUNKS, my_chunk = lane % L::CHUNKS;
     const char* k_lane = static_cast<const char*>(a.pool.k) + my_chunk * 16;
     const char* v_lane = static_cast<const char*>(a.pool.v) + my_chunk * 16;
+    const int to_lane = L::at(my_row, my_chunk);
     auto copy_next = [&](char* slot) {
         while (f.st >= f.end) {
             if (f.at >= s.hi) {
@@ -302,14 +307,14 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
             if (page >= 0 && page < a.pool.num_pages) row = (page * a.pool.heads + f.hk) * P + (t - j * P);
             else if (a.error_flag) atomicExch(a.error_flag, 1);
         }
-        const uint32_t to = shared_address(slot);
+        const uint32_t to = shared_address(slot), to_rows = to + L::K + to_lane;
         if (lane < 16) *reinterpret_cast<int*>(slot + L::ID + 4 * lane) = row;
         if (p16 && exact) {
             const char* k = k_lane + (int64_t)(first + my_row) * L::ROW;
             const char* v = v_lane + (int64_t)(first + my_row) * L::ROW;
 #pragma unroll
             for (int i = 0; i < COPIES; ++i) {
-                const uint32_t y = to + L::K + L::at(my_row + i * STEP, my_chunk);
+                const uint32_t y = L::step(to_rows, i, STEP);
                 copy_async<16>(y, k + i * STEP * L::ROW);
                 copy_async<16>(y + L::V, v + i * STEP * L::ROW);
             }
@@ -317,7 +322,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
 #pragma unroll
             for (int i = 0; i < COPIES; ++i) {
                 const int r = p16 ? first + my_row + i * STEP : max(__shfl_sync(0xffffffffu, row, my_row + i * STEP), 0);
-                const uint32_t y = to + L::K + L::at(my_row + i * STEP, my_chunk);
+                const uint32_t y = L::step(to_rows, i, STEP);
                 if (my_chunk * 16 < row_bytes) {
                     copy_async<16>(y, k_lane + (int64_t)r * row_bytes);
                     copy_async<16>(y + L::V, v_lane + (int64_t)r * row_bytes);
