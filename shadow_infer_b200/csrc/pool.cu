@@ -47,7 +47,7 @@ struct TurnedRow {
 
 // Any D, group, strides and alignment: a warp per (token, head) row of q, k or v.
 template <class T>
-__global__ void __launch_bounds__(32 * kPoolWarps) pool_append_kernel(const __grid_constant__ skv_pool_append_args a) {
+__global__ void __launch_bounds__(32 * kPoolWarps) pool_append_any_kernel(const __grid_constant__ skv_pool_append_args a) {
     const int lane = threadIdx.x & 31;
     const int H = a.q.heads + 2 * a.pool.heads;
     const int64_t item = (int64_t)blockIdx.x * kPoolWarps + (threadIdx.x >> 5);
@@ -118,9 +118,127 @@ __global__ void __launch_bounds__(32 * kPoolWarps) pool_append_kernel(const __gr
     }
 }
 
-// A warp per (token, head) row of K and of V.
+// 8 values a lane: blockDim = (lanes a row: a power of two >= D / 8, rows at a time, tokens at a time).  A thread keeps one
+// chunk of one token, reads its cos and sin and finds its page once, and walks the q, k and v heads with two rows on the way
+// at a time.  Every thread stays to the end: rows and int4 groups reduce over aligned lane blocks.
+template <class T, bool SPLIT>
+__global__ void __launch_bounds__(256) pool_append_kernel(const __grid_constant__ skv_pool_append_args a) {
+    const int D = a.pool.head_dim, Hk = a.pool.heads, Hq = a.q.heads, H = Hq + 2 * Hk, half = a.rope.rot / 2;
+    const int tokens = a.pool.batch * a.S, token = blockIdx.x * blockDim.z + threadIdx.z;
+    const int d = 8 * threadIdx.x;
+    const bool there = token < tokens && d < D;
+    const int b = there ? token / a.S : 0, s = there ? token - b * a.S : 0;
+    const int64_t t = there ? (int64_t)a.lengths[b] + s : 0;
+    const bool turns = there && d < a.rope.rot, second = SPLIT && d >= half;
+    float c[8], w[8];
+    bool known = true;
+    if (turns) {
+        const int64_t pos = rope_position(a.rope, b, s, t);
+        known = pos >= 0 && pos < a.rope.max_positions;
+        if (known) {
+            const float* cs = a.rope.cos + pos * half + (SPLIT ? d - (second ? half : 0) : d / 2);
+            const float* sn = a.rope.sin + pos * half + (SPLIT ? d - (second ? half : 0) : d / 2);
+            if constexpr (SPLIT) {
+                load8(cs, c);
+                load8(sn, w);
+            } else {
+                const float4 u = *reinterpret_cast<const float4*>(cs), v = *reinterpret_cast<const float4*>(sn);
+                c[0] = u.x; c[1] = u.y; c[2] = u.z; c[3] = u.w;
+                w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) c[i] = w[i] = __int_as_float(0x7fffffff);
+        }
+    }
+    const bool stored = there && (a.new_lengths == nullptr || s < a.new_lengths[b]);
+    const int64_t row0 = stored ? pool_row(a.pool, b, t) : -1;
+    if (stored && (row0 < 0 || !known) && a.error_flag) atomicExch(a.error_flag, 1);
+    // a key whose position is not known is not stored; its row's first lane speaks for the row
+    const bool key_known = __shfl_sync(0xffffffffu, (int)known, (threadIdx.y * blockDim.x + threadIdx.z * blockDim.x * blockDim.y) & 31);
+    const int p = a.pool.precision, lanes = p == 3 ? a.pool.int4_group / 8 : blockDim.x;
+    const int64_t row_bytes = pool_row_bytes(p, D);
+    const int step = blockDim.y * gridDim.y;
+    const int partner = SPLIT ? (second ? -half : half) : 0;
+    for (int h0 = blockIdx.y * blockDim.y; h0 < H; h0 += 2 * step) {   // alike for all threads of the block
+        float x[2][8], o[2][8];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int h = h0 + threadIdx.y + i * step;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[i][e] = 0.0f;
+            const bool is_q = h < Hq, is_k = !is_q && h < Hq + Hk;
+            if (there && h < H && (is_q || row0 >= 0)) {
+                const skv_rows& in = is_q ? a.q : is_k ? a.k : a.v;
+                const T* q = static_cast<const T*>(in.ptr) + b * in.stride_b + (is_q ? h : is_k ? h - Hq : h - Hq - Hk) * in.stride_h +
+                             s * in.stride_s + d;
+                load8(q, x[i]);
+                if (SPLIT && turns && (is_q || is_k)) load8(q + partner, o[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int h = h0 + threadIdx.y + i * step;
+            const bool is_q = h < Hq, is_k = !is_q && h < Hq + Hk;
+            float (&y)[8] = x[i];
+            if (turns && (is_q || is_k)) {
+                if constexpr (SPLIT) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        y[e] = second ? rope_second(o[i][e], y[e], c[e], w[e]) : rope_first(y[e], o[i][e], c[e], w[e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float u = rope_first(y[2 * e], y[2 * e + 1], c[e], w[e]);
+                        y[2 * e + 1] = rope_second(y[2 * e], y[2 * e + 1], c[e], w[e]);
+                        y[2 * e] = u;
+                    }
+                }
+            }
+            float scale = 1.0f;
+            if (p >= 2) {
+                float m = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(y[e]));
+                scale = quant_scale(group_max(m, lanes), p == 2 ? 127.0f : 7.0f);
+            }
+            if (!there || h >= H) continue;
+            if (is_q) {
+                store8(static_cast<T*>(a.q_out.ptr) + b * a.q_out.stride_b + h * a.q_out.stride_h + s * a.q_out.stride_s + d, y);
+                continue;
+            }
+            if (row0 < 0 || (is_k && !key_known)) continue;
+            const int64_t row = row0 + (int64_t)(is_k ? h - Hq : h - Hq - Hk) * a.pool.page_size;
+            uint8_t* to = static_cast<uint8_t*>(is_k ? a.pool.k : a.pool.v) + row * row_bytes;
+            float* sc = is_k ? a.pool.scale_k : a.pool.scale_v;
+            if (p == 0) {
+                store8(reinterpret_cast<float*>(to) + d, y);
+            } else if (p == 1) {
+                store8(reinterpret_cast<__half*>(to) + d, y);
+            } else {
+                const float rcp = __frcp_rn(scale);
+                uint32_t u[2] = {0, 0};
+                if (p == 2) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        u[e / 4] |= (uint32_t)(quant_value_fast(y[e], scale, rcp, -128, 127) & 0xFF) << (8 * (e & 3));
+                    *reinterpret_cast<uint2*>(to + d) = make_uint2(u[0], u[1]);
+                    if (d == 0) sc[row] = scale;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        u[0] |= ((uint32_t)(quant_value_fast(y[e], scale, rcp, -8, 7) + 8) & 15u) << (8 * (e / 2) + (e & 1 ? 0 : 4));
+                    *reinterpret_cast<uint32_t*>(to + d / 2) = u[0];
+                    if (d % a.pool.int4_group == 0) sc[row * (D / a.pool.int4_group) + d / a.pool.int4_group] = scale;
+                }
+            }
+        }
+    }
+}
+
+// A warp per (token, head) row of K and of V; any D, group, strides and alignment.
 template <class T>
-__global__ void __launch_bounds__(32 * kPoolWarps) pool_read_kernel(const __grid_constant__ skv_pool_read_args a) {
+__global__ void __launch_bounds__(32 * kPoolWarps) pool_read_any_kernel(const __grid_constant__ skv_pool_read_args a) {
     const int lane = threadIdx.x & 31;
     const int64_t item = (int64_t)blockIdx.x * kPoolWarps + (threadIdx.x >> 5);
     const int H = a.pool.heads, D = a.pool.head_dim;
@@ -140,6 +258,91 @@ __global__ void __launch_bounds__(32 * kPoolWarps) pool_read_kernel(const __grid
         for (int d = lane; d < D; d += kWarp)
             out[d] = from_float<T>(row < 0 ? 0.0f : pool_value(a.pool, v, row, d));
     }
+}
+
+// 8 values a lane, K and V, four tokens on the way: blockDim = (D / 8, tokens), grid (token blocks, B * heads).
+template <class T>
+__global__ void __launch_bounds__(256) pool_read_kernel(const __grid_constant__ skv_pool_read_args a) {
+    const int b = blockIdx.y / a.pool.heads, h = blockIdx.y - b * a.pool.heads, d = 8 * threadIdx.x;
+    const int64_t first = a.start ? (int64_t)a.start[b] : 0, length = a.lengths[b];
+    const int s0 = blockIdx.x * blockDim.y * 4 + threadIdx.y;
+    float x[4][2][8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int s = s0 + i * blockDim.y;
+        const int64_t t = first + s;
+        const bool held = s < a.S && t >= 0 && t < length;
+        int64_t row = held ? pool_row(a.pool, b, t) : -1;
+        if (held && row < 0 && a.error_flag) atomicExch(a.error_flag, 1);
+        if (row >= 0) {
+            row += (int64_t)h * a.pool.page_size;
+            pool_values8(a.pool, false, row, d, x[i][0]);
+            pool_values8(a.pool, true, row, d, x[i][1]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[i][0][e] = x[i][1][e] = 0.0f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int s = s0 + i * blockDim.y;
+        if (s >= a.S) break;
+        store8(static_cast<T*>(a.k_out.ptr) + b * a.k_out.stride_b + h * a.k_out.stride_h + s * a.k_out.stride_s + d, x[i][0]);
+        store8(static_cast<T*>(a.v_out.ptr) + b * a.v_out.stride_b + h * a.v_out.stride_h + s * a.v_out.stride_s + d, x[i][1]);
+    }
+}
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <class T>
+int launch_append(const skv_pool_append_args& a, cudaStream_t st) {
+    const int D = a.pool.head_dim, H = a.q.heads + 2 * a.pool.heads;
+    const int64_t tokens = (int64_t)a.pool.batch * a.S;
+    const bool split = !a.rope.interleaved;
+    const int lanes4 = a.pool.precision == 3 ? a.pool.int4_group / 8 : 1;   // of an int4 group
+    const bool vec = D % 8 == 0 && D <= 256 && a.rope.rot % (split ? 16 : 8) == 0 && rows_aligned(a.q) && rows_aligned(a.k) &&
+                     rows_aligned(a.v) && rows_aligned(a.q_out) && aligned16(a.pool.k) && aligned16(a.pool.v) &&
+                     aligned16(a.rope.cos) && aligned16(a.rope.sin) &&
+                     (a.pool.precision != 3 || (a.pool.int4_group % 8 == 0 && (lanes4 & (lanes4 - 1)) == 0));
+    if (!vec) {
+        const int64_t blocks = (tokens * H + kPoolWarps - 1) / kPoolWarps;
+        pool_append_any_kernel<T><<<(unsigned)blocks, 32 * kPoolWarps, 0, st>>>(a);
+        return check_launch("pool_append");
+    }
+    int lanes = 1;
+    while (lanes * 8 < D) lanes *= 2;
+    // rows of a token in as few equal steps of up to 256 threads as fit; rows over more blocks while there are too few
+    // tokens to fill the GPU; whole warps
+    const int fit = 256 / lanes, whole = 32 / lanes > 1 ? 32 / lanes : 1, steps = (H + fit - 1) / fit;
+    int rows = (H + steps - 1) / steps, slices = 1, z = 1;
+    while (rows > whole && tokens * slices < 2 * sm_count()) {
+        slices *= 2;
+        rows = (rows + 1) / 2;
+    }
+    rows = (rows + whole - 1) / whole * whole;
+    while (z * 2 * rows <= fit && tokens * slices >= 8ll * sm_count() * z) z *= 2;
+    const dim3 block(lanes, rows, z), grid((unsigned)((tokens + z - 1) / z), slices);
+    if (split) pool_append_kernel<T, true><<<grid, block, 0, st>>>(a);
+    else pool_append_kernel<T, false><<<grid, block, 0, st>>>(a);
+    return check_launch("pool_append");
+}
+
+template <class T>
+int launch_read(const skv_pool_read_args& a, cudaStream_t st) {
+    const int D = a.pool.head_dim;
+    const int64_t rows = (int64_t)a.pool.batch * a.pool.heads;
+    const bool vec = D % 8 == 0 && D <= 2048 && rows <= 65535 && rows_aligned(a.k_out) && rows_aligned(a.v_out) && aligned16(a.pool.k) &&
+                     aligned16(a.pool.v) && (a.pool.precision != 3 || a.pool.int4_group % 8 == 0);
+    if (!vec) {
+        const int64_t blocks = (rows * a.S + kPoolWarps - 1) / kPoolWarps;
+        pool_read_any_kernel<T><<<(unsigned)blocks, 32 * kPoolWarps, 0, st>>>(a);
+        return check_launch("pool_read");
+    }
+    int tokens = 256 / (D / 8);
+    tokens = tokens < 1 ? 1 : tokens > a.S ? a.S : tokens;
+    const dim3 block(D / 8, tokens), grid((a.S + tokens * 4 - 1) / (tokens * 4), (unsigned)rows);
+    pool_read_kernel<T><<<grid, block, 0, st>>>(a);
+    return check_launch("pool_read");
 }
 
 }  // namespace skv
@@ -166,11 +369,9 @@ int skv_pool_append(const skv_pool_append_args* args, void* stream) {
     const int64_t blocks = ((int64_t)a.pool.batch * a.S * (a.q.heads + 2 * a.pool.heads) + kPoolWarps - 1) / kPoolWarps;
     if (blocks > 0x7fffffff) return fail(SKV_ERR_TOO_LARGE, "pool_append: too many rows");
     cudaStream_t st = as_stream(stream);
-    const int threads = 32 * kPoolWarps;
-    if (a.k.dtype == kF32) pool_append_kernel<float><<<(unsigned)blocks, threads, 0, st>>>(a);
-    else if (a.k.dtype == kF16) pool_append_kernel<__half><<<(unsigned)blocks, threads, 0, st>>>(a);
-    else pool_append_kernel<__nv_bfloat16><<<(unsigned)blocks, threads, 0, st>>>(a);
-    return check_launch("pool_append");
+    if (a.k.dtype == kF32) return launch_append<float>(a, st);
+    if (a.k.dtype == kF16) return launch_append<__half>(a, st);
+    return launch_append<__nv_bfloat16>(a, st);
 }
 
 int skv_pool_read(const skv_pool_read_args* args, void* stream) {
@@ -188,11 +389,9 @@ int skv_pool_read(const skv_pool_read_args* args, void* stream) {
     const int64_t blocks = ((int64_t)a.pool.batch * a.S * a.pool.heads + kPoolWarps - 1) / kPoolWarps;
     if (blocks > 0x7fffffff) return fail(SKV_ERR_TOO_LARGE, "pool_read: too many rows");
     cudaStream_t st = as_stream(stream);
-    const int threads = 32 * kPoolWarps;
-    if (a.k_out.dtype == kF32) pool_read_kernel<float><<<(unsigned)blocks, threads, 0, st>>>(a);
-    else if (a.k_out.dtype == kF16) pool_read_kernel<__half><<<(unsigned)blocks, threads, 0, st>>>(a);
-    else pool_read_kernel<__nv_bfloat16><<<(unsigned)blocks, threads, 0, st>>>(a);
-    return check_launch("pool_read");
+    if (a.k_out.dtype == kF32) return launch_read<float>(a, st);
+    if (a.k_out.dtype == kF16) return launch_read<__half>(a, st);
+    return launch_read<__nv_bfloat16>(a, st);
 }
 
 }  // extern "C"

@@ -26,7 +26,7 @@ int check_rope(const skv_rope& r, int D, const char* what) {
 
 // Any D, strides and alignment: grid (B * S, head slices), a thread per value.
 template <class T>
-__global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ skv_rotary_args a) {
+__global__ void __launch_bounds__(256) rotary_any_kernel(const __grid_constant__ skv_rotary_args a) {
     const int bs = blockIdx.x, b = bs / a.S, s = bs % a.S;
     const int64_t pos = rope_position(a.rope, b, s, s);
     const bool known = pos >= 0 && pos < a.rope.max_positions;
@@ -54,6 +54,117 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ skv
     }
 }
 
+// 8 values a load.  A row is cut into items: 16 half-split values (8 of each half) or 8 interleaved ones that turn, or 8 that
+// are copied.  blockDim = (items, heads at a time, tokens at a time): a thread keeps its item of one token, so it reads cos and
+// sin once and walks the heads, two rows on the way at a time.
+template <class T, bool SPLIT>
+__global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ skv_rotary_args a, int turned, int tokens) {
+    const int token = blockIdx.x * blockDim.z + threadIdx.z;
+    if (token >= tokens) return;
+    const int b = token / a.S, s = token - b * a.S, item = threadIdx.x, half = a.rope.rot / 2;
+    const bool turns = item < turned;
+    const int d = SPLIT ? (turns ? 8 * item : a.rope.rot + 8 * (item - turned)) : 8 * item;
+    float c[8], w[8];
+    if (turns) {
+        const int64_t pos = rope_position(a.rope, b, s, s);
+        if (pos >= 0 && pos < a.rope.max_positions) {
+            const float* cs = a.rope.cos + pos * half + (SPLIT ? d : d / 2);
+            const float* sn = a.rope.sin + pos * half + (SPLIT ? d : d / 2);
+            if constexpr (SPLIT) {
+                load8(cs, c);
+                load8(sn, w);
+            } else {
+                const float4 u = *reinterpret_cast<const float4*>(cs), v = *reinterpret_cast<const float4*>(sn);
+                c[0] = u.x; c[1] = u.y; c[2] = u.z; c[3] = u.w;
+                w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+            }
+            if (a.rope.inverse)
+#pragma unroll
+                for (int i = 0; i < (SPLIT ? 8 : 4); ++i) w[i] = -w[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) c[i] = w[i] = __int_as_float(0x7fffffff);
+        }
+    }
+    const T* q = static_cast<const T*>(a.q.ptr) + b * a.q.stride_b + s * a.q.stride_s + d;
+    const T* k = static_cast<const T*>(a.k.ptr) + b * a.k.stride_b + s * a.k.stride_s + d;
+    T* qo = static_cast<T*>(a.q_out.ptr) + b * a.q_out.stride_b + s * a.q_out.stride_s + d;
+    T* ko = static_cast<T*>(a.k_out.ptr) + b * a.k_out.stride_b + s * a.k_out.stride_s + d;
+    const int H = a.q.heads + a.k.heads, step = blockDim.y * gridDim.y;
+    for (int h0 = blockIdx.y * blockDim.y + threadIdx.y; h0 < H; h0 += 2 * step) {
+        float x[2][8], y[2][8];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int h = h0 + i * step;
+            if (h < H) {
+                const T* p = h < a.q.heads ? q + h * a.q.stride_h : k + (h - a.q.heads) * a.k.stride_h;
+                load8(p, x[i]);
+                if (SPLIT && turns) load8(p + half, y[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int h = h0 + i * step;
+            if (h >= H) break;
+            T* p = h < a.q.heads ? qo + h * a.q_out.stride_h : ko + (h - a.q.heads) * a.k_out.stride_h;
+            if (turns) {
+                if constexpr (SPLIT) {
+                    float u[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        u[e] = rope_first(x[i][e], y[i][e], c[e], w[e]);
+                        y[i][e] = rope_second(x[i][e], y[i][e], c[e], w[e]);
+                    }
+                    store8(p, u);
+                    store8(p + half, y[i]);
+                    continue;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float u = rope_first(x[i][2 * e], x[i][2 * e + 1], c[e], w[e]);
+                        x[i][2 * e + 1] = rope_second(x[i][2 * e], x[i][2 * e + 1], c[e], w[e]);
+                        x[i][2 * e] = u;
+                    }
+                }
+            }
+            store8(p, x[i]);
+        }
+    }
+}
+
+template <class T>
+int launch_rotary(const skv_rotary_args& a, cudaStream_t st) {
+    const int tokens = a.B * a.S, H = a.q.heads + a.k.heads;
+    const bool split = !a.rope.interleaved;
+    // 8-value items: rows on 16-byte boundaries, turned parts of whole items, tables on 16 bytes too
+    const bool vec = a.D % 8 == 0 && a.rope.rot % (split ? 16 : 8) == 0 && a.D <= 1024 && rows_aligned(a.q) && rows_aligned(a.k) &&
+                     rows_aligned(a.q_out) && rows_aligned(a.k_out) &&
+                     ((reinterpret_cast<uintptr_t>(a.rope.cos) | reinterpret_cast<uintptr_t>(a.rope.sin)) & 15) == 0;
+    if (!vec) {
+        const int64_t slices = ((int64_t)H * a.D + 1023) / 1024;
+        rotary_any_kernel<T><<<dim3((unsigned)tokens, (unsigned)(slices < 65535 ? slices : 65535)), 256, 0, st>>>(a);
+        return check_launch("rotary");
+    }
+    const int turned = split ? a.rope.rot / 16 : a.rope.rot / 8;
+    const int items = turned + (a.D - a.rope.rot) / 8;
+    // a block of up to 256 threads: the heads in as few equal steps as fit, then more tokens; heads over more blocks
+    // while there are too few tokens to fill the GPU
+    int steps = (H * items + 255) / 256;
+    while ((H + steps - 1) / steps * items > 256) ++steps;
+    int heads = (H + steps - 1) / steps;
+    int slices = 1;
+    while (heads > 1 && (int64_t)tokens * slices < sm_count() && slices * 2 <= H) {
+        slices *= 2;
+        heads = (H + slices * steps - 1) / (slices * steps);
+    }
+    const int together = 256 / (items * heads) > 1 ? 256 / (items * heads) : 1;
+    const int z = (int64_t)tokens * slices >= (int64_t)together * 4 * sm_count() ? (together < 64 ? together : 64) : 1;
+    const dim3 block(items, heads, z), grid((tokens + z - 1) / z, slices);
+    if (split) rotary_kernel<T, true><<<grid, block, 0, st>>>(a, turned, tokens);
+    else rotary_kernel<T, false><<<grid, block, 0, st>>>(a, turned, tokens);
+    return check_launch("rotary");
+}
+
 }  // namespace skv
 
 using namespace skv;
@@ -75,10 +186,7 @@ extern "C" int skv_rotary(const skv_rotary_args* args, void* stream) {
     if (tokens == 0 || H == 0) return SKV_OK;
     if (tokens > 0x7fffffff || H * a.D > 0x7fffffff) return fail(SKV_ERR_TOO_LARGE, "rotary: too many rows");
     cudaStream_t st = as_stream(stream);
-    const int64_t slices = (H * a.D + 1023) / 1024;
-    const dim3 grid((unsigned)tokens, (unsigned)(slices < 65535 ? slices : 65535));
-    if (a.q.dtype == kF32) rotary_kernel<float><<<grid, 256, 0, st>>>(a);
-    else if (a.q.dtype == kF16) rotary_kernel<__half><<<grid, 256, 0, st>>>(a);
-    else rotary_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a);
-    return check_launch("rotary");
+    if (a.q.dtype == kF32) return launch_rotary<float>(a, st);
+    if (a.q.dtype == kF16) return launch_rotary<__half>(a, st);
+    return launch_rotary<__nv_bfloat16>(a, st);
 }
