@@ -119,17 +119,35 @@ __global__ void __launch_bounds__(32 * kPoolWarps) pool_append_any_kernel(const 
 }
 
 // 8 values a lane: blockDim = (lanes a row: a power of two >= D / 8, rows at a time, tokens at a time).  A thread keeps one
-// chunk of one token, reads its cos and sin and finds its page once, and walks the q, k and v heads with two rows on the way
-// at a time.  Every thread stays to the end: rows and int4 groups reduce over aligned lane blocks.
+// chunk of one token, reads its cos and sin and finds its page once, and walks the q, k and v heads with FLY rows on the way,
+// the first ones asked for before anything else.  Every thread stays to the end: rows and int4 groups reduce over aligned lane blocks.
 template <class T, bool SPLIT>
 __global__ void __launch_bounds__(256) pool_append_kernel(const __grid_constant__ skv_pool_append_args a) {
+    constexpr int FLY = sizeof(T) == 2 ? 4 : 2;
     const int D = a.pool.head_dim, Hk = a.pool.heads, Hq = a.q.heads, H = Hq + 2 * Hk, half = a.rope.rot / 2;
     const int tokens = a.pool.batch * a.S, token = blockIdx.x * blockDim.z + threadIdx.z;
     const int d = 8 * threadIdx.x;
     const bool there = token < tokens && d < D;
     const int b = there ? token / a.S : 0, s = there ? token - b * a.S : 0;
-    const int64_t t = there ? (int64_t)a.lengths[b] + s : 0;
     const bool turns = there && d < a.rope.rot, second = SPLIT && d >= half;
+    const int step = blockDim.y * gridDim.y, partner = SPLIT ? (second ? -half : half) : 0;
+    Raw8<T> u[FLY], v[FLY];
+    auto fetch = [&](int h0) {
+#pragma unroll
+        for (int i = 0; i < FLY; ++i) {
+            const int h = h0 + threadIdx.y + i * step;
+            if (there && h < H) {
+                const bool is_q = h < Hq, is_k = !is_q && h < Hq + Hk;
+                const skv_rows& in = is_q ? a.q : is_k ? a.k : a.v;
+                const T* x = static_cast<const T*>(in.ptr) + b * in.stride_b + (is_q ? h : is_k ? h - Hq : h - Hq - Hk) * in.stride_h +
+                             s * in.stride_s + d;
+                u[i].load(x);
+                if (SPLIT && turns && (is_q || is_k)) v[i].load(x + partner);
+            }
+        }
+    };
+    fetch(blockIdx.y * blockDim.y);
+    const int64_t t = there ? (int64_t)a.lengths[b] + s : 0;
     float c[8], w[8];
     bool known = true;
     if (turns) {
@@ -158,40 +176,31 @@ __global__ void __launch_bounds__(256) pool_append_kernel(const __grid_constant_
     const bool key_known = __shfl_sync(0xffffffffu, (int)known, (threadIdx.y * blockDim.x + threadIdx.z * blockDim.x * blockDim.y) & 31);
     const int p = a.pool.precision, lanes = p == 3 ? a.pool.int4_group / 8 : blockDim.x;
     const int64_t row_bytes = pool_row_bytes(p, D);
-    const int step = blockDim.y * gridDim.y;
-    const int partner = SPLIT ? (second ? -half : half) : 0;
-    for (int h0 = blockIdx.y * blockDim.y; h0 < H; h0 += 2 * step) {   // alike for all threads of the block
-        float x[2][8], o[2][8];
+    for (int h0 = blockIdx.y * blockDim.y; h0 < H;) {   // alike for all threads of the block
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < FLY; ++i) {
             const int h = h0 + threadIdx.y + i * step;
+            const bool is_q = h < Hq, is_k = !is_q && h < Hq + Hk, here = there && h < H;
+            float y[8];
+            if (here) {
+                u[i].get(y);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[i][e] = 0.0f;
-            const bool is_q = h < Hq, is_k = !is_q && h < Hq + Hk;
-            if (there && h < H && (is_q || row0 >= 0)) {
-                const skv_rows& in = is_q ? a.q : is_k ? a.k : a.v;
-                const T* q = static_cast<const T*>(in.ptr) + b * in.stride_b + (is_q ? h : is_k ? h - Hq : h - Hq - Hk) * in.stride_h +
-                             s * in.stride_s + d;
-                load8(q, x[i]);
-                if (SPLIT && turns && (is_q || is_k)) load8(q + partner, o[i]);
+                for (int e = 0; e < 8; ++e) y[e] = 0.0f;
             }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int h = h0 + threadIdx.y + i * step;
-            const bool is_q = h < Hq, is_k = !is_q && h < Hq + Hk;
-            float (&y)[8] = x[i];
-            if (turns && (is_q || is_k)) {
+            if (turns && here && (is_q || is_k)) {
                 if constexpr (SPLIT) {
+                    float o[8];
+                    v[i].get(o);
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        y[e] = second ? rope_second(o[i][e], y[e], c[e], w[e]) : rope_first(y[e], o[i][e], c[e], w[e]);
+                        y[e] = second ? rope_second(o[e], y[e], c[e], w[e]) : rope_first(y[e], o[e], c[e], w[e]);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float u = rope_first(y[2 * e], y[2 * e + 1], c[e], w[e]);
+                        const float z = rope_first(y[2 * e], y[2 * e + 1], c[e], w[e]);
                         y[2 * e + 1] = rope_second(y[2 * e], y[2 * e + 1], c[e], w[e]);
-                        y[2 * e] = u;
+                        y[2 * e] = z;
                     }
                 }
             }
@@ -202,7 +211,7 @@ __global__ void __launch_bounds__(256) pool_append_kernel(const __grid_constant_
                 for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(y[e]));
                 scale = quant_scale(group_max(m, lanes), p == 2 ? 127.0f : 7.0f);
             }
-            if (!there || h >= H) continue;
+            if (!here) continue;
             if (is_q) {
                 store8(static_cast<T*>(a.q_out.ptr) + b * a.q_out.stride_b + h * a.q_out.stride_h + s * a.q_out.stride_s + d, y);
                 continue;
@@ -217,22 +226,24 @@ __global__ void __launch_bounds__(256) pool_append_kernel(const __grid_constant_
                 store8(reinterpret_cast<__half*>(to) + d, y);
             } else {
                 const float rcp = __frcp_rn(scale);
-                uint32_t u[2] = {0, 0};
+                uint32_t n[2] = {0, 0};
                 if (p == 2) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        u[e / 4] |= (uint32_t)(quant_value_fast(y[e], scale, rcp, -128, 127) & 0xFF) << (8 * (e & 3));
-                    *reinterpret_cast<uint2*>(to + d) = make_uint2(u[0], u[1]);
+                        n[e / 4] |= (uint32_t)(quant_value_fast(y[e], scale, rcp, -128, 127) & 0xFF) << (8 * (e & 3));
+                    *reinterpret_cast<uint2*>(to + d) = make_uint2(n[0], n[1]);
                     if (d == 0) sc[row] = scale;
                 } else {
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        u[0] |= ((uint32_t)(quant_value_fast(y[e], scale, rcp, -8, 7) + 8) & 15u) << (8 * (e / 2) + (e & 1 ? 0 : 4));
-                    *reinterpret_cast<uint32_t*>(to + d / 2) = u[0];
+                        n[0] |= ((uint32_t)(quant_value_fast(y[e], scale, rcp, -8, 7) + 8) & 15u) << (8 * (e / 2) + (e & 1 ? 0 : 4));
+                    *reinterpret_cast<uint32_t*>(to + d / 2) = n[0];
                     if (d % a.pool.int4_group == 0) sc[row * (D / a.pool.int4_group) + d / a.pool.int4_group] = scale;
                 }
             }
         }
+        h0 += FLY * step;
+        if (h0 < H) fetch(h0);
     }
 }
 
@@ -260,35 +271,53 @@ __global__ void __launch_bounds__(32 * kPoolWarps) pool_read_any_kernel(const __
     }
 }
 
-// 8 values a lane, K and V, four tokens on the way: blockDim = (D / 8, tokens), grid (token blocks, B * heads).
-template <class T>
+// 16 bytes of output a lane (V values), of K and V, FLY tokens on the way: blockDim = (D / V, tokens), grid (token blocks,
+// B * heads).
+template <class T, int PREC>
 __global__ void __launch_bounds__(256) pool_read_kernel(const __grid_constant__ skv_pool_read_args a) {
-    const int b = blockIdx.y / a.pool.heads, h = blockIdx.y - b * a.pool.heads, d = 8 * threadIdx.x;
+    constexpr int V = 16 / sizeof(T), FLY = 4;
+    const int b = blockIdx.y / a.pool.heads, h = blockIdx.y - b * a.pool.heads, d = V * threadIdx.x;
     const int64_t first = a.start ? (int64_t)a.start[b] : 0, length = a.lengths[b];
-    const int s0 = blockIdx.x * blockDim.y * 4 + threadIdx.y;
-    float x[4][2][8];
+    const int s0 = blockIdx.x * blockDim.y * FLY + threadIdx.y;
+    PoolRaw<PREC, V> k[FLY], v[FLY];
+    int64_t row[FLY];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < FLY; ++i) {
         const int s = s0 + i * blockDim.y;
         const int64_t t = first + s;
         const bool held = s < a.S && t >= 0 && t < length;
-        int64_t row = held ? pool_row(a.pool, b, t) : -1;
-        if (held && row < 0 && a.error_flag) atomicExch(a.error_flag, 1);
-        if (row >= 0) {
-            row += (int64_t)h * a.pool.page_size;
-            pool_values8(a.pool, false, row, d, x[i][0]);
-            pool_values8(a.pool, true, row, d, x[i][1]);
-        } else {
+        row[i] = held ? pool_row(a.pool, b, t) : -1;
+        if (held && row[i] < 0 && a.error_flag) atomicExch(a.error_flag, 1);
+    }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[i][0][e] = x[i][1][e] = 0.0f;
+    for (int i = 0; i < FLY; ++i) {
+        if (row[i] >= 0) {
+            k[i].load(a.pool, false, row[i] + (int64_t)h * a.pool.page_size, d);
+            v[i].load(a.pool, true, row[i] + (int64_t)h * a.pool.page_size, d);
+        } else {
+            k[i].zero();
+            v[i].zero();
         }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < FLY; ++i) {
         const int s = s0 + i * blockDim.y;
         if (s >= a.S) break;
-        store8(static_cast<T*>(a.k_out.ptr) + b * a.k_out.stride_b + h * a.k_out.stride_h + s * a.k_out.stride_s + d, x[i][0]);
-        store8(static_cast<T*>(a.v_out.ptr) + b * a.v_out.stride_b + h * a.v_out.stride_h + s * a.v_out.stride_s + d, x[i][1]);
+        float x[V], y[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            x[e] = k[i].get(e);
+            y[e] = v[i].get(e);
+        }
+        T* to = static_cast<T*>(a.k_out.ptr) + b * a.k_out.stride_b + h * a.k_out.stride_h + s * a.k_out.stride_s + d;
+        T* vo = static_cast<T*>(a.v_out.ptr) + b * a.v_out.stride_b + h * a.v_out.stride_h + s * a.v_out.stride_s + d;
+        if constexpr (V == 4) {
+            *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4*>(vo) = make_float4(y[0], y[1], y[2], y[3]);
+        } else {
+            store8(to, x);
+            store8(vo, y);
+        }
     }
 }
 
@@ -311,10 +340,11 @@ int launch_append(const skv_pool_append_args& a, cudaStream_t st) {
     }
     int lanes = 1;
     while (lanes * 8 < D) lanes *= 2;
-    // rows of a token in as few equal steps of up to 256 threads as fit; rows over more blocks while there are too few
-    // tokens to fill the GPU; whole warps
-    const int fit = 256 / lanes, whole = 32 / lanes > 1 ? 32 / lanes : 1, steps = (H + fit - 1) / fit;
-    int rows = (H + steps - 1) / steps, slices = 1, z = 1;
+    // a token's rows in one pass of FLY rows a thread where up to 256 threads hold them; rows over more blocks while there are
+    // too few tokens to fill the GPU; whole warps
+    constexpr int FLY = sizeof(T) == 2 ? 4 : 2;
+    const int fit = 256 / lanes, whole = 32 / lanes > 1 ? 32 / lanes : 1;
+    int rows = (H + FLY - 1) / FLY < fit ? (H + FLY - 1) / FLY : fit, slices = 1, z = 1;
     while (rows > whole && tokens * slices < 2 * sm_count()) {
         slices *= 2;
         rows = (rows + 1) / 2;
@@ -331,17 +361,23 @@ template <class T>
 int launch_read(const skv_pool_read_args& a, cudaStream_t st) {
     const int D = a.pool.head_dim;
     const int64_t rows = (int64_t)a.pool.batch * a.pool.heads;
-    const bool vec = D % 8 == 0 && D <= 2048 && rows <= 65535 && rows_aligned(a.k_out) && rows_aligned(a.v_out) && aligned16(a.pool.k) &&
+    const bool vec = D % 8 == 0 && D <= 1024 && rows <= 65535 && rows_aligned(a.k_out) && rows_aligned(a.v_out) && aligned16(a.pool.k) &&
                      aligned16(a.pool.v) && (a.pool.precision != 3 || a.pool.int4_group % 8 == 0);
     if (!vec) {
         const int64_t blocks = (rows * a.S + kPoolWarps - 1) / kPoolWarps;
         pool_read_any_kernel<T><<<(unsigned)blocks, 32 * kPoolWarps, 0, st>>>(a);
         return check_launch("pool_read");
     }
-    int tokens = 256 / (D / 8);
+    const int lanes = D / (16 / (int)sizeof(T));
+    int tokens = 256 / lanes;
     tokens = tokens < 1 ? 1 : tokens > a.S ? a.S : tokens;
-    const dim3 block(D / 8, tokens), grid((a.S + tokens * 4 - 1) / (tokens * 4), (unsigned)rows);
-    pool_read_kernel<T><<<grid, block, 0, st>>>(a);
+    const dim3 block(lanes, tokens), grid((a.S + tokens * 4 - 1) / (tokens * 4), (unsigned)rows);
+    switch (a.pool.precision) {
+        case 0: pool_read_kernel<T, 0><<<grid, block, 0, st>>>(a); break;
+        case 1: pool_read_kernel<T, 1><<<grid, block, 0, st>>>(a); break;
+        case 2: pool_read_kernel<T, 2><<<grid, block, 0, st>>>(a); break;
+        default: pool_read_kernel<T, 3><<<grid, block, 0, st>>>(a);
+    }
     return check_launch("pool_read");
 }
 

@@ -20,6 +20,31 @@ template <> __device__ __forceinline__ float from_float<float>(float x) { return
 template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// 8 consecutive values as loaded, so that several loads are on the way before the first is widened.
+template <class T> struct Raw8 {   // 16-bit types
+    uint4 v;
+    __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const T* h = reinterpret_cast<const T*>(&w[i]);
+            x[2 * i] = to_float(h[0]);
+            x[2 * i + 1] = to_float(h[1]);
+        }
+    }
+};
+template <> struct Raw8<float> {
+    float4 u, v;
+    __device__ __forceinline__ void load(const float* p) {
+        u = reinterpret_cast<const float4*>(p)[0];
+        v = reinterpret_cast<const float4*>(p)[1];
+    }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w; x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
+    }
+};
+
 // 8 consecutive values (16-byte aligned rows).
 __device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
     const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
@@ -98,31 +123,43 @@ __device__ __forceinline__ float pool_value(const skv_pool& p, bool is_v, int64_
     }
 }
 
-// 8 consecutive values of a pool row (D and the int4 group multiples of 8, aligned payload).
-__device__ __forceinline__ void pool_values8(const skv_pool& p, bool is_v, int64_t row, int col, float (&x)[8]) {
-    const uint8_t* base = static_cast<const uint8_t*>(is_v ? p.v : p.k);
-    const float* sc = is_v ? p.scale_v : p.scale_k;
-    const int D = p.head_dim;
-    if (p.precision == 0) {
-        load8(reinterpret_cast<const float*>(base) + row * D + col, x);
-    } else if (p.precision == 1) {
-        load8(reinterpret_cast<const __half*>(base) + row * D + col, x);
-    } else if (p.precision == 2) {
-        const uint2 u = *reinterpret_cast<const uint2*>(base + row * D + col);
-        const float s = sc[row];
+// V consecutive values (4 or 8) of a pool row as loaded, with their scale; D and the int4 group multiples of 8, aligned payload.
+template <int PREC, int V> struct PoolRaw {
+    static constexpr int BYTES = V * (PREC == 0 ? 4 : PREC == 1 ? 2 : 1) / (PREC == 3 ? 2 : 1), WORDS = (BYTES + 3) / 4;
+    uint32_t w[WORDS];
+    float s;
+    __device__ __forceinline__ void load(const skv_pool& p, bool is_v, int64_t row, int col) {
+        const char* base = static_cast<const char*>(is_v ? p.v : p.k) + (PREC == 3 ? (row * p.head_dim + col) / 2
+                                                                                   : (row * p.head_dim + col) * (PREC == 0 ? 4 : PREC == 1 ? 2 : 1));
+        if constexpr (BYTES == 2) {
+            w[0] = *reinterpret_cast<const uint16_t*>(base);
+        } else if constexpr (BYTES == 4) {
+            w[0] = *reinterpret_cast<const uint32_t*>(base);
+        } else if constexpr (BYTES == 8) {
+            const uint2 u = *reinterpret_cast<const uint2*>(base);
+            w[0] = u.x; w[1] = u.y;
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = __fmul_rn((float)(int8_t)((i < 4 ? u.x : u.y) >> (8 * (i & 3))), s);
-    } else {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(base + (row * D + col) / 2);
-        const float s = sc[row * (D / p.int4_group) + col / p.int4_group];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t byte = (w >> (8 * i)) & 0xFFu;
-            x[2 * i] = __fmul_rn((float)((int)(byte >> 4) - 8), s);
-            x[2 * i + 1] = __fmul_rn((float)((int)(byte & 15u) - 8), s);
+            for (int i = 0; i < BYTES / 16; ++i) {
+                const uint4 u = reinterpret_cast<const uint4*>(base)[i];
+                w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
+            }
         }
+        const float* sc = is_v ? p.scale_v : p.scale_k;
+        s = PREC == 2 ? sc[row] : PREC == 3 ? sc[row * (p.head_dim / p.int4_group) + col / p.int4_group] : 1.0f;
     }
-}
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) w[i] = PREC == 3 ? 0x88888888u : 0u;
+        s = 0.0f;
+    }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (PREC == 0) return __uint_as_float(w[i]);
+        else if constexpr (PREC == 1) return __half2float(__ushort_as_half((unsigned short)(w[i / 2] >> (16 * (i & 1)))));
+        else if constexpr (PREC == 2) return __fmul_rn((float)(int8_t)(w[i / 4] >> (8 * (i & 3))), s);
+        else return __fmul_rn((float)((int)((w[i / 8] >> (8 * ((i % 8) / 2) + (i & 1 ? 0 : 4))) & 15u) - 8), s);
+    }
+};
 
 // The position of token s of sequence b: rope.positions, or `own`.
 __device__ __forceinline__ int64_t rope_position(const skv_rope& r, int b, int s, int64_t own) {

@@ -56,14 +56,34 @@ __global__ void __launch_bounds__(256) rotary_any_kernel(const __grid_constant__
 
 // 8 values a load.  A row is cut into items: 16 half-split values (8 of each half) or 8 interleaved ones that turn, or 8 that
 // are copied.  blockDim = (items, heads at a time, tokens at a time): a thread keeps its item of one token, so it reads cos and
-// sin once and walks the heads, two rows on the way at a time.
+// sin once, and walks the heads with FLY rows on the way; the first rows are asked for before the position is known.
 template <class T, bool SPLIT>
 __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ skv_rotary_args a, int turned, int tokens) {
+    constexpr int FLY = sizeof(T) == 2 ? 4 : 2;
     const int token = blockIdx.x * blockDim.z + threadIdx.z;
     if (token >= tokens) return;
     const int b = token / a.S, s = token - b * a.S, item = threadIdx.x, half = a.rope.rot / 2;
     const bool turns = item < turned;
     const int d = SPLIT ? (turns ? 8 * item : a.rope.rot + 8 * (item - turned)) : 8 * item;
+    const T* q = static_cast<const T*>(a.q.ptr) + b * a.q.stride_b + s * a.q.stride_s + d;
+    const T* k = static_cast<const T*>(a.k.ptr) + b * a.k.stride_b + s * a.k.stride_s + d;
+    T* qo = static_cast<T*>(a.q_out.ptr) + b * a.q_out.stride_b + s * a.q_out.stride_s + d;
+    T* ko = static_cast<T*>(a.k_out.ptr) + b * a.k_out.stride_b + s * a.k_out.stride_s + d;
+    const int H = a.q.heads + a.k.heads, step = blockDim.y * gridDim.y;
+    Raw8<T> u[FLY], v[FLY];
+    auto fetch = [&](int h0) {
+#pragma unroll
+        for (int i = 0; i < FLY; ++i) {
+            const int h = h0 + i * step;
+            if (h < H) {
+                const T* p = h < a.q.heads ? q + h * a.q.stride_h : k + (h - a.q.heads) * a.k.stride_h;
+                u[i].load(p);
+                if (SPLIT && turns) v[i].load(p + half);
+            }
+        }
+    };
+    int h0 = blockIdx.y * blockDim.y + threadIdx.y;
+    fetch(h0);
     float c[8], w[8];
     if (turns) {
         const int64_t pos = rope_position(a.rope, b, s, s);
@@ -74,9 +94,9 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ skv
                 load8(cs, c);
                 load8(sn, w);
             } else {
-                const float4 u = *reinterpret_cast<const float4*>(cs), v = *reinterpret_cast<const float4*>(sn);
-                c[0] = u.x; c[1] = u.y; c[2] = u.z; c[3] = u.w;
-                w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+                const float4 x = *reinterpret_cast<const float4*>(cs), y = *reinterpret_cast<const float4*>(sn);
+                c[0] = x.x; c[1] = x.y; c[2] = x.z; c[3] = x.w;
+                w[0] = y.x; w[1] = y.y; w[2] = y.z; w[3] = y.w;
             }
             if (a.rope.inverse)
 #pragma unroll
@@ -86,49 +106,40 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ skv
             for (int i = 0; i < 8; ++i) c[i] = w[i] = __int_as_float(0x7fffffff);
         }
     }
-    const T* q = static_cast<const T*>(a.q.ptr) + b * a.q.stride_b + s * a.q.stride_s + d;
-    const T* k = static_cast<const T*>(a.k.ptr) + b * a.k.stride_b + s * a.k.stride_s + d;
-    T* qo = static_cast<T*>(a.q_out.ptr) + b * a.q_out.stride_b + s * a.q_out.stride_s + d;
-    T* ko = static_cast<T*>(a.k_out.ptr) + b * a.k_out.stride_b + s * a.k_out.stride_s + d;
-    const int H = a.q.heads + a.k.heads, step = blockDim.y * gridDim.y;
-    for (int h0 = blockIdx.y * blockDim.y + threadIdx.y; h0 < H; h0 += 2 * step) {
-        float x[2][8], y[2][8];
+    for (;;) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int h = h0 + i * step;
-            if (h < H) {
-                const T* p = h < a.q.heads ? q + h * a.q.stride_h : k + (h - a.q.heads) * a.k.stride_h;
-                load8(p, x[i]);
-                if (SPLIT && turns) load8(p + half, y[i]);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < FLY; ++i) {
             const int h = h0 + i * step;
             if (h >= H) break;
             T* p = h < a.q.heads ? qo + h * a.q_out.stride_h : ko + (h - a.q.heads) * a.k_out.stride_h;
+            float x[8];
+            u[i].get(x);
             if (turns) {
                 if constexpr (SPLIT) {
-                    float u[8];
+                    float y[8], z[8];
+                    v[i].get(y);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        u[e] = rope_first(x[i][e], y[i][e], c[e], w[e]);
-                        y[i][e] = rope_second(x[i][e], y[i][e], c[e], w[e]);
+                        z[e] = rope_first(x[e], y[e], c[e], w[e]);
+                        y[e] = rope_second(x[e], y[e], c[e], w[e]);
                     }
-                    store8(p, u);
-                    store8(p + half, y[i]);
+                    store8(p, z);
+                    store8(p + half, y);
                     continue;
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float u = rope_first(x[i][2 * e], x[i][2 * e + 1], c[e], w[e]);
-                        x[i][2 * e + 1] = rope_second(x[i][2 * e], x[i][2 * e + 1], c[e], w[e]);
-                        x[i][2 * e] = u;
+                        const float z = rope_first(x[2 * e], x[2 * e + 1], c[e], w[e]);
+                        x[2 * e + 1] = rope_second(x[2 * e], x[2 * e + 1], c[e], w[e]);
+                        x[2 * e] = z;
                     }
                 }
             }
-            store8(p, x[i]);
+            store8(p, x);
         }
+        h0 += FLY * step;
+        if (h0 >= H) break;
+        fetch(h0);
     }
 }
 
@@ -147,9 +158,10 @@ int launch_rotary(const skv_rotary_args& a, cudaStream_t st) {
     }
     const int turned = split ? a.rope.rot / 16 : a.rope.rot / 8;
     const int items = turned + (a.D - a.rope.rot) / 8;
-    // a block of up to 256 threads: the heads in as few equal steps as fit, then more tokens; heads over more blocks
-    // while there are too few tokens to fill the GPU
-    int steps = (H * items + 255) / 256;
+    // a block of up to 256 threads: a token's heads in as many steps as a thread has rows on the way (more where they do not
+    // fit), then more tokens; heads over more blocks while there are too few tokens to fill the GPU
+    constexpr int FLY = sizeof(T) == 2 ? 4 : 2;
+    int steps = H < FLY ? H : FLY;
     while ((H + steps - 1) / steps * items > 256) ++steps;
     int heads = (H + steps - 1) / steps;
     int slices = 1;
