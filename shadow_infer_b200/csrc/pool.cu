@@ -118,102 +118,126 @@ __global__ void __launch_bounds__(32 * kPoolWarps) pool_append_any_kernel(const 
     }
 }
 
-// 8 values a lane: blockDim = (lanes a row: a power of two >= D / 8, rows at a time, tokens at a time).  A thread keeps one
-// chunk of one token, reads its cos and sin and finds its page once, and walks the q, k and v heads with FLY rows on the way,
-// the first ones asked for before anything else.  Every thread stays to the end: rows and int4 groups reduce over aligned lane blocks.
+// 16 values a lane, two chunks of 8: where halves are paired (SPLIT) chunk i of each half of the turned part, then of the rest;
+// else 16 neighbours.  blockDim = (lanes a row: a power of two >= D / 16, rows at a time, tokens at a time).  A thread keeps its
+// chunks of one token, reads their cos and sin and finds the token's page once, and walks the q, k and v heads with FLY rows on
+// the way, the first ones asked for before anything else.  Every thread stays to the end: rows and int4 groups reduce
+// over aligned lane blocks.
 template <class T, bool SPLIT>
 __global__ void __launch_bounds__(256) pool_append_kernel(const __grid_constant__ skv_pool_append_args a) {
     constexpr int FLY = sizeof(T) == 2 ? 4 : 2;
-    const int D = a.pool.head_dim, Hk = a.pool.heads, Hq = a.q.heads, H = Hq + 2 * Hk, half = a.rope.rot / 2;
+    const int D = a.pool.head_dim, Hk = a.pool.heads, Hq = a.q.heads, H = Hq + 2 * Hk, rot = a.rope.rot, half = rot / 2;
     const int tokens = a.pool.batch * a.S, token = blockIdx.x * blockDim.z + threadIdx.z;
-    const int d = 8 * threadIdx.x;
-    const bool there = token < tokens && d < D;
+    const int i0 = threadIdx.x;
+    const bool there = token < tokens && 16 * i0 < D, paired = SPLIT && 16 * i0 < rot;
+    const int d0 = SPLIT ? (paired ? 8 * i0 : half + 8 * i0) : 16 * i0;   // copied chunks start at rot: lane rot / 16 is the first
+    const int d1 = SPLIT ? d0 + (paired ? half : (D - rot) / 2) : d0 + 8;
     const int b = there ? token / a.S : 0, s = there ? token - b * a.S : 0;
-    const bool turns = there && d < a.rope.rot, second = SPLIT && d >= half;
-    const int step = blockDim.y * gridDim.y, partner = SPLIT ? (second ? -half : half) : 0;
+    const int step = blockDim.y * gridDim.y;
     Raw8<T> u[FLY], v[FLY];
     auto fetch = [&](int h0) {
 #pragma unroll
         for (int i = 0; i < FLY; ++i) {
             const int h = h0 + threadIdx.y + i * step;
             if (there && h < H) {
-                const bool is_q = h < Hq, is_k = !is_q && h < Hq + Hk;
-                const skv_rows& in = is_q ? a.q : is_k ? a.k : a.v;
-                const T* x = static_cast<const T*>(in.ptr) + b * in.stride_b + (is_q ? h : is_k ? h - Hq : h - Hq - Hk) * in.stride_h +
-                             s * in.stride_s + d;
-                u[i].load(x);
-                if (SPLIT && turns && (is_q || is_k)) v[i].load(x + partner);
+                const skv_rows& in = h < Hq ? a.q : h < Hq + Hk ? a.k : a.v;
+                const T* x = static_cast<const T*>(in.ptr) + b * in.stride_b +
+                             (h < Hq ? h : h < Hq + Hk ? h - Hq : h - Hq - Hk) * in.stride_h + s * in.stride_s;
+                u[i].load(x + d0);
+                v[i].load(x + d1);
             }
         }
     };
     fetch(blockIdx.y * blockDim.y);
     const int64_t t = there ? (int64_t)a.lengths[b] + s : 0;
+    // cos and sin of 8 pairs: of both chunks (SPLIT), or 4 of each
     float c[8], w[8];
     bool known = true;
-    if (turns) {
+    const bool turn0 = there && d0 < rot, turn1 = there && d1 < rot;
+    if (turn0) {
         const int64_t pos = rope_position(a.rope, b, s, t);
         known = pos >= 0 && pos < a.rope.max_positions;
-        if (known) {
-            const float* cs = a.rope.cos + pos * half + (SPLIT ? d - (second ? half : 0) : d / 2);
-            const float* sn = a.rope.sin + pos * half + (SPLIT ? d - (second ? half : 0) : d / 2);
-            if constexpr (SPLIT) {
-                load8(cs, c);
-                load8(sn, w);
-            } else {
-                const float4 u = *reinterpret_cast<const float4*>(cs), v = *reinterpret_cast<const float4*>(sn);
-                c[0] = u.x; c[1] = u.y; c[2] = u.z; c[3] = u.w;
-                w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-            }
+        if (known && (SPLIT || turn1)) {
+            load8(a.rope.cos + pos * half + (SPLIT ? d0 : d0 / 2), c);
+            load8(a.rope.sin + pos * half + (SPLIT ? d0 : d0 / 2), w);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) c[i] = w[i] = __int_as_float(0x7fffffff);
+            for (int i = 0; i < 8; ++i) {
+                const bool have = known && i < 4;
+                c[i] = have ? a.rope.cos[pos * half + d0 / 2 + i] : __int_as_float(0x7fffffff);
+                w[i] = have ? a.rope.sin[pos * half + d0 / 2 + i] : __int_as_float(0x7fffffff);
+            }
         }
+        if (a.rope.inverse)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = -w[i];
     }
     const bool stored = there && (a.new_lengths == nullptr || s < a.new_lengths[b]);
     const int64_t row0 = stored ? pool_row(a.pool, b, t) : -1;
     if (stored && (row0 < 0 || !known) && a.error_flag) atomicExch(a.error_flag, 1);
-    // a key whose position is not known is not stored; its row's first lane speaks for the row
+    // a key whose position is not known is not stored: the row's first lane speaks for the row
     const bool key_known = __shfl_sync(0xffffffffu, (int)known, (threadIdx.y * blockDim.x + threadIdx.z * blockDim.x * blockDim.y) & 31);
-    const int p = a.pool.precision, lanes = p == 3 ? a.pool.int4_group / 8 : blockDim.x;
+    const int p = a.pool.precision, G = p == 3 ? a.pool.int4_group : 16;
     const int64_t row_bytes = pool_row_bytes(p, D);
     for (int h0 = blockIdx.y * blockDim.y; h0 < H;) {   // alike for all threads of the block
 #pragma unroll
         for (int i = 0; i < FLY; ++i) {
             const int h = h0 + threadIdx.y + i * step;
             const bool is_q = h < Hq, is_k = !is_q && h < Hq + Hk, here = there && h < H;
-            float y[8];
+            float x[8], y[8];   // the chunks
             if (here) {
-                u[i].get(y);
+                u[i].get(x);
+                v[i].get(y);
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = 0.0f;
+                for (int e = 0; e < 8; ++e) x[e] = y[e] = 0.0f;
             }
-            if (turns && here && (is_q || is_k)) {
+            if (is_q || is_k) {
                 if constexpr (SPLIT) {
-                    float o[8];
-                    v[i].get(o);
+                    if (turn0)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        y[e] = second ? rope_second(o[e], y[e], c[e], w[e]) : rope_first(y[e], o[e], c[e], w[e]);
+                        for (int e = 0; e < 8; ++e) {
+                            const float z = rope_first(x[e], y[e], c[e], w[e]);
+                            y[e] = rope_second(x[e], y[e], c[e], w[e]);
+                            x[e] = z;
+                        }
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float z = rope_first(y[2 * e], y[2 * e + 1], c[e], w[e]);
-                        y[2 * e + 1] = rope_second(y[2 * e], y[2 * e + 1], c[e], w[e]);
-                        y[2 * e] = z;
+                        if (turn0) {
+                            const float z = rope_first(x[2 * e], x[2 * e + 1], c[e], w[e]);
+                            x[2 * e + 1] = rope_second(x[2 * e], x[2 * e + 1], c[e], w[e]);
+                            x[2 * e] = z;
+                        }
+                        if (turn1) {
+                            const float z = rope_first(y[2 * e], y[2 * e + 1], c[4 + e], w[4 + e]);
+                            y[2 * e + 1] = rope_second(y[2 * e], y[2 * e + 1], c[4 + e], w[4 + e]);
+                            y[2 * e] = z;
+                        }
                     }
                 }
             }
-            float scale = 1.0f;
+            float m0 = 0.0f, m1 = 0.0f;
             if (p >= 2) {
-                float m = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(y[e]));
-                scale = quant_scale(group_max(m, lanes), p == 2 ? 127.0f : 7.0f);
+                for (int e = 0; e < 8; ++e) {
+                    m0 = fmaxf(m0, fabsf(x[e]));
+                    m1 = fmaxf(m1, fabsf(y[e]));
+                }
+                if (p == 2) {
+                    m0 = m1 = group_max(fmaxf(m0, m1), blockDim.x);
+                } else if (SPLIT) {           // a group is the same chunk of G / 8 lanes
+                    m0 = group_max(m0, G / 8);
+                    m1 = group_max(m1, G / 8);
+                } else if (G > 8) {           // both chunks of G / 16 lanes
+                    m0 = m1 = group_max(fmaxf(m0, m1), G / 16);
+                }
             }
             if (!here) continue;
             if (is_q) {
-                store8(static_cast<T*>(a.q_out.ptr) + b * a.q_out.stride_b + h * a.q_out.stride_h + s * a.q_out.stride_s + d, y);
+                T* to = static_cast<T*>(a.q_out.ptr) + b * a.q_out.stride_b + h * a.q_out.stride_h + s * a.q_out.stride_s;
+                store8(to + d0, x);
+                store8(to + d1, y);
                 continue;
             }
             if (row0 < 0 || (is_k && !key_known)) continue;
@@ -221,24 +245,34 @@ __global__ void __launch_bounds__(256) pool_append_kernel(const __grid_constant_
             uint8_t* to = static_cast<uint8_t*>(is_k ? a.pool.k : a.pool.v) + row * row_bytes;
             float* sc = is_k ? a.pool.scale_k : a.pool.scale_v;
             if (p == 0) {
-                store8(reinterpret_cast<float*>(to) + d, y);
+                store8(reinterpret_cast<float*>(to) + d0, x);
+                store8(reinterpret_cast<float*>(to) + d1, y);
             } else if (p == 1) {
-                store8(reinterpret_cast<__half*>(to) + d, y);
+                store8(reinterpret_cast<__half*>(to) + d0, x);
+                store8(reinterpret_cast<__half*>(to) + d1, y);
             } else {
-                const float rcp = __frcp_rn(scale);
-                uint32_t n[2] = {0, 0};
+                int q[8];
+                float f[8];
+                const float s0 = quant_scale(m0, p == 2 ? 127.0f : 7.0f), s1 = m1 == m0 ? s0 : quant_scale(m1, p == 2 ? 127.0f : 7.0f);
+                const float r0 = __frcp_rn(s0), r1 = __frcp_rn(s1);
                 if (p == 2) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        n[e / 4] |= (uint32_t)(quant_value_fast(y[e], scale, rcp, -128, 127) & 0xFF) << (8 * (e & 3));
-                    *reinterpret_cast<uint2*>(to + d) = make_uint2(n[0], n[1]);
-                    if (d == 0) sc[row] = scale;
+                    quant_values<0>(x, s0, r0, -128, 127, q, f);
+                    *reinterpret_cast<uint2*>(to + d0) = make_uint2(pack_s8(q[1], q[0], pack_s8(q[3], q[2], 0u)),
+                                                                    pack_s8(q[5], q[4], pack_s8(q[7], q[6], 0u)));
+                    quant_values<0>(y, s0, r0, -128, 127, q, f);
+                    *reinterpret_cast<uint2*>(to + d1) = make_uint2(pack_s8(q[1], q[0], pack_s8(q[3], q[2], 0u)),
+                                                                    pack_s8(q[5], q[4], pack_s8(q[7], q[6], 0u)));
+                    if (i0 == 0) sc[row] = s0;
                 } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        n[0] |= ((uint32_t)(quant_value_fast(y[e], scale, rcp, -8, 7) + 8) & 15u) << (8 * (e / 2) + (e & 1 ? 0 : 4));
-                    *reinterpret_cast<uint32_t*>(to + d / 2) = n[0];
-                    if (d % a.pool.int4_group == 0) sc[row * (D / a.pool.int4_group) + d / a.pool.int4_group] = scale;
+                    quant_values<8>(x, s0, r0, -8, 7, q, f);
+                    *reinterpret_cast<uint32_t*>(to + d0 / 2) =
+                        pack_u4(q[0], q[1], pack_u4(q[2], q[3], pack_u4(q[4], q[5], pack_u4(q[6], q[7], 0u))));
+                    quant_values<8>(y, s1, r1, -8, 7, q, f);
+                    *reinterpret_cast<uint32_t*>(to + d1 / 2) =
+                        pack_u4(q[0], q[1], pack_u4(q[2], q[3], pack_u4(q[4], q[5], pack_u4(q[6], q[7], 0u))));
+                    float* g = sc + row * (D / G);
+                    if (d0 % G == 0) g[d0 / G] = s0;
+                    if (d1 % G == 0) g[d1 / G] = s1;
                 }
             }
         }
@@ -327,19 +361,21 @@ template <class T>
 int launch_append(const skv_pool_append_args& a, cudaStream_t st) {
     const int D = a.pool.head_dim, H = a.q.heads + 2 * a.pool.heads;
     const int64_t tokens = (int64_t)a.pool.batch * a.S;
-    const bool split = !a.rope.interleaved;
-    const int lanes4 = a.pool.precision == 3 ? a.pool.int4_group / 8 : 1;   // of an int4 group
-    const bool vec = D % 8 == 0 && D <= 256 && a.rope.rot % (split ? 16 : 8) == 0 && rows_aligned(a.q) && rows_aligned(a.k) &&
-                     rows_aligned(a.v) && rows_aligned(a.q_out) && aligned16(a.pool.k) && aligned16(a.pool.v) &&
-                     aligned16(a.rope.cos) && aligned16(a.rope.sin) &&
-                     (a.pool.precision != 3 || (a.pool.int4_group % 8 == 0 && (lanes4 & (lanes4 - 1)) == 0));
+    // halves are paired only where something turns that way; int4 groups must be whole lane blocks of a chunk then
+    const int rot = a.rope.rot, G = a.pool.precision == 3 ? a.pool.int4_group : 16;
+    const bool split = rot > 0 && !a.rope.interleaved;
+    const auto power = [](int n) { return n > 0 && (n & (n - 1)) == 0; };
+    bool vec = D % 16 == 0 && D <= 512 && rows_aligned(a.q) && rows_aligned(a.k) && rows_aligned(a.v) && rows_aligned(a.q_out) &&
+               aligned16(a.pool.k) && aligned16(a.pool.v) && aligned16(a.rope.cos) && aligned16(a.rope.sin);
+    if (split) vec = vec && rot % 16 == 0 && (a.pool.precision != 3 || (G % 8 == 0 && power(G / 8) && rot / 2 % G == 0 && (D - rot) / 2 % G == 0));
+    else vec = vec && rot % 8 == 0 && (a.pool.precision != 3 || G == 8 || (G % 16 == 0 && power(G / 16)));
     if (!vec) {
         const int64_t blocks = (tokens * H + kPoolWarps - 1) / kPoolWarps;
         pool_append_any_kernel<T><<<(unsigned)blocks, 32 * kPoolWarps, 0, st>>>(a);
         return check_launch("pool_append");
     }
     int lanes = 1;
-    while (lanes * 8 < D) lanes *= 2;
+    while (lanes * 16 < D) lanes *= 2;
     // a token's rows in one pass of FLY rows a thread where up to 256 threads hold them; rows over more blocks while there are
     // too few tokens to fill the GPU; whole warps
     constexpr int FLY = sizeof(T) == 2 ? 4 : 2;
