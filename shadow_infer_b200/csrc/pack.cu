@@ -101,6 +101,58 @@ __device__ __forceinline__ void stage_put(float4* stage, int r, int l, const flo
         stage[r * CPR + stage_chunk(4 * l + j)] = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
 }
 
+// d = (c << 16) | (sat_s8(a) << 8) | sat_s8(b)
+__device__ __forceinline__ uint32_t pack_s8(int a, int b, uint32_t c) {
+    uint32_t d;
+    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+// d = (c << 8) | (sat_u4(a) << 4) | sat_u4(b)
+__device__ __forceinline__ uint32_t pack_u4(int a, int b, uint32_t c) {
+    uint32_t d;
+    asm("cvt.pack.sat.u4.s32.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+
+constexpr float kRoundMagic = 12582912.0f;   // 1.5 * 2^23: adding it rounds |y| < 2^22 to an integer
+
+// max that propagates NaN (so a NaN deviation still sends the values to the exact path)
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+// q[i] = clamp(rint(fl(x[i] / s)), lo, hi) + OFF for 16 values; qf[i] = the rounded value without
+// OFF.  OFF (8 for int4 nibbles) rides in the rounding constant: the integer part of
+// y + 1.5*2^23 + OFF is rint(y) + OFF.  Values are rounded from the exact product y = x * rcp(s)
+// (one fma with the constant), and the deviation y - rint(y) comes from a second fma; if any value
+// lies within 1e-4 of a half-integer (or is not finite) all 16 take the exact IEEE division.  Away
+// from ties rint(x * rcp(s)) == rint(fl(x / s)): the two differ by far less than 1e-4 for the
+// |q| <= 128 range.  Out-of-range codes are clamped by the saturating packs that consume q.
+template <int OFF>
+__device__ __forceinline__ void quant16(const float (&x)[16], float s, float r, int lo, int hi, int (&q)[16],
+                                        float (&qf)[16]) {
+    constexpr float kM = kRoundMagic + (float)OFF;
+    float dev = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float t = __fmaf_rn(x[i], r, kM);
+        const float rf = __fsub_rn(t, kM);
+        dev = max_nan(dev, fabsf(__fmaf_rn(x[i], r, -rf)));
+        q[i] = __float_as_int(t) - 0x4B400000;
+        qf[i] = rf;
+    }
+    if (!(dev < 0.4999f)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int v = quant_value(x[i], s, lo, hi);
+            q[i] = v + OFF;
+            qf[i] = (float)v;
+        }
+    }
+}
+
 // ---------------------------------------------------------------------------------------
 // pack
 // ---------------------------------------------------------------------------------------
@@ -138,7 +190,7 @@ __device__ __forceinline__ void pack_lane(const float (&x)[16], int code, int64_
         const float r = __frcp_rn(s);
         int q[16];
         if (i4) {
-            quant_values<8>(x, s, r, -8, 7, q, dense);         // q = code + 8, the stored nibble
+            quant16<8>(x, s, r, -8, 7, q, dense);         // q = code + 8, the stored nibble
             uint32_t w[2];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -153,7 +205,7 @@ __device__ __forceinline__ void pack_lane(const float (&x)[16], int code, int64_
             const int lpg = G >> 4;   // lanes per int4 group
             if ((l & (lpg - 1)) == 0) scale[row * (D / G) + (l * 16) / G] = s;
         } else {
-            quant_values<0>(x, s, r, -128, 127, q, dense);
+            quant16<0>(x, s, r, -128, 127, q, dense);
             uint32_t w[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) w[k] = pack_s8(q[4 * k + 1], q[4 * k], pack_s8(q[4 * k + 3], q[4 * k + 2], 0u));

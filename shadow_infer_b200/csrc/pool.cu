@@ -118,37 +118,72 @@ __global__ void __launch_bounds__(32 * kPoolWarps) pool_append_any_kernel(const 
     }
 }
 
-// 16 values a lane, two chunks of 8: where halves are paired (SPLIT) chunk i of each half of the turned part, then of the rest;
-// else 16 neighbours.  blockDim = (lanes a row: a power of two >= D / 16, rows at a time, tokens at a time).  A thread keeps its
-// chunks of one token, reads their cos and sin and finds the token's page once, and walks the q, k and v heads with FLY rows on
-// the way, the first ones asked for before anything else.  Every thread stays to the end: rows and int4 groups reduce
-// over aligned lane blocks.
-template <class T, bool SPLIT>
-__global__ void __launch_bounds__(256) pool_append_kernel(const __grid_constant__ skv_pool_append_args a) {
-    constexpr int FLY = sizeof(T) == 2 ? 4 : 2;
-    const int D = a.pool.head_dim, Hk = a.pool.heads, Hq = a.q.heads, H = Hq + 2 * Hk, rot = a.rope.rot, half = rot / 2;
-    const int tokens = a.pool.batch * a.S, token = blockIdx.x * blockDim.z + threadIdx.z;
-    const int i0 = threadIdx.x;
-    const bool there = token < tokens && 16 * i0 < D, paired = SPLIT && 16 * i0 < rot;
-    const int d0 = SPLIT ? (paired ? 8 * i0 : half + 8 * i0) : 16 * i0;   // copied chunks start at rot: lane rot / 16 is the first
-    const int d1 = SPLIT ? d0 + (paired ? half : (D - rot) / 2) : d0 + 8;
-    const int b = there ? token / a.S : 0, s = there ? token - b * a.S : 0;
-    const int step = blockDim.y * gridDim.y;
-    Raw8<T> u[FLY], v[FLY];
-    auto fetch = [&](int h0) {
+constexpr float kRoundMagic = 12582912.0f;   // 1.5 2^23: x + this has rint(x) in its low bits for |x| < 2^22
+
+// max that keeps a NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+// t[e] = 1.5 2^23 + add + rint(fl(x[e] / s)), whose low byte is the integer (+ add) that is stored.  r is the correctly
+// rounded 1 / s; then q + r (x - q s), the residual by one fma, is the correctly rounded quotient (Markstein's correction,
+// IBM J. Res. Dev. 34, 1990), so the integers are those of a division at a third of its instructions.  `odd`: the
+// row's values or its scale leave that theorem's range (NaN, infinities, scales near the ends of fp32); then the division is
+// made.
+__device__ __forceinline__ void quotients(const float (&x)[8], float s, float r, bool odd, int lo, int hi, float add, float (&t)[8]) {
 #pragma unroll
-        for (int i = 0; i < FLY; ++i) {
-            const int h = h0 + threadIdx.y + i * step;
-            if (there && h < H) {
-                const skv_rows& in = h < Hq ? a.q : h < Hq + Hk ? a.k : a.v;
-                const T* x = static_cast<const T*>(in.ptr) + b * in.stride_b +
-                             (h < Hq ? h : h < Hq + Hk ? h - Hq : h - Hq - Hk) * in.stride_h + s * in.stride_s;
-                u[i].load(x + d0);
-                v[i].load(x + d1);
-            }
+    for (int e = 0; e < 8; ++e) {
+        const float q = __fmul_rn(x[e], r);
+        t[e] = __fadd_rn(__fmaf_rn(__fmaf_rn(-q, s, x[e]), r, q), kRoundMagic + add);
+    }
+    if (__builtin_expect(odd, 0)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] = (kRoundMagic + add) + (float)quant_value(x[e], s, lo, hi);
+    }
+}
+// The low bytes of four of them.
+__device__ __forceinline__ uint32_t low_bytes(float a, float b, float c, float d) {
+    return __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040), __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040),
+                       0x5410);
+}
+
+// Division of a non-negative m by 7 or 127 (r: its correctly rounded reciprocal), as quant_scale.
+__device__ __forceinline__ float scale_of(float m, float top, float r) {
+    const float q = __fmul_rn(m, r), s = __fmaf_rn(__fmaf_rn(-q, top, m), r, q);
+    return m > 1e-30f && m < 1e30f ? s : quant_scale(m, top);
+}
+
+// 16 values a lane, two chunks of 8: where halves are paired (SPLIT) chunk i of each half of the turned part, then of the rest;
+// else 16 neighbours.  blockDim = (lanes a row: a power of two >= D / 16, rows at a time, tokens at a time); a block takes
+// FLY * rows heads of q, of k or of v (blockIdx.y: first the slices of q, then of k, then of v), every row asked for before the
+// token's position and page are known.  Every thread stays to the end: rows and int4 groups reduce over aligned lane blocks.
+template <class T, bool SPLIT>
+__global__ void __launch_bounds__(256) pool_append_kernel(const __grid_constant__ skv_pool_append_args a, int q_slices, int kv_slices) {
+    constexpr int FLY = sizeof(T) == 2 ? 4 : 2;
+    const int D = a.pool.head_dim, half = a.rope.rot / 2, i0 = threadIdx.x;
+    const int slice = blockIdx.y, kind = slice < q_slices ? 0 : slice < q_slices + kv_slices ? 1 : 2;   // q, k, v
+    const int rot = kind == 2 ? 0 : a.rope.rot, H = kind == 0 ? a.q.heads : a.pool.heads;
+    const int h0 = (kind == 0 ? slice : kind == 1 ? slice - q_slices : slice - q_slices - kv_slices) * FLY * blockDim.y + threadIdx.y;
+    const int tokens = a.pool.batch * a.S, token = blockIdx.x * blockDim.z + threadIdx.z;
+    const bool there = token < tokens && 16 * i0 < D;
+    const int b = there ? token / a.S : 0, s = there ? token - b * a.S : 0;
+    const bool paired = SPLIT && 16 * i0 < a.rope.rot;
+    const int d0 = SPLIT ? (paired ? 8 * i0 : half + 8 * i0) : 16 * i0;   // copied chunks start at rot: lane rot / 16 is the first
+    const int d1 = SPLIT ? d0 + (paired ? half : (D - a.rope.rot) / 2) : d0 + 8;
+    const skv_rows& in = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+    const T* from = static_cast<const T*>(in.ptr) + b * in.stride_b + s * in.stride_s;
+    const int64_t stride_h = in.stride_h;
+    Raw8<T> u[FLY], v[FLY];
+#pragma unroll
+    for (int i = 0; i < FLY; ++i) {
+        const int h = h0 + i * blockDim.y;
+        if (there && h < H) {
+            u[i].load(from + h * stride_h + d0);
+            v[i].load(from + h * stride_h + d1);
         }
-    };
-    fetch(blockIdx.y * blockDim.y);
+    }
     const int64_t t = there ? (int64_t)a.lengths[b] + s : 0;
     // cos and sin of 8 pairs: of both chunks (SPLIT), or 4 of each
     float c[8], w[8];
@@ -172,112 +207,116 @@ __global__ void __launch_bounds__(256) pool_append_kernel(const __grid_constant_
 #pragma unroll
             for (int i = 0; i < 8; ++i) w[i] = -w[i];
     }
-    const bool stored = there && (a.new_lengths == nullptr || s < a.new_lengths[b]);
+    const bool stored = kind != 0 && there && (a.new_lengths == nullptr || s < a.new_lengths[b]);
     const int64_t row0 = stored ? pool_row(a.pool, b, t) : -1;
     if (stored && (row0 < 0 || !known) && a.error_flag) atomicExch(a.error_flag, 1);
     // a key whose position is not known is not stored: the row's first lane speaks for the row
-    const bool key_known = __shfl_sync(0xffffffffu, (int)known, (threadIdx.y * blockDim.x + threadIdx.z * blockDim.x * blockDim.y) & 31);
-    const int p = a.pool.precision, G = p == 3 ? a.pool.int4_group : 16;
-    const int64_t row_bytes = pool_row_bytes(p, D);
-    for (int h0 = blockIdx.y * blockDim.y; h0 < H;) {   // alike for all threads of the block
+    const bool ok = __shfl_sync(0xffffffffu, (int)known, (threadIdx.y * blockDim.x + threadIdx.z * blockDim.x * blockDim.y) & 31);
+    const int p = kind == 0 ? 0 : a.pool.precision, G = p == 3 ? a.pool.int4_group : 16;
+    const int row_bytes = (int)pool_row_bytes(p, D), groups = D / G;
+    uint8_t* to = static_cast<uint8_t*>(kind == 1 ? a.pool.k : a.pool.v) + row0 * row_bytes;
+    float* sc = (kind == 1 ? a.pool.scale_k : a.pool.scale_v) + row0 * (p == 3 ? groups : 1);
+    T* q_to = static_cast<T*>(a.q_out.ptr) + b * a.q_out.stride_b + s * a.q_out.stride_s;
 #pragma unroll
-        for (int i = 0; i < FLY; ++i) {
-            const int h = h0 + threadIdx.y + i * step;
-            const bool is_q = h < Hq, is_k = !is_q && h < Hq + Hk, here = there && h < H;
-            float x[8], y[8];   // the chunks
-            if (here) {
-                u[i].get(x);
-                v[i].get(y);
-            } else {
+    for (int i = 0; i < FLY; ++i) {
+        const int h = h0 + i * blockDim.y;
+        const bool here = there && h < H;
+        float x[8], y[8];   // the chunks
+        if (here) {
+            u[i].get(x);
+            v[i].get(y);
+        } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = y[e] = 0.0f;
-            }
-            if (is_q || is_k) {
-                if constexpr (SPLIT) {
-                    if (turn0)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const float z = rope_first(x[e], y[e], c[e], w[e]);
-                            y[e] = rope_second(x[e], y[e], c[e], w[e]);
-                            x[e] = z;
-                        }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (turn0) {
-                            const float z = rope_first(x[2 * e], x[2 * e + 1], c[e], w[e]);
-                            x[2 * e + 1] = rope_second(x[2 * e], x[2 * e + 1], c[e], w[e]);
-                            x[2 * e] = z;
-                        }
-                        if (turn1) {
-                            const float z = rope_first(y[2 * e], y[2 * e + 1], c[4 + e], w[4 + e]);
-                            y[2 * e + 1] = rope_second(y[2 * e], y[2 * e + 1], c[4 + e], w[4 + e]);
-                            y[2 * e] = z;
-                        }
-                    }
-                }
-            }
-            float m0 = 0.0f, m1 = 0.0f;
-            if (p >= 2) {
+            for (int e = 0; e < 8; ++e) x[e] = y[e] = 0.0f;
+        }
+        if constexpr (SPLIT) {
+            if (turn0)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    m0 = fmaxf(m0, fabsf(x[e]));
-                    m1 = fmaxf(m1, fabsf(y[e]));
+                    const float z = rope_first(x[e], y[e], c[e], w[e]);
+                    y[e] = rope_second(x[e], y[e], c[e], w[e]);
+                    x[e] = z;
                 }
-                if (p == 2) {
-                    m0 = m1 = group_max(fmaxf(m0, m1), blockDim.x);
-                } else if (SPLIT) {           // a group is the same chunk of G / 8 lanes
-                    m0 = group_max(m0, G / 8);
-                    m1 = group_max(m1, G / 8);
-                } else if (G > 8) {           // both chunks of G / 16 lanes
-                    m0 = m1 = group_max(fmaxf(m0, m1), G / 16);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (turn0) {
+                    const float z = rope_first(x[2 * e], x[2 * e + 1], c[e], w[e]);
+                    x[2 * e + 1] = rope_second(x[2 * e], x[2 * e + 1], c[e], w[e]);
+                    x[2 * e] = z;
                 }
-            }
-            if (!here) continue;
-            if (is_q) {
-                T* to = static_cast<T*>(a.q_out.ptr) + b * a.q_out.stride_b + h * a.q_out.stride_h + s * a.q_out.stride_s;
-                store8(to + d0, x);
-                store8(to + d1, y);
-                continue;
-            }
-            if (row0 < 0 || (is_k && !key_known)) continue;
-            const int64_t row = row0 + (int64_t)(is_k ? h - Hq : h - Hq - Hk) * a.pool.page_size;
-            uint8_t* to = static_cast<uint8_t*>(is_k ? a.pool.k : a.pool.v) + row * row_bytes;
-            float* sc = is_k ? a.pool.scale_k : a.pool.scale_v;
-            if (p == 0) {
-                store8(reinterpret_cast<float*>(to) + d0, x);
-                store8(reinterpret_cast<float*>(to) + d1, y);
-            } else if (p == 1) {
-                store8(reinterpret_cast<__half*>(to) + d0, x);
-                store8(reinterpret_cast<__half*>(to) + d1, y);
-            } else {
-                int q[8];
-                float f[8];
-                const float s0 = quant_scale(m0, p == 2 ? 127.0f : 7.0f), s1 = m1 == m0 ? s0 : quant_scale(m1, p == 2 ? 127.0f : 7.0f);
-                const float r0 = __frcp_rn(s0), r1 = __frcp_rn(s1);
-                if (p == 2) {
-                    quant_values<0>(x, s0, r0, -128, 127, q, f);
-                    *reinterpret_cast<uint2*>(to + d0) = make_uint2(pack_s8(q[1], q[0], pack_s8(q[3], q[2], 0u)),
-                                                                    pack_s8(q[5], q[4], pack_s8(q[7], q[6], 0u)));
-                    quant_values<0>(y, s0, r0, -128, 127, q, f);
-                    *reinterpret_cast<uint2*>(to + d1) = make_uint2(pack_s8(q[1], q[0], pack_s8(q[3], q[2], 0u)),
-                                                                    pack_s8(q[5], q[4], pack_s8(q[7], q[6], 0u)));
-                    if (i0 == 0) sc[row] = s0;
-                } else {
-                    quant_values<8>(x, s0, r0, -8, 7, q, f);
-                    *reinterpret_cast<uint32_t*>(to + d0 / 2) =
-                        pack_u4(q[0], q[1], pack_u4(q[2], q[3], pack_u4(q[4], q[5], pack_u4(q[6], q[7], 0u))));
-                    quant_values<8>(y, s1, r1, -8, 7, q, f);
-                    *reinterpret_cast<uint32_t*>(to + d1 / 2) =
-                        pack_u4(q[0], q[1], pack_u4(q[2], q[3], pack_u4(q[4], q[5], pack_u4(q[6], q[7], 0u))));
-                    float* g = sc + row * (D / G);
-                    if (d0 % G == 0) g[d0 / G] = s0;
-                    if (d1 % G == 0) g[d1 / G] = s1;
+                if (turn1) {
+                    const float z = rope_first(y[2 * e], y[2 * e + 1], c[4 + e], w[4 + e]);
+                    y[2 * e + 1] = rope_second(y[2 * e], y[2 * e + 1], c[4 + e], w[4 + e]);
+                    y[2 * e] = z;
                 }
             }
         }
-        h0 += FLY * step;
-        if (h0 < H) fetch(h0);
+        if (kind == 0) {
+            if (here) {
+                store8(q_to + h * a.q_out.stride_h + d0, x);
+                store8(q_to + h * a.q_out.stride_h + d1, y);
+            }
+            continue;
+        }
+        const int64_t off = (int64_t)h * a.pool.page_size;
+        const bool write = here && row0 >= 0 && ok;
+        if (p < 2) {
+            if (!write) continue;
+            if (p == 0) {
+                store8(reinterpret_cast<float*>(to + off * row_bytes) + d0, x);
+                store8(reinterpret_cast<float*>(to + off * row_bytes) + d1, y);
+            } else {
+                store8(reinterpret_cast<__half*>(to + off * row_bytes) + d0, x);
+                store8(reinterpret_cast<__half*>(to + off * row_bytes) + d1, y);
+            }
+            continue;
+        }
+        float m0 = 0.0f, m1 = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            m0 = max_nan(m0, fabsf(x[e]));
+            m1 = max_nan(m1, fabsf(y[e]));
+        }
+        const bool nan = m0 != m0 || m1 != m1;
+        if (__any_sync(0xffffffffu, nan)) {   // a NaN does not count for its row's scale
+            m0 = m1 = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                m0 = fmaxf(m0, fabsf(x[e]));
+                m1 = fmaxf(m1, fabsf(y[e]));
+            }
+        }
+        float f[8], g[8];
+        if (p == 2) {
+            const float m = group_max(fmaxf(m0, m1), blockDim.x);
+            if (!write) continue;
+            const float scale = scale_of(m, 127.0f, 1.0f / 127.0f), rcp = __frcp_rn(scale);
+            const bool odd = nan || !(scale > 1e-30f && scale < 1e30f);
+            quotients(x, scale, rcp, odd, -128, 127, 0.0f, f);
+            quotients(y, scale, rcp, odd, -128, 127, 0.0f, g);
+            uint8_t* dst = to + off * row_bytes;
+            *reinterpret_cast<uint2*>(dst + d0) = make_uint2(low_bytes(f[0], f[1], f[2], f[3]), low_bytes(f[4], f[5], f[6], f[7]));
+            *reinterpret_cast<uint2*>(dst + d1) = make_uint2(low_bytes(g[0], g[1], g[2], g[3]), low_bytes(g[4], g[5], g[6], g[7]));
+            if (i0 == 0) sc[off] = scale;
+        } else {
+            if (SPLIT) {           // a group is the same chunk of G / 8 lanes
+                m0 = group_max(m0, G / 8);
+                m1 = group_max(m1, G / 8);
+            } else if (G > 8) {    // both chunks of G / 16 lanes
+                m0 = m1 = group_max(fmaxf(m0, m1), G / 16);
+            }
+            if (!write) continue;
+            const float s0 = scale_of(m0, 7.0f, 1.0f / 7.0f), s1 = scale_of(m1, 7.0f, 1.0f / 7.0f);
+            const bool odd = nan || !(fminf(s0, s1) > 1e-30f && fmaxf(s0, s1) < 1e30f);
+            quotients(x, s0, __frcp_rn(s0), odd, -8, 7, 8.0f, f);
+            quotients(y, s1, __frcp_rn(s1), odd, -8, 7, 8.0f, g);
+            uint8_t* dst = to + off * row_bytes;
+            *reinterpret_cast<uint32_t*>(dst + d0 / 2) = low_bytes(f[0], f[2], f[4], f[6]) << 4 | low_bytes(f[1], f[3], f[5], f[7]);
+            *reinterpret_cast<uint32_t*>(dst + d1 / 2) = low_bytes(g[0], g[2], g[4], g[6]) << 4 | low_bytes(g[1], g[3], g[5], g[7]);
+            if (d0 % G == 0) sc[off * groups + d0 / G] = s0;
+            if (d1 % G == 0) sc[off * groups + d1 / G] = s1;
+        }
     }
 }
 
@@ -374,22 +413,18 @@ int launch_append(const skv_pool_append_args& a, cudaStream_t st) {
         pool_append_any_kernel<T><<<(unsigned)blocks, 32 * kPoolWarps, 0, st>>>(a);
         return check_launch("pool_append");
     }
-    int lanes = 1;
-    while (lanes * 16 < D) lanes *= 2;
-    // a token's rows in one pass of FLY rows a thread where up to 256 threads hold them; rows over more blocks while there are
-    // too few tokens to fill the GPU; whole warps
+    // a block takes FLY rows a thread of a token's heads of one kind, or one row a thread while there are too few tokens to
+    // fill the GPU; the rest of 256 threads takes other tokens
     constexpr int FLY = sizeof(T) == 2 ? 4 : 2;
-    const int fit = 256 / lanes, whole = 32 / lanes > 1 ? 32 / lanes : 1;
-    int rows = (H + FLY - 1) / FLY < fit ? (H + FLY - 1) / FLY : fit, slices = 1, z = 1;
-    while (rows > whole && tokens * slices < 2 * sm_count()) {
-        slices *= 2;
-        rows = (rows + 1) / 2;
-    }
-    rows = (rows + whole - 1) / whole * whole;
-    while (z * 2 * rows <= fit && tokens * slices >= 8ll * sm_count() * z) z *= 2;
-    const dim3 block(lanes, rows, z), grid((unsigned)((tokens + z - 1) / z), slices);
-    if (split) pool_append_kernel<T, true><<<grid, block, 0, st>>>(a);
-    else pool_append_kernel<T, false><<<grid, block, 0, st>>>(a);
+    int lanes = 1, rows = 1, z = 1;
+    while (lanes * 16 < D) lanes *= 2;
+    const int want = tokens * (a.q.heads + 2 * a.pool.heads) * lanes < 256ll * 2 * sm_count() ? a.pool.heads : (a.pool.heads + FLY - 1) / FLY;
+    while (rows < want && lanes * rows < 256) rows *= 2;
+    while (lanes * rows * z < 32 || (lanes * rows * z * 2 <= 256 && tokens >= 8ll * sm_count() * z)) z *= 2;
+    const int q_slices = (a.q.heads + rows * FLY - 1) / (rows * FLY), kv_slices = (a.pool.heads + rows * FLY - 1) / (rows * FLY);
+    const dim3 block(lanes, rows, z), grid((unsigned)((tokens + z - 1) / z), q_slices + 2 * kv_slices);
+    if (split) pool_append_kernel<T, true><<<grid, block, 0, st>>>(a, q_slices, kv_slices);
+    else pool_append_kernel<T, false><<<grid, block, 0, st>>>(a, q_slices, kv_slices);
     return check_launch("pool_append");
 }
 

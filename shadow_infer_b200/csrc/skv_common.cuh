@@ -121,58 +121,6 @@ __device__ __forceinline__ int quant_value_fast(float x, float scale, float rcp,
     return (int)q;
 }
 
-// d = (c << 16) | (sat_s8(a) << 8) | sat_s8(b)
-__device__ __forceinline__ uint32_t pack_s8(int a, int b, uint32_t c) {
-    uint32_t d;
-    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-    return d;
-}
-// d = (c << 8) | (sat_u4(a) << 4) | sat_u4(b)
-__device__ __forceinline__ uint32_t pack_u4(int a, int b, uint32_t c) {
-    uint32_t d;
-    asm("cvt.pack.sat.u4.s32.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-    return d;
-}
-
-constexpr float kRoundMagic = 12582912.0f;   // 1.5 * 2^23: adding it rounds |y| < 2^22 to an integer
-
-// max that propagates NaN (so a NaN deviation still sends the values to the exact path)
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
-}
-
-// q[i] = clamp(rint(fl(x[i] / s)), lo, hi) + OFF for N values; qf[i] = the rounded value without
-// OFF.  OFF (8 for int4 nibbles) rides in the rounding constant: the integer part of
-// y + 1.5*2^23 + OFF is rint(y) + OFF.  Values are rounded from the exact product y = x * rcp(s)
-// (one fma with the constant), and the deviation y - rint(y) comes from a second fma; if any value
-// lies within 1e-4 of a half-integer (or is not finite) all N take the exact IEEE division.  Away
-// from ties rint(x * rcp(s)) == rint(fl(x / s)): the two differ by far less than 1e-4 for the
-// |q| <= 128 range.  Out-of-range codes are clamped by the saturating packs that consume q.
-template <int OFF, int N>
-__device__ __forceinline__ void quant_values(const float (&x)[N], float s, float r, int lo, int hi, int (&q)[N],
-                                             float (&qf)[N]) {
-    constexpr float kM = kRoundMagic + (float)OFF;
-    float dev = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const float t = __fmaf_rn(x[i], r, kM);
-        const float rf = __fsub_rn(t, kM);
-        dev = max_nan(dev, fabsf(__fmaf_rn(x[i], r, -rf)));
-        q[i] = __float_as_int(t) - 0x4B400000;
-        qf[i] = rf;
-    }
-    if (!(dev < 0.4999f)) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int v = quant_value(x[i], s, lo, hi);
-            q[i] = v + OFF;
-            qf[i] = (float)v;
-        }
-    }
-}
-
 // Copies `bytes` bytes with a warp, using 16-byte vectors when both ends allow.
 __device__ __forceinline__ void warp_copy(void* dst, const void* src, int64_t bytes, int lane) {
     const uintptr_t a = reinterpret_cast<uintptr_t>(dst) | reinterpret_cast<uintptr_t>(src);
