@@ -160,7 +160,7 @@ __device__ __forceinline__ float scale_of(float m, float top, float r) {
 // FLY * rows heads of q, of k or of v (blockIdx.y: first the slices of q, then of k, then of v), every row asked for before the
 // token's position and page are known.  Every thread stays to the end: rows and int4 groups reduce over aligned lane blocks.
 template <class T, bool SPLIT>
-__global__ void __launch_bounds__(256) pool_append_kernel(const __grid_constant__ skv_pool_append_args a, int q_slices, int kv_slices) {
+__global__ void __launch_bounds__(256, 3) pool_append_kernel(const __grid_constant__ skv_pool_append_args a, int q_slices, int kv_slices) {
     constexpr int FLY = sizeof(T) == 2 ? 4 : 2;
     const int D = a.pool.head_dim, half = a.rope.rot / 2, i0 = threadIdx.x;
     const int slice = blockIdx.y, kind = slice < q_slices ? 0 : slice < q_slices + kv_slices ? 1 : 2;   // q, k, v
@@ -211,6 +211,7 @@ __global__ void __launch_bounds__(256) pool_append_kernel(const __grid_constant_
     const int64_t row0 = stored ? pool_row(a.pool, b, t) : -1;
     if (stored && (row0 < 0 || !known) && a.error_flag) atomicExch(a.error_flag, 1);
     // a key whose position is not known is not stored: the row's first lane speaks for the row
+    if (kind != 0 && !__any_sync(0xffffffffu, row0 >= 0)) return;   // padding of a ragged prompt
     const bool ok = __shfl_sync(0xffffffffu, (int)known, (threadIdx.y * blockDim.x + threadIdx.z * blockDim.x * blockDim.y) & 31);
     const int p = kind == 0 ? 0 : a.pool.precision, G = p == 3 ? a.pool.int4_group : 16;
     const int row_bytes = (int)pool_row_bytes(p, D), groups = D / G;

@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(256) rotary_any_kernel(const __grid_constant__
 // are copied.  blockDim = (items, heads at a time, tokens at a time): a thread keeps its item of one token, so it reads cos and
 // sin once, and walks the heads with FLY rows on the way; the first rows are asked for before the position is known.
 template <class T, bool SPLIT>
-__global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ skv_rotary_args a, int turned, int tokens) {
+__global__ void __launch_bounds__(256, 3) rotary_kernel(const __grid_constant__ skv_rotary_args a, int turned, int tokens) {
     constexpr int FLY = sizeof(T) == 2 ? 4 : 2;
     const int token = blockIdx.x * blockDim.z + threadIdx.z;
     if (token >= tokens) return;
