@@ -26,6 +26,8 @@
 // vote and no shuffles; row sums stay in the lanes until the segment ends.
 #pragma once
 
+#include <atomic>
+
 #include "pool_attention.cuh"
 
 namespace skv {
@@ -824,7 +826,13 @@ int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
     constexpr size_t smem = mma_smem<PREC, DP, NT, NQ>();
     static_assert(Shape::CTAS * (smem + 2048) <= 228 * 1024, "an SM holds the CTAs");
     const auto kernel = pool_attention_mma_kernel<PREC, DP, NT, NQ, NP>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<uint64_t> allowed{0};   // devices whose limit on the kernel's shared memory was raised
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev >= 64 || !(allowed.load(std::memory_order_relaxed) >> dev & 1))) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e == cudaSuccess && dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
     if (e != cudaSuccess) return fail(SKV_ERR_CUDA, "pool_attention: %s", cudaGetErrorString(e));
     const int R = a.q.heads / a.pool.heads * a.S_q;
     PageDivide magic;

@@ -30,7 +30,7 @@ import torch
 
 from .. import _lib
 from .._device import as_device, back, compute_device, device_ctx
-from .rotary import _DTYPE_CODE, _NO_ROWS, _as_rows, _rope_fields, _rows_fields
+from .rotary import _DTYPE_CODE, _NO_ROWS, _launch, _like, _rope_fields, _rows
 
 _PRECISION_CODE = {torch.float32: 0, torch.float16: 1, torch.int8: 2, torch.uint8: 3}
 _POOL, _ROWS, _ROPE = "QQQQQqiiiiiiii", "Qqqqii", "QQQqqiiiiii"
@@ -42,15 +42,18 @@ _NO_ROPE = (0,) * 11
 _SCRATCH = {}   # (device, stream) -> attention scratch
 
 
-def _scratch(dev: torch.device, stream: int, D: int) -> torch.Tensor:
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+
+
+def _scratch(dev: torch.device, stream: int) -> torch.Tensor:
     """The attention's scratch on a stream: partial results and arrival counters that every call leaves zero.  Calls
     of one stream follow each other, so they share one; a graph being captured gets its own."""
     t = _SCRATCH.get((dev.index, stream))
-    capturing = torch.cuda.is_current_stream_capturing()
+    capturing = _capturing()
     if t is None or capturing:
         lib = _lib.load()
         # sized for any head the kernels take, so that it is made once
-        t = torch.empty(lib.skv_pool_attention_scratch_bytes(max(D, 512)), dtype=torch.uint8, device=dev)
+        t = torch.empty(lib.skv_pool_attention_scratch_bytes(512), dtype=torch.uint8, device=dev)
         t[:lib.skv_pool_attention_scratch_zeros()].zero_()
         if not capturing:
             _SCRATCH[dev.index, stream] = t
@@ -65,15 +68,17 @@ def _index(t: torch.Tensor, shape: Tuple[int, ...], dev: torch.device, name: str
         if t.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"{name} must be int32 or int64, got {t.dtype}")
         t = t.to(device=dev, dtype=torch.int32)
-    return t if t.stride(-1) == 1 or shape[-1] <= 1 else t.contiguous()
+    return t if t.is_contiguous() or t.stride(-1) == 1 else t.contiguous()
 
 
 def _pool_fields(k_pages, v_pages, block_table, scale_k, scale_v, batch: int, head_dim: Optional[int]):
     """The ``skv_pool`` fields, the pool's device and the table that was used (kept until the launch)."""
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype is not v_pages.dtype:
+    shape = k_pages.shape
+    dtype = k_pages.dtype
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype is not dtype:
         raise ValueError("k_pages/v_pages must be alike [num_pages, heads, page_size, row], got "
                          f"{tuple(k_pages.shape)} {k_pages.dtype} and {tuple(v_pages.shape)} {v_pages.dtype}")
-    code = _PRECISION_CODE.get(k_pages.dtype)
+    code = _PRECISION_CODE.get(dtype)
     if code is None:
         raise ValueError(f"Unsupported page precision: {k_pages.dtype}")
     if not k_pages.is_cuda:
@@ -82,29 +87,30 @@ def _pool_fields(k_pages, v_pages, block_table, scale_k, scale_v, batch: int, he
     dev = k_pages.device
     if v_pages.device != dev or not k_pages.is_contiguous() or not v_pages.is_contiguous():
         raise ValueError("the pages must be contiguous tensors on one device")
-    N, H, P, row = k_pages.shape
-    D, group, scales = (2 * row if code == 3 else row) if head_dim is None else head_dim, 0, (0, 0)
+    N, H, P, row = shape
+    D = (2 * row if code == 3 else row) if head_dim is None else head_dim
     if row != ((D + 1) // 2 if code == 3 else D):
         raise ValueError(f"page rows of {row} do not hold a head_dim of {D}")
+    group = sk = sv = 0
     if code >= 2:
         if scale_k is None or scale_v is None:
             raise ValueError("int8/int4 pages need scale_k and scale_v")
-        want = 4 if code == 2 else 5
+        tail = scale_k.shape[3:]
         for s in (scale_k, scale_v):
-            if s.dtype is not torch.float32 or s.device != dev or not s.is_contiguous() or s.dim() != want \
-                    or s.shape[:3] != (N, H, P) or s.shape[-1] != 1:
+            if s.dtype is not torch.float32 or s.device != dev or s.shape[:3] != (N, H, P) or len(s.shape) != code + 2 \
+                    or s.shape[-1] != 1 or not s.is_contiguous():
                 raise ValueError(f"scales must be contiguous float32 [{N}, {H}, {P}, {'1' if code == 2 else 'groups, 1'}] "
                                  f"on {dev}, got {tuple(s.shape)} {s.dtype}")
         if code == 3:
-            groups = scale_k.shape[3]
-            if groups < 1 or D % groups or scale_v.shape != scale_k.shape:
-                raise ValueError(f"{groups} int4 groups do not divide a head_dim of {D}")
-            group = D // groups
-        scales = (scale_k.data_ptr(), scale_v.data_ptr())
-    if block_table.dim() != 2 or block_table.shape[0] != batch:
+            if tail[0] < 1 or D % tail[0] or scale_v.shape[3:] != tail:
+                raise ValueError(f"{tail[0]} int4 groups do not divide a head_dim of {D}")
+            group = D // tail[0]
+        sk, sv = scale_k.data_ptr(), scale_v.data_ptr()
+    table_shape = block_table.shape
+    if len(table_shape) != 2 or table_shape[0] != batch:
         raise ValueError(f"block_table must be [batch={batch}, width], got {tuple(block_table.shape)}")
-    table = _index(block_table, block_table.shape, dev, "block_table")
-    return ((k_pages.data_ptr(), v_pages.data_ptr(), *scales, table.data_ptr(), table.stride(0), table.shape[1], N, P, H,
+    table = _index(block_table, table_shape, dev, "block_table")
+    return ((k_pages.data_ptr(), v_pages.data_ptr(), sk, sv, table.data_ptr(), table.stride(0), table_shape[1], N, P, H,
              D, group, code, batch), dev, table)
 
 
@@ -112,8 +118,8 @@ def _flag(check: bool, dev: torch.device) -> Optional[torch.Tensor]:
     return torch.zeros(1, dtype=torch.int32, device=dev) if check else None
 
 
-def _raise_flag(flag: Optional[torch.Tensor], what: str) -> None:
-    if flag is not None and int(flag.item()):
+def _raise_flag(flag: torch.Tensor, what: str) -> None:
+    if int(flag.item()):
         raise ValueError(f"{what}: a page number, length or position lies outside the pool or the tables")
 
 
@@ -158,29 +164,29 @@ def paged_append(
         raise ValueError("cos and sin must be given together")
     lens = _index(lengths, (B,), dev, "lengths")
     new = None if new_lengths is None else _index(new_lengths, (B,), dev, "new_lengths")
-    kd = _as_rows(k, dev)
-    vd = _as_rows(v, dev, kd.dtype)
+    kd, k_rows = _rows(k, dev)
+    vd, v_rows = _rows(v, dev, kd.dtype)
     q_rows = q_out_rows = _NO_ROWS
-    q_out = None
+    qd = q_out = None
     if q is not None:
         if q.dim() != 4 or (q.shape[0], q.shape[2], q.shape[3]) != (B, S, D):
             raise ValueError(f"q must be [batch, heads, {S}, {D}], got {tuple(q.shape)}")
         if cos is None:
             raise ValueError("q without cos and sin has nothing to be rotated by")
-        qd = _as_rows(q, dev, kd.dtype)
-        q_out = torch.empty(qd.shape, dtype=qd.dtype, device=dev)
-        q_rows, q_out_rows = _rows_fields(qd), _rows_fields(q_out)
+        qd, q_rows = _rows(q, dev, kd.dtype)
+        q_out, q_out_rows = _like(qd)
     rope, keep = _NO_ROPE, None
     if cos is not None:
-        rope, keep = _rope_fields(cos, sin, positions, B, S, D, interleaved, False, dev)
+        rope, keep = _rope_fields(cos, sin, positions, B, S, D, bool(interleaved), False, dev)
     flag = _flag(check, dev)
-    args = _APPEND.pack(*pool, *_rows_fields(kd), *_rows_fields(vd), *q_rows, *q_out_rows, *rope, lens.data_ptr(),
+    args = _APPEND.pack(*pool, *k_rows, *v_rows, *q_rows, *q_out_rows, *rope, lens.data_ptr(),
                         0 if new is None else new.data_ptr(), 0 if flag is None else flag.data_ptr(), S, 0)
-    with device_ctx(dev):
-        st = _lib.load().skv_pool_append(args, _lib.stream_of(dev))
-    _lib.check(st, "paged_append")
-    del table, keep
-    _raise_flag(flag, "paged_append")
+    st = _launch(_lib.load().skv_pool_append, args, dev)
+    if st:
+        _lib.check(st, "paged_append")
+    del table, keep, vd, qd
+    if flag is not None:
+        _raise_flag(flag, "paged_append")
     return None if q_out is None else back(q_out, q.device)
 
 
@@ -212,14 +218,17 @@ def paged_read(
     first = None if start is None else _index(start, (B,), dev, "start")
     k = torch.empty((B, pool[9], tokens, pool[10]), dtype=dtype, device=dev)
     v = torch.empty_like(k)
+    st = k.stride()
+    rows = (st[0], st[1], st[2], _DTYPE_CODE[dtype], pool[9])
     flag = _flag(check, dev)
-    args = _READ.pack(*pool, *_rows_fields(k), *_rows_fields(v), 0 if first is None else first.data_ptr(),
+    args = _READ.pack(*pool, k.data_ptr(), *rows, v.data_ptr(), *rows, 0 if first is None else first.data_ptr(),
                       lens.data_ptr(), 0 if flag is None else flag.data_ptr(), tokens, 0)
-    with device_ctx(dev):
-        st = _lib.load().skv_pool_read(args, _lib.stream_of(dev))
-    _lib.check(st, "paged_read")
+    st = _launch(_lib.load().skv_pool_read, args, dev)
+    if st:
+        _lib.check(st, "paged_read")
     del table
-    _raise_flag(flag, "paged_read")
+    if flag is not None:
+        _raise_flag(flag, "paged_read")
     return k, v
 
 
@@ -246,6 +255,9 @@ def paged_attention(
     ``new_lengths[b]``).  A query that sees nothing (padding, an empty sequence) gives zeros.
     ``scale`` defaults to ``1/sqrt(D)``.
 
+    The result has ``q``'s dimension order in memory (as torch's own operators keep it), so that the output of a
+    ``[B, S, H, D]`` projection goes back to one without a copy.
+
     Scores, softmax and sums are fp32.  Every page is read once for all the query rows that share its key
     head.  The sequences are split over the whole GPU by their lengths on the device, long ones into
     parts that are joined in token order, so equal calls give equal bits.
@@ -258,21 +270,22 @@ def paged_attention(
         raise ValueError(f"{Hq} query heads do not share {pool[9]} key heads evenly")
     lens = _index(lengths, (B,), dev, "lengths")
     new = None if new_lengths is None else _index(new_lengths, (B,), dev, "new_lengths")
-    qd = _as_rows(q, dev)
-    out = torch.empty((B, Hq, S_q, D), dtype=qd.dtype, device=dev)
-    lib = _lib.load()
+    qd, q_rows = _rows(q, dev)
+    out, out_rows = _like(qd)
+    flag = _flag(check, dev)
+    entry = _lib.load().skv_pool_attention
     with device_ctx(dev):
         stream = _lib.stream_of(dev)
-        scratch = _scratch(dev, stream, D)
-        flag = _flag(check, dev)
-        args = _ATTENTION.pack(*pool, *_rows_fields(qd), *_rows_fields(out), lens.data_ptr(),
-                               0 if new is None else new.data_ptr(), scratch.data_ptr(), scratch.numel(),
-                               0 if flag is None else flag.data_ptr(), S_q, bool(causal),
+        scratch = _scratch(dev, stream)
+        args = _ATTENTION.pack(*pool, *q_rows, *out_rows, lens.data_ptr(), 0 if new is None else new.data_ptr(),
+                               scratch.data_ptr(), scratch.numel(), 0 if flag is None else flag.data_ptr(), S_q, bool(causal),
                                1.0 / math.sqrt(D) if scale is None else scale, 0)
-        st = lib.skv_pool_attention(args, stream)
-    _lib.check(st, "paged_attention")
-    del table
-    _raise_flag(flag, "paged_attention")
+        st = entry(args, stream)
+    if st:
+        _lib.check(st, "paged_attention")
+    del table, qd
+    if flag is not None:
+        _raise_flag(flag, "paged_attention")
     return back(out, q.device)
 
 

@@ -67,21 +67,37 @@ def rotary_tables(
     return (angle.cos() * gain).float(), (angle.sin() * gain).float()
 
 
-def _as_rows(t: torch.Tensor, dev: torch.device, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """``t`` [B, H, S, D] as the kernels read it: on ``dev``, fp32 / fp16 / bf16, the last dimension contiguous."""
-    if t.requires_grad:
-        t = t.detach()
-    if dtype is None:
-        dtype = t.dtype if t.dtype in _DTYPE_CODE else torch.float32
-    if t.dtype is not dtype or not t.is_cuda or t.get_device() != dev.index:
-        t = t.to(device=dev, dtype=dtype)
-    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
-
-
-def _rows_fields(t: torch.Tensor) -> Tuple[int, int, int, int, int, int]:
-    """The ``skv_rows`` fields of a tensor from ``_as_rows``."""
+def _rows(t: torch.Tensor, dev: torch.device, dtype: Optional[torch.dtype] = None):
+    """``t`` [B, H, S, D] as the kernels read it (on ``dev``, fp32 / fp16 / bf16, the last dimension contiguous), and its
+    ``skv_rows`` fields."""
+    have = t.dtype
+    code = _DTYPE_CODE.get(have)
+    if t.requires_grad or code is None or (dtype is not None and have is not dtype) or not t.is_cuda or t.get_device() != dev.index:
+        if dtype is None:
+            dtype = have if code is not None else torch.float32
+        t = t.detach().to(device=dev, dtype=dtype)
+        code = _DTYPE_CODE[dtype]
     st = t.stride()
-    return (t.data_ptr(), st[0], st[1], st[2], _DTYPE_CODE[t.dtype], t.shape[1])
+    if st[3] != 1 and t.shape[3] != 1:
+        t = t.contiguous()
+        st = t.stride()
+    return t, (t.data_ptr(), st[0], st[1], st[2], code, t.shape[1])
+
+
+def _like(t: torch.Tensor):
+    """An output laid out like ``t`` (dense, dimensions in the order of ``t``'s strides), and its ``skv_rows`` fields."""
+    out = torch.empty_like(t)
+    st = out.stride()
+    if st[3] != 1 and t.shape[3] != 1:
+        out = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        st = out.stride()
+    return out, (out.data_ptr(), st[0], st[1], st[2], _DTYPE_CODE[out.dtype], t.shape[1])
+
+
+def _launch(entry, args: bytes, dev: torch.device) -> int:
+    """``entry(args, stream)`` on ``dev`` and its current stream."""
+    with device_ctx(dev):
+        return entry(args, _lib.stream_of(dev))
 
 
 def _table_checked(t: torch.Tensor, dev: torch.device, name: str) -> torch.Tensor:
@@ -95,25 +111,28 @@ def _table_checked(t: torch.Tensor, dev: torch.device, name: str) -> torch.Tenso
 def _rope_fields(cos, sin, positions, B: int, S: int, D: int, interleaved: bool, inverse: bool, dev: torch.device):
     """The ``skv_rope`` fields, and the tensors they point into (to be kept until the launch)."""
     cos, sin = _table_checked(cos, dev, "cos"), _table_checked(sin, dev, "sin")
-    if cos.shape != sin.shape:
+    count, half = cos.shape
+    if sin.shape != (count, half):
         raise ValueError(f"cos/sin shapes disagree: {tuple(cos.shape)} vs {tuple(sin.shape)}")
-    rot = 2 * cos.shape[1]
-    if rot < 2 or rot > D:
-        raise ValueError(f"the tables rotate {rot} values of a head of {D}")
-    at = (0, 0, 0, 0)
-    if positions is not None:
-        if positions.dtype not in (torch.int32, torch.int64):
-            raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
-        if not positions.is_cuda or positions.get_device() != dev.index:
-            positions = positions.to(dev)
-        if positions.shape != (B, S):
-            try:
-                positions = positions.expand(B, S)
-            except RuntimeError:
-                raise ValueError(f"positions must broadcast to [{B}, {S}], got {tuple(positions.shape)}") from None
-        st = positions.stride()
-        at = (positions.data_ptr(), st[0], st[1], positions.element_size())
-    return ((cos.data_ptr(), sin.data_ptr(), *at, rot, cos.shape[0], bool(interleaved), bool(inverse), 0),
+    if half < 1 or 2 * half > D:
+        raise ValueError(f"the tables rotate {2 * half} values of a head of {D}")
+    if positions is None:
+        return (cos.data_ptr(), sin.data_ptr(), 0, 0, 0, 0, 2 * half, count, interleaved, inverse, 0), (cos, sin)
+    if positions.dtype is torch.int64:
+        size = 8
+    elif positions.dtype is torch.int32:
+        size = 4
+    else:
+        raise ValueError(f"positions must be int32 or int64, got {positions.dtype}")
+    if not positions.is_cuda or positions.get_device() != dev.index:
+        positions = positions.to(dev)
+    if positions.shape != (B, S):
+        try:
+            positions = positions.expand(B, S)
+        except RuntimeError:
+            raise ValueError(f"positions must broadcast to [{B}, {S}], got {tuple(positions.shape)}") from None
+    st = positions.stride()
+    return ((cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), st[0], st[1], size, 2 * half, count, interleaved, inverse, 0),
             (cos, sin, positions))
 
 
@@ -143,21 +162,20 @@ def apply_rotary(
     B, _, S, D = q.shape
     if k is not None and (k.dim() != 4 or (k.shape[0], k.shape[2], k.shape[3]) != (B, S, D)):
         raise ValueError(f"q/k shapes disagree: {tuple(q.shape)} vs {tuple(k.shape)}")
-    dev = compute_device(q, k, cos)
-    qd = _as_rows(q, dev)
-    q_out = torch.empty(qd.shape, dtype=qd.dtype, device=dev)
+    dev = q.device if q.is_cuda else compute_device(k, cos)
+    qd, q_rows = _rows(q, dev)
+    q_out, q_out_rows = _like(qd)
+    kd = k_out = None
+    k_rows = k_out_rows = _NO_ROWS
     if k is not None:
-        kd = _as_rows(k, dev, qd.dtype)
-        k_out = torch.empty(kd.shape, dtype=qd.dtype, device=dev)
-        k_rows, k_out_rows = _rows_fields(kd), _rows_fields(k_out)
-    else:
-        k_rows = k_out_rows = _NO_ROWS
-    rope, keep = _rope_fields(cos, sin, positions, B, S, D, interleaved, inverse, dev)
-    args = _ARGS.pack(*_rows_fields(qd), *k_rows, *_rows_fields(q_out), *k_out_rows, *rope, B, S, D, 0)
-    with device_ctx(dev):
-        st = _lib.load().skv_rotary(args, _lib.stream_of(dev))
-    _lib.check(st, "apply_rotary")
-    del keep
+        kd, k_rows = _rows(k, dev, qd.dtype)
+        k_out, k_out_rows = _like(kd)
+    rope, keep = _rope_fields(cos, sin, positions, B, S, D, bool(interleaved), bool(inverse), dev)
+    args = _ARGS.pack(*q_rows, *k_rows, *q_out_rows, *k_out_rows, *rope, B, S, D, 0)
+    st = _launch(_lib.load().skv_rotary, args, dev)
+    if st:
+        _lib.check(st, "apply_rotary")
+    del keep, kd
     if k is None:
         return back(q_out, q.device)
     return back(q_out, q.device), back(k_out, k.device)
