@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(256, 3) pool_append_kernel(const __grid_consta
 }
 
 // A warp per (token, head) row of K and of V; any D, group, strides and alignment.
-template <class T>
+template <class T, int PREC>
 __global__ void __launch_bounds__(32 * kPoolWarps) pool_read_any_kernel(const __grid_constant__ skv_pool_read_args a) {
     const int lane = threadIdx.x & 31;
     const int64_t item = (int64_t)blockIdx.x * kPoolWarps + (threadIdx.x >> 5);
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(32 * kPoolWarps) pool_read_any_kernel(const __
         const skv_rows& o = v ? a.v_out : a.k_out;
         T* out = static_cast<T*>(o.ptr) + b * o.stride_b + h * o.stride_h + s * o.stride_s;
         for (int d = lane; d < D; d += kWarp)
-            out[d] = from_float<T>(row < 0 ? 0.0f : pool_value(a.pool, v, row, d));
+            out[d] = from_float<T>(row < 0 ? 0.0f : pool_value<PREC>(a.pool, v, row, d, PREC == 3 ? d / a.pool.int4_group : 0));
     }
 }
 
@@ -437,7 +437,12 @@ int launch_read(const skv_pool_read_args& a, cudaStream_t st) {
                      aligned16(a.pool.v) && (a.pool.precision != 3 || a.pool.int4_group % 8 == 0);
     if (!vec) {
         const int64_t blocks = (rows * a.S + kPoolWarps - 1) / kPoolWarps;
-        pool_read_any_kernel<T><<<(unsigned)blocks, 32 * kPoolWarps, 0, st>>>(a);
+        switch (a.pool.precision) {
+            case 0: pool_read_any_kernel<T, 0><<<(unsigned)blocks, 32 * kPoolWarps, 0, st>>>(a); break;
+            case 1: pool_read_any_kernel<T, 1><<<(unsigned)blocks, 32 * kPoolWarps, 0, st>>>(a); break;
+            case 2: pool_read_any_kernel<T, 2><<<(unsigned)blocks, 32 * kPoolWarps, 0, st>>>(a); break;
+            default: pool_read_any_kernel<T, 3><<<(unsigned)blocks, 32 * kPoolWarps, 0, st>>>(a);
+        }
         return check_launch("pool_read");
     }
     const int lanes = D / (16 / (int)sizeof(T));

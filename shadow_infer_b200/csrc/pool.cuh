@@ -106,20 +106,19 @@ __host__ __device__ inline int64_t pool_row_bytes(int precision, int D) {
     return precision == 0 ? (int64_t)D * 4 : precision == 1 ? (int64_t)D * 2 : precision == 2 ? D : ((int64_t)D + 1) / 2;
 }
 
-// One value of a pool row, any D and group.
-__device__ __forceinline__ float pool_value(const skv_pool& p, bool is_v, int64_t row, int col) {
+// Value col of pool rows, any D and group; block: col / int4_group.
+template <int PREC>
+__device__ __forceinline__ float pool_value(const skv_pool& p, bool is_v, int64_t row, int col, int block) {
     const uint8_t* base = static_cast<const uint8_t*>(is_v ? p.v : p.k);
     const float* sc = is_v ? p.scale_v : p.scale_k;
     const int D = p.head_dim;
-    switch (p.precision) {
-        case 0: return reinterpret_cast<const float*>(base)[row * D + col];
-        case 1: return __half2float(reinterpret_cast<const __half*>(base)[row * D + col]);
-        case 2: return __fmul_rn((float)reinterpret_cast<const int8_t*>(base)[row * D + col], sc[row]);
-        default: {
-            const uint8_t byte = base[row * ((D + 1) / 2) + col / 2];
-            const int q = (col & 1) ? (byte & 15) : (byte >> 4);
-            return __fmul_rn((float)(q - 8), sc[row * (D / p.int4_group) + col / p.int4_group]);
-        }
+    if constexpr (PREC == 0) return __ldg(reinterpret_cast<const float*>(base) + row * D + col);
+    else if constexpr (PREC == 1) return __half2float(__ldg(reinterpret_cast<const __half*>(base) + row * D + col));
+    else if constexpr (PREC == 2) return __fmul_rn((float)__ldg(reinterpret_cast<const signed char*>(base) + row * D + col), __ldg(sc + row));
+    else {
+        const uint8_t byte = __ldg(base + row * ((D + 1) / 2) + col / 2);
+        const int q = (col & 1) ? (byte & 15) : (byte >> 4);
+        return __fmul_rn((float)(q - 8), __ldg(sc + row * (D / p.int4_group) + block));
     }
 }
 

@@ -16,8 +16,9 @@
 namespace skv {
 
 // --------------------------------------------------------------------------- any size and alignment
-// Products on the FMA pipe from fp32 tiles in shared memory: 8 rows, 32 tokens at a time.  Thread =
-// (token, rows w and w + 4) for the scores, value d for the sums.
+// Products on the FMA pipe from fp32 tiles in shared memory: 8 rows, 32 tokens at a time.  Thread = (token, rows w and
+// w + 4) for the scores, value d for the sums.  A warp widens 8 tokens a tile, a lane a value of each, so that 16 loads are on
+// their way; the lanes look up the tokens' rows one tile ahead.
 constexpr int kAnyRows = 8, kAnyTile = 32, kAnyThreads = 128, kAnyMaxD = 512, kAnyParts = 64;
 
 __host__ __device__ inline size_t any_smem(int D) {
@@ -25,7 +26,7 @@ __host__ __device__ inline size_t any_smem(int D) {
             join_floats<kAnyRows, kAnyThreads, kAnyParts>()) * 4;
 }
 
-template <class T>
+template <class T, int PREC>
 __global__ void __launch_bounds__(kAnyThreads) pool_attention_any_kernel(const __grid_constant__ skv_pool_attention_args a,
                                                                          int row_tiles) {
     extern __shared__ float any_sm[];
@@ -60,18 +61,38 @@ __global__ void __launch_bounds__(kAnyThreads) pool_attention_any_kernel(const _
         for (int j = 0; j < kAnyRows; ++j)
 #pragma unroll
             for (int i = 0; i < kAnyMaxD / kAnyThreads; ++i) o[j][i] = 0.0f;
+        // the pool row of token lane % 8 of this warp's eight, -1 where there is none
+        auto row_of = [&](int first) -> int64_t {
+            const int t = first + warp * 8 + (lane & 7);
+            if (t >= g.tokens) return -1;
+            const int64_t r = pool_row(a.pool, g.b, t);
+            if (r < 0 && a.error_flag) atomicExch(a.error_flag, 1);
+            return r < 0 ? -1 : r + (int64_t)g.hk * a.pool.page_size;
+        };
+        int64_t next_row = row_of(g.t0 * kAnyTile);
         for (int t = g.t0; t < g.t1; ++t) {
             const int tok0 = t * kAnyTile;
             __syncthreads();
-            for (int j = warp; j < kAnyTile; j += kAnyThreads / 32) {
-                int64_t row = tok0 + j < g.tokens ? pool_row(a.pool, g.b, tok0 + j) : -1;
-                if (row < 0 && tok0 + j < g.tokens && lane == 0 && a.error_flag) atomicExch(a.error_flag, 1);
-                if (row >= 0) row += (int64_t)g.hk * a.pool.page_size;
-                for (int d = lane; d < D; d += 32) {
-                    sk[j * (D + 1) + d] = row >= 0 ? pool_value(a.pool, false, row, d) : 0.0f;
-                    sv[j * D + d] = row >= 0 ? pool_value(a.pool, true, row, d) : 0.0f;
+            const int64_t row = next_row;
+            if (t + 1 < g.t1) next_row = row_of(tok0 + kAnyTile);
+            if (lane < 8) sp[warp * 8 + lane] = row >= 0 ? 1.0f : 0.0f;   // whether there is such a token
+            int64_t rows[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) rows[j] = __shfl_sync(0xffffffffu, row, j);
+            for (int d = lane; d < D; d += 32) {
+                const int block = PREC == 3 ? d / a.pool.int4_group : 0;
+                float x[8], y[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int64_t r = rows[j];
+                    x[j] = r >= 0 ? pool_value<PREC>(a.pool, false, r, d, block) : 0.0f;
+                    y[j] = r >= 0 ? pool_value<PREC>(a.pool, true, r, d, block) : 0.0f;
                 }
-                if (lane == 0) sp[j] = row >= 0 ? 1.0f : 0.0f;   // whether there is such a token
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    sk[(warp * 8 + j) * (D + 1) + d] = x[j];
+                    sv[(warp * 8 + j) * D + d] = y[j];
+                }
             }
             __syncthreads();
             const bool held = sp[lane] != 0.0f;
@@ -149,20 +170,30 @@ __global__ void __launch_bounds__(kAnyThreads) pool_attention_any_kernel(const _
     }
 }
 
-template <class T>
-int launch_any(const skv_pool_attention_args& a, cudaStream_t st) {
+template <class T, int PREC>
+int launch_any_prec(const skv_pool_attention_args& a, cudaStream_t st) {
     const int R = a.q.heads / a.pool.heads * a.S_q, row_tiles = (R + kAnyRows - 1) / kAnyRows;
     const size_t smem = any_smem(a.pool.head_dim);
-    cudaError_t e = cudaFuncSetAttribute(pool_attention_any_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(pool_attention_any_kernel<T, PREC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)smem);
     int per_sm = 1;
     if (e == cudaSuccess)
-        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, pool_attention_any_kernel<T>, kAnyThreads, smem);
+        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, pool_attention_any_kernel<T, PREC>, kAnyThreads, smem);
     if (e != cudaSuccess) return fail(SKV_ERR_CUDA, "pool_attention: %s", cudaGetErrorString(e));
     int grid = sm_count() * (per_sm < 1 ? 1 : per_sm > 8 ? 8 : per_sm);
     if (grid > kMaxCtas) grid = kMaxCtas;
-    pool_attention_any_kernel<T><<<grid, kAnyThreads, smem, st>>>(a, row_tiles);
+    pool_attention_any_kernel<T, PREC><<<grid, kAnyThreads, smem, st>>>(a, row_tiles);
     return check_launch("pool_attention");
+}
+
+template <class T>
+int launch_any(const skv_pool_attention_args& a, cudaStream_t st) {
+    switch (a.pool.precision) {
+        case 0: return launch_any_prec<T, 0>(a, st);
+        case 1: return launch_any_prec<T, 1>(a, st);
+        case 2: return launch_any_prec<T, 2>(a, st);
+        default: return launch_any_prec<T, 3>(a, st);
+    }
 }
 
 // The tensor-core kernels (pool_attention_mma.cuh), one translation unit a precision.
