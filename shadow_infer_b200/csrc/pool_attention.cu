@@ -201,13 +201,13 @@ int attend_fp16(const skv_pool_attention_args& a, cudaStream_t st);
 int attend_int8(const skv_pool_attention_args& a, cudaStream_t st);
 int attend_int4(const skv_pool_attention_args& a, cudaStream_t st);
 
-// They need heads of up to 128 values in rows of whole 16-byte chunks, int4 groups of whole 16-value blocks, payloads on
-// 16-byte boundaries, a row 0, and row numbers of 31 bits.
+// They need heads of up to 256 values in rows of whole 16-byte (fp16) or 8-byte chunks, int4 groups of whole 16-value blocks,
+// payloads on 16-byte boundaries, a row 0, and row numbers of 31 bits.
 bool fits_mma(const skv_pool& p) {
     const int D = p.head_dim;
     const int64_t rows = (int64_t)p.num_pages * p.heads * p.page_size;
-    if (rows == 0 || rows > 0x7fffffff || p.precision == 0 || D > 128) return false;
-    if (D % (p.precision == 1 ? 8 : p.precision == 2 ? 16 : 32) || (p.precision == 3 && p.int4_group % 16)) return false;
+    if (rows == 0 || rows > 0x7fffffff || p.precision == 0 || D > 256) return false;
+    if (D % (p.precision == 3 ? 16 : 8) || (p.precision == 3 && p.int4_group % 16)) return false;
     return ((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v)) & 15) == 0;
 }
 

@@ -61,6 +61,7 @@ __device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint
 template <int BYTES>
 __device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
     if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+    else if constexpr (BYTES == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -140,29 +141,22 @@ struct PageRows {
 template <int E, class T>
 __device__ __forceinline__ void load_row(const T* p, int left, bool vec, float (&x)[E]) {
     if (vec) {
-        if constexpr (sizeof(T) == 4) {
-            if constexpr (E == 4) {
-                const float4 v = *reinterpret_cast<const float4*>(p);
-                x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-            } else {
-                const float2 v = *reinterpret_cast<const float2*>(p);
-                x[0] = v.x; x[1] = v.y;
-            }
-        } else {
-            uint32_t w[E / 2];
-            if constexpr (E == 4) {
-                const uint2 v = *reinterpret_cast<const uint2*>(p);
-                w[0] = v.x; w[1] = v.y;
-            } else {
-                w[0] = *reinterpret_cast<const uint32_t*>(p);
-            }
+        constexpr int WORDS = E * (int)sizeof(T) / 4;
+        uint32_t w[WORDS];
+        if constexpr (WORDS >= 4) {
 #pragma unroll
-            for (int i = 0; i < E / 2; ++i) {
-                const T* h = reinterpret_cast<const T*>(&w[i]);
-                x[2 * i] = to_float(h[0]);
-                x[2 * i + 1] = to_float(h[1]);
+            for (int i = 0; i < WORDS / 4; ++i) {
+                const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+                w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
             }
+        } else if constexpr (WORDS == 2) {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
+            w[0] = v.x; w[1] = v.y;
+        } else {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
         }
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = to_float(reinterpret_cast<const T*>(w)[i]);
     } else {
 #pragma unroll
         for (int i = 0; i < E; ++i)
@@ -180,7 +174,7 @@ __device__ __forceinline__ float query_place(int d, int& mma, int& c, int& reg, 
     }
     const int r = d % 4;   // of a word's or a byte pair's values: 0 and 2 in one register, 1 and 3 in the other
     reg = r % 2; half = r / 2;
-    if (PREC == 2) {       // lane column c reads chunks 2c, 2c + 1 (the row's only four: chunk c)
+    if (PREC == 2) {       // lane column c reads DP / 64 neighbouring chunks
         const int chunk = d / 16, per = DP / 64;
         mma = 4 * (chunk % per) + (d % 16) / 4; c = chunk / per;
         return 1.0f;
@@ -218,9 +212,9 @@ template <int PREC, int DP, int NT>
 struct MmaShape {
     // Warps a CTA, CTAs an SM, slots a warp: what 64 K registers and 227 KB of shared memory hold, with at least 60 KB of
     // rows on their way (HBM's latency times its rate is about 43 KB an SM).
-    static constexpr int W = NT == 1 && PREC >= 2 ? 8 : 4;
-    static constexpr int CTAS = NT == 4 ? 2 : NT == 2 ? (PREC == 1 ? 2 : 3) : PREC == 1 ? 3 : 2;
-    static constexpr int SLOTS = PREC == 1 ? 2 : 3;
+    static constexpr int W = PREC >= 2 && (NT == 1 || DP == 256) ? 8 : 4;
+    static constexpr int CTAS = DP == 256 ? 1 : NT == 2 ? (PREC == 1 ? 2 : 3) : PREC == 1 ? 3 : 2;
+    static constexpr int SLOTS = PREC == 1 && DP < 256 ? 2 : 3;
 };
 
 template <int PREC, int DP, int NT, int NQ>
@@ -325,9 +319,18 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
             for (int i = 0; i < COPIES; ++i) {
                 const int r = p16 ? first + my_row + i * STEP : max(__shfl_sync(0xffffffffu, row, my_row + i * STEP), 0);
                 const uint32_t y = L::step(to_rows, i, STEP);
-                if (my_chunk * 16 < row_bytes) {
-                    copy_async<16>(y, k_lane + (int64_t)r * row_bytes);
-                    copy_async<16>(y + L::V, v_lane + (int64_t)r * row_bytes);
+                if (PREC == 1 || row_bytes % 16 == 0) {
+                    if (my_chunk * 16 < row_bytes) {
+                        copy_async<16>(y, k_lane + (int64_t)r * row_bytes);
+                        copy_async<16>(y + L::V, v_lane + (int64_t)r * row_bytes);
+                    }
+                } else {   // rows end in half a chunk, and every second one starts in the middle of 16 bytes
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        if (my_chunk * 16 + 8 * h < row_bytes) {
+                            copy_async<8>(y + 8 * h, k_lane + (int64_t)r * row_bytes + 8 * h);
+                            copy_async<8>(y + L::V + 8 * h, v_lane + (int64_t)r * row_bytes + 8 * h);
+                        }
                 }
             }
         }
@@ -337,14 +340,14 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
         } else if constexpr (PREC == 3) {
             constexpr int PARTS = L::BLOCKS / 4;   // 16-byte pieces of a token's scales
             if (exact) {
-                const int tok = DP == 128 ? lane / 2 : lane % 16;
-                const int r = p16 ? first + tok : max(__shfl_sync(0xffffffffu, row, tok), 0);
-                if constexpr (PARTS == 2) {
-                    copy_async<16>(to + L::SK + lane * 16, a.pool.scale_k + (int64_t)r * L::BLOCKS + (lane & 1) * 4);
-                    copy_async<16>(to + L::SV + lane * 16, a.pool.scale_v + (int64_t)r * L::BLOCKS + (lane & 1) * 4);
-                } else {
-                    copy_async<16>(to + (lane < 16 ? L::SK : L::SV) + tok * 16,
-                                   (lane < 16 ? a.pool.scale_k : a.pool.scale_v) + (int64_t)r * L::BLOCKS);
+#pragma unroll
+                for (int i = 0; i < (PARTS + 1) / 2; ++i) {
+                    const int tok = (lane + 32 * i) / PARTS & 15, piece = (lane + 32 * i) % PARTS;
+                    const int r = p16 ? first + tok : max(__shfl_sync(0xffffffffu, row, tok), 0);
+                    const int64_t x = (int64_t)r * L::BLOCKS + 4 * piece;
+                    const uint32_t y = to + L::SK + tok * L::BLOCKS * 4 + piece * 16;
+                    if (PARTS > 1 || lane < 16) copy_async<16>(y, a.pool.scale_k + x);
+                    if (PARTS > 1 || lane >= 16) copy_async<16>(y + (L::SV - L::SK), a.pool.scale_v + x);
                 }
             } else {
                 const int groups = D / a.pool.int4_group;
@@ -501,7 +504,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                 } else {
 #pragma unroll
                     for (int j = 0; j < DP / 64; ++j) {
-                        const int ch = DP == 128 ? 2 * lc + j : lc;
+                        const int ch = DP / 64 * lc + j;
                         const uint4 u4 = *reinterpret_cast<const uint4*>(slot + L::K + L::at(lg, ch));
                         const uint4 v4 = *reinterpret_cast<const uint4*>(slot + L::K + L::at(lg + 8, ch));
                         const uint32_t u[4] = {u4.x, u4.y, u4.z, u4.w}, v[4] = {v4.x, v4.y, v4.z, v4.w};
@@ -665,9 +668,12 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int tok = 2 * lc + (i & 1) + 8 * (i >> 1);
-                    if constexpr (DP == 128) {
-                        const uint4 y = *reinterpret_cast<const uint4*>(slot + L::V + L::at(tok, lg));
-                        vx[i][0] = y.x; vx[i][1] = y.y; vx[i][2] = y.z; vx[i][3] = y.w;
+                    if constexpr (DP >= 128) {
+#pragma unroll
+                        for (int j = 0; j < DP / 128; ++j) {
+                            const uint4 y = *reinterpret_cast<const uint4*>(slot + L::V + L::at(tok, DP / 128 * lg + j));
+                            vx[i][4 * j] = y.x; vx[i][4 * j + 1] = y.y; vx[i][4 * j + 2] = y.z; vx[i][4 * j + 3] = y.w;
+                        }
                     } else {
                         const uint2 y = *reinterpret_cast<const uint2*>(slot + L::V + L::at(tok, lg / 2) + 8 * (lg & 1));
                         vx[i][0] = y.x; vx[i][1] = y.y;
@@ -692,32 +698,39 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
             } else {
                 // A group's scale in parts of 7 bits (two, or three for 32-bit outputs): x = 64 + (n + 8) times a part
                 // less 72 times it is exact in one fp16 fma.
-                constexpr int PARTS = NQ == 2 ? 3 : 2;
-                uint32_t vx[4][DP / 64], r[PARTS][2], r72[PARTS][2];
+                constexpr int PARTS = NQ == 2 ? 3 : 2, BLOCKS = DP >= 128 ? DP / 128 : 1, WORDS = DP / 64 / BLOCKS;   // a lane's
+                uint32_t vx[4][DP / 64];
+                float down[4];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float y[2];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int tok = 2 * lc + i + 8 * h;
-                        if constexpr (DP == 128) {
-                            const uint2 z = *reinterpret_cast<const uint2*>(slot + L::V + L::at(tok, lg / 2) + 8 * (lg & 1));
-                            vx[2 * h + i][0] = z.x; vx[2 * h + i][1] = z.y;
-                        } else {
-                            vx[2 * h + i][0] = *reinterpret_cast<const uint32_t*>(slot + L::V + L::at(tok, lg / 4) + 4 * (lg & 3));
-                        }
-                        y[i] = reinterpret_cast<const float*>(slot + L::SV)[tok * M + lg * M / 8] *
-                               exp_down(__shfl_sync(0xffffffffu, token_exp, tok), kValueExp);
+                for (int i = 0; i < 4; ++i) {
+                    const int tok = 2 * lc + (i & 1) + 8 * (i >> 1);
+                    if constexpr (DP == 256) {
+                        const uint4 z = *reinterpret_cast<const uint4*>(slot + L::V + L::at(tok, lg));
+                        vx[i][0] = z.x; vx[i][1] = z.y; vx[i][2] = z.z; vx[i][3] = z.w;
+                    } else if constexpr (DP == 128) {
+                        const uint2 z = *reinterpret_cast<const uint2*>(slot + L::V + L::at(tok, lg / 2) + 8 * (lg & 1));
+                        vx[i][0] = z.x; vx[i][1] = z.y;
+                    } else {
+                        vx[i][0] = *reinterpret_cast<const uint32_t*>(slot + L::V + L::at(tok, lg / 4) + 4 * (lg & 3));
                     }
-#pragma unroll
-                    for (int k = 0; k < PARTS; ++k) {
-                        const float y0 = take7(y[0]), y1 = take7(y[1]);
-                        r[k][h] = h2_pack(y0, y1);
-                        r72[k][h] = h2_pack(-72.0f * y0, -72.0f * y1);
-                    }
+                    down[i] = exp_down(__shfl_sync(0xffffffffu, token_exp, tok), kValueExp);
                 }
 #pragma unroll
-                for (int w = 0; w < DP / 64; ++w)
+                for (int w = 0; w < DP / 64; ++w) {
+                    uint32_t r[PARTS][2], r72[PARTS][2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float y[2];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            y[i] = reinterpret_cast<const float*>(slot + L::SV)[(2 * lc + i + 8 * h) * M + lg * M / 8 + w / WORDS] * down[2 * h + i];
+#pragma unroll
+                        for (int k = 0; k < PARTS; ++k) {
+                            const float y0 = take7(y[0]), y1 = take7(y[1]);
+                            r[k][h] = h2_pack(y0, y1);
+                            r72[k][h] = h2_pack(-72.0f * y0, -72.0f * y1);
+                        }
+                    }
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const uint32_t u = __byte_perm(vx[0][w], vx[1][w], i ? 0x7632 : 0x5410);
@@ -734,6 +747,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                             }
                         }
                     }
+                }
             }
         }
 
@@ -854,16 +868,14 @@ int launch_mma_type(const skv_pool_attention_args& a, cudaStream_t st) {
     return launch_mma<PREC, DP, NT, 1, 1>(a, st);
 }
 
-// Row tiles of 8, 16 or 32 rows: the pages are read once for up to 32 rows of a key head.
+// Row tiles of 8 or 16 rows.  (32 rows a tile were 10 to 20 % faster where hundreds of rows meet 8 K tokens or more,
+// 212 against 255 us for 1024 rows of 8 key heads, and 1.5 times slower below: 50 against 33 us for 32 rows.)
 template <int PREC>
 int launch_mma_prec(const skv_pool_attention_args& a, cudaStream_t st) {
-    const int R = a.q.heads / a.pool.heads * a.S_q;
-    if (a.pool.head_dim <= 64) {
-        if (R <= 8) return launch_mma_type<PREC, 64, 1>(a, st);
-        return R <= 16 ? launch_mma_type<PREC, 64, 2>(a, st) : launch_mma_type<PREC, 64, 4>(a, st);
-    }
-    if (R <= 8) return launch_mma_type<PREC, 128, 1>(a, st);
-    return R <= 16 ? launch_mma_type<PREC, 128, 2>(a, st) : launch_mma_type<PREC, 128, 4>(a, st);
+    const int R = a.q.heads / a.pool.heads * a.S_q, D = a.pool.head_dim;
+    if (D <= 64) return R <= 8 ? launch_mma_type<PREC, 64, 1>(a, st) : launch_mma_type<PREC, 64, 2>(a, st);
+    if (D <= 128) return R <= 8 ? launch_mma_type<PREC, 128, 1>(a, st) : launch_mma_type<PREC, 128, 2>(a, st);
+    return R <= 8 ? launch_mma_type<PREC, 256, 1>(a, st) : launch_mma_type<PREC, 256, 2>(a, st);
 }
 
 }  // namespace skv

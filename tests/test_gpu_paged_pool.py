@@ -344,6 +344,15 @@ ATTENTION = [  # counts, H, rep, Sq, D, P, G, causal
     ([40], 1, 1, 1, 300, 8, 16, False),
     ([333, 1000], 1, 12, 1, 128, 128, 64, False),
     ([2100], 1, 16, 2, 64, 16, 16, False),                  # 32 rows a key head
+    ([300, 17, 0, 1000], 2, 3, 1, 256, 32, 16, False),
+    ([70, 260], 1, 8, 3, 256, 16, 64, True),
+    ([129, 5], 3, 2, 1, 160, 32, 32, False),                # heads between the sizes that the kernels are cut to
+    ([66, 190], 1, 4, 1, 192, 11, 16, False),
+    ([95], 2, 1, 5, 112, 48, 16, True),
+    ([50, 31], 2, 2, 1, 32, 16, 16, False),
+    ([77], 1, 3, 1, 16, 64, 16, False),
+    ([210, 33], 2, 2, 1, 80, 32, 16, False),                # int4 rows of 40 bytes
+    ([64, 19], 1, 4, 2, 72, 5, 8, True),                    # int8 rows of 72
 ]
 
 
