@@ -19,7 +19,7 @@ namespace skv {
 // Products on the FMA pipe from fp32 tiles in shared memory: 8 rows, 32 tokens at a time.  Thread = (token, rows w and
 // w + 4) for the scores, value d for the sums.  A warp widens 8 tokens a tile, a lane a value of each, so that 16 loads are on
 // their way; the lanes look up the tokens' rows one tile ahead.
-constexpr int kAnyRows = 8, kAnyTile = 32, kAnyThreads = 128, kAnyMaxD = 512, kAnyParts = 64;
+constexpr int kAnyRows = 8, kAnyTile = 32, kAnyThreads = 128, kAnyMaxD = 512, kAnyParts = 64, kAnyPad = 1;
 
 __host__ __device__ inline size_t any_smem(int D) {
     return ((size_t)kAnyRows * D + (size_t)kAnyTile * (D + 1) + (size_t)kAnyTile * D + kAnyRows * kAnyTile + kAnyRows +
@@ -39,11 +39,12 @@ __global__ void __launch_bounds__(kAnyThreads) pool_attention_any_kernel(const _
     float* sc = sp + kAnyRows * kAnyTile;
     float* sj = sc + kAnyRows;
     const int rep = a.q.heads / a.pool.heads, R = rep * a.S_q;
-    take_share<kAnyThreads>(a, kAnyTile, a.pool.heads * row_tiles, 2, &s);
+    take_share<kAnyThreads>(a, kAnyTile, a.pool.heads * row_tiles, kAnyPad, 2, &s);
     int b = s.b, base = s.base;
     for (int at = s.lo; at < s.hi;) {
         const Segment g = segment_at(a, s, at, kAnyTile, row_tiles, b, base);
-        at += g.t1 - g.t0;
+        at = g.next;
+        if (g.t0 >= g.t1) continue;
         const int r0 = g.rt * kAnyRows;
         __syncthreads();
         for (int i = tid; i < kAnyRows * D; i += kAnyThreads) {
@@ -240,7 +241,7 @@ int skv_pool_attention(const skv_pool_attention_args* args, void* stream) {
         return fail(SKV_ERR_UNSUPPORTED, "pool_attention: head_dim %d above %d", a.pool.head_dim, kAnyMaxD);
     if ((int64_t)a.q.heads * a.S_q > (1 << 28) || a.pool.batch > (1 << 24))
         return fail(SKV_ERR_TOO_LARGE, "pool_attention: too many rows");
-    const int64_t tiles = ((int64_t)a.pool.table_width * a.pool.page_size + kAnyTile - 1) / kAnyTile + 1;
+    const int64_t tiles = ((int64_t)a.pool.table_width * a.pool.page_size + kAnyTile - 1) / kAnyTile + 8;   // at least what a unit counts on top
     if (tiles * a.pool.batch > 0x7fffffff / ((int64_t)a.q.heads * a.S_q))   // row tiles hold one row at least
         return fail(SKV_ERR_TOO_LARGE, "pool_attention: more than 2^31 tiles of work");
     if (a.scratch_bytes < (int64_t)skv_pool_attention_scratch_bytes(a.pool.head_dim))

@@ -15,6 +15,7 @@ struct Share {
     int lo, hi, total;         // this CTA's tiles [lo, hi) of all
     int base;                  // tiles of the sequences before b
     int b;                     // the sequence that holds tile lo
+    int pad;                   // tiles that a unit costs on top of its own
     int each, more;            // a share is `each` tiles, one more for the first `more` CTAs
     __device__ __forceinline__ int first_of(int cta) const { return cta * each + min(cta, more); }
     __device__ __forceinline__ int owner_of(int tile) const {
@@ -29,16 +30,19 @@ __device__ __forceinline__ int seq_tokens(const skv_pool_attention_args& a, int 
 }
 // Tiles of a sequence for one row tile of one head; an empty sequence keeps one, to write its zeros.
 __device__ __forceinline__ int seq_tiles(int tokens, int tile) { return max(1, (tokens + tile - 1) / tile); }
+// A unit costs its tiles and what it takes to lay out its queries and to join its warps' sums, about as long as `pad` tiles
+// more: the shares count them as tiles behind the unit's own, in which nothing is done.  (Without them a CTA that got only
+// short sequences was the last by far: 32 int8 sequences of 1 to 4096 tokens took 68 us, with three tiles a unit 45.)
 
 // Every thread of the block calls this; *s is valid for all after it.  At least min_tiles a CTA.
 template <int THREADS>
-__device__ __forceinline__ void take_share(const skv_pool_attention_args& a, int tile, int units, int min_tiles,
+__device__ __forceinline__ void take_share(const skv_pool_attention_args& a, int tile, int units, int pad, int min_tiles,
                                            Share* s) {
     __shared__ int s_part[THREADS / 32];
     const int tid = threadIdx.x, lane = tid & 31, B = a.pool.batch;
     const int per = (B + THREADS - 1) / THREADS, b0 = min(B, tid * per), b1 = min(B, b0 + per);
     int mine = 0;
-    for (int b = b0; b < b1; ++b) mine += seq_tiles(seq_tokens(a, b), tile) * units;
+    for (int b = b0; b < b1; ++b) mine += (seq_tiles(seq_tokens(a, b), tile) + pad) * units;
     int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -59,6 +63,7 @@ __device__ __forceinline__ void take_share(const skv_pool_attention_args& a, int
     t.each = total / ctas;
     t.more = total - t.each * ctas;
     t.total = total;
+    t.pad = pad;
     const int c = blockIdx.x;
     t.lo = c < ctas ? t.first_of(c) : total;
     t.hi = c < ctas ? t.first_of(c + 1) : total;
@@ -67,7 +72,7 @@ __device__ __forceinline__ void take_share(const skv_pool_attention_args& a, int
     if (t.lo >= before && t.lo < before + mine) {   // one thread
         t.base = before;
         for (t.b = b0;; ++t.b) {
-            const int n = seq_tiles(seq_tokens(a, t.b), tile) * units;
+            const int n = (seq_tiles(seq_tokens(a, t.b), tile) + pad) * units;
             if (t.lo < t.base + n) break;
             t.base += n;
         }
@@ -87,7 +92,8 @@ __device__ __forceinline__ int seen_by(const skv_pool_attention_args& a, int b, 
 struct Segment {
     int b, hk, rt;             // unit
     int tokens;                // of the sequence
-    int t0, t1;                // its tiles [t0, t1) are this CTA's
+    int t0, t1;                // its tiles [t0, t1) are this CTA's (none: the share starts behind the unit's last)
+    int next;                  // the tile of the share behind them
     int first, last;           // global numbers of the unit's first and last tile
     bool whole;
     int slot;                  // partial slot of this CTA (0 or 1) if not whole
@@ -100,22 +106,23 @@ __device__ __forceinline__ Segment segment_at(const skv_pool_attention_args& a, 
     const int units = a.pool.heads * row_tiles;
     for (;;) {
         g.tokens = seq_tokens(a, b);
-        const int nt = seq_tiles(g.tokens, tile);
-        if (at < base + nt * units) {
-            const int u = (at - base) / nt;
+        const int nt = seq_tiles(g.tokens, tile), all = nt + s.pad;
+        if (at < base + all * units) {
+            const int u = (at - base) / all;
             g.b = b;
             g.hk = u / row_tiles;
             g.rt = u - g.hk * row_tiles;
-            g.first = base + u * nt;
+            g.first = base + u * all;
             g.last = g.first + nt - 1;
             g.t0 = at - g.first;
-            g.t1 = min(nt, g.t0 + (s.hi - at));
+            g.next = min(g.first + all, s.hi);
+            g.t1 = min(nt, g.next - g.first);
             g.whole = g.t0 == 0 && g.t1 == nt;
             g.slot = at == s.lo ? 0 : 1;
             if (a.error_flag && a.lengths[b] > g.tokens && threadIdx.x == 0) atomicExch(a.error_flag, 1);
             return g;
         }
-        base += nt * units;
+        base += all * units;
         ++b;
     }
 }

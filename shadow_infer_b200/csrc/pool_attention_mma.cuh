@@ -32,6 +32,7 @@
 
 namespace skv {
 
+constexpr int kMmaPad = 3, kMinTiles = 2;   // what a unit costs on top of its tiles, and the least that a CTA takes
 constexpr int kMmaParts = 64;       // parts whose factors a joining CTA holds at a time
 constexpr float kRefDrop = 5.0f;    // a fresh maximum's weight is 2^5: small weights keep their bits in fp16
 constexpr float kRefRoom = 14.0f;   // weights may grow to 2^14 (times a mantissa < 2) before ref moves
@@ -249,7 +250,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
     const int rep = a.q.heads / a.pool.heads, R = rep * a.S_q;
     const bool p16 = P % 16 == 0;   // a tile lies in one page
     auto page_of = [&](int t) { return (int)(((uint64_t)(uint32_t)t * magic.mul) >> magic.shift); };
-    take_share<THREADS>(a, TILE, a.pool.heads * row_tiles, 2, &s);
+    take_share<THREADS>(a, TILE, a.pool.heads * row_tiles, kMmaPad, kMinTiles, &s);
     if (s.lo >= s.hi) return;
     char* ring = s_ring + warp * S * L::BYTES;
     if (!exact) {   // chunks that the head does not have are never copied: they count as zero
@@ -280,7 +281,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                 return;
             }
             const Segment g = segment_at(a, s, f.at, TILE, row_tiles, f.b, f.base);
-            f.at += g.t1 - g.t0;
+            f.at = g.next;
             f.hk = g.hk;
             f.tokens = g.tokens;
             f.end = min(g.t1 * W, (g.tokens + 15) / 16);
@@ -373,7 +374,8 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
     int at = s.lo, b = s.b, base = s.base;
     while (at < s.hi) {
         const Segment g = segment_at(a, s, at, TILE, row_tiles, b, base);
-        at += g.t1 - g.t0;
+        at = g.next;
+        if (g.t0 >= g.t1) continue;
         const int n = g.tokens, r0 = g.rt * ROWS;
         // ---- queries: a power of two taken out of each row, laid out as B operands
         __syncthreads();
