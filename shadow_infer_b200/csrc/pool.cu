@@ -409,6 +409,7 @@ int launch_append(const skv_pool_append_args& a, cudaStream_t st) {
                aligned16(a.pool.k) && aligned16(a.pool.v) && aligned16(a.rope.cos) && aligned16(a.rope.sin);
     if (split) vec = vec && rot % 16 == 0 && (a.pool.precision != 3 || (G % 8 == 0 && power(G / 8) && rot / 2 % G == 0 && (D - rot) / 2 % G == 0));
     else vec = vec && rot % 8 == 0 && (a.pool.precision != 3 || G == 8 || (G % 16 == 0 && power(G / 16)));
+    vec = vec && H <= 65535;   // grid.y
     if (!vec) {
         const int64_t blocks = (tokens * H + kPoolWarps - 1) / kPoolWarps;
         pool_append_any_kernel<T><<<(unsigned)blocks, 32 * kPoolWarps, 0, st>>>(a);

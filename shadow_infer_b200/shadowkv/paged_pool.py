@@ -39,22 +39,24 @@ _READ = struct.Struct("<" + _POOL + _ROWS * 2 + "QQQii")
 _ATTENTION = struct.Struct("<" + _POOL + _ROWS * 2 + "QQQqQiifi")
 assert (_APPEND.size, _READ.size, _ATTENTION.size) == (336, 192, 216)
 _NO_ROPE = (0,) * 11
-_SCRATCH = {}   # (device, stream) -> attention scratch
+_SCRATCH = {}         # (device, stream) -> attention scratch
+_SCRATCH_BYTES = {}   # head_dim -> its size
 
 
 _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 
 
-def _scratch(dev: torch.device, stream: int) -> torch.Tensor:
+def _scratch(dev: torch.device, stream: int, head_dim: int) -> torch.Tensor:
     """The attention's scratch on a stream: partial results and arrival counters that every call leaves zero.  Calls
     of one stream follow each other, so they share one; a graph being captured gets its own."""
+    need = _SCRATCH_BYTES.get(head_dim)
+    if need is None:
+        need = _SCRATCH_BYTES[head_dim] = _lib.load().skv_pool_attention_scratch_bytes(head_dim)
     t = _SCRATCH.get((dev.index, stream))
     capturing = _capturing()
-    if t is None or capturing:
-        lib = _lib.load()
-        # sized for any head the kernels take, so that it is made once
-        t = torch.empty(lib.skv_pool_attention_scratch_bytes(512), dtype=torch.uint8, device=dev)
-        t[:lib.skv_pool_attention_scratch_zeros()].zero_()
+    if t is None or capturing or t.numel() < need:
+        t = torch.empty(need, dtype=torch.uint8, device=dev)
+        t[:_lib.load().skv_pool_attention_scratch_zeros()].zero_()
         if not capturing:
             _SCRATCH[dev.index, stream] = t
     return t
@@ -276,7 +278,7 @@ def paged_attention(
     entry = _lib.load().skv_pool_attention
     with device_ctx(dev):
         stream = _lib.stream_of(dev)
-        scratch = _scratch(dev, stream)
+        scratch = _scratch(dev, stream, D)
         args = _ATTENTION.pack(*pool, *q_rows, *out_rows, lens.data_ptr(), 0 if new is None else new.data_ptr(),
                                scratch.data_ptr(), scratch.numel(), 0 if flag is None else flag.data_ptr(), S_q, bool(causal),
                                1.0 / math.sqrt(D) if scale is None else scale, 0)
