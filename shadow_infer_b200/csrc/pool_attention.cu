@@ -198,6 +198,7 @@ int launch_any(const skv_pool_attention_args& a, cudaStream_t st) {
 }
 
 // The tensor-core kernels (pool_attention_mma.cuh), one translation unit a precision.
+int attend_fp32(const skv_pool_attention_args& a, cudaStream_t st);
 int attend_fp16(const skv_pool_attention_args& a, cudaStream_t st);
 int attend_int8(const skv_pool_attention_args& a, cudaStream_t st);
 int attend_int4(const skv_pool_attention_args& a, cudaStream_t st);
@@ -207,7 +208,7 @@ int attend_int4(const skv_pool_attention_args& a, cudaStream_t st);
 bool fits_mma(const skv_pool& p) {
     const int D = p.head_dim;
     const int64_t rows = (int64_t)p.num_pages * p.heads * p.page_size;
-    if (rows == 0 || rows > 0x7fffffff || p.precision == 0 || D > 256) return false;
+    if (rows == 0 || rows > 0x7fffffff || D > 256) return false;
     if (D % (p.precision == 3 ? 16 : 8) || (p.precision == 3 && p.int4_group % 16)) return false;
     return ((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v)) & 15) == 0;
 }
@@ -248,7 +249,7 @@ int skv_pool_attention(const skv_pool_attention_args* args, void* stream) {
         return fail(SKV_ERR_SCRATCH, "pool_attention: scratch of %lld bytes", (long long)a.scratch_bytes);
     cudaStream_t st = as_stream(stream);
     if (fits_mma(a.pool))
-        return a.pool.precision == 1 ? attend_fp16(a, st) : a.pool.precision == 2 ? attend_int8(a, st) : attend_int4(a, st);
+        return a.pool.precision == 0 ? attend_fp32(a, st) : a.pool.precision == 1 ? attend_fp16(a, st) : a.pool.precision == 2 ? attend_int8(a, st) : attend_int4(a, st);
     if (a.q.dtype == kF32) return launch_any<float>(a, st);
     if (a.q.dtype == kF16) return launch_any<__half>(a, st);
     return launch_any<__nv_bfloat16>(a, st);

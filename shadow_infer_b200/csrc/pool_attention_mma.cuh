@@ -48,10 +48,24 @@ __device__ __forceinline__ void mma16816_from(float (&c)[4], const uint32_t (&a)
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y), "f"(c0), "f"(c1));
 }
+// c += a b of tf32 operands (fp32 bits whose lower 13 do not count), 16 x 8 by 8 x 8.
+__device__ __forceinline__ void mma1688(float (&c)[4], const uint32_t (&a)[4], uint2 b) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
+}
+// The first 11 significant bits of x, cut off or rounded.  (Rounding hides a NaN of all ones, which what is left then shows.)
+__device__ __forceinline__ uint32_t tf32_cut(float x) { return __float_as_uint(x) & 0xFFFFE000u; }
+__device__ __forceinline__ uint32_t tf32_round(float x) { return (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u; }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
+}
+// Two columns of an 8 x 8 matrix of 32-bit words, 16 bits at a time: of the result's row, columns 2c and 2c + 1.
+__device__ __forceinline__ uint2 transpose8x8(uint32_t x, uint32_t y) {
+    const uint32_t lo = transpose8x8(__byte_perm(x, y, 0x5410)), hi = transpose8x8(__byte_perm(x, y, 0x7632));
+    return make_uint2(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
 }
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;
@@ -166,9 +180,14 @@ __device__ __forceinline__ void load_row(const T* p, int left, bool vec, float (
 }
 
 // Where value d of a query row sits in the B operands (MMA, lane column c, register and half), and what it is
-// multiplied by there: the high nibbles of int4 bytes are read as 16 (n + 8).
-template <int PREC, int DP>
+// multiplied by there: the high nibbles of int4 bytes are read as 16 (n + 8) (32-bit queries: both as 64 (n + 8)).
+template <int PREC, int DP, int NQ>
 __device__ __forceinline__ float query_place(int d, int& mma, int& c, int& reg, int& half) {
+    if (PREC == 0) {   // lane column c reads every second chunk of 4 values
+        const int chunk = d / 4;
+        mma = 2 * (2 * (chunk / 8) + chunk % 2) + d % 4 / 2; c = chunk % 8 / 2; reg = d % 2; half = 0;
+        return 1.0f;
+    }
     if (PREC == 1) {   // ldmatrix order
         mma = d / 16; c = (d % 8) / 2; reg = (d % 16) / 8; half = d % 2;
         return 1.0f;
@@ -181,17 +200,21 @@ __device__ __forceinline__ float query_place(int d, int& mma, int& c, int& reg, 
         return 1.0f;
     }
     mma = d / 16; c = (d % 16) / 4;
-    return r % 2 ? 1.0f : 0.0625f;
+    return NQ == 2 || r % 2 ? 1.0f : 0.0625f;
 }
-constexpr float kSubnormal = 5.9604644775390625e-08f;   // 2^-24: an fp16 whose bits are m has the value m 2^-24
+// An fp16 whose bits are m < 1024 has the value m 2^-24.  The tensor cores align a product by its factors' exponent fields, so
+// a small m loses as many of the sum's last bits as it has leading zeros: for 32-bit queries int4 values are moved up to m's top
+// (without that the output was 1.2e-6 off, with it 3e-7; an int8 value has 8 of the 10 bits).
+template <int PREC, int NQ>
+__host__ __device__ constexpr float subnormal_unit() { return PREC == 3 && NQ == 2 ? 3.814697265625e-06f : 5.9604644775390625e-08f; }
 template <int PREC, int DP>
 __host__ __device__ constexpr int bias_blocks() { return PREC == 3 ? DP / 16 : 1; }
 
 // A slot: 16 rows of K and of V, their scales (int4: one for each 16 values), and the tokens' pool rows.
 template <int PREC, int DP>
 struct Slot {
-    static constexpr int ROW = PREC == 1 ? 2 * DP : PREC == 2 ? DP : DP / 2, CHUNKS = ROW / 16, BLOCKS = DP / 16;
-    static constexpr int SCALES = PREC == 1 ? 0 : PREC == 2 ? 1 : BLOCKS;   // a token
+    static constexpr int ROW = PREC == 0 ? 4 * DP : PREC == 1 ? 2 * DP : PREC == 2 ? DP : DP / 2, CHUNKS = ROW / 16, BLOCKS = DP / 16;
+    static constexpr int SCALES = PREC <= 1 ? 0 : PREC == 2 ? 1 : BLOCKS;   // a token
     static constexpr int K = 0, V = 16 * ROW, SK = 2 * V, SV = SK + 64 * SCALES, ID = SV + 64 * SCALES, USED = ID + 64;
     static constexpr int MERGE = 8 * (DP + 4) * 4;   // the warp's sums of 8 rows pass through a free slot
     static constexpr int BYTES = ((USED > MERGE ? USED : MERGE) + 127) & ~127;   // lines stay on 128-byte boundaries
@@ -213,15 +236,16 @@ template <int PREC, int DP, int NT>
 struct MmaShape {
     // Warps a CTA, CTAs an SM, slots a warp: what 64 K registers and 227 KB of shared memory hold, with at least 60 KB of
     // rows on their way (HBM's latency times its rate is about 43 KB an SM).
-    static constexpr int W = PREC >= 2 && (NT == 1 || DP == 256) ? 8 : 4;
-    static constexpr int CTAS = DP == 256 ? 1 : NT == 2 ? (PREC == 1 ? 2 : 3) : PREC == 1 ? 3 : 2;
+    static constexpr int W = PREC == 0 ? 512 / DP : PREC >= 2 && (NT == 1 || DP == 256) ? 8 : 4;
+    static constexpr int CTAS = PREC == 0 || DP == 256 ? 1 : NT == 2 ? (PREC == 1 ? 2 : 3) : PREC == 1 ? 3 : 2;
     static constexpr int SLOTS = PREC == 1 && DP < 256 ? 2 : 3;
+    static constexpr int MQ = PREC == 0 ? DP / 8 : DP / 16;   // MMAs that a tile's scores take a term
 };
 
 template <int PREC, int DP, int NT, int NQ>
 __host__ __device__ constexpr size_t mma_smem() {
     constexpr int W = MmaShape<PREC, DP, NT>::W, ROWS = 8 * NT;
-    return (size_t)W * MmaShape<PREC, DP, NT>::SLOTS * Slot<PREC, DP>::BYTES + (size_t)(DP / 16) * NT * NQ * 32 * 8 +
+    return (size_t)W * MmaShape<PREC, DP, NT>::SLOTS * Slot<PREC, DP>::BYTES + (size_t)MmaShape<PREC, DP, NT>::MQ * NT * NQ * 32 * 8 +
            (join_floats<ROWS, 32 * W, kMmaParts>() + (3 * W + 2 + bias_blocks<PREC, DP>()) * ROWS) * 4;
 }
 
@@ -231,14 +255,14 @@ __global__ void __launch_bounds__(32 * MmaShape<PREC, DP, NT>::W, MmaShape<PREC,
 pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int row_tiles, PageDivide magic, bool exact, bool q_vec,
                           bool out_vec) {
     using L = Slot<PREC, DP>;
-    constexpr int M = DP / 16, ROWS = 8 * NT, W = MmaShape<PREC, DP, NT>::W, S = MmaShape<PREC, DP, NT>::SLOTS;
+    constexpr int M = DP / 16, MQ = MmaShape<PREC, DP, NT>::MQ, ROWS = 8 * NT, W = MmaShape<PREC, DP, NT>::W, S = MmaShape<PREC, DP, NT>::SLOTS;
     constexpr int THREADS = 32 * W, TILE = 16 * W;
     extern __shared__ __align__(128) char mma_sm[];
     __shared__ Share s;
     __shared__ int s_free[W];
     char* s_ring = mma_sm;                                                       // [W][S] slots
-    uint2* s_q = reinterpret_cast<uint2*>(s_ring + W * S * L::BYTES);            // [M][NT][NQ][32]
-    float* s_join = reinterpret_cast<float*>(s_q + M * NT * NQ * 32);
+    uint2* s_q = reinterpret_cast<uint2*>(s_ring + W * S * L::BYTES);            // [MQ][NT][NQ][32]
+    float* s_join = reinterpret_cast<float*>(s_q + MQ * NT * NQ * 32);
     float* s_ref = s_join + join_floats<ROWS, THREADS, kMmaParts>();             // [W][ROWS]
     float* s_sum = s_ref + W * ROWS;                                             // [W][ROWS]
     float* s_w = s_sum + W * ROWS;                                               // [W][ROWS]
@@ -268,8 +292,9 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
     f.base = s.base;
     f.st = f.end = f.hk = f.tokens = 0;
     PageRows pages;
-    const int row_bytes = PREC == 1 ? 2 * D : PREC == 2 ? D : D / 2;
-    constexpr int STEP = 32 / L::CHUNKS, COPIES = 16 / STEP;   // rows a warp's copy takes, copies a tile takes
+    const int row_bytes = PREC == 0 ? 4 * D : PREC == 1 ? 2 * D : PREC == 2 ? D : D / 2;
+    constexpr int WIDE = L::CHUNKS > 32 ? L::CHUNKS / 32 : 1;   // copies a row takes
+    constexpr int STEP = 32 * WIDE / L::CHUNKS, COPIES = 16 / STEP;   // rows a warp's copy takes, copies a tile takes
     const int my_row = lane / L::CHUNKS, my_chunk = lane % L::CHUNKS;
     const char* k_lane = static_cast<const char*>(a.pool.k) + my_chunk * 16;
     const char* v_lane = static_cast<const char*>(a.pool.v) + my_chunk * 16;
@@ -312,19 +337,24 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
 #pragma unroll
             for (int i = 0; i < COPIES; ++i) {
                 const uint32_t y = L::step(to_rows, i, STEP);
-                copy_async<16>(y, k + i * STEP * L::ROW);
-                copy_async<16>(y + L::V, v + i * STEP * L::ROW);
+#pragma unroll
+                for (int h = 0; h < WIDE; ++h) {   // 512 bytes on, a chunk has the same place in its line
+                    copy_async<16>(y + 512 * h, k + i * STEP * L::ROW + 512 * h);
+                    copy_async<16>(y + 512 * h + L::V, v + i * STEP * L::ROW + 512 * h);
+                }
             }
         } else {
 #pragma unroll
             for (int i = 0; i < COPIES; ++i) {
                 const int r = p16 ? first + my_row + i * STEP : max(__shfl_sync(0xffffffffu, row, my_row + i * STEP), 0);
                 const uint32_t y = L::step(to_rows, i, STEP);
-                if (PREC == 1 || row_bytes % 16 == 0) {
-                    if (my_chunk * 16 < row_bytes) {
-                        copy_async<16>(y, k_lane + (int64_t)r * row_bytes);
-                        copy_async<16>(y + L::V, v_lane + (int64_t)r * row_bytes);
-                    }
+                if (PREC <= 1 || row_bytes % 16 == 0) {
+#pragma unroll
+                    for (int h = 0; h < WIDE; ++h)
+                        if (my_chunk * 16 + 512 * h < row_bytes) {
+                            copy_async<16>(y + 512 * h, k_lane + (int64_t)r * row_bytes + 512 * h);
+                            copy_async<16>(y + 512 * h + L::V, v_lane + (int64_t)r * row_bytes + 512 * h);
+                        }
                 } else {   // rows end in half a chunk, and every second one starts in the middle of 16 bytes
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
@@ -401,13 +431,19 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                 for (int k = 0; k < E; ++k) top = fmaxf(top, fabsf(x[i][k]));
                 const int e = clamp_exp(__float_as_uint(warp_max(top)));
                 const float down = exp_down(e, kQueryExp);
-                if (lane == 0) s_c[j] = a.scale * 1.4426950408889634f * exp_up(e, kQueryExp) * (PREC == 1 ? 1.0f : 1.0f / kSubnormal);
+                if (lane == 0) s_c[j] = a.scale * 1.4426950408889634f * exp_up(e, kQueryExp) * (PREC <= 1 ? 1.0f : 1.0f / subnormal_unit<PREC, NQ>());
                 float total = 0.0f;
 #pragma unroll
                 for (int k = 0; k < E; ++k) {
                     int mma, c, reg, half;
-                    const float part = query_place<PREC, DP>(lane * E + k, mma, c, reg, half);
+                    const float part = query_place<PREC, DP, NQ>(lane * E + k, mma, c, reg, half);
                     const float y = x[i][k] * down * part;
+                    if constexpr (PREC == 0) {
+                        uint32_t* q = reinterpret_cast<uint32_t*>(s_q + ((mma * NT + j / 8) * NQ) * 32 + (j % 8) * 4 + c) + reg;
+                        q[0] = NQ == 1 ? tf32_cut(y) : tf32_round(y);   // all of it where the query has 16 bits
+                        if (NQ == 2) q[32 * 2] = __float_as_uint(y - __uint_as_float(tf32_round(y)));
+                        continue;
+                    }
                     const __half hi = __float2half_rn(y);
                     __half* q = reinterpret_cast<__half*>(s_q + ((mma * NT + j / 8) * NQ) * 32 + (j % 8) * 4 + c) + 2 * reg + half;
                     q[0] = hi;
@@ -423,7 +459,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                     constexpr int LANES = PREC == 2 ? 32 : 16 / E;   // that share a bias
 #pragma unroll
                     for (int w = 1; w < LANES; w <<= 1) total += __shfl_xor_sync(0xffffffffu, total, w);
-                    if (lane % LANES == 0) s_bias[lane / LANES * ROWS + j] = total * ((PREC == 2 ? -128.0f : -8.0f) * kSubnormal);
+                    if (lane % LANES == 0) s_bias[lane / LANES * ROWS + j] = total * ((PREC == 2 ? -128.0f : -8.0f) * subnormal_unit<PREC, NQ>());
                 }
             }
         }
@@ -470,7 +506,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                 for (int i = 0; i < 2; ++i) here[i] = __shfl_sync(0xffffffffu, (int)held, lg + 8 * i);
                 // a weight of zero would not hide a NaN in what an absent token's row or scale happens to hold
                 if (!held && lane < 16) {
-                    if constexpr (PREC == 1)
+                    if constexpr (PREC <= 1)
                         for (int i = 0; i < L::CHUNKS; ++i) *reinterpret_cast<uint4*>(slot + L::V + lane * L::ROW + i * 16) = make_uint4(0, 0, 0, 0);
                     else
                         for (int i = 0; i < L::SCALES; ++i) reinterpret_cast<float*>(slot + L::SV)[lane * L::SCALES + i] = 1.0f;
@@ -495,7 +531,47 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                             else mma16816(acc[h][t], f, bq);
                         }
                 };
-                if constexpr (PREC == 1) {
+                if constexpr (PREC == 0) {
+                    // high part times the query's first term; the terms 2^-12 of that (low times first, high times second)
+                    // have a chain of their own, where an MMA cuts off less
+                    float small[NT][4];
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            small[t][i] = 0.0f;
+#pragma unroll
+                            for (int h = 0; h < CH; ++h) acc[h][t][i] = 0.0f;
+                        }
+#pragma unroll
+                    for (int j = 0; j < DP / 16; ++j) {
+                        const int ch = 8 * (j / 2) + 2 * lc + j % 2;
+                        const float4 u = *reinterpret_cast<const float4*>(slot + L::K + L::at(lg, ch));
+                        const float4 v = *reinterpret_cast<const float4*>(slot + L::K + L::at(lg + 8, ch));
+                        const float y[2][4] = {{u.x, v.x, u.y, v.y}, {u.z, v.z, u.w, v.w}};
+#pragma unroll
+                        for (int w = 0; w < 2; ++w) {
+                            const int m = 2 * j + w;
+                            uint32_t hi[4], lo[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                hi[i] = tf32_round(y[w][i]);
+                                lo[i] = __float_as_uint(y[w][i] - __uint_as_float(hi[i]));
+                            }
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) {
+                                const uint2 bq = s_q[(m * NT + t) * NQ * 32 + lane];
+                                mma1688(acc[m % CH][t], hi, bq);
+                                mma1688(small[t], lo, bq);
+                                if constexpr (NQ == 2) mma1688(small[t], hi, s_q[((m * NT + t) * NQ + 1) * 32 + lane]);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[0][t][i] += small[t][i];
+                } else if constexpr (PREC == 1) {
                     const uint32_t k = shared_address(slot + L::K);
 #pragma unroll
                     for (int m = 0; m < M; ++m) {
@@ -550,8 +626,12 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const int m = k + M / 2 * h;
+                        constexpr uint32_t mask = 0x03C003C0u;
                         const uint32_t uh = u >> (8 * h), vh = v >> (8 * h);
-                        const uint32_t f[4] = {uh & 0x00F000F0u, vh & 0x00F000F0u, uh & 0x000F000Fu, vh & 0x000F000Fu};
+                        const uint32_t f[4] = {NQ == 2 ? (h ? u >> 6 : u << 2) & mask : uh & 0x00F000F0u,
+                                               NQ == 2 ? (h ? v >> 6 : v << 2) & mask : vh & 0x00F000F0u,
+                                               NQ == 2 ? (h ? u >> 2 : u << 6) & mask : uh & 0x000F000Fu,
+                                               NQ == 2 ? (h ? v >> 2 : v << 6) & mask : vh & 0x000F000Fu};
 #pragma unroll
                         for (int t = 0; t < NT; ++t) {
                             float acc[4];
@@ -629,7 +709,8 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                         }
                     }
             }
-            uint2 p[NT][NP];
+            uint2 p[NT][NP];   // (PREC 0: of tokens 0 to 7, and in p8 of 8 to 15)
+            uint2 p8[NT][NP];
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 float w[4];
@@ -639,6 +720,20 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                     const float y = fast_exp2(x[t][i] - base_of[t][col]);
                     sum[t][col] = PREC >= 2 ? fmaf(y, v_sum[tok], sum[t][col]) : sum[t][col] + y;
                     w[i] = PREC == 2 ? y * v_mul[tok] : y;
+                }
+                if constexpr (PREC == 0) {   // (a NaN that rounding would hide is in the sum)
+#pragma unroll
+                    for (int k = 0; k < NP; ++k) {
+                        uint32_t r[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            r[i] = tf32_round(w[i]);
+                            w[i] -= __uint_as_float(r[i]);
+                        }
+                        p[t][k] = transpose8x8(r[0], r[1]);
+                        p8[t][k] = transpose8x8(r[2], r[3]);
+                    }
+                    continue;
                 }
                 const uint32_t lo = h2_pack(w[0], w[1]), hi = h2_pack(w[2], w[3]);
                 p[t][0] = make_uint2(transpose8x8(lo), transpose8x8(hi));
@@ -650,20 +745,73 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                 }
             }
             // ---- values
-            auto pv = [&](const uint32_t (&f)[4], int m, int terms) {
+            // An MMA cuts its sum off where an addition would round: a relative 2^-24 of the sums is lost with each on average,
+            // all in one direction.  32-bit outputs add a tile's own sums to those before instead (256 tiles a warp cost
+            // 3e-5 of the result; 16-bit outputs, whose rounding is 100 times that, let the MMAs add).
+            constexpr bool kFresh = NQ == 2;
+            float fresh[NT][4];
+            auto pv = [&](const uint32_t (&f)[4], int m, int terms, bool first, bool last) {
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
+                for (int t = 0; t < NT; ++t) {
 #pragma unroll
-                    for (int q = 0; q < NP; ++q)
-                        if (q < terms) mma16816(o[t][m], f, p[t][q]);
+                    for (int i = 0; i < NP; ++i) {
+                        const int q = kFresh ? NP - 1 - i : i;   // the small term first
+                        if (q >= terms) continue;
+                        if (!kFresh) mma16816(o[t][m], f, p[t][q]);
+                        else if (first && q == terms - 1) mma16816_from(fresh[t], f, p[t][q], 0.0f, 0.0f);
+                        else mma16816(fresh[t], f, p[t][q]);
+                    }
+                    if (kFresh && last)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[t][m][i] += fresh[t][i];
+                }
             };
-            if constexpr (PREC == 1) {
+            if constexpr (PREC == 0) {
+#pragma unroll
+                for (int j = 0; j < DP / 32; ++j) {
+                    float4 y[2][2];   // tokens 8 h + 2 c and the next, values 4 (8 j + g) ..
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            y[h][i] = *reinterpret_cast<const float4*>(slot + L::V + L::at(8 * h + 2 * lc + i, 8 * j + lg));
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        float acc[NT][4];
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) acc[t][i] = kFresh ? 0.0f : o[t][2 * j + w][i];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float z[4] = {w ? y[h][0].z : y[h][0].x, w ? y[h][0].w : y[h][0].y,
+                                                w ? y[h][1].z : y[h][1].x, w ? y[h][1].w : y[h][1].y};
+                            uint32_t hi[4], lo[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                hi[i] = tf32_round(z[i]);
+                                lo[i] = __float_as_uint(z[i] - __uint_as_float(hi[i]));
+                            }
+#pragma unroll
+                            for (int t = 0; t < NT; ++t) {
+                                mma1688(acc[t], lo, h ? p8[t][0] : p[t][0]);
+                                if constexpr (NP == 2) mma1688(acc[t], hi, h ? p8[t][1] : p[t][1]);
+                                mma1688(acc[t], hi, h ? p8[t][0] : p[t][0]);
+                            }
+                        }
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[t][2 * j + w][i] = kFresh ? o[t][2 * j + w][i] + acc[t][i] : acc[t][i];
+                    }
+                }
+            } else if constexpr (PREC == 1) {
                 const uint32_t v = shared_address(slot + L::V);
 #pragma unroll
                 for (int m = 0; m < M; ++m) {
                     uint32_t f[4];
                     load_matrix_trans(f, v + L::at((lane & 7) + (lane >> 4) * 8, 2 * m + ((lane >> 3) & 1)));
-                    pv(f, m, NP);
+                    pv(f, m, NP, true, true);
                 }
             } else if constexpr (PREC == 2) {
                 uint32_t vx[4][DP / 32];   // values DP/8 g .. of tokens 2c, 2c + 1, 2c + 8, 2c + 9
@@ -694,7 +842,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                     for (int i = 0; i < 2; ++i) {
                         const uint32_t f[4] = {i8_pair(y[0][i], 0x4140), i8_pair(y[0][i], 0x4342),
                                                i8_pair(y[1][i], 0x4140), i8_pair(y[1][i], 0x4342)};
-                        pv(f, 2 * w + i, NP);
+                        pv(f, 2 * w + i, NP, true, true);
                     }
                 }
             } else {
@@ -742,10 +890,11 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                             const uint32_t f[4] = {i4_pair(h ? u >> 8 : u), i4_pair(h ? u >> 4 : u << 4),
                                                    i4_pair(h ? v >> 8 : v), i4_pair(h ? v >> 4 : v << 4)};
 #pragma unroll
-                            for (int k = 0; k < PARTS; ++k) {
+                            for (int n = 0; n < PARTS; ++n) {
+                                const int k = kFresh ? PARTS - 1 - n : n;
                                 const uint32_t y[4] = {h2_fma(f[0], r[k][0], r72[k][0]), h2_fma(f[1], r[k][0], r72[k][0]),
                                                        h2_fma(f[2], r[k][1], r72[k][1]), h2_fma(f[3], r[k][1], r72[k][1])};
-                                pv(y, 4 * w + 2 * i + h, k == 0 ? NP : 1);
+                                pv(y, 4 * w + 2 * i + h, k == 0 || k < PARTS - 1 ? NP : 1, k == PARTS - 1, k == 0);
                             }
                         }
                     }
@@ -779,7 +928,9 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                 float* row = mine + (2 * lc + i) * (DP + 4);
 #pragma unroll
                 for (int m = 0; m < M; ++m) {
-                    if constexpr (PREC == 1) {
+                    if constexpr (PREC == 0) {
+                        *reinterpret_cast<float2*>(row + 32 * (m / 2) + 4 * lg + 2 * (m % 2)) = make_float2(o[t][m][i], o[t][m][i + 2]);
+                    } else if constexpr (PREC == 1) {
                         row[16 * m + lg] = o[t][m][i];
                         row[16 * m + 8 + lg] = o[t][m][i + 2];
                     } else {
@@ -877,7 +1028,8 @@ int launch_mma_prec(const skv_pool_attention_args& a, cudaStream_t st) {
     const int R = a.q.heads / a.pool.heads * a.S_q, D = a.pool.head_dim;
     if (D <= 64) return R <= 8 ? launch_mma_type<PREC, 64, 1>(a, st) : launch_mma_type<PREC, 64, 2>(a, st);
     if (D <= 128) return R <= 8 ? launch_mma_type<PREC, 128, 1>(a, st) : launch_mma_type<PREC, 128, 2>(a, st);
-    return R <= 8 ? launch_mma_type<PREC, 256, 1>(a, st) : launch_mma_type<PREC, 256, 2>(a, st);
+    if constexpr (PREC == 0) return launch_mma_type<0, 256, 1>(a, st);   // slots of 32 KB leave no room for more rows
+    else return R <= 8 ? launch_mma_type<PREC, 256, 1>(a, st) : launch_mma_type<PREC, 256, 2>(a, st);
 }
 
 }  // namespace skv
