@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kAnyThreads) pool_attention_any_kernel(const _
             part[kAnyRows * D + tid] = sp[kAnyRows + tid];
             part[kAnyRows * D + kAnyRows + tid] = sp[tid];
         }
-        if (arrive(a, s, g)) join<kAnyRows, kAnyThreads, 1, kAnyParts>(a, s, g, R, sj);
+        if (arrive(a, s, g)) join<kAnyRows, kAnyThreads, 1, kAnyParts>(a, s, g, r0, min(kAnyRows, R - r0), sj);
     }
 }
 
@@ -203,6 +203,9 @@ int attend_fp16(const skv_pool_attention_args& a, cudaStream_t st);
 int attend_int8(const skv_pool_attention_args& a, cudaStream_t st);
 int attend_int4(const skv_pool_attention_args& a, cudaStream_t st);
 
+// The tcgen05 kernel (pool_attention_tc.cuh).
+int attend_many(const skv_pool_attention_args& a, cudaStream_t st);
+
 // They need heads of up to 256 values in rows of whole 16-byte (fp16) or 8-byte chunks, int4 groups of whole 16-value blocks,
 // payloads on 16-byte boundaries, a row 0, and row numbers of 31 bits.
 bool fits_mma(const skv_pool& p) {
@@ -211,6 +214,18 @@ bool fits_mma(const skv_pool& p) {
     if (rows == 0 || rows > 0x7fffffff || D > 256) return false;
     if (D % (p.precision == 3 ? 16 : 8) || (p.precision == 3 && p.int4_group % 16)) return false;
     return ((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v)) & 15) == 0;
+}
+
+// The tcgen05 kernel takes fp16 and int8 pages whose values are exact in fp16, 16-bit queries (32-bit ones want sums that the
+// tensor cores do not cut off), heads of up to 128 values in whole swizzled chunks of 16.  It is taken where its units fill
+// three quarters of the SMs: with fewer, long sequences are cut into parts whose joining (128 rows each) costs more than the
+// MMAs save.  8 key heads of 4 query heads over fp16 pages, us here and on the small kernel: one prompt of 4096 tokens 314 / 1720,
+// of 1024 74 / 155, of 512 (128 units) 59 / 66; 128 new tokens of one sequence of 2048 (32 units) 72 / 45.
+bool fits_tc(const skv_pool_attention_args& a) {
+    const int rep = a.q.heads / a.pool.heads;
+    const int64_t tiles = a.S_q >= 128 ? (int64_t)rep * ((a.S_q + 127) / 128) : ((int64_t)rep * a.S_q + 127) / 128;
+    return rep * (int64_t)a.S_q >= 64 && a.pool.batch * tiles * a.pool.heads * 4 >= sm_count() * 3 && a.q.dtype != kF32 && (a.pool.precision == 1 || a.pool.precision == 2) && a.pool.head_dim <= 128 &&
+           a.pool.head_dim % 16 == 0 && rows_aligned(a.q);
 }
 
 }  // namespace skv
@@ -248,6 +263,7 @@ int skv_pool_attention(const skv_pool_attention_args* args, void* stream) {
     if (a.scratch_bytes < (int64_t)skv_pool_attention_scratch_bytes(a.pool.head_dim))
         return fail(SKV_ERR_SCRATCH, "pool_attention: scratch of %lld bytes", (long long)a.scratch_bytes);
     cudaStream_t st = as_stream(stream);
+    if (fits_mma(a.pool) && fits_tc(a)) return attend_many(a, st);
     if (fits_mma(a.pool))
         return a.pool.precision == 0 ? attend_fp32(a, st) : a.pool.precision == 1 ? attend_fp16(a, st) : a.pool.precision == 2 ? attend_int8(a, st) : attend_int4(a, st);
     if (a.q.dtype == kF32) return launch_any<float>(a, st);

@@ -7,7 +7,7 @@
 namespace skv {
 
 constexpr int kMaxCtas = 4096;      // arrival counters in the scratch
-constexpr int kRowsPerSm = 128;     // rows of partial results in the scratch for each SM: CTAs x 2 slots x rows
+constexpr int kRowsPerSm = 512;     // rows of partial results in the scratch for each SM: CTAs x 2 slots x rows
 
 // ------------------------------------------------------------------------------ shares of the work
 // Tile numbers fit 31 bits (the launch checks the most that the table allows).
@@ -35,14 +35,14 @@ __device__ __forceinline__ int seq_tiles(int tokens, int tile) { return max(1, (
 // short sequences was the last by far: 32 int8 sequences of 1 to 4096 tokens took 68 us, with three tiles a unit 45.)
 
 // Every thread of the block calls this; *s is valid for all after it.  At least min_tiles a CTA.
-template <int THREADS>
-__device__ __forceinline__ void take_share(const skv_pool_attention_args& a, int tile, int units, int pad, int min_tiles,
-                                           Share* s) {
+// cost(b): the tiles of sequence b's units, with what each counts on top.
+template <int THREADS, class Cost>
+__device__ __forceinline__ void take_share(const skv_pool_attention_args& a, Cost cost, int pad, int min_tiles, Share* s) {
     __shared__ int s_part[THREADS / 32];
     const int tid = threadIdx.x, lane = tid & 31, B = a.pool.batch;
     const int per = (B + THREADS - 1) / THREADS, b0 = min(B, tid * per), b1 = min(B, b0 + per);
     int mine = 0;
-    for (int b = b0; b < b1; ++b) mine += (seq_tiles(seq_tokens(a, b), tile) + pad) * units;
+    for (int b = b0; b < b1; ++b) mine += cost(b);
     int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -72,7 +72,7 @@ __device__ __forceinline__ void take_share(const skv_pool_attention_args& a, int
     if (t.lo >= before && t.lo < before + mine) {   // one thread
         t.base = before;
         for (t.b = b0;; ++t.b) {
-            const int n = (seq_tiles(seq_tokens(a, t.b), tile) + pad) * units;
+            const int n = cost(t.b);
             if (t.lo < t.base + n) break;
             t.base += n;
         }
@@ -81,6 +81,13 @@ __device__ __forceinline__ void take_share(const skv_pool_attention_args& a, int
         *s = t;
     }
     __syncthreads();
+}
+
+// The same for units that all see their whole sequence.
+template <int THREADS>
+__device__ __forceinline__ void take_share(const skv_pool_attention_args& a, int tile, int units, int pad, int min_tiles,
+                                           Share* s) {
+    take_share<THREADS>(a, [&](int b) { return (seq_tiles(seq_tokens(a, b), tile) + pad) * units; }, pad, min_tiles, s);
 }
 
 // Tokens [0, n) of its sequence that query i of sequence b sees.
@@ -136,11 +143,21 @@ __device__ __forceinline__ float* slot_of(const skv_pool_attention_args& a, int 
            ((int64_t)2 * cta + slot) * rows * (a.pool.head_dim + 2);
 }
 
-// Called by all threads once the CTA's part is in its slot; true for the CTA that joins.  The barrier puts
+// The threads that publish and join: the whole block, or the first THREADS of it.
+struct BlockSync {
+    __device__ static __forceinline__ void sync() { __syncthreads(); }
+};
+template <int THREADS>
+struct FirstThreadsSync {
+    __device__ static __forceinline__ void sync() { asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory"); }
+};
+
+// Called by all of them once the CTA's part is in its slot; true for the CTA that joins.  The barrier puts
 // every thread's stores before thread 0's fence, which puts them before its arrival.
+template <class Sync = BlockSync>
 __device__ __forceinline__ bool arrive(const skv_pool_attention_args& a, const Share& s, const Segment& g) {
     __shared__ int s_last;
-    __syncthreads();
+    Sync::sync();
     if (threadIdx.x == 0) {
         __threadfence();
         const int c0 = s.owner_of(g.first), c1 = s.owner_of(g.last);
@@ -149,7 +166,7 @@ __device__ __forceinline__ bool arrive(const skv_pool_attention_args& a, const S
         if (s_last) *count = 0;
         __threadfence();
     }
-    __syncthreads();
+    Sync::sync();
     return s_last;
 }
 
@@ -212,14 +229,14 @@ __device__ __forceinline__ void load_part(const float* p, float (&x)[VEC]) {
 // other, so loads are issued in batches of 16 a thread: first the maxima and sums of all parts (THREADS / ROWS
 // threads a row), which leave the parts' factors in shared memory, then the values, VEC to a load.  Where
 // the rows have fewer loads than the block has threads, `ways` threads take every ways-th part of a value, and
-// their sums are added in order.  buf: join_floats of shared memory.
+// their sums are added in order.  r0, rows: the unit's query rows.  buf: join_floats of shared memory.
 constexpr int kJoinWays = 8;
 template <int ROWS, int THREADS, int PARTS>
 __host__ __device__ constexpr int join_floats() { return (PARTS * ROWS > THREADS * 4 ? PARTS * ROWS : THREADS * 4) + 2 * ROWS; }
 
-template <int ROWS, int THREADS, int VEC, int PARTS>
-__device__ __forceinline__ void join(const skv_pool_attention_args& a, const Share& s, const Segment& g, int R, float* buf, bool out_vec = false) {
-    const int D = a.pool.head_dim, tid = threadIdx.x, rows = min(ROWS, R - g.rt * ROWS), items = rows * D / VEC;
+template <int ROWS, int THREADS, int VEC, int PARTS, class Sync = BlockSync>
+__device__ __forceinline__ void join(const skv_pool_attention_args& a, const Share& s, const Segment& g, int r0, int rows, float* buf, bool out_vec = false) {
+    const int D = a.pool.head_dim, tid = threadIdx.x, items = rows * D / VEC;
     const int c0 = s.owner_of(g.first), parts = s.owner_of(g.last) - c0 + 1;
     // part i lies at base + i * stride, the first one in its CTA's second slot unless it starts that CTA's share
     const int64_t stride = (int64_t)2 * ROWS * (D + 2);
@@ -230,7 +247,7 @@ __device__ __forceinline__ void join(const skv_pool_attention_args& a, const Sha
     float* s_l = s_m + ROWS;           // [ROWS] sum over all parts
     float* s_f = s_l + ROWS;           // [PARTS][ROWS] 2^(m_i - m) of a block of parts
     float* s_add = s_f;                // [THREADS][VEC] once the factors are used
-    __syncthreads();
+    Sync::sync();
     {
         constexpr int TPR = THREADS / ROWS;   // a power of two, at most 32
         const int j = tid / TPR, sub = tid % TPR;
@@ -269,7 +286,7 @@ __device__ __forceinline__ void join(const skv_pool_attention_args& a, const Sha
             s_l[j] = l;
         }
     }
-    __syncthreads();
+    Sync::sync();
     const int ways = items >= THREADS ? 1 : min(THREADS / items, kJoinWays), wide = THREADS / ways;
     const int way = tid / wide;
     constexpr int I = ROWS >= 16 ? 4 : 2;   // values of a thread at a time
@@ -286,12 +303,12 @@ __device__ __forceinline__ void join(const skv_pool_attention_args& a, const Sha
         for (int i0 = 0; i0 < parts; i0 += PARTS) {
             const int count = min(PARTS, parts - i0);
             if (parts > PARTS) {   // more parts than factors fit: block by block
-                __syncthreads();
+                Sync::sync();
                 for (int i = tid; i < count * rows; i += THREADS) {
                     const int k = i / rows, r = i - k * rows;
                     s_f[k * ROWS + r] = exp2f(__ldcg(part(i0 + k) + ROWS * D + r) - s_m[r]);
                 }
-                __syncthreads();
+                Sync::sync();
             }
             if (way >= ways) continue;
             for (int k0 = way; k0 < count; k0 += 16 / I * ways) {
@@ -317,10 +334,10 @@ __device__ __forceinline__ void join(const skv_pool_attention_args& a, const Sha
             }
         }
         if (ways > 1) {   // items < THREADS: one value a thread, n = 0
-            __syncthreads();
+            Sync::sync();
 #pragma unroll
             for (int e = 0; e < VEC; ++e) s_add[tid * VEC + e] = y[0][e];
-            __syncthreads();
+            Sync::sync();
             if (way == 0)
                 for (int w = 1; w < ways; ++w)
 #pragma unroll
@@ -332,12 +349,12 @@ __device__ __forceinline__ void join(const skv_pool_attention_args& a, const Sha
                 if (v[n] < items && (ways == 1 || n == 0)) {
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) y[n][e] = s_l[row[n]] == 0.0f ? 0.0f : y[n][e] / s_l[row[n]];
-                    if constexpr (VEC == 4) store_row(a, g, g.rt * ROWS + row[n], v[n] * VEC - row[n] * D, out_vec, y[n]);
-                    else store_out<1>(a, g.b, g.hk, g.rt * ROWS + row[n], v[n] - row[n] * D, y[n]);
+                    if constexpr (VEC == 4) store_row(a, g, r0 + row[n], v[n] * VEC - row[n] * D, out_vec, y[n]);
+                    else store_out<1>(a, g.b, g.hk, r0 + row[n], v[n] - row[n] * D, y[n]);
                 }
         }
     }
-    __syncthreads();
+    Sync::sync();
 }
 
 }  // namespace skv

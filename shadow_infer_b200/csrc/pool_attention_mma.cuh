@@ -34,7 +34,7 @@ namespace skv {
 
 constexpr int kMmaPad = 3, kMinTiles = 2;   // what a unit costs on top of its tiles, and the least that a CTA takes
 constexpr int kMmaParts = 64;       // parts whose factors a joining CTA holds at a time
-constexpr float kRefDrop = 5.0f;    // a fresh maximum's weight is 2^5: small weights keep their bits in fp16
+constexpr float kRefDrop = 11.0f;   // a fresh maximum's weight is 2^11: fp16's last step, 2^-25, is then 2^-36 of it
 constexpr float kRefRoom = 14.0f;   // weights may grow to 2^14 (times a mantissa < 2) before ref moves
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint2 b) {
@@ -398,6 +398,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
         f.st += W;
     };
     int head = 0;   // slot of the tile to multiply; the one before it is free
+    int merged = -1;   // the slot that held sums when the segment before ended
 #pragma unroll
     for (int i = 0; i < S - 1; ++i) copy_next(ring + i * L::BYTES);
 
@@ -409,6 +410,10 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
         const int n = g.tokens, r0 = g.rt * ROWS;
         // ---- queries: a power of two taken out of each row, laid out as B operands
         __syncthreads();
+        if (!exact && merged >= 0) {   // chunks that are never copied count as zero again
+            for (int i = lane; i < L::BYTES / 16; i += 32) reinterpret_cast<uint4*>(s_ring + merged)[i] = make_uint4(0, 0, 0, 0);
+            __syncwarp();
+        }
         {
             constexpr int RW = ROWS / W, E = DP / 32;   // a warp's rows, a lane's values of each
             float x[RW][E];
@@ -917,6 +922,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                 }
             }
         const int free_at = (warp * S + (head == 0 ? S - 1 : head - 1)) * L::BYTES;
+        merged = free_at;
         if (lane == 0) s_free[warp] = free_at;
         float* part = slot_of(a, blockIdx.x, g.slot, ROWS);
 #pragma unroll
@@ -981,7 +987,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                 part[ROWS * D + tid] = s_c[tid];
                 part[ROWS * D + ROWS + tid] = s_l[tid];
             }
-            if (arrive(a, s, g)) join<ROWS, THREADS, 4, kMmaParts>(a, s, g, R, s_join, out_vec);
+            if (arrive(a, s, g)) join<ROWS, THREADS, 4, kMmaParts>(a, s, g, r0, min(ROWS, R - r0), s_join, out_vec);
         }
     }
 }

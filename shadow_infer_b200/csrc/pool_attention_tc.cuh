@@ -1,0 +1,582 @@
+// Attention over the page pool for many query rows a key head: blocks of new tokens and whole prompts.
+//
+// A few query rows leave tcgen05 idle (pool_attention_mma.cuh), 128 fill it: a unit is (sequence, key head, 128 query rows), and
+//     S [128 rows x 128 tokens] = Q K^T,     O [128 rows x D] += P V
+// run as tcgen05.mma with the sums in TMEM.  Where a head has 128 new tokens or more a unit's rows are neighbours of one head, and
+// with a causal limit the unit ends at the last token that its rows see: the shares count each unit's own tiles, by a closed
+// form, so a prompt costs its triangle.
+//
+// A CTA is a pipeline of two roles:
+//     warps 0-3   softmax, a query row a thread (TMEM lane): S from TMEM, the running maximum (moved lazily), weights P as fp16
+//                 back into TMEM over S's first columns; O read, divided and stored, or published for the join, at a unit's end.
+//                 They also lay out Q once a unit (a power of two taken out of each row).  Thread 0 issues the MMAs in between (they are on this role's path in any case, so a warp for them would
+//                 only take registers: 256 threads leave two CTAs 128 each, with 96 the softmax spilled);
+//     warps 4-7   each tile's page rows: fp16 copied, int8 made fp16 integers (exact), in the swizzled layout that the tensor
+//                 cores read, and what a token's scales do to scores and weights; they run ahead across units.
+// Two CTAs share an SM (TMEM: 128 columns of S and P, 128 of O each), so that one's MMAs run during the other's softmax.
+//
+// Numbers: as in pool_attention_mma.cuh.  Page values and queries are exact in fp16, an int8 row's scale multiplies its scores (K)
+// and weights (V) in fp32, a weight is rounded once, to fp16, at no more than 2^15.
+//
+// Every wait is bounded: after a second without progress the roles leave, TMEM is freed and the outputs are NaN.
+#pragma once
+
+#include <atomic>
+
+#include "pool_attention.cuh"
+#include "sm100_ptx.cuh"
+
+namespace skv {
+
+constexpr int kTcTile = 128, kTcRows = 128, kTcThreads = 256, kTcPad = 1, kTcParts = 16, kTcColumns = 256;
+// A fresh maximum's weight is 2^10 to 2^11 and may grow to 2^15: with one fp16 operand a weight, its subnormals' 2^-25 is then
+// 2^-35 of the largest weight.
+constexpr float kTcDrop = 11.0f, kTcRoom = 14.0f;
+
+// The units of a sequence and key head, and what each costs.
+struct TcUnits {
+    int S_q, rep, blocks, row_tiles;   // blocks: of 128 new tokens of a head (0: a unit's rows are any heads' and tokens')
+    bool causal;
+    __device__ __forceinline__ TcUnits(const skv_pool_attention_args& a)
+        : S_q(a.S_q), rep(a.q.heads / a.pool.heads), blocks(a.S_q >= kTcRows ? (a.S_q + kTcRows - 1) / kTcRows : 0),
+          row_tiles(blocks ? rep * blocks : (rep * a.S_q + kTcRows - 1) / kTcRows), causal(a.causal && blocks) {}
+    // With n tiles and `past` tiles before the new tokens, block i sees past + i + 1 tiles, at least one and no more than n.
+    __device__ __forceinline__ int tiles(int i, int n, int past) const { return causal ? min(max(past + i + 1, 1), n) : n; }
+    // What blocks [0, k) cost.
+    __device__ __forceinline__ int before(int k, int n, int past, int pad) const {
+        if (!causal) return k * (n + pad);
+        const int lo = min(max(-past, 0), k), hi = min(max(n - past, lo), k);   // blocks below lo see one tile, from hi on n
+        return lo + (hi - lo) * (past + 1) + (hi * (hi - 1) - lo * (lo - 1)) / 2 + (k - hi) * n + k * pad;
+    }
+    __device__ __forceinline__ void sequence(const skv_pool_attention_args& a, int b, int& tokens, int& n, int& past) const {
+        tokens = seq_tokens(a, b);
+        n = seq_tiles(tokens, kTcTile);
+        const int old = tokens - (a.new_lengths ? __ldg(a.new_lengths + b) : S_q);
+        past = old >= 0 ? (old + kTcTile - 1) / kTcTile : -((-old) / kTcTile);
+    }
+    __device__ __forceinline__ int a_head(int n, int past, int pad) const {   // a key head's units
+        return blocks ? rep * before(blocks, n, past, pad) : row_tiles * (n + pad);
+    }
+};
+
+struct TcSegment : Segment {
+    int r0, rows;   // the unit's query rows
+};
+
+__device__ __forceinline__ TcSegment tc_segment_at(const skv_pool_attention_args& a, const TcUnits& u, const Share& s, int at, int& b,
+                                                   int& base) {
+    TcSegment g;
+    for (;;) {
+        int n, past;
+        u.sequence(a, b, g.tokens, n, past);
+        const int each = u.a_head(n, past, s.pad);
+        if (at >= base + each * a.pool.heads) {
+            base += each * a.pool.heads;
+            ++b;
+            continue;
+        }
+        g.b = b;
+        g.hk = (at - base) / each;
+        g.first = base + g.hk * each;
+        int nt = n;
+        if (u.blocks) {
+            const int head = each / u.rep, h = (at - g.first) / head;
+            g.first += h * head;
+            int i = 0, end = u.blocks;   // the block that holds `at`
+            while (end - i > 1) {
+                const int m = (i + end) / 2;
+                if (g.first + u.before(m, n, past, s.pad) <= at) i = m;
+                else end = m;
+            }
+            nt = u.tiles(i, n, past);
+            g.first += u.before(i, n, past, s.pad);
+            g.rt = h * u.blocks + i;
+            g.r0 = h * u.S_q + i * kTcRows;
+            g.rows = min(kTcRows, u.S_q - i * kTcRows);
+        } else {
+            g.rt = (at - g.first) / (n + s.pad);
+            g.first += g.rt * (n + s.pad);
+            g.r0 = g.rt * kTcRows;
+            g.rows = min(kTcRows, u.rep * u.S_q - g.r0);
+        }
+        g.last = g.first + nt - 1;
+        g.t0 = at - g.first;
+        g.next = min(g.first + nt + s.pad, s.hi);
+        g.t1 = min(nt, g.next - g.first);
+        g.whole = g.t0 == 0 && g.t1 == nt;
+        g.slot = at == s.lo ? 0 : 1;
+        if (a.error_flag && a.lengths[b] > g.tokens && threadIdx.x == 0) atomicExch(a.error_flag, 1);
+        return g;
+    }
+}
+
+// Shared memory of a CTA.
+template <int DP>
+struct TcLayout {
+    static constexpr int TILE = DP / 64 * 128 * 128;   // atoms of 128 rows of 64 values
+    static constexpr int Q = 0, K = TILE, V = 2 * TILE;
+    static constexpr int TOKENS = 3 * TILE;            // [2][4][128] of a tile's tokens: score factor, score term, weight factor, 1 / sum factor
+    static constexpr int JOIN = TOKENS + 2 * 4 * 128 * 4;
+    static constexpr int BARS = JOIN + (join_floats<kTcRows, 128, kTcParts>() * 4 + 15) / 16 * 16;
+    static constexpr int BYTES = BARS + 80, ALLOC = BYTES + 1024;   // tiles start on 1024-byte boundaries
+};
+
+__device__ __forceinline__ float tc_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 32 lanes x 16 consecutive 32-bit columns: thread t of the warp gets lane (base_lane + t).
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ uint32_t tc_pack(float a, float b) {
+    const __half2 r = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+// Bytes n + 128 as fp16 n: 1024 + b has b in its low bits.
+__device__ __forceinline__ uint32_t tc_i8_pair(uint32_t biased, uint32_t sel) {
+    const uint32_t x = __byte_perm(biased, 0x64646464u, sel), c = 0x64806480u;
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&c));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+template <int PREC, int DP>
+__global__ void __launch_bounds__(kTcThreads, 2) pool_attention_tc_kernel(const __grid_constant__ skv_pool_attention_args a, bool out_vec) {
+    using namespace sm100;
+    using L = TcLayout<DP>;
+    using Sync = FirstThreadsSync<128>;
+    extern __shared__ uint8_t tc_raw[];
+    __shared__ Share s;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_error;
+    __shared__ __align__(16) int s_gap[2][4];   // whether the tile misses a token of the sequence, by the warp that looked it up
+    uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tc_raw) + 1023) & ~uintptr_t(1023));
+    float* s_tokens = reinterpret_cast<float*>(sm + L::TOKENS);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::BARS);
+    uint64_t *k_full = bars, *k_free = bars + 2, *v_full = bars + 3, *v_free = bars + 4, *s_full = bars + 5, *o_full = bars + 6,
+             *drained = bars + 7;   // k_full: of even and of odd tiles (the softmax may look when the next is full)
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int D = a.pool.head_dim, P = a.pool.page_size, rep = a.q.heads / a.pool.heads;
+    const TcUnits u(a);
+    if (tid == 0) {
+        mbar_init(k_full, 4);
+        mbar_init(k_full + 1, 4);
+        mbar_init(k_free, 1);
+        mbar_init(v_full, 4);
+        mbar_init(v_free, 1);
+        mbar_init(s_full, 1);
+        mbar_init(o_full, 1);
+        mbar_init(drained, 1);
+        fence_mbarrier_init();
+        s_error = 0;
+    }
+    take_share<kTcThreads>(a, [&](int b) {
+        int tokens, n, past;
+        u.sequence(a, b, tokens, n, past);
+        return u.a_head(n, past, kTcPad) * a.pool.heads;
+    }, kTcPad, 1, &s);
+    if (s.lo >= s.hi) return;
+    if (warp == 0) {
+        tmem_alloc(&s_tmem, kTcColumns);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    int at = s.lo, b = s.b, base = s.base;
+    int g = 0;      // tiles so far: the barriers complete once a tile (k_full: every second, o_full: once a unit)
+    int units = 0;  // units so far
+    bool ok = true;
+
+    if (warp < 4) {
+        // ------------------------------------------------------------------- softmax, and the MMAs
+        const uint32_t t_s = tmem + ((uint32_t)(warp * 32) << 16), t_o = t_s + 128;
+        const uint32_t k_tile = smem_u32(sm + L::K), v_tile = smem_u32(sm + L::V), q_tile = smem_u32(sm + L::Q);
+        bool issued = false;
+        for (; at < s.hi;) {
+            const TcSegment sg = tc_segment_at(a, u, s, at, b, base);
+            at = sg.next;
+            if (sg.t0 >= sg.t1) continue;
+            const int r = sg.r0 + tid;
+            const int see = tid < sg.rows ? seen_by(a, sg.b, sg.tokens, r % a.S_q) : 0;
+            const int see_min = __reduce_min_sync(0xffffffffu, tid < sg.rows ? see : 0x7fffffff);
+            float ref = -INFINITY, base_of = 0.0f, l = 0.0f, c_row = 0.0f;
+            {   // a power of two taken out of the row (the MMAs of the unit before, which read Q, are done: O was)
+                const bool have = tid < sg.rows;
+                const uint16_t* from = have ? row_ptr<const uint16_t>(a.q, a.S_q, rep, sg.b, sg.hk, r) : nullptr;
+                uint4 q[DP / 8];
+#pragma unroll
+                for (int i = 0; i < DP / 8; ++i)
+                    q[i] = have && i * 8 < D ? __ldg(reinterpret_cast<const uint4*>(from) + i) : make_uint4(0, 0, 0, 0);
+                // the largest magnitude by its bits (a NaN is left to the score); it goes to [2^10, 2^11)
+                uint32_t top = 0;
+#pragma unroll
+                for (int i = 0; i < DP / 8; ++i) {
+                    const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top = max(max(top, w[e] & 0x7fffu), w[e] >> 16 & 0x7fffu);
+                }
+                const bool half = a.q.dtype == kF16;
+                const float most = half ? __half2float(__ushort_as_half((unsigned short)top)) : __uint_as_float(top << 16);
+                const int e2 = min(max((int)(__float_as_uint(most) >> 23), 35), 219);
+                const float down = __uint_as_float((uint32_t)(264 - e2) << 23);
+                c_row = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(e2 - 10) << 23);
+                uint8_t* to = sm + L::Q;
+#pragma unroll
+                for (int i = 0; i < DP / 8; ++i) {
+                    uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+                    if (half) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+                            w[e] = tc_pack(f.x * down, f.y * down);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] = tc_pack(__uint_as_float(w[e] << 16) * down, __uint_as_float(w[e] & 0xffff0000u) * down);
+                    }
+                    *reinterpret_cast<uint4*>(to + i / 8 * 128 * 128 + sw128_offset(tid, i % 8)) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            fence_proxy_async_smem();
+            Sync::sync();
+            for (int t = sg.t0; t < sg.t1; ++t, ++g) {
+                if (tid == 0 && ok && mbar_wait_spin(k_full + (g & 1), g >> 1 & 1, &s_error, 1)) {
+                    tc_fence_after();
+#pragma unroll
+                    for (int i = 0; i < DP / 16; ++i) {
+                        const uint32_t off = (i >> 2) * (128 * 128) + (i & 3) * 32;
+                        umma_f16(tmem, smem_desc_sw128(q_tile + off, 16, 1024), smem_desc_sw128(k_tile + off, 16, 1024),
+                                 idesc_f16_f32(128, 128, false, false), i > 0);
+                    }
+                    umma_commit(s_full);
+                    umma_commit(k_free);
+                    issued = true;
+                }
+                __syncwarp();
+                // (k_full has completed before s_full: this makes the producers' plain stores visible here)
+                ok = ok && __all_sync(0xffffffffu, mbar_wait_spin(s_full, g & 1, &s_error, 2) &&
+                                                       mbar_wait_spin(k_full + (g & 1), g >> 1 & 1, &s_error, 3));
+                tc_fence_after();
+                const float* tk = s_tokens + (g & 1) * 4 * 128;
+                const int left = see - t * kTcTile;   // columns that this row sees
+                const int4 gaps = *reinterpret_cast<const int4*>(s_gap[g & 1]);
+                const bool masked = see_min - t * kTcTile < kTcTile, gap = gaps.x | gaps.y | gaps.z | gaps.w;
+                // 32 columns at a time.  The reference is an integer that moves only where a weight would grow too large; what the
+                // old one scaled (O, the sum, the columns before) is a power of two off, which is exact.  (O holds the tiles
+                // before: s_full says that their MMAs are done.  16 columns of P replace S's that have been read.)
+#pragma unroll 1
+                for (int c = 0; c < 4 && ok; ++c) {
+                    float y[32];
+                    {
+                        uint32_t x[32];
+                        tmem_ld32(t_s + c * 32, x);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            if constexpr (PREC == 2) {
+                                const float4 k = *reinterpret_cast<const float4*>(tk + c * 32 + i);
+                                const float4 add = *reinterpret_cast<const float4*>(tk + 128 + c * 32 + i);
+                                y[i] = fmaf(__uint_as_float(x[i]), k.x * c_row, add.x);
+                                y[i + 1] = fmaf(__uint_as_float(x[i + 1]), k.y * c_row, add.y);
+                                y[i + 2] = fmaf(__uint_as_float(x[i + 2]), k.z * c_row, add.z);
+                                y[i + 3] = fmaf(__uint_as_float(x[i + 3]), k.w * c_row, add.w);
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) y[i + e] = __uint_as_float(x[i + e]) * c_row;
+                            }
+                        }
+                    }
+                    if (masked) {
+                        const int there = left - c * 32;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (i >= there) y[i] = -INFINITY;
+                    }
+                    if (gap) {
+#pragma unroll 1
+                        for (int i = 0; i < 32; i += 8)
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (e / 8 * 8 == i && tk[128 + c * 32 + e] == -INFINITY) y[e] = -INFINITY;
+                    }
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], y[i]);
+                    const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                    if (__any_sync(0xffffffffu, high > ref + kTcRoom)) {
+                        const float now = fmaxf(ref, ceilf(high - kTcDrop)), f = now == -INFINITY ? 1.0f : tc_exp2(ref - now);
+                        ref = now;
+                        base_of = now == -INFINITY ? 0.0f : now;
+                        l *= f;
+                        if (t > sg.t0) {
+#pragma unroll 1
+                            for (int d = 0; d < DP / 32; ++d) {
+                                uint32_t o[32];
+                                tmem_ld32(t_o + d * 32, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                                tmem_st32(t_o + d * 32, o);
+                            }
+                        }
+#pragma unroll 1
+                        for (int d = 0; d < c; ++d) {
+                            uint32_t w[16];
+                            tmem_wait_st();
+                            tmem_ld16(t_s + d * 16, w);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const float2 z = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));   // (f may be below fp16's range)
+                                w[i] = tc_pack(z.x * f, z.y * f);
+                            }
+                            tmem_st16(t_s + d * 16, w);
+                        }
+                    }
+                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    uint32_t p[16];
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) y[i + e] = tc_exp2(y[i + e] - base_of);
+                        if constexpr (PREC == 2) {
+                            const float4 v = *reinterpret_cast<const float4*>(tk + 256 + c * 32 + i);
+                            const float4 w = *reinterpret_cast<const float4*>(tk + 384 + c * 32 + i);
+                            sum[0] = fmaf(y[i], w.x, sum[0]);
+                            sum[1] = fmaf(y[i + 1], w.y, sum[1]);
+                            sum[2] = fmaf(y[i + 2], w.z, sum[2]);
+                            sum[3] = fmaf(y[i + 3], w.w, sum[3]);
+                            y[i] *= v.x; y[i + 1] *= v.y; y[i + 2] *= v.z; y[i + 3] *= v.w;
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) sum[e] += y[i + e];
+                        }
+                        p[i / 2] = tc_pack(y[i], y[i + 1]);
+                        p[i / 2 + 1] = tc_pack(y[i + 2], y[i + 3]);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tmem_st16(t_s + c * 16, p);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                Sync::sync();
+                if (tid == 0 && ok && mbar_wait_spin(v_full, g & 1, &s_error, 4)) {
+                    tc_fence_after();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        umma_f16_ts(tmem + 128, tmem + i * 8, smem_desc_sw128(v_tile + i * 16 * 128, 128 * 128, 1024),
+                                    idesc_f16_f32(128, DP, false, true), t > sg.t0 || i > 0);
+                    umma_commit(v_free);
+                    if (t + 1 == sg.t1) umma_commit(o_full);
+                }
+                __syncwarp();
+            }
+            // ------------------------------------------------------------------------ the unit's end
+            ok = ok && __all_sync(0xffffffffu, mbar_wait_spin(o_full, units & 1, &s_error, 5));
+            ++units;
+            tc_fence_after();
+            float* part = slot_of(a, blockIdx.x, sg.slot, kTcRows);
+            const float nan = __int_as_float(0x7fc00000);
+            const float mul = !ok ? nan : !sg.whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll 1
+            for (int c = 0; c < DP / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld32(t_o + c * 32, o);
+                tmem_wait_ld();
+                float y[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) y[i] = l == 0.0f && ok ? 0.0f : __uint_as_float(o[i]) * mul;
+                if (tid < sg.rows) {
+                    if (!sg.whole) {
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            if (c * 32 + i < D) *reinterpret_cast<float4*>(part + tid * D + c * 32 + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+                    } else if (out_vec) {   // 16 bytes a store
+                        uint4* to = reinterpret_cast<uint4*>(row_ptr<uint16_t>(a.out, a.S_q, rep, sg.b, sg.hk, r) + c * 32);
+                        uint32_t w[16];
+                        if (a.out.dtype == kF16) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) w[i] = tc_pack(y[2 * i], y[2 * i + 1]);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const __nv_bfloat162 z = __floats2bfloat162_rn(y[2 * i], y[2 * i + 1]);
+                                w[i] = *reinterpret_cast<const uint32_t*>(&z);
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (c * 32 + i * 8 < D) to[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (c * 32 + i < D) {
+                                const float one[1] = {y[i]};
+                                store_out<1>(a, sg.b, sg.hk, r, c * 32 + i, one);
+                            }
+                    }
+                }
+                __syncwarp();
+            }
+            tc_fence_before();
+            if (!sg.whole) {
+                if (tid < sg.rows) {
+                    part[kTcRows * D + tid] = ref;
+                    part[kTcRows * D + kTcRows + tid] = ok ? l : nan;
+                }
+                if (arrive<Sync>(a, s, sg))
+                    join<kTcRows, 128, 4, kTcParts, Sync>(a, s, sg, sg.r0, sg.rows, reinterpret_cast<float*>(sm + L::JOIN), out_vec);
+            }
+        }
+        if (tid == 0 && issued) {   // every MMA has completed before TMEM is freed
+            umma_commit(drained);
+            int none = 0;
+            mbar_wait_spin(drained, 0, &none, 6);
+        }
+        __syncwarp();
+    } else {
+        // ------------------------------------------------------------------------- pages and queries
+        const int pw = warp - 4;
+        constexpr int CHUNKS = PREC == 1 ? DP / 8 : DP / 16;   // 16-byte chunks of a row
+        constexpr int STEP = 32 / CHUNKS, N = 32 / STEP;       // rows that a warp takes at a time; a warp has 32 of a tile
+        const int my_chunk = lane % CHUNKS, my_row = lane / CHUNKS;
+        const bool have_chunk = my_chunk * (PREC == 1 ? 8 : 16) < D;
+        const int row_bytes = PREC == 1 ? 2 * D : D;
+        uint4 k_raw[PREC == 2 ? N : 1], v_raw[PREC == 2 ? N : 1];   // int8: the next tile's, on their way
+        auto load = [&](uint4 (&raw)[PREC == 2 ? N : 1], const void* pages, int row) {
+            if constexpr (PREC == 2) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int x = __shfl_sync(0xffffffffu, row, i * STEP + my_row);
+                    raw[i] = make_uint4(0, 0, 0, 0);
+                    if (x >= 0 && have_chunk)
+                        raw[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const char*>(pages) + (int64_t)x * row_bytes + my_chunk * 16));
+                }
+            }
+        };
+        auto write = [&](const uint4 (&raw)[PREC == 2 ? N : 1], uint8_t* tile) {
+            if constexpr (PREC == 2) {   // 16 values: two chunks of an atom, exchanged for every second atom (banks)
+                const int atom = my_chunk / 4, swap = atom & 1, c = my_chunk % 4 * 2;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int x = pw * 32 + i * STEP + my_row;
+                    const uint32_t w[4] = {raw[i].x ^ 0x80808080u, raw[i].y ^ 0x80808080u, raw[i].z ^ 0x80808080u, raw[i].w ^ 0x80808080u};
+                    const uint4 lo = make_uint4(tc_i8_pair(w[0], 0x4140), tc_i8_pair(w[0], 0x4342), tc_i8_pair(w[1], 0x4140), tc_i8_pair(w[1], 0x4342));
+                    const uint4 hi = make_uint4(tc_i8_pair(w[2], 0x4140), tc_i8_pair(w[2], 0x4342), tc_i8_pair(w[3], 0x4140), tc_i8_pair(w[3], 0x4342));
+                    uint8_t* line = tile + atom * 128 * 128;
+                    *reinterpret_cast<uint4*>(line + sw128_offset(x, c + swap)) = swap ? hi : lo;
+                    *reinterpret_cast<uint4*>(line + sw128_offset(x, c + 1 - swap)) = swap ? lo : hi;
+                }
+            }
+        };
+        auto copy = [&](uint8_t* tile, const void* pages, int row) {
+            if constexpr (PREC == 1) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int x = __shfl_sync(0xffffffffu, row, i * STEP + my_row);
+                    const uint32_t to = smem_u32(tile + my_chunk / 8 * 128 * 128 + sw128_offset(pw * 32 + i * STEP + my_row, my_chunk % 8));
+                    const bool there = x >= 0 && have_chunk;
+                    const char* from = static_cast<const char*>(pages) + (there ? (int64_t)x * row_bytes + my_chunk * 16 : 0);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+                }
+            }
+        };
+        auto publish = [&](uint64_t* full) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(full);
+        };
+        for (; ok && at < s.hi;) {
+            const TcSegment sg = tc_segment_at(a, u, s, at, b, base);
+            at = sg.next;
+            if (sg.t0 >= sg.t1) continue;
+            // the pool row of this lane's token of a tile (tokens 32 pw .. of it), -1 where there is none
+            bool gap;
+            auto row_of = [&](int t) -> int {
+                const int tok = t * kTcTile + pw * 32 + lane;
+                gap = false;
+                if (t >= sg.t1 || tok >= sg.tokens) return -1;
+                const int64_t row = pool_row(a.pool, sg.b, tok);
+                if (row < 0 && a.error_flag) atomicExch(a.error_flag, 1);
+                gap = row < 0;
+                return row < 0 ? -1 : (int)row + sg.hk * P;
+            };
+            int row = row_of(sg.t0);
+            load(k_raw, a.pool.k, row);
+            load(v_raw, a.pool.v, row);
+            for (int t = sg.t0; t < sg.t1; ++t, ++g) {
+                float* tk = s_tokens + (g & 1) * 4 * 128 + pw * 32 + lane;
+                float sk = 0.0f, sv = 1.0f;
+                if (PREC == 2 && row >= 0) {
+                    sk = __ldg(a.pool.scale_k + row);
+                    sv = __ldg(a.pool.scale_v + row);
+                }
+                const bool any_gap = __any_sync(0xffffffffu, gap);
+                const int next = row_of(t + 1);
+                // the scores of the tile before are done: K is free, and what the softmax of the tile before that read
+                if (g > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait_spin(k_free, (g - 1) & 1, &s_error, 7));
+                if (!ok) break;
+                write(k_raw, sm + L::K);
+                copy(sm + L::K, a.pool.k, row);
+                if constexpr (PREC == 2) {   // V's scale as a power of two in the exponent and a factor in [1, 2)
+                    const int e = min(max((int)((__float_as_uint(sv) & 0x7fffffffu) >> 23), 35), 219);
+                    const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+                    tk[0] = sk;
+                    tk[128] = row >= 0 ? (float)(e - 127) : -INFINITY;
+                    tk[256] = sv * down;
+                    tk[384] = down;
+                } else {
+                    tk[128] = row >= 0 ? 0.0f : -INFINITY;
+                }
+                if (lane == 0) s_gap[g & 1][pw] = any_gap;
+                if constexpr (PREC == 1) asm volatile("cp.async.wait_all;" ::: "memory");
+                publish(k_full + (g & 1));
+                load(k_raw, a.pool.k, next);
+                if (g > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait_spin(v_free, (g - 1) & 1, &s_error, 8));
+                if (!ok) break;
+                write(v_raw, sm + L::V);
+                copy(sm + L::V, a.pool.v, row);
+                if constexpr (PREC == 1) asm volatile("cp.async.wait_all;" ::: "memory");
+                publish(v_full);
+                load(v_raw, a.pool.v, next);
+                row = next;
+            }
+            ++units;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kTcColumns);
+    }
+    if (tid == 0 && s_error && a.error_flag) atomicExch(a.error_flag, 1);
+}
+
+template <int PREC, int DP>
+int launch_tc(const skv_pool_attention_args& a, cudaStream_t st) {
+    using L = TcLayout<DP>;
+    static_assert(2 * 2 * kTcRows <= kRowsPerSm, "the scratch holds every CTA's slots");
+    static_assert(2 * (L::ALLOC + 2048) <= 228 * 1024, "an SM holds two CTAs");
+    const auto kernel = pool_attention_tc_kernel<PREC, DP>;
+    static std::atomic<uint64_t> allowed{0};   // devices whose limit on the kernel's shared memory was raised
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev >= 64 || !(allowed.load(std::memory_order_relaxed) >> dev & 1))) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC);
+        if (e == cudaSuccess && dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
+    if (e != cudaSuccess) return fail(SKV_ERR_CUDA, "pool_attention: %s", cudaGetErrorString(e));
+    kernel<<<sm_count() * 2, kTcThreads, L::ALLOC, st>>>(a, rows_aligned(a.out));
+    return check_launch("pool_attention");
+}
+
+}  // namespace skv

@@ -387,6 +387,73 @@ def test_attention_ragged_prompt(skv, kv, causal):
         assert (got[b, :, n:] == 0).all()
 
 
+MANY_ROWS = [  # counts, H, rep, Sq, D, P, new, causal: 48 query rows a key head and more, from 1 to some hundred units of 128
+    ([300, 0, 1, 127, 128, 129] * 5, 4, 4, 16, 128, 32, None, False),
+    ([300, 0, 1, 127, 128, 129] * 5, 4, 4, 16, 128, 32, None, True),
+    ([9000, 16, 2500], 2, 4, 31, 128, 16, None, True),       # parts that are joined
+    ([3000, 20] * 10, 8, 2, 33, 128, 16, None, True),
+    ([5000], 1, 3, 33, 64, 64, None, False),
+    ([700, 130, 64], 19, 2, 130, 64, 7, None, True),         # blocks of one head's tokens, the last of two
+    ([700, 130, 64], 19, 2, 130, 64, 7, [130, 60, 0], True), # and padding of a ragged prompt
+    ([1000, 400], 15, 1, 400, 128, 32, [400, 257], True),
+    ([515], 24, 1, 515, 128, 128, None, True),               # a whole prompt
+    ([515], 1, 1, 515, 128, 128, None, True),
+    ([515, 200], 14, 2, 200, 96, 24, None, False),
+    ([140], 38, 3, 128, 80, 16, None, True),
+    ([333, 90] * 16, 4, 8, 9, 112, 11, [9, 4] * 16, True),
+    ([260, 33] * 16, 4, 64, 1, 32, 16, None, False),         # many heads, one token
+    ([77, 12], 1, 50, 1, 16, 64, None, False),
+]
+
+
+@pytest.mark.parametrize("counts,H,rep,Sq,D,P,new,causal", MANY_ROWS)
+@pytest.mark.parametrize("kv", ["fp32", "fp16", "int8", "int4"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_attention_of_many_rows(skv, counts, H, rep, Sq, D, P, new, causal, kv, dtype):
+    pages, scales, table, lens = _filled(skv, kv, counts, H, P, D, 16, sum(counts) + D, channels=3.0)
+    gen = _gen(17)
+    fresh = None if new is None else torch.tensor(new, dtype=torch.int32, device="cuda")
+    for layout in ("bhsd", "projection", "odd"):
+        q = _rows(gen, len(counts), H * rep, Sq, D, dtype, layout)
+        got = skv.paged_attention(q, *pages, table, lens, *scales, causal=causal, new_lengths=fresh, check=True)
+        want, bound = _attention64(q, pages, scales, table, counts, new or [Sq] * len(counts), causal)
+        off = (got.double() - want).abs() - bound
+        assert off.max() <= 0, (layout, float(off.max()))
+        assert torch.equal(got, skv.paged_attention(q, *pages, table, lens, *scales, causal=causal, new_lengths=fresh))
+
+
+@pytest.mark.parametrize("kv", ["fp16", "int8"])
+def test_attention_of_many_rows_extremes(skv, kv):
+    """A NaN row, rows of very different size and a page outside the pool, for a prompt."""
+    counts, H, D, P, Sq = [600, 300], 15, 128, 32, 140
+    pages, scales, table, lens = _filled(skv, kv, counts, H, P, D, 16, 8)
+    q = _rows(_gen(5), 2, 2 * H, Sq, D, torch.float16)
+    q *= 10.0 ** torch.linspace(-4, 2, Sq, device="cuda").half()[:, None]
+    clean = skv.paged_attention(q, *pages, table, lens, *scales, causal=True)
+    want, bound = _attention64(q, pages, scales, table, counts, [Sq] * 2, True)
+    assert ((clean.double() - want).abs() <= bound).all()
+    p = q.clone()
+    p[0, 1, 3, 5] = math.nan
+    got = skv.paged_attention(p, *pages, table, lens, *scales, causal=True)
+    assert torch.isnan(got[0, 1, 3]).all()
+    got[0, 1, 3] = clean[0, 1, 3]
+    assert torch.equal(got, clean)
+    bad = table.clone()
+    bad[0, 3] = -5
+    with pytest.raises(ValueError, match="outside"):
+        skv.paged_attention(q, *pages, bad, lens, *scales, causal=True, check=True)
+    # the tokens of that page count as absent
+    got = skv.paged_attention(q, *pages, bad, lens, *scales)
+    keep = torch.ones(600, dtype=torch.bool, device="cuda")
+    keep[3 * P:4 * P] = False
+    k, v = (_dense64(x, y, table, 0, 600, D)[:, keep] for x, y in zip(pages, scales))
+    w = torch.softmax(torch.einsum("grsd,gtd->grst", q[0].double().unflatten(0, (H, -1)), k) / math.sqrt(D), -1)
+    exact = torch.einsum("grst,gtd->grsd", w, v).flatten(0, 1)
+    _, bound = _attention64(q, pages, scales, table, counts, [Sq] * 2, False)
+    # (the bound of all tokens' weights, at least half of which are these)
+    assert ((got[0].double() - exact).abs() <= 2 * bound[0] + 2.0 ** -11 * exact.abs()).float().mean() > 0.999
+
+
 @pytest.mark.parametrize("kv", ["fp32", "fp16", "int8", "int4"])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 def test_attention_of_extreme_values(skv, kv, dtype):
