@@ -203,7 +203,10 @@ int attend_fp16(const skv_pool_attention_args& a, cudaStream_t st);
 int attend_int8(const skv_pool_attention_args& a, cudaStream_t st);
 int attend_int4(const skv_pool_attention_args& a, cudaStream_t st);
 
-// The tcgen05 kernel (pool_attention_tc.cuh).
+// The tcgen05 kernel (pool_attention_tc.cuh), and the query rows a key head from which it is taken.  8 key heads of 4 query heads
+// and 128 values, us there / on the small kernel: 32 rows over 4 x 4096 fp16 tokens 32.5 / 34.7, int8 37.9 / 34.1; 48 rows 35.0 /
+// 40.8, int8 38.4 / 41.9; 64 rows 34.3 / 47.3, int8 39.8 / 49.1; 128 rows over 512 tokens 20.2 / 17.5, over 16384 45.6 / 73.1.
+constexpr int kManyRows = 48;
 int attend_many(const skv_pool_attention_args& a, cudaStream_t st);
 
 // They need heads of up to 256 values in rows of whole 16-byte (fp16) or 8-byte chunks, int4 groups of whole 16-value blocks,
@@ -216,16 +219,11 @@ bool fits_mma(const skv_pool& p) {
     return ((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v)) & 15) == 0;
 }
 
-// The tcgen05 kernel takes fp16 and int8 pages whose values are exact in fp16, 16-bit queries (32-bit ones want sums that the
-// tensor cores do not cut off), heads of up to 128 values in whole swizzled chunks of 16.  It is taken where its units fill
-// three quarters of the SMs: with fewer, long sequences are cut into parts whose joining (128 rows each) costs more than the
-// MMAs save.  8 key heads of 4 query heads over fp16 pages, us here and on the small kernel: one prompt of 4096 tokens 314 / 1720,
-// of 1024 74 / 155, of 512 (128 units) 59 / 66; 128 new tokens of one sequence of 2048 (32 units) 72 / 45.
+// The tcgen05 kernel takes fp16 and int8 pages, whose values are exact in fp16, 16-bit queries (32-bit ones want sums that the
+// tensor cores do not cut off), heads of up to 128 values in whole swizzled chunks of 16.
 bool fits_tc(const skv_pool_attention_args& a) {
-    const int rep = a.q.heads / a.pool.heads;
-    const int64_t tiles = a.S_q >= 128 ? (int64_t)rep * ((a.S_q + 127) / 128) : ((int64_t)rep * a.S_q + 127) / 128;
-    return rep * (int64_t)a.S_q >= 64 && a.pool.batch * tiles * a.pool.heads * 4 >= sm_count() * 3 && a.q.dtype != kF32 && (a.pool.precision == 1 || a.pool.precision == 2) && a.pool.head_dim <= 128 &&
-           a.pool.head_dim % 16 == 0 && rows_aligned(a.q);
+    return a.q.heads / a.pool.heads * (int64_t)a.S_q >= kManyRows && a.q.dtype != kF32 &&
+           (a.pool.precision == 1 || a.pool.precision == 2) && a.pool.head_dim <= kManyD && a.pool.head_dim % 16 == 0 && rows_aligned(a.q);
 }
 
 }  // namespace skv
@@ -235,7 +233,7 @@ using namespace skv;
 extern "C" {
 
 size_t skv_pool_attention_scratch_bytes(int D) {
-    return D <= 0 ? 0 : (size_t)kMaxCtas * 4 + (size_t)sm_count() * kRowsPerSm * (D + 2) * 4;
+    return D <= 0 ? 0 : (size_t)kMaxCtas * 4 + (size_t)sm_count() * (D <= kManyD ? kManyRowsPerSm : kRowsPerSm) * (D + 2) * 4;
 }
 
 size_t skv_pool_attention_scratch_zeros(void) { return (size_t)kMaxCtas * 4; }

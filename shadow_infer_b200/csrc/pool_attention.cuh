@@ -7,7 +7,8 @@
 namespace skv {
 
 constexpr int kMaxCtas = 4096;      // arrival counters in the scratch
-constexpr int kRowsPerSm = 512;     // rows of partial results in the scratch for each SM: CTAs x 2 slots x rows
+// Rows of partial results in the scratch for each SM, CTAs x 2 slots x rows: for heads that the tcgen05 kernel takes, and others.
+constexpr int kRowsPerSm = 128, kManyRowsPerSm = 512, kManyD = 128;
 
 // ------------------------------------------------------------------------------ shares of the work
 // Tile numbers fit 31 bits (the launch checks the most that the table allows).
@@ -17,6 +18,15 @@ struct Share {
     int b;                     // the sequence that holds tile lo
     int pad;                   // tiles that a unit costs on top of its own
     int each, more;            // a share is `each` tiles, one more for the first `more` CTAs
+    // `total` tiles over at most `grid` CTAs, at least min_tiles each; returns how many CTAs have a share.
+    __device__ __forceinline__ int cut(int all, int grid, int min_tiles, int on_top) {
+        const int ctas = min(grid, max(1, (all + min_tiles - 1) / min_tiles));
+        each = all / ctas;
+        more = all - each * ctas;
+        total = all;
+        pad = on_top;
+        return ctas;
+    }
     __device__ __forceinline__ int first_of(int cta) const { return cta * each + min(cta, more); }
     __device__ __forceinline__ int owner_of(int tile) const {
         const int head = more * (each + 1);
@@ -58,12 +68,8 @@ __device__ __forceinline__ void take_share(const skv_pool_attention_args& a, Cos
         total += s_part[w];
     }
     before += incl - mine;
-    const int ctas = min((int)gridDim.x, max(1, (total + min_tiles - 1) / min_tiles));
     Share t;
-    t.each = total / ctas;
-    t.more = total - t.each * ctas;
-    t.total = total;
-    t.pad = pad;
+    const int ctas = t.cut(total, gridDim.x, min_tiles, pad);
     const int c = blockIdx.x;
     t.lo = c < ctas ? t.first_of(c) : total;
     t.hi = c < ctas ? t.first_of(c + 1) : total;
@@ -135,29 +141,18 @@ __device__ __forceinline__ Segment segment_at(const skv_pool_attention_args& a, 
 }
 
 // ------------------------------------------------------------------------------------- publishing
-// Scratch: kMaxCtas arrival counters (zero between launches: the last to arrive resets its counter), then two
-// slots a CTA of
-// rows * (D + 2) floats (rounded up to 16 bytes): O [rows][D], max [rows], sum [rows].
+// Scratch: kMaxCtas arrival counters (zero between launches: the last to arrive resets its counter), then two slots a CTA of
+// rows * (D + 2) floats: O [rows][D], max [rows], sum [rows].
 __device__ __forceinline__ float* slot_of(const skv_pool_attention_args& a, int cta, int slot, int rows) {
     return reinterpret_cast<float*>(static_cast<char*>(a.scratch) + kMaxCtas * 4) +
            ((int64_t)2 * cta + slot) * rows * (a.pool.head_dim + 2);
 }
 
-// The threads that publish and join: the whole block, or the first THREADS of it.
-struct BlockSync {
-    __device__ static __forceinline__ void sync() { __syncthreads(); }
-};
-template <int THREADS>
-struct FirstThreadsSync {
-    __device__ static __forceinline__ void sync() { asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory"); }
-};
-
-// Called by all of them once the CTA's part is in its slot; true for the CTA that joins.  The barrier puts
+// Called by all threads once the CTA's part is in its slot; true for the CTA that joins.  The barrier puts
 // every thread's stores before thread 0's fence, which puts them before its arrival.
-template <class Sync = BlockSync>
 __device__ __forceinline__ bool arrive(const skv_pool_attention_args& a, const Share& s, const Segment& g) {
     __shared__ int s_last;
-    Sync::sync();
+    __syncthreads();
     if (threadIdx.x == 0) {
         __threadfence();
         const int c0 = s.owner_of(g.first), c1 = s.owner_of(g.last);
@@ -166,7 +161,7 @@ __device__ __forceinline__ bool arrive(const skv_pool_attention_args& a, const S
         if (s_last) *count = 0;
         __threadfence();
     }
-    Sync::sync();
+    __syncthreads();
     return s_last;
 }
 
@@ -234,7 +229,7 @@ constexpr int kJoinWays = 8;
 template <int ROWS, int THREADS, int PARTS>
 __host__ __device__ constexpr int join_floats() { return (PARTS * ROWS > THREADS * 4 ? PARTS * ROWS : THREADS * 4) + 2 * ROWS; }
 
-template <int ROWS, int THREADS, int VEC, int PARTS, class Sync = BlockSync>
+template <int ROWS, int THREADS, int VEC, int PARTS>
 __device__ __forceinline__ void join(const skv_pool_attention_args& a, const Share& s, const Segment& g, int r0, int rows, float* buf, bool out_vec = false) {
     const int D = a.pool.head_dim, tid = threadIdx.x, items = rows * D / VEC;
     const int c0 = s.owner_of(g.first), parts = s.owner_of(g.last) - c0 + 1;
@@ -247,7 +242,7 @@ __device__ __forceinline__ void join(const skv_pool_attention_args& a, const Sha
     float* s_l = s_m + ROWS;           // [ROWS] sum over all parts
     float* s_f = s_l + ROWS;           // [PARTS][ROWS] 2^(m_i - m) of a block of parts
     float* s_add = s_f;                // [THREADS][VEC] once the factors are used
-    Sync::sync();
+    __syncthreads();
     {
         constexpr int TPR = THREADS / ROWS;   // a power of two, at most 32
         const int j = tid / TPR, sub = tid % TPR;
@@ -286,7 +281,7 @@ __device__ __forceinline__ void join(const skv_pool_attention_args& a, const Sha
             s_l[j] = l;
         }
     }
-    Sync::sync();
+    __syncthreads();
     const int ways = items >= THREADS ? 1 : min(THREADS / items, kJoinWays), wide = THREADS / ways;
     const int way = tid / wide;
     constexpr int I = ROWS >= 16 ? 4 : 2;   // values of a thread at a time
@@ -303,12 +298,12 @@ __device__ __forceinline__ void join(const skv_pool_attention_args& a, const Sha
         for (int i0 = 0; i0 < parts; i0 += PARTS) {
             const int count = min(PARTS, parts - i0);
             if (parts > PARTS) {   // more parts than factors fit: block by block
-                Sync::sync();
+                __syncthreads();
                 for (int i = tid; i < count * rows; i += THREADS) {
                     const int k = i / rows, r = i - k * rows;
                     s_f[k * ROWS + r] = exp2f(__ldcg(part(i0 + k) + ROWS * D + r) - s_m[r]);
                 }
-                Sync::sync();
+                __syncthreads();
             }
             if (way >= ways) continue;
             for (int k0 = way; k0 < count; k0 += 16 / I * ways) {
@@ -334,10 +329,10 @@ __device__ __forceinline__ void join(const skv_pool_attention_args& a, const Sha
             }
         }
         if (ways > 1) {   // items < THREADS: one value a thread, n = 0
-            Sync::sync();
+            __syncthreads();
 #pragma unroll
             for (int e = 0; e < VEC; ++e) s_add[tid * VEC + e] = y[0][e];
-            Sync::sync();
+            __syncthreads();
             if (way == 0)
                 for (int w = 1; w < ways; ++w)
 #pragma unroll
@@ -354,7 +349,7 @@ __device__ __forceinline__ void join(const skv_pool_attention_args& a, const Sha
                 }
         }
     }
-    Sync::sync();
+    __syncthreads();
 }
 
 }  // namespace skv

@@ -28,7 +28,7 @@
 
 namespace skv {
 
-constexpr int kTcTile = 128, kTcRows = 128, kTcThreads = 256, kTcPad = 1, kTcParts = 16, kTcColumns = 256;
+constexpr int kTcTile = 128, kTcRows = 128, kTcThreads = 256, kTcPad = 1, kTcColumns = 256;
 // A fresh maximum's weight is 2^10 to 2^11 and may grow to 2^15: with one fp16 operand a weight, its subnormals' 2^-25 is then
 // 2^-35 of the largest weight.
 constexpr float kTcDrop = 11.0f, kTcRoom = 14.0f;
@@ -116,11 +116,11 @@ struct TcLayout {
     static constexpr int TILE = DP / 64 * 128 * 128;   // atoms of 128 rows of 64 values
     static constexpr int Q = 0, K = TILE, V = 2 * TILE;
     static constexpr int TOKENS = 3 * TILE;            // [2][4][128] of a tile's tokens: score factor, score term, weight factor, 1 / sum factor
-    static constexpr int JOIN = TOKENS + 2 * 4 * 128 * 4;
-    static constexpr int BARS = JOIN + (join_floats<kTcRows, 128, kTcParts>() * 4 + 15) / 16 * 16;
+    static constexpr int BARS = TOKENS + 2 * 4 * 128 * 4;
     static constexpr int BYTES = BARS + 80, ALLOC = BYTES + 1024;   // tiles start on 1024-byte boundaries
 };
 
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }   // warps 0 to 3
 __device__ __forceinline__ float tc_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -150,7 +150,6 @@ template <int PREC, int DP>
 __global__ void __launch_bounds__(kTcThreads, 2) pool_attention_tc_kernel(const __grid_constant__ skv_pool_attention_args a, bool out_vec) {
     using namespace sm100;
     using L = TcLayout<DP>;
-    using Sync = FirstThreadsSync<128>;
     extern __shared__ uint8_t tc_raw[];
     __shared__ Share s;
     __shared__ uint32_t s_tmem;
@@ -246,7 +245,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) pool_attention_tc_kernel(const 
                 }
             }
             fence_proxy_async_smem();
-            Sync::sync();
+            softmax_sync();
             for (int t = sg.t0; t < sg.t1; ++t, ++g) {
                 if (tid == 0 && ok && mbar_wait_spin(k_full + (g & 1), g >> 1 & 1, &s_error, 1)) {
                     tc_fence_after();
@@ -367,7 +366,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) pool_attention_tc_kernel(const 
                 }
                 tmem_wait_st();
                 tc_fence_before();
-                Sync::sync();
+                softmax_sync();
                 if (tid == 0 && ok && mbar_wait_spin(v_full, g & 1, &s_error, 4)) {
                     tc_fence_after();
 #pragma unroll
@@ -427,13 +426,9 @@ __global__ void __launch_bounds__(kTcThreads, 2) pool_attention_tc_kernel(const 
                 __syncwarp();
             }
             tc_fence_before();
-            if (!sg.whole) {
-                if (tid < sg.rows) {
-                    part[kTcRows * D + tid] = ref;
-                    part[kTcRows * D + kTcRows + tid] = ok ? l : nan;
-                }
-                if (arrive<Sync>(a, s, sg))
-                    join<kTcRows, 128, 4, kTcParts, Sync>(a, s, sg, sg.r0, sg.rows, reinterpret_cast<float*>(sm + L::JOIN), out_vec);
+            if (!sg.whole && tid < sg.rows) {
+                part[kTcRows * D + tid] = ref;
+                part[kTcRows * D + kTcRows + tid] = ok ? l : nan;
             }
         }
         if (tid == 0 && issued) {   // every MMA has completed before TMEM is freed
@@ -561,10 +556,136 @@ __global__ void __launch_bounds__(kTcThreads, 2) pool_attention_tc_kernel(const 
     if (tid == 0 && s_error && a.error_flag) atomicExch(a.error_flag, 1);
 }
 
+// Joins the parts of the units that the shares of `ctas` CTAs cut, in token order.  A launch of its own: a part is 64 KB, and one
+// CTA would fetch no more than 30 GB/s of them (with the last CTA to arrive joining, 128 rows of 8 key heads over 16384 tokens
+// took 228 us, so 56).  Few units have many parts each: a block takes 16 rows of unit blockIdx.x.  Many have few: with `by_cta` it
+// takes all rows of the unit that CTA blockIdx.x began and did not finish.
+constexpr int kTcMaxParts = 512, kTcJoinRows = 16;
+template <int DP>
+__global__ void __launch_bounds__(256) pool_attention_tc_join_kernel(const __grid_constant__ skv_pool_attention_args a, int ctas, bool by_cta,
+                                                                     bool out_vec) {
+    __shared__ Share s;
+    __shared__ int s_sum[2];
+    __shared__ float s_f[kTcMaxParts][kTcJoinRows];   // 2^(m_i - m) of a part
+    __shared__ float s_l[kTcJoinRows];
+    const int tid = threadIdx.x, D = a.pool.head_dim;
+    const TcUnits u(a);
+    int b, base, at;
+    const auto cost = [&](int i) {
+        int tokens, n, past;
+        u.sequence(a, i, tokens, n, past);
+        return u.a_head(n, past, kTcPad) * a.pool.heads;
+    };
+    Share sh;
+    if (by_cta) {
+        take_share<256>(a, cost, kTcPad, 1, &s);
+        sh = s;
+        if (sh.lo >= sh.hi) return;
+        b = sh.b;
+        base = sh.base;
+        at = sh.hi - 1;
+    } else {
+        const int per = u.row_tiles * a.pool.heads;
+        b = blockIdx.x / per;
+        int before = 0, all = 0;
+        for (int i = tid; i < a.pool.batch; i += 256) {
+            const int c = cost(i);
+            all += c;
+            before += i < b ? c : 0;
+        }
+        if (tid < 2) s_sum[tid] = 0;
+        __syncthreads();
+        before = __reduce_add_sync(0xffffffffu, before);
+        all = __reduce_add_sync(0xffffffffu, all);
+        if (tid % 32 == 0) {
+            atomicAdd(&s_sum[0], before);
+            atomicAdd(&s_sum[1], all);
+        }
+        __syncthreads();
+        base = s_sum[0];
+        sh.cut(s_sum[1], ctas, 1, kTcPad);
+        sh.lo = 0;
+        sh.hi = sh.total;
+        int tokens, n, past;
+        u.sequence(a, b, tokens, n, past);
+        const int unit = blockIdx.x - b * per, hk = unit / u.row_tiles, rt = unit - hk * u.row_tiles, each = u.a_head(n, past, kTcPad);
+        at = base + hk * each + (u.blocks ? rt / u.blocks * (each / u.rep) + u.before(rt % u.blocks, n, past, kTcPad) : rt * (n + kTcPad));
+    }
+    const TcSegment g = tc_segment_at(a, u, sh, at, b, base);
+    const int c0 = sh.owner_of(g.first), parts = sh.owner_of(g.last) - c0 + 1;
+    if (parts == 1 || (by_cta && c0 != (int)blockIdx.x)) return;
+    const int64_t stride = (int64_t)2 * kTcRows * (D + 2);
+    const float* next = slot_of(a, c0, 0, kTcRows);
+    const float* part0 = slot_of(a, c0, g.first == sh.first_of(c0) ? 0 : 1, kTcRows);
+    auto part = [&](int i) { return i == 0 ? part0 : next + i * stride; };
+    for (int r_block = blockIdx.y * kTcJoinRows; r_block < g.rows; r_block += gridDim.y * kTcJoinRows) {
+        __syncthreads();
+        {
+            const int j = tid / 16, sub = tid % 16, row = min(r_block + j, g.rows - 1);
+            float m = -INFINITY, l = 0.0f;
+            for (int i = sub; i < parts; i += 16) {
+                const float mi = __ldcg(part(i) + kTcRows * D + row);
+                s_f[i][j] = mi;
+                m = fmaxf(m, mi);
+            }
+#pragma unroll
+            for (int w = 1; w < 16; w <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+            const float r = m == -INFINITY ? 0.0f : m;
+            for (int i = sub; i < parts; i += 16) {
+                const float f = exp2f(s_f[i][j] - r);
+                s_f[i][j] = f;
+                l += __ldcg(part(i) + kTcRows * D + kTcRows + row) * f;
+            }
+#pragma unroll
+            for (int w = 1; w < 16; w <<= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+            if (sub == 0) s_l[j] = l;
+        }
+        __syncthreads();
+        constexpr int PER = kTcJoinRows * DP / 4 / 256;   // values (4 at a time) of a thread
+        float y[PER][4];
+        int row[PER], d[PER];
+#pragma unroll
+        for (int n = 0; n < PER; ++n) {
+            row[n] = (tid + 256 * n) / (DP / 4);
+            d[n] = (tid + 256 * n) % (DP / 4) * 4;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[n][e] = 0.0f;
+        }
+        for (int i0 = 0; i0 < parts; i0 += 8) {
+            float x[8][PER][4];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int n = 0; n < PER; ++n) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[i][n][e] = 0.0f;
+                    if (i0 + i < parts && r_block + row[n] < g.rows && d[n] < D)
+                        load_part<4>(part(i0 + i) + (r_block + row[n]) * D + d[n], x[i][n]);
+                }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int n = 0; n < PER; ++n) {
+                    const float f = i0 + i < parts ? s_f[i0 + i][row[n]] : 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[n][e] = fmaf(x[i][n][e], f, y[n][e]);
+                }
+        }
+#pragma unroll
+        for (int n = 0; n < PER; ++n) {
+            if (r_block + row[n] >= g.rows || d[n] >= D) continue;
+            const float l = s_l[row[n]];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[n][e] = l == 0.0f ? 0.0f : y[n][e] / l;
+            store_row(a, g, g.r0 + r_block + row[n], d[n], out_vec, y[n]);
+        }
+    }
+}
+
 template <int PREC, int DP>
 int launch_tc(const skv_pool_attention_args& a, cudaStream_t st) {
     using L = TcLayout<DP>;
-    static_assert(2 * 2 * kTcRows <= kRowsPerSm, "the scratch holds every CTA's slots");
+    static_assert(DP <= kManyD && 2 * 2 * kTcRows <= kManyRowsPerSm, "the scratch holds every CTA's slots");
     static_assert(2 * (L::ALLOC + 2048) <= 228 * 1024, "an SM holds two CTAs");
     const auto kernel = pool_attention_tc_kernel<PREC, DP>;
     static std::atomic<uint64_t> allowed{0};   // devices whose limit on the kernel's shared memory was raised
@@ -575,7 +696,15 @@ int launch_tc(const skv_pool_attention_args& a, cudaStream_t st) {
         if (e == cudaSuccess && dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
     }
     if (e != cudaSuccess) return fail(SKV_ERR_CUDA, "pool_attention: %s", cudaGetErrorString(e));
-    kernel<<<sm_count() * 2, kTcThreads, L::ALLOC, st>>>(a, rows_aligned(a.out));
+    const int ctas = min(sm_count() * 2, kTcMaxParts);
+    const bool out_vec = rows_aligned(a.out);
+    kernel<<<ctas, kTcThreads, L::ALLOC, st>>>(a, out_vec);
+    const int rep = a.q.heads / a.pool.heads;
+    const int64_t units = a.pool.batch * (int64_t)a.pool.heads *
+                          (a.S_q >= kTcRows ? rep * ((a.S_q + kTcRows - 1) / kTcRows) : (rep * a.S_q + kTcRows - 1) / kTcRows);
+    const bool by_cta = units > ctas;
+    pool_attention_tc_join_kernel<DP><<<dim3(by_cta ? ctas : (int)units, by_cta ? 1 : kTcRows / kTcJoinRows), 256, 0, st>>>(a, ctas, by_cta,
+                                                                                                                  out_vec);
     return check_launch("pool_attention");
 }
 
