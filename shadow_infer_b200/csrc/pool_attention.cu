@@ -11,12 +11,17 @@
 //
 // Numbers.  Scores, the running maximum and sum and the accumulators are fp32; the scale and
 // log2(e) are folded into q.
+//
+// Three kernels: tensor cores for a few query rows a key head (pool_attention_mma.cuh), tcgen05 for many
+// (pool_attention_tc.cuh), and the one below for what neither takes: heads above 256 values or of odd sizes, pages that
+// are not on 16-byte boundaries.
 #include "pool_attention.cuh"
 
 namespace skv {
 
 // --------------------------------------------------------------------------- any size and alignment
-// Products on the FMA pipe from fp32 tiles in shared memory: 8 rows, 32 tokens at a time.  Thread = (token, rows w and
+// Products on the FMA pipe from fp32 tiles in shared memory: 8 rows, 32 tokens at a time (16384 tokens of 8 fp32 key heads of 128
+// values in 97 us, bound by the tiles' latency at 1.4 TB/s).  Thread = (token, rows w and
 // w + 4) for the scores, value d for the sums.  A warp widens 8 tokens a tile, a lane a value of each, so that 16 loads are on
 // their way; the lanes look up the tokens' rows one tile ahead.
 constexpr int kAnyRows = 8, kAnyTile = 32, kAnyThreads = 128, kAnyMaxD = 512, kAnyParts = 64, kAnyPad = 1;

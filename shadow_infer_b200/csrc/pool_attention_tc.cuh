@@ -15,6 +15,12 @@
 //                 cores read, and what a token's scales do to scores and weights; they run ahead across units.
 // Two CTAs share an SM (TMEM: 128 columns of S and P, 128 of O each), so that one's MMAs run during the other's softmax.
 //
+// What bounds it: neither pipe but the chain S -> softmax -> P V of two CTAs, 70 % of it softmax instructions (about 10 a weight of
+// int8 pages, 6 of fp16).  8 key heads of 4 query heads of 128 values: a prompt of 4096 fp16 tokens in 300 us (460 TFLOP/s of the
+// causal half's operations, 0.27 of cuBLAS's burst), int8 384 us, 8192 tokens 930 and 1240 us; 128 new tokens behind 16384 in 82
+// and 99 us.  Measured and dropped: a warp of its own for the MMAs (96 registers a thread: spills, twice the time), weights of all
+// 128 columns in registers until the maximum is known (spills), the next 32 scores fetched ahead (spills, 15 % slower).
+//
 // Numbers: as in pool_attention_mma.cuh.  Page values and queries are exact in fp16, an int8 row's scale multiplies its scores (K)
 // and weights (V) in fp32, a weight is rounded once, to fp16, at no more than 2^15.
 //
@@ -153,7 +159,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) pool_attention_tc_kernel(const 
     extern __shared__ uint8_t tc_raw[];
     __shared__ Share s;
     __shared__ uint32_t s_tmem;
-    __shared__ int s_error;
+    __shared__ int s_error, s_late;
     __shared__ __align__(16) int s_gap[2][4];   // whether the tile misses a token of the sequence, by the warp that looked it up
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tc_raw) + 1023) & ~uintptr_t(1023));
     float* s_tokens = reinterpret_cast<float*>(sm + L::TOKENS);
@@ -173,7 +179,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) pool_attention_tc_kernel(const 
         mbar_init(o_full, 1);
         mbar_init(drained, 1);
         fence_mbarrier_init();
-        s_error = 0;
+        s_error = s_late = 0;
     }
     take_share<kTcThreads>(a, [&](int b) {
         int tokens, n, past;
@@ -433,8 +439,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) pool_attention_tc_kernel(const 
         }
         if (tid == 0 && issued) {   // every MMA has completed before TMEM is freed
             umma_commit(drained);
-            int none = 0;
-            mbar_wait_spin(drained, 0, &none, 6);
+            mbar_wait_spin(drained, 0, &s_late, 6);   // (also after an error elsewhere, so not with s_error)
         }
         __syncwarp();
     } else {
