@@ -162,8 +162,8 @@ __device__ __forceinline__ float scale_of(float m, float top, float r) {
 // else 16 neighbours.  blockDim = (lanes a row: a power of two >= D / 16, rows at a time, tokens at a time); a block takes
 // FLY * rows heads of q, of k or of v (blockIdx.y: first the slices of q, then of k, then of v), every row asked for before the
 // token's position and page are known.  Every thread stays to the end: rows and int4 groups reduce over aligned lane blocks.
-// (16 values rather than 8 a lane halve what a row pays for its position, page and scale; three blocks an SM rather than two
-// hide what four rows on the way a thread do not: 112 us against 131 for the prompt above.)
+// (The prompt above with a warp a row: 845 us for append and read; blocks of one kind of rows and quotients without
+// divisions: append 163 -> 130; three blocks an SM, which hide what four rows on the way a thread do not: 112.)
 template <class T, bool SPLIT>
 __global__ void __launch_bounds__(256, 3) pool_append_kernel(const __grid_constant__ skv_pool_append_args a, int q_slices, int kv_slices) {
     constexpr int FLY = sizeof(T) == 2 ? 4 : 2;

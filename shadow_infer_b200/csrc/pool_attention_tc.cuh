@@ -15,8 +15,8 @@
 //                 cores read, and what a token's scales do to scores and weights; they run ahead across units.
 // Two CTAs share an SM (TMEM: 128 columns of S and P, 128 of O each), so that one's MMAs run during the other's softmax.
 //
-// What bounds it: neither pipe but the chain S -> softmax -> P V of two CTAs, 70 % of it softmax instructions (about 10 a weight of
-// int8 pages, 6 of fp16).  8 key heads of 4 query heads of 128 values: a prompt of 4096 fp16 tokens in 300 us (460 TFLOP/s of the
+// What bounds it: instructions and the chain S -> softmax -> P V of two CTAs; a tile of int8 pages takes 10 thousand warp
+// instructions (41 % of the issue slots; tensor pipe 20 %, exponentials 21 % busy).  8 key heads of 4 query heads of 128 values: a prompt of 4096 fp16 tokens in 300 us (460 TFLOP/s of the
 // causal half's operations, 0.27 of cuBLAS's burst), int8 384 us, 8192 tokens 930 and 1240 us; 128 new tokens behind 16384 in 82
 // and 99 us.  Measured and dropped: a warp of its own for the MMAs (96 registers a thread: spills, twice the time), weights of all
 // 128 columns in registers until the maximum is known (spills), the next 32 scores fetched ahead (spills, 15 % slower).
