@@ -46,8 +46,9 @@ __device__ __forceinline__ int seq_tiles(int tokens, int tile) { return max(1, (
 
 // Every thread of the block calls this; *s is valid for all after it.  At least min_tiles a CTA.
 // cost(b): the tiles of sequence b's units, with what each counts on top.
+// few: units that are not to be cut, as no sequence has more than min_tiles tiles (0: cut anywhere).
 template <int THREADS, class Cost>
-__device__ __forceinline__ void take_share(const skv_pool_attention_args& a, Cost cost, int pad, int min_tiles, Share* s) {
+__device__ __forceinline__ void take_share(const skv_pool_attention_args& a, Cost cost, int pad, int min_tiles, Share* s, int few = 0) {
     __shared__ int s_part[THREADS / 32];
     const int tid = threadIdx.x, lane = tid & 31, B = a.pool.batch;
     const int per = (B + THREADS - 1) / THREADS, b0 = min(B, tid * per), b1 = min(B, b0 + per);
@@ -69,7 +70,7 @@ __device__ __forceinline__ void take_share(const skv_pool_attention_args& a, Cos
     }
     before += incl - mine;
     Share t;
-    const int ctas = t.cut(total, gridDim.x, min_tiles, pad);
+    const int ctas = t.cut(total, few > 0 && few <= (int)gridDim.x ? few : gridDim.x, min_tiles, pad);
     const int c = blockIdx.x;
     t.lo = c < ctas ? t.first_of(c) : total;
     t.hi = c < ctas ? t.first_of(c + 1) : total;
@@ -93,7 +94,9 @@ __device__ __forceinline__ void take_share(const skv_pool_attention_args& a, Cos
 template <int THREADS>
 __device__ __forceinline__ void take_share(const skv_pool_attention_args& a, int tile, int units, int pad, int min_tiles,
                                            Share* s) {
-    take_share<THREADS>(a, [&](int b) { return (seq_tiles(seq_tokens(a, b), tile) + pad) * units; }, pad, min_tiles, s);
+    // a single short sequence: a CTA a unit and nothing to join (128 tokens of 32 fp16 heads 11.3 -> 7.8 us)
+    const bool whole = a.pool.batch == 1 && seq_tiles(seq_tokens(a, 0), tile) <= min_tiles;
+    take_share<THREADS>(a, [&](int b) { return (seq_tiles(seq_tokens(a, b), tile) + pad) * units; }, pad, min_tiles, s, whole ? units : 0);
 }
 
 // Tokens [0, n) of its sequence that query i of sequence b sees.
