@@ -211,7 +211,9 @@ int attend_int4(const skv_pool_attention_args& a, cudaStream_t st);
 // The tcgen05 kernel (pool_attention_tc.cuh), and the query rows a key head from which it is taken.  8 key heads of 4 query heads
 // and 128 values, us there / on the small kernel: 32 rows over 4 x 4096 fp16 tokens 32.5 / 34.7, int8 37.9 / 34.1; 48 rows 35.0 /
 // 40.8, int8 38.4 / 41.9; 64 rows 34.3 / 47.3, int8 39.8 / 49.1; 128 rows over 512 tokens 20.2 / 17.5, over 16384 45.6 / 73.1.
-constexpr int kManyRows = 48;
+// Heads of 256 values (2 query heads), which leave an SM one CTA: 48 rows over 4096 fp16 tokens 37.4 / 38.1, int8 40.8 / 31.8; 64
+// rows over 4 x 4096 65 / 96, int8 79 / 81; a prompt of 2048 145 / 603, int8 159 / 525.
+constexpr int many_rows(int D) { return D <= 128 ? 48 : 64; }
 int attend_many(const skv_pool_attention_args& a, cudaStream_t st);
 
 // They need heads of up to 256 values in rows of whole 16-byte (fp16) or 8-byte chunks, int4 groups of whole 16-value blocks,
@@ -225,9 +227,9 @@ bool fits_mma(const skv_pool& p) {
 }
 
 // The tcgen05 kernel takes fp16 and int8 pages, whose values are exact in fp16, 16-bit queries (32-bit ones want sums that the
-// tensor cores do not cut off), heads of up to 128 values in whole swizzled chunks of 16.
+// tensor cores do not cut off), heads of up to 256 values in whole swizzled chunks of 16.
 bool fits_tc(const skv_pool_attention_args& a) {
-    return a.q.heads / a.pool.heads * (int64_t)a.S_q >= kManyRows && a.q.dtype != kF32 &&
+    return a.q.heads / a.pool.heads * (int64_t)a.S_q >= many_rows(a.pool.head_dim) && a.q.dtype != kF32 &&
            (a.pool.precision == 1 || a.pool.precision == 2) && a.pool.head_dim <= kManyD && a.pool.head_dim % 16 == 0 && rows_aligned(a.q);
 }
 
@@ -238,7 +240,7 @@ using namespace skv;
 extern "C" {
 
 size_t skv_pool_attention_scratch_bytes(int D) {
-    return D <= 0 ? 0 : (size_t)kMaxCtas * 4 + (size_t)sm_count() * (D <= kManyD ? kManyRowsPerSm : kRowsPerSm) * (D + 2) * 4;
+    return D <= 0 ? 0 : (size_t)kMaxCtas * 4 + (size_t)sm_count() * rows_per_sm(D) * (D + 2) * 4;
 }
 
 size_t skv_pool_attention_scratch_zeros(void) { return (size_t)kMaxCtas * 4; }

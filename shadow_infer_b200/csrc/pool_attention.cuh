@@ -7,8 +7,9 @@
 namespace skv {
 
 constexpr int kMaxCtas = 4096;      // arrival counters in the scratch
-// Rows of partial results in the scratch for each SM, CTAs x 2 slots x rows: for heads that the tcgen05 kernel takes, and others.
-constexpr int kRowsPerSm = 128, kManyRowsPerSm = 512, kManyD = 128;
+// Rows of partial results in the scratch for each SM, CTAs x 2 slots x rows; the tcgen05 kernel takes heads of up to kManyD values.
+constexpr int kRowsPerSm = 128, kManyD = 256;
+__host__ __device__ constexpr int rows_per_sm(int D) { return D <= 128 ? 512 : D <= kManyD ? 256 : kRowsPerSm; }
 
 // ------------------------------------------------------------------------------ shares of the work
 // Tile numbers fit 31 bits (the launch checks the most that the table allows).

@@ -3,8 +3,8 @@
 
 namespace skv {
 int attend_many(const skv_pool_attention_args& a, cudaStream_t st) {
-    const bool narrow = a.pool.head_dim <= 64;
-    if (a.pool.precision == 1) return narrow ? launch_tc<1, 64>(a, st) : launch_tc<1, 128>(a, st);
-    return narrow ? launch_tc<2, 64>(a, st) : launch_tc<2, 128>(a, st);
+    const int D = a.pool.head_dim;
+    if (a.pool.precision == 1) return D <= 64 ? launch_tc<1, 64>(a, st) : D <= 128 ? launch_tc<1, 128>(a, st) : launch_tc<1, 256>(a, st);
+    return D <= 64 ? launch_tc<2, 64>(a, st) : D <= 128 ? launch_tc<2, 128>(a, st) : launch_tc<2, 256>(a, st);
 }
 }  // namespace skv

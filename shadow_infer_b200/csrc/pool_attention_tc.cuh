@@ -13,7 +13,8 @@
 //                 only take registers: 256 threads leave two CTAs 128 each, with 96 the softmax spilled);
 //     warps 4-7   each tile's page rows: fp16 copied, int8 made fp16 integers (exact), in the swizzled layout that the tensor
 //                 cores read, and what a token's scales do to scores and weights; they run ahead across units.
-// Two CTAs share an SM (TMEM: 128 columns of S and P, 128 of O each), so that one's MMAs run during the other's softmax.
+// Two CTAs share an SM (TMEM: 128 columns of S and P, 128 of O each), so that one's MMAs run during the other's softmax.  Heads
+// of more than 128 values leave room for one.
 //
 // What bounds it: instructions and the chain S -> softmax -> P V of two CTAs; a tile of int8 pages takes 10 thousand warp
 // instructions (41 % of the issue slots; tensor pipe 20 %, exponentials 21 % busy).  8 key heads of 4 query heads of 128 values: a prompt of 4096 fp16 tokens in 300 us (460 TFLOP/s of the
@@ -34,7 +35,7 @@
 
 namespace skv {
 
-constexpr int kTcTile = 128, kTcRows = 128, kTcThreads = 256, kTcPad = 1, kTcColumns = 256;
+constexpr int kTcTile = 128, kTcRows = 128, kTcThreads = 256, kTcPad = 1;
 // A fresh maximum's weight is 2^10 to 2^11 and may grow to 2^15: with one fp16 operand a weight, its subnormals' 2^-25 is then
 // 2^-35 of the largest weight.
 constexpr float kTcDrop = 11.0f, kTcRoom = 14.0f;
@@ -122,6 +123,7 @@ struct TcLayout {
     static constexpr int TILE = DP / 64 * 128 * 128;   // atoms of 128 rows of 64 values
     static constexpr int Q = 0, K = TILE, V = 2 * TILE;
     static constexpr int TOKENS = 3 * TILE;            // [2][4][128] of a tile's tokens: score factor, score term, weight factor, 1 / sum factor
+    static constexpr int CTAS = DP > 128 ? 1 : 2, COLUMNS = DP > 128 ? 512 : 256;   // on an SM; of TMEM (128 for S, DP for O)
     static constexpr int BARS = TOKENS + 2 * 4 * 128 * 4;
     static constexpr int BYTES = BARS + 80, ALLOC = BYTES + 1024;   // tiles start on 1024-byte boundaries
 };
@@ -153,7 +155,7 @@ __device__ __forceinline__ uint32_t tc_i8_pair(uint32_t biased, uint32_t sel) {
 }
 
 template <int PREC, int DP>
-__global__ void __launch_bounds__(kTcThreads, 2) pool_attention_tc_kernel(const __grid_constant__ skv_pool_attention_args a, bool out_vec) {
+__global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention_tc_kernel(const __grid_constant__ skv_pool_attention_args a, bool out_vec) {
     using namespace sm100;
     using L = TcLayout<DP>;
     extern __shared__ uint8_t tc_raw[];
@@ -188,7 +190,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) pool_attention_tc_kernel(const 
     }, kTcPad, 1, &s);
     if (s.lo >= s.hi) return;
     if (warp == 0) {
-        tmem_alloc(&s_tmem, kTcColumns);
+        tmem_alloc(&s_tmem, L::COLUMNS);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -556,7 +558,7 @@ __global__ void __launch_bounds__(kTcThreads, 2) pool_attention_tc_kernel(const 
     __syncthreads();
     if (warp == 0) {
         tc_fence_after();
-        tmem_dealloc(tmem, kTcColumns);
+        tmem_dealloc(tmem, L::COLUMNS);
     }
     if (tid == 0 && s_error && a.error_flag) atomicExch(a.error_flag, 1);
 }
@@ -690,8 +692,8 @@ __global__ void __launch_bounds__(256) pool_attention_tc_join_kernel(const __gri
 template <int PREC, int DP>
 int launch_tc(const skv_pool_attention_args& a, cudaStream_t st) {
     using L = TcLayout<DP>;
-    static_assert(DP <= kManyD && 2 * 2 * kTcRows <= kManyRowsPerSm, "the scratch holds every CTA's slots");
-    static_assert(2 * (L::ALLOC + 2048) <= 228 * 1024, "an SM holds two CTAs");
+    static_assert(L::CTAS * 2 * kTcRows <= rows_per_sm(DP), "the scratch holds every CTA's slots");
+    static_assert(L::CTAS * (L::ALLOC + 2048) <= 228 * 1024, "an SM holds the CTAs");
     const auto kernel = pool_attention_tc_kernel<PREC, DP>;
     static std::atomic<uint64_t> allowed{0};   // devices whose limit on the kernel's shared memory was raised
     int dev = 0;
@@ -701,7 +703,7 @@ int launch_tc(const skv_pool_attention_args& a, cudaStream_t st) {
         if (e == cudaSuccess && dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
     }
     if (e != cudaSuccess) return fail(SKV_ERR_CUDA, "pool_attention: %s", cudaGetErrorString(e));
-    const int ctas = min(sm_count() * 2, kTcMaxParts);
+    const int ctas = min(sm_count() * L::CTAS, kTcMaxParts);
     const bool out_vec = rows_aligned(a.out);
     kernel<<<ctas, kTcThreads, L::ALLOC, st>>>(a, out_vec);
     const int rep = a.q.heads / a.pool.heads;

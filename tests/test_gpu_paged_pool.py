@@ -403,6 +403,9 @@ MANY_ROWS = [  # counts, H, rep, Sq, D, P, new, causal: 48 query rows a key head
     ([333, 90] * 16, 4, 8, 9, 112, 11, [9, 4] * 16, True),
     ([260, 33] * 16, 4, 64, 1, 32, 16, None, False),         # many heads, one token
     ([77, 12], 1, 50, 1, 16, 64, None, False),
+    ([300, 77, 0] * 6, 8, 2, 33, 256, 32, None, True),       # heads of more than 128 values
+    ([900, 140], 3, 2, 140, 160, 17, None, True),
+    ([2500], 1, 8, 31, 192, 16, None, False),
 ]
 
 
