@@ -226,11 +226,12 @@ bool fits_mma(const skv_pool& p) {
     return ((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v)) & 15) == 0;
 }
 
-// The tcgen05 kernel takes fp16 and int8 pages, whose values are exact in fp16, 16-bit queries (32-bit ones want sums that the
-// tensor cores do not cut off), heads of up to 256 values in whole swizzled chunks of 16.
+// The tcgen05 kernel takes 16-bit queries (32-bit ones want sums that the tensor cores do not cut off) over fp16, int8 and int4
+// pages, heads of up to 256 values in whole swizzled chunks of 16, int4 rows in whole 16-byte chunks.
 bool fits_tc(const skv_pool_attention_args& a) {
-    return a.q.heads / a.pool.heads * (int64_t)a.S_q >= many_rows(a.pool.head_dim) && a.q.dtype != kF32 &&
-           (a.pool.precision == 1 || a.pool.precision == 2) && a.pool.head_dim <= kManyD && a.pool.head_dim % 16 == 0 && rows_aligned(a.q);
+    const int D = a.pool.head_dim;
+    return a.q.heads / a.pool.heads * (int64_t)a.S_q >= many_rows(D) && a.q.dtype != kF32 && a.pool.precision != 0 && D <= kManyD &&
+           D % (a.pool.precision == 3 ? 32 : 16) == 0 && rows_aligned(a.q);
 }
 
 }  // namespace skv

@@ -1,7 +1,7 @@
 // Attention over the page pool for many query rows a key head: blocks of new tokens and whole prompts.
 //
 // A few query rows leave tcgen05 idle (pool_attention_mma.cuh), 128 fill it: a unit is (sequence, key head, 128 query rows), and
-//     S [128 rows x 128 tokens] = Q K^T,     O [128 rows x D] += P V
+//     S [128 rows x 128 tokens] = Q K^T,     O [128 rows x D] += P V     (int4 pages: 64 tokens)
 // run as tcgen05.mma with the sums in TMEM.  Where a head has 128 new tokens or more a unit's rows are neighbours of one head, and
 // with a causal limit the unit ends at the last token that its rows see: the shares count each unit's own tiles, by a closed
 // form, so a prompt costs its triangle.
@@ -11,19 +11,19 @@
 //                 back into TMEM over S's first columns; O read, divided and stored, or published for the join, at a unit's end.
 //                 They also lay out Q once a unit (a power of two taken out of each row).  Thread 0 issues the MMAs in between (they are on this role's path in any case, so a warp for them would
 //                 only take registers: 256 threads leave two CTAs 128 each, with 96 the softmax spilled);
-//     warps 4-7   each tile's page rows: fp16 copied, int8 made fp16 integers (exact), in the swizzled layout that the tensor
-//                 cores read, and what a token's scales do to scores and weights; they run ahead across units.
+//     warps 4-7   each tile's page rows: fp16 copied, int8 made fp16 integers (exact), int4 fp16 values in two parts (so its
+//                 tiles have 64 tokens, in the same memory), in the swizzled layout that the tensor cores read, and what a token's scales do to scores and weights; they run ahead across units.
 // Two CTAs share an SM (TMEM: 128 columns of S and P, 128 of O each), so that one's MMAs run during the other's softmax.  Heads
 // of more than 128 values leave room for one.
 //
 // What bounds it: instructions and the chain S -> softmax -> P V of two CTAs; a tile of int8 pages takes 10 thousand warp
 // instructions (41 % of the issue slots; tensor pipe 20 %, exponentials 21 % busy).  8 key heads of 4 query heads of 128 values: a prompt of 4096 fp16 tokens in 300 us (460 TFLOP/s of the
-// causal half's operations, 0.27 of cuBLAS's burst), int8 384 us, 8192 tokens 930 and 1240 us; 128 new tokens behind 16384 in 82
-// and 99 us.  Measured and dropped: a warp of its own for the MMAs (96 registers a thread: spills, twice the time), weights of all
+// causal half's operations, 0.27 of cuBLAS's burst), int8 384 us, int4 535 us; 128 new tokens behind 16384 in 82, 99 and 135 us.
+// Measured and dropped: a warp of its own for the MMAs (96 registers a thread: spills, twice the time), weights of all
 // 128 columns in registers until the maximum is known (spills), the next 32 scores fetched ahead (spills, 15 % slower).
 //
 // Numbers: as in pool_attention_mma.cuh.  Page values and queries are exact in fp16, an int8 row's scale multiplies its scores (K)
-// and weights (V) in fp32, a weight is rounded once, to fp16, at no more than 2^15.
+// and weights (V) in fp32, int4 values are two operands (18 bits), a weight is rounded once, to fp16, at no more than 2^15.
 //
 // Every wait is bounded: after a second without progress the roles leave, TMEM is freed and the outputs are NaN.
 #pragma once
@@ -35,31 +35,36 @@
 
 namespace skv {
 
-constexpr int kTcTile = 128, kTcRows = 128, kTcThreads = 256, kTcPad = 1;
+constexpr int kTcRows = 128, kTcThreads = 256, kTcPad = 1;
 // A fresh maximum's weight is 2^10 to 2^11 and may grow to 2^15: with one fp16 operand a weight, its subnormals' 2^-25 is then
 // 2^-35 of the largest weight.
 constexpr float kTcDrop = 11.0f, kTcRoom = 14.0f;
 
+// Tokens a tile: an int4 value takes two operands, so its tiles are half as long.
+__host__ __device__ constexpr int tc_tile(int precision) { return precision == 3 ? 64 : 128; }
+
 // The units of a sequence and key head, and what each costs.
+template <int TILE>
 struct TcUnits {
+    static constexpr int STEP = kTcRows / TILE;   // tiles that a block sees more than the one before
     int S_q, rep, blocks, row_tiles;   // blocks: of 128 new tokens of a head (0: a unit's rows are any heads' and tokens')
     bool causal;
     __device__ __forceinline__ TcUnits(const skv_pool_attention_args& a)
         : S_q(a.S_q), rep(a.q.heads / a.pool.heads), blocks(a.S_q >= kTcRows ? (a.S_q + kTcRows - 1) / kTcRows : 0),
           row_tiles(blocks ? rep * blocks : (rep * a.S_q + kTcRows - 1) / kTcRows), causal(a.causal && blocks) {}
-    // With n tiles and `past` tiles before the new tokens, block i sees past + i + 1 tiles, at least one and no more than n.
-    __device__ __forceinline__ int tiles(int i, int n, int past) const { return causal ? min(max(past + i + 1, 1), n) : n; }
+    // With n tiles and `past` tiles before the new tokens, block i sees past + (i + 1) STEP tiles, at least one and no more than n.
+    __device__ __forceinline__ int tiles(int i, int n, int past) const { return causal ? min(max(past + (i + 1) * STEP, 1), n) : n; }
     // What blocks [0, k) cost.
     __device__ __forceinline__ int before(int k, int n, int past, int pad) const {
         if (!causal) return k * (n + pad);
-        const int lo = min(max(-past, 0), k), hi = min(max(n - past, lo), k);   // blocks below lo see one tile, from hi on n
-        return lo + (hi - lo) * (past + 1) + (hi * (hi - 1) - lo * (lo - 1)) / 2 + (k - hi) * n + k * pad;
+        const int lo = min(max(-past, 0) / STEP, k), hi = min(max((n - past) / STEP, lo), k);   // blocks below lo see one tile, from hi on n
+        return lo + (hi - lo) * past + STEP * (hi * (hi + 1) - lo * (lo + 1)) / 2 + (k - hi) * n + k * pad;
     }
     __device__ __forceinline__ void sequence(const skv_pool_attention_args& a, int b, int& tokens, int& n, int& past) const {
         tokens = seq_tokens(a, b);
-        n = seq_tiles(tokens, kTcTile);
+        n = seq_tiles(tokens, TILE);
         const int old = tokens - (a.new_lengths ? __ldg(a.new_lengths + b) : S_q);
-        past = old >= 0 ? (old + kTcTile - 1) / kTcTile : -((-old) / kTcTile);
+        past = old >= 0 ? (old + TILE - 1) / TILE : -((-old) / TILE);
     }
     __device__ __forceinline__ int a_head(int n, int past, int pad) const {   // a key head's units
         return blocks ? rep * before(blocks, n, past, pad) : row_tiles * (n + pad);
@@ -70,7 +75,8 @@ struct TcSegment : Segment {
     int r0, rows;   // the unit's query rows
 };
 
-__device__ __forceinline__ TcSegment tc_segment_at(const skv_pool_attention_args& a, const TcUnits& u, const Share& s, int at, int& b,
+template <int TILE>
+__device__ __forceinline__ TcSegment tc_segment_at(const skv_pool_attention_args& a, const TcUnits<TILE>& u, const Share& s, int at, int& b,
                                                    int& base) {
     TcSegment g;
     for (;;) {
@@ -121,6 +127,7 @@ __device__ __forceinline__ TcSegment tc_segment_at(const skv_pool_attention_args
 template <int DP>
 struct TcLayout {
     static constexpr int TILE = DP / 64 * 128 * 128;   // atoms of 128 rows of 64 values
+    static constexpr int PART = TILE / 2;              // of a tile of 64 tokens whose values have two parts
     static constexpr int Q = 0, K = TILE, V = 2 * TILE;
     static constexpr int TOKENS = 3 * TILE;            // [2][4][128] of a tile's tokens: score factor, score term, weight factor, 1 / sum factor
     static constexpr int CTAS = DP > 128 ? 1 : 2, COLUMNS = DP > 128 ? 512 : 256;   // on an SM; of TMEM (128 for S, DP for O)
@@ -170,7 +177,8 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
              *drained = bars + 7;   // k_full: of even and of odd tiles (the softmax may look when the next is full)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int D = a.pool.head_dim, P = a.pool.page_size, rep = a.q.heads / a.pool.heads;
-    const TcUnits u(a);
+    constexpr int TILE = tc_tile(PREC), PARTS = 128 / TILE;   // operands a value
+    const TcUnits<TILE> u(a);
     if (tid == 0) {
         mbar_init(k_full, 4);
         mbar_init(k_full + 1, 4);
@@ -258,11 +266,14 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
                 if (tid == 0 && ok && mbar_wait_spin(k_full + (g & 1), g >> 1 & 1, &s_error, 1)) {
                     tc_fence_after();
 #pragma unroll
-                    for (int i = 0; i < DP / 16; ++i) {
-                        const uint32_t off = (i >> 2) * (128 * 128) + (i & 3) * 32;
-                        umma_f16(tmem, smem_desc_sw128(q_tile + off, 16, 1024), smem_desc_sw128(k_tile + off, 16, 1024),
-                                 idesc_f16_f32(128, 128, false, false), i > 0);
-                    }
+                    for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+                        for (int i = 0; i < DP / 16; ++i) {
+                            const uint32_t in = (i & 3) * 32, atom = i >> 2;
+                            umma_f16(tmem, smem_desc_sw128(q_tile + atom * (128 * 128) + in, 16, 1024),
+                                     smem_desc_sw128(k_tile + part * L::PART + atom * (TILE * 128) + in, 16, 1024),
+                                     idesc_f16_f32(128, TILE, false, false), part + i > 0);
+                        }
                     umma_commit(s_full);
                     umma_commit(k_free);
                     issued = true;
@@ -273,14 +284,14 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
                                                        mbar_wait_spin(k_full + (g & 1), g >> 1 & 1, &s_error, 3));
                 tc_fence_after();
                 const float* tk = s_tokens + (g & 1) * 4 * 128;
-                const int left = see - t * kTcTile;   // columns that this row sees
+                const int left = see - t * TILE;   // columns that this row sees
                 const int4 gaps = *reinterpret_cast<const int4*>(s_gap[g & 1]);
-                const bool masked = see_min - t * kTcTile < kTcTile, gap = gaps.x | gaps.y | gaps.z | gaps.w;
+                const bool masked = see_min - t * TILE < TILE, gap = gaps.x | gaps.y | gaps.z | gaps.w;
                 // 32 columns at a time.  The reference is an integer that moves only where a weight would grow too large; what the
                 // old one scaled (O, the sum, the columns before) is a power of two off, which is exact.  (O holds the tiles
                 // before: s_full says that their MMAs are done.  16 columns of P replace S's that have been read.)
 #pragma unroll 1
-                for (int c = 0; c < 4 && ok; ++c) {
+                for (int c = 0; c < TILE / 32 && ok; ++c) {
                     float y[32];
                     {
                         uint32_t x[32];
@@ -288,7 +299,7 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
                         tmem_wait_ld();
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) {
-                            if constexpr (PREC == 2) {
+                            if constexpr (PREC >= 2) {
                                 const float4 k = *reinterpret_cast<const float4*>(tk + c * 32 + i);
                                 const float4 add = *reinterpret_cast<const float4*>(tk + 128 + c * 32 + i);
                                 y[i] = fmaf(__uint_as_float(x[i]), k.x * c_row, add.x);
@@ -354,14 +365,16 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
                     for (int i = 0; i < 32; i += 4) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) y[i + e] = tc_exp2(y[i + e] - base_of);
-                        if constexpr (PREC == 2) {
-                            const float4 v = *reinterpret_cast<const float4*>(tk + 256 + c * 32 + i);
+                        if constexpr (PREC >= 2) {
                             const float4 w = *reinterpret_cast<const float4*>(tk + 384 + c * 32 + i);
                             sum[0] = fmaf(y[i], w.x, sum[0]);
                             sum[1] = fmaf(y[i + 1], w.y, sum[1]);
                             sum[2] = fmaf(y[i + 2], w.z, sum[2]);
                             sum[3] = fmaf(y[i + 3], w.w, sum[3]);
-                            y[i] *= v.x; y[i + 1] *= v.y; y[i + 2] *= v.z; y[i + 3] *= v.w;
+                            if constexpr (PREC == 2) {
+                                const float4 v = *reinterpret_cast<const float4*>(tk + 256 + c * 32 + i);
+                                y[i] *= v.x; y[i + 1] *= v.y; y[i + 2] *= v.z; y[i + 3] *= v.w;
+                            }
                         } else {
 #pragma unroll
                             for (int e = 0; e < 4; ++e) sum[e] += y[i + e];
@@ -378,9 +391,11 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
                 if (tid == 0 && ok && mbar_wait_spin(v_full, g & 1, &s_error, 4)) {
                     tc_fence_after();
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        umma_f16_ts(tmem + 128, tmem + i * 8, smem_desc_sw128(v_tile + i * 16 * 128, 128 * 128, 1024),
-                                    idesc_f16_f32(128, DP, false, true), t > sg.t0 || i > 0);
+                    for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+                        for (int i = 0; i < TILE / 16; ++i)
+                            umma_f16_ts(tmem + 128, tmem + i * 8, smem_desc_sw128(v_tile + part * L::PART + i * 16 * 128, TILE * 128, 1024),
+                                        idesc_f16_f32(128, DP, false, true), t > sg.t0 || part + i > 0);
                     umma_commit(v_free);
                     if (t + 1 == sg.t1) umma_commit(o_full);
                 }
@@ -447,30 +462,93 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
     } else {
         // ------------------------------------------------------------------------- pages and queries
         const int pw = warp - 4;
-        constexpr int CHUNKS = PREC == 1 ? DP / 8 : DP / 16;   // 16-byte chunks of a row
-        constexpr int STEP = 32 / CHUNKS, N = 32 / STEP;       // rows that a warp takes at a time; a warp has 32 of a tile
+        constexpr int VALUES = PREC == 1 ? 8 : PREC == 2 ? 16 : 32;   // of a 16-byte chunk
+        constexpr int CHUNKS = DP / VALUES, ROWS = TILE / 4;          // chunks of a row, rows that a warp has of a tile
+        constexpr int STEP = 32 / CHUNKS, N = ROWS / STEP;            // rows that it takes at a time
         const int my_chunk = lane % CHUNKS, my_row = lane / CHUNKS;
-        const bool have_chunk = my_chunk * (PREC == 1 ? 8 : 16) < D;
-        const int row_bytes = PREC == 1 ? 2 * D : D;
-        uint4 k_raw[PREC == 2 ? N : 1], v_raw[PREC == 2 ? N : 1];   // int8: the next tile's, on their way
-        auto load = [&](uint4 (&raw)[PREC == 2 ? N : 1], const void* pages, int row) {
-            if constexpr (PREC == 2) {
+        const bool have_chunk = my_chunk * VALUES < D;
+        const int row_bytes = D / VALUES * 16;
+        const int groups = PREC == 3 ? D / a.pool.int4_group : 1;
+        const int block0 = PREC == 3 ? my_chunk * 32 / a.pool.int4_group : 0, block1 = PREC == 3 ? (my_chunk * 32 + 16) / a.pool.int4_group : 0;
+        // int8, int4: the next tile's chunks, and int4's scales of their halves, on their way
+        struct Ahead {
+            uint4 raw[PREC >= 2 ? N : 1];
+            float scale[PREC == 3 ? N : 1][2];
+            // the exponent field of the largest of row i's scales
+            __device__ __forceinline__ int exponent(int i) const {
+                uint32_t top = max(__float_as_uint(scale[i][0]) & 0x7fffffffu, __float_as_uint(scale[i][1]) & 0x7fffffffu);
+#pragma unroll
+                for (int w = 1; w < CHUNKS; w <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, w));
+                return min(max((int)(top >> 23), 35), 219);
+            }
+        } k_next, v_next;
+        auto load = [&](Ahead& next, const void* pages, const float* scales, int row) {
+            if constexpr (PREC >= 2) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const int x = __shfl_sync(0xffffffffu, row, i * STEP + my_row);
-                    raw[i] = make_uint4(0, 0, 0, 0);
-                    if (x >= 0 && have_chunk)
-                        raw[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const char*>(pages) + (int64_t)x * row_bytes + my_chunk * 16));
+                    const bool there = x >= 0 && have_chunk;
+                    next.raw[i] = make_uint4(0, 0, 0, 0);
+                    if (there)
+                        next.raw[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const char*>(pages) + (int64_t)x * row_bytes + my_chunk * 16));
+                    if constexpr (PREC == 3) {
+                        next.scale[i][0] = there ? __ldg(scales + (int64_t)x * groups + block0) : 0.0f;
+                        next.scale[i][1] = there ? __ldg(scales + (int64_t)x * groups + block1) : 0.0f;
+                    }
                 }
             }
         };
-        auto write = [&](const uint4 (&raw)[PREC == 2 ? N : 1], uint8_t* tile) {
+        auto write = [&](const Ahead& next, uint8_t* tile) {
+            if constexpr (PREC == 3) {
+                // A value is its integer times its scale (a power of two a token taken out), in two parts: times the scale's first 7
+                // bits, which is exact, and times the rest, rounded at 2^-18 of the value.  A byte becomes
+                // 1024 + 16 (n + 8) of its high nibble and 1024 + (n + 8) of its low one, and one exact fma both n.  Four chunks
+                // of an atom, the order exchanged for every second one (banks).
+                const int atom = my_chunk / 2, swap = atom & 1, c = my_chunk % 2 * 4;
+                const __half2 by = __floats2half2_rn(0.0625f, 1.0f), add = __floats2half2_rn(-72.0f, -1032.0f);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int x = pw * ROWS + i * STEP + my_row;
+                    const float down = __uint_as_float((uint32_t)(262 - next.exponent(i)) << 23);   // the largest scale to [2^8, 2^9)
+                    const uint32_t w[4] = {next.raw[i].x, next.raw[i].y, next.raw[i].z, next.raw[i].w};
+                    __half2 y[4][4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t z = (__byte_perm(w[j], 0, 0x4040 + 0x0101 * e) & 0x000F00F0u) | 0x64006400u;
+                            y[j][e] = __hfma2(*reinterpret_cast<const __half2*>(&z), by, add);
+                        }
+#pragma unroll
+                    for (int part = 0; part < 2; ++part) {
+                        __half2 f[2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float scale = next.scale[i][h] * down;
+                            const float first = __uint_as_float((__float_as_uint(scale) + 0x10000u) & 0xFFFE0000u);
+                            f[h] = __float2half2_rn(part == 0 ? first : scale - first);
+                        }
+                        uint8_t* line = tile + part * L::PART + atom * TILE * 128;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            uint32_t r[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const __half2 one = __hmul2(y[j][e], f[j / 2]), other = __hmul2(y[j ^ 2][e], f[1 - j / 2]);
+                                r[e] = swap ? *reinterpret_cast<const uint32_t*>(&other) : *reinterpret_cast<const uint32_t*>(&one);
+                            }
+                            *reinterpret_cast<uint4*>(line + sw128_offset(x, c + (swap ? j ^ 2 : j))) = make_uint4(r[0], r[1], r[2], r[3]);
+                        }
+                    }
+                }
+            }
             if constexpr (PREC == 2) {   // 16 values: two chunks of an atom, exchanged for every second atom (banks)
                 const int atom = my_chunk / 4, swap = atom & 1, c = my_chunk % 4 * 2;
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const int x = pw * 32 + i * STEP + my_row;
-                    const uint32_t w[4] = {raw[i].x ^ 0x80808080u, raw[i].y ^ 0x80808080u, raw[i].z ^ 0x80808080u, raw[i].w ^ 0x80808080u};
+                    const int x = pw * ROWS + i * STEP + my_row;
+                    const uint4 raw = next.raw[i];
+                    const uint32_t w[4] = {raw.x ^ 0x80808080u, raw.y ^ 0x80808080u, raw.z ^ 0x80808080u, raw.w ^ 0x80808080u};
                     const uint4 lo = make_uint4(tc_i8_pair(w[0], 0x4140), tc_i8_pair(w[0], 0x4342), tc_i8_pair(w[1], 0x4140), tc_i8_pair(w[1], 0x4342));
                     const uint4 hi = make_uint4(tc_i8_pair(w[2], 0x4140), tc_i8_pair(w[2], 0x4342), tc_i8_pair(w[3], 0x4140), tc_i8_pair(w[3], 0x4342));
                     uint8_t* line = tile + atom * 128 * 128;
@@ -484,7 +562,7 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const int x = __shfl_sync(0xffffffffu, row, i * STEP + my_row);
-                    const uint32_t to = smem_u32(tile + my_chunk / 8 * 128 * 128 + sw128_offset(pw * 32 + i * STEP + my_row, my_chunk % 8));
+                    const uint32_t to = smem_u32(tile + my_chunk / 8 * 128 * 128 + sw128_offset(pw * ROWS + i * STEP + my_row, my_chunk % 8));
                     const bool there = x >= 0 && have_chunk;
                     const char* from = static_cast<const char*>(pages) + (there ? (int64_t)x * row_bytes + my_chunk * 16 : 0);
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
@@ -500,10 +578,10 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
             const TcSegment sg = tc_segment_at(a, u, s, at, b, base);
             at = sg.next;
             if (sg.t0 >= sg.t1) continue;
-            // the pool row of this lane's token of a tile (tokens 32 pw .. of it), -1 where there is none
+            // the pool row of token lane % ROWS of this warp's ROWS of a tile, -1 where there is none
             bool gap;
             auto row_of = [&](int t) -> int {
-                const int tok = t * kTcTile + pw * 32 + lane;
+                const int tok = t * TILE + pw * ROWS + lane % ROWS;
                 gap = false;
                 if (t >= sg.t1 || tok >= sg.tokens) return -1;
                 const int64_t row = pool_row(a.pool, sg.b, tok);
@@ -512,10 +590,10 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
                 return row < 0 ? -1 : (int)row + sg.hk * P;
             };
             int row = row_of(sg.t0);
-            load(k_raw, a.pool.k, row);
-            load(v_raw, a.pool.v, row);
+            load(k_next, a.pool.k, a.pool.scale_k, row);
+            load(v_next, a.pool.v, a.pool.scale_v, row);
             for (int t = sg.t0; t < sg.t1; ++t, ++g) {
-                float* tk = s_tokens + (g & 1) * 4 * 128 + pw * 32 + lane;
+                float* tk = s_tokens + (g & 1) * 4 * 128 + pw * ROWS + lane % ROWS;
                 float sk = 0.0f, sv = 1.0f;
                 if (PREC == 2 && row >= 0) {
                     sk = __ldg(a.pool.scale_k + row);
@@ -526,7 +604,7 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
                 // the scores of the tile before are done: K is free, and what the softmax of the tile before that read
                 if (g > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait_spin(k_free, (g - 1) & 1, &s_error, 7));
                 if (!ok) break;
-                write(k_raw, sm + L::K);
+                write(k_next, sm + L::K);
                 copy(sm + L::K, a.pool.k, row);
                 if constexpr (PREC == 2) {   // V's scale as a power of two in the exponent and a factor in [1, 2)
                     const int e = min(max((int)((__float_as_uint(sv) & 0x7fffffffu) >> 23), 35), 219);
@@ -535,20 +613,32 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
                     tk[128] = row >= 0 ? (float)(e - 127) : -INFINITY;
                     tk[256] = sv * down;
                     tk[384] = down;
+                } else if constexpr (PREC == 3) {   // of the rows that this lane took, by the first lane of each
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const int ek = k_next.exponent(i), ev = v_next.exponent(i), x = i * STEP + my_row;
+                        const bool there = __shfl_sync(0xffffffffu, row, x) >= 0;
+                        float* of = s_tokens + (g & 1) * 4 * 128 + pw * ROWS + x;
+                        if (my_chunk == 0) {
+                            of[0] = __uint_as_float((uint32_t)(ek - 8) << 23);
+                            of[128] = there ? (float)(ev - 135) : -INFINITY;
+                            of[384] = __uint_as_float((uint32_t)(262 - ev) << 23);
+                        }
+                    }
                 } else {
                     tk[128] = row >= 0 ? 0.0f : -INFINITY;
                 }
                 if (lane == 0) s_gap[g & 1][pw] = any_gap;
                 if constexpr (PREC == 1) asm volatile("cp.async.wait_all;" ::: "memory");
                 publish(k_full + (g & 1));
-                load(k_raw, a.pool.k, next);
+                load(k_next, a.pool.k, a.pool.scale_k, next);
                 if (g > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait_spin(v_free, (g - 1) & 1, &s_error, 8));
                 if (!ok) break;
-                write(v_raw, sm + L::V);
+                write(v_next, sm + L::V);
                 copy(sm + L::V, a.pool.v, row);
                 if constexpr (PREC == 1) asm volatile("cp.async.wait_all;" ::: "memory");
                 publish(v_full);
-                load(v_raw, a.pool.v, next);
+                load(v_next, a.pool.v, a.pool.scale_v, next);
                 row = next;
             }
             ++units;
@@ -568,7 +658,7 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
 // took 228 us, so 56).  Few units have many parts each: a block takes 16 rows of unit blockIdx.x.  Many have few: with `by_cta` it
 // takes all rows of the unit that CTA blockIdx.x began and did not finish.
 constexpr int kTcMaxParts = 512, kTcJoinRows = 16;
-template <int DP>
+template <int DP, int TILE>
 __global__ void __launch_bounds__(256) pool_attention_tc_join_kernel(const __grid_constant__ skv_pool_attention_args a, int ctas, bool by_cta,
                                                                      bool out_vec) {
     __shared__ Share s;
@@ -576,7 +666,7 @@ __global__ void __launch_bounds__(256) pool_attention_tc_join_kernel(const __gri
     __shared__ float s_f[kTcMaxParts][kTcJoinRows];   // 2^(m_i - m) of a part
     __shared__ float s_l[kTcJoinRows];
     const int tid = threadIdx.x, D = a.pool.head_dim;
-    const TcUnits u(a);
+    const TcUnits<TILE> u(a);
     int b, base, at;
     const auto cost = [&](int i) {
         int tokens, n, past;
@@ -710,7 +800,7 @@ int launch_tc(const skv_pool_attention_args& a, cudaStream_t st) {
     const int64_t units = a.pool.batch * (int64_t)a.pool.heads *
                           (a.S_q >= kTcRows ? rep * ((a.S_q + kTcRows - 1) / kTcRows) : (rep * a.S_q + kTcRows - 1) / kTcRows);
     const bool by_cta = units > ctas;
-    pool_attention_tc_join_kernel<DP><<<dim3(by_cta ? ctas : (int)units, by_cta ? 1 : kTcRows / kTcJoinRows), 256, 0, st>>>(a, ctas, by_cta,
+    pool_attention_tc_join_kernel<DP, tc_tile(PREC)><<<dim3(by_cta ? ctas : (int)units, by_cta ? 1 : kTcRows / kTcJoinRows), 256, 0, st>>>(a, ctas, by_cta,
                                                                                                                   out_vec);
     return check_launch("pool_attention");
 }
