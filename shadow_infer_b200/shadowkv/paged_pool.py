@@ -29,8 +29,8 @@ from typing import Any, List, Optional, Sequence, Tuple
 import torch
 
 from .. import _lib
-from .._device import as_device, back, compute_device, device_ctx
-from .rotary import _DTYPE_CODE, _NO_ROWS, _launch, _like, _rope_fields, _rows
+from .._device import as_device, compute_device, device_ctx
+from .rotary import _DTYPE_CODE, _NO_ROWS, _back, _launch, _like, _rope_fields, _rows
 
 _PRECISION_CODE = {torch.float32: 0, torch.float16: 1, torch.int8: 2, torch.uint8: 3}
 _POOL, _ROWS, _ROPE = "QQQQQqiiiiiiii", "Qqqqii", "QQQqqiiiiii"
@@ -87,7 +87,7 @@ def _pool_fields(k_pages, v_pages, block_table, scale_k, scale_v, batch: int, he
         compute_device()   # raises where there is no CUDA device at all
         raise ValueError("the pages must be CUDA tensors")
     dev = k_pages.device
-    if v_pages.device != dev or not k_pages.is_contiguous() or not v_pages.is_contiguous():
+    if v_pages.get_device() != dev.index or not k_pages.is_contiguous() or not v_pages.is_contiguous():
         raise ValueError("the pages must be contiguous tensors on one device")
     N, H, P, row = shape
     D = (2 * row if code == 3 else row) if head_dim is None else head_dim
@@ -99,7 +99,7 @@ def _pool_fields(k_pages, v_pages, block_table, scale_k, scale_v, batch: int, he
             raise ValueError("int8/int4 pages need scale_k and scale_v")
         tail = scale_k.shape[3:]
         for s in (scale_k, scale_v):
-            if s.dtype is not torch.float32 or s.device != dev or s.shape[:3] != (N, H, P) or len(s.shape) != code + 2 \
+            if s.dtype is not torch.float32 or s.get_device() != dev.index or s.shape[:3] != (N, H, P) or len(s.shape) != code + 2 \
                     or s.shape[-1] != 1 or not s.is_contiguous():
                 raise ValueError(f"scales must be contiguous float32 [{N}, {H}, {P}, {'1' if code == 2 else 'groups, 1'}] "
                                  f"on {dev}, got {tuple(s.shape)} {s.dtype}")
@@ -154,14 +154,15 @@ def paged_append(
     The pages' precision is their type.  Rows and scales are those of ``PagedKVStore.append``
     (paged_kv_store.py:189-224): int8 ``amax / 127`` a row, int4 ``amax / 7`` a group.  One launch.
     """
-    if k.dim() != 4 or v.dim() != 4:
-        raise ValueError(f"k/v must be 4-D [batch, heads, tokens, head_dim], got k.dim={k.dim()}, v.dim={v.dim()}")
-    if k.shape != v.shape:
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape:
+        if k.dim() != 4 or v.dim() != 4:
+            raise ValueError(f"k/v must be 4-D [batch, heads, tokens, head_dim], got k.dim={k.dim()}, v.dim={v.dim()}")
         raise ValueError(f"k/v shapes disagree: {tuple(k.shape)} vs {tuple(v.shape)}")
-    B, H, S, D = k.shape
+    B, H, S, D = shape
     pool, dev, table = _pool_fields(k_pages, v_pages, block_table, scale_k, scale_v, B, D)
-    if H != k_pages.shape[1]:
-        raise ValueError(f"k/v have {H} heads, the pool has {k_pages.shape[1]}")
+    if H != pool[9]:
+        raise ValueError(f"k/v have {H} heads, the pool has {pool[9]}")
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin must be given together")
     lens = _index(lengths, (B,), dev, "lengths")
@@ -171,7 +172,8 @@ def paged_append(
     q_rows = q_out_rows = _NO_ROWS
     qd = q_out = None
     if q is not None:
-        if q.dim() != 4 or (q.shape[0], q.shape[2], q.shape[3]) != (B, S, D):
+        shape = q.shape
+        if len(shape) != 4 or shape != (B, shape[1], S, D):
             raise ValueError(f"q must be [batch, heads, {S}, {D}], got {tuple(q.shape)}")
         if cos is None:
             raise ValueError("q without cos and sin has nothing to be rotated by")
@@ -189,7 +191,7 @@ def paged_append(
     del table, keep, vd, qd
     if flag is not None:
         _raise_flag(flag, "paged_append")
-    return None if q_out is None else back(q_out, q.device)
+    return None if q_out is None else _back(q_out, q, dev)
 
 
 def paged_read(
@@ -265,9 +267,10 @@ def paged_attention(
     head.  The sequences are split over the whole GPU by their lengths on the device, long ones into
     parts that are joined in token order, so equal calls give equal bits.
     """
-    if q.dim() != 4:
+    shape = q.shape
+    if len(shape) != 4:
         raise ValueError(f"q must be 4-D [batch, heads, seq, head_dim], got shape {tuple(q.shape)}")
-    B, Hq, S_q, D = q.shape
+    B, Hq, S_q, D = shape
     pool, dev, table = _pool_fields(k_pages, v_pages, block_table, scale_k, scale_v, B, D)
     if Hq % pool[9]:
         raise ValueError(f"{Hq} query heads do not share {pool[9]} key heads evenly")
@@ -280,16 +283,15 @@ def paged_attention(
     with device_ctx(dev):
         stream = _lib.stream_of(dev)
         scratch = _scratch(dev, stream, D)
-        args = _ATTENTION.pack(*pool, *q_rows, *out_rows, lens.data_ptr(), 0 if new is None else new.data_ptr(),
-                               scratch.data_ptr(), scratch.numel(), 0 if flag is None else flag.data_ptr(), S_q, bool(causal),
-                               1.0 / math.sqrt(D) if scale is None else scale, 0)
-        st = entry(args, stream)
+        st = entry(_ATTENTION.pack(*pool, *q_rows, *out_rows, lens.data_ptr(), 0 if new is None else new.data_ptr(),
+                                   scratch.data_ptr(), scratch.numel(), 0 if flag is None else flag.data_ptr(), S_q, bool(causal),
+                                   1.0 / math.sqrt(D) if scale is None else scale, 0), stream)
     if st:
         _lib.check(st, "paged_attention")
     del table, qd
     if flag is not None:
         _raise_flag(flag, "paged_attention")
-    return back(out, q.device)
+    return _back(out, q, dev)
 
 
 class PagedKVPool:

@@ -14,7 +14,7 @@ from typing import Any, Optional, Tuple
 import torch
 
 from .. import _lib
-from .._device import as_device, back, compute_device, device_ctx
+from .._device import _get_device, as_device, back, compute_device, device_ctx
 
 _DTYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _ARGS = struct.Struct("<" + "Qqqqii" * 4 + "QQQqqiiiiii" + "iiii")   # skv_rotary_args
@@ -96,8 +96,15 @@ def _like(t: torch.Tensor):
 
 def _launch(entry, args: bytes, dev: torch.device) -> int:
     """``entry(args, stream)`` on ``dev`` and its current stream."""
+    if _get_device is not None and _get_device() == dev.index:
+        return entry(args, _lib.stream_of(dev))
     with device_ctx(dev):
         return entry(args, _lib.stream_of(dev))
+
+
+def _back(out: torch.Tensor, given: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """``out``, which lies on ``dev``, where ``given`` lies."""
+    return out if given.is_cuda and given.get_device() == dev.index else back(out, given.device)
 
 
 def _table_checked(t: torch.Tensor, dev: torch.device, name: str) -> torch.Tensor:
@@ -157,10 +164,11 @@ def apply_rotary(
     (slices of one projection's output, transposed views); products and sums are fp32, rounded once to the
     rows' type.  One launch for both tensors.
     """
-    if q.dim() != 4:
+    shape = q.shape
+    if len(shape) != 4:
         raise ValueError(f"q must be 4-D [batch, heads, seq, head_dim], got shape {tuple(q.shape)}")
-    B, _, S, D = q.shape
-    if k is not None and (k.dim() != 4 or (k.shape[0], k.shape[2], k.shape[3]) != (B, S, D)):
+    B, _, S, D = shape
+    if k is not None and (k.dim() != 4 or k.shape != (B, k.shape[1], S, D)):
         raise ValueError(f"q/k shapes disagree: {tuple(q.shape)} vs {tuple(k.shape)}")
     dev = q.device if q.is_cuda else compute_device(k, cos)
     qd, q_rows = _rows(q, dev)
@@ -177,5 +185,5 @@ def apply_rotary(
         _lib.check(st, "apply_rotary")
     del keep, kd
     if k is None:
-        return back(q_out, q.device)
-    return back(q_out, q.device), back(k_out, k.device)
+        return _back(q_out, q, dev)
+    return _back(q_out, q, dev), _back(k_out, k, dev)
