@@ -18,12 +18,14 @@
 //
 // What bounds it: instructions and the chain S -> softmax -> P V of two CTAs; a tile of int8 pages takes 10 thousand warp
 // instructions (41 % of the issue slots; tensor pipe 20 %, exponentials 21 % busy).  8 key heads of 4 query heads of 128 values: a prompt of 4096 fp16 tokens in 300 us (460 TFLOP/s of the
-// causal half's operations, 0.27 of cuBLAS's burst), int8 384 us, int4 535 us; 128 new tokens behind 16384 in 82, 99 and 135 us.
+// causal half's operations, 0.27 of cuBLAS's burst), int8 384 us, int4 535 us; 128 new tokens behind 16384 in 82, 99 and 135 us
+// (bf16; fp16 queries 5 to 15 % more).
 // Measured and dropped: a warp of its own for the MMAs (96 registers a thread: spills, twice the time), weights of all
 // 128 columns in registers until the maximum is known (spills), the next 32 scores fetched ahead (spills, 15 % slower).
 //
 // Numbers: as in pool_attention_mma.cuh.  Page values and queries are exact in fp16, an int8 row's scale multiplies its scores (K)
-// and weights (V) in fp32, int4 values are two operands (18 bits), a weight is rounded once, to fp16, at no more than 2^15.
+// and weights (V) in fp32, int4 values are two operands (18 bits).  A weight of at most 2^15 is one fp16 operand for bf16 outputs,
+// whose own rounding is 8 times coarser, else two (with one, fp16 outputs were up to twice as far off as rounding alone).
 //
 // Every wait is bounded: after a second without progress the roles leave, TMEM is freed and the outputs are NaN.
 #pragma once
@@ -161,7 +163,8 @@ __device__ __forceinline__ uint32_t tc_i8_pair(uint32_t biased, uint32_t sel) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-template <int PREC, int DP>
+// NP: fp16 operands of a weight.
+template <int PREC, int DP, int NP>
 __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention_tc_kernel(const __grid_constant__ skv_pool_attention_args a, bool out_vec) {
     using namespace sm100;
     using L = TcLayout<DP>;
@@ -178,6 +181,7 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int D = a.pool.head_dim, P = a.pool.page_size, rep = a.q.heads / a.pool.heads;
     constexpr int TILE = tc_tile(PREC), PARTS = 128 / TILE;   // operands a value
+    constexpr int COLUMNS = 16 * NP;                           // of P for 32 of S
     const TcUnits<TILE> u(a);
     if (tid == 0) {
         mbar_init(k_full, 4);
@@ -289,7 +293,7 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
                 const bool masked = see_min - t * TILE < TILE, gap = gaps.x | gaps.y | gaps.z | gaps.w;
                 // 32 columns at a time.  The reference is an integer that moves only where a weight would grow too large; what the
                 // old one scaled (O, the sum, the columns before) is a power of two off, which is exact.  (O holds the tiles
-                // before: s_full says that their MMAs are done.  16 columns of P replace S's that have been read.)
+                // before: s_full says that their MMAs are done.  P's columns replace S's that have been read.)
 #pragma unroll 1
                 for (int c = 0; c < TILE / 32 && ok; ++c) {
                     float y[32];
@@ -346,7 +350,7 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
                             }
                         }
 #pragma unroll 1
-                        for (int d = 0; d < c; ++d) {
+                        for (int d = 0; d < c * NP; ++d) {
                             uint32_t w[16];
                             tmem_wait_st();
                             tmem_ld16(t_s + d * 16, w);
@@ -360,7 +364,7 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
                         }
                     }
                     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    uint32_t p[16];
+                    uint32_t p[16], rest[NP == 2 ? 16 : 1];
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
 #pragma unroll
@@ -381,9 +385,17 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
                         }
                         p[i / 2] = tc_pack(y[i], y[i + 1]);
                         p[i / 2 + 1] = tc_pack(y[i + 2], y[i + 3]);
+                        if constexpr (NP == 2) {
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p[i / 2 + e]));
+                                rest[i / 2 + e] = tc_pack(y[i + 2 * e] - f.x, y[i + 2 * e + 1] - f.y);
+                            }
+                        }
                     }
                     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    tmem_st16(t_s + c * 16, p);
+                    tmem_st16(t_s + c * COLUMNS, p);
+                    if constexpr (NP == 2) tmem_st16(t_s + c * COLUMNS + 16, rest);
                 }
                 tmem_wait_st();
                 tc_fence_before();
@@ -391,11 +403,16 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
                 if (tid == 0 && ok && mbar_wait_spin(v_full, g & 1, &s_error, 4)) {
                     tc_fence_after();
 #pragma unroll
-                    for (int part = 0; part < PARTS; ++part)
+                    for (int w = 0; w < NP; ++w)
 #pragma unroll
-                        for (int i = 0; i < TILE / 16; ++i)
-                            umma_f16_ts(tmem + 128, tmem + i * 8, smem_desc_sw128(v_tile + part * L::PART + i * 16 * 128, TILE * 128, 1024),
-                                        idesc_f16_f32(128, DP, false, true), t > sg.t0 || part + i > 0);
+                        for (int part = 0; part < PARTS; ++part) {
+                            if (w + part > 1) continue;   // the small part of a value and the rest of a weight
+#pragma unroll
+                            for (int i = 0; i < TILE / 16; ++i)
+                                umma_f16_ts(tmem + 128, tmem + i / 2 * COLUMNS + i % 2 * 8 + w * 16,
+                                            smem_desc_sw128(v_tile + part * L::PART + i * 16 * 128, TILE * 128, 1024),
+                                            idesc_f16_f32(128, DP, false, true), t > sg.t0 || w + part + i > 0);
+                        }
                     umma_commit(v_free);
                     if (t + 1 == sg.t1) umma_commit(o_full);
                 }
@@ -779,12 +796,12 @@ __global__ void __launch_bounds__(256) pool_attention_tc_join_kernel(const __gri
     }
 }
 
-template <int PREC, int DP>
-int launch_tc(const skv_pool_attention_args& a, cudaStream_t st) {
+template <int PREC, int DP, int NP>
+int launch_tc_weights(const skv_pool_attention_args& a, cudaStream_t st) {
     using L = TcLayout<DP>;
     static_assert(L::CTAS * 2 * kTcRows <= rows_per_sm(DP), "the scratch holds every CTA's slots");
     static_assert(L::CTAS * (L::ALLOC + 2048) <= 228 * 1024, "an SM holds the CTAs");
-    const auto kernel = pool_attention_tc_kernel<PREC, DP>;
+    const auto kernel = pool_attention_tc_kernel<PREC, DP, NP>;
     static std::atomic<uint64_t> allowed{0};   // devices whose limit on the kernel's shared memory was raised
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -803,6 +820,11 @@ int launch_tc(const skv_pool_attention_args& a, cudaStream_t st) {
     pool_attention_tc_join_kernel<DP, tc_tile(PREC)><<<dim3(by_cta ? ctas : (int)units, by_cta ? 1 : kTcRows / kTcJoinRows), 256, 0, st>>>(a, ctas, by_cta,
                                                                                                                   out_vec);
     return check_launch("pool_attention");
+}
+
+template <int PREC, int DP>
+int launch_tc(const skv_pool_attention_args& a, cudaStream_t st) {
+    return a.q.dtype == kF16 ? launch_tc_weights<PREC, DP, 2>(a, st) : launch_tc_weights<PREC, DP, 1>(a, st);
 }
 
 }  // namespace skv
