@@ -17,6 +17,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from typing import List
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -60,16 +61,21 @@ def build(force: bool = False, ptxas_verbose: bool = False, verbose: bool = Fals
     os.makedirs(OBJ_DIR, exist_ok=True)
     os.makedirs(LIB_DIR, exist_ok=True)
     headers = _headers()
-    objs = []
+    objs, commands = [], []
     extra = ["-Xptxas", "-v"] if ptxas_verbose else []
     for src in _sources():
         obj = os.path.join(OBJ_DIR, os.path.basename(src)[:-3] + ".o")
         objs.append(obj)
         if force or ptxas_verbose or _stale(obj, [src] + headers):
-            cmd = [nvcc()] + ARCH_FLAGS + NVCC_FLAGS + extra + ["-c", src, "-o", obj]
-            if verbose:
-                print(" ".join(cmd), flush=True)
-            subprocess.run(cmd, check=True)
+            commands.append([nvcc()] + ARCH_FLAGS + NVCC_FLAGS + extra + ["-c", src, "-o", obj])
+
+    def run(cmd: List[str]) -> None:
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.run(cmd, check=True)
+
+    with ThreadPoolExecutor(max(1, min(8, os.cpu_count() or 1))) as pool:   # the sources compile side by side
+        list(pool.map(run, commands))
     if force or _stale(LIB_PATH, objs):
         cmd = [nvcc()] + ARCH_FLAGS + ["-shared", "-o", LIB_PATH] + objs + ["-cudart", "static"]
         if verbose:
