@@ -179,6 +179,8 @@ __global__ void __launch_bounds__(kAnyThreads) pool_attention_any_kernel(const _
 template <class T, int PREC>
 int launch_any_prec(const skv_pool_attention_args& a, cudaStream_t st) {
     const int R = a.q.heads / a.pool.heads * a.S_q, row_tiles = (R + kAnyRows - 1) / kAnyRows;
+    const int64_t step = sequences_a_launch(a, row_tiles, kAnyTile, kAnyPad);
+    if (step == 0) return SKV_ERR_TOO_LARGE;
     const size_t smem = any_smem(a.pool.head_dim);
     cudaError_t e = cudaFuncSetAttribute(pool_attention_any_kernel<T, PREC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)smem);
@@ -188,8 +190,10 @@ int launch_any_prec(const skv_pool_attention_args& a, cudaStream_t st) {
     if (e != cudaSuccess) return fail(SKV_ERR_CUDA, "pool_attention: %s", cudaGetErrorString(e));
     int grid = sm_count() * (per_sm < 1 ? 1 : per_sm > 8 ? 8 : per_sm);
     if (grid > kMaxCtas) grid = kMaxCtas;
-    pool_attention_any_kernel<T, PREC><<<grid, kAnyThreads, smem, st>>>(a, row_tiles);
-    return check_launch("pool_attention");
+    return by_sequences(a, step, [&](const skv_pool_attention_args& part) {
+        pool_attention_any_kernel<T, PREC><<<grid, kAnyThreads, smem, st>>>(part, row_tiles);
+        return check_launch("pool_attention");
+    });
 }
 
 template <class T>
@@ -263,9 +267,6 @@ int skv_pool_attention(const skv_pool_attention_args* args, void* stream) {
         return fail(SKV_ERR_UNSUPPORTED, "pool_attention: head_dim %d above %d", a.pool.head_dim, kAnyMaxD);
     if ((int64_t)a.q.heads * a.S_q > (1 << 28) || a.pool.batch > (1 << 24))
         return fail(SKV_ERR_TOO_LARGE, "pool_attention: too many rows");
-    const int64_t tiles = ((int64_t)a.pool.table_width * a.pool.page_size + kAnyTile - 1) / kAnyTile + 8;   // at least what a unit counts on top
-    if (tiles * a.pool.batch > 0x7fffffff / ((int64_t)a.q.heads * a.S_q))   // row tiles hold one row at least
-        return fail(SKV_ERR_TOO_LARGE, "pool_attention: more than 2^31 tiles of work");
     if (a.scratch_bytes < (int64_t)skv_pool_attention_scratch_bytes(a.pool.head_dim))
         return fail(SKV_ERR_SCRATCH, "pool_attention: scratch of %lld bytes", (long long)a.scratch_bytes);
     cudaStream_t st = as_stream(stream);

@@ -12,7 +12,7 @@ constexpr int kRowsPerSm = 128, kManyD = 256;
 __host__ __device__ constexpr int rows_per_sm(int D) { return D <= 128 ? 512 : D <= kManyD ? 256 : kRowsPerSm; }
 
 // ------------------------------------------------------------------------------ shares of the work
-// Tile numbers fit 31 bits (the launch checks the most that the table allows).
+// Tile numbers fit 31 bits: a launch takes no more sequences than the most that their tables allow (by_sequences).
 struct Share {
     int lo, hi, total;         // this CTA's tiles [lo, hi) of all
     int base;                  // tiles of the sequences before b
@@ -35,8 +35,13 @@ struct Share {
     }
 };
 
+// The most tokens of a sequence: what its table names, and what leaves room to round up to a tile in 31 bits.
+__host__ __device__ inline int64_t token_cap(const skv_pool_attention_args& a) {
+    const int64_t cap = (int64_t)a.pool.table_width * a.pool.page_size;
+    return cap < 0x7fffff00 ? cap : 0x7fffff00;
+}
 __device__ __forceinline__ int seq_tokens(const skv_pool_attention_args& a, int b) {
-    const int64_t n = __ldg(a.lengths + b), cap = (int64_t)a.pool.table_width * a.pool.page_size;
+    const int64_t n = __ldg(a.lengths + b), cap = token_cap(a);
     return (int)(n < 0 ? 0 : n > cap ? cap : n);
 }
 // Tiles of a sequence for one row tile of one head; an empty sequence keeps one, to write its zeros.
@@ -354,6 +359,33 @@ __device__ __forceinline__ void join(const skv_pool_attention_args& a, const Sha
         }
     }
     __syncthreads();
+}
+
+// How many sequences a launch takes at most, so that tile numbers hold their tiles (the lengths are on the device, so the tables'
+// width counts): row_tiles a key head, `tile` tokens each, `pad` on top of a unit.  0, with the failure recorded: not even one.
+inline int64_t sequences_a_launch(const skv_pool_attention_args& a, int64_t row_tiles, int tile, int pad) {
+    constexpr int64_t most = 1 << 30;   // half of 31 bits: sums on the way stay below them too
+    const int64_t tiles = (token_cap(a) + tile - 1) / tile, units = row_tiles * a.pool.heads, each = (tiles > 1 ? tiles : 1) + pad;
+    if (units <= most / each) return most / (units * each);
+    fail(SKV_ERR_TOO_LARGE, "pool_attention: %lld units of up to %lld tiles of %d tokens in one sequence", (long long)units, (long long)each, tile);
+    return 0;
+}
+
+// Launches the call, `step` sequences at a time.
+template <class Launch>
+int by_sequences(const skv_pool_attention_args& a, int64_t step, Launch launch) {
+    for (int64_t b = 0; b < a.pool.batch; b += step) {
+        skv_pool_attention_args part = a;
+        part.pool.batch = (int32_t)(a.pool.batch - b < step ? a.pool.batch - b : step);
+        part.pool.block_table += b * a.pool.table_stride;
+        part.q.ptr = static_cast<char*>(a.q.ptr) + b * a.q.stride_b * dtype_bytes(a.q.dtype);
+        part.out.ptr = static_cast<char*>(a.out.ptr) + b * a.out.stride_b * dtype_bytes(a.out.dtype);
+        part.lengths += b;
+        if (part.new_lengths) part.new_lengths += b;
+        const int rc = launch(part);
+        if (rc != SKV_OK) return rc;
+    }
+    return SKV_OK;
 }
 
 }  // namespace skv

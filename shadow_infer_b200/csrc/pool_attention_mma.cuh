@@ -1005,6 +1005,9 @@ int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
     static_assert(Shape::CTAS * 2 * 8 * NT <= kRowsPerSm, "the scratch holds every CTA's slots");
     constexpr size_t smem = mma_smem<PREC, DP, NT, NQ>();
     static_assert(Shape::CTAS * (smem + 2048) <= 228 * 1024, "an SM holds the CTAs");
+    const int R = a.q.heads / a.pool.heads * a.S_q, row_tiles = (R + 8 * NT - 1) / (8 * NT);
+    const int64_t step = sequences_a_launch(a, row_tiles, 16 * Shape::W, kMmaPad);
+    if (step == 0) return SKV_ERR_TOO_LARGE;
     const auto kernel = pool_attention_mma_kernel<PREC, DP, NT, NQ, NP>;
     static std::atomic<uint64_t> allowed{0};   // devices whose limit on the kernel's shared memory was raised
     int dev = 0;
@@ -1014,7 +1017,6 @@ int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
         if (e == cudaSuccess && dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
     }
     if (e != cudaSuccess) return fail(SKV_ERR_CUDA, "pool_attention: %s", cudaGetErrorString(e));
-    const int R = a.q.heads / a.pool.heads * a.S_q;
     PageDivide magic;
     magic.shift = 31;
     while ((1ll << (magic.shift - 31)) < a.pool.page_size) ++magic.shift;
@@ -1022,9 +1024,11 @@ int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
     const bool exact = a.pool.head_dim == DP &&
                        (PREC != 3 || (a.pool.int4_group == 16 && ((reinterpret_cast<uintptr_t>(a.pool.scale_k) |
                                                                    reinterpret_cast<uintptr_t>(a.pool.scale_v)) & 15) == 0));
-    kernel<<<sm_count() * Shape::CTAS, 32 * Shape::W, smem, st>>>(a, (R + 8 * NT - 1) / (8 * NT), magic, exact, rows_aligned(a.q),
-                                                                  rows_aligned(a.out));
-    return check_launch("pool_attention");
+    const bool q_vec = rows_aligned(a.q), out_vec = rows_aligned(a.out);
+    return by_sequences(a, step, [&](const skv_pool_attention_args& part) {
+        kernel<<<sm_count() * Shape::CTAS, 32 * Shape::W, smem, st>>>(part, row_tiles, magic, exact, q_vec, out_vec);
+        return check_launch("pool_attention");
+    });
 }
 
 template <int PREC, int DP, int NT>

@@ -801,6 +801,10 @@ int launch_tc_weights(const skv_pool_attention_args& a, cudaStream_t st) {
     using L = TcLayout<DP>;
     static_assert(L::CTAS * 2 * kTcRows <= rows_per_sm(DP), "the scratch holds every CTA's slots");
     static_assert(L::CTAS * (L::ALLOC + 2048) <= 228 * 1024, "an SM holds the CTAs");
+    const int rep = a.q.heads / a.pool.heads;
+    const int64_t row_tiles = a.S_q >= kTcRows ? (int64_t)rep * ((a.S_q + kTcRows - 1) / kTcRows) : ((int64_t)rep * a.S_q + kTcRows - 1) / kTcRows;
+    const int64_t step = sequences_a_launch(a, row_tiles, tc_tile(PREC), kTcPad);
+    if (step == 0) return SKV_ERR_TOO_LARGE;
     const auto kernel = pool_attention_tc_kernel<PREC, DP, NP>;
     static std::atomic<uint64_t> allowed{0};   // devices whose limit on the kernel's shared memory was raised
     int dev = 0;
@@ -812,14 +816,14 @@ int launch_tc_weights(const skv_pool_attention_args& a, cudaStream_t st) {
     if (e != cudaSuccess) return fail(SKV_ERR_CUDA, "pool_attention: %s", cudaGetErrorString(e));
     const int ctas = min(sm_count() * L::CTAS, kTcMaxParts);
     const bool out_vec = rows_aligned(a.out);
-    kernel<<<ctas, kTcThreads, L::ALLOC, st>>>(a, out_vec);
-    const int rep = a.q.heads / a.pool.heads;
-    const int64_t units = a.pool.batch * (int64_t)a.pool.heads *
-                          (a.S_q >= kTcRows ? rep * ((a.S_q + kTcRows - 1) / kTcRows) : (rep * a.S_q + kTcRows - 1) / kTcRows);
-    const bool by_cta = units > ctas;
-    pool_attention_tc_join_kernel<DP, tc_tile(PREC)><<<dim3(by_cta ? ctas : (int)units, by_cta ? 1 : kTcRows / kTcJoinRows), 256, 0, st>>>(a, ctas, by_cta,
-                                                                                                                  out_vec);
-    return check_launch("pool_attention");
+    return by_sequences(a, step, [&](const skv_pool_attention_args& part) {
+        kernel<<<ctas, kTcThreads, L::ALLOC, st>>>(part, out_vec);
+        const int64_t units = part.pool.batch * part.pool.heads * row_tiles;
+        const bool by_cta = units > ctas;
+        const dim3 grid(by_cta ? ctas : (int)units, by_cta ? 1 : kTcRows / kTcJoinRows);
+        pool_attention_tc_join_kernel<DP, tc_tile(PREC)><<<grid, 256, 0, st>>>(part, ctas, by_cta, out_vec);
+        return check_launch("pool_attention");
+    });
 }
 
 template <int PREC, int DP>

@@ -1,0 +1,66 @@
+"""The page pool's operators where they could go wrong: the largest and oddest calls, values that are not finite, and what
+a call may and may not write.  Bounds are those of test_gpu_paged_pool, whose helpers these tests use."""
+
+import math
+
+import pytest
+import torch
+from test_gpu_paged_pool import (  # noqa: F401  (skv is a fixture)
+    HALF, TINY, U, _attention64, _dense64, _filled, _gen, _pool, _rows, _table, _turn32, _turn64, skv)
+
+pytestmark = pytest.mark.gpu
+
+
+def _one64(q, pages, scales, table, b, n, D):
+    """Queries q [H_q, D] of sequence b over its first n tokens: in 64 bits, and the bound of test_gpu_paged_pool."""
+    wide = q.dtype == torch.float32
+    es, ep = (2.0 ** -19, 2.0 ** -19) if wide else (2.0 ** -17, 2.0 ** -11)
+    k, v = (_dense64(p, s, table, b, n, D) for p, s in zip(pages, scales))
+    qb = q.double().unflatten(0, (k.shape[0], -1))
+    s, size = (torch.einsum("grd,gtd->grt", x, y) / math.sqrt(D) for x, y in ((qb, k), (qb.abs(), k.abs())))
+    w = torch.softmax(s, -1)
+    out, spread = (torch.einsum("grt,gtd->grd", w, x).flatten(0, 1) for x in (v, v.abs()))
+    ds = ((D * U + es) * size + 4 * U * s.abs()).amax(-1).flatten()[:, None]
+    bound = (2 * ds + n * U + ep) * spread
+    return out, bound + HALF[q.dtype] * (out.abs() + bound) + TINY[q.dtype]
+
+
+def _widened(table, width):
+    """The same table with room for `width` pages."""
+    wide = torch.full((table.shape[0], width), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    return wide
+
+
+# ------------------------------------------------------------------------------------- how large a call may be
+WIDE = [(1, 16384, 131072), (8, 8192, 32768), (32, 2048, 32768), (64, 1024, 32768), (64, 4096, 8192)]   # sequences, tokens, room
+
+
+@pytest.mark.parametrize("B,S,room,kv,dtype", [(*w, *t) for w in WIDE for t in (("fp16", torch.bfloat16), ("int8", torch.float16))] +
+                         [(*WIDE[0], "fp16", torch.float32)])
+def test_prompts_behind_wide_tables(skv, B, S, room, kv, dtype):
+    """Whole prompts of 32 query heads, in pools whose tables have room for much longer sequences."""
+    H, rep, D, P = 4, 8, 64, 32
+    counts = [S - 7 * b for b in range(B)]
+    pages, scales, table, lens = _filled(skv, kv, counts, H, P, D, 16, 3)
+    q = torch.randn(B, S, H * rep, D, generator=_gen(4), device="cuda", dtype=dtype).transpose(1, 2)
+    got = skv.paged_attention(q, *pages, _widened(table, room // P), lens, *scales, causal=True, new_lengths=lens, check=True)
+    for b in {0, B // 2, B - 1}:
+        for i in (0, 130, counts[b] // 2, counts[b] - 1):
+            want, bound = _one64(q[b, :, i], pages, scales, table, b, i + 1, D)
+            assert ((got[b, :, i].double() - want).abs() <= bound).all(), (b, i)
+        assert (got[b, :, counts[b]:] == 0).all()
+
+
+@pytest.mark.parametrize("D,rep,Sq,dtype", [(64, 2, 64, torch.float32), (300, 2, 24, torch.float16), (64, 4, 256, torch.bfloat16)])
+def test_calls_in_parts_of_their_sequences(skv, D, rep, Sq, dtype):
+    """Tables so wide that one launch's tile numbers could not count all sequences."""
+    H, P, B = 2, 512, 40
+    counts = [Sq + 11 * (b % 5) for b in range(B)]
+    pages, scales, table, lens = _filled(skv, "fp16", counts, H, P, D, 16, 5)
+    q = _rows(_gen(6), B, H * rep, Sq, D, dtype)
+    wide = _widened(table, 2 ** 19 if D == 64 else 2 ** 18)
+    got = skv.paged_attention(q, *pages, wide, lens, causal=True, check=True)
+    assert torch.equal(got, skv.paged_attention(q, *pages, wide, lens, causal=True, new_lengths=torch.full_like(lens, Sq)))
+    want, bound = _attention64(q, pages, scales, table, counts, [Sq] * B, True)
+    assert ((got.double() - want).abs() <= bound).all()

@@ -116,3 +116,18 @@ def test_no_cpu_fallback():
         PagedKVPool(1, 1, 1, 8, 8, precision="int3")
     with pytest.raises(ValueError, match=">= 1"):
         PagedKVPool(0, 1, 1, 8, 8)
+
+
+def test_attention_refuses_only_what_tile_numbers_cannot_count():
+    """One sequence whose table could hold more tiles than a launch counts is refused before any launch."""
+    from shadow_infer_b200 import _lib
+    from shadow_infer_b200.shadowkv import paged_pool
+    lib = _lib.load()
+
+    def attend(width, page, heads, S_q, D=128, dtype=0):
+        pool = (16, 16, 0, 0, 16, width, width, 4, page, 1, D, 0, 0, 1)
+        rows = (16, 0, 0, 0, dtype, heads)
+        return lib.skv_pool_attention(paged_pool._ATTENTION.pack(*pool, *rows, *rows, 16, 0, 16, 1 << 40, 0, S_q, 0, 1.0, 0), None)
+
+    assert attend(2 ** 26, 32, 1 << 14, 1 << 10) == _lib.SKV_ERR_TOO_LARGE
+    assert "units" in _lib.last_error()
