@@ -427,7 +427,7 @@ int launch_append(const skv_pool_append_args& a, cudaStream_t st) {
     while (lanes * 16 < D) lanes *= 2;
     const int want = tokens * (a.q.heads + 2 * a.pool.heads) * lanes < 256ll * 2 * sm_count() ? a.pool.heads : (a.pool.heads + FLY - 1) / FLY;
     while (rows < want && lanes * rows < 256) rows *= 2;
-    while (lanes * rows * z < 32 || (lanes * rows * z * 2 <= 256 && tokens >= 8ll * sm_count() * z)) z *= 2;
+    while (lanes * rows * z < 32 || (z < 64 && lanes * rows * z * 2 <= 256 && tokens >= 8ll * sm_count() * z)) z *= 2;   // blockDim.z <= 64
     const int q_slices = (a.q.heads + rows * FLY - 1) / (rows * FLY), kv_slices = (a.pool.heads + rows * FLY - 1) / (rows * FLY);
     const dim3 block(lanes, rows, z), grid((unsigned)((tokens + z - 1) / z), q_slices + 2 * kv_slices);
     if (split) pool_append_kernel<T, true><<<grid, block, 0, st>>>(a, q_slices, kv_slices);

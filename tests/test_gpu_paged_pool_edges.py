@@ -64,3 +64,24 @@ def test_calls_in_parts_of_their_sequences(skv, D, rep, Sq, dtype):
     assert torch.equal(got, skv.paged_attention(q, *pages, wide, lens, causal=True, new_lengths=torch.full_like(lens, Sq)))
     want, bound = _attention64(q, pages, scales, table, counts, [Sq] * B, True)
     assert ((got.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("B,S,H,D,kv,dtype", [
+    (64, 1200, 2, 32, "fp16", torch.bfloat16), (40, 2000, 4, 32, "int8", torch.float16), (64, 1300, 1, 16, "int4", torch.float32),
+    (160, 1000, 1, 16, "fp32", torch.float16),
+])
+def test_append_of_many_small_rows(skv, B, S, H, D, kv, dtype):
+    """So many tokens of so few values that a block could take more than 64 of them."""
+    P = 100
+    table, N = _table([S] * B, P, 1)
+    (kp, vp), (sk, sv) = _pool(kv, N, H, P, D)
+    gen = _gen(3)
+    k, v = (_rows(gen, B, H, S, D, dtype) for _ in range(2))
+    cos, sin = skv.rotary_tables(D, S)
+    skv.paged_append(k, v, kp, vp, table, torch.zeros(B, dtype=torch.int32, device="cuda"), sk, sv, cos=cos, sin=sin, check=True)
+    store = skv.PagedKVStore(B, H, D, page_size=S, device="cuda")
+    store.append(_turn32(k, cos[None], sin[None], False).contiguous(), v.float().contiguous(), kv)
+    page, ids = store.pages[0], table[:, :S // P].long()
+    for mine, theirs in ((kp, page.k), (vp, page.v), (sk, page.scale_k), (sv, page.scale_v)):
+        if mine is not None:
+            assert torch.equal(mine[ids].transpose(1, 2).flatten(2, 3), theirs)
