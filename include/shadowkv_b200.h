@@ -481,7 +481,8 @@ typedef struct skv_pool_attention_args {
  * Query head h reads key head h / (H_q / heads).  scratch: skv_pool_attention_scratch_bytes
  * bytes, 16-byte aligned, with the first skv_pool_attention_scratch_zeros bytes zero before the
  * first call that uses it (arrival counters, which every call leaves zero).  Calls that may overlap
- * on the GPU use scratch of their own.
+ * on the GPU use scratch of their own; host threads that call on one stream may share one (a call's launches
+ * stay together).
  * SKV_ERR_TOO_LARGE, before any launch: H_q * S_q above 2^28, a batch above 2^24, or a single sequence whose table has
  * room for more than 2^30 tiles of work (units of 8 to 128 query rows times tiles of 32 to 128 tokens). */
 size_t skv_pool_attention_scratch_bytes(int D);

@@ -2,6 +2,11 @@
 #include "pool_attention_tc.cuh"
 
 namespace skv {
+std::mutex& tc_launches() {
+    static std::mutex m;
+    return m;
+}
+
 int attend_many(const skv_pool_attention_args& a, cudaStream_t st) {
     const int D = a.pool.head_dim;
     if (a.pool.precision == 1) return D <= 64 ? launch_tc<1, 64>(a, st) : D <= 128 ? launch_tc<1, 128>(a, st) : launch_tc<1, 256>(a, st);

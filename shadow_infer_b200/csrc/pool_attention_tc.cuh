@@ -31,6 +31,7 @@
 #pragma once
 
 #include <atomic>
+#include <mutex>
 
 #include "pool_attention.cuh"
 #include "sm100_ptx.cuh"
@@ -796,6 +797,10 @@ __global__ void __launch_bounds__(256) pool_attention_tc_join_kernel(const __gri
     }
 }
 
+// Held while the two launches of a call are put on their stream: the second reads what the first left in the scratch, and another
+// host thread's call on the same stream (and so with the same scratch) must not come between them.
+std::mutex& tc_launches();
+
 template <int PREC, int DP, int NP>
 int launch_tc_weights(const skv_pool_attention_args& a, cudaStream_t st) {
     using L = TcLayout<DP>;
@@ -817,6 +822,7 @@ int launch_tc_weights(const skv_pool_attention_args& a, cudaStream_t st) {
     const int ctas = min(sm_count() * L::CTAS, kTcMaxParts);
     const bool out_vec = rows_aligned(a.out);
     return by_sequences(a, step, [&](const skv_pool_attention_args& part) {
+        const std::lock_guard<std::mutex> both(tc_launches());
         kernel<<<ctas, kTcThreads, L::ALLOC, st>>>(part, out_vec);
         const int64_t units = part.pool.batch * part.pool.heads * row_tiles;
         const bool by_cta = units > ctas;

@@ -85,3 +85,31 @@ def test_append_of_many_small_rows(skv, B, S, H, D, kv, dtype):
     for mine, theirs in ((kp, page.k), (vp, page.v), (sk, page.scale_k), (sv, page.scale_v)):
         if mine is not None:
             assert torch.equal(mine[ids].transpose(1, 2).flatten(2, 3), theirs)
+
+
+# ----------------------------------------------------------------------------------------- threads and scratch
+def test_attention_from_two_threads_on_one_stream(skv):
+    """Calls whose parts are joined by a second launch, from two host threads on one stream, which share their scratch."""
+    import threading
+
+    calls = []
+    for seed, (counts, H, rep, Sq) in enumerate((([9000, 16], 2, 4, 31), ([7000, 3000, 5], 1, 3, 33))):
+        pages, scales, table, lens = _filled(skv, "fp16", counts, H, 32, 128, 16, seed)
+        q = _rows(_gen(seed), len(counts), H * rep, Sq, 128, torch.bfloat16)
+        calls.append(lambda q=q, pages=pages, table=table, lens=lens: skv.paged_attention(q, *pages, table, lens))
+    want = [call() for call in calls]
+    torch.cuda.synchronize()
+    wrong, go = [], threading.Barrier(2)
+
+    def work(i):
+        go.wait()
+        for _ in range(300):
+            if not torch.equal(calls[i](), want[i]):
+                wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
