@@ -40,7 +40,7 @@ _ATTENTION = struct.Struct("<" + _POOL + _ROWS * 2 + "QQQqQiifi")
 assert (_APPEND.size, _READ.size, _ATTENTION.size) == (336, 192, 216)
 _NO_ROPE = (0,) * 11
 _SCRATCH = {}         # (device, stream) -> attention scratch
-_SCRATCH_BYTES = {}   # head_dim -> its size
+_SCRATCH_BYTES = {}   # (device, head_dim) -> its size
 
 
 _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
@@ -48,10 +48,11 @@ _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_c
 
 def _scratch(dev: torch.device, stream: int, head_dim: int) -> torch.Tensor:
     """The attention's scratch on a stream: partial results and arrival counters that every call leaves zero.  Calls
-    of one stream follow each other, so they share one; a graph being captured gets its own."""
-    need = _SCRATCH_BYTES.get(head_dim)
-    if need is None:
-        need = _SCRATCH_BYTES[head_dim] = _lib.load().skv_pool_attention_scratch_bytes(head_dim)
+    of one stream follow each other, so they share one; a graph being captured gets its own.  (Found by the stream's handle,
+    like the blocks of torch's own allocator: an external stream outlives its calls.)"""
+    need = _SCRATCH_BYTES.get((dev.index, head_dim))
+    if need is None:   # by the SMs of dev, which is the current device
+        need = _SCRATCH_BYTES[dev.index, head_dim] = _lib.load().skv_pool_attention_scratch_bytes(head_dim)
     t = _SCRATCH.get((dev.index, stream))
     capturing = _capturing()
     if t is None or capturing or t.numel() < need:

@@ -131,3 +131,18 @@ def test_attention_refuses_only_what_tile_numbers_cannot_count():
 
     assert attend(2 ** 26, 32, 1 << 14, 1 << 10) == _lib.SKV_ERR_TOO_LARGE
     assert "units" in _lib.last_error()
+
+
+def test_attention_scratch_is_sized_by_device(monkeypatch):
+    """The scratch a device needs depends on its SMs: what one device needed is not taken for another's."""
+    from types import SimpleNamespace
+
+    from shadow_infer_b200.shadowkv import paged_pool
+    sms = iter((100, 160))
+    fake = SimpleNamespace(skv_pool_attention_scratch_bytes=lambda D: next(sms) * D, skv_pool_attention_scratch_zeros=lambda: 16)
+    monkeypatch.setattr(paged_pool._lib, "load", lambda: fake)
+    monkeypatch.setattr(paged_pool, "_capturing", lambda: False)
+    monkeypatch.setattr(paged_pool, "_SCRATCH", {})
+    monkeypatch.setattr(paged_pool, "_SCRATCH_BYTES", {})
+    got = [paged_pool._scratch(torch.device("meta", i), 7, 128).numel() for i in (0, 1, 0, 1)]
+    assert got == [12800, 20480, 12800, 20480]
