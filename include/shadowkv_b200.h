@@ -380,9 +380,12 @@ int skv_irap_importance(const float* scores, int B, int H, int Sq, int Sk, int i
  * page_size] (int8) or [num_pages, heads, page_size, D/G] (int4); token t of sequence b is row
  * t % page_size of page block_table[b][t / page_size].  Lengths and tables are DEVICE memory, so
  * nothing here waits for the host and every call can be captured in a graph.  A page number
- * outside [0, num_pages), a token past the table's width or a position past the rotary tables is
- * never followed: the row is not written / not attended to / zero when read / NaN when rotated,
- * and *error_flag (device int32, where not NULL) is set to 1.
+ * outside [0, num_pages) or a token past the table's width is never followed: its rows are not
+ * written / not attended to / zero when read.  A token whose position lies outside the rotary
+ * tables is not written either, key or value (its rows keep what they held: do not count it), and
+ * a row that skv_rotary turns, or a query of skv_pool_append, is NaN there.  Where error_flag (device int32) is not
+ * NULL, the first two and the unwritten token set it to 1.
+ * Outputs share no memory with inputs.
  * ------------------------------------------------------------------------------------- */
 typedef struct skv_pool {
     void* k;                     /* K pages */

@@ -4,6 +4,7 @@
 // value are stored in the pool's precision, bit-identical to the paged store's rows (paged.cu):
 //     int8: scale = amax / 127 over the row, int4: amax / 7 over a group; 1 where the amax is 0;
 //     n = rint(x / scale), clamped; int4 keeps n + 8, the even value in the high nibble.
+// A token without a page, or whose position the rotary tables do not hold, leaves its rows as they were.
 // Everything is read once and written once.  A token a sequence is bound by its latency: 8 sequences, 32 + 8 + 8 heads of 128
 // values, 3.0 us.  A prompt is bound by what it computes: 8 x 2048 fp16 tokens of 32 + 32 heads into int8 take 112 us, about 320
 // instructions for 4 rows of a warp (77 M in all, three quarters of the issue slots) at 3.3 TB/s.  Reading them back as fp32
@@ -69,7 +70,7 @@ __global__ void __launch_bounds__(32 * kPoolWarps) pool_append_any_kernel(const 
     x.half = a.rope.rot / 2;
     x.interleaved = a.rope.interleaved;
     x.sign = a.rope.inverse ? -1.0f : 1.0f;
-    x.known = x.rot == 0 || (pos >= 0 && pos < a.rope.max_positions);
+    x.known = a.rope.rot == 0 || (pos >= 0 && pos < a.rope.max_positions);   // a value goes with its key
     x.cs = a.rope.cos + pos * x.half;
     x.sn = a.rope.sin + pos * x.half;
     const int D = a.pool.head_dim;
@@ -211,11 +212,14 @@ __global__ void __launch_bounds__(256, 3) pool_append_kernel(const __grid_consta
         if (a.rope.inverse)
 #pragma unroll
             for (int i = 0; i < 8; ++i) w[i] = -w[i];
+    } else if (kind == 2 && there && a.rope.rot > 0) {   // a value goes with its key
+        const int64_t pos = rope_position(a.rope, b, s, t);
+        known = pos >= 0 && pos < a.rope.max_positions;
     }
     const bool stored = kind != 0 && there && (a.new_lengths == nullptr || s < a.new_lengths[b]);
     const int64_t row0 = stored ? pool_row(a.pool, b, t) : -1;
     if (stored && (row0 < 0 || !known) && a.error_flag) atomicExch(a.error_flag, 1);
-    // a key whose position is not known is not stored: the row's first lane speaks for the row
+    // a key whose position is not known is not stored, and neither is its value: the row's first lane speaks for the row
     if (kind != 0 && !__any_sync(0xffffffffu, row0 >= 0)) return;   // padding of a ragged prompt
     const bool ok = __shfl_sync(0xffffffffu, (int)known, (threadIdx.y * blockDim.x + threadIdx.z * blockDim.x * blockDim.y) & 31);
     const int p = kind == 0 ? 0 : a.pool.precision, G = p == 3 ? a.pool.int4_group : 16;

@@ -15,9 +15,10 @@ table for all layers) or let ``PagedKVPool`` do it:
 
 Tables and lengths stay on the device: no call waits for the GPU (unless ``check`` asks for it), and
 every call can be captured in a CUDA graph.  Entries of the table past a sequence's length are not
-read, and neither are rows past it.  A page number outside the pool or a position outside the
-rotary tables is never followed (the row is not written, not attended to, zero when read); ``check=True``
-waits for the call and raises ``ValueError`` if that happened.
+read, and neither are rows past it.  A page number outside the pool is never followed: its tokens are not written,
+not attended to, zero when read.  A token whose position lies outside the rotary tables is not written either, key or value;
+its rows keep what they held, so a program does not count it.  ``check=True`` waits for the call and raises
+``ValueError`` if either happened.
 """
 
 from __future__ import annotations
@@ -358,9 +359,13 @@ class PagedKVPool:
         new_lengths: Optional[Sequence[int]] = None,
         positions: Optional[torch.Tensor] = None,
         interleaved: bool = False,
+        check: bool = False,
     ) -> Optional[torch.Tensor]:
         """``paged_append`` behind each sequence's tokens (``new_lengths``: host numbers, default all rows).  A call
-        that the free pages or the table cannot hold raises ``RuntimeError`` and changes nothing."""
+        that the free pages or the table cannot hold raises ``RuntimeError``, and one whose tokens the rotary tables do not
+        reach ``ValueError``; neither changes anything.  ``positions`` are on the device: only ``check=True``, which
+        waits for the call, refuses those outside the tables (without it their tokens count as held, but are not
+        written)."""
         S = int(k.shape[2]) if k.dim() == 4 else 0
         new = [S] * self.batch_size if new_lengths is None else [int(n) for n in new_lengths]
         if len(new) != self.batch_size or min(new) < 0 or max(new) > S:
@@ -373,6 +378,9 @@ class PagedKVPool:
                                f"the table of {self._table.shape[1]} pages of {P}")
         if sum(wanted) > len(self._free):
             raise RuntimeError(f"{sum(wanted)} pages wanted, {len(self._free)} free")
+        last = max((c + n for c, n in zip(self.token_counts, new) if n), default=0)
+        if cos is not None and positions is None and last > cos.shape[0]:
+            raise ValueError(f"position {last - 1} lies outside rotary tables of {cos.shape[0]} positions")
         table = self._table
         if sum(wanted):
             table = table.clone()
@@ -387,7 +395,7 @@ class PagedKVPool:
             block_table = self.block_table
         fresh = None if new_lengths is None else torch.tensor(new, dtype=torch.int32, device=self.lengths.device)
         out = paged_append(k, v, self.k_pages, self.v_pages, block_table, self.lengths, self.scale_k, self.scale_v, fresh,
-                           q, cos, sin, positions, interleaved)
+                           q, cos, sin, positions, interleaved, check)
         if sum(wanted):
             del self._free[len(self._free) - sum(wanted):]
             self._table = table

@@ -87,6 +87,63 @@ def test_append_of_many_small_rows(skv, B, S, H, D, kv, dtype):
             assert torch.equal(mine[ids].transpose(1, 2).flatten(2, 3), theirs)
 
 
+# -------------------------------------------------------------------------------------- what an append leaves
+@pytest.mark.parametrize("kv", ["fp32", "fp16", "int8", "int4"])
+@pytest.mark.parametrize("D,interleaved,layout", [(64, False, "bhsd"), (64, True, "bhsd"), (40, False, "bhsd"), (64, False, "odd")])
+def test_append_of_unknown_positions_writes_nothing(skv, kv, D, interleaved, layout):
+    """A token whose position the tables do not hold: neither its key nor its value, nor their scales; the others' are."""
+    B, H, S, P = 2, 3, 5, 4
+    table, N = _table([S] * B, P, 1)
+    pages, scales = _pool(kv, N, H, P, D, 8)
+    gen = _gen(2)
+    for t in (*pages, *scales):
+        if t is not None:
+            t.copy_(torch.randint(1, 100, t.shape, generator=gen, device="cuda"))
+    before = [None if t is None else t.clone() for t in (*pages, *scales)]
+    k, v = (_rows(gen, B, H, S, D, torch.float32, layout) for _ in range(2))
+    cos, sin = skv.rotary_tables(16, 10)
+    zero = torch.zeros(B, dtype=torch.int32, device="cuda")
+    good = [(0, 0), (0, 2), (1, 1), (1, 4)]
+    for dtype in (torch.int32, torch.int64):
+        at = torch.tensor([[0, 10, 9, -1, 1000], [-7, 3, 10, 11, 9]], dtype=dtype, device="cuda")
+        now = [None if t is None else t.clone() for t in before]
+        args = (k, v, *now[:2], table, zero, *now[2:], None, None, cos, sin)
+        skv.paged_append(*args, positions=at, interleaved=interleaved)
+        want = [None if t is None else t.clone() for t in before]
+        inside = at.clamp(0, 9)
+        skv.paged_append(k, v, *want[:2], table, zero, *want[2:], None, None, cos, sin, positions=inside, interleaved=interleaved)
+        for mine, same, old in zip(now, want, before):
+            if mine is None:
+                continue
+            for b in range(B):
+                for s in range(S):
+                    where = (int(table[b, s // P]), slice(None), s % P)
+                    assert torch.equal(mine[where], (same if (b, s) in good else old)[where]), (b, s)
+        with pytest.raises(ValueError, match="position"):
+            skv.paged_append(*args, positions=at, interleaved=interleaved, check=True)
+
+
+def test_pool_refuses_positions_behind_the_tables(skv):
+    """The pool's lengths never pass what was written: positions that the tables do not hold are refused."""
+    pool = skv.PagedKVPool(8, 2, 2, 32, max_tokens=64, page_size=16, precision="fp16")
+    cos, sin = skv.rotary_tables(32, 20)
+    x = torch.ones(2, 2, 15, 32, device="cuda")
+    pool.append(x, x, cos=cos, sin=sin, new_lengths=[15, 2])
+    held = [t.clone() for t in (pool.k_pages, pool.v_pages, pool.block_table, pool.lengths)]
+    free = pool.free_pages
+    with pytest.raises(ValueError, match="position"):
+        pool.append(x, x, cos=cos, sin=sin, new_lengths=[6, 1])
+    with pytest.raises(ValueError, match="position"):
+        pool.append(x, x, cos=cos, sin=sin, new_lengths=[1, 6], positions=torch.full((2, 15), 20, device="cuda"), check=True)
+    assert pool.token_counts == [15, 2] and pool.free_pages == free
+    for t, old in zip((pool.k_pages, pool.v_pages, pool.block_table, pool.lengths), held):
+        assert torch.equal(t, old)
+    pool.append(x, x, cos=cos, sin=sin, new_lengths=[5, 1])                                  # up to the last position
+    pool.append(x, x, cos=cos, sin=sin, new_lengths=[1, 6], positions=torch.full((2, 15), 19, device="cuda"), check=True)
+    pool.append(x, x, new_lengths=[1, 1])                                                    # no rotation, no limit
+    assert pool.token_counts == [22, 10] == pool.lengths.tolist()
+
+
 # ----------------------------------------------------------------------------------------- threads and scratch
 def test_attention_from_two_threads_on_one_stream(skv):
     """Calls whose parts are joined by a second launch, from two host threads on one stream, which share their scratch."""
