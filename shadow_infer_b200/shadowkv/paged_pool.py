@@ -71,6 +71,8 @@ def _index(t: torch.Tensor, shape: Tuple[int, ...], dev: torch.device, name: str
     if t.dtype is not torch.int32 or not t.is_cuda or t.get_device() != dev.index:
         if t.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"{name} must be int32 or int64, got {t.dtype}")
+        if t.dtype is torch.int64:   # numbers that 32 bits do not hold stay outside of every pool
+            t = t.clamp(-2 ** 31, 2 ** 31 - 1)
         t = t.to(device=dev, dtype=torch.int32)
     return t if t.is_contiguous() or t.stride(-1) == 1 else t.contiguous()
 

@@ -144,6 +144,27 @@ def test_pool_refuses_positions_behind_the_tables(skv):
     assert pool.token_counts == [22, 10] == pool.lengths.tolist()
 
 
+def test_tables_of_64_bit_numbers(skv):
+    """int64 tables and lengths mean what int32 ones do, and numbers beyond 32 bits name nothing."""
+    pages, scales, table, lens = _filled(skv, "fp16", [100, 40], 2, 32, 64, 16, 2)
+    q = _rows(_gen(3), 2, 4, 1, 64, torch.float16)
+    want = skv.paged_attention(q, *pages, table, lens)
+    for where in ("cuda", "cpu"):
+        assert torch.equal(skv.paged_attention(q, *pages, table.long().to(where), lens.long().to(where)), want)
+    far = table.long()
+    far[0, 1] += 2 ** 32
+    far[1, 0] -= 2 ** 33
+    with pytest.raises(ValueError, match="outside the pool"):
+        skv.paged_attention(q, *pages, far, lens, check=True)
+    k, _ = skv.paged_read(*pages, far, lens, 100)
+    assert (k[0, :, 32:64] == 0).all() and (k[1, :, :32] == 0).all() and (k[0, :, :32] != 0).any()
+    rows = torch.ones(2, 2, 1, 64, device="cuda")
+    held = [t.clone() for t in pages]
+    with pytest.raises(ValueError, match="outside the pool"):
+        skv.paged_append(rows, rows, *pages, table, torch.tensor([2 ** 32, -2 ** 32], device="cuda"), check=True)
+    assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(pages, held))
+
+
 # ----------------------------------------------------------------------------------------- threads and scratch
 def test_attention_from_two_threads_on_one_stream(skv):
     """Calls whose parts are joined by a second launch, from two host threads on one stream, which share their scratch."""
