@@ -31,7 +31,7 @@ import torch
 
 from .. import _lib
 from .._device import as_device, compute_device, device_ctx
-from .rotary import _DTYPE_CODE, _NO_ROWS, _back, _launch, _like, _rope_fields, _rows
+from .rotary import _DTYPE_CODE, _NO_ROWS, _back, _common, _launch, _like, _rope_fields, _rows
 
 _PRECISION_CODE = {torch.float32: 0, torch.float16: 1, torch.int8: 2, torch.uint8: 3}
 _POOL, _ROWS, _ROPE = "QQQQQqiiiiiiii", "Qqqqii", "QQQqqiiiiii"
@@ -171,7 +171,7 @@ def paged_append(
         raise ValueError("cos and sin must be given together")
     lens = _index(lengths, (B,), dev, "lengths")
     new = None if new_lengths is None else _index(new_lengths, (B,), dev, "new_lengths")
-    kd, k_rows = _rows(k, dev)
+    kd, k_rows = _rows(k, dev, _common(k, v, q))
     vd, v_rows = _rows(v, dev, kd.dtype)
     q_rows = q_out_rows = _NO_ROWS
     qd = q_out = None

@@ -84,6 +84,15 @@ def _rows(t: torch.Tensor, dev: torch.device, dtype: Optional[torch.dtype] = Non
     return t, (t.data_ptr(), st[0], st[1], st[2], code, t.shape[1])
 
 
+def _common(t: torch.Tensor, *others: Optional[torch.Tensor]) -> Optional[torch.dtype]:
+    """The type of rows that share a launch: their own (None), or fp32, which holds fp16 and bf16, where they differ."""
+    have = t.dtype
+    for o in others:
+        if o is not None and o.dtype is not have:
+            return torch.float32
+    return None
+
+
 def _like(t: torch.Tensor):
     """An output laid out like ``t`` (dense, dimensions in the order of ``t``'s strides), and its ``skv_rows`` fields."""
     out = torch.empty_like(t)
@@ -103,7 +112,9 @@ def _launch(entry, args: bytes, dev: torch.device) -> int:
 
 
 def _back(out: torch.Tensor, given: torch.Tensor, dev: torch.device) -> torch.Tensor:
-    """``out``, which lies on ``dev``, where ``given`` lies."""
+    """``out``, which lies on ``dev``, in ``given``'s type where that is one of floating numbers, and where ``given`` lies."""
+    if out.dtype is not given.dtype and given.dtype.is_floating_point:
+        out = out.to(given.dtype)
     return out if given.is_cuda and given.get_device() == dev.index else back(out, given.device)
 
 
@@ -171,7 +182,7 @@ def apply_rotary(
     if k is not None and (k.dim() != 4 or k.shape != (B, k.shape[1], S, D)):
         raise ValueError(f"q/k shapes disagree: {tuple(q.shape)} vs {tuple(k.shape)}")
     dev = q.device if q.is_cuda else compute_device(k, cos)
-    qd, q_rows = _rows(q, dev)
+    qd, q_rows = _rows(q, dev, _common(q, k))
     q_out, q_out_rows = _like(qd)
     kd = k_out = None
     k_rows = k_out_rows = _NO_ROWS

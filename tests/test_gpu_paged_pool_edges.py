@@ -165,6 +165,33 @@ def test_tables_of_64_bit_numbers(skv):
     assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(pages, held))
 
 
+@pytest.mark.parametrize("kt,vt,qt", [(torch.bfloat16, torch.float32, torch.float16), (torch.float16, torch.bfloat16, torch.bfloat16),
+                                      (torch.float32, torch.float16, torch.float64)])
+def test_rows_of_different_types(skv, kt, vt, qt):
+    """Keys, values and queries of different types: each row as it is, not rounded to another's type."""
+    B, H, S, D = 2, 2, 9, 64
+    gen = _gen(6)
+    k, v, q = (torch.randn(B, H, S, D, generator=gen, device="cuda").to(t) for t in (kt, vt, qt))
+    cos, sin = skv.rotary_tables(D, 64)
+    at = torch.arange(S, device="cuda").expand(B, S)
+    for kv in ("fp32", "int8"):
+        (kp, vp), (sk, sv) = _pool(kv, 2, H, 16, D)
+        table = torch.tensor([[0], [1]], dtype=torch.int32, device="cuda")
+        out = skv.paged_append(k, v, kp, vp, table, torch.zeros(B, dtype=torch.int32, device="cuda"), sk, sv, q=q, cos=cos, sin=sin)
+        assert out.dtype == qt and torch.equal(out, _turn32(q, cos[at], sin[at], False).to(qt))
+        store = skv.PagedKVStore(B, H, D, page_size=S, device="cuda")
+        store.append(_turn32(k, cos[at], sin[at], False), v.float(), kv)
+        page = store.pages[0]
+        for mine, theirs in ((kp, page.k), (vp, page.v), (sk, page.scale_k), (sv, page.scale_v)):
+            assert mine is None or torch.equal(mine[:, :, :S], theirs)
+        got = skv.paged_attention(q, kp, vp, table, torch.full((B,), S, dtype=torch.int32, device="cuda"), sk, sv)
+        assert got.dtype == qt
+    for x, y in ((q, k), (k, v)):
+        turned = skv.apply_rotary(x, cos, sin, k=y)
+        for a, b in zip((x, y), turned):
+            assert b.dtype == a.dtype and torch.equal(b, skv.apply_rotary(a, cos, sin))
+
+
 # ----------------------------------------------------------------------------------------- threads and scratch
 def test_attention_from_two_threads_on_one_stream(skv):
     """Calls whose parts are joined by a second launch, from two host threads on one stream, which share their scratch."""
