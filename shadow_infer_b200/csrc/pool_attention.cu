@@ -36,6 +36,7 @@ __global__ void __launch_bounds__(kAnyThreads) pool_attention_any_kernel(const _
                                                                          int row_tiles) {
     extern __shared__ float any_sm[];
     __shared__ Share s;
+    __shared__ int s_see[kAnyRows];   // tokens that each row sees
     const int D = a.pool.head_dim, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     float* sq = any_sm;
     float* sk = sq + kAnyRows * D;
@@ -63,6 +64,7 @@ __global__ void __launch_bounds__(kAnyThreads) pool_attention_any_kernel(const _
 #pragma unroll
         for (int i = 0; i < 2; ++i)
             see[i] = seen_by(a, g.b, g.tokens, (r0 + warp + 4 * i) % a.S_q);
+        if (lane < 2) s_see[warp + 4 * lane] = lane ? see[1] : see[0];
 #pragma unroll
         for (int j = 0; j < kAnyRows; ++j)
 #pragma unroll
@@ -102,6 +104,10 @@ __global__ void __launch_bounds__(kAnyThreads) pool_attention_any_kernel(const _
             }
             __syncthreads();
             const bool held = sp[lane] != 0.0f;
+            int see_least = g.tokens;
+            for (int j = 0; j < kAnyRows; ++j)
+                if (s_see[j] > 0) see_least = min(see_least, s_see[j]);
+            const bool not_all = tok0 >= not_all_from(see_least, g.tokens, kAnyTile);
             float x[2] = {0.0f, 0.0f};
 #pragma unroll 4
             for (int d = 0; d < D; ++d) {
@@ -133,6 +139,12 @@ __global__ void __launch_bounds__(kAnyThreads) pool_attention_any_kernel(const _
 #pragma unroll 4
                 for (int k = 0; k < kAnyTile; ++k) {
                     const float v = sv[k * D + d];
+                    if (not_all && !finite(v)) {   // (pool_attention.cuh)
+#pragma unroll
+                        for (int j = 0; j < kAnyRows; ++j)
+                            if (tok0 + k < s_see[j]) o[j][i] += v;
+                        continue;
+                    }
 #pragma unroll
                     for (int j = 0; j < kAnyRows; ++j) o[j][i] = fmaf(sp[j * kAnyTile + k], v, o[j][i]);
                 }

@@ -361,6 +361,54 @@ __device__ __forceinline__ void join(const skv_pool_attention_args& a, const Sha
     __syncthreads();
 }
 
+// ------------------------------------------------------------------------ values that are not finite
+// A weight of zero does not hide an infinite or NaN value: 0 x inf is NaN.  Under a causal limit a tile has tokens that only
+// some of a unit's rows see, so from the first such tile on (not_all_from: a multiple of the tile) the kernels put zeros for
+// values that are not finite, remember that they did, and add them at the unit's end to the rows that see them.  A weight is
+// positive, so what a value that is not finite contributes is that value.
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+__device__ __forceinline__ int not_all_from(int see_least, int tokens, int tile) { return see_least < tokens ? see_least / tile * tile : 0x7fffffff; }
+// Bits that are set if one of two fp16 values is not finite (its exponent's bits are all ones: one more carries out of them).
+__device__ __forceinline__ uint32_t odd_halves(uint32_t w) { return ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u; }
+__device__ __forceinline__ uint32_t odd_halves(uint4 w) { return odd_halves(w.x) | odd_halves(w.y) | odd_halves(w.z) | odd_halves(w.w); }
+// The two values, zero for those.
+__device__ __forceinline__ uint32_t finite_halves(uint32_t w) {
+    const uint32_t odd = odd_halves(w);
+    return w & ~((odd & 0x8000u ? 0xffffu : 0u) | (odd >> 16 ? 0xffff0000u : 0u));
+}
+__device__ __forceinline__ uint4 finite_halves(uint4 w) {
+    return make_uint4(finite_halves(w.x), finite_halves(w.y), finite_halves(w.z), finite_halves(w.w));
+}
+
+// Adds what is not finite among the values of tokens [from, to) to rows r0 .. r0 + rows - 1 of a unit, in its part or, where that is
+// null, in the output.  Rare, so it is slow and reads the pages again; thread tid of `threads`, between barriers of them.
+template <int PREC>
+__device__ __noinline__ void add_not_finite(const skv_pool_attention_args& a, int b, int hk, int tokens, int r0, int rows, int from, int to,
+                                            float* part, int tid, int threads) {
+    const int D = a.pool.head_dim, rep = a.q.heads / a.pool.heads;
+    for (int i = tid; i < rows * D; i += threads) {
+        const int j = i / D, d = i - j * D, r = r0 + j;
+        const int end = min(to, seen_by(a, b, tokens, r % a.S_q));
+        float sum = 0.0f;
+        for (int t = from; t < end; ++t) {
+            const int64_t row = pool_row(a.pool, b, t);
+            if (row < 0) continue;
+            const float v = pool_value<PREC>(a.pool, true, row + (int64_t)hk * a.pool.page_size, d, PREC == 3 ? d / a.pool.int4_group : 0);
+            if (!finite(v)) sum += v;
+        }
+        if (sum == 0.0f) continue;
+        if (part) {
+            part[i] += sum;
+        } else {
+            const float x = a.out.dtype == kF32   ? row_ptr<float>(a.out, a.S_q, rep, b, hk, r)[d]
+                            : a.out.dtype == kF16 ? to_float(row_ptr<__half>(a.out, a.S_q, rep, b, hk, r)[d])
+                                                  : to_float(row_ptr<__nv_bfloat16>(a.out, a.S_q, rep, b, hk, r)[d]);
+            const float one[1] = {x + sum};
+            store_out<1>(a, b, hk, r, d, one);
+        }
+    }
+}
+
 // How many sequences a launch takes at most, so that tile numbers hold their tiles (the lengths are on the device, so the tables'
 // width counts): row_tiles a key head, `tile` tokens each, `pad` on top of a unit.  0, with the failure recorded: not even one.
 inline int64_t sequences_a_launch(const skv_pool_attention_args& a, int64_t row_tiles, int tile, int pad) {

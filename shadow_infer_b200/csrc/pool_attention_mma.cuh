@@ -249,6 +249,26 @@ struct MmaShape {
     static constexpr int MQ = PREC == 0 ? DP / 8 : DP / 16;   // MMAs that a tile's scores take a term
 };
 
+// Zeros for what is not finite in a warp's fp16 or fp32 values; whether this lane found any.
+template <int PREC, int PIECES>
+__device__ __noinline__ bool leave_out(uint4* values) {
+    bool any = false;
+#pragma unroll 4
+    for (int i = threadIdx.x & 31; i < PIECES; i += 32) {
+        const uint4 u = values[i];
+        if constexpr (PREC == 1) {
+            if (odd_halves(u) == 0) continue;
+            values[i] = finite_halves(u);
+        } else {
+            const bool x = finite(__uint_as_float(u.x)), y = finite(__uint_as_float(u.y)), z = finite(__uint_as_float(u.z)), w = finite(__uint_as_float(u.w));
+            if (x && y && z && w) continue;
+            values[i] = make_uint4(x ? u.x : 0u, y ? u.y : 0u, z ? u.z : 0u, w ? u.w : 0u);
+        }
+        any = true;
+    }
+    return any;
+}
+
 template <int PREC, int DP, int NT, int NQ>
 __host__ __device__ constexpr size_t mma_smem() {
     constexpr int W = MmaShape<PREC, DP, NT>::W, ROWS = 8 * NT;
@@ -267,6 +287,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
     extern __shared__ __align__(128) char mma_sm[];
     __shared__ Share s;
     __shared__ int s_free[W];
+    __shared__ int s_odd;   // whether values of the segment that are not finite were left out
     char* s_ring = mma_sm;                                                       // [W][S] slots
     uint2* s_q = reinterpret_cast<uint2*>(s_ring + W * S * L::BYTES);            // [MQ][NT][NQ][32]
     float* s_join = reinterpret_cast<float*>(s_q + MQ * NT * NQ * 32);
@@ -417,6 +438,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
         const int n = g.tokens, r0 = g.rt * ROWS;
         // ---- queries: a power of two taken out of each row, laid out as B operands
         __syncthreads();
+        if (tid == 0) s_odd = 0;
         if (!exact && merged >= 0) {   // chunks that are never copied count as zero again
             for (int i = lane; i < L::BYTES / 16; i += 32) reinterpret_cast<uint4*>(s_ring + merged)[i] = make_uint4(0, 0, 0, 0);
             __syncwarp();
@@ -478,7 +500,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
         __syncthreads();
         float start_at[NT][2];   // of the score sums
         float cf[NT][2], ref[NT][2], base_of[NT][2], sum[NT][2], o[NT][M][4];   // base_of: ref, or 0 before there is one
-        int see[NT][2], see_all = n;
+        int see[NT][2], see_all = n, see_least = n;   // tokens that a row sees, that all do, that all do which see any
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -491,9 +513,13 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                 sum[t][i] = 0.0f;
                 see[t][i] = r0 + j < R ? seen_by(a, g.b, n, (r0 + j) % a.S_q) : n;
                 see_all = min(see_all, see[t][i]);
+                if (see[t][i] > 0) see_least = min(see_least, see[t][i]);
             }
         see_all = min(see_all, __shfl_xor_sync(0xffffffffu, see_all, 1));
         see_all = min(see_all, __shfl_xor_sync(0xffffffffu, see_all, 2));
+        see_least = min(see_least, __shfl_xor_sync(0xffffffffu, see_least, 1));
+        see_least = min(see_least, __shfl_xor_sync(0xffffffffu, see_least, 2));
+        const int not_all = not_all_from(see_least, n, 16);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -524,6 +550,13 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                         for (int i = 0; i < L::SCALES; ++i) reinterpret_cast<float*>(slot + L::SV)[lane * L::SCALES + i] = 1.0f;
                 }
                 __syncwarp();
+            }
+            if constexpr (PREC <= 1) {
+                if (t0 >= not_all) {   // values that are not finite wait until the rows that see them are known apart
+                    const bool odd = leave_out<PREC, 16 * L::CHUNKS>(reinterpret_cast<uint4*>(slot + L::V));
+                    if (odd) s_odd = 1;
+                    __syncwarp();
+                }
             }
             // ---- scores
             float x[NT][4], k_factor[2] = {1.0f, 1.0f};
@@ -680,6 +713,19 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                     const uint4 y = *reinterpret_cast<const uint4*>(slot + L::SV + ((lane & 15) * M + 4 * k) * 4);
                     top = max(max(top, y.x & 0x7fffffffu), max(y.y & 0x7fffffffu, max(y.z & 0x7fffffffu, y.w & 0x7fffffffu)));
                 }
+                if (__any_sync(0xffffffffu, top >= 0x7f800000u)) {   // a group that is not finite says nothing of the others' size
+                    __syncwarp();
+                    top = 0;
+#pragma unroll 1
+                    for (int k = 0; k < M; ++k) {
+                        uint32_t* at = reinterpret_cast<uint32_t*>(slot + L::SV) + (lane & 15) * M + k;
+                        const uint32_t y = *at & 0x7fffffffu;
+                        if (y < 0x7f800000u) top = max(top, y);
+                        else if (lane < 16) *at = 0;
+                    }
+                    s_odd = 1;
+                    __syncwarp();
+                }
                 token_exp = clamp_exp(top);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
@@ -732,6 +778,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                     const float y = fast_exp2(x[t][i] - base_of[t][col]);
                     sum[t][col] = PREC >= 2 ? fmaf(y, v_sum[tok], sum[t][col]) : sum[t][col] + y;
                     w[i] = PREC == 2 ? y * v_mul[tok] : y;
+                    if (PREC == 2 && !all && x[t][i] == -INFINITY) w[i] = 0.0f;   // (a scale may be infinite)
                 }
                 if constexpr (PREC == 0) {   // (a NaN that rounding would hide is in the sum)
 #pragma unroll
@@ -988,6 +1035,12 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                 store_row(a, g, r0 + j, d, out_vec, y);
             }
             if (t + 1 < NT) __syncthreads();
+        }
+        if (PREC != 2 && s_odd) {   // (set before the barriers above)
+            const int first = g.t0 * TILE;
+            __syncthreads();
+            add_not_finite<PREC>(a, g.b, g.hk, n, r0, min(ROWS, R - r0), PREC == 3 ? first : max(first, not_all), min(n, g.t1 * TILE),
+                                 g.whole ? nullptr : part, tid, THREADS);
         }
         if (!g.whole) {
             if (tid < ROWS) {

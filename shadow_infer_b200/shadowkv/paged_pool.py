@@ -266,8 +266,8 @@ def paged_attention(
     The result has ``q``'s dimension order in memory (as torch's own operators keep it), so that the output of a
     ``[B, S, H, D]`` projection goes back to one without a copy.
 
-    Scores, softmax and sums are fp32; a weight below 2^-36 of its query's largest is rounded to that step.  Values that are
-    not finite make the queries that see them not finite.  Every page is read once for all the query rows that share its key
+    Scores, softmax and sums are fp32; a weight below 2^-36 of its query's largest is rounded to that step.  What is
+    not finite reaches the queries that see it and no others: a key all of their values, a value its own ones.  Every page is read once for all the query rows that share its key
     head.  The sequences are split over the whole GPU by their lengths on the device, long ones into
     parts that are joined in token order, so equal calls give equal bits.
     """

@@ -192,6 +192,65 @@ def test_rows_of_different_types(skv, kt, vt, qt):
             assert b.dtype == a.dtype and torch.equal(b, skv.apply_rotary(a, cos, sin))
 
 
+# ------------------------------------------------------------------------------------ values that are not finite
+ODD = [  # counts, H, rep, Sq, D, P, new: kernels for few rows, for many, and for any size
+    ([200, 37], 2, 2, 9, 128, 16, None),
+    ([70, 260, 7], 1, 5, 7, 64, 32, [7, 3, 0]),
+    ([130, 77], 3, 3, 3, 80, 7, None),
+    ([5000], 2, 2, 5, 128, 32, None),              # parts that are joined
+    ([300, 70], 2, 1, 30, 256, 32, None),
+    ([700, 150], 15, 2, 130, 128, 32, None),       # a prompt: blocks of one head's tokens
+    ([700, 150], 2, 2, 130, 64, 7, [130, 60]),
+    ([300, 90], 2, 8, 16, 128, 32, None),          # rows of several heads
+    ([9000, 20], 2, 4, 31, 96, 16, None),
+    ([260], 2, 2, 140, 256, 16, None),
+    ([60, 33], 2, 2, 5, 300, 8, None),
+    ([3000, 33], 1, 2, 6, 35, 8, None),
+]
+
+
+@pytest.mark.parametrize("counts,H,rep,Sq,D,P,new", ODD)
+@pytest.mark.parametrize("kv", ["fp32", "fp16", "int8", "int4"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_attention_of_values_that_are_not_finite(skv, counts, H, rep, Sq, D, P, new, kv, dtype):
+    """Infinite and NaN values among the newest tokens, and in one value or int4 group of an old one, reach the queries that
+    see them, in their own values, and nothing else."""
+    pages, scales, table, lens = _filled(skv, kv, counts, H, P, D, 16, sum(counts) + D)
+    q = _rows(_gen(5), len(counts), H * rep, Sq, D, dtype)
+    at = [(b, n - 1 - (i * Sq // 3), i % H, i) for b, n in enumerate(counts) for i in range(3) if n > i * Sq // 3]
+    if kv != "int8":
+        at.append((0, 3, 0, 1))
+    for b, t, h, i in at:
+        page, x = int(table[b, t // P]), (math.inf, math.nan, -math.inf)[i]
+        if scales[1] is None:
+            pages[1][page, h, t % P, (7 * i + 3) % D] = x
+        else:
+            scales[1][page, h, t % P, ((i + 1) % scales[1].shape[3]) if kv == "int4" else 0] = x
+    fresh = None if new is None else torch.tensor(new, dtype=torch.int32, device="cuda")
+    got = skv.paged_attention(q, *pages, table, lens, *scales, causal=True, new_lengths=fresh, check=True)
+    es, ep = (2.0 ** -19, 2.0 ** -19) if dtype == torch.float32 else (2.0 ** -17, 2.0 ** -11)
+    for b, n in enumerate(counts):
+        k, v = (_dense64(p, s, table, b, n, D) for p, s in zip(pages, scales))
+        odd = ~torch.isfinite(v)
+        v = v.masked_fill(odd, 0)
+        qb = q[b].double().unflatten(0, (H, rep))
+        s = torch.einsum("grsd,gtd->grst", qb, k) / math.sqrt(D)
+        size = torch.einsum("grsd,gtd->grst", qb.abs(), k.abs()) / math.sqrt(D)
+        i, t = torch.arange(Sq, device="cuda")[:, None], torch.arange(n, device="cuda")
+        m = Sq if new is None else new[b]
+        seen = (i < m) & (t <= n - m + i)
+        w = torch.nan_to_num(torch.softmax(s.masked_fill(~seen, -math.inf), -1), nan=0.0)
+        ds = ((D * U + es) * size + 4 * U * s.abs()).masked_fill(~seen, 0).amax(-1, keepdim=True)
+        want = torch.einsum("grst,gtd->grsd", w, v)
+        bound = (2 * ds + n * U + ep) * torch.einsum("grst,gtd->grsd", w, v.abs())
+        bound = bound + HALF[dtype] * (want.abs() + bound) + TINY[dtype]
+        hit = (torch.einsum("st,gtd->gsd", seen.double(), odd.double()) > 0)[:, None].expand(H, rep, Sq, D)
+        mine = got[b].double().unflatten(0, (H, rep))
+        assert torch.equal(~torch.isfinite(mine), hit)
+        off = torch.where(hit, -1.0, (mine - want).abs() - bound)
+        assert off.max() <= 0, float(off.max())
+
+
 # ----------------------------------------------------------------------------------------- threads and scratch
 def test_attention_from_two_threads_on_one_stream(skv):
     """Calls whose parts are joined by a second launch, from two host threads on one stream, which share their scratch."""
