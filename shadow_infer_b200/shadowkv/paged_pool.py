@@ -19,6 +19,9 @@ read, and neither are rows past it.  A page number outside the pool is never fol
 not attended to, zero when read.  A token whose position lies outside the rotary tables is not written either, key or value;
 its rows keep what they held, so a program does not count it.  ``check=True`` waits for the call and raises
 ``ValueError`` if either happened.
+
+Like the other caches' operators these serve: rows that require a gradient are read as constants
+(``apply_rotary`` by itself has a gradient).
 """
 
 from __future__ import annotations

@@ -154,6 +154,29 @@ def _rope_fields(cos, sin, positions, B: int, S: int, D: int, interleaved: bool,
             (cos, sin, positions))
 
 
+class _Turn(torch.autograd.Function):
+    """``apply_rotary`` of rows that a gradient is wanted of: it is the gradient of the result, turned the other way."""
+
+    @staticmethod
+    def forward(ctx, q, k, cos, sin, positions, interleaved, inverse):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(cos, sin, *(() if positions is None else (positions,)))
+        ctx.how = dict(interleaved=interleaved, inverse=not inverse)
+        return apply_rotary(q, cos, sin, k, positions, interleaved, inverse)
+
+    @staticmethod
+    def backward(ctx, gq, gk=None):
+        cos, sin, *positions = ctx.saved_tensors
+        how = dict(ctx.how, positions=positions[0] if positions else None)
+        if gq is not None and gk is not None:
+            gq, gk = apply_rotary(gq, cos, sin, gk, **how)
+        elif gq is not None:
+            gq = apply_rotary(gq, cos, sin, **how)
+        elif gk is not None:
+            gk = apply_rotary(gk, cos, sin, **how)
+        return gq, gk, None, None, None, None, None
+
+
 def apply_rotary(
     q: torch.Tensor,
     cos: torch.Tensor,
@@ -169,7 +192,8 @@ def apply_rotary(
     are ``(x[i], x[i + rot/2])``, or ``(x[2i], x[2i+1])`` with ``interleaved``, over the first
     ``rot = 2 * cos.shape[1]`` values of a head; the others are copied.  ``positions``: int32 or int64, broadcast to
     ``[B, S]`` (default: 0 .. S-1); rows whose position the tables do not hold become NaN.
-    ``inverse`` turns back, which is also the gradient with respect to the rows.
+    ``inverse`` turns by minus the angle: the gradient with respect to the rows, and, where the tables have no gain (that of
+    ``"ntk_parts"`` comes in a second time), back.  Rows that require a gradient get theirs; the tables get none.
 
     fp32, fp16 and bf16 rows are read in place with any strides over the first three dimensions
     (slices of one projection's output, transposed views); products and sums are fp32, rounded once to the
@@ -181,6 +205,8 @@ def apply_rotary(
     B, _, S, D = shape
     if k is not None and (k.dim() != 4 or k.shape != (B, k.shape[1], S, D)):
         raise ValueError(f"q/k shapes disagree: {tuple(q.shape)} vs {tuple(k.shape)}")
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _Turn.apply(q, k, cos, sin, positions, interleaved, inverse)
     dev = q.device if q.is_cuda else compute_device(k, cos)
     qd, q_rows = _rows(q, dev, _common(q, k))
     q_out, q_out_rows = _like(qd)

@@ -251,6 +251,46 @@ def test_attention_of_values_that_are_not_finite(skv, counts, H, rep, Sq, D, P, 
         assert off.max() <= 0, float(off.max())
 
 
+# ------------------------------------------------------------------------------------------------ gradients
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_backward(skv, dtype, interleaved):
+    """Rows that require a gradient get the formula's: queries and keys, slices of one projection, a key head that all
+    share, turned either way, one of the two results unused."""
+    B, H, S, D, rot = 2, 3, 7, 48, 32
+    cos, sin = skv.rotary_tables(rot, 64, scaling="ntk_parts", factor=4.0, original_positions=8)
+    pos = torch.randint(0, 64, (B, S), generator=_gen(1), device="cuda")
+    gen = _gen(2)
+    x = torch.randn(B, S, H + 1, D, generator=gen, device="cuda").to(dtype).requires_grad_()
+    for inverse in (False, True):
+        for used in ("qk", "q", "k"):
+            rows = x.transpose(1, 2)
+            q, k = rows[:, :H], rows[:, H:].expand(B, H, S, D)
+            yq, yk = skv.apply_rotary(q, cos, sin, k, pos, interleaved, inverse)
+            gq, gk = (torch.randn(B, H, S, D, generator=gen, device="cuda").to(dtype) for _ in range(2))
+            x.grad = None
+            torch.autograd.backward([y for n, y in (("q", yq), ("k", yk)) if n in used], [g for n, g in (("q", gq), ("k", gk)) if n in used])
+            want, bound = torch.zeros(2, B, S, H + 1, D, dtype=torch.float64, device="cuda")
+            for n, g, to in (("q", gq, slice(0, H)), ("k", gk, None)):
+                if n in used:
+                    turned, off = (t.transpose(1, 2) for t in _turn64(g, cos[pos], sin[pos], interleaved, not inverse))
+                    off = off + HALF[dtype] * (turned.abs() + off) + TINY[dtype]
+                    if to is not None:
+                        want[:, :, to] += turned
+                        bound[:, :, to] += off
+                    else:   # the sum over the heads that share the key, rounded H - 1 times, and added to the rest
+                        want[:, :, H] += turned.sum(2)
+                        bound[:, :, H] += off.sum(2) + H * HALF[dtype] * (turned.abs() + off).sum(2)
+            assert ((x.grad.double() - want).abs() <= bound + HALF[dtype] * want.abs() + TINY[dtype]).all(), (inverse, used)
+    one = x.detach().transpose(1, 2).contiguous().requires_grad_()
+    y = skv.apply_rotary(one, cos, sin, positions=pos, interleaved=interleaved)
+    assert torch.equal(y, skv.apply_rotary(one.detach(), cos, sin, positions=pos, interleaved=interleaved)) and y.requires_grad
+    (g,) = torch.autograd.grad(y, one, torch.ones_like(y), create_graph=True)   # linear: the second turn is the first one's inverse's inverse
+    assert torch.equal(g, skv.apply_rotary(torch.ones_like(y), cos, sin, positions=pos, interleaved=interleaved, inverse=True))
+    with torch.no_grad():
+        assert not skv.apply_rotary(one, cos, sin, positions=pos).requires_grad
+
+
 # ----------------------------------------------------------------------------------------- threads and scratch
 def test_attention_from_two_threads_on_one_stream(skv):
     """Calls whose parts are joined by a second launch, from two host threads on one stream, which share their scratch."""
