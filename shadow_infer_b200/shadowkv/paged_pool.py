@@ -123,6 +123,11 @@ def _pool_fields(k_pages, v_pages, block_table, scale_k, scale_v, batch: int, he
              D, group, code, batch), dev, table)
 
 
+def _staged(host: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """``host`` on ``dev`` without waiting for the GPU: through pinned memory, which torch keeps until the copy is done."""
+    return host.pin_memory().to(dev, non_blocking=True)
+
+
 def _flag(check: bool, dev: torch.device) -> Optional[torch.Tensor]:
     return torch.zeros(1, dtype=torch.int32, device=dev) if check else None
 
@@ -395,10 +400,10 @@ class PagedKVPool:
                 if n:
                     table[b, grown[b] - n:grown[b]] = torch.tensor(taken[at:at + n], dtype=torch.int32)
                     at += n
-            block_table = table.to(self.lengths.device)
+            block_table = _staged(table, self.lengths.device)
         else:
             block_table = self.block_table
-        fresh = None if new_lengths is None else torch.tensor(new, dtype=torch.int32, device=self.lengths.device)
+        fresh = None if new_lengths is None else _staged(torch.tensor(new, dtype=torch.int32), self.lengths.device)
         out = paged_append(k, v, self.k_pages, self.v_pages, block_table, self.lengths, self.scale_k, self.scale_v, fresh,
                            q, cos, sin, positions, interleaved, check)
         if sum(wanted):
@@ -427,8 +432,8 @@ class PagedKVPool:
         n = self._pages_held(b)
         self._free.extend(reversed(self._table[b, :n].tolist()))
         self._table[b] = -1
-        self.block_table[b] = -1
-        self.lengths[b] = 0
+        self.block_table[b].fill_(-1)
+        self.lengths[b:b + 1 or None].zero_()   # (an assignment to one element waits for the GPU)
         self.token_counts[b] = 0
         return n
 
@@ -462,7 +467,7 @@ def paged_block_forward(block, hidden: torch.Tensor, pool: PagedKVPool, cos: Opt
         pool.append(k, v, new_lengths=new_lengths)
     else:
         q = pool.append(k, v, q=q, cos=cos, sin=sin, new_lengths=new_lengths)
-    fresh = None if new_lengths is None else torch.tensor(list(new_lengths), dtype=torch.int32, device=hidden.device)
+    fresh = None if new_lengths is None else _staged(torch.tensor(list(new_lengths), dtype=torch.int32), pool.lengths.device)
     attn = pool.attention(q, causal=causal, new_lengths=fresh).transpose(1, 2).reshape(B, S, nh * hd)
     hidden = hidden + block.o_proj(attn)
     return hidden + block.down_proj(F.gelu(block.up_proj(block.ln2(hidden))))

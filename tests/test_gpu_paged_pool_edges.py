@@ -291,6 +291,43 @@ def test_rotary_backward(skv, dtype, interleaved):
         assert not skv.apply_rotary(one, cos, sin, positions=pos).requires_grad
 
 
+def test_pool_does_not_wait_for_the_gpu(skv):
+    """Taking pages, ragged appends, the block's forward and the end of a sequence put work on the stream and return."""
+    pool = skv.PagedKVPool(64, 2, 2, 32, max_tokens=128, page_size=8, precision="int8")
+    cos, sin = skv.rotary_tables(32, 128)
+
+    class Block(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.hidden_dim, self.num_heads, self.head_dim = 64, 2, 32
+            self.ln1, self.ln2 = torch.nn.LayerNorm(64), torch.nn.LayerNorm(64)
+            self.q_proj, self.k_proj, self.v_proj, self.o_proj, self.up_proj, self.down_proj = (torch.nn.Linear(64, 64) for _ in range(6))
+
+    block = Block().cuda()
+    x = torch.randn(2, 2, 20, 32, generator=_gen(1), device="cuda")
+    hidden = torch.randn(2, 9, 64, generator=_gen(2), device="cuda")
+
+    def steps():
+        pool.append(x, x, q=x, cos=cos, sin=sin, new_lengths=[20, 3])
+        pool.append(x[:, :, :5], x[:, :, :5])
+        y = skv.paged_block_forward(block, hidden, pool, cos, sin, causal=True, new_lengths=[9, 4])
+        pool.read(10)
+        pool.release(1)
+        return y
+
+    with torch.no_grad():
+        steps()
+        pool.release(0)
+        torch.cuda.synchronize()
+        torch.cuda.set_sync_debug_mode("error")
+        try:
+            steps()
+        finally:
+            torch.cuda.set_sync_debug_mode("default")
+    assert pool.lengths.tolist() == pool.token_counts == [34, 0]
+    assert pool.block_table[0, :5].tolist() == pool._table[0, :5].tolist() and (pool.block_table[1] == -1).all()
+
+
 # ----------------------------------------------------------------------------------------- threads and scratch
 def test_attention_from_two_threads_on_one_stream(skv):
     """Calls whose parts are joined by a second launch, from two host threads on one stream, which share their scratch."""
