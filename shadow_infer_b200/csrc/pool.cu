@@ -418,7 +418,7 @@ int launch_append(const skv_pool_append_args& a, cudaStream_t st) {
                aligned16(a.pool.k) && aligned16(a.pool.v) && aligned16(a.rope.cos) && aligned16(a.rope.sin);
     if (split) vec = vec && rot % 16 == 0 && (a.pool.precision != 3 || (G % 8 == 0 && power(G / 8) && rot / 2 % G == 0 && (D - rot) / 2 % G == 0));
     else vec = vec && rot % 8 == 0 && (a.pool.precision != 3 || G == 8 || (G % 16 == 0 && power(G / 16)));
-    vec = vec && H <= 65535;   // grid.y
+    vec = vec && H <= 65535 && tokens <= 0x7fffffff - 64;   // grid.y; tokens are numbered in 31 bits there
     if (!vec) {
         const int64_t blocks = (tokens * H + kPoolWarps - 1) / kPoolWarps;
         pool_append_any_kernel<T><<<(unsigned)blocks, 32 * kPoolWarps, 0, st>>>(a);
@@ -509,6 +509,7 @@ int skv_pool_read(const skv_pool_read_args* args, void* stream) {
         return fail(SKV_ERR_SHAPE, "pool_read: outputs disagree in heads or dtype");
     if (a.pool.batch == 0 || a.S == 0) return SKV_OK;
     if (!a.lengths) return fail(SKV_ERR_INVALID_ARGUMENT, "pool_read: lengths is null");
+    if (a.S > 0x7fffffff - 4096) return fail(SKV_ERR_TOO_LARGE, "pool_read: too many tokens");   // a block's last is numbered in 31 bits
     const int64_t blocks = ((int64_t)a.pool.batch * a.S * a.pool.heads + kPoolWarps - 1) / kPoolWarps;
     if (blocks > 0x7fffffff) return fail(SKV_ERR_TOO_LARGE, "pool_read: too many rows");
     cudaStream_t st = as_stream(stream);

@@ -197,7 +197,7 @@ extern "C" int skv_rotary(const skv_rotary_args* args, void* stream) {
         return fail(SKV_ERR_SHAPE, "rotary: q, k and their outputs disagree in heads or dtype");
     const int64_t tokens = (int64_t)a.B * a.S, H = (int64_t)a.q.heads + a.k.heads;
     if (tokens == 0 || H == 0) return SKV_OK;
-    if (tokens > 0x7fffffff || H * a.D > 0x7fffffff) return fail(SKV_ERR_TOO_LARGE, "rotary: too many rows");
+    if (tokens > 0x7fffffff - 64 || H * a.D > 0x7fffffff) return fail(SKV_ERR_TOO_LARGE, "rotary: too many rows");
     cudaStream_t st = as_stream(stream);
     if (a.q.dtype == kF32) return launch_rotary<float>(a, st);
     if (a.q.dtype == kF16) return launch_rotary<__half>(a, st);

@@ -192,6 +192,20 @@ def test_rows_of_different_types(skv, kt, vt, qt):
             assert b.dtype == a.dtype and torch.equal(b, skv.apply_rotary(a, cos, sin))
 
 
+def test_append_of_more_rows_than_31_bits_number(skv):
+    """2^31 rows and more, nearly all of them padding: the tokens are written all the same."""
+    S, D = 2 ** 30 + 100, 16
+    pages, _ = _pool("fp32", 2, 1, 8, D)
+    table = torch.tensor([[1], [0]], dtype=torch.int32, device="cuda")
+    k, v = (_rows(_gen(i), 2, 1, 1, D, torch.float32) for i in range(2))
+    new = torch.tensor([5, 8], dtype=torch.int32, device="cuda")
+    skv.paged_append(k.expand(2, 1, S, D), v.expand(2, 1, S, D), *pages, table, torch.zeros_like(new), new_lengths=new, check=True)
+    for mine, rows in zip(pages, (k, v)):
+        want = torch.zeros_like(mine)
+        want[1, 0, :5], want[0, 0] = rows[0, 0], rows[1, 0]
+        assert torch.equal(mine, want)
+
+
 # ------------------------------------------------------------------------------------ values that are not finite
 ODD = [  # counts, H, rep, Sq, D, P, new: kernels for few rows, for many, and for any size
     ([200, 37], 2, 2, 9, 128, 16, None),

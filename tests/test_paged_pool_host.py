@@ -146,3 +146,15 @@ def test_attention_scratch_is_sized_by_device(monkeypatch):
     monkeypatch.setattr(paged_pool, "_SCRATCH_BYTES", {})
     got = [paged_pool._scratch(torch.device("meta", i), 7, 128).numel() for i in (0, 1, 0, 1)]
     assert got == [12800, 20480, 12800, 20480]
+
+
+def test_rows_that_31_bits_do_not_number_are_refused():
+    from shadow_infer_b200 import _lib
+    from shadow_infer_b200.shadowkv import paged_pool, rotary
+    lib = _lib.load()
+    rows, none = (16, 0, 0, 0, 0, 1), (0,) * 6
+    for S in (2 ** 31 - 1, 2 ** 31 - 10):
+        assert lib.skv_rotary(rotary._ARGS.pack(*rows, *none, *rows, *none, 16, 16, 0, 0, 0, 0, 8, 4, 0, 0, 0, 1, S, 8, 0),
+                              None) == _lib.SKV_ERR_TOO_LARGE
+        pool = (16, 16, 0, 0, 16, 4, 4, 4, 8, 1, 8, 0, 0, 1)
+        assert lib.skv_pool_read(paged_pool._READ.pack(*pool, *rows, *rows, 0, 16, 0, S, 0), None) == _lib.SKV_ERR_TOO_LARGE
