@@ -275,6 +275,7 @@ int skv_pool_attention(const skv_pool_attention_args* args, void* stream) {
                     a.pool.heads);
     if (a.pool.batch == 0 || a.S_q == 0 || a.q.heads == 0) return SKV_OK;
     if (!a.lengths || !a.scratch) return fail(SKV_ERR_INVALID_ARGUMENT, "pool_attention: null pointer");
+    if (reinterpret_cast<uintptr_t>(a.scratch) & 15) return fail(SKV_ERR_INVALID_ARGUMENT, "pool_attention: scratch is not on a 16-byte boundary");
     if (a.pool.head_dim > kAnyMaxD)
         return fail(SKV_ERR_UNSUPPORTED, "pool_attention: head_dim %d above %d", a.pool.head_dim, kAnyMaxD);
     if ((int64_t)a.q.heads * a.S_q > (1 << 28) || a.pool.batch > (1 << 24))

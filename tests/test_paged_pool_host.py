@@ -158,3 +158,15 @@ def test_rows_that_31_bits_do_not_number_are_refused():
                               None) == _lib.SKV_ERR_TOO_LARGE
         pool = (16, 16, 0, 0, 16, 4, 4, 4, 8, 1, 8, 0, 0, 1)
         assert lib.skv_pool_read(paged_pool._READ.pack(*pool, *rows, *rows, 0, 16, 0, S, 0), None) == _lib.SKV_ERR_TOO_LARGE
+
+
+def test_attention_refuses_scratch_between_16_byte_boundaries():
+    """Parts go to the scratch 16 bytes at a time."""
+    from shadow_infer_b200 import _lib
+    from shadow_infer_b200.shadowkv import paged_pool
+    lib = _lib.load()
+    pool, rows = (16, 16, 0, 0, 16, 4, 4, 4, 8, 2, 8, 0, 0, 1), (16, 8, 8, 8, 0, 2)
+    for scratch in (4, 24, 40):   # (with too few bytes too: nothing is launched either way)
+        args = paged_pool._ATTENTION.pack(*pool, *rows, *rows, 16, 0, scratch, 100, 0, 1, 0, 1.0, 0)
+        assert lib.skv_pool_attention(args, None) == _lib.SKV_ERR_INVALID_ARGUMENT
+        assert "boundary" in _lib.last_error()
