@@ -384,7 +384,7 @@ int skv_irap_importance(const float* scores, int B, int H, int Sq, int Sk, int i
  * written / not attended to / zero when read.  A token whose position lies outside the rotary
  * tables is not written either, key or value (its rows keep what they held: do not count it), and
  * a row that skv_rotary turns, or a query of skv_pool_append, is NaN there.  Where error_flag (device int32) is not
- * NULL, the first two and the unwritten token set it to 1.
+ * NULL, the first two, the unwritten token and a negative length (nothing is held) set it to 1.
  * Outputs share no memory with inputs.
  * ------------------------------------------------------------------------------------- */
 typedef struct skv_pool {

@@ -342,6 +342,7 @@ __global__ void __launch_bounds__(32 * kPoolWarps) pool_read_any_kernel(const __
     const int b = (int)(bh / H), h = (int)(bh % H);
     const int64_t t = (a.start ? (int64_t)a.start[b] : 0) + s;
     const bool held = t >= 0 && t < a.lengths[b];
+    if (a.lengths[b] < 0 && lane == 0 && a.error_flag) atomicExch(a.error_flag, 1);
     int64_t row = held ? pool_row(a.pool, b, t) : -1;
     if (held && row < 0 && lane == 0 && a.error_flag) atomicExch(a.error_flag, 1);
     if (row >= 0) row += (int64_t)h * a.pool.page_size;
@@ -362,6 +363,7 @@ __global__ void __launch_bounds__(256) pool_read_kernel(const __grid_constant__ 
     const int b = blockIdx.y / a.pool.heads, h = blockIdx.y - b * a.pool.heads, d = V * threadIdx.x;
     const int64_t first = a.start ? (int64_t)a.start[b] : 0, length = a.lengths[b];
     const int s0 = blockIdx.x * blockDim.y * FLY + threadIdx.y;
+    if (length < 0 && threadIdx.x == 0 && a.error_flag) atomicExch(a.error_flag, 1);
     PoolRaw<PREC, V> k[FLY], v[FLY];
     int64_t row[FLY];
 #pragma unroll

@@ -141,7 +141,7 @@ __device__ __forceinline__ Segment segment_at(const skv_pool_attention_args& a, 
             g.t1 = min(nt, g.next - g.first);
             g.whole = g.t0 == 0 && g.t1 == nt;
             g.slot = at == s.lo ? 0 : 1;
-            if (a.error_flag && a.lengths[b] > g.tokens && threadIdx.x == 0) atomicExch(a.error_flag, 1);
+            if (a.error_flag && a.lengths[b] != g.tokens && threadIdx.x == 0) atomicExch(a.error_flag, 1);
             return g;
         }
         base += all * units;

@@ -121,7 +121,7 @@ __device__ __forceinline__ TcSegment tc_segment_at(const skv_pool_attention_args
         g.t1 = min(nt, g.next - g.first);
         g.whole = g.t0 == 0 && g.t1 == nt;
         g.slot = at == s.lo ? 0 : 1;
-        if (a.error_flag && a.lengths[b] > g.tokens && threadIdx.x == 0) atomicExch(a.error_flag, 1);
+        if (a.error_flag && a.lengths[b] != g.tokens && threadIdx.x == 0) atomicExch(a.error_flag, 1);
         return g;
     }
 }

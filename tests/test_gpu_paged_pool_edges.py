@@ -192,6 +192,19 @@ def test_rows_of_different_types(skv, kt, vt, qt):
             assert b.dtype == a.dtype and torch.equal(b, skv.apply_rotary(a, cos, sin))
 
 
+@pytest.mark.parametrize("Sq,D", [(1, 64), (60, 64), (1, 33)])
+def test_negative_lengths_hold_nothing_and_are_named(skv, Sq, D):
+    pages, scales, table, lens = _filled(skv, "fp16", [100, 40], 2, 32, D, 16, 2)
+    q = _rows(_gen(3), 2, 4, Sq, D, torch.float16)
+    lens[1] = -1
+    got = skv.paged_attention(q, *pages, table, lens)
+    assert (got[1] == 0).all() and (got[0] != 0).any() and (skv.paged_read(*pages, table, lens, 40)[0][1] == 0).all()
+    with pytest.raises(ValueError, match="length"):
+        skv.paged_attention(q, *pages, table, lens, check=True)
+    with pytest.raises(ValueError, match="length"):
+        skv.paged_read(*pages, table, lens, 40, head_dim=D, check=True)
+
+
 def test_append_of_more_rows_than_31_bits_number(skv):
     """2^31 rows and more, nearly all of them padding: the tokens are written all the same."""
     S, D = 2 ** 30 + 100, 16
