@@ -4,6 +4,7 @@
 // value are stored in the pool's precision, bit-identical to the paged store's rows (paged.cu):
 //     int8: scale = amax / 127 over the row, int4: amax / 7 over a group; 1 where the amax is 0;
 //     n = rint(x / scale), clamped; int4 keeps n + 8, the even value in the high nibble.
+// A NaN makes its scale NaN, so that its row or group is read as NaN (paged.cu's leaves it out of the scale).
 // A token without a page, or whose position the rotary tables do not hold, leaves its rows as they were.
 // Everything is read once and written once.  A token a sequence is bound by its latency: 8 sequences, 32 + 8 + 8 heads of 128
 // values, 3.0 us.  A prompt is bound by what it computes: 8 x 2048 fp16 tokens of 32 + 32 heads into int8 take 112 us, about 320
@@ -27,6 +28,19 @@ int check_pool(const skv_pool& p, const char* what) {
 }
 
 constexpr int kPoolWarps = 4;
+
+// max that keeps a NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+// Over aligned groups of `width` lanes (a power of two <= 32).
+__device__ __forceinline__ float group_max_nan(float x, int width) {
+    for (int o = width >> 1; o > 0; o >>= 1) x = max_nan(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
+}
 
 // A warp's view of one source row: value d, turned where the row is a query or a key.
 template <class T>
@@ -94,15 +108,15 @@ __global__ void __launch_bounds__(32 * kPoolWarps) pool_append_any_kernel(const 
         for (int d = lane; d < D; d += kWarp) reinterpret_cast<__half*>(base)[row * D + d] = __float2half_rn(x(d));
     } else if (a.pool.precision == 2) {
         float m = 0.0f;
-        for (int d = lane; d < D; d += kWarp) m = fmaxf(m, fabsf(x(d)));
-        const float scale = quant_scale(warp_max(m), 127.0f), rcp = __frcp_rn(scale);
+        for (int d = lane; d < D; d += kWarp) m = max_nan(m, fabsf(x(d)));
+        const float scale = quant_scale(group_max_nan(m, kWarp), 127.0f), rcp = __frcp_rn(scale);
         for (int d = lane; d < D; d += kWarp) base[row * D + d] = (uint8_t)quant_value_fast(x(d), scale, rcp, -128, 127);
         if (lane == 0) sc[row] = scale;
     } else {
         const int G = a.pool.int4_group, ng = D / G;
         for (int g = lane; g < ng; g += kWarp) {
             float m = 0.0f;
-            for (int d = g * G; d < (g + 1) * G; ++d) m = fmaxf(m, fabsf(x(d)));
+            for (int d = g * G; d < (g + 1) * G; ++d) m = max_nan(m, fabsf(x(d)));
             sc[row * ng + g] = quant_scale(m, 7.0f);
         }
         __syncwarp();
@@ -124,18 +138,10 @@ __global__ void __launch_bounds__(32 * kPoolWarps) pool_append_any_kernel(const 
 
 constexpr float kRoundMagic = 12582912.0f;   // 1.5 2^23: x + this has rint(x) in its low bits for |x| < 2^22
 
-// max that keeps a NaN
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
-}
-
 // t[e] = 1.5 2^23 + add + rint(fl(x[e] / s)), whose low byte is the integer (+ add) that is stored.  r is the correctly
 // rounded 1 / s; then q + r (x - q s), the residual by one fma, is the correctly rounded quotient (Markstein's correction,
 // IBM J. Res. Dev. 34, 1990), so the integers are those of a division at a third of its instructions.  `odd`: the
-// row's values or its scale leave that theorem's range (NaN, infinities, scales near the ends of fp32); then the division is
-// made.
+// row's scale leaves that theorem's range (NaN, infinite, near the ends of fp32); then the division is made.
 __device__ __forceinline__ void quotients(const float (&x)[8], float s, float r, bool odd, int lo, int hi, float add, float (&t)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -288,21 +294,12 @@ __global__ void __launch_bounds__(256, 3) pool_append_kernel(const __grid_consta
             m0 = max_nan(m0, fabsf(x[e]));
             m1 = max_nan(m1, fabsf(y[e]));
         }
-        const bool nan = m0 != m0 || m1 != m1;
-        if (__any_sync(0xffffffffu, nan)) {   // a NaN does not count for its row's scale
-            m0 = m1 = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                m0 = fmaxf(m0, fabsf(x[e]));
-                m1 = fmaxf(m1, fabsf(y[e]));
-            }
-        }
         float f[8], g[8];
         if (p == 2) {
-            const float m = group_max(fmaxf(m0, m1), blockDim.x);
+            const float m = group_max_nan(max_nan(m0, m1), blockDim.x);
             if (!write) continue;
             const float scale = scale_of(m, 127.0f, 1.0f / 127.0f), rcp = __frcp_rn(scale);
-            const bool odd = nan || !(scale > 1e-30f && scale < 1e30f);
+            const bool odd = !(scale > 1e-30f && scale < 1e30f);
             quotients(x, scale, rcp, odd, -128, 127, 0.0f, f);
             quotients(y, scale, rcp, odd, -128, 127, 0.0f, g);
             uint8_t* dst = to + off * row_bytes;
@@ -311,14 +308,14 @@ __global__ void __launch_bounds__(256, 3) pool_append_kernel(const __grid_consta
             if (i0 == 0) sc[off] = scale;
         } else {
             if (SPLIT) {           // a group is the same chunk of G / 8 lanes
-                m0 = group_max(m0, G / 8);
-                m1 = group_max(m1, G / 8);
+                m0 = group_max_nan(m0, G / 8);
+                m1 = group_max_nan(m1, G / 8);
             } else if (G > 8) {    // both chunks of G / 16 lanes
-                m0 = m1 = group_max(fmaxf(m0, m1), G / 16);
+                m0 = m1 = group_max_nan(max_nan(m0, m1), G / 16);
             }
             if (!write) continue;
             const float s0 = scale_of(m0, 7.0f, 1.0f / 7.0f), s1 = scale_of(m1, 7.0f, 1.0f / 7.0f);
-            const bool odd = nan || !(fminf(s0, s1) > 1e-30f && fmaxf(s0, s1) < 1e30f);
+            const bool odd = !(s0 > 1e-30f && s1 > 1e-30f && s0 < 1e30f && s1 < 1e30f);
             quotients(x, s0, __frcp_rn(s0), odd, -8, 7, 8.0f, f);
             quotients(y, s1, __frcp_rn(s1), odd, -8, 7, 8.0f, g);
             uint8_t* dst = to + off * row_bytes;

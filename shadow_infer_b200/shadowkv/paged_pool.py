@@ -164,7 +164,8 @@ def paged_append(
     ``apply_rotary``; default: the token's index.
 
     The pages' precision is their type.  Rows and scales are those of ``PagedKVStore.append``
-    (paged_kv_store.py:189-224): int8 ``amax / 127`` a row, int4 ``amax / 7`` a group.  One launch.
+    (paged_kv_store.py:189-224): int8 ``amax / 127`` a row, int4 ``amax / 7`` a group; one that holds a NaN has
+    the scale NaN and is read as NaN.  One launch.
     """
     shape = k.shape
     if len(shape) != 4 or v.shape != shape:

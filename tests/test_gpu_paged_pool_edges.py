@@ -205,6 +205,87 @@ def test_negative_lengths_hold_nothing_and_are_named(skv, Sq, D):
         skv.paged_read(*pages, table, lens, 40, head_dim=D, check=True)
 
 
+def _alike(a, b, but=None):
+    """Equal, NaN where the other is, apart from `but`."""
+    same = (a == b) | (a.isnan() & b.isnan()) if a.dtype.is_floating_point else a == b
+    return bool((same if but is None else same | but).all())
+
+
+PROMPTS = [  # B, Hq, Hk, S, D, rot, P, G: enough tokens that a thread takes several rows, and a block several tokens
+    (2, 8, 5, 400, 128, 128, 32, 16), (3, 0, 7, 900, 64, 32, 16, 16), (2, 6, 9, 500, 96, 96, 17, 8), (1, 4, 3, 2000, 256, 128, 64, 32),
+    (8, 4, 1, 1200, 128, 64, 32, 16), (4, 2, 2, 4000, 64, 64, 128, 32), (2, 5, 6, 600, 80, 0, 32, 16),
+]
+
+
+@pytest.mark.parametrize("B,Hq,Hk,S,D,rot,P,G", PROMPTS)
+@pytest.mark.parametrize("kv", ["fp32", "fp16", "int8", "int4"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_of_prompts(skv, B, Hq, Hk, S, D, rot, P, G, kv, dtype, interleaved):
+    """Ragged prompts: the paged store's rows, those with infinite, NaN, very large and very small values too."""
+    gen = _gen(S)
+    first, new = [5 * b for b in range(B)], [S - 13 * b for b in range(B)]
+    table, N = _table([a + n for a, n in zip(first, new)], P, S)
+    (kp, vp), (sk, sv) = _pool(kv, N, Hk, P, D, G)
+    k, v = (_rows(gen, B, Hk, S, D, dtype, "projection") for _ in range(2))
+    for x in (k, v):
+        x[0, 0, 3::50, 2], x[0, -1, 7::50, 5], x[0, 0, 11::50, 1] = math.inf, math.nan, -math.inf
+        x[:, :, 17::40] *= 1e-6
+        x[:, 0, 23::40] *= 1e4
+        x[:, :, 29::60] = 0
+        x[0, :, 31::60] = math.nan
+    q = _rows(gen, B, Hq, S, D, dtype, "projection") if Hq and rot else None
+    cos, sin = skv.rotary_tables(rot, S + 100) if rot else (None, None)
+    lens, fresh = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in (first, new))
+    out = skv.paged_append(k, v, kp, vp, table, lens, sk, sv, fresh, q, cos, sin, interleaved=interleaved, check=True)
+    at = lens.long()[:, None] + torch.arange(S, device="cuda")
+    turned = _turn32(k, cos[at], sin[at], interleaved) if rot else k.float()
+    if q is not None:
+        assert _alike(out, _turn32(q, cos[at], sin[at], interleaved).to(dtype))
+    store = skv.PagedKVStore(B, Hk, D, page_size=S, device="cuda", int4_group_size=G)
+    store.append(turned.contiguous(), v.float().contiguous(), kv)
+    for b in range(B):
+        where = torch.arange(first[b], first[b] + new[b], device="cuda")
+        ids, row = table[b].long()[where // P], where % P
+        for pages, scale, rows, theirs in ((kp, sk, turned, (store.pages[0].k, store.pages[0].scale_k)),
+                                           (vp, sv, v.float(), (store.pages[0].v, store.pages[0].scale_v))):
+            mine, nan = pages[ids, :, row].transpose(0, 1), None
+            if scale is not None:   # a row or group that holds a NaN has a scale of NaN, and integers that mean nothing
+                kept = scale[ids, :, row].transpose(0, 1)
+                groups = kept.shape[2] if kv == "int4" else 1
+                nan = rows[b, :, :new[b]].unflatten(-1, (groups, -1)).isnan().any(-1)
+                assert torch.equal(kept.isnan().view(nan.shape), nan)
+                assert _alike(kept, theirs[1][b, :, :new[b]], nan.view(kept.shape))
+                scale[ids, :, row] = 1
+                nan = nan[..., None].expand(*nan.shape, mine.shape[-1] // groups).flatten(-2)
+            assert _alike(mine, theirs[0][b, :, :new[b]], nan), b
+            pages[ids, :, row] = 0
+    assert all((t == 0).all() for t in (kp, vp)) and all(t is None or (t == 1).all() for t in (sk, sv))   # nothing else was written
+
+
+@pytest.mark.parametrize("D,G,layout", [(64, 16, "bhsd"), (64, 32, "projection"), (40, 8, "bhsd"), (33, 33, "bhsd"), (96, 16, "odd")])
+@pytest.mark.parametrize("kv", ["fp32", "fp16", "int8", "int4"])
+def test_a_nan_is_read_as_one(skv, D, G, layout, kv):
+    """A NaN among the values of a row: what its scale is shared by is NaN when read, everything else is as without it."""
+    (kp, vp), (sk, sv) = _pool(kv, 2, 2, 8, D, G)
+    table, zero = torch.tensor([[1]], dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    k, v = (_rows(_gen(i), 1, 2, 8, D, torch.float32, layout) for i in range(2))
+    seen = torch.full((1,), 8, dtype=torch.int32, device="cuda")
+
+    def held():
+        skv.paged_append(k, v, kp, vp, table, zero, sk, sv, check=True)
+        return skv.paged_read(kp, vp, table, seen, 8, sk, sv, head_dim=D, check=True)
+
+    clean = held()
+    k[0, 0, 3, 5] = v[0, 1, 6, D - 1] = math.nan
+    odd = held()
+    wide = {"int8": D, "int4": G if D % G == 0 else D}.get(kv, 1)
+    for t, (h, s, d), before, now in ((k, (0, 3, 5), clean[0], odd[0]), (v, (1, 6, D - 1), clean[1], odd[1])):
+        nan = torch.zeros(1, 2, 8, D, dtype=torch.bool, device="cuda")
+        nan[0, h, s, d // wide * wide:d // wide * wide + wide] = True
+        assert torch.equal(now.isnan(), nan) and torch.equal(now[~nan], before[~nan])
+
+
 def test_append_of_more_rows_than_31_bits_number(skv):
     """2^31 rows and more, nearly all of them padding: the tokens are written all the same."""
     S, D = 2 ** 30 + 100, 16
@@ -276,6 +357,20 @@ def test_attention_of_values_that_are_not_finite(skv, counts, H, rep, Sq, D, P, 
         assert torch.equal(~torch.isfinite(mine), hit)
         off = torch.where(hit, -1.0, (mine - want).abs() - bound)
         assert off.max() <= 0, float(off.max())
+
+
+@pytest.mark.parametrize("B,Hq,Hk,S,D,rot", [(2, 1, 0, 8000, 128, 128), (3, 2, 1, 6000, 64, 32), (1, 5, 3, 20000, 64, 64), (1, 40, 8, 3000, 128, 128)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_of_prompts(skv, B, Hq, Hk, S, D, rot, dtype, interleaved):
+    """Enough tokens that a block takes several."""
+    gen = _gen(S)
+    cos, sin = skv.rotary_tables(rot, S)
+    q, k = (_rows(gen, B, max(H, 1), S, D, dtype, "projection") for H in (Hq, Hk))
+    got = skv.apply_rotary(q, cos, sin, k=k if Hk else None, interleaved=interleaved)
+    at = torch.arange(S, device="cuda").expand(B, S)
+    for x, y in zip((q, k), got if Hk else (got,)):
+        assert torch.equal(y, _turn32(x, cos[at], sin[at], interleaved).to(dtype))
 
 
 # ------------------------------------------------------------------------------------------------ gradients
