@@ -359,6 +359,33 @@ def test_attention_of_values_that_are_not_finite(skv, counts, H, rep, Sq, D, P, 
         assert off.max() <= 0, float(off.max())
 
 
+@pytest.mark.parametrize("counts,H,rep,Sq,D,P,new", ODD)
+@pytest.mark.parametrize("kv", ["fp32", "fp16", "int8", "int4"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_attention_of_keys_that_are_nan(skv, counts, H, rep, Sq, D, P, new, kv, dtype):
+    """A NaN among the newest keys: the queries of its head that see it are NaN, the others are what they were."""
+    pages, scales, table, lens = _filled(skv, kv, counts, H, P, D, 16, sum(counts) + D)
+    q = _rows(_gen(5), len(counts), H * rep, Sq, D, dtype)
+    new = new or [Sq] * len(counts)
+    want, bound = _attention64(q, pages, scales, table, counts, new, True)
+    hit = torch.zeros(q.shape[:3], dtype=torch.bool, device="cuda")
+    for b, n in enumerate(counts):
+        t, h = n - 1 - Sq // 3, b % H
+        if t < 0:
+            continue
+        page = int(table[b, t // P])
+        if scales[0] is None:
+            pages[0][page, h, t % P, 3] = math.nan
+        else:
+            scales[0][page, h, t % P, 0] = math.nan
+        i = torch.arange(Sq, device="cuda")
+        hit[b, h * rep:(h + 1) * rep] |= (i < new[b]) & (t <= n - new[b] + i)
+    got = skv.paged_attention(q, *pages, table, lens, *scales, causal=True, new_lengths=torch.tensor(new, dtype=torch.int32, device="cuda"))
+    assert got[hit].isnan().all() and not got[~hit].isnan().any()
+    off = (got[~hit].double() - want[~hit]).abs() - bound[~hit]
+    assert off.max() <= 0, float(off.max())
+
+
 @pytest.mark.parametrize("B,Hq,Hk,S,D,rot", [(2, 1, 0, 8000, 128, 128), (3, 2, 1, 6000, 64, 32), (1, 5, 3, 20000, 64, 64), (1, 40, 8, 3000, 128, 128)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("interleaved", [False, True])
