@@ -381,30 +381,32 @@ __device__ __forceinline__ uint4 finite_halves(uint4 w) {
 }
 
 // Adds what is not finite among the values of tokens [from, to) to rows r0 .. r0 + rows - 1 of a unit, in its part or, where that is
-// null, in the output.  Rare, so it is slow and reads the pages again; thread tid of `threads`, between barriers of them.
+// null, in the output.  Rare, so it reads the pages again; thread tid of `threads`, which has every threads-th value of a row,
+// between barriers of them.
 template <int PREC>
 __device__ __noinline__ void add_not_finite(const skv_pool_attention_args& a, int b, int hk, int tokens, int r0, int rows, int from, int to,
                                             float* part, int tid, int threads) {
     const int D = a.pool.head_dim, rep = a.q.heads / a.pool.heads;
-    for (int i = tid; i < rows * D; i += threads) {
-        const int j = i / D, d = i - j * D, r = r0 + j;
-        const int end = min(to, seen_by(a, b, tokens, r % a.S_q));
-        float sum = 0.0f;
-        for (int t = from; t < end; ++t) {
+    for (int d = tid; d < D; d += threads) {
+        const int block = PREC == 3 ? d / a.pool.int4_group : 0;
+#pragma unroll 4
+        for (int t = from; t < to; ++t) {
             const int64_t row = pool_row(a.pool, b, t);
-            if (row < 0) continue;
-            const float v = pool_value<PREC>(a.pool, true, row + (int64_t)hk * a.pool.page_size, d, PREC == 3 ? d / a.pool.int4_group : 0);
-            if (!finite(v)) sum += v;
-        }
-        if (sum == 0.0f) continue;
-        if (part) {
-            part[i] += sum;
-        } else {
-            const float x = a.out.dtype == kF32   ? row_ptr<float>(a.out, a.S_q, rep, b, hk, r)[d]
-                            : a.out.dtype == kF16 ? to_float(row_ptr<__half>(a.out, a.S_q, rep, b, hk, r)[d])
-                                                  : to_float(row_ptr<__nv_bfloat16>(a.out, a.S_q, rep, b, hk, r)[d]);
-            const float one[1] = {x + sum};
-            store_out<1>(a, b, hk, r, d, one);
+            const float v = row < 0 ? 0.0f : pool_value<PREC>(a.pool, true, row + (int64_t)hk * a.pool.page_size, d, block);
+            if (finite(v)) continue;
+            for (int j = 0; j < rows; ++j) {
+                const int r = r0 + j;
+                if (t >= seen_by(a, b, tokens, r % a.S_q)) continue;
+                if (part) {
+                    part[j * D + d] += v;
+                } else {
+                    const float x = a.out.dtype == kF32   ? row_ptr<float>(a.out, a.S_q, rep, b, hk, r)[d]
+                                    : a.out.dtype == kF16 ? to_float(row_ptr<__half>(a.out, a.S_q, rep, b, hk, r)[d])
+                                                          : to_float(row_ptr<__nv_bfloat16>(a.out, a.S_q, rep, b, hk, r)[d]);
+                    const float one[1] = {x + v};
+                    store_out<1>(a, b, hk, r, d, one);
+                }
+            }
         }
     }
 }

@@ -277,7 +277,9 @@ __host__ __device__ constexpr size_t mma_smem() {
 }
 
 // exact: the head has DP values (and, for int4, groups of 16): rows and scales are copied whole, in steps known here.
-template <int PREC, int DP, int NT, int NQ, int NP>
+// LIMIT: rows may see different tokens (several new ones under a causal limit).  Without it the look at fp16 and fp32 values is
+// left out, which costs a call of one token 3 %.
+template <int PREC, int DP, int NT, int NQ, int NP, bool LIMIT>
 __global__ void __launch_bounds__(32 * MmaShape<PREC, DP, NT>::W, MmaShape<PREC, DP, NT>::CTAS)
 pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int row_tiles, PageDivide magic, bool exact, bool q_vec,
                           bool out_vec) {
@@ -551,7 +553,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                 }
                 __syncwarp();
             }
-            if constexpr (PREC <= 1) {
+            if constexpr (PREC <= 1 && LIMIT) {
                 if (t0 >= not_all) {   // values that are not finite wait until the rows that see them are known apart
                     const bool odd = leave_out<PREC, 16 * L::CHUNKS>(reinterpret_cast<uint4*>(slot + L::V));
                     if (odd) s_odd = 1;
@@ -1036,7 +1038,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
             }
             if (t + 1 < NT) __syncthreads();
         }
-        if (PREC != 2 && s_odd) {   // (set before the barriers above)
+        if ((PREC == 3 || (PREC <= 1 && LIMIT)) && s_odd) {   // (set before the barriers above)
             const int first = g.t0 * TILE;
             __syncthreads();
             add_not_finite<PREC>(a, g.b, g.hk, n, r0, min(ROWS, R - r0), PREC == 3 ? first : max(first, not_all), min(n, g.t1 * TILE),
@@ -1052,7 +1054,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
     }
 }
 
-template <int PREC, int DP, int NT, int NQ, int NP>
+template <int PREC, int DP, int NT, int NQ, int NP, bool LIMIT>
 int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
     using Shape = MmaShape<PREC, DP, NT>;
     static_assert(Shape::CTAS * 2 * 8 * NT <= kRowsPerSm, "the scratch holds every CTA's slots");
@@ -1061,7 +1063,7 @@ int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
     const int R = a.q.heads / a.pool.heads * a.S_q, row_tiles = (R + 8 * NT - 1) / (8 * NT);
     const int64_t step = sequences_a_launch(a, row_tiles, 16 * Shape::W, kMmaPad);
     if (step == 0) return SKV_ERR_TOO_LARGE;
-    const auto kernel = pool_attention_mma_kernel<PREC, DP, NT, NQ, NP>;
+    const auto kernel = pool_attention_mma_kernel<PREC, DP, NT, NQ, NP, LIMIT>;
     static std::atomic<uint64_t> allowed{0};   // devices whose limit on the kernel's shared memory was raised
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -1084,11 +1086,18 @@ int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
     });
 }
 
+template <int PREC, int DP, int NT, int NQ, int NP>
+int launch_mma_limit(const skv_pool_attention_args& a, cudaStream_t st) {
+    if constexpr (PREC <= 1)
+        if (a.causal && a.S_q > 1) return launch_mma<PREC, DP, NT, NQ, NP, true>(a, st);
+    return launch_mma<PREC, DP, NT, NQ, NP, false>(a, st);
+}
+
 template <int PREC, int DP, int NT>
 int launch_mma_type(const skv_pool_attention_args& a, cudaStream_t st) {
-    if (a.q.dtype == kF32) return launch_mma<PREC, DP, NT, 2, 2>(a, st);
-    if (a.q.dtype == kF16) return launch_mma<PREC, DP, NT, 1, 2>(a, st);
-    return launch_mma<PREC, DP, NT, 1, 1>(a, st);
+    if (a.q.dtype == kF32) return launch_mma_limit<PREC, DP, NT, 2, 2>(a, st);
+    if (a.q.dtype == kF16) return launch_mma_limit<PREC, DP, NT, 1, 2>(a, st);
+    return launch_mma_limit<PREC, DP, NT, 1, 1>(a, st);
 }
 
 // Row tiles of 8 or 16 rows.  (32 rows a tile were 10 to 20 % faster where hundreds of rows meet 8 K tokens or more,

@@ -38,7 +38,7 @@
 
 namespace skv {
 
-constexpr int kTcRows = 128, kTcThreads = 256, kTcPad = 1;
+constexpr int kTcRows = 128, kTcThreads = 256, kTcPad = 1, kTcOddWords = 8;
 // A fresh maximum's weight is 2^10 to 2^11 and may grow to 2^15: with one fp16 operand a weight, its subnormals' 2^-25 is then
 // 2^-35 of the largest weight.
 constexpr float kTcDrop = 11.0f, kTcRoom = 14.0f;
@@ -126,12 +126,6 @@ __device__ __forceinline__ TcSegment tc_segment_at(const skv_pool_attention_args
     }
 }
 
-// What add_not_finite needs of a unit, written as the unit begins so that none of it stays in registers.  unit: its number among
-// the CTA's, once values of it that are not finite were left out.
-struct TcLeftOut {
-    int unit, b, hk, tokens, r0, rows, from, to, slot;   // slot: of the unit's part, -1 where it is whole
-};
-
 // Shared memory of a CTA.
 template <int DP>
 struct TcLayout {
@@ -179,7 +173,7 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
     __shared__ Share s;
     __shared__ uint32_t s_tmem;
     __shared__ int s_error, s_late;
-    __shared__ TcLeftOut s_odd[4];   // of units u, u + 1, ..: at u & 3
+    __shared__ uint32_t s_odd[kTcOddWords];   // a bit a unit (of its number's last ones): values of it that are not finite were left out
     __shared__ __align__(16) int s_gap[2][4];   // whether the tile misses a token of the sequence, by the warp that looked it up
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(tc_raw) + 1023) & ~uintptr_t(1023));
     float* s_tokens = reinterpret_cast<float*>(sm + L::TOKENS);
@@ -202,7 +196,7 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
         mbar_init(drained, 1);
         fence_mbarrier_init();
         s_error = s_late = 0;
-        for (int i = 0; i < 4; ++i) s_odd[i].unit = -1;
+        for (int i = 0; i < kTcOddWords; ++i) s_odd[i] = 0;
     }
     take_share<kTcThreads>(a, [&](int b) {
         int tokens, n, past;
@@ -222,20 +216,18 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
     int g = 0;      // tiles so far: the barriers complete once a tile (k_full: every second, o_full: once a unit)
     int units = 0;  // units so far
     bool ok = true;
+    // the first token of the tiles that not all rows of a unit see (or an earlier one where the rows are of several heads)
+    auto odd_from = [&](const TcSegment& sg) {
+        const int new_before = u.blocks ? sg.rt % u.blocks * kTcRows : 0;
+        const int old = sg.tokens - (a.new_lengths ? __ldg(a.new_lengths + sg.b) : a.S_q);
+        return not_all_from(a.causal ? max(1, old + 1 + new_before) : sg.tokens, sg.tokens, TILE);
+    };
 
     if (warp < 4) {
         // ------------------------------------------------------------------- softmax, and the MMAs
         const uint32_t t_s = tmem + ((uint32_t)(warp * 32) << 16), t_o = t_s + 128;
         const uint32_t k_tile = smem_u32(sm + L::K), v_tile = smem_u32(sm + L::V), q_tile = smem_u32(sm + L::Q);
         bool issued = false;
-        // What was left out of the unit before, after a barrier behind its outputs.  (Thread 0 has waited for all its values, so what
-        // the other warps noted of them is here.  They note nothing of unit u + 4 before this unit's first weights are done.)
-        auto add_left_out = [&]() {
-            const TcLeftOut& x = s_odd[(units - 1) & 3];
-            if (units > 0 && x.unit == units - 1)
-                add_not_finite<PREC>(a, x.b, x.hk, x.tokens, x.r0, x.rows, x.from, x.to,
-                                     x.slot < 0 ? nullptr : slot_of(a, blockIdx.x, x.slot, kTcRows), tid, 128);
-        };
         for (; at < s.hi;) {
             const TcSegment sg = tc_segment_at(a, u, s, at, b, base);
             at = sg.next;
@@ -283,7 +275,6 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
             }
             fence_proxy_async_smem();
             softmax_sync();
-            add_left_out();
             for (int t = sg.t0; t < sg.t1; ++t, ++g) {
                 if (tid == 0 && ok && mbar_wait_spin(k_full + (g & 1), g >> 1 & 1, &s_error, 1)) {
                     tc_fence_after();
@@ -489,13 +480,33 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
                 part[kTcRows * D + kTcRows + tid] = ok ? l : nan;
             }
         }
-        softmax_sync();
-        add_left_out();
         if (tid == 0 && issued) {   // every MMA has completed before TMEM is freed
             umma_commit(drained);
             mbar_wait_spin(drained, 0, &s_late, 6);   // (also after an error elsewhere, so not with s_error)
         }
         __syncwarp();
+        // What was left out, unit by unit.  (Thread 0 has waited for all values, so what the other warps noted of them is here, and so
+        // are the outputs, behind this barrier.  In the loop above the call would cost it 2 %, for the registers it takes.)
+        softmax_sync();
+        uint32_t any = 0;
+        for (int i = 0; i < kTcOddWords; ++i) any |= s_odd[i];
+        if (any) {
+            at = s.lo;
+            b = s.b;
+            base = s.base;
+            units = 0;
+            while (at < s.hi) {
+                const TcSegment sg = tc_segment_at(a, u, s, at, b, base);
+                at = sg.next;
+                if (sg.t0 >= sg.t1) continue;
+                if (s_odd[units / 32 % kTcOddWords] >> (units % 32) & 1) {
+                    const int first = sg.t0 * TILE;
+                    add_not_finite<PREC>(a, sg.b, sg.hk, sg.tokens, sg.r0, sg.rows, PREC == 3 ? first : max(first, odd_from(sg)),
+                                         min(sg.tokens, sg.t1 * TILE), sg.whole ? nullptr : slot_of(a, blockIdx.x, sg.slot, kTcRows), tid, 128);
+                }
+                ++units;
+            }
+        }
     } else {
         // ------------------------------------------------------------------------- pages and queries
         const int pw = warp - 4;
@@ -606,23 +617,28 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
                 }
             }
         };
-        // Zeros for what is not finite in the chunks of a tile that this lane copied; whether there was any.
-        auto clean = [&](uint8_t* tile) -> bool {
+        auto note = [&]() { atomicOr(&s_odd[units / 32 % kTcOddWords], 1u << (units % 32)); };
+        // Whether one of a tile's fp16 values is not finite: looked at while the tile before is still multiplied.  (A prompt of 4096 tokens
+        // 296 -> 302 us; on their way to the tile, or in shared memory behind it, 302 to 305.)
+        auto any_odd = [&](const void* pages, int row) -> bool {
+            uint32_t out = 0;
             if constexpr (PREC == 1) {
-                uint32_t odd = 0;
-                const int at = my_chunk / 8 * 128 * 128;
 #pragma unroll 8
-                for (int i = 0; i < N; ++i)
-                    odd |= odd_halves(*reinterpret_cast<const uint4*>(tile + at + sw128_offset(pw * ROWS + i * STEP + my_row, my_chunk % 8)));
-                if (odd == 0) return false;
-#pragma unroll 1
                 for (int i = 0; i < N; ++i) {
-                    uint4* x = reinterpret_cast<uint4*>(tile + at + sw128_offset(pw * ROWS + i * STEP + my_row, my_chunk % 8));
-                    *x = finite_halves(*x);
+                    const int x = __shfl_sync(0xffffffffu, row, i * STEP + my_row);
+                    if (x >= 0 && have_chunk) out |= odd_halves(__ldg(reinterpret_cast<const uint4*>(static_cast<const char*>(pages) + (int64_t)x * row_bytes + my_chunk * 16)));
                 }
-                return true;
             }
-            return false;
+            return __any_sync(0xffffffffu, out != 0);
+        };
+        // Zeros for them, in the chunks that this lane copied.
+        auto clean = [&](uint8_t* tile) {
+#pragma unroll 1
+            for (int i = 0; i < N; ++i) {
+                uint4* x = reinterpret_cast<uint4*>(tile + my_chunk / 8 * 128 * 128 + sw128_offset(pw * ROWS + i * STEP + my_row, my_chunk % 8));
+                *x = finite_halves(*x);
+            }
+            note();
         };
         auto publish = [&](uint64_t* full) {
             fence_proxy_async_smem();
@@ -644,17 +660,7 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
                 gap = row < 0;
                 return row < 0 ? -1 : (int)row + sg.hk * P;
             };
-            // the first token of the tiles that not all rows see (or an earlier one where the unit's rows are of several heads)
-            const int new_before = u.blocks ? sg.rt % u.blocks * kTcRows : 0;
-            const int odd_from = not_all_from(a.causal ? max(1, sg.tokens - (a.new_lengths ? __ldg(a.new_lengths + sg.b) : a.S_q) + 1 + new_before)
-                                                       : sg.tokens, sg.tokens, TILE);
-            if (tid == 128) {
-                TcLeftOut& x = s_odd[units & 3];
-                const int first = sg.t0 * TILE;
-                x.b = sg.b; x.hk = sg.hk; x.tokens = sg.tokens; x.r0 = sg.r0; x.rows = sg.rows; x.slot = sg.whole ? -1 : sg.slot;
-                x.from = PREC == 3 ? first : max(first, odd_from);
-                x.to = min(sg.tokens, sg.t1 * TILE);
-            }
+            const int odd = odd_from(sg);
             int row = row_of(sg.t0);
             load(k_next, a.pool.k, a.pool.scale_k, row);
             load(v_next, a.pool.v, a.pool.scale_v, row);
@@ -673,26 +679,26 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
                 write(k_next, sm + L::K);
                 copy(sm + L::K, a.pool.k, row);
                 if constexpr (PREC == 2) {   // V's scale as a power of two in the exponent and a factor in [1, 2)
-                    const bool odd = t * TILE >= odd_from && !finite(sv);
-                    if (odd) {
+                    const bool out = t * TILE >= odd && !finite(sv);
+                    if (out) {
                         sv = 1.0f;
-                        s_odd[units & 3].unit = units;
+                        note();
                     }
                     const int e = min(max((int)((__float_as_uint(sv) & 0x7fffffffu) >> 23), 35), 219);
                     const float down = __uint_as_float((uint32_t)(254 - e) << 23);
                     tk[0] = sk;
                     tk[128] = row >= 0 ? (float)(e - 127) : -INFINITY;
-                    tk[256] = odd ? 0.0f : sv * down;
+                    tk[256] = out ? 0.0f : sv * down;
                     tk[384] = down;
                 } else if constexpr (PREC == 3) {   // of the rows that this lane took, by the first lane of each
-                    bool odd = false;
+                    bool out = false;
 #pragma unroll
-                    for (int i = 0; i < 2 * N; ++i) odd |= !finite(v_next.scale[i / 2][i % 2]);
-                    if (odd) {   // a group that is not finite says nothing of the others' size
+                    for (int i = 0; i < 2 * N; ++i) out |= !finite(v_next.scale[i / 2][i % 2]);
+                    if (out) {   // a group that is not finite says nothing of the others' size
 #pragma unroll
                         for (int i = 0; i < 2 * N; ++i)
                             if (!finite(v_next.scale[i / 2][i % 2])) v_next.scale[i / 2][i % 2] = 0.0f;
-                        s_odd[units & 3].unit = units;
+                        note();
                     }
                     __syncwarp();
 #pragma unroll
@@ -713,12 +719,15 @@ __global__ void __launch_bounds__(kTcThreads, TcLayout<DP>::CTAS) pool_attention
                 if constexpr (PREC == 1) asm volatile("cp.async.wait_all;" ::: "memory");
                 publish(k_full + (g & 1));
                 load(k_next, a.pool.k, a.pool.scale_k, next);
+                const bool dirty = PREC == 1 && t * TILE >= odd && any_odd(a.pool.v, row);
                 if (g > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait_spin(v_free, (g - 1) & 1, &s_error, 8));
                 if (!ok) break;
                 write(v_next, sm + L::V);
                 copy(sm + L::V, a.pool.v, row);
-                if constexpr (PREC == 1) asm volatile("cp.async.wait_all;" ::: "memory");
-                if (t * TILE >= odd_from && clean(sm + L::V)) s_odd[units & 3].unit = units;
+                if constexpr (PREC == 1) {
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    if (dirty) clean(sm + L::V);
+                }
                 publish(v_full);
                 load(v_next, a.pool.v, a.pool.scale_v, next);
                 row = next;
