@@ -7,9 +7,9 @@
 // A NaN makes its scale NaN, so that its row or group is read as NaN (paged.cu's leaves it out of the scale).
 // A token without a page, or whose position the rotary tables do not hold, leaves its rows as they were.
 // Everything is read once and written once.  A token a sequence is bound by its latency: 8 sequences, 32 + 8 + 8 heads of 128
-// values, 3.0 us.  A prompt is bound by what it computes: 8 x 2048 fp16 tokens of 32 + 32 heads into int8 take 112 us, about 320
-// instructions for 4 rows of a warp (77 M in all, three quarters of the issue slots) at 3.3 TB/s.  Reading them back as fp32
-// writes 4 bytes for one read: 107 us, 6.1 TB/s.
+// values, 3.0 us.  A prompt is bound by what it computes: 8 x 2048 fp16 tokens of 32 + 32 heads into int8 take 107 us, about 320
+// instructions for 4 rows of a warp (77 M in all, three quarters of the issue slots) at 3.4 TB/s.  The rows of padding are read
+// too (13398 of the 16384 are tokens).  Reading them back as fp32 writes 4 bytes for one read: 105 us, 6.2 TB/s.
 #include "pool.cuh"
 
 namespace skv {
@@ -170,7 +170,8 @@ __device__ __forceinline__ float scale_of(float m, float top, float r) {
 // FLY * rows heads of q, of k or of v (blockIdx.y: first the slices of q, then of k, then of v), every row asked for before the
 // token's position and page are known.  Every thread stays to the end: rows and int4 groups reduce over aligned lane blocks.
 // (The prompt above with a warp a row: 845 us for append and read; blocks of one kind of rows and quotients without
-// divisions: append 163 -> 130; three blocks an SM, which hide what four rows on the way a thread do not: 112.)
+// divisions: append 163 -> 130; three blocks an SM, which hide what four rows on the way a thread do not: 112; NaN kept in the maxima, so
+// no second pass: 107.)
 template <class T, bool SPLIT>
 __global__ void __launch_bounds__(256, 3) pool_append_kernel(const __grid_constant__ skv_pool_append_args a, int q_slices, int kv_slices) {
     constexpr int FLY = sizeof(T) == 2 ? 4 : 2;

@@ -21,7 +21,7 @@ namespace skv {
 
 // --------------------------------------------------------------------------- any size and alignment
 // Products on the FMA pipe from fp32 tiles in shared memory: 8 rows, 32 tokens at a time (16384 tokens of 8 fp32 key heads of 128
-// values in 97 us, bound by the tiles' latency at 1.4 TB/s).  Thread = (token, rows w and
+// values in 102 us, bound by the tiles' latency at 1.3 TB/s).  Thread = (token, rows w and
 // w + 4) for the scores, value d for the sums.  A warp widens 8 tokens a tile, a lane a value of each, so that 16 loads are on
 // their way; the lanes look up the tokens' rows one tile ahead.
 constexpr int kAnyRows = 8, kAnyTile = 32, kAnyThreads = 128, kAnyMaxD = 512, kAnyParts = 64, kAnyPad = 1;
@@ -224,11 +224,18 @@ int attend_fp16(const skv_pool_attention_args& a, cudaStream_t st);
 int attend_int8(const skv_pool_attention_args& a, cudaStream_t st);
 int attend_int4(const skv_pool_attention_args& a, cudaStream_t st);
 
-// The tcgen05 kernel (pool_attention_tc.cuh), and the query rows a key head from which it is taken.  8 key heads of 4 query heads
-// and 128 values, us there / on the small kernel: 32 rows over 4 x 4096 fp16 tokens 32.5 / 34.7, int8 37.9 / 34.1; 48 rows 35.0 /
-// 40.8, int8 38.4 / 41.9; 64 rows 34.3 / 47.3, int8 39.8 / 49.1; 128 rows over 512 tokens 20.2 / 17.5, over 16384 45.6 / 73.1.
-// Heads of 256 values (2 query heads), which leave an SM one CTA: 48 rows over 4096 fp16 tokens 37.4 / 38.1, int8 40.8 / 31.8; 64
-// rows over 4 x 4096 65 / 96, int8 79 / 81; a prompt of 2048 145 / 603, int8 159 / 525.
+// The tcgen05 kernel (pool_attention_tc.cuh), and the query rows a key head from which it is taken.  The lengths are on the device,
+// so the rule cannot look at them; it is set by long sequences, and short ones lose a few us by it.  8 key heads of 128
+// values, causal, us there / on the small kernel, for fp16, int8 and int4 pages:
+//     32 rows over 4 x 4096 tokens   36.3 / 37.6   41.0 / 36.5   46.2 / 40.5      (fp16 queries 38.1 / 38.3   43.5 / 37.5   48.2 / 41.6)
+//     48 rows                        37.1 / 41.6   41.6 / 44.6   47.3 / 50.6                   (39.6 / 45.0   44.3 / 46.4   49.4 / 53.4)
+//     64 rows                        38.5 / 49.7   42.7 / 52.4   49.6 / 63.0                   (38.4 / 53.3   45.4 / 55.4   50.8 / 66.9)
+//     48 rows over 512 tokens        18.0 / 16.8   21.0 / 17.4   20.0 / 18.8                   (19.0 / 17.3   21.9 / 18.2   20.3 / 19.2)
+//     128 rows over 512 tokens       21.1 / 18.0   23.2 / 20.4   22.1 / 21.5                   (21.6 / 18.5   24.1 / 20.8   22.6 / 22.0)
+// Heads of 256 values (2 query heads), which leave an SM one CTA:
+//     48 rows over 4 x 4096 tokens   70.1 / 83.1   84.2 / 64.6   110 / 89                      (74.1 / 91.0   84.4 / 71.4   111 / 96)
+//     64 rows                        73.4 / 99.5   86.0 / 78.8   111 / 112                     (77.1 / 109    87.0 / 88.1   110 / 122)
+//     128 rows                       88.8 / 174    98.2 / 133    124 / 198                     (92.4 / 197    100 / 149     125 / 216)
 constexpr int many_rows(int D) { return D <= 128 ? 48 : 64; }
 int attend_many(const skv_pool_attention_args& a, cudaStream_t st);
 

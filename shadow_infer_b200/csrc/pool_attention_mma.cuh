@@ -13,10 +13,10 @@
 // free as long as both operands agree: the queries are laid out, once a segment, in the order the words come in.  P^T's
 // operand is S^T's result transposed by movmatrix.  fp32 pages run as m16n8k8 of tf32 terms instead.
 //
-// What bounds it (8 key heads of 4 query heads, 128 values).  fp16: the pages' bytes, 64 sequences of up to 8192 tokens in 162 us
+// What bounds it (8 key heads of 4 query heads, 128 values).  fp16: the pages' bytes, 64 sequences of up to 8192 tokens in 163 us
 // = the copy rate.  int8 and int4: the instructions that make operands of the bytes, about 540 and 725 a warp for a tile of 16
-// tokens: 131071 int8 tokens with fp32 queries in 76 us (57 % of the copy rate), 32768 int4 tokens of 32 heads in 81 us (38 %).
-// fp32: 16 KB a tile leave room for 4 warps an SM, 16384 tokens in 35 us (59 %).  Small calls: 4 to 5 us until the first rows
+// tokens: 131071 int8 tokens with fp32 queries in 76 us (57 % of the copy rate), 32768 int4 tokens of 32 heads in 82 us (38 %).
+// fp32: 16 KB a tile leave room for 4 warps an SM, 16384 tokens in 36 us (57 %).  Small calls: 4 to 5 us until the first rows
 // are there, 1.7 us a unit and 3 to 6 us for a join; 512 tokens of 32 heads in 12 us, 8 int8 sequences of up to 2048 tokens in 18.
 //
 // Exactness.  Page values enter the MMAs exactly: fp16 as it is, int8 and int4 as small integers, fp32 as two terms of 11 bits
@@ -27,7 +27,7 @@
 // parts of 7 bits, an MMA each, that times a 4-bit integer are exact in fp16 (V), after a power of two a token is taken out
 // into its weight.  Queries are scaled by a power of two a row; 16-bit ones fit one fp16 operand, fp32 ones take two
 // (22 bits).  Weights are 2^(z - ref) <= 2^15 with z the score plus the exponent of V's scale; one operand for bf16
-// outputs, whose own rounding is 8 times coarser, else two.  Against 64 bits fp32 outputs are 2e-7 to 5e-7 off.
+// outputs, whose own rounding is 8 times coarser (two cost calls of one token up to 5 %, prompts 4 to 15), else two.  Against 64 bits fp32 outputs are 2e-7 to 5e-7 off.
 //
 // ref follows the running maximum lazily (sums are rescaled only when a weight would pass 2^15), so most tiles need one
 // vote and no shuffles; row sums stay in the lanes until the segment ends.

@@ -17,9 +17,9 @@
 // of more than 128 values leave room for one.
 //
 // What bounds it: instructions and the chain S -> softmax -> P V of two CTAs; a tile of int8 pages takes 10 thousand warp
-// instructions (41 % of the issue slots; tensor pipe 20 %, exponentials 21 % busy).  8 key heads of 4 query heads of 128 values: a prompt of 4096 fp16 tokens in 300 us (460 TFLOP/s of the
-// causal half's operations, 0.27 of cuBLAS's burst), int8 384 us, int4 535 us; 128 new tokens behind 16384 in 82, 99 and 135 us
-// (bf16; fp16 queries 5 to 15 % more).
+// instructions (41 % of the issue slots; tensor pipe 20 %, exponentials 21 % busy).  8 key heads of 4 query heads of 128 values: a prompt of 4096 fp16 tokens in 303 us (453 TFLOP/s of the
+// causal half's operations, 0.27 of cuBLAS's burst), int8 383 us, int4 541 us; 128 new tokens behind 16384 in 84, 101 and 135 us
+// (bf16; fp16 queries 5 to 11 % more).
 // Measured and dropped: a warp of its own for the MMAs (96 registers a thread: spills, twice the time), weights of all
 // 128 columns in registers until the maximum is known (spills), the next 32 scores fetched ahead (spills, 15 % slower).
 //
