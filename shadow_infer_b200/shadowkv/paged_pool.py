@@ -279,7 +279,7 @@ def paged_attention(
     exponent of its token's V scale) is one fp16 operand of 11 bits for bf16 results and two (22 bits) else, and below 2^-36 of
     its query's largest it is rounded to that step; an int4 scale of V has 14 bits for 16-bit results of a few queries, 18 for
     many, 21 for fp32 ones; for 16-bit results the sums over a sequence's tiles are cut off, not rounded, at 2^-24 a step.  Queries of
-    2^97 and more in magnitude leave that range (NaN).  What is
+    2^98 and more in magnitude leave that range (NaN).  What is
     not finite reaches the queries that see it and no others: a key all of their values, a value its own ones.  Every page is read once for all the query rows that share its key
     head.  The sequences are split over the whole GPU by their lengths on the device, long ones into
     parts that are joined in token order, so equal calls give equal bits.
