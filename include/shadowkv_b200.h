@@ -492,6 +492,115 @@ size_t skv_pool_attention_scratch_bytes(int D);
 size_t skv_pool_attention_scratch_zeros(void);
 int skv_pool_attention(const skv_pool_attention_args* args, void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Attention over the pages that matter: bounds of each page's keys, the pages that they rank
+ * highest for a query, and the attention of these.  No counterpart in the reference.
+ *
+ * Bounds int8 [num_pages, heads, 2, D] (lows, then highs) and steps float [num_pages, heads]: a
+ * page's key values k_d (as they are read: q * scale in fp32) of the rows that are tokens satisfy
+ * lows_d * step <= k_d <= highs_d * step.  step is the least power of two (2^-126 and up) of which 127
+ * reach max |k|, 1 where all are zero, and +inf (lows and highs 0) where a value is not finite.
+ * ------------------------------------------------------------------------------------- */
+typedef struct skv_pool_bounds_args {
+    skv_pool pool;               /* v and scale_v are not read and may be NULL */
+    const int32_t* start;        /* NULL: 0 */
+    const int32_t* lengths;
+    int8_t* bounds;
+    float* steps;
+    int32_t* error_flag;
+} skv_pool_bounds_args;          /* 120 bytes */
+
+/* Writes the bounds of the pages that hold tokens start[b] .. lengths[b] - 1, each from all of its tokens. */
+int skv_pool_bounds(const skv_pool_bounds_args* args, void* stream);
+
+typedef struct skv_pool_select_args {
+    skv_rows q;                  /* [B, H_q, S_q, D], H_q a multiple of heads */
+    const int8_t* bounds;
+    const float* steps;
+    const int32_t* block_table;  /* [batch, table_width] */
+    const int32_t* lengths;      /* tokens of each sequence, the new ones included */
+    const int32_t* new_lengths;  /* queries of each sequence that are tokens; NULL: all S_q */
+    int32_t* pages;              /* out [batch, heads, S_q, keep] */
+    void* scratch;
+    int32_t* error_flag;
+    int64_t table_stride;
+    int64_t scratch_bytes;
+    int32_t table_width, num_pages, page_size, heads, head_dim, batch;
+    int32_t S_q, keep, first, recent, causal, reserved;
+} skv_pool_select_args;          /* 168 bytes */
+
+/* The `keep` pages (numbers within the sequence, ascending, then -1) of each query and key head: all that the query
+ * sees, where they are no more than keep; else the first `first`, the last `recent` (first + recent <=
+ * keep, recent >= 1), and those of the largest score, ties to the lowest page.  score = the largest, over the
+ * query heads that share the key head, of t * step * sum_d n_d (n_d > 0 ? highs_d : lows_d) with n = rint(q / t) and
+ * t the least power of two of which 127 reach max |q| (a query row that is not finite scores 0).  The sum is exact.  A page
+ * whose step is not finite comes before all others, one that the table does not name behind.
+ * scratch: skv_pool_select_scratch_bytes bytes, 16-byte aligned. */
+size_t skv_pool_select_scratch_bytes(int batch, int heads, int S_q, int table_width);
+int skv_pool_select(const skv_pool_select_args* args, void* stream);
+
+typedef struct skv_pool_sparse_args {
+    skv_pool_attention_args attention;
+    const int32_t* pages;        /* [batch, heads, S_q, keep] by its strides, the last dimension contiguous */
+    int64_t pages_stride_b, pages_stride_h, pages_stride_s;
+    void* tables;                /* scratch: batch * S_q * heads * (keep + 1) int32 */
+    int64_t tables_bytes;
+    int32_t keep, reserved;
+} skv_pool_sparse_args;          /* 272 bytes */
+
+/* skv_pool_attention of the tokens that lie in the listed pages: an entry counts if it is one of the pages the
+ * query sees and larger than every entry before it.  The rows of (sequence, new token, key head) in this order must be
+ * evenly spaced in q and out, as they are in a tensor laid out [B, S_q, H_q, D].
+ * At most 2^24 such units, and num_pages * heads within 31 bits (SKV_ERR_TOO_LARGE). */
+int skv_pool_sparse_attention(const skv_pool_sparse_args* args, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Beam search over the page pool: the best continuations, and sequences that go on from others.
+ * No counterpart in the reference.
+ * ------------------------------------------------------------------------------------- */
+typedef struct skv_beam_args {
+    const void* logits;          /* [B, beams, V], V contiguous */
+    int64_t stride_b, stride_r;  /* in values */
+    const float* scores;         /* [B, beams] */
+    const uint8_t* finished;     /* [B, beams]; NULL: none */
+    float* values;               /* out [B, keep] */
+    int64_t* parents;            /* out [B, keep] */
+    int64_t* tokens;             /* out [B, keep] */
+    void* scratch;
+    int64_t scratch_bytes;
+    int32_t dtype;               /* as skv_rows.dtype */
+    int32_t B, beams, V, keep, pad_token;
+} skv_beam_args;                 /* 104 bytes */
+
+/* The keep <= 128 best of the beams * V continuations of each of B searches, best first, ties to the lowest beam, then
+ * token: scores[b, r] + log softmax(logits[b, r])[token], compared in 64 bits.  A finished beam
+ * has one continuation, pad_token, at its score.  A NaN logit counts as -inf; logits of +inf share their beam's whole
+ * probability.  A beam whose score is -inf, NaN or +inf, or whose logits are all -inf, has continuations of -inf only.
+ * keep <= beams * V; beams <= 4096.  scratch: skv_beam_scratch_bytes bytes, 16-byte aligned. */
+size_t skv_beam_scratch_bytes(int B, int beams, int V, int keep);
+int skv_beam_select(const skv_beam_args* args, void* stream);
+
+typedef struct skv_pool_reorder_args {
+    skv_pool pool;               /* batch = groups * beams */
+    const int32_t* lengths;      /* [batch] */
+    const void* parents;         /* [groups, beams], numbers within the group, int32 or int64 */
+    int32_t* new_table;          /* out [batch, table_width] */
+    int32_t* new_lengths;        /* out [batch] */
+    int8_t* bounds;              /* as in skv_pool_bounds_args; NULL: none */
+    float* steps;
+    int32_t* error_flag;
+    int32_t parents_bytes;       /* 4 or 8 */
+    int32_t beams;
+} skv_pool_reorder_args;         /* 144 bytes */
+
+/* Beam c of a group goes on from beam parents[c]: the pages and the length of its table row are its parent's.  Full pages are shared.  A
+ * last page that is partly filled must be its sequence's own: it goes to the parent itself, if it goes on from itself, else to the
+ * first child; the n-th of the other children takes the page that the n-th beam without children has in
+ * that place of its table, and the tokens (and bounds) are copied there.  The beams of a group are equally long (else that
+ * place may be empty: its table entry is -1 then and error_flag set, as by a parent outside the group, whose child is empty).
+ * Table entries behind the tokens (pages taken ahead) stay where they are.  beams <= 1024. */
+int skv_pool_reorder(const skv_pool_reorder_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

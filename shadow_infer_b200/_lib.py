@@ -135,6 +135,13 @@ _SIGNATURES = {
     "skv_pool_attention_scratch_bytes": (c_size_t, [c_int]),
     "skv_pool_attention_scratch_zeros": (c_size_t, []),
     "skv_pool_attention": (c_int, [ctypes.c_char_p, c_void_p]),
+    "skv_pool_bounds": (c_int, [ctypes.c_char_p, c_void_p]),
+    "skv_pool_select_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "skv_pool_select": (c_int, [ctypes.c_char_p, c_void_p]),
+    "skv_pool_sparse_attention": (c_int, [ctypes.c_char_p, c_void_p]),
+    "skv_beam_scratch_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "skv_beam_select": (c_int, [ctypes.c_char_p, c_void_p]),
+    "skv_pool_reorder": (c_int, [ctypes.c_char_p, c_void_p]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES.keys())

@@ -8,9 +8,11 @@ from .kv_cache_manager import (
     LeastImportantEvictionPolicy,
     TokenHeadScore,
 )
+from .beam import beam_select, paged_reorder
 from .importance_model import compute_irap_importance
 from .packed_attention import packed_attention, packed_block_forward
 from .packed_kv_cache import PackedKVCache
+from .page_selection import page_bounds, page_select
 from .paged_kv_store import PagedKVStore
 from .paged_pool import PagedKVPool, paged_append, paged_attention, paged_block_forward, paged_read
 from .precision_plan import (
@@ -31,5 +33,5 @@ __all__ = [
     "predict_codes_bytes", "packed_attention", "packed_block_forward", "KVCacheManager", "KVCacheEntry", "TokenHeadScore",
     "EvictionPolicy", "LeastImportantEvictionPolicy", "ImportanceAgeEvictionPolicy", "PagedKVStore",
     "compute_irap_importance", "apply_rotary", "rotary_tables", "PagedKVPool", "paged_append", "paged_read",
-    "paged_attention", "paged_block_forward",
+    "paged_attention", "paged_block_forward", "page_bounds", "page_select", "beam_select", "paged_reorder",
 ]

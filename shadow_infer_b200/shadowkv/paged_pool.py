@@ -41,7 +41,8 @@ _POOL, _ROWS, _ROPE = "QQQQQqiiiiiiii", "Qqqqii", "QQQqqiiiiii"
 _APPEND = struct.Struct("<" + _POOL + _ROWS * 4 + _ROPE + "QQQii")
 _READ = struct.Struct("<" + _POOL + _ROWS * 2 + "QQQii")
 _ATTENTION = struct.Struct("<" + _POOL + _ROWS * 2 + "QQQqQiifi")
-assert (_APPEND.size, _READ.size, _ATTENTION.size) == (336, 192, 216)
+_SPARSE = struct.Struct("<" + _POOL + _ROWS * 2 + "QQQqQiifi" + "QqqqQqii")
+assert (_APPEND.size, _READ.size, _ATTENTION.size, _SPARSE.size) == (336, 192, 216, 272)
 _NO_ROPE = (0,) * 11
 _SCRATCH = {}         # (device, stream) -> attention scratch
 _SCRATCH_BYTES = {}   # (device, head_dim) -> its size
@@ -249,6 +250,33 @@ def paged_read(
     return k, v
 
 
+def _listed_pages(pages: torch.Tensor, shape: Tuple[int, int, int], dev: torch.device) -> torch.Tensor:
+    """``pages`` as int32 ``[*shape, keep]`` on ``dev`` whose last dimension is contiguous."""
+    if pages.dim() != 4 or pages.shape[3] < 1:
+        raise ValueError(f"pages must be [batch, heads, seq, keep], got {tuple(pages.shape)}")
+    if pages.shape[:3] != shape:
+        try:
+            pages = pages.expand(*shape, -1)
+        except RuntimeError:
+            raise ValueError(f"pages must broadcast to {[*shape, 'keep']}, got {tuple(pages.shape)}") from None
+    return _index(pages, pages.shape, dev, "pages")
+
+
+def _evenly_spaced(q: torch.Tensor, heads: int) -> bool:
+    """Whether the rows of (sequence, new token, key head), in this order, are evenly spaced in ``q``."""
+    (B, Hq, S, D), (sb, sh, ss, sd) = q.shape, q.stride()
+    if sd != 1 and D != 1:
+        return False
+    units, step = 1, 0
+    for n, s in ((heads, Hq // heads * sh), (S, ss), (B, sb)):
+        if n > 1:
+            if units > 1 and s != units * step:
+                return False
+            step = s if units == 1 else step
+            units *= n
+    return True
+
+
 def paged_attention(
     q: torch.Tensor,
     k_pages: torch.Tensor,
@@ -261,6 +289,7 @@ def paged_attention(
     causal: bool = False,
     new_lengths: Optional[torch.Tensor] = None,
     check: bool = False,
+    pages: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """Attention of each sequence's newest tokens over its pages; returns ``[B, H_q, S_q, D]`` in ``q``'s type.
 
@@ -272,8 +301,14 @@ def paged_attention(
     ``new_lengths[b]``).  A query that sees nothing (padding, an empty sequence) gives zeros.
     ``scale`` defaults to ``1/sqrt(D)``.
 
+    ``pages`` (int32 or int64, broadcast to ``[B, heads, S_q, keep]``; ``page_select`` finds them) leaves each query, of those
+    tokens, the ones in the listed pages, which are all that is read: an entry counts if it is one of the pages
+    that the query sees and larger than every entry before it, so lists are ascending and anything else in them, -1 among it, stands
+    for no page.  One launch more.
+
     The result has ``q``'s dimension order in memory (as torch's own operators keep it), so that the output of a
-    ``[B, S, H, D]`` projection goes back to one without a copy.
+    ``[B, S, H, D]`` projection goes back to one without a copy.  (With ``pages``, several new tokens of another order are
+    copied to that one, and the result has it.)
 
     Scores, softmax and sums are fp32.  What the tensor cores multiply is rounded less than the result is: a weight (times the
     exponent of its token's V scale) is one fp16 operand of 11 bits for bf16 results and two (22 bits) else, and below 2^-36 of
@@ -293,16 +328,27 @@ def paged_attention(
         raise ValueError(f"{Hq} query heads do not share {pool[9]} key heads evenly")
     lens = _index(lengths, (B,), dev, "lengths")
     new = None if new_lengths is None else _index(new_lengths, (B,), dev, "new_lengths")
+    if pages is not None:
+        listed = _listed_pages(pages, (B, pool[9], S_q), dev)
+        tables = torch.empty(B * S_q * pool[9] * (listed.shape[3] + 1), dtype=torch.int32, device=dev)
     qd, q_rows = _rows(q, dev)
+    if pages is not None and not _evenly_spaced(qd, pool[9]):
+        qd, q_rows = _rows(qd.transpose(1, 2).contiguous().transpose(1, 2), dev)
     out, out_rows = _like(qd)
+    if pages is not None and not _evenly_spaced(out, pool[9]):
+        out, out_rows = _like(torch.empty((B, S_q, Hq, D), dtype=qd.dtype, device=dev).transpose(1, 2))
     flag = _flag(check, dev)
-    entry = _lib.load().skv_pool_attention
+    lib = _lib.load()
     with device_ctx(dev):
         stream = _lib.stream_of(dev)
         scratch = _scratch(dev, stream, D)
-        st = entry(_ATTENTION.pack(*pool, *q_rows, *out_rows, lens.data_ptr(), 0 if new is None else new.data_ptr(),
-                                   scratch.data_ptr(), scratch.numel(), 0 if flag is None else flag.data_ptr(), S_q, bool(causal),
-                                   1.0 / math.sqrt(D) if scale is None else scale, 0), stream)
+        fields = (*pool, *q_rows, *out_rows, lens.data_ptr(), 0 if new is None else new.data_ptr(), scratch.data_ptr(), scratch.numel(),
+                  0 if flag is None else flag.data_ptr(), S_q, bool(causal), 1.0 / math.sqrt(D) if scale is None else scale, 0)
+        if pages is None:
+            st = lib.skv_pool_attention(_ATTENTION.pack(*fields), stream)
+        else:
+            st = lib.skv_pool_sparse_attention(_SPARSE.pack(*fields, listed.data_ptr(), *listed.stride()[:3], tables.data_ptr(),
+                                                            tables.numel() * 4, listed.shape[3], 0), stream)
     if st:
         _lib.check(st, "paged_attention")
     del table, qd
@@ -311,12 +357,24 @@ def paged_attention(
     return _back(out, q, dev)
 
 
+class _Family:
+    """Sequences that may share pages, and the pages taken for those of them that have ended."""
+
+    def __init__(self, b: int) -> None:
+        self.rows = {b}
+        self.pages: List[int] = []
+
+
 class PagedKVPool:
     """The pages of one layer for ``batch_size`` sequences of different lengths, and their bookkeeping.
 
     ``append`` takes pages from the free list, writes the new tokens and advances the lengths; ``attention`` and
     ``read`` use what is held; ``release`` ends a sequence and returns its pages.  ``block_table`` and ``lengths``
     are device tensors (for graphs and for the functions above); ``token_counts`` are the lengths on the host.
+
+    ``fork`` lets empty sequences go on from a sequence, and ``reorder`` lets the beams of a search go on from one another; sequences that
+    share pages in these ways return them when the last of them is released.  With ``bounds``, ``append`` keeps the
+    pages' bounds (``page_bounds``) and ``attention`` can be told to read the pages that they rank highest only.
     """
 
     def __init__(
@@ -330,6 +388,7 @@ class PagedKVPool:
         precision: str = "fp16",
         int4_group_size: int = 16,
         device: Any = "cuda",
+        bounds: bool = False,
     ) -> None:
         if min(num_pages, batch_size, num_heads, head_dim, max_tokens, page_size) < 1:
             raise ValueError("PagedKVPool sizes must be >= 1")
@@ -351,11 +410,17 @@ class PagedKVPool:
         tail = {"int8": (1,), "int4": (head_dim // group, 1)}.get(precision)
         self.k_pages, self.v_pages = (torch.zeros(*shape, row, dtype=dtype, device=dev) for _ in range(2))
         self.scale_k, self.scale_v = (None if tail is None else torch.ones(*shape, *tail, device=dev) for _ in range(2))
+        self.bounds = self.steps = None
+        if bounds:
+            self.bounds = torch.zeros(num_pages, num_heads, 2, head_dim, dtype=torch.int8, device=dev)
+            self.steps = torch.ones(num_pages, num_heads, device=dev)
+        # the pages taken for each sequence; which of them it holds is known to the device alone once beams were reordered
         self._table = torch.full((batch_size, -(-max_tokens // page_size)), -1, dtype=torch.int32)
         self.block_table = self._table.to(dev)
         self.lengths = torch.zeros(batch_size, dtype=torch.int32, device=dev)
         self.token_counts: List[int] = [0] * batch_size
         self._free = list(range(num_pages - 1, -1, -1))
+        self._family = [_Family(b) for b in range(batch_size)]
 
     @property
     def free_pages(self) -> int:
@@ -388,42 +453,62 @@ class PagedKVPool:
         P = self.page_size
         grown = [-(-(c + n) // P) for c, n in zip(self.token_counts, new)]
         wanted = [g - self._pages_held(b) for b, g in enumerate(grown)]
-        if max(grown) > self._table.shape[1]:
+        if max(grown) > self.block_table.shape[1]:
             raise RuntimeError(f"a sequence of {max(c + n for c, n in zip(self.token_counts, new))} tokens does not fit "
-                               f"the table of {self._table.shape[1]} pages of {P}")
+                               f"the table of {self.block_table.shape[1]} pages of {P}")
         if sum(wanted) > len(self._free):
             raise RuntimeError(f"{sum(wanted)} pages wanted, {len(self._free)} free")
         last = max((c + n for c, n in zip(self.token_counts, new) if n), default=0)
         if cos is not None and positions is None and last > cos.shape[0]:
             raise ValueError(f"position {last - 1} lies outside rotary tables of {cos.shape[0]} positions")
-        table = self._table
-        if sum(wanted):
-            table = table.clone()
-            taken = self._free[len(self._free) - sum(wanted):][::-1]
-            at = 0
-            for b, n in enumerate(wanted):
-                if n:
-                    table[b, grown[b] - n:grown[b]] = torch.tensor(taken[at:at + n], dtype=torch.int32)
-                    at += n
-            block_table = _staged(table, self.lengths.device)
-        else:
-            block_table = self.block_table
+        block_table = self.block_table
+        taken = self._free[len(self._free) - sum(wanted):][::-1]
+        places = [(b, g - n + i) for b, (g, n) in enumerate(zip(grown, wanted)) for i in range(n)]
+        if taken:
+            block_table = self._with_pages(places, taken)
         fresh = None if new_lengths is None else _staged(torch.tensor(new, dtype=torch.int32), self.lengths.device)
         out = paged_append(k, v, self.k_pages, self.v_pages, block_table, self.lengths, self.scale_k, self.scale_v, fresh,
                            q, cos, sin, positions, interleaved, check)
-        if sum(wanted):
-            del self._free[len(self._free) - sum(wanted):]
-            self._table = table
+        if taken:
+            self._take(places, taken)
             self.block_table.copy_(block_table)
+        start = None if self.bounds is None else self.lengths.clone()
         self.lengths += S if fresh is None else fresh
         self.token_counts = [c + n for c, n in zip(self.token_counts, new)]
+        if start is not None:
+            from .page_selection import page_bounds
+
+            page_bounds(self.k_pages, self.block_table, self.lengths, self.scale_k, start, self.bounds, self.steps, self.head_dim)
         return out
 
+    def _take(self, places: List[Tuple[int, int]], pages: List[int]) -> None:
+        """``pages``, the last of the free ones, are taken for ``places``."""
+        rows, columns = zip(*places)
+        del self._free[len(self._free) - len(pages):]
+        self._table[list(rows), list(columns)] = torch.tensor(pages, dtype=torch.int32)
+
+    def _with_pages(self, places: List[Tuple[int, int]], pages: List[int]) -> torch.Tensor:
+        """The block table with ``pages`` at ``places`` (sequence, number), without waiting for the GPU."""
+        rows, columns = zip(*places)
+        at = _staged(torch.tensor([rows, columns, pages], dtype=torch.int64), self.lengths.device)
+        table = self.block_table.clone()
+        table[at[0], at[1]] = at[2].to(torch.int32)
+        return table
+
     def attention(self, q: torch.Tensor, scale: Optional[float] = None, causal: bool = False,
-                  new_lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """``paged_attention`` over everything held."""
+                  new_lengths: Optional[torch.Tensor] = None, keep: Optional[int] = None, first: int = 1,
+                  recent: int = 1) -> torch.Tensor:
+        """``paged_attention`` over everything held, or with ``keep`` over the pages that ``page_select`` chooses."""
+        pages = None
+        if keep is not None:
+            if self.bounds is None:
+                raise ValueError("a choice of pages needs PagedKVPool(..., bounds=True)")
+            from .page_selection import page_select
+
+            pages = page_select(q, self.bounds, self.steps, self.block_table, self.lengths, self.page_size, keep, first, recent, causal,
+                                new_lengths)
         return paged_attention(q, self.k_pages, self.v_pages, self.block_table, self.lengths, self.scale_k, self.scale_v,
-                               scale, causal, new_lengths)
+                               scale, causal, new_lengths, pages=pages)
 
     def read(self, tokens: Optional[int] = None, start: Optional[torch.Tensor] = None,
              dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -432,13 +517,86 @@ class PagedKVPool:
                           max(self.token_counts) if tokens is None else tokens, self.scale_k, self.scale_v, start,
                           self.head_dim, dtype)
 
+    def fork(self, b: int, others: Sequence[int]) -> None:
+        """The empty sequences ``others`` go on from sequence ``b``: its full pages are shared, a last page that is partly filled is
+        copied to a page of their own.  Raises ``ValueError`` for sequences that are not empty and ``RuntimeError`` where too few pages are free;
+        nothing has changed then."""
+        rows = [range(self.batch_size)[i] for i in (b, *others)]
+        if len(set(rows)) != len(rows) or any(self.token_counts[r] for r in rows[1:]):
+            raise ValueError(f"sequences {rows[1:]} are to be different, empty, and not {rows[0]}")
+        if len(rows) == 1 or self.token_counts[rows[0]] == 0:
+            return
+        j, partly = divmod(self.token_counts[rows[0]], self.page_size)
+        taken = self._free[len(self._free) - len(rows) + 1:][::-1] if partly else []
+        if partly and len(taken) < len(rows) - 1:
+            raise RuntimeError(f"{len(rows) - 1} pages wanted, {len(self._free)} free")
+        if len(rows) > 1024:
+            raise ValueError(f"{len(rows) - 1} sequences go on from one, 1023 at most")
+        from .beam import paged_reorder
+
+        places = [(r, j) for r in rows[1:]]
+        table = self._with_pages(places, taken) if taken else self.block_table
+        at = _staged(torch.tensor(rows, dtype=torch.int64), self.lengths.device)
+        parents = torch.zeros(1, len(rows), dtype=torch.int64, device=self.lengths.device)
+        new_table, new_lengths = paged_reorder(self.k_pages, self.v_pages, table[at], self.lengths[at], parents, self.scale_k, self.scale_v,
+                                               self.bounds, self.steps, self.head_dim)
+        self.block_table.index_copy_(0, at, new_table)
+        self.lengths.index_copy_(0, at, new_lengths)
+        if taken:
+            self._take(places, taken)
+        self._join(rows)
+        for r in rows[1:]:
+            self.token_counts[r] = self.token_counts[rows[0]]
+
+    def reorder(self, parents: torch.Tensor, check: bool = False) -> None:
+        """``paged_reorder`` of all sequences: ``parents`` ``[groups, beams]``, ``groups * beams`` the batch size.  The sequences of a group
+        must be equally long (``ValueError``).  The parents stay on the device; one outside its group leaves an empty sequence
+        there that the host counts as long as the others, unless ``check=True``, which waits, refuses it by ``ValueError``."""
+        if parents.dim() != 2 or parents.numel() != self.batch_size:
+            raise ValueError(f"parents must be [groups, beams] of {self.batch_size} sequences, got {tuple(parents.shape)}")
+        groups, beams = parents.shape
+        for g in range(groups):
+            counts = self.token_counts[g * beams:(g + 1) * beams]
+            if min(counts) != max(counts):
+                raise ValueError(f"the sequences of group {g} are not equally long: {counts}")
+        if check and not bool(((parents >= 0) & (parents < beams)).all()):
+            raise ValueError(f"a parent lies outside its group of {beams}")
+        from .beam import paged_reorder
+
+        table, lengths = paged_reorder(self.k_pages, self.v_pages, self.block_table, self.lengths, parents, self.scale_k, self.scale_v,
+                                       self.bounds, self.steps, self.head_dim)
+        self.block_table.copy_(table)
+        self.lengths.copy_(lengths)
+        for g in range(groups):
+            if self.token_counts[g * beams]:
+                self._join(range(g * beams, (g + 1) * beams))
+
+    def _join(self, rows: Sequence[int]) -> None:
+        """Sequences ``rows``, and those that they share pages with, return their pages together from now on."""
+        family = self._family[rows[0]]
+        for r in rows[1:]:
+            other = self._family[r]
+            if other is not family:
+                family.rows |= other.rows
+                family.pages.extend(other.pages)
+                for o in other.rows:
+                    self._family[o] = family
+
     def release(self, b: int) -> int:
-        """End sequence ``b``: its pages are free again.  Returns how many."""
-        n = self._pages_held(b)
-        self._free.extend(reversed(self._table[b, :n].tolist()))
+        """End sequence ``b``: its pages are free again, once no sequence is left that it shared pages with.  Returns how many
+        became free."""
+        b = range(self.batch_size)[b]
+        family = self._family[b]
+        family.rows.discard(b)
+        family.pages.extend(p for p in self._table[b].tolist() if p >= 0)
         self._table[b] = -1
+        self._family[b] = _Family(b)
+        n = 0
+        if not family.rows:
+            n = len(family.pages)
+            self._free.extend(reversed(family.pages))
         self.block_table[b].fill_(-1)
-        self.lengths[b:b + 1 or None].zero_()   # (an assignment to one element waits for the GPU)
+        self.lengths[b:b + 1].zero_()   # (an assignment to one element waits for the GPU)
         self.token_counts[b] = 0
         return n
 
@@ -450,14 +608,15 @@ class PagedKVPool:
 
 def paged_block_forward(block, hidden: torch.Tensor, pool: PagedKVPool, cos: Optional[torch.Tensor] = None,
                         sin: Optional[torch.Tensor] = None, causal: bool = False,
-                        new_lengths: Optional[Sequence[int]] = None) -> torch.Tensor:
+                        new_lengths: Optional[Sequence[int]] = None, keep: Optional[int] = None, first: int = 1,
+                        recent: int = 1) -> torch.Tensor:
     """One transformer block over a page pool, for prompts and for single tokens: the block's own modules (the layout
     of ``packed_block_forward``; ``num_kv_heads`` where the keys are shared) around ``pool.append`` (queries and keys
     rotated, keys and values quantised into their pages) and ``pool.attention``.
 
     ``hidden`` [B, S, hidden_dim] are the S newest tokens; returns their new hidden states.  Rows s >=
     ``new_lengths[b]`` (host numbers, default all S) are the padding of a ragged prompt: nothing is stored for
-    them and their outputs mean nothing.
+    them and their outputs mean nothing.  ``keep`` / ``first`` / ``recent`` as for ``pool.attention``: each query reads ``keep`` pages only.
     """
     import torch.nn.functional as F
 
@@ -473,6 +632,6 @@ def paged_block_forward(block, hidden: torch.Tensor, pool: PagedKVPool, cos: Opt
     else:
         q = pool.append(k, v, q=q, cos=cos, sin=sin, new_lengths=new_lengths)
     fresh = None if new_lengths is None else _staged(torch.tensor(list(new_lengths), dtype=torch.int32), pool.lengths.device)
-    attn = pool.attention(q, causal=causal, new_lengths=fresh).transpose(1, 2).reshape(B, S, nh * hd)
+    attn = pool.attention(q, causal=causal, new_lengths=fresh, keep=keep, first=first, recent=recent).transpose(1, 2).reshape(B, S, nh * hd)
     hidden = hidden + block.o_proj(attn)
     return hidden + block.down_proj(F.gelu(block.up_proj(block.ln2(hidden))))
