@@ -2,35 +2,53 @@
 // follow them.
 //
 // Selection.  A continuation's score is  s_r + x_rv - m_r - ln sum_v e^(x_rv - m_r),  m_r the row's largest logit.  Within a row
-// scores are ordered as logits are, so one pass over the logits is enough: a block takes a part of a row, 4096 logits at a time,
-// adds up its maximum and sum, and keeps the part's `keep` best logits; a second launch, a block a search, joins the
-// sums, turns the lists' logits into scores in 64 bits and merges the lists.  Bound by reading the logits.
+// scores are ordered as logits are, so one pass over the logits is enough.  A warp takes a block of a row into its registers,
+// up to 128 logits a lane, and leaves the block's maximum, its sum and its `keep` best logits: the keep-th largest of the lanes'
+// maxima is no more than the keep-th largest logit, so the few logits that are not below it are all that have to be ranked.  A
+// second launch, a block a search, joins the sums, turns the lists' logits into scores in 64 bits, and finds the best of all
+// in the same way from the lists' fronts.
 #include <float.h>
+
+#include <type_traits>
 
 #include "pool.cuh"
 
 namespace skv {
 
-constexpr int kBeamThreads = 256, kBeamValues = 16, kBeamChunk = kBeamThreads * kBeamValues;   // logits a thread, a block at a time
-constexpr int kBeamKeep = 128, kBeamMost = 4096;      // most continuations; most beams, and most lists of a search
-constexpr int kBeamHeld = 1024;                       // candidates that a block holds before it ranks them
+constexpr int kBeamKeep = 128, kBeamMost = 4096;      // most continuations; most beams of a search
+constexpr int kMergeEntries = 16384;                  // entries of lists whose scores a merge holds; half of it is aimed at
+constexpr int kBeamWarps = 4, kBeamHeld = 256;        // warps of a block, candidates that a warp holds
+constexpr int kManyLoads = 8, kFewLoads = 4;          // 16-byte loads a lane, of a block
+constexpr int kBeamBatch = 16;                        // blocks between two looks for candidates
+constexpr int kBeamPieces = 128;                      // (lane, block) pieces that are looked through then
 
-// What a part of a row leaves for the merge; its list follows the headers.
+// What a warp leaves for the merge; its list follows the headers.
 struct BeamPart {
     double sum;     // of e^(x - top), or how many are +inf where top is
     float top;
     int count;      // entries of the list: logits above -inf, best first
 };
 
-__host__ __device__ inline int64_t beam_chunks(int V) { return ((int64_t)V + kBeamChunk - 1) / kBeamChunk; }
-
-// Parts of a row: enough blocks to fill the GPU, no less than a chunk each, and no more lists than a merge takes.
-inline int beam_parts(int B, int beams, int V) {
+// Blocks of a row that are taken at once, and warps that share a row.
+struct BeamShape {
+    int loads, parts;
+    int64_t block, blocks;
+};
+inline BeamShape beam_shape(int B, int beams, int V, int keep, int bytes, bool aligned) {
+    BeamShape s;
     const int64_t rows = (int64_t)B * beams;
-    int64_t parts = ((int64_t)sm_count() * 6 + rows - 1) / rows;
-    if (parts > beam_chunks(V)) parts = beam_chunks(V);
-    if (parts > kBeamMost / beams) parts = kBeamMost / beams;
-    return parts < 1 ? 1 : (int)parts;
+    auto cut = [&](int loads) {
+        s.loads = loads;
+        s.block = 32ll * loads * (16 / bytes);
+        s.blocks = (V + (aligned ? 0 : 16 / bytes - 1) + s.block - 1) / s.block;   // (a row may begin inside of 16 bytes)
+    };
+    cut(kManyLoads);
+    if (rows * s.blocks < sm_count() * 8) cut(kFewLoads);          // too few warps to fill the GPU: more and smaller blocks
+    int64_t most = kMergeEntries / 2 / keep / beams, resident = sm_count() * 16 / rows;   // 16 warps an SM at a time
+    if (most > resident) most = resident;
+    if (most < 1) most = 1;
+    s.parts = (int)(s.blocks < most ? s.blocks : most);
+    return s;
 }
 
 // Whether beam r of search b has continuations of its own, and whether it has but one.
@@ -44,301 +62,479 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 constexpr float kLog2e = 1.4426950408889634f;
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+// 32 bits of logits: one or two.
+template <class T> struct Word {
+    static constexpr int N = 2;
+    using Pair = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    static __device__ __forceinline__ Pair pair(uint32_t w) { return *reinterpret_cast<const Pair*>(&w); }
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {   // of a number and a NaN: the number
+        const Pair m = __hmax2(pair(a), pair(b));
+        return *reinterpret_cast<const uint32_t*>(&m);
+    }
+    static __device__ __forceinline__ uint32_t larger_nan(uint32_t a, uint32_t b) {   // the NaN
+        const Pair m = __hmax2_nan(pair(a), pair(b));
+        return *reinterpret_cast<const uint32_t*>(&m);
+    }
+    static __device__ __forceinline__ uint32_t bits(__half x) { return __half_as_ushort(x); }
+    static __device__ __forceinline__ uint32_t bits(__nv_bfloat16 x) { return __bfloat16_as_ushort(x); }
+    static __device__ __forceinline__ uint32_t from(T x, T y) { return bits(x) | bits(y) << 16; }
+    static __device__ __forceinline__ uint32_t both(float x) { return from(from_float<T>(x), from_float<T>(x)); }
+    static __device__ __forceinline__ bool any_from(uint32_t w, uint32_t low) { return __hge2_mask(pair(w), pair(low)) != 0; }
+    static __device__ __forceinline__ float at(uint32_t w, int i) {
+        if constexpr (std::is_same_v<T, __half>) return __half2float(__ushort_as_half((unsigned short)(i ? w >> 16 : w & 0xffff)));
+        else return __uint_as_float(i ? w & 0xffff0000u : w << 16);
+    }
+    static __device__ __forceinline__ float largest(uint32_t w) { return max_nan(at(w, 0), at(w, 1)); }
+    static constexpr float kLowest = std::is_same_v<T, __half> ? -65504.0f : -3.3895313892515355e38f;
+};
+template <> struct Word<float> {
+    static constexpr int N = 1;
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
+    static __device__ __forceinline__ uint32_t larger_nan(uint32_t a, uint32_t b) { return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b))); }
+    static __device__ __forceinline__ uint32_t both(float x) { return __float_as_uint(x); }
+    static __device__ __forceinline__ bool any_from(uint32_t w, uint32_t low) { return __uint_as_float(w) >= __uint_as_float(low); }
+    static __device__ __forceinline__ float at(uint32_t w, int) { return __uint_as_float(w); }
+    static __device__ __forceinline__ float largest(uint32_t w) { return __uint_as_float(w); }
+    static constexpr float kLowest = -FLT_MAX;
+};
+
+__device__ __forceinline__ uint64_t pack2(float x, float y) { return (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x); }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float low_of(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float high_of(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+
 // Whether (x, i) comes before (y, j).
 __device__ __forceinline__ bool ahead(float x, int i, float y, int j) { return x > y || (x == y && i < j); }
 
-// Entries of the list [0, n) ranked, the best `keep` of them in order at its front; returns how many are left.  Every
-// entry counts the entries ahead of it.  All threads call this; barriers before and after.
-__device__ __forceinline__ int rank_list(float* value, int* index, int n, int keep, float* value2, int* index2) {
-    for (int i = threadIdx.x; i < n; i += kBeamThreads) {
-        const float x = value[i];
-        const int at = index[i];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += ahead(value[j], index[j], x, at);
-        if (rank < keep) { value2[rank] = x; index2[rank] = at; }
-    }
-    __syncthreads();
-    n = min(n, keep);
-    for (int i = threadIdx.x; i < n; i += kBeamThreads) { value[i] = value2[i]; index[i] = index2[i]; }
-    __syncthreads();
-    return n;
+// The value of rank `rank` (0: the largest) among the lanes' values, none a NaN: sorted by compare and exchange.
+__device__ __forceinline__ float warp_ranked(float x, int rank) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int o = size >> 1; o > 0; o >>= 1) {
+            const float y = __shfl_xor_sync(0xffffffffu, x, o);
+            x = ((lane & o) == 0) == ((lane & size) == 0) ? fmaxf(x, y) : fminf(x, y);
+        }
+    return __shfl_sync(0xffffffffu, x, rank);
 }
 
+// Logits [first, first + count) of a row have more candidates, from `from` to `most`, than were collected (many are equal, or many are
+// to be kept): halves the range of their images until a list with `held` entries has room for what is left, at the end with the
+// place up to which equal ones are taken.  Returns the entries of the list then.  A warp calls this, seldom: the logits are read again.
 template <class T>
-__global__ void __launch_bounds__(kBeamThreads) beam_parts_kernel(const __grid_constant__ skv_beam_args a, int parts) {
-    constexpr int PER = 16 / (int)sizeof(T), LOADS = kBeamValues / PER;
-    __shared__ float s_value[kBeamHeld], s_value2[kBeamKeep];
-    __shared__ int s_index[kBeamHeld], s_index2[kBeamKeep];
-    __shared__ float s_low[kBeamThreads / 32], s_top[kBeamThreads / 32];
-    __shared__ double s_sum[kBeamThreads / 32];
-    __shared__ int s_count[3], s_held;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, keep = a.keep;
-    const int64_t row = blockIdx.x / parts;
-    const int part = blockIdx.x % parts;
+__device__ __noinline__ int beam_many(const T* x0, int first, int count, int V, float from, float most, int keep, int held, float2* list,
+                                      int* s_count) {
+    const int lane = threadIdx.x & 31, begin = max(first, 0), end = min((int64_t)V, (int64_t)first + count), room = kBeamHeld - held;
+    auto logit = [&](int i) { return fmaxf(to_float(x0[i]), -INFINITY); };
+    auto count_from = [&](uint32_t image) {
+        int m = 0;
+        for (int i = begin + lane; i < end; i += 32) m += score_bits(logit(i)) >= image;
+        return __reduce_add_sync(0xffffffffu, m);
+    };
+    uint32_t lo = score_bits(from), hi = score_bits(most);   // if more than `room` are from lo on, the keep-th largest is in [lo, hi]
+    int from_lo = count_from(lo);
+    while (lo < hi && from_lo > room) {
+        const uint32_t mid = lo + (hi - lo + 1) / 2;
+        const int m = count_from(mid);
+        if (m >= keep) { lo = mid; from_lo = m; } else hi = mid - 1;
+    }
+    const float cut = __uint_as_float(lo & 0x80000000u ? lo ^ 0x80000000u : ~lo);
+    int last = end - 1;                                       // equal ones up to here are taken
+    if (from_lo > room) {                                     // (then fewer than `keep` are larger)
+        int lower = begin - 1;                                // there is room for those up to here
+        last = end - 1;
+        while (lower < last) {
+            const int mid = lower + (last - lower + 1) / 2;
+            int m = 0;
+            for (int i = begin + lane; i < end; i += 32) { const float x = logit(i); m += x > cut || (x == cut && i <= mid); }
+            m = __reduce_add_sync(0xffffffffu, m);
+            if (m <= room) lower = mid; else last = mid - 1;
+        }
+    }
+    if (lane == 0) *s_count = held;
+    __syncwarp();
+    for (int i = begin + lane; i < end; i += 32) {
+        const float x = logit(i);
+        if (x > cut || (x == cut && i <= last)) list[atomicAdd(s_count, 1)] = make_float2(x, __int_as_float(i));
+    }
+    __syncwarp();
+    return *s_count;
+}
+
+// A row's part in batches of up to kBeamBatch blocks.  The first look at a batch adds up its exponentials and keeps the largest logit of
+// every lane and block; the keep-th largest of the lanes' largest is a bound that few (lane, block) pieces reach, about `keep` and a
+// half, and only these are read again (they are in L2 still) for their candidates.  (Candidates looked for block by block, as they
+// come, took as many instructions again as all else: 34 us for 33.5 M 16-bit logits, 20 without them.)
+template <class T, int LOADS>
+__global__ void __launch_bounds__(32 * kBeamWarps, LOADS == kManyLoads ? 4 : 6) beam_lists_kernel(const __grid_constant__ skv_beam_args a, int parts, int64_t blocks) {
+    using W = Word<T>;
+    constexpr int PER = 16 / (int)sizeof(T), WORDS = 4 * LOADS, BLOCK = 32 * LOADS * PER;
+    __shared__ float2 s_list[kBeamWarps][kBeamHeld], s_ranked[kBeamWarps][kBeamKeep];
+    __shared__ float s_best[kBeamWarps][kBeamBatch][32];
+    __shared__ int s_piece[kBeamWarps][kBeamPieces], s_held[kBeamWarps];
+    start_dependents();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, keep = a.keep;
+    const int64_t job = (int64_t)blockIdx.x * kBeamWarps + warp, row = job / parts;
+    if (row >= (int64_t)a.B * a.beams) return;
+    const int part = (int)(job - row * parts);
     if (beam_dead(a, row) || beam_done(a, row)) return;   // the merge does not look at their lists
     const T* x0 = static_cast<const T*>(a.logits) + row / a.beams * a.stride_b + row % a.beams * a.stride_r;
     // 16-byte pieces on their boundaries: piece i holds logits i * PER - shift and on, the first and the last piece not all of theirs
     const int shift = (int)((reinterpret_cast<uintptr_t>(x0) & 15) / sizeof(T));
-    const int64_t pieces = ((int64_t)a.V + shift + PER - 1) / PER, chunk_pieces = kBeamThreads * LOADS;
-    const int64_t chunks = (pieces + chunk_pieces - 1) / chunk_pieces;
-    const int64_t c0 = chunks * part / parts, c1 = chunks * (part + 1) / parts;
-    int groups = kBeamThreads / 32;                       // threads in groups, at least `keep` of them
-    while (groups < keep) groups *= 2;
-    const int members = kBeamThreads / groups;
-    float top = -INFINITY, sum = 0.0f, low = -INFINITY;   // low: candidates are at least this
-    int held = 0, rounds = 0;
-    bool full = false;                                    // the list has `keep` entries
-    if (tid < 3) s_count[tid] = 0;
-    if (tid == 0) s_held = 0;
-    __syncthreads();
-    // How many of the block's predicates hold, summed over the threads.
-    auto total_of = [&](int n) {
-        n = __reduce_add_sync(0xffffffffu, n);
-        if (lane == 0 && n) atomicAdd(&s_count[rounds % 3], n);
-        if (tid == 0) s_count[(rounds + 1) % 3] = 0;
-        __syncthreads();
-        return s_count[rounds++ % 3];
+    float2* list = s_list[warp];
+    const int b0 = (int)(blocks * part / parts), b1 = (int)(blocks * (part + 1) / parts);
+    float top = -INFINITY;                                // of the warp
+    double sum = 0.0;
+    int held = 0;
+    float low = -INFINITY;                                // the keep-th best so far
+    // The list's n entries ranked (each counts those ahead of it), the best `keep` of them in order at its front.
+    auto rank = [&](int n) {
+        for (int i = lane; i < n; i += 32) {
+            const float2 e = list[i];
+            int before = 0;
+            for (int j = 0; j < n; ++j) {
+                const float2 f = list[j];
+                before += ahead(f.x, __float_as_int(f.y), e.x, __float_as_int(e.y));
+            }
+            if (before < keep) s_ranked[warp][before] = e;
+        }
+        __syncwarp();
+        held = min(n, keep);
+        for (int i = lane; i < held; i += 32) list[i] = s_ranked[warp][i];
+        __syncwarp();
+        if (held == keep) low = list[keep - 1].x;
     };
-    for (int64_t chunk = c0; chunk < c1; ++chunk) {
-        float x[kBeamValues];
-        const int64_t piece0 = chunk * chunk_pieces + tid;
+    auto word = [&](int i) {                              // logit i, and the next one, one by one
+        const T none = from_float<T>(-INFINITY), x = i >= 0 && i < a.V ? x0[i] : none;
+        if constexpr (W::N == 2) return W::from(x, i + 1 >= 0 && i + 1 < a.V ? x0[i + 1] : none);
+        else return __float_as_uint(x);
+    };
+    uint32_t next[WORDS];                                 // the block after the one at work, on its way
+    auto load = [&](int block) {
+        const int first0 = (block * 32 * LOADS + lane) * PER - shift;
+        if (block * BLOCK >= shift && (block + 1) * BLOCK - shift <= a.V) {
+            const uint4* y = reinterpret_cast<const uint4*>(x0 + first0);
 #pragma unroll
-        for (int l = 0; l < LOADS; ++l) {
-            const int64_t first = (piece0 + (int64_t)l * kBeamThreads) * PER - shift;
-            if (first >= 0 && first + PER <= a.V) {
-                const uint4 u = __ldcs(reinterpret_cast<const uint4*>(x0 + first));
-                const T* y = reinterpret_cast<const T*>(&u);
+            for (int l = 0; l < LOADS; ++l) {
+                const uint4 u = __ldg(y + 32 * l);
+                next[4 * l] = u.x; next[4 * l + 1] = u.y; next[4 * l + 2] = u.z; next[4 * l + 3] = u.w;
+            }
+            return;
+        }
 #pragma unroll
-                for (int i = 0; i < PER; ++i) x[l * PER + i] = fmaxf(to_float(y[i]), -INFINITY);   // (a NaN becomes -inf)
+        for (int l = 0; l < LOADS; ++l)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) next[4 * l + k] = word(first0 + 32 * PER * l + k * W::N);
+    };
+    load(b0);
+    for (int batch = b0; batch < b1; batch += kBeamBatch) {
+        const int count = min(kBeamBatch, b1 - batch);
+        float mine = -INFINITY;                           // the lane's largest of the batch
+        for (int i = 0; i < count; ++i) {
+            const int block = batch + i;
+            uint32_t w[WORDS];
+#pragma unroll
+            for (int k = 0; k < WORDS; ++k) w[k] = next[k];
+            if (block + 1 < b1) load(block + 1);
+            auto find_best = [&]() {
+                uint32_t best[4];
+#pragma unroll
+                for (int k = 0; k < WORDS; ++k) best[k % 4] = k < 4 ? w[k] : W::larger_nan(best[k % 4], w[k]);
+                return W::largest(W::larger_nan(W::larger_nan(best[0], best[1]), W::larger_nan(best[2], best[3])));
+            };
+            float best = find_best();
+            if (__any_sync(0xffffffffu, best != best)) {  // a NaN becomes -inf
+                const uint32_t none = W::both(-INFINITY);
+#pragma unroll
+                for (int k = 0; k < WORDS; ++k) w[k] = W::larger(w[k], none);
+                best = find_best();
+            }
+            s_best[warp][i][lane] = best;
+            mine = fmaxf(mine, best);
+            const float most = warp_max(best);
+            if (most == -INFINITY) continue;
+            // ---- the sum, relative to the block's largest logit
+            float more;
+            if (most == INFINITY) {
+                int n = 0;                                // (seldom: the logits are read again)
+                for (int j = max(block * BLOCK - shift, 0) + lane; j < min(a.V, (block + 1) * BLOCK - shift); j += 32)
+                    n += to_float(x0[j]) == INFINITY;
+                more = (float)__reduce_add_sync(0xffffffffu, n);
             } else {
+                // (sums of 32 or 16 terms in 32 bits each, two apart, so that their rounding stays below the exponentials')
+                const uint64_t less = pack2(-most, -most), by = pack2(kLog2e, kLog2e);
+                uint64_t total = 0;
+                more = 0.0f;
 #pragma unroll
-                for (int i = 0; i < PER; ++i)
-                    x[l * PER + i] = first + i >= 0 && first + i < a.V ? fmaxf(to_float(x0[first + i]), -INFINITY) : -INFINITY;
+                for (int k = 0; k < WORDS; k += W::N == 2 ? 1 : 2) {
+                    const float x = W::at(w[k], 0), y = W::N == 2 ? W::at(w[k], 1) : W::at(w[k + 1], 0);
+                    const uint64_t d = mul2(add2(pack2(x, y), less), by);
+                    total = add2(total, pack2(exp2_fast(low_of(d)), exp2_fast(high_of(d))));
+                    if (k % 16 >= (W::N == 2 ? 15 : 14)) {
+                        more += low_of(total) + high_of(total);
+                        total = 0;
+                    }
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
+            }
+            if (most > top) {
+                sum = sum * exp2_fast((top - most) * kLog2e) + more;     // (of -inf: 0)
+                top = most;
+            } else if (top < INFINITY || most == INFINITY) {
+                sum += most == top ? more : more * exp2_fast((most - top) * kLog2e);
             }
         }
-        float most = x[0];
-#pragma unroll
-        for (int i = 1; i < kBeamValues; ++i) most = fmaxf(most, x[i]);
-        if (most > top) {
-            sum *= exp2_fast((top - most) * kLog2e);      // (of -inf: 0)
-            top = most;
+        // ---- candidates: larger than the keep-th best so far (equal ones come behind it), not below the bound
+        const float most = warp_max(mine);
+        if (most <= low || most == -INFINITY) continue;
+        float from = W::kLowest;
+        if (low > -INFINITY) {                            // the next number of the type
+            uint32_t u = W::both(low == 0.0f ? 0.0f : low);
+            if constexpr (W::N == 2) u &= 0xffffu;
+            u = u & (W::N == 2 ? 0x8000u : 0x80000000u) ? u - 1 : u + 1;
+            from = W::at(u, 0);
         }
-        if (top == INFINITY) {
-            if (most == INFINITY)
-#pragma unroll
-                for (int i = 0; i < kBeamValues; ++i) sum += x[i] == INFINITY ? 1.0f : 0.0f;
-        } else {
-            const float from = top == -INFINITY ? 0.0f : top;
-            float more = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kBeamValues; ++i) more += exp2_fast((x[i] - from) * kLog2e);
-            sum += more;
-        }
-        if (!full) {
-            // the best of each group of threads are `keep` different logits: what is below all of them is not among the best
-            float best = most;
-            for (int o = 1; o < members; o <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) best = fminf(best, __shfl_xor_sync(0xffffffffu, best, o));
-            if (lane == 0) s_low[warp] = best;
-            __syncthreads();
-            best = s_low[0];
-            for (int w = 1; w < kBeamThreads / 32; ++w) best = fminf(best, s_low[w]);
-            low = fmaxf(best, -FLT_MAX);                  // -inf is no candidate
-        }
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < kBeamValues; ++i) n += x[i] >= low;
-        const int total = total_of(n);
-        float cut = low;                                  // candidates are above `cut`, or equal to it with a piece up to last
-        int64_t last = INT64_MAX;
-        if (held + total > kBeamHeld) {
-            // more than the list holds (many equal logits): the keep-th largest by halving the range of their images, then the
-            // place up to which those equal to it are taken
-            uint32_t at = 0;
-            for (int bit = 31; bit >= 0; --bit) {
-                const uint32_t y = at | 1u << bit;
+        if (keep <= 32) {
+            from = fmaxf(from, warp_ranked(mine, keep - 1));
+        } else if (count * 32 >= keep) {                  // of all that was kept: the range of their images is halved
+            uint32_t lo = score_bits(from), hi = score_bits(most);
+            while (lo < hi) {
+                const uint32_t mid = lo + (hi - lo + 1) / 2;
                 int m = 0;
-#pragma unroll
-                for (int i = 0; i < kBeamValues; ++i) m += x[i] >= low && score_bits(x[i]) >= y;
-                if (total_of(m) >= keep) at = y;
+                for (int i = 0; i < count; ++i) m += score_bits(s_best[warp][i][lane]) >= mid;
+                if (__reduce_add_sync(0xffffffffu, m) >= keep) lo = mid; else hi = mid - 1;
             }
-            cut = __uint_as_float(at & 0x80000000u ? at ^ 0x80000000u : ~at);
-            int m = 0;
-#pragma unroll
-            for (int i = 0; i < kBeamValues; ++i) m += x[i] > cut;
-            const int ties = keep - total_of(m);
-            // places in the chunk run over 4096 numbers
-            int end = 0;                                  // the largest number below which there are at most `ties`
-            for (int bit = 12; bit >= 0; --bit) {
-                const int y = end | 1 << bit;
-                m = 0;
-#pragma unroll
-                for (int i = 0; i < kBeamValues; ++i) m += x[i] == cut && (tid + i / PER * kBeamThreads) * PER + i % PER < y;
-                if (total_of(m) <= ties) end = y;
-            }
-            last = end;
-            n = 0;
-#pragma unroll
-            for (int i = 0; i < kBeamValues; ++i)
-                n += x[i] > cut || (x[i] == cut && (tid + i / PER * kBeamThreads) * PER + i % PER < last);
+            from = fmaxf(from, __uint_as_float(lo & 0x80000000u ? lo ^ 0x80000000u : ~lo));
         }
-        if (__any_sync(0xffffffffu, n)) {
-            int incl = n;
+        int n = held, pieces = 0;
+        for (int i = 0; i < count; ++i) {
+            const unsigned these = __ballot_sync(0xffffffffu, s_best[warp][i][lane] >= from);
+            const int to = pieces + __popc(these & ((1u << lane) - 1));
+            if (these >> lane & 1 && to < kBeamPieces) s_piece[warp][to] = ((batch + i) * 32 * LOADS + lane) * PER - shift;
+            pieces += __popc(these);
+        }
+        __syncwarp();
+        const bool many = pieces > kBeamPieces;           // (many equal logits)
+        // a load of one piece a lane, two at a time
+        constexpr int AT_ONCE = 32 / LOADS;
+        for (int i = lane / LOADS; i - lane / LOADS < pieces && !many; i += 2 * AT_ONCE) {
+            uint32_t y[2][4];
+            int first[2];
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += y;
+            for (int h = 0; h < 2; ++h) {
+                const bool is = i + h * AT_ONCE < pieces;
+                first[h] = (is ? s_piece[warp][i + h * AT_ONCE] : 0) + lane % LOADS * 32 * PER;
+                if (is && first[h] >= 0 && first[h] + PER <= a.V) {
+                    const uint4 u = __ldg(reinterpret_cast<const uint4*>(x0 + first[h]));
+                    y[h][0] = u.x; y[h][1] = u.y; y[h][2] = u.z; y[h][3] = u.w;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) y[h][k] = is ? word(first[h] + k * W::N) : W::both(-INFINITY);
+                }
             }
-            int at = lane == 31 ? atomicAdd(&s_held, incl) : 0;
-            at = __shfl_sync(0xffffffffu, at, 31) + incl - n;
 #pragma unroll
-            for (int i = 0; i < kBeamValues; ++i)
-                if (x[i] > cut || (x[i] == cut && (tid + i / PER * kBeamThreads) * PER + i % PER < last)) {
-                    s_value[at] = x[i];
-                    s_index[at++] = (int)((piece0 + i / PER * kBeamThreads) * PER + i % PER - shift);
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int k = 0; k < PER; ++k) {
+                    const float x = W::at(y[h][k / W::N], k % W::N);
+                    const unsigned is = __ballot_sync(0xffffffffu, x >= from);
+                    const int to = n + __popc(is & ((1u << lane) - 1));
+                    if (x >= from && to < kBeamHeld) list[to] = make_float2(x, __int_as_float(first[h] + k));
+                    n += __popc(is);
                 }
         }
-        __syncthreads();
-        held = s_held;
-        if (held > 2 * keep + 64 || (!full && held >= keep) || (chunk + 1 == c1 && held > 0)) {
-            held = rank_list(s_value, s_index, held, keep, s_value2, s_index2);
-            full = held == keep;
-            if (full) {
-                // a later logit has to be larger than the last of the list
-                const float v = s_value[keep - 1];
-                low = v == INFINITY ? NAN : v == 0.0f ? FLT_TRUE_MIN : __int_as_float(__float_as_int(v) + (v > 0.0f ? 1 : -1));
-            }
-            if (tid == 0) s_held = held;
-            __syncthreads();
-        }
+        __syncwarp();
+        if (many || n > kBeamHeld) n = beam_many(x0, batch * BLOCK - shift, count * BLOCK, a.V, from, most, keep, held, list, s_held + warp);
+        rank(n);
     }
-    // the part's sum, relative to its largest logit
-    float most = top;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    if (lane == 0) s_top[warp] = most;
-    __syncthreads();
-    for (int w = 0; w < kBeamThreads / 32; ++w) most = fmaxf(most, s_top[w]);
-    double whole = top == most ? (double)sum : most == INFINITY || top == -INFINITY ? 0.0 : (double)sum * exp2((double)(top - most) * 1.4426950408889634);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) whole += __shfl_xor_sync(0xffffffffu, whole, o);
-    if (lane == 0) s_sum[warp] = whole;
-    __syncthreads();
-    const int64_t list = blockIdx.x, lists = (int64_t)a.B * a.beams * parts;
-    if (tid == 0) {
-        double s = 0.0;
-        for (int w = 0; w < kBeamThreads / 32; ++w) s += s_sum[w];
-        static_cast<BeamPart*>(a.scratch)[list] = BeamPart{s, most, held};
-    }
-    float2* out = reinterpret_cast<float2*>(static_cast<BeamPart*>(a.scratch) + lists) + list * keep;
-    for (int i = tid; i < held; i += kBeamThreads) out[i] = make_float2(s_value[i], __int_as_float(s_index[i]));
+    if (lane == 0) static_cast<BeamPart*>(a.scratch)[job] = BeamPart{sum, top, held};
+    float2* out = reinterpret_cast<float2*>(static_cast<BeamPart*>(a.scratch) + (int64_t)a.B * a.beams * parts) + job * keep;
+    for (int i = lane; i < held; i += 32) out[i] = list[i];
 }
 
 // ------------------------------------------------------------------------------------------ the merge
+constexpr int kMergeThreads = 256, kMergeHeld = 768;
+
 struct BeamBest {
     double score;
     uint64_t place;    // beam * 2^32 + token; the largest number for none
-    int list;
     __device__ __forceinline__ bool before(const BeamBest& o) const { return score > o.score || (score == o.score && place < o.place); }
 };
 
-// A block a search.  Each list's front is in shared memory; `keep` times the best of the fronts is taken.
+// A block a search.
 template <class T>
-__global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(const __grid_constant__ skv_beam_args a, int parts, bool staged) {
+__global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_constant__ skv_beam_args a, int parts) {
     extern __shared__ __align__(16) unsigned char s_raw[];
-    __shared__ BeamBest s_best[2][kBeamThreads / 32];
-    __shared__ int s_part[2][kBeamThreads / 32];
+    __shared__ BeamBest s_held[kMergeHeld];
+    __shared__ BeamBest s_best[2][kMergeThreads / 32];
+    __shared__ float s_front[2][kMergeThreads / 32];
+    __shared__ int s_part[2][kMergeThreads / 32], s_n, s_owner[2][kMergeThreads / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, keep = a.keep, beams = a.beams, lists = beams * parts;
     const int64_t row0 = (int64_t)blockIdx.x * beams;
-    double* s_front = reinterpret_cast<double*>(s_raw);             // [lists] score of each list's front
-    double* s_from = s_front + lists;                               // [beams] what a logit less the largest is added to
-    int* s_token = reinterpret_cast<int*>(s_from + beams);          // [lists] token of the front
-    float* s_most = reinterpret_cast<float*>(s_token + lists);      // [beams] the largest logit
-    int* s_at = reinterpret_cast<int*>(s_most + beams);             // [lists] places of the fronts
-    int* s_count = s_at + lists;                                    // [lists]
-    float2* s_list = reinterpret_cast<float2*>(reinterpret_cast<uintptr_t>(s_count + lists + 1) & ~(uintptr_t)7);   // staged: [lists][keep]
+    double* s_from = reinterpret_cast<double*>(s_raw);              // [beams] what a logit less the largest is added to
+    float* s_most = reinterpret_cast<float*>(s_from + beams);       // [beams] the largest logit
+    int* s_count = reinterpret_cast<int*>(s_most + beams);          // [lists] entries
     const BeamPart* part = static_cast<const BeamPart*>(a.scratch) + row0 * parts;
     const float2* entries = reinterpret_cast<const float2*>(static_cast<const BeamPart*>(a.scratch) + (int64_t)a.B * lists) +
                             row0 * parts * keep;
-    if (staged)
-        for (int i = tid; i < lists * keep; i += kBeamThreads) s_list[i] = entries[i];
-    for (int r = tid; r < beams; r += kBeamThreads) {
-        const double cum = __ldg(a.scores + row0 + r);
-        if (beam_dead(a, row0 + r) || beam_done(a, row0 + r)) {
-            s_from[r] = cum;
-            s_most[r] = -INFINITY;
-            continue;
-        }
+    if (tid == 0) s_n = 0;
+    // what the scores need is on its way before the sums are looked at
+    const int entries_all = lists * keep;
+    constexpr int FLY = 6;
+    float2 early[FLY];
+    wait_for_dependency();
+#pragma unroll
+    for (int k = 0; k < FLY; ++k) early[k] = tid + k * kMergeThreads < entries_all ? __ldcg(entries + tid + k * kMergeThreads) : make_float2(0.0f, 0.0f);
+    for (int r = warp; r < beams; r += kMergeThreads / 32) {        // a warp a beam
+        const float cum = __ldg(a.scores + row0 + r);
+        const bool done = beam_done(a, row0 + r), dead = !(fabsf(cum) < INFINITY);
         float most = -INFINITY;
-        for (int p = 0; p < parts; ++p) most = fmaxf(most, part[r * parts + p].top);
         double sum = 0.0;
-        for (int p = 0; p < parts; ++p) {
-            const BeamPart& y = part[r * parts + p];
-            if (y.top == most) sum += y.sum;
-            else if (most < INFINITY && y.top > -INFINITY) sum += y.sum * exp((double)y.top - (double)most);
+        for (int p0 = 0; p0 < parts; p0 += 32) {
+            BeamPart y{0.0, -INFINITY, 0};
+            if (p0 + lane < parts && !done && !dead) y = part[r * parts + p0 + lane];
+            if (p0 + lane < parts) s_count[r * parts + p0 + lane] = y.count;
+            const float now = fmaxf(most, warp_max(y.top));
+            double x = y.top == -INFINITY ? 0.0 : y.sum;
+            if (y.top < now) x = now < INFINITY ? x * exp2_fast((y.top - now) * kLog2e) : 0.0;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+            if (most < now) sum = most == -INFINITY || now == INFINITY ? 0.0 : sum * exp2_fast((most - now) * kLog2e);
+            sum += x;
+            most = now;
         }
-        s_from[r] = cum - log(sum);                                 // (without a logit above -inf: not used)
-        s_most[r] = most;
+        if (lane == 0) {
+            s_from[r] = done || dead ? (double)cum : cum - log(sum);   // (without a logit above -inf: not used)
+            s_most[r] = done || dead ? -INFINITY : most;
+            if (done && !dead) s_count[r * parts] = -1;
+        }
     }
     __syncthreads();
-    auto score_of = [&](int r, float x) {
-        return x == s_most[r] ? s_from[r] : s_most[r] == INFINITY ? -(double)INFINITY : s_from[r] + ((double)x - (double)s_most[r]);
+    // entry `at` of list l, x as it was left; false: there is none, or it scores -inf
+    const float by_parts = 1.0f / (float)parts, by_keep = 1.0f / (float)keep;   // (numbers below 2^20: half of a unit is more than the error)
+    auto entry_of = [&](int l, int at, float2 x, BeamBest& e) {
+        const int r = (int)(((float)l + 0.5f) * by_parts), count = s_count[l];
+        if (at >= count) {                                          // (-1: a finished beam's one continuation)
+            e = BeamBest{s_from[r], (uint64_t)r << 32 | (uint32_t)a.pad_token};
+            return count < 0 && at == 0;
+        }
+        const float most = s_most[r];
+        e.score = x.x == most ? s_from[r] : s_from[r] + ((double)x.x - (double)most);
+        e.place = (uint64_t)r << 32 | (uint32_t)__float_as_int(x.y);
+        return x.x == most || most < INFINITY;
     };
-    auto place_front = [&](int l) {
-        const int at = s_at[l];
-        if (at >= s_count[l]) { s_front[l] = -(double)INFINITY; return; }
-        const float2 e = staged ? s_list[(int64_t)l * keep + at] : entries[(int64_t)l * keep + at];
-        s_front[l] = score_of(l / parts, e.x);
-        s_token[l] = __float_as_int(e.y);
-    };
-    for (int l = tid; l < lists; l += kBeamThreads) {
-        const int r = l / parts;
-        s_at[l] = 0;
-        if (beam_dead(a, row0 + r)) {
-            s_count[l] = 0;
-            s_front[l] = -(double)INFINITY;
-        } else if (beam_done(a, row0 + r)) {                        // the one continuation, no list behind it
-            s_count[l] = 0;
-            s_front[l] = l % parts == 0 ? s_from[r] : -(double)INFINITY;
-            s_token[l] = a.pad_token;
-        } else {
-            s_count[l] = part[l].count;
-            place_front(l);
+    auto entry = [&](int l, int at, BeamBest& e) { return entry_of(l, at, at < s_count[l] ? __ldcg(entries + (int64_t)l * keep + at) : make_float2(0.0f, 0.0f), e); };
+    // ---- candidates: scores as 32-bit numbers, from one on that keep of them, and not many more, reach
+    BeamBest e;
+    int round = 0, n = kMergeHeld + 1;
+    if (entries_all <= kMergeEntries) {
+        float* s_score = reinterpret_cast<float*>(s_count + lists);   // [lists][keep]
+        float best = -INFINITY, front = -INFINITY;                  // of a thread's entries, of a thread's lists' fronts
+        auto put_score = [&](int i, float2 y) {
+            const int l = (int)(((float)i + 0.5f) * by_keep);
+            const float x = entry_of(l, i - l * keep, y, e) ? fmaxf((float)e.score, -FLT_MAX) : -INFINITY;
+            s_score[i] = x;
+            best = fmaxf(best, x);
+        };
+#pragma unroll
+        for (int k = 0; k < FLY; ++k)
+            if (tid + k * kMergeThreads < entries_all) put_score(tid + k * kMergeThreads, early[k]);
+        for (int i = tid + FLY * kMergeThreads; i < entries_all; i += kMergeThreads) put_score(i, __ldcg(entries + i));
+        __syncthreads();
+        for (int l = tid; l < lists; l += kMergeThreads) front = fmaxf(front, s_score[l * keep]);
+        front = keep <= 32 ? warp_ranked(front, keep - 1) : -INFINITY;
+        best = warp_max(best);
+        if (lane == 0) { s_front[0][warp] = front; s_front[1][warp] = best; }
+        __syncthreads();
+        for (int w = 0; w < kMergeThreads / 32; ++w) { front = fmaxf(front, s_front[0][w]); best = fmaxf(best, s_front[1][w]); }
+        auto count_from = [&](float x) {
+            int m = 0;
+            for (int i = tid; i < entries_all; i += kMergeThreads) m += s_score[i] >= x;
+            m = __reduce_add_sync(0xffffffffu, m);
+            if (lane == 0) s_part[round & 1][warp] = m;
+            __syncthreads();
+            m = 0;
+            for (int w = 0; w < kMergeThreads / 32; ++w) m += s_part[round & 1][w];
+            ++round;
+            return m;
+        };
+        auto value_of = [](uint32_t image) { return __uint_as_float(image & 0x80000000u ? image ^ 0x80000000u : ~image); };
+        uint32_t lo = score_bits(fmaxf(front, -FLT_MAX)), hi = score_bits(fmaxf(best, -FLT_MAX));
+        n = count_from(value_of(lo));
+        while (lo < hi && n > keep + 64) {
+            const uint32_t mid = lo + (hi - lo + 1) / 2;
+            const int m = count_from(value_of(mid));
+            if (m >= keep) { lo = mid; n = m; } else hi = mid - 1;
+        }
+        if (n <= kMergeHeld) {
+            const float least = value_of(lo);
+            for (int i = tid; i < entries_all; i += kMergeThreads)
+                if (s_score[i] >= least && entry((int)(((float)i + 0.5f) * by_keep), i % keep, e)) s_held[atomicAdd(&s_n, 1)] = e;
+            __syncthreads();
+            n = s_n;
         }
     }
     int found = 0;
-    for (; found < keep; ++found) {
-        BeamBest best{-(double)INFINITY, ~0ull, -1};
-        for (int l = tid; l < lists; l += kBeamThreads) {           // (each thread reads and advances its own lists only)
-            const BeamBest y{s_front[l], (uint64_t)(l / parts) << 32 | (uint32_t)s_token[l], l};
-            if (y.score > -(double)INFINITY && y.before(best)) best = y;
+    auto put = [&](int rank, const BeamBest& x) {
+        const int64_t to = (int64_t)blockIdx.x * keep + rank;
+        a.values[to] = (float)x.score;
+        a.parents[to] = (int64_t)(x.place >> 32);
+        a.tokens[to] = (int64_t)(x.place & 0xffffffffu);
+    };
+    if (n <= kMergeHeld) {
+        for (int i = tid; i < n; i += kMergeThreads) {
+            const BeamBest x = s_held[i];
+            int rank = 0;
+            for (int j = 0; j < n; ++j) rank += s_held[j].before(x);
+            if (rank < keep) put(rank, x);
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const BeamBest y{__shfl_xor_sync(0xffffffffu, best.score, o), __shfl_xor_sync(0xffffffffu, best.place, o),
-                             __shfl_xor_sync(0xffffffffu, best.list, o)};
-            if (y.before(best)) best = y;
-        }
-        if (lane == 0) s_best[found & 1][warp] = best;
+        found = min(n, keep);
+    } else {
+        // more candidates than are held (many equal ones): the best of the lists' fronts, `keep` times
         __syncthreads();
-        best = s_best[found & 1][0];
-        for (int w = 1; w < kBeamThreads / 32; ++w)
-            if (s_best[found & 1][w].before(best)) best = s_best[found & 1][w];
-        if (best.list < 0) break;
-        if (tid == 0) {
-            const int64_t to = (int64_t)blockIdx.x * keep + found;
-            a.values[to] = (float)best.score;
-            a.parents[to] = (int64_t)(best.place >> 32);
-            a.tokens[to] = (int64_t)(best.place & 0xffffffffu);
-        }
-        if (best.list % kBeamThreads == tid) {
-            ++s_at[best.list];
-            place_front(best.list);
+        int* s_at = s_count + lists;                                // [lists] places of the fronts
+        for (int l = tid; l < lists; l += kMergeThreads) s_at[l] = 0;
+        for (; found < keep; ++found) {
+            BeamBest best{-(double)INFINITY, ~0ull};
+            int owner = -1;
+            for (int l = tid; l < lists; l += kMergeThreads)        // (each thread reads and advances its own lists only)
+                if (entry(l, s_at[l], e) && e.before(best)) { best = e; owner = l; }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                const BeamBest y{__shfl_xor_sync(0xffffffffu, best.score, o), __shfl_xor_sync(0xffffffffu, best.place, o)};
+                const int y_owner = __shfl_xor_sync(0xffffffffu, owner, o);
+                if (y.before(best)) { best = y; owner = y_owner; }
+            }
+            if (lane == 0) { s_best[found & 1][warp] = best; s_owner[found & 1][warp] = owner; }
+            __syncthreads();
+            best = s_best[found & 1][0];
+            owner = s_owner[found & 1][0];
+            for (int w = 1; w < kMergeThreads / 32; ++w)
+                if (s_best[found & 1][w].before(best)) { best = s_best[found & 1][w]; owner = s_owner[found & 1][w]; }
+            if (owner < 0) break;
+            if (tid == 0) put(found, best);
+            if (owner % kMergeThreads == tid) ++s_at[owner];
         }
     }
-    // too few: continuations of -inf, from the first on
-    for (int64_t i0 = 0, round = 0; found < keep; i0 += kBeamThreads, ++round) {
+    // ---- too few: continuations of -inf, from the first on
+    for (int64_t i0 = 0; found < keep && i0 < (int64_t)beams * a.V; i0 += kMergeThreads, ++round) {
         const int64_t i = i0 + tid;
         bool none = false;
         int64_t r = 0, t = 0;
@@ -356,7 +552,7 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(const __grid_c
         if (lane == 0) s_part[round & 1][warp] = __popc(these);
         __syncthreads();
         int before = 0, total = 0;
-        for (int w = 0; w < kBeamThreads / 32; ++w) {
+        for (int w = 0; w < kMergeThreads / 32; ++w) {
             if (w < warp) before += s_part[round & 1][w];
             total += s_part[round & 1][w];
         }
@@ -367,24 +563,26 @@ __global__ void __launch_bounds__(kBeamThreads) beam_merge_kernel(const __grid_c
             a.tokens[(int64_t)blockIdx.x * keep + to] = t;
         }
         found += total;
-        if (i0 >= (int64_t)beams * a.V) break;
     }
 }
 
 template <class T>
 int launch_beam(const skv_beam_args& a, cudaStream_t st) {
-    const int parts = beam_parts(a.B, a.beams, a.V), lists = a.beams * parts;
-    beam_parts_kernel<T><<<(unsigned)((int64_t)a.B * lists), kBeamThreads, 0, st>>>(a, parts);
+    const bool aligned = (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 && a.stride_b % (16 / (int)sizeof(T)) == 0 &&
+                         a.stride_r % (16 / (int)sizeof(T)) == 0;
+    const BeamShape s = beam_shape(a.B, a.beams, a.V, a.keep, sizeof(T), aligned);
+    const int64_t jobs = (int64_t)a.B * a.beams * s.parts;
+    const unsigned grid = (unsigned)((jobs + kBeamWarps - 1) / kBeamWarps);
+    if (s.loads == kManyLoads) beam_lists_kernel<T, kManyLoads><<<grid, 32 * kBeamWarps, 0, st>>>(a, s.parts, s.blocks);
+    else beam_lists_kernel<T, kFewLoads><<<grid, 32 * kBeamWarps, 0, st>>>(a, s.parts, s.blocks);
     if (const int rc = check_launch("beam_select")) return rc;
-    size_t smem = (size_t)lists * 20 + (size_t)a.beams * 12 + 16;
-    const size_t with = smem + (size_t)lists * a.keep * 8;
-    const bool staged = with <= 96 * 1024;
-    if (staged) smem = with;
-    if (smem > 40 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(beam_merge_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 140 * 1024);
+    const int64_t lists = (int64_t)a.beams * s.parts, entries = lists * a.keep;
+    const size_t smem = (size_t)a.beams * 12 + (lists + (entries <= kMergeEntries ? entries : lists)) * 4;   // at most 48 + 32 + 64 KB
+    if (smem > 24 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(beam_merge_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 144 * 1024);
         if (e != cudaSuccess) return fail(SKV_ERR_CUDA, "beam_select: %s", cudaGetErrorString(e));
     }
-    beam_merge_kernel<T><<<a.B, kBeamThreads, smem, st>>>(a, parts, staged);
+    launch_after(beam_merge_kernel<T>, dim3(a.B), kMergeThreads, smem, st, a, s.parts);
     return check_launch("beam_select");
 }
 
@@ -501,7 +699,8 @@ extern "C" {
 
 size_t skv_beam_scratch_bytes(int B, int beams, int V, int keep) {
     if (B <= 0 || beams <= 0 || beams > kBeamMost || V <= 0 || keep <= 0) return 0;
-    return (size_t)B * beams * beam_parts(B, beams, V) * (sizeof(BeamPart) + (size_t)keep * 8);
+    const int wide = beam_shape(B, beams, V, keep, 4, false).parts, narrow = beam_shape(B, beams, V, keep, 2, false).parts;
+    return (size_t)B * beams * (wide > narrow ? wide : narrow) * (sizeof(BeamPart) + (size_t)keep * 8);
 }
 
 int skv_beam_select(const skv_beam_args* args, void* stream) {
@@ -513,7 +712,7 @@ int skv_beam_select(const skv_beam_args* args, void* stream) {
         return fail(SKV_ERR_SHAPE, "beam_select: %d continuations of %d beams and %d tokens", a.keep, a.beams, a.V);
     if (a.finished && (a.pad_token < 0 || a.pad_token >= a.V))
         return fail(SKV_ERR_INVALID_ARGUMENT, "beam_select: pad token %d", a.pad_token);
-    if (a.keep > kBeamKeep || a.beams > kBeamMost || a.V > 0x7fffffff - kBeamChunk)
+    if (a.keep > kBeamKeep || a.beams > kBeamMost || a.V > 0x7fff0000)
         return fail(SKV_ERR_TOO_LARGE, "beam_select: keep %d (at most %d), %d beams (at most %d), %d tokens", a.keep, kBeamKeep, a.beams,
                     kBeamMost, a.V);
     if (a.B == 0) return SKV_OK;
@@ -521,8 +720,7 @@ int skv_beam_select(const skv_beam_args* args, void* stream) {
         return fail(SKV_ERR_INVALID_ARGUMENT, "beam_select: null pointer");
     if (reinterpret_cast<uintptr_t>(a.scratch) & 15 || reinterpret_cast<uintptr_t>(a.logits) % dtype_bytes(a.dtype))
         return fail(SKV_ERR_INVALID_ARGUMENT, "beam_select: scratch or logits are not aligned");
-    const int64_t blocks = (int64_t)a.B * a.beams * beam_parts(a.B, a.beams, a.V);
-    if (blocks > 0x7fffffff) return fail(SKV_ERR_TOO_LARGE, "beam_select: too many rows");
+    if ((int64_t)a.B * a.beams > 0x7fffffff / kBeamMost) return fail(SKV_ERR_TOO_LARGE, "beam_select: too many rows");
     if (a.scratch_bytes < (int64_t)skv_beam_scratch_bytes(a.B, a.beams, a.V, a.keep))
         return fail(SKV_ERR_SCRATCH, "beam_select: scratch of %lld bytes", (long long)a.scratch_bytes);
     cudaStream_t st = as_stream(stream);
