@@ -61,9 +61,8 @@ struct TouchedPages {
         return a.start ? max(0, __ldg(a.start + b)) / a.pool.page_size : 0;
     }
     static __device__ __forceinline__ int count(const skv_pool_bounds_args& a, int b) {
-        const int n = tokens(a, b);
-        if (a.start && __ldg(a.start + b) >= n) return 0;
-        return n > 0 ? (n - 1) / a.pool.page_size + 1 - first(a, b) : 0;
+        const int start = a.start ? __ldg(a.start + b) : 0, n = tokens(a, b);
+        return start >= n ? 0 : (n - 1) / a.pool.page_size + 1 - max(0, start) / a.pool.page_size;
     }
     __device__ __forceinline__ void prepare(const skv_pool_bounds_args& a) {
         const int tid = threadIdx.x, lane = tid & 31, B = a.pool.batch, per = (B + kBoundsThreads - 1) / kBoundsThreads;
@@ -101,98 +100,171 @@ struct TouchedPages {
     }
 };
 
-// A warp a (page, head): its rows are one block of memory, 8 values a lane.  VEC: D a multiple of 8, at most 256,
-// int4 groups of whole lanes, payload on 16-byte boundaries; else value by value, the rows read twice.
+// The least and the largest of 8 columns over the rows that a lane has seen.  fp16 rows are compared two values at a time as they are.
+template <int PREC> struct Extremes {
+    float lo[8], hi[8];
+    __device__ __forceinline__ void start() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { lo[i] = INFINITY; hi[i] = -INFINITY; }
+    }
+    __device__ __forceinline__ void add(const PoolRaw<PREC, 8>& x) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float y = x.get(i);
+            lo[i] = min_nan(lo[i], y);
+            hi[i] = max_nan(hi[i], y);
+        }
+    }
+    __device__ __forceinline__ void join(int from) {   // with lane `from`'s
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            lo[i] = min_nan(lo[i], __shfl_sync(0xffffffffu, lo[i], from));
+            hi[i] = max_nan(hi[i], __shfl_sync(0xffffffffu, hi[i], from));
+        }
+    }
+    __device__ __forceinline__ float low(int i) const { return lo[i]; }
+    __device__ __forceinline__ float high(int i) const { return hi[i]; }
+};
+template <> struct Extremes<1> {
+    __half2 lo[4], hi[4];
+    __device__ __forceinline__ void start() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { lo[i] = __float2half2_rn(INFINITY); hi[i] = __float2half2_rn(-INFINITY); }
+    }
+    __device__ __forceinline__ void add(const PoolRaw<1, 8>& x) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2 y = *reinterpret_cast<const __half2*>(&x.w[i]);
+            lo[i] = __hmin2_nan(lo[i], y);
+            hi[i] = __hmax2_nan(hi[i], y);
+        }
+    }
+    __device__ __forceinline__ void join(int from) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            lo[i] = __hmin2_nan(lo[i], __shfl_sync(0xffffffffu, lo[i], from));
+            hi[i] = __hmax2_nan(hi[i], __shfl_sync(0xffffffffu, hi[i], from));
+        }
+    }
+    __device__ __forceinline__ float low(int i) const { return i & 1 ? __high2float(lo[i / 2]) : __low2float(lo[i / 2]); }
+    __device__ __forceinline__ float high(int i) const { return i & 1 ? __high2float(hi[i / 2]) : __low2float(hi[i / 2]); }
+};
+
+// A warp a run of (page, head) items: an item's rows are one block of memory, 8 values a lane.  VEC: D a multiple of 8, at most
+// 256, int4 groups of whole lanes, payload on 16-byte boundaries; else value by value, the rows read twice.
 template <int PREC, bool VEC>
 __global__ void __launch_bounds__(kBoundsThreads) pool_bounds_kernel(const __grid_constant__ skv_pool_bounds_args a) {
     __shared__ TouchedPages s;
-    s.prepare(a);
     const int lane = threadIdx.x & 31, D = a.pool.head_dim, P = a.pool.page_size, H = a.pool.heads;
-    const int64_t items = s.total() * H, stride = (int64_t)gridDim.x * (kBoundsThreads / 32);
-    for (int64_t item = (int64_t)blockIdx.x * (kBoundsThreads / 32) + (threadIdx.x >> 5); item < items; item += stride) {
-        int b, j;
-        s.find(a, item / H, b, j);
-        const int h = (int)(item % H);
-        const int64_t first_row = pool_row(a.pool, b, (int64_t)j * P);
-        if (first_row < 0) {
-            if (a.error_flag) atomicExch(a.error_flag, 1);
-            continue;
+    // up to 32 sequences a warp numbers by itself, a lane a sequence
+    const bool few = a.pool.batch <= 32;
+    int64_t mine = 0, before = 0, all;
+    if (few) {
+        before = mine = lane < a.pool.batch ? TouchedPages::count(a, lane) : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t x = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += x;
         }
-        const int64_t row = first_row + (int64_t)h * P, page_head = row / P;
-        const int rows = min(P, TouchedPages::tokens(a, b) - j * P);
-        int8_t* out = a.bounds + page_head * 2 * D;
-        if constexpr (VEC) {
-            const int lanes = D / 8, at_once = 32 / lanes, r0 = lane / lanes, col = lane % lanes * 8;
-            constexpr int FLY = PREC == 0 ? 4 : 8;
-            float lo[8], hi[8];
+        all = __shfl_sync(0xffffffffu, before, 31);
+        before -= mine;
+    } else {
+        s.prepare(a);
+        all = s.total();
+    }
+    const int64_t items = all * H, warp = (int64_t)blockIdx.x * (kBoundsThreads / 32) + (threadIdx.x >> 5);
+    const int64_t warps = (int64_t)gridDim.x * (kBoundsThreads / 32);
+    const int64_t each = items < warps ? 0 : items >> 32 ? items / warps : (uint32_t)items / (uint32_t)warps, more = items - each * warps;
+    const int64_t i0 = each * warp + min(warp, more), i1 = i0 + each + (warp < more);
+    if (i0 >= i1) return;
+    const int64_t page0 = i0 >> 32 ? i0 / H : (uint32_t)i0 / (uint32_t)H;
+    int b = 0, j = 0, h = (int)(i0 - page0 * H), left = 0, rows = 0;   // left: pages of the sequence from this one on
+    int64_t page = -1;
+    auto take_page = [&]() {
+        const int64_t first_row = pool_row(a.pool, b, (int64_t)j * P);
+        if (first_row < 0 && a.error_flag) atomicExch(a.error_flag, 1);
+        page = first_row < 0 ? -1 : first_row >> 32 ? first_row / P : (uint32_t)first_row / (uint32_t)P;   // counted in (page, head) blocks
+        rows = min(P, TouchedPages::tokens(a, b) - j * P);
+    };
+    if (few) {
+        b = 31 - __clz(__ballot_sync(0xffffffffu, mine > 0 && before <= page0));   // (the last sequence with pages that starts there or before)
+        j = TouchedPages::first(a, b) + (int)(page0 - __shfl_sync(0xffffffffu, before, b));
+    } else {
+        s.find(a, page0, b, j);
+    }
+    left = TouchedPages::first(a, b) + TouchedPages::count(a, b) - j;
+    take_page();
+    for (int64_t item = i0;;) {
+        if (page >= 0) {
+            const int64_t page_head = page + h, row = page_head * P;
+            int8_t* out = a.bounds + page_head * 2 * D;
+            if constexpr (VEC) {
+                const int lanes = D / 8, at_once = 32 / lanes, r0 = lane / lanes, col = lane % lanes * 8;
+                constexpr int FLY = PREC == 0 ? 4 : 8;
+                Extremes<PREC> x;
+                x.start();
+                // (a row that is not there is read as the page's first again: its values change nothing)
+                for (int r = 0; r < rows; r += FLY * at_once) {
+                    PoolRaw<PREC, 8> y[FLY];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                lo[i] = INFINITY;
-                hi[i] = -INFINITY;
-            }
-            // (a row that is not there is read as the page's first again: its values change nothing)
-            for (int r = 0; r < rows; r += FLY * at_once) {
-                PoolRaw<PREC, 8> x[FLY];
+                    for (int f = 0; f < FLY; ++f) {
+                        const int mine = r + f * at_once + r0;
+                        y[f].load(a.pool, false, row + (r0 < at_once && mine < rows ? mine : 0), col);
+                    }
 #pragma unroll
-                for (int f = 0; f < FLY; ++f) {
-                    const int mine = r + f * at_once + r0;
-                    x[f].load(a.pool, false, row + (r0 < at_once && mine < rows ? mine : 0), col);
+                    for (int f = 0; f < FLY; ++f) x.add(y[f]);
                 }
+                for (int g = 1; g < at_once; ++g) x.join((lane + g * lanes) % (at_once * lanes));   // (lanes behind the groups: unused)
+                float top = 0.0f;
 #pragma unroll
-                for (int f = 0; f < FLY; ++f)
+                for (int i = 0; i < 8; ++i) top = max_nan(top, max_nan(fabsf(x.low(i)), fabsf(x.high(i))));
+                top = warp_max_nan(top);
+                const bool finite = top < INFINITY;
+                const int e = finite ? step_exp(top) : 127;
+                const float inverse = exp_of(254 - e);
+                // the first group of lanes writes the lows, the second the highs; one group writes both
+                for (int side = r0 >= at_once ? 2 : at_once > 1 ? r0 : 0; side < 2; side += at_once > 1 ? 2 : 1) {
+                    uint32_t w[2] = {0, 0};
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const float y = x[f].get(i);
-                        lo[i] = min_nan(lo[i], y);
-                        hi[i] = max_nan(hi[i], y);
+                        const int n = down(side ? -x.high(i) : x.low(i), inverse);
+                        w[i / 4] |= (uint32_t)((side ? -n : n) & 255) << (8 * (i % 4));
                     }
-            }
-            float top = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                for (int g = 1; g < at_once; ++g) {   // (lanes from `lanes` on end with what no one uses)
-                    lo[i] = min_nan(lo[i], __shfl_sync(0xffffffffu, lo[i], col / 8 + g * lanes));
-                    hi[i] = max_nan(hi[i], __shfl_sync(0xffffffffu, hi[i], col / 8 + g * lanes));
+                    *reinterpret_cast<uint2*>(out + side * D + col) = finite ? make_uint2(w[0], w[1]) : make_uint2(0, 0);
                 }
-                top = max_nan(top, max_nan(fabsf(lo[i]), fabsf(hi[i])));
-            }
-            top = warp_max_nan(top);
-            const bool finite = top < INFINITY;
-            const int e = finite ? step_exp(top) : 127;
-            const float inverse = exp_of(254 - e);
-            if (lane < lanes) {
-                uint32_t w[2][2] = {{0, 0}, {0, 0}};
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (!finite) continue;
-                    w[0][i / 4] |= (uint32_t)(down(lo[i], inverse) & 255) << (8 * (i % 4));
-                    w[1][i / 4] |= (uint32_t)(up(hi[i], inverse) & 255) << (8 * (i % 4));
+                if (lane == 0) a.steps[page_head] = finite ? exp_of(e) : INFINITY;
+            } else {
+                float top = 0.0f;
+                for (int r = 0; r < rows; ++r)
+                    for (int d = lane; d < D; d += 32)
+                        top = max_nan(top, fabsf(pool_value<PREC>(a.pool, false, row + r, d, PREC == 3 ? d / a.pool.int4_group : 0)));
+                top = warp_max_nan(top);
+                const bool finite = top < INFINITY;
+                const int e = finite ? step_exp(top) : 127;
+                const float inverse = exp_of(254 - e);
+                for (int d = lane; d < D; d += 32) {
+                    float lo = INFINITY, hi = -INFINITY;
+                    for (int r = 0; r < rows; ++r) {
+                        const float y = pool_value<PREC>(a.pool, false, row + r, d, PREC == 3 ? d / a.pool.int4_group : 0);
+                        lo = fminf(lo, y);
+                        hi = fmaxf(hi, y);
+                    }
+                    out[d] = (int8_t)(finite ? down(lo, inverse) : 0);
+                    out[D + d] = (int8_t)(finite ? up(hi, inverse) : 0);
                 }
-                *reinterpret_cast<uint2*>(out + col) = make_uint2(w[0][0], w[0][1]);
-                *reinterpret_cast<uint2*>(out + D + col) = make_uint2(w[1][0], w[1][1]);
+                if (lane == 0) a.steps[page_head] = finite ? exp_of(e) : INFINITY;
             }
-            if (lane == 0) a.steps[page_head] = finite ? exp_of(e) : INFINITY;
-        } else {
-            float top = 0.0f;
-            for (int r = 0; r < rows; ++r)
-                for (int d = lane; d < D; d += 32)
-                    top = max_nan(top, fabsf(pool_value<PREC>(a.pool, false, row + r, d, PREC == 3 ? d / a.pool.int4_group : 0)));
-            top = warp_max_nan(top);
-            const bool finite = top < INFINITY;
-            const int e = finite ? step_exp(top) : 127;
-            const float inverse = exp_of(254 - e);
-            for (int d = lane; d < D; d += 32) {
-                float lo = INFINITY, hi = -INFINITY;
-                for (int r = 0; r < rows; ++r) {
-                    const float y = pool_value<PREC>(a.pool, false, row + r, d, PREC == 3 ? d / a.pool.int4_group : 0);
-                    lo = fminf(lo, y);
-                    hi = fmaxf(hi, y);
-                }
-                out[d] = (int8_t)(finite ? down(lo, inverse) : 0);
-                out[D + d] = (int8_t)(finite ? up(hi, inverse) : 0);
-            }
-            if (lane == 0) a.steps[page_head] = finite ? exp_of(e) : INFINITY;
         }
+        if (++item >= i1) break;
+        if (++h < H) continue;
+        h = 0;
+        if (--left > 0) {
+            ++j;
+        } else {
+            do ++b; while ((left = TouchedPages::count(a, b)) == 0);
+            j = TouchedPages::first(a, b);
+        }
+        take_page();
     }
 }
 
