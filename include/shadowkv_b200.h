@@ -535,7 +535,7 @@ typedef struct skv_pool_select_args {
  * query heads that share the key head, of t * step * sum_d n_d (n_d > 0 ? highs_d : lows_d) with n = rint(q / t) and
  * t the least power of two of which 127 reach max |q| (a query row that is not finite scores 0).  The sum is exact.  A page
  * whose step is not finite comes before all others, one that the table does not name behind.
- * scratch: skv_pool_select_scratch_bytes bytes, 16-byte aligned. */
+ * scratch: skv_pool_select_scratch_bytes bytes, 16-byte aligned; calls that may overlap on the GPU use scratch of their own. */
 size_t skv_pool_select_scratch_bytes(int batch, int heads, int S_q, int table_width);
 int skv_pool_select(const skv_pool_select_args* args, void* stream);
 

@@ -298,26 +298,39 @@ __device__ __forceinline__ uint32_t score_key(float dot, float t, float step) {
     return score_bits(step < INFINITY ? __fmul_rn(__fmul_rn(dot, t), step) : INFINITY);
 }
 
-// Query rows n = rint(q / t) as [min(n, 0) (D), max(n, 0) (D)], put(place, n) for each place, and t; a warp a row.
-// Returns the sum of all n.
-template <class T, class Put>
-__device__ __forceinline__ int whole_query(const T* q, int D, Put put, float* t_out) {
+// A query row n = rint(q / t) as [min(n, 0) (D), max(n, 0) (D)], put(place, n) for each place, and t; a warp a row, N values a lane
+// that are loaded first.  Returns the sum of all n.
+template <int N, class T>
+__device__ __forceinline__ void load_query(const T* q, int D, float (&x)[N]) {
     const int lane = threadIdx.x & 31;
-    float top = 0.0f;
-    for (int d = lane; d < D; d += 32) top = max_nan(top, fabsf(to_float(q[d])));
-    top = warp_max_nan(top);
+#pragma unroll
+    for (int k = 0; k < N; ++k) x[k] = 32 * k + lane < D ? to_float(q[32 * k + lane]) : 0.0f;
+}
+template <int N, class Put>
+__device__ __forceinline__ int whole_query(const float (&x)[N], int D, float top, Put put, float* t_out) {
+    const int lane = threadIdx.x & 31;
     const bool finite = top < INFINITY;
     const int e = finite ? step_exp(top) : 127;
     const float inverse = exp_of(254 - e);
     int sum = 0;
-    for (int d = lane; d < D; d += 32) {
-        const int n = finite ? (int)rintf(__fmul_rn(to_float(q[d]), inverse)) : 0;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int d = 32 * k + lane;
+        if (d >= D) continue;
+        const int n = finite ? (int)rintf(__fmul_rn(x[k], inverse)) : 0;
         sum += n;
         put(d, min(n, 0));
         put(D + d, max(n, 0));
     }
     if (lane == 0) *t_out = exp_of(e);
-    return __reduce_add_sync(0xffffffffu, sum);
+    return sum;
+}
+template <int N>
+__device__ __forceinline__ float largest_of(const float (&x)[N]) {
+    float top = 0.0f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) top = max_nan(top, fabsf(x[k]));
+    return warp_max_nan(top);
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -325,7 +338,10 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-constexpr int kScoreWarps = 8, kScoreTiles = 4;   // column tiles of 8 that a block takes
+constexpr int kSelectWarps = 8, kSelectThreads = 32 * kSelectWarps, kScoreTiles = 4;   // column tiles of 8 that a block takes
+constexpr int kSelectCluster = 8;       // most blocks that share a (sequence, key head)
+constexpr int kSelectKeys = 4096;        // keys that a block keeps in shared memory
+
 
 // Scores of 16 pages a warp for the columns of a block.  Columns are (new token, query head): the rep heads of a token fill
 // `span` (a power of two up to 8) of them, the head repeated in those that are over, so that the largest of a token
@@ -333,116 +349,133 @@ constexpr int kScoreWarps = 8, kScoreTiles = 4;   // column tiles of 8 that a bl
 // of pages g and g + 8.  A byte x becomes an fp16 operand by its place alone: the bits of x + 128 are those of the subnormal
 // (x + 128) 2^-24, so an MMA over a word of 4 bytes a lane gives 2^-24 (n . x + 128 sum n), exactly (at most 255 * 127 * 256 < 2^23 of
 // these units); the accumulators start at what is too much.  (Integer MMAs are not native here.)
+// A call of one token runs through this once, so the time is latency, that of fetching the instructions too: loops are left rolled
+// where their bodies follow one another anyway, and the pages' loads stand in one place, an iteration ahead of their use, the first
+// ones on their way while the queries are laid out.
 template <class T, int SEGS>
-__global__ void __launch_bounds__(32 * kScoreWarps) page_scores_kernel(const __grid_constant__ skv_pool_select_args a, int span) {
-    extern __shared__ __align__(16) __half s_raw[];
-    __half* s_q = s_raw;                                          // [columns][64 * SEGS + 8], the bytes 0, 2, 1, 3 of each word
-    __shared__ float s_t[8 * kScoreTiles], s_start[8 * kScoreTiles];
+__device__ __forceinline__ void score_pages(const skv_pool_select_args& a, int log_span, int b, int h, int pages, int i0, int block_tokens,
+                                            __half* s_q, float* s_t, float* s_start, uint32_t* keys, int pitch) {
     constexpr int BYTES = 64 * SEGS, PITCH = BYTES + 8;
-    const int D = a.head_dim, H = a.heads, rep = a.q.heads / H, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int b = blockIdx.z / H, h = blockIdx.z % H;
-    const int pages = (select_tokens(a, b) + a.page_size - 1) / a.page_size;
-    if (pages <= a.keep || blockIdx.x * kScoreWarps * 16 >= pages) return;   // (all are kept, or none here)
-    const int head_tiles = (rep + span - 1) / span;               // tiles of a token (1 unless rep > 8)
-    const int block_tokens = head_tiles > 1 ? 1 : 8 * kScoreTiles / span;
-    const int i0 = blockIdx.y * block_tokens;
+    const int D = a.head_dim, H = a.heads, rep = a.q.heads / H, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, span = 1 << log_span;
+    const int head_tiles = (rep + span - 1) >> log_span;          // tiles of a token (1 unless rep > 8)
+    const int g = lane >> 2, c = lane & 3;
+    const int32_t* table = a.block_table + b * a.table_stride;
+    const int p_first = (blockIdx.x * kSelectWarps + warp) * 16, p_step = gridDim.x * kSelectWarps * 16;
     for (int first = 0; first < head_tiles; first += kScoreTiles) {
         // (further rounds are for more than 8 * kScoreTiles heads only: their largest joins what is written already)
         const int tiles = head_tiles > 1 ? min(kScoreTiles, head_tiles - first)
-                                         : (min(block_tokens, a.S_q - i0) * span + 7) / 8;
-        __syncthreads();
-        for (int col = warp; col < 8 * tiles; col += kScoreWarps) {
-            const int i = head_tiles > 1 ? i0 : min(a.S_q - 1, i0 + col / span);
-            int head = head_tiles > 1 ? 8 * first + col : col % span;
-            if (head >= rep) head = rep - 1;
-            __half* to = s_q + col * PITCH;
-            for (int p = 2 * D + lane; p < BYTES; p += 32) to[p] = __float2half_rn(0.0f);   // (whole words: D is a multiple of 8)
-            const int sum = whole_query(
-                static_cast<const T*>(a.q.ptr) + b * a.q.stride_b + (int64_t)(h * rep + head) * a.q.stride_h + i * a.q.stride_s, D,
-                [&](int p, int n) { to[(p & ~3) + (p & 1) * 2 + (p >> 1 & 1)] = __int2half_rn(n); }, s_t + col);
-            if (lane == 0) s_start[col] = -128.0f * (float)sum * 0x1p-24f;
-        }
-        __syncthreads();
-        const int g = lane >> 2, c = lane & 3;
-        for (int p0 = (blockIdx.x * kScoreWarps + warp) * 16; p0 < pages; p0 += gridDim.x * kScoreWarps * 16) {
-            uint4 x[2][SEGS];
+                                         : ((min(block_tokens, a.S_q - i0) << log_span) + 7) / 8;
+        int ahead[2];                                             // numbers of the pages that are loaded next
+#pragma unroll
+        for (int r = 0; r < 2; ++r) ahead[r] = p_first + g + 8 * r < pages ? __ldg(table + p_first + g + 8 * r) : -1;
+        uint4 next[2][SEGS];
+        float next_step[2] = {1.0f, 1.0f};
+        bool next_named[2] = {false, false};
+        if (first > 0) __syncthreads();
+#pragma unroll 1
+        for (int p0 = p_first - p_step; p0 < pages; p0 += p_step) {
+            uint32_t y[2][4 * SEGS];
             float step[2];
             bool named[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const int j = p0 + g + 8 * r;
-                const int page = j < pages ? __ldg(a.block_table + b * a.table_stride + j) : -1;
-                named[r] = page >= 0 && page < a.num_pages;
-                if (j < pages && !named[r] && a.error_flag) atomicExch(a.error_flag, 1);
-                const int64_t at = named[r] ? (int64_t)page * H + h : 0;
-                step[r] = named[r] ? __ldg(a.steps + at) : 1.0f;
-                const uint4* row = reinterpret_cast<const uint4*>(a.bounds + at * 2 * D);
 #pragma unroll
-                for (int s = 0; s < SEGS; ++s)
-                    x[r][s] = named[r] && 64 * s + 16 * c < 2 * D ? __ldg(row + 4 * s + c) : make_uint4(0, 0, 0, 0);
+                for (int s = 0; s < SEGS; ++s) {
+                    y[r][4 * s] = next[r][s].x; y[r][4 * s + 1] = next[r][s].y; y[r][4 * s + 2] = next[r][s].z; y[r][4 * s + 3] = next[r][s].w;
+                }
+                step[r] = next_step[r];
+                named[r] = next_named[r];
+                const int j = p0 + p_step + g + 8 * r, page = ahead[r];
+                next_named[r] = j < pages && page >= 0 && page < a.num_pages;
+                if (j < pages && !next_named[r] && a.error_flag) atomicExch(a.error_flag, 1);
+                ahead[r] = j + p_step < pages ? __ldg(table + j + p_step) : -1;
+                if (next_named[r]) {
+                    const int64_t at = (int64_t)page * H + h;
+                    const int8_t* row = a.bounds + at * (2 * D) + 16 * c;
+                    next_step[r] = __ldg(a.steps + at);
+#pragma unroll
+                    for (int s = 0; s < SEGS; ++s)
+                        next[r][s] = 64 * s + 16 * c < 2 * D ? __ldg(reinterpret_cast<const uint4*>(row + 64 * s)) : make_uint4(0, 0, 0, 0);
+                }
+            }
+            if (p0 < p_first) {                                   // nothing to score yet
+#pragma unroll 1
+                for (int col = warp; col < 8 * tiles; col += kSelectWarps) {
+                    const int i = head_tiles > 1 ? i0 : min(a.S_q - 1, i0 + (col >> log_span));
+                    const int head = min(rep - 1, head_tiles > 1 ? 8 * first + col : col & (span - 1));
+                    float x[SEGS];
+                    load_query(static_cast<const T*>(a.q.ptr) + b * a.q.stride_b + (int64_t)(h * rep + head) * a.q.stride_h + i * a.q.stride_s, D, x);
+                    __half* to = s_q + col * PITCH;
+#pragma unroll 1
+                    for (int p = 2 * D + lane; p < BYTES; p += 32) to[p] = __float2half_rn(0.0f);   // (whole words: D is a multiple of 8)
+                    const int sum = __reduce_add_sync(0xffffffffu, whole_query(x, D, largest_of(x),
+                        [&](int p, int n) { to[(p & ~3) + (p & 1) * 2 + (p >> 1 & 1)] = __int2half_rn(n); }, s_t + col));
+                    if (lane == 0) s_start[col] = -128.0f * (float)sum * 0x1p-24f;
+                }
+                __syncthreads();
+                continue;
             }
             float best[2] = {-INFINITY, -INFINITY};               // more than 8 heads
+#pragma unroll 1
             for (int t = 0; t < tiles; ++t) {
                 const float at0 = s_start[8 * t + 2 * c], at1 = s_start[8 * t + 2 * c + 1];
-                float acc[4] = {at0, at1, at0, at1};
+                float acc[2][4] = {{at0, at1, at0, at1}, {}};     // (chains of their own: whole numbers add up in any order)
                 const __half* column = s_q + (8 * t + g) * PITCH + 16 * c;
 #pragma unroll
                 for (int s = 0; s < SEGS; ++s) {
-                    const uint4 y0 = *reinterpret_cast<const uint4*>(column + 64 * s), y1 = *reinterpret_cast<const uint4*>(column + 64 * s + 8);
-                    const uint32_t u[4] = {x[0][s].x, x[0][s].y, x[0][s].z, x[0][s].w}, v[4] = {x[1][s].x, x[1][s].y, x[1][s].z, x[1][s].w};
-                    const uint32_t y[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
+                    const uint4 z0 = *reinterpret_cast<const uint4*>(column + 64 * s), z1 = *reinterpret_cast<const uint4*>(column + 64 * s + 8);
+                    const uint32_t z[8] = {z0.x, z0.y, z0.z, z0.w, z1.x, z1.y, z1.z, z1.w};
 #pragma unroll
-                    for (int w = 0; w < 4; ++w)
-                        mma_f16(acc, (u[w] & 0x00FF00FFu) ^ 0x00800080u, (v[w] & 0x00FF00FFu) ^ 0x00800080u,
-                                ((u[w] >> 8) & 0x00FF00FFu) ^ 0x00800080u, ((v[w] >> 8) & 0x00FF00FFu) ^ 0x00800080u, y[2 * w], y[2 * w + 1]);
+                    for (int w = 0; w < 4; ++w) {
+                        const uint32_t u = y[0][4 * s + w], v = y[1][4 * s + w];
+                        mma_f16(acc[w & 1], (u & 0x00FF00FFu) ^ 0x00800080u, (v & 0x00FF00FFu) ^ 0x00800080u,
+                                ((u >> 8) & 0x00FF00FFu) ^ 0x00800080u, ((v >> 8) & 0x00FF00FFu) ^ 0x00800080u, z[2 * w], z[2 * w + 1]);
+                    }
                 }
                 // columns 2 c and 2 c + 1 of pages g (acc 0, 1) and g + 8
-                const float t0 = s_t[8 * t + 2 * c], t1 = s_t[8 * t + 2 * c + 1];
+                const float t0 = s_t[8 * t + 2 * c] * 0x1p24f, t1 = s_t[8 * t + 2 * c + 1] * 0x1p24f;
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    float u = __fmul_rn(acc[2 * r] * 0x1p24f, t0), v = __fmul_rn(acc[2 * r + 1] * 0x1p24f, t1);
-                    if (span > 1) u = v = fmaxf(u, v);
-                    if (span > 2) u = v = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, 1));
-                    if (span > 4) u = v = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, 2));
+                    float u = __fmul_rn(acc[0][2 * r] + acc[1][2 * r], t0), v = __fmul_rn(acc[0][2 * r + 1] + acc[1][2 * r + 1], t1);
+                    if (span > 1) u = fmaxf(u, v);
+                    if (span > 2) u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, 1));
+                    if (span > 4) u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, 2));
                     const int j = p0 + g + 8 * r;
                     if (head_tiles > 1) {
                         best[r] = fmaxf(best[r], u);
                         if (t + 1 < tiles) continue;
-                        u = v = best[r];
+                        u = best[r];
                     }
-                    if (j >= pages) continue;
-                    const int i_u = head_tiles > 1 ? i0 : i0 + (8 * t + 2 * c) / span, i_v = i0 + (8 * t + 2 * c + 1) / span;
-                    uint32_t* keys = static_cast<uint32_t*>(a.scratch) + ((int64_t)blockIdx.z * a.S_q) * a.table_width + j;
-                    if ((head_tiles > 1 ? c == 0 : 2 * c % span == 0) && i_u < a.S_q) {
-                        uint32_t key = named[r] ? score_key(u, 1.0f, step[r]) : 0;
-                        if (first > 0) key = max(key, keys[(int64_t)i_u * a.table_width]);
-                        keys[(int64_t)i_u * a.table_width] = key;
+                    // each lane that has a token's largest writes it, two where a token is a column
+                    const int writers = head_tiles > 1 ? 3 : span > 1 ? (span >> 1) - 1 : 0;
+                    if (j >= pages || (c & writers)) continue;
+                    const int i = head_tiles > 1 ? i0 : i0 + ((8 * t + 2 * c) >> log_span);
+                    uint32_t* to = keys + (int64_t)i * pitch + j;
+                    if (i < a.S_q) {
+                        const uint32_t key = named[r] ? score_key(u, 1.0f, step[r]) : 1;
+                        to[0] = first > 0 ? max(key, to[0]) : key;
                     }
-                    if (span == 1 && i_v < a.S_q) keys[(int64_t)i_v * a.table_width] = named[r] ? score_key(v, 1.0f, step[r]) : 0;
+                    if (span == 1 && i + 1 < a.S_q) to[pitch] = named[r] ? score_key(v, 1.0f, step[r]) : 1;
                 }
             }
         }
     }
 }
 
-// Heads that are not whole 16-byte rows of bounds, or above 256 values: a warp a page and column.
+// Heads that are not whole 16-byte rows of bounds, or above 256 values: a warp a page, a column at a time.
 template <class T>
-__global__ void __launch_bounds__(32 * kScoreWarps) page_scores_any_kernel(const __grid_constant__ skv_pool_select_args a) {
-    extern __shared__ __align__(16) __half s_raw[];
-    int8_t* s_q = reinterpret_cast<int8_t*>(s_raw);               // [2 D]
-    __shared__ float s_t;
+__device__ __forceinline__ void score_pages_any(const skv_pool_select_args& a, int b, int h, int pages, int i, int8_t* s_q, float* s_t,
+                                                uint32_t* keys, int pitch) {
     const int D = a.head_dim, H = a.heads, rep = a.q.heads / H, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int b = blockIdx.z / H, h = blockIdx.z % H, i = blockIdx.y;
-    const int pages = (select_tokens(a, b) + a.page_size - 1) / a.page_size;
-    if (pages <= a.keep) return;
-    uint32_t* keys = static_cast<uint32_t*>(a.scratch) + ((int64_t)blockIdx.z * a.S_q + i) * a.table_width;
     for (int head = 0; head < rep; ++head) {
         __syncthreads();
-        if (warp == 0)
-            whole_query(static_cast<const T*>(a.q.ptr) + b * a.q.stride_b + (int64_t)(h * rep + head) * a.q.stride_h + i * a.q.stride_s, D,
-                        [&](int p, int n) { s_q[p] = (int8_t)n; }, &s_t);
+        if (warp == 0) {
+            float x[32];                                          // (of up to 1024 values)
+            load_query<32>(static_cast<const T*>(a.q.ptr) + b * a.q.stride_b + (int64_t)(h * rep + head) * a.q.stride_h + i * a.q.stride_s, D, x);
+            whole_query(x, D, largest_of(x), [&](int p, int n) { s_q[p] = (int8_t)n; }, s_t);
+        }
         __syncthreads();
-        for (int j = blockIdx.x * kScoreWarps + warp; j < pages; j += gridDim.x * kScoreWarps) {
+        for (int j = blockIdx.x * kSelectWarps + warp; j < pages; j += gridDim.x * kSelectWarps) {
             const int page = __ldg(a.block_table + b * a.table_stride + j);
             const bool named = page >= 0 && page < a.num_pages;
             if (!named && lane == 0 && a.error_flag) atomicExch(a.error_flag, 1);
@@ -452,124 +485,262 @@ __global__ void __launch_bounds__(32 * kScoreWarps) page_scores_any_kernel(const
                 for (int d = lane; d < 2 * D; d += 32) sum += (int)s_q[d] * (int)__ldg(a.bounds + at * 2 * D + d);
             sum = __reduce_add_sync(0xffffffffu, sum);
             if (lane == 0) {
-                const uint32_t key = named ? score_key((float)sum, s_t, __ldg(a.steps + at)) : 0;
-                keys[j] = head == 0 ? key : max(keys[j], key);
+                const uint32_t key = named ? score_key((float)sum, *s_t, __ldg(a.steps + at)) : 1;
+                keys[(int64_t)i * pitch + j] = head == 0 ? key : max(key, keys[(int64_t)i * pitch + j]);
             }
         }
     }
 }
 
 // ---------------------------------------------------------------------------------------- the choice
-constexpr int kSelectThreads = 256, kSelectHeld = 8;   // keys that a thread keeps in registers
+constexpr int kSelectBins = 2048, kSelectList = 256;
 
-// A block a (sequence, key head, new token).  The want-th largest key is found bit by bit (how many keys are at least a
-// candidate), then the pages above it, and the first of those equal to it, are listed in order.
-__global__ void __launch_bounds__(kSelectThreads) page_select_kernel(const __grid_constant__ skv_pool_select_args a) {
-    __shared__ int s_count[3], s_part[2][kSelectThreads / 32];
-    __shared__ uint32_t s_min[kSelectThreads / 32], s_max[kSelectThreads / 32];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t unit = blockIdx.x;
-    const int i = (int)(unit % a.S_q), b = (int)(unit / a.S_q / a.heads);
-    const int pages = select_pages(a, b, i);
-    int32_t* out = a.pages + unit * a.keep;
-    if (tid == 0 && a.error_flag && __ldg(a.lengths + b) != select_tokens(a, b)) atomicExch(a.error_flag, 1);
-    if (pages <= a.keep) {
-        for (int k = tid; k < a.keep; k += kSelectThreads) out[k] = k < pages ? k : -1;
-        return;
+struct SelectShared {                       // of a block, or a part of each array for each warp
+    int bins[kSelectBins];
+    uint32_t keys[kSelectKeys];
+    uint32_t list[kSelectList];             // keys of one bin and their pages
+    int page[kSelectList];
+    uint32_t bits[kSelectKeys / 32];        // pages that are taken, and how many before each word
+    int before[kSelectKeys / 32];
+    int part[2][kSelectWarps];
+    uint32_t least[kSelectWarps], most[kSelectWarps];
+    int bin[kSelectWarps], above[kSelectWarps], inside[kSelectWarps], listed[kSelectWarps];
+    uint32_t cut_key[kSelectWarps];
+    int cut_page[kSelectWarps];
+};
+
+// Of the keys of pages [lo, hi), more than `want` > 0, the `want` largest, equal ones from the lowest page on, listed in order.
+// WARPS warps together: all of the block, or each warp by itself.  The range of the keys is cut into bins; the bin in which the
+// want-th largest lies holds a few keys, which are ranked one by one.  Where it holds many (equal scores), the want-th
+// largest key, and the page up to which equal ones are taken, are found by halving their ranges instead.
+template <int WARPS>
+__device__ __forceinline__ void choose_pages(SelectShared& s, const uint32_t* global, int lo, int hi, int want, int32_t* out, int tid) {
+    constexpr int THREADS = 32 * WARPS, SHARE = kSelectWarps / WARPS;   // of the arrays
+    constexpr int BINS = kSelectBins / SHARE, LIST = kSelectList / SHARE, KEYS = kSelectKeys / SHARE, EACH = BINS / THREADS;
+    const int lane = tid & 31, warp = tid >> 5, w0 = WARPS > 1 ? 0 : threadIdx.x >> 5;   // w0: the warp's own part
+    int* bins = s.bins + w0 * BINS;
+    uint32_t* list = s.list + w0 * LIST;
+    int* listed_page = s.page + w0 * LIST;
+    auto sync = [] {
+        if constexpr (WARPS > 1) __syncthreads();
+        else __syncwarp();
+    };
+    const bool kept = hi - lo <= KEYS;
+    const uint32_t* keys = kept ? s.keys + w0 * KEYS - lo : global;
+    uint32_t least = 0xffffffffu, most = 0;
+#pragma unroll 4
+    for (int j = lo + tid; j < hi; j += THREADS) {
+        const uint32_t x = __ldcg(global + j);
+        if (kept) s.keys[w0 * KEYS + j - lo] = x;
+        least = min(least, x);
+        most = max(most, x);
     }
-    const int lo = a.first, hi = pages - a.recent, want = a.keep - a.first - a.recent;   // of the pages [lo, hi), more than want
-    const uint32_t* keys = static_cast<const uint32_t*>(a.scratch) + unit * a.table_width;
-    for (int k = tid; k < a.first; k += kSelectThreads) out[k] = k;
-    for (int k = tid; k < a.recent; k += kSelectThreads) out[a.keep - a.recent + k] = hi + k;
-    if (want == 0) return;
-    uint32_t held[kSelectHeld], least = 0xffffffffu, most = 0;
-    const bool all = hi - lo <= kSelectThreads * kSelectHeld;
-    if (all) {
 #pragma unroll
-        for (int k = 0; k < kSelectHeld; ++k) {
-            const int j = lo + tid + k * kSelectThreads;
-            held[k] = j < hi ? keys[j] : 0;
-            if (j < hi) { least = min(least, held[k]); most = max(most, held[k]); }
-        }
-    } else {
-        for (int j = lo + tid; j < hi; j += kSelectThreads) { least = min(least, keys[j]); most = max(most, keys[j]); }
-    }
+    for (int i = 0; i < EACH; i += 4) *reinterpret_cast<int4*>(bins + EACH * tid + i) = make_int4(0, 0, 0, 0);
+    if (tid == 0) s.listed[w0] = 0;
     least = __reduce_min_sync(0xffffffffu, least);
     most = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 0) { s_min[warp] = least; s_max[warp] = most; }
-    if (tid < 3) s_count[tid] = 0;
-    __syncthreads();
-    for (int w = 0; w < kSelectThreads / 32; ++w) { least = min(least, s_min[w]); most = max(most, s_max[w]); }
-    int round = 0;
-    auto count_from = [&](uint32_t x) {   // keys >= x; x > 0
-        int n = 0;
-        if (all) {
+    if constexpr (WARPS > 1)
+        if (lane == 0) { s.least[warp] = least; s.most[warp] = most; }
+    sync();
+    if constexpr (WARPS > 1) {
+        least = __reduce_min_sync(0xffffffffu, s.least[lane % WARPS]);
+        most = __reduce_max_sync(0xffffffffu, s.most[lane % WARPS]);
+    }
+    const int shift = max(0, 32 - __clz(most - least) - (31 - __clz(BINS)));
+#pragma unroll 1
+    for (int j = lo + tid; j < hi; j += THREADS) atomicAdd(bins + ((keys[j] - least) >> shift), 1);
+    sync();
+    // the bin from which on there are `want`: sums from the last bin down
+    int sum = 0;
 #pragma unroll
-            for (int k = 0; k < kSelectHeld; ++k) n += held[k] >= x;
+    for (int i = 0; i < EACH; i += 4) {
+        const int4 u = *reinterpret_cast<const int4*>(bins + EACH * tid + i);
+        sum += u.x + u.y + u.z + u.w;
+    }
+    int from = sum;                                                   // keys in this thread's bins and those above
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_down_sync(0xffffffffu, from, o);
+        if (lane + o < 32) from += x;
+    }
+    if constexpr (WARPS > 1) {
+        if (lane == 0) s.part[0][warp] = from;
+        sync();
+        from += __reduce_add_sync(0xffffffffu, lane > warp && lane < WARPS ? s.part[0][lane] : 0);
+    }
+    if (from >= want && from - sum < want) {                          // one thread
+        int above = from - sum, i = EACH * tid + EACH - 1;
+        while (above + bins[i] < want) above += bins[i--];
+        s.bin[w0] = i;
+        s.above[w0] = above;
+        s.inside[w0] = bins[i];
+    }
+    sync();
+    const int bin = s.bin[w0], need = want - s.above[w0], inside = s.inside[w0];
+    uint32_t cut_key = least + ((uint32_t)bin << shift);              // taken: larger keys, and equal ones up to cut_page
+    int cut_page = 0x7fffffff;
+    if (inside > need && inside <= LIST) {
+#pragma unroll 1
+        for (int j = lo + tid; j < hi; j += THREADS) {
+            const uint32_t x = keys[j];
+            if ((int)((x - least) >> shift) != bin) continue;
+            const int to = atomicAdd(&s.listed[w0], 1);
+            list[to] = x;
+            listed_page[to] = j;
+        }
+        sync();
+#pragma unroll 1
+        for (int i = tid; i < inside; i += THREADS) {
+            const uint32_t x = list[i];
+            const int j = listed_page[i];
+            int rank = 0;
+#pragma unroll 1
+            for (int o = 0; o < inside; ++o) rank += list[o] > x || (list[o] == x && listed_page[o] < j);
+            if (rank == need - 1) { s.cut_key[w0] = x; s.cut_page[w0] = j; }
+        }
+        sync();
+        cut_key = s.cut_key[w0];
+        cut_page = s.cut_page[w0];
+    } else if (inside > need) {
+        int round = 0;
+        auto taken_with = [&](uint32_t x, int page) {                 // keys above x, and equal ones up to the page
+            int n = 0;
+#pragma unroll 1
+            for (int j = lo + tid; j < hi; j += THREADS) n += keys[j] > x || (keys[j] == x && j <= page);
+            n = __reduce_add_sync(0xffffffffu, n);
+            if constexpr (WARPS > 1) {
+                if (lane == 0) s.part[round & 1][warp] = n;
+                sync();
+                n = __reduce_add_sync(0xffffffffu, lane < WARPS ? s.part[round & 1][lane] : 0);
+                ++round;
+            }
+            return n;
+        };
+        sync();
+        uint32_t below = cut_key, over = most - cut_key >> shift ? cut_key + ((1u << shift) - 1) : most;   // the want-th largest is in [below, over]
+#pragma unroll 1
+        while (below < over) {
+            const uint32_t x = below + (over - below + 1) / 2;
+            if (taken_with(x, 0x7fffffff) >= want) below = x; else over = x - 1;
+        }
+        cut_key = below;
+        int first = lo, last = hi - 1;                                // the least page up to which, with the larger keys, there are `want`
+#pragma unroll 1
+        while (first < last) {
+            const int x = first + (last - first) / 2;
+            if (taken_with(cut_key, x) >= want) last = x; else first = x + 1;
+        }
+        cut_page = first;
+    }
+    // listed in order, KEYS pages at a time
+    uint32_t* bits = s.bits + w0 * (KEYS / 32);
+    int* before = s.before + w0 * (KEYS / 32);
+#pragma unroll 1
+    for (int base = lo; base < hi; base += KEYS) {
+        const int n = min(KEYS, hi - base);
+        auto takes = [&](int i) {
+            const uint32_t x = i < n ? keys[base + i] : 0;
+            return x > cut_key || (x == cut_key && i < n && base + i <= cut_page);
+        };
+#pragma unroll 1
+        for (int i = tid; i < (n + 31 & ~31); i += THREADS) {
+            const unsigned these = __ballot_sync(0xffffffffu, takes(i));
+            if (lane == 0) bits[i / 32] = these;
+        }
+        sync();
+        int at = 0;                                                   // taken in the words before this thread's (every warp adds up all)
+#pragma unroll 1
+        for (int w = 0; w < (n + 31) / 32; w += 32) {
+            const int mine = w + lane < (n + 31) / 32 ? __popc(bits[w + lane]) : 0;
+            int incl = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += x;
+            }
+            if (warp == 0 && w + lane < (n + 31) / 32) before[w + lane] = at + incl - mine;
+            at += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        sync();
+#pragma unroll 1
+        for (int i = tid; i < n; i += THREADS) {
+            const uint32_t word = bits[i / 32];
+            if (word >> (i & 31) & 1) out[before[i / 32] + __popc(word & ((1u << (i & 31)) - 1))] = base + i;
+        }
+        out += at;
+        sync();                                                       // (the memory is used again)
+    }
+}
+
+// A block scores a share of a (sequence, key head)'s pages for up to 32 columns of queries.  The blocks that share them are a cluster:
+// once all of its scores are there, each chooses for some of the queries.
+template <class T, int SEGS>
+__global__ void __launch_bounds__(kSelectThreads, SEGS == 8 ? 1 : 2) page_select_kernel(const __grid_constant__ skv_pool_select_args a, int log_span, int block_tokens) {
+    extern __shared__ __align__(16) __half s_raw[];               // SEGS: [columns][64 SEGS + 8], the bytes 0, 2, 1, 3 of each word; else [2 D] bytes
+    __shared__ float s_t[8 * kScoreTiles], s_start[8 * kScoreTiles];
+    SelectShared& s_choice = *reinterpret_cast<SelectShared*>(s_raw);   // (the queries are not needed any more then)
+    start_dependents();
+    wait_for_dependency();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, H = a.heads;
+    const int b = blockIdx.z / H, h = blockIdx.z % H, i0 = blockIdx.y * block_tokens, i1 = min(a.S_q, i0 + block_tokens);
+    const int pages = (select_tokens(a, b) + a.page_size - 1) / a.page_size, want = a.keep - a.first - a.recent;
+    const int pitch = a.table_width;
+    uint32_t* keys = static_cast<uint32_t*>(a.scratch) + (int64_t)blockIdx.z * a.S_q * pitch;
+    if (pages > a.keep && want > 0) {
+        if constexpr (SEGS > 0) score_pages<T, SEGS>(a, log_span, b, h, pages, i0, block_tokens, s_raw, s_t, s_start, keys, pitch);
+        else score_pages_any<T>(a, b, h, pages, i0, reinterpret_cast<int8_t*>(s_raw), s_t, keys, pitch);
+        if (gridDim.x > 1) {
+            asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+            asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         } else {
-            for (int j = lo + tid; j < hi; j += kSelectThreads) n += keys[j] >= x;
+            __syncthreads();
         }
-        n = __reduce_add_sync(0xffffffffu, n);
-        if (lane == 0 && n) atomicAdd(&s_count[round % 3], n);
-        if (tid == 0) s_count[(round + 1) % 3] = 0;
-        __syncthreads();
-        return s_count[round++ % 3];
-    };
-    const int differ = 32 - __clz(least ^ most);                 // bits below those that all keys share
-    uint32_t at = differ == 32 ? 0 : most >> differ << differ;
-    bool exact = false;                                          // as many keys are at least `at` as are wanted
-    for (int bit = differ - 1; bit >= 0 && !exact; --bit) {
-        const uint32_t x = at | 1u << bit;
-        const int n = count_from(x);
-        if (n >= want) at = x;
-        exact = n == want;
     }
-    const int above = exact ? want : at == 0xffffffffu ? 0 : count_from(at + 1), ties = want - above;
-    int before = 0, equal_before = 0;                            // of the keys below those looked at
-    for (int j0 = lo, k = 0; j0 < hi; j0 += kSelectThreads, ++k) {
-        const int j = j0 + tid;
-        const uint32_t key = j < hi ? keys[j] : 0;
-        const bool over = j < hi && (exact ? key >= at : key > at), equal = j < hi && !exact && key == at;
-        const unsigned o = __ballot_sync(0xffffffffu, over), e = __ballot_sync(0xffffffffu, equal), mask = (1u << lane) - 1;
-        if (lane == 0) s_part[k & 1][warp] = __popc(o) | __popc(e) << 16;
-        __syncthreads();
-        int packed = 0, total = 0;
-        for (int w = 0; w < kSelectThreads / 32; ++w) {
-            if (w < warp) packed += s_part[k & 1][w];
-            total += s_part[k & 1][w];
+    if (tid == 0 && a.error_flag && __ldg(a.lengths + b) != select_tokens(a, b)) atomicExch(a.error_flag, 1);
+    const bool by_warp = i1 - i0 > 2 * (int)gridDim.x && pages <= kSelectKeys / kSelectWarps;
+    const int one_of = by_warp ? gridDim.x * kSelectWarps : gridDim.x, first_of = by_warp ? blockIdx.x * kSelectWarps + warp : blockIdx.x;
+    for (int i = i0 + first_of; i < i1; i += one_of) {
+        const int n = select_pages(a, b, i), step = by_warp ? 32 : kSelectThreads, me = by_warp ? lane : tid;
+        int32_t* out = a.pages + ((int64_t)blockIdx.z * a.S_q + i) * a.keep;
+        if (n <= a.keep) {
+            for (int k = me; k < a.keep; k += step) out[k] = k < n ? k : -1;
+            continue;
         }
-        const int o_before = before + (packed & 0xffff) + __popc(o & mask), e_before = equal_before + (packed >> 16) + __popc(e & mask);
-        if (over || (equal && e_before < ties)) out[a.first + o_before + min(e_before, ties)] = j;
-        before += total & 0xffff;
-        equal_before += total >> 16;
+        for (int k = me; k < a.first; k += step) out[k] = k;
+        for (int k = me; k < a.recent; k += step) out[a.keep - a.recent + k] = n - a.recent + k;
+        if (want == 0) continue;
+        if (by_warp) choose_pages<1>(s_choice, keys + (int64_t)i * pitch, a.first, n - a.recent, want, out + a.first, lane);
+        else choose_pages<kSelectWarps>(s_choice, keys + (int64_t)i * pitch, a.first, n - a.recent, want, out + a.first, tid);
     }
+}
+
+template <class T, int SEGS>
+int launch_select_kernel(const skv_pool_select_args& a, int log_span, int block_tokens, size_t smem, cudaStream_t st) {
+    const int groups = a.batch * a.heads, y = (a.S_q + block_tokens - 1) / block_tokens;
+    // as many blocks as fill the GPU, no more than there are shares and a cluster has
+    const int share = SEGS > 0 ? 16 * kSelectWarps : 8 * kSelectWarps;
+    const int64_t all = (int64_t)groups * y, fill = (2ll * sm_count() + all - 1) / all;
+    if (smem < sizeof(SelectShared)) smem = sizeof(SelectShared);
+    int x = (a.table_width + share - 1) / share;
+    if (x > fill) x = (int)fill;
+    if (x > kSelectCluster) x = kSelectCluster;
+    if (x < 1) x = 1;
+    launch_cluster_after(page_select_kernel<T, SEGS>, dim3(x, y, groups), dim3(x), kSelectThreads, smem, st, a, log_span, block_tokens);
+    return check_launch("pool_select");
 }
 
 template <class T>
 int launch_select(const skv_pool_select_args& a, cudaStream_t st) {
-    const int D = a.head_dim, H = a.heads, rep = a.q.heads / H;
-    const int64_t groups = (int64_t)a.batch * H;
-    const bool vec = D % 8 == 0 && D <= 256 && (reinterpret_cast<uintptr_t>(a.bounds) & 15) == 0;
-    if (a.table_width > a.keep && a.keep > a.first + a.recent) {
-        if (vec) {
-            int span = 1;
-            while (span < rep && span < 8) span *= 2;
-            const int block_tokens = rep > 8 ? 1 : 8 * kScoreTiles / span;
-            const int chunks = (a.table_width + 16 * kScoreWarps - 1) / (16 * kScoreWarps);
-            const dim3 grid(chunks, (a.S_q + block_tokens - 1) / block_tokens, (unsigned)groups);
-            const int segs = D <= 64 ? 2 : D <= 128 ? 4 : 8;
-            const size_t smem = (size_t)8 * kScoreTiles * (64 * segs + 8) * sizeof(__half);
-            if (segs == 2) page_scores_kernel<T, 2><<<grid, 32 * kScoreWarps, smem, st>>>(a, span);
-            else if (segs == 4) page_scores_kernel<T, 4><<<grid, 32 * kScoreWarps, smem, st>>>(a, span);
-            else page_scores_kernel<T, 8><<<grid, 32 * kScoreWarps, smem, st>>>(a, span);
-        } else {
-            const dim3 grid((a.table_width + 8 * kScoreWarps - 1) / (8 * kScoreWarps), a.S_q, (unsigned)groups);
-            page_scores_any_kernel<T><<<grid, 32 * kScoreWarps, 2 * (size_t)D, st>>>(a);
-        }
-        if (const int rc = check_launch("pool_select")) return rc;
-    }
-    page_select_kernel<<<(unsigned)(groups * a.S_q), kSelectThreads, 0, st>>>(a);
-    return check_launch("pool_select");
+    const int D = a.head_dim, rep = a.q.heads / a.heads;
+    if (D % 8 || D > 256 || (reinterpret_cast<uintptr_t>(a.bounds) & 15)) return launch_select_kernel<T, 0>(a, 0, 1, 2 * (size_t)D, st);
+    int log_span = 0;
+    while (1 << log_span < rep && log_span < 3) ++log_span;
+    const int block_tokens = rep > 8 ? 1 : 8 * kScoreTiles >> log_span;
+    const auto smem = [](int segs) { return (size_t)8 * kScoreTiles * (64 * segs + 8) * sizeof(__half); };
+    if (D <= 64) return launch_select_kernel<T, 2>(a, log_span, block_tokens, smem(2), st);
+    if (D <= 128) return launch_select_kernel<T, 4>(a, log_span, block_tokens, smem(4), st);
+    return launch_select_kernel<T, 8>(a, log_span, block_tokens, smem(8), st);
 }
 
 }  // namespace skv
@@ -612,6 +783,7 @@ int skv_pool_select(const skv_pool_select_args* args, void* stream) {
     if (a.batch == 0 || a.S_q == 0) return SKV_OK;
     if (!a.lengths || !a.pages || (a.table_width > 0 && (!a.block_table || !a.scratch)) || (a.num_pages > 0 && (!a.bounds || !a.steps)))
         return fail(SKV_ERR_INVALID_ARGUMENT, "pool_select: null pointer");
+    if (reinterpret_cast<uintptr_t>(a.scratch) & 15) return fail(SKV_ERR_INVALID_ARGUMENT, "pool_select: scratch is not on a 16-byte boundary");
     if (a.head_dim > 1024) return fail(SKV_ERR_UNSUPPORTED, "pool_select: head_dim %d above 1024", a.head_dim);
     if ((int64_t)a.batch * a.heads > 65535 || a.S_q > 65535 || (int64_t)a.batch * a.heads * a.S_q > 0x7fffffff)
         return fail(SKV_ERR_TOO_LARGE, "pool_select: %d sequences of %d heads and %d queries", a.batch, a.heads, a.S_q);

@@ -124,18 +124,26 @@ __device__ __forceinline__ int quant_value_fast(float x, float scale, float rcp,
 // A launch whose blocks may be set up while the kernel before it on the stream still runs (which allows it by start_dependents); it
 // reads what that kernel writes only after wait_for_dependency.  (A launch's latency of 2 to 3 us is mostly hidden.)
 template <class... Params, class... Args>
-inline void launch_after(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, const Args&... args) {
+inline void launch_cluster_after(void (*kernel)(Params...), dim3 grid, dim3 cluster, unsigned threads, size_t smem, cudaStream_t st, const Args&... args) {
     cudaLaunchConfig_t config = {};
     config.gridDim = grid;
     config.blockDim = dim3(threads);
     config.dynamicSmemBytes = smem;
     config.stream = st;
-    cudaLaunchAttribute attribute;
-    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &attribute;
-    config.numAttrs = 1;
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = cluster.x;
+    attributes[1].val.clusterDim.y = cluster.y;
+    attributes[1].val.clusterDim.z = cluster.z;
+    config.attrs = attributes;
+    config.numAttrs = cluster.x * cluster.y * cluster.z > 1 ? 2 : 1;
     cudaLaunchKernelEx(&config, kernel, args...);   // (an error is found by check_launch)
+}
+template <class... Params, class... Args>
+inline void launch_after(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st, const Args&... args) {
+    launch_cluster_after(kernel, grid, dim3(1), threads, smem, st, args...);
 }
 __device__ __forceinline__ void start_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_dependency() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

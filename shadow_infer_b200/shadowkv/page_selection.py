@@ -19,8 +19,8 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _lib
-from .._device import compute_device
-from .paged_pool import _POOL, _ROWS, _flag, _index, _pool_fields, _raise_flag
+from .._device import compute_device, device_ctx
+from .paged_pool import _POOL, _ROWS, _flag, _index, _pool_fields, _raise_flag, _workspace
 from .rotary import _launch, _rows
 
 _BOUNDS = struct.Struct("<" + _POOL + "QQQQQ")
@@ -104,7 +104,7 @@ def page_select(
     with the query in 8 bits: ``n = rint(q / t)``, ``t`` the least power of two of which 127 reach the row's largest
     magnitude.  The products and sums are whole numbers and exact, so equal inputs give equal pages on any device.  A page whose step is
     not finite goes before all others, one that the table does not name behind them; a query row that is not finite scores 0.
-    Rows that require a gradient are read as constants.  Two launches.
+    Rows that require a gradient are read as constants.  One launch.
     """
     if q.dim() != 4:
         raise ValueError(f"q must be 4-D [batch, heads, seq, head_dim], got shape {tuple(q.shape)}")
@@ -131,13 +131,15 @@ def page_select(
     new = None if new_lengths is None else _index(new_lengths, (B,), dev, "new_lengths")
     qd, q_rows = _rows(q, dev)
     pages = torch.empty((B, H, S_q, keep), dtype=torch.int32, device=dev)
-    scratch = torch.empty(B * H * S_q * width, dtype=torch.int32, device=dev)
     flag = _flag(check, dev)
-    args = _SELECT.pack(*q_rows, bounds.data_ptr(), steps.data_ptr(), table.data_ptr(), lens.data_ptr(),
-                        0 if new is None else new.data_ptr(), pages.data_ptr(), scratch.data_ptr(),
-                        0 if flag is None else flag.data_ptr(), table.stride(0), scratch.numel() * 4, width, N, page_size, H, D, B,
-                        S_q, keep, first, recent, bool(causal), 0)
-    st = _launch(_lib.load().skv_pool_select, args, dev)
+    lib = _lib.load()
+    with device_ctx(dev):
+        stream = _lib.stream_of(dev)
+        scratch = _workspace("select", dev, stream, B * H * S_q * (width + 3) * 4 + 16)   # (no less than the library asks for)
+        st = lib.skv_pool_select(_SELECT.pack(
+            *q_rows, bounds.data_ptr(), steps.data_ptr(), table.data_ptr(), lens.data_ptr(), 0 if new is None else new.data_ptr(),
+            pages.data_ptr(), scratch.data_ptr(), 0 if flag is None else flag.data_ptr(), table.stride(0), scratch.numel(), width, N,
+            page_size, H, D, B, S_q, keep, first, recent, bool(causal), 0), stream)
     if st:
         _lib.check(st, "page_select")
     del table, qd

@@ -68,6 +68,21 @@ def _scratch(dev: torch.device, stream: int, head_dim: int) -> torch.Tensor:
     return t
 
 
+_WORK = {}            # (operator, device, stream) -> its workspace
+_WORK_KEPT = 1 << 26  # larger workspaces are a call's own
+
+
+def _workspace(what: str, dev: torch.device, stream: int, need: int) -> torch.Tensor:
+    """``need`` bytes for an operator's calls on a stream: shared and kept like the attention's scratch."""
+    t = _WORK.get((what, dev.index, stream))
+    capturing = _capturing()
+    if t is None or capturing or t.numel() < need:
+        t = torch.empty(need if capturing or need > _WORK_KEPT else 1 << (need - 1).bit_length(), dtype=torch.uint8, device=dev)
+        if not capturing and need <= _WORK_KEPT:
+            _WORK[what, dev.index, stream] = t
+    return t
+
+
 def _index(t: torch.Tensor, shape: Tuple[int, ...], dev: torch.device, name: str) -> torch.Tensor:
     """An int32 table on ``dev`` whose last dimension is contiguous."""
     if t.shape != shape:
