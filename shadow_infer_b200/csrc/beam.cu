@@ -9,6 +9,7 @@
 // in the same way from the lists' fronts.
 #include <float.h>
 
+#include <mutex>
 #include <type_traits>
 
 #include "pool.cuh"
@@ -573,6 +574,8 @@ int launch_beam(const skv_beam_args& a, cudaStream_t st) {
     const BeamShape s = beam_shape(a.B, a.beams, a.V, a.keep, sizeof(T), aligned);
     const int64_t jobs = (int64_t)a.B * a.beams * s.parts;
     const unsigned grid = (unsigned)((jobs + kBeamWarps - 1) / kBeamWarps);
+    static std::mutex launches;   // a call's two launches stay together: host threads may share a stream and its scratch
+    const std::lock_guard<std::mutex> both(launches);
     if (s.loads == kManyLoads) beam_lists_kernel<T, kManyLoads><<<grid, 32 * kBeamWarps, 0, st>>>(a, s.parts, s.blocks);
     else beam_lists_kernel<T, kFewLoads><<<grid, 32 * kBeamWarps, 0, st>>>(a, s.parts, s.blocks);
     if (const int rc = check_launch("beam_select")) return rc;

@@ -15,6 +15,8 @@
 // Three kernels: tensor cores for a few query rows a key head (pool_attention_mma.cuh), tcgen05 for many
 // (pool_attention_tc.cuh), and the one below for what neither takes: heads above 256 values or of odd sizes, pages that
 // are not on 16-byte boundaries.
+#include <mutex>
+
 #include "pool_attention.cuh"
 
 namespace skv {
@@ -316,6 +318,8 @@ constexpr int kTableWarps = 8;
 // A warp a unit.
 __global__ void __launch_bounds__(32 * kTableWarps) sparse_tables_kernel(const __grid_constant__ skv_pool_sparse_args s, int units) {
     const skv_pool_attention_args& a = s.attention;
+    start_dependents();
+    wait_for_dependency();
     const int lane = threadIdx.x & 31, u = blockIdx.x * kTableWarps + (threadIdx.x >> 5), P = a.pool.page_size;
     if (u >= units) return;
     const int h = u % a.pool.heads, bi = u / a.pool.heads, i = bi % a.S_q, b = bi / a.S_q;
@@ -375,8 +379,10 @@ extern "C" {
 int skv_pool_attention(const skv_pool_attention_args* args, void* stream) {
     if (!args) return fail(SKV_ERR_INVALID_ARGUMENT, "pool_attention: null pointer");
     bool nothing;
-    const int rc = check_attention(*args, nothing);
-    return rc || nothing ? rc : attend(*args, as_stream(stream));
+    skv_pool_attention_args a = *args;
+    a.reserved = 0;
+    const int rc = check_attention(a, nothing);
+    return rc || nothing ? rc : attend(a, as_stream(stream));
 }
 
 int skv_pool_sparse_attention(const skv_pool_sparse_args* args, void* stream) {
@@ -397,7 +403,9 @@ int skv_pool_sparse_attention(const skv_pool_sparse_args* args, void* stream) {
         !unit_stride(a.out, a.pool.batch, a.S_q, a.pool.heads, a.out.stride_b))
         return fail(SKV_ERR_UNSUPPORTED, "pool_sparse_attention: rows are not evenly spaced");
     cudaStream_t st = as_stream(stream);
-    sparse_tables_kernel<<<(unsigned)((units + kTableWarps - 1) / kTableWarps), 32 * kTableWarps, 0, st>>>(s, (int)units);
+    static std::mutex launches;   // the tables stay with the attention that reads them: host threads may share a stream and its scratch
+    const std::lock_guard<std::mutex> together(launches);
+    launch_after(sparse_tables_kernel, dim3((unsigned)((units + kTableWarps - 1) / kTableWarps)), 32 * kTableWarps, 0, st, s, (int)units);
     if (const int launched = check_launch("pool_sparse_attention")) return launched;
     a.q.heads = a.out.heads = a.q.heads / a.pool.heads;
     a.pool.num_pages *= a.pool.heads;
@@ -408,6 +416,7 @@ int skv_pool_sparse_attention(const skv_pool_sparse_args* args, void* stream) {
     a.lengths = a.pool.block_table + units * s.keep;
     a.new_lengths = nullptr;
     a.causal = 0;
+    a.reserved = 1;   // (units may be split by their number: see launch_mma)
     return attend(a, st);
 }
 

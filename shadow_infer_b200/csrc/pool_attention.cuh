@@ -105,6 +105,28 @@ __device__ __forceinline__ void take_share(const skv_pool_attention_args& a, int
     take_share<THREADS>(a, [&](int b) { return (seq_tiles(seq_tokens(a, b), tile) + pad) * units; }, pad, min_tiles, s, whole ? units : 0);
 }
 
+// Instead of an even share of everything: the tiles of one unit (a sequence of one head, a row tile) over `splits` CTAs.  Tiles are
+// numbered as if every CTA of a unit had `each`, so that a tile's CTA is found as in a share.
+template <int THREADS>
+__device__ __forceinline__ void take_split(const skv_pool_attention_args& a, int tile, int row_tiles, int splits, Share* s) {
+    if (threadIdx.x == 0) {
+        const int unit = blockIdx.x / splits, b = unit / row_tiles, rt = unit - b * row_tiles;
+        const int tiles = seq_tiles(seq_tokens(a, b), tile);
+        Share t;
+        t.each = (tiles + splits - 1) / splits;
+        t.more = 0;
+        t.pad = 0;
+        const int first = unit * splits * t.each;
+        t.lo = (int)blockIdx.x * t.each;
+        t.hi = min(t.lo + t.each, first + tiles);
+        t.total = 0x7fffffff;
+        t.b = b;
+        t.base = first - rt * tiles;
+        *s = t;
+    }
+    __syncthreads();
+}
+
 // Tokens [0, n) of its sequence that query i of sequence b sees.
 __device__ __forceinline__ int seen_by(const skv_pool_attention_args& a, int b, int tokens, int i) {
     const int n_new = a.new_lengths ? __ldg(a.new_lengths + b) : a.S_q;

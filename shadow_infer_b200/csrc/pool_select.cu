@@ -389,14 +389,14 @@ __device__ __forceinline__ void score_pages(const skv_pool_select_args& a, int l
                 next_named[r] = j < pages && page >= 0 && page < a.num_pages;
                 if (j < pages && !next_named[r] && a.error_flag) atomicExch(a.error_flag, 1);
                 ahead[r] = j + p_step < pages ? __ldg(table + j + p_step) : -1;
-                if (next_named[r]) {
-                    const int64_t at = (int64_t)page * H + h;
-                    const int8_t* row = a.bounds + at * (2 * D) + 16 * c;
-                    next_step[r] = __ldg(a.steps + at);
+                // (page 0 in place of none, the row's first bytes in place of those behind it: loads without a branch that waits for
+                // them; their scores are not used, the queries are zero there)
+                const int64_t at = next_named[r] ? (int64_t)page * H + h : 0;
+                const int8_t* row = a.bounds + at * (2 * D);
+                next_step[r] = __ldg(a.steps + at);
 #pragma unroll
-                    for (int s = 0; s < SEGS; ++s)
-                        next[r][s] = 64 * s + 16 * c < 2 * D ? __ldg(reinterpret_cast<const uint4*>(row + 64 * s)) : make_uint4(0, 0, 0, 0);
-                }
+                for (int s = 0; s < SEGS; ++s)
+                    next[r][s] = __ldg(reinterpret_cast<const uint4*>(row + (64 * s + 16 * c < 2 * D ? 64 * s + 16 * c : 0)));
             }
             if (p0 < p_first) {                                   // nothing to score yet
 #pragma unroll 1
@@ -684,11 +684,15 @@ __global__ void __launch_bounds__(kSelectThreads, SEGS == 8 ? 1 : 2) page_select
     wait_for_dependency();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, H = a.heads;
     const int b = blockIdx.z / H, h = blockIdx.z % H, i0 = blockIdx.y * block_tokens, i1 = min(a.S_q, i0 + block_tokens);
-    const int pages = (select_tokens(a, b) + a.page_size - 1) / a.page_size, want = a.keep - a.first - a.recent;
+    const int tokens = select_tokens(a, b), pages = (tokens + a.page_size - 1) / a.page_size, want = a.keep - a.first - a.recent;
     const int pitch = a.table_width;
     uint32_t* keys = static_cast<uint32_t*>(a.scratch) + (int64_t)blockIdx.z * a.S_q * pitch;
     if (pages > a.keep && want > 0) {
-        if constexpr (SEGS > 0) score_pages<T, SEGS>(a, log_span, b, h, pages, i0, block_tokens, s_raw, s_t, s_start, keys, pitch);
+        if (a.num_pages == 0) {                                   // no table can name a page
+            for (int i = i0; i < i1; ++i)
+                for (int j = blockIdx.x * kSelectThreads + tid; j < pages; j += gridDim.x * kSelectThreads) keys[(int64_t)i * pitch + j] = 1;
+            if (a.error_flag) atomicExch(a.error_flag, 1);
+        } else if constexpr (SEGS > 0) score_pages<T, SEGS>(a, log_span, b, h, pages, i0, block_tokens, s_raw, s_t, s_start, keys, pitch);
         else score_pages_any<T>(a, b, h, pages, i0, reinterpret_cast<int8_t*>(s_raw), s_t, keys, pitch);
         if (gridDim.x > 1) {
             asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");

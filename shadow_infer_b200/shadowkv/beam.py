@@ -15,7 +15,7 @@ import torch
 
 from .. import _lib
 from .._device import back, compute_device, device_ctx
-from .paged_pool import _POOL, _flag, _index, _pool_fields, _raise_flag
+from .paged_pool import _POOL, _flag, _index, _pool_fields, _raise_flag, _workspace
 from .page_selection import _bounds_checked
 from .rotary import _DTYPE_CODE, _launch
 
@@ -57,26 +57,36 @@ def beam_select(
     if finished is not None and not 0 <= pad_token < V:
         raise ValueError(f"pad_token {pad_token} is not in a vocabulary of {V}")
     dev = logits.device if logits.is_cuda else compute_device(scores)
-    dtype = logits.dtype if logits.dtype in _DTYPE_CODE else torch.float32
-    x = logits.detach().to(device=dev, dtype=dtype)
-    if x.stride(2) != 1 and V != 1:
+    x, code = logits, _DTYPE_CODE.get(logits.dtype)
+    if code is None or not x.is_cuda or x.requires_grad:
+        x = x.detach().to(device=dev, dtype=x.dtype if code is not None else torch.float32)
+        code = _DTYPE_CODE[x.dtype]
+    sb, sr, sv = x.stride()
+    if sv != 1 and V != 1:
         x = x.contiguous()
-    cum = scores.detach().to(device=dev, dtype=torch.float32).contiguous()
-    done = None if finished is None else finished.to(dev).contiguous()
+        sb, sr, sv = x.stride()
+    cum = scores
+    if cum.dtype is not torch.float32 or not cum.is_contiguous() or cum.get_device() != dev.index or cum.requires_grad:
+        cum = cum.detach().to(device=dev, dtype=torch.float32).contiguous()
+    done = finished
+    if done is not None and (done.get_device() != dev.index or not done.is_contiguous()):
+        done = done.to(dev).contiguous()
     values = torch.empty((B, keep), dtype=torch.float32, device=dev)
-    parents = torch.empty((B, keep), dtype=torch.int64, device=dev)
-    tokens = torch.empty((B, keep), dtype=torch.int64, device=dev)
+    parents, tokens = torch.empty((2, B, keep), dtype=torch.int64, device=dev).unbind()
     lib = _lib.load()
     with device_ctx(dev):   # (the size depends on the device's SMs)
-        scratch = torch.empty(lib.skv_beam_scratch_bytes(B, beams, V, keep), dtype=torch.uint8, device=dev)
-        args = _BEAM.pack(x.data_ptr(), x.stride(0), x.stride(1), cum.data_ptr(), 0 if done is None else done.data_ptr(),
-                          values.data_ptr(), parents.data_ptr(), tokens.data_ptr(), scratch.data_ptr(), scratch.numel(),
-                          _DTYPE_CODE[dtype], B, beams, V, keep, pad_token if finished is not None else 0)
-        st = lib.skv_beam_select(args, _lib.stream_of(dev))
+        stream = _lib.stream_of(dev)
+        scratch = _workspace("beam", dev, stream, max(16, lib.skv_beam_scratch_bytes(B, beams, V, keep)))
+        st = lib.skv_beam_select(_BEAM.pack(
+            x.data_ptr(), sb, sr, cum.data_ptr(), 0 if done is None else done.data_ptr(), values.data_ptr(), parents.data_ptr(),
+            tokens.data_ptr(), scratch.data_ptr(), scratch.numel(), code, B, beams, V, keep, pad_token if finished is not None else 0),
+            stream)
     if st:
         _lib.check(st, "beam_select")
     del x, cum, done
-    return tuple(back(t, logits.device) for t in (values, parents, tokens))
+    if logits.is_cuda:
+        return values, parents, tokens
+    return back(values, logits.device), back(parents, logits.device), back(tokens, logits.device)
 
 
 def paged_reorder(
@@ -118,15 +128,17 @@ def paged_reorder(
         raise ValueError("bounds and steps must be given together")
     if bounds is not None:
         _bounds_checked(bounds, steps, (pool[7], pool[9], 2, pool[10]), dev)
-    new_table = torch.empty(table.shape, dtype=torch.int32, device=dev)
-    new_lengths = torch.empty(B, dtype=torch.int32, device=dev)
+    new_table = torch.empty_like(table, memory_format=torch.contiguous_format)
+    new_lengths = torch.empty_like(lens)
     if B == 0:
         return new_table, new_lengths
-    from_ = parents.to(dev).contiguous()
+    from_ = parents
+    if from_.get_device() != dev.index or not from_.is_contiguous():
+        from_ = from_.to(dev).contiguous()
     flag = _flag(check, dev)
     args = _REORDER.pack(*pool, lens.data_ptr(), from_.data_ptr(), new_table.data_ptr(), new_lengths.data_ptr(),
                          0 if bounds is None else bounds.data_ptr(), 0 if steps is None else steps.data_ptr(),
-                         0 if flag is None else flag.data_ptr(), from_.element_size(), beams)
+                         0 if flag is None else flag.data_ptr(), 8 if from_.dtype is torch.int64 else 4, beams)
     st = _launch(_lib.load().skv_pool_reorder, args, dev)
     if st:
         _lib.check(st, "paged_reorder")

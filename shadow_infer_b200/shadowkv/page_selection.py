@@ -29,10 +29,10 @@ assert (_BOUNDS.size, _SELECT.size) == (120, 168)
 
 
 def _bounds_checked(bounds: torch.Tensor, steps: torch.Tensor, shape: Tuple[int, ...], dev: torch.device) -> None:
-    if (bounds.dtype is not torch.int8 or bounds.shape != shape or not bounds.is_cuda or bounds.get_device() != dev.index
+    if (bounds.shape != shape or bounds.dtype is not torch.int8 or bounds.get_device() != dev.index
             or not bounds.is_contiguous()):
         raise ValueError(f"bounds must be a contiguous int8 tensor {list(shape)} on {dev}, got {tuple(bounds.shape)} {bounds.dtype}")
-    if (steps.dtype is not torch.float32 or steps.shape != shape[:2] or not steps.is_cuda or steps.get_device() != dev.index
+    if (steps.shape != shape[:2] or steps.dtype is not torch.float32 or steps.get_device() != dev.index
             or not steps.is_contiguous()):
         raise ValueError(f"steps must be a contiguous float32 tensor {list(shape[:2])} on {dev}, got {tuple(steps.shape)} {steps.dtype}")
 
@@ -106,16 +106,18 @@ def page_select(
     not finite goes before all others, one that the table does not name behind them; a query row that is not finite scores 0.
     Rows that require a gradient are read as constants.  One launch.
     """
-    if q.dim() != 4:
+    shape = q.shape
+    if len(shape) != 4:
         raise ValueError(f"q must be 4-D [batch, heads, seq, head_dim], got shape {tuple(q.shape)}")
-    B, Hq, S_q, D = q.shape
-    if bounds.dim() != 4:
+    B, Hq, S_q, D = shape
+    shape = bounds.shape
+    if len(shape) != 4:
         raise ValueError(f"bounds must be [num_pages, heads, 2, head_dim], got {tuple(bounds.shape)}")
     if not bounds.is_cuda:
         compute_device()   # raises where there is no CUDA device at all
         raise ValueError("the bounds must be CUDA tensors")
     dev = bounds.device
-    N, H = bounds.shape[:2]
+    N, H = shape[0], shape[1]
     _bounds_checked(bounds, steps, (N, H, 2, D), dev)
     if H < 1 or Hq < 1 or Hq % H:
         raise ValueError(f"{Hq} query heads do not share {H} key heads evenly")
@@ -123,10 +125,11 @@ def page_select(
         raise ValueError(f"page_size must be >= 1, got {page_size}")
     if first < 0 or recent < 1 or first + recent > keep:
         raise ValueError(f"keep {keep} pages with the first {first} (>= 0) and the last {recent} (>= 1) of them")
-    if block_table.dim() != 2 or block_table.shape[0] != B:
+    shape = block_table.shape
+    if len(shape) != 2 or shape[0] != B:
         raise ValueError(f"block_table must be [batch={B}, width], got {tuple(block_table.shape)}")
-    table = _index(block_table, block_table.shape, dev, "block_table")
-    width = table.shape[1]
+    width = shape[1]
+    table = _index(block_table, shape, dev, "block_table")
     lens = _index(lengths, (B,), dev, "lengths")
     new = None if new_lengths is None else _index(new_lengths, (B,), dev, "new_lengths")
     qd, q_rows = _rows(q, dev)

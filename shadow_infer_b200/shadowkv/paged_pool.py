@@ -100,7 +100,8 @@ def _pool_fields(k_pages, v_pages, block_table, scale_k, scale_v, batch: int, he
     """The ``skv_pool`` fields, the pool's device and the table that was used (kept until the launch)."""
     shape = k_pages.shape
     dtype = k_pages.dtype
-    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype is not dtype:
+    same = v_pages is k_pages
+    if len(shape) != 4 or not (same or (v_pages.shape == shape and v_pages.dtype is dtype)):
         raise ValueError("k_pages/v_pages must be alike [num_pages, heads, page_size, row], got "
                          f"{tuple(k_pages.shape)} {k_pages.dtype} and {tuple(v_pages.shape)} {v_pages.dtype}")
     code = _PRECISION_CODE.get(dtype)
@@ -110,7 +111,7 @@ def _pool_fields(k_pages, v_pages, block_table, scale_k, scale_v, batch: int, he
         compute_device()   # raises where there is no CUDA device at all
         raise ValueError("the pages must be CUDA tensors")
     dev = k_pages.device
-    if v_pages.get_device() != dev.index or not k_pages.is_contiguous() or not v_pages.is_contiguous():
+    if not k_pages.is_contiguous() or not (same or (v_pages.get_device() == dev.index and v_pages.is_contiguous())):
         raise ValueError("the pages must be contiguous tensors on one device")
     N, H, P, row = shape
     D = (2 * row if code == 3 else row) if head_dim is None else head_dim
@@ -120,16 +121,18 @@ def _pool_fields(k_pages, v_pages, block_table, scale_k, scale_v, batch: int, he
     if code >= 2:
         if scale_k is None or scale_v is None:
             raise ValueError("int8/int4 pages need scale_k and scale_v")
-        tail = scale_k.shape[3:]
-        for s in (scale_k, scale_v):
-            if s.dtype is not torch.float32 or s.get_device() != dev.index or s.shape[:3] != (N, H, P) or len(s.shape) != code + 2 \
-                    or s.shape[-1] != 1 or not s.is_contiguous():
+        groups = scale_k.shape[3] if code == 3 and scale_k.dim() == 5 else 1
+        want = (N, H, P, 1) if code == 2 else (N, H, P, groups, 1)
+        for s in (scale_k,) if scale_v is scale_k else (scale_k, scale_v):
+            if s.shape != want or s.dtype is not torch.float32 or s.get_device() != dev.index or not s.is_contiguous():
+                if code == 3 and s.dim() == 5 and s.shape != want and s.shape[:3] + s.shape[4:] == (N, H, P, 1):
+                    raise ValueError(f"{groups} int4 groups do not divide a head_dim of {D}, or scale_v has others: {s.shape[3]}")
                 raise ValueError(f"scales must be contiguous float32 [{N}, {H}, {P}, {'1' if code == 2 else 'groups, 1'}] "
                                  f"on {dev}, got {tuple(s.shape)} {s.dtype}")
         if code == 3:
-            if tail[0] < 1 or D % tail[0] or scale_v.shape[3:] != tail:
-                raise ValueError(f"{tail[0]} int4 groups do not divide a head_dim of {D}")
-            group = D // tail[0]
+            if groups < 1 or D % groups:
+                raise ValueError(f"{groups} int4 groups do not divide a head_dim of {D}")
+            group = D // groups
         sk, sv = scale_k.data_ptr(), scale_v.data_ptr()
     table_shape = block_table.shape
     if len(table_shape) != 2 or table_shape[0] != batch:
@@ -267,29 +270,22 @@ def paged_read(
 
 def _listed_pages(pages: torch.Tensor, shape: Tuple[int, int, int], dev: torch.device) -> torch.Tensor:
     """``pages`` as int32 ``[*shape, keep]`` on ``dev`` whose last dimension is contiguous."""
-    if pages.dim() != 4 or pages.shape[3] < 1:
+    have = pages.shape
+    if len(have) != 4 or have[3] < 1:
         raise ValueError(f"pages must be [batch, heads, seq, keep], got {tuple(pages.shape)}")
-    if pages.shape[:3] != shape:
+    want = (*shape, have[3])
+    if have != want:
         try:
-            pages = pages.expand(*shape, -1)
+            pages = pages.expand(want)
         except RuntimeError:
             raise ValueError(f"pages must broadcast to {[*shape, 'keep']}, got {tuple(pages.shape)}") from None
-    return _index(pages, pages.shape, dev, "pages")
+    return _index(pages, want, dev, "pages")
 
 
-def _evenly_spaced(q: torch.Tensor, heads: int) -> bool:
-    """Whether the rows of (sequence, new token, key head), in this order, are evenly spaced in ``q``."""
-    (B, Hq, S, D), (sb, sh, ss, sd) = q.shape, q.stride()
-    if sd != 1 and D != 1:
-        return False
-    units, step = 1, 0
-    for n, s in ((heads, Hq // heads * sh), (S, ss), (B, sb)):
-        if n > 1:
-            if units > 1 and s != units * step:
-                return False
-            step = s if units == 1 else step
-            units *= n
-    return True
+def _evenly_spaced(rows: Tuple[int, ...], B: int, S: int, heads: int) -> bool:
+    """Whether the rows (their ``skv_rows`` fields) of (sequence, token, head), in this order, are evenly spaced."""
+    _, sb, sh, ss, _, _ = rows
+    return (S == 1 or heads == 1 or ss == heads * sh) and (B == 1 or (heads == 1 and S == 1) or sb == (S * ss if S > 1 else heads * sh))
 
 
 def paged_attention(
@@ -345,12 +341,11 @@ def paged_attention(
     new = None if new_lengths is None else _index(new_lengths, (B,), dev, "new_lengths")
     if pages is not None:
         listed = _listed_pages(pages, (B, pool[9], S_q), dev)
-        tables = torch.empty(B * S_q * pool[9] * (listed.shape[3] + 1), dtype=torch.int32, device=dev)
     qd, q_rows = _rows(q, dev)
-    if pages is not None and not _evenly_spaced(qd, pool[9]):
+    if pages is not None and not _evenly_spaced(q_rows, B, S_q, Hq):
         qd, q_rows = _rows(qd.transpose(1, 2).contiguous().transpose(1, 2), dev)
     out, out_rows = _like(qd)
-    if pages is not None and not _evenly_spaced(out, pool[9]):
+    if pages is not None and not _evenly_spaced(out_rows, B, S_q, Hq):
         out, out_rows = _like(torch.empty((B, S_q, Hq, D), dtype=qd.dtype, device=dev).transpose(1, 2))
     flag = _flag(check, dev)
     lib = _lib.load()
@@ -362,8 +357,11 @@ def paged_attention(
         if pages is None:
             st = lib.skv_pool_attention(_ATTENTION.pack(*fields), stream)
         else:
-            st = lib.skv_pool_sparse_attention(_SPARSE.pack(*fields, listed.data_ptr(), *listed.stride()[:3], tables.data_ptr(),
-                                                            tables.numel() * 4, listed.shape[3], 0), stream)
+            sb, sh, ss, _ = listed.stride()
+            keep = listed.shape[3]
+            tables = _workspace("tables", dev, stream, B * S_q * pool[9] * (keep + 1) * 4)
+            st = lib.skv_pool_sparse_attention(_SPARSE.pack(*fields, listed.data_ptr(), sb, sh, ss, tables.data_ptr(), tables.numel(),
+                                                            keep, 0), stream)
     if st:
         _lib.check(st, "paged_attention")
     del table, qd

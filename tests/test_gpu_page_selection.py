@@ -230,6 +230,16 @@ def test_selection_names_bad_lengths(skv, n):
     assert got.flatten().tolist() == ([-1, -1] if n < 0 else [0, 4])
 
 
+def test_selection_over_a_pool_without_pages(skv):
+    """No table entry can name a page: the pages that are always read, then the lowest, and no memory of the pool is looked at."""
+    bounds, steps = torch.zeros(0, 2, 2, 64, dtype=torch.int8, device="cuda"), torch.ones(0, 2, device="cuda")
+    q, table = torch.randn(1, 4, 3, 64, device="cuda"), torch.zeros(1, 50, dtype=torch.int32, device="cuda")
+    got = skv.page_select(q, bounds, steps, table, _lens([400]), 8, 5)
+    assert (got == torch.tensor([0, 1, 2, 3, 49], device="cuda")).all()
+    with pytest.raises(ValueError, match="outside"):
+        skv.page_select(q, bounds, steps, table, _lens([400]), 8, 5, check=True)
+
+
 def test_selection_refusals(skv):
     bounds, steps = torch.zeros(4, 2, 2, 16, dtype=torch.int8, device="cuda"), torch.ones(4, 2, device="cuda")
     q, table, lens = torch.randn(1, 4, 1, 16, device="cuda"), torch.zeros(1, 5, dtype=torch.int32, device="cuda"), _lens([9])
