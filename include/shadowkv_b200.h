@@ -543,7 +543,7 @@ typedef struct skv_pool_sparse_args {
     skv_pool_attention_args attention;
     const int32_t* pages;        /* [batch, heads, S_q, keep] by its strides, the last dimension contiguous */
     int64_t pages_stride_b, pages_stride_h, pages_stride_s;
-    void* tables;                /* scratch: batch * S_q * heads * (keep + 1) int32 */
+    void* tables;                /* scratch: batch * S_q * heads * (keep, rounded up to 32, + 1) int32, 128-byte aligned */
     int64_t tables_bytes;
     int32_t keep, reserved;
 } skv_pool_sparse_args;          /* 272 bytes */

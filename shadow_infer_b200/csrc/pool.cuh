@@ -97,7 +97,7 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8]) {
 __device__ __forceinline__ int64_t pool_row(const skv_pool& p, int b, int64_t t) {
     if (t < 0 || t >= (int64_t)p.table_width * p.page_size) return -1;
     const int64_t j = t <= 0xffffffffll ? (int64_t)((uint32_t)t / (uint32_t)p.page_size) : t / p.page_size;
-    const int page = __ldg(p.block_table + b * p.table_stride + j);
+    const int page = p.block_table[b * p.table_stride + j];   // (may have been written by this kernel: no read-only load)
     if (page < 0 || page >= p.num_pages) return -1;
     return (int64_t)page * p.heads * p.page_size + (t - j * p.page_size);
 }

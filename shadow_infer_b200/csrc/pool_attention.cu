@@ -300,8 +300,11 @@ int check_attention(const skv_pool_attention_args& a, bool& nothing) {
 }
 
 int attend(const skv_pool_attention_args& a, cudaStream_t st) {
-    if (fits_mma(a.pool) && fits_tc(a)) return attend_many(a, st);
-    if (fits_mma(a.pool))
+    const bool mma = fits_mma(a.pool), many = mma && fits_tc(a);
+    if (a.reserved < 0 && (!mma || many))
+        if (const int rc = launch_tables(*static_cast<const AttentionCall&>(a).lists, st)) return rc;
+    if (many) return attend_many(a, st);
+    if (mma)
         return a.pool.precision == 0 ? attend_fp32(a, st) : a.pool.precision == 1 ? attend_fp16(a, st) : a.pool.precision == 2 ? attend_int8(a, st) : attend_int4(a, st);
     if (a.q.dtype == kF32) return launch_any<float>(a, st);
     if (a.q.dtype == kF16) return launch_any<__half>(a, st);
@@ -309,51 +312,19 @@ int attend(const skv_pool_attention_args& a, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------------------- listed pages only
-// A query's own choice of pages makes a (sequence, new token, key head) a sequence of its own: its table holds the listed pages,
-// its length their tokens, and its one head is that head's block of a page (a pool of num_pages * heads pages of one head is the
-// same memory).  The last page that the query sees, the only one that may be partly seen, comes last in an ascending list, so
-// the tokens seen are a prefix as they are of any other sequence, and the kernels above need no other case.
 constexpr int kTableWarps = 8;
 
 // A warp a unit.
 __global__ void __launch_bounds__(32 * kTableWarps) sparse_tables_kernel(const __grid_constant__ skv_pool_sparse_args s, int units) {
-    const skv_pool_attention_args& a = s.attention;
-    start_dependents();
     wait_for_dependency();
-    const int lane = threadIdx.x & 31, u = blockIdx.x * kTableWarps + (threadIdx.x >> 5), P = a.pool.page_size;
-    if (u >= units) return;
-    const int h = u % a.pool.heads, bi = u / a.pool.heads, i = bi % a.S_q, b = bi / a.S_q;
-    const int tokens = seq_tokens(a, b), seen = seen_by(a, b, tokens, i), pages = seen > 0 ? (seen - 1) / P + 1 : 0;
-    const int32_t* list = s.pages + b * s.pages_stride_b + h * s.pages_stride_h + i * s.pages_stride_s;
-    int32_t* table = static_cast<int32_t*>(s.tables) + (int64_t)u * s.keep;
-    int top = -1, count = 0, last = -1;   // the largest entry so far, those that count and the last of them
-    bool bad = a.lengths[b] != tokens;
-    for (int k0 = 0; k0 < s.keep; k0 += 32) {
-        const int e = k0 + lane < s.keep ? list[k0 + lane] : -1;
-        int before = e;   // the largest of the lanes up to this one
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, before, o);
-            if (lane >= o) before = max(before, x);
-        }
-        const int upto = max(top, before);
-        before = __shfl_up_sync(0xffffffffu, before, 1);
-        before = lane ? max(top, before) : top;
-        const bool counts = e > before && e < pages;
-        bad |= e < -1 || e >= a.pool.table_width || (e >= 0 && e <= before);
-        const unsigned these = __ballot_sync(0xffffffffu, counts);
-        if (counts) {
-            const int page = __ldg(a.pool.block_table + b * a.pool.table_stride + e);
-            table[count + __popc(these & ((1u << lane) - 1))] = page >= 0 && page < a.pool.num_pages ? page * a.pool.heads + h : -1;
-        }
-        if (these) last = __shfl_sync(0xffffffffu, e, 31 - __clz(these));
-        count += __popc(these);
-        top = __shfl_sync(0xffffffffu, upto, 31);
-    }
-    if (bad && a.error_flag) atomicExch(a.error_flag, 1);
-    if (lane == 0)
-        static_cast<int32_t*>(s.tables)[(int64_t)units * s.keep + u] =
-            count == 0 ? 0 : last == pages - 1 ? (count - 1) * P + (seen - last * P) : count * P;
+    const int u = blockIdx.x * kTableWarps + (threadIdx.x >> 5);
+    if (u < units) list_table(s, u, units);
+}
+
+int launch_tables(const skv_pool_sparse_args& s, cudaStream_t st) {
+    const int units = s.attention.pool.batch * s.attention.S_q * s.attention.pool.heads;
+    launch_after(sparse_tables_kernel, dim3((unsigned)((units + kTableWarps - 1) / kTableWarps)), 32 * kTableWarps, 0, st, s, units);
+    return check_launch("pool_sparse_attention");
 }
 
 // Values from one unit's rows to the next one's, units counted (sequence, new token, key head); false where they are not evenly spaced.
@@ -388,16 +359,19 @@ int skv_pool_attention(const skv_pool_attention_args* args, void* stream) {
 int skv_pool_sparse_attention(const skv_pool_sparse_args* args, void* stream) {
     if (!args) return fail(SKV_ERR_INVALID_ARGUMENT, "pool_sparse_attention: null pointer");
     const skv_pool_sparse_args& s = *args;
-    skv_pool_attention_args a = s.attention;
+    AttentionCall a;
+    static_cast<skv_pool_attention_args&>(a) = s.attention;
+    a.lists = &s;
     bool nothing;
     const int rc = check_attention(a, nothing);
     if (rc || nothing) return rc;
+    if (reinterpret_cast<uintptr_t>(s.tables) & 127) return fail(SKV_ERR_INVALID_ARGUMENT, "pool_sparse_attention: tables are not on a 128-byte boundary");
     if (s.keep < 1) return fail(SKV_ERR_INVALID_ARGUMENT, "pool_sparse_attention: %d pages a query", s.keep);
     if (!s.pages || !s.tables) return fail(SKV_ERR_INVALID_ARGUMENT, "pool_sparse_attention: null pointer");
     const int64_t units = (int64_t)a.pool.batch * a.S_q * a.pool.heads;
     if (units > (1 << 24) || (int64_t)a.pool.num_pages * a.pool.heads > 0x7fffffff)
         return fail(SKV_ERR_TOO_LARGE, "pool_sparse_attention: %lld units over %d pages", (long long)units, a.pool.num_pages);
-    if (s.tables_bytes < units * ((int64_t)s.keep + 1) * 4)
+    if (s.tables_bytes < units * (list_stride(s.keep) + 1) * 4)
         return fail(SKV_ERR_SCRATCH, "pool_sparse_attention: tables of %lld bytes", (long long)s.tables_bytes);
     if (!unit_stride(a.q, a.pool.batch, a.S_q, a.pool.heads, a.q.stride_b) ||
         !unit_stride(a.out, a.pool.batch, a.S_q, a.pool.heads, a.out.stride_b))
@@ -405,18 +379,17 @@ int skv_pool_sparse_attention(const skv_pool_sparse_args* args, void* stream) {
     cudaStream_t st = as_stream(stream);
     static std::mutex launches;   // the tables stay with the attention that reads them: host threads may share a stream and its scratch
     const std::lock_guard<std::mutex> together(launches);
-    launch_after(sparse_tables_kernel, dim3((unsigned)((units + kTableWarps - 1) / kTableWarps)), 32 * kTableWarps, 0, st, s, (int)units);
-    if (const int launched = check_launch("pool_sparse_attention")) return launched;
     a.q.heads = a.out.heads = a.q.heads / a.pool.heads;
     a.pool.num_pages *= a.pool.heads;
     a.pool.heads = a.S_q = 1;
     a.pool.batch = (int)units;
     a.pool.block_table = static_cast<const int32_t*>(s.tables);
-    a.pool.table_stride = a.pool.table_width = s.keep;
-    a.lengths = a.pool.block_table + units * s.keep;
+    a.pool.table_stride = list_stride(s.keep);
+    a.pool.table_width = s.keep;
+    a.lengths = a.pool.block_table + units * list_stride(s.keep);
     a.new_lengths = nullptr;
     a.causal = 0;
-    a.reserved = 1;   // (units may be split by their number: see launch_mma)
+    a.reserved = -1;
     return attend(a, st);
 }
 

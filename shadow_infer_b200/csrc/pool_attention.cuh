@@ -41,7 +41,7 @@ __host__ __device__ inline int64_t token_cap(const skv_pool_attention_args& a) {
     return cap < 0x7fffff00 ? cap : 0x7fffff00;
 }
 __device__ __forceinline__ int seq_tokens(const skv_pool_attention_args& a, int b) {
-    const int64_t n = __ldg(a.lengths + b), cap = token_cap(a);
+    const int64_t n = a.lengths[b], cap = token_cap(a);   // (may have been written by this kernel)
     return (int)(n < 0 ? 0 : n > cap ? cap : n);
 }
 // Tiles of a sequence for one row tile of one head; an empty sequence keeps one, to write its zeros.
@@ -104,6 +104,59 @@ __device__ __forceinline__ void take_share(const skv_pool_attention_args& a, int
     const bool whole = a.pool.batch == 1 && seq_tiles(seq_tokens(a, 0), tile) <= min_tiles;
     take_share<THREADS>(a, [&](int b) { return (seq_tiles(seq_tokens(a, b), tile) + pad) * units; }, pad, min_tiles, s, whole ? units : 0);
 }
+
+// ------------------------------------------------------------------------------- listed pages only
+// A query's own choice of pages makes a (sequence, new token, key head) a sequence of its own: its table holds the listed pages,
+// its length their tokens, and its one head is that head's block of a page (a pool of num_pages * heads pages of one head is the
+// same memory).  The last page that the query sees, the only one that may be partly seen, comes last in an ascending list, so
+// the tokens seen are a prefix as they are of any other sequence, and the kernels need no other case.  The tables are made by a
+// launch of their own, or where units are split by their number by every CTA for its own unit.
+struct AttentionCall : skv_pool_attention_args {
+    const skv_pool_sparse_args* lists;   // where reserved < 0 (in a kernel's arguments it is the CTAs of a unit, or 0)
+};
+__host__ __device__ inline int64_t list_stride(int keep) { return ((int64_t)keep + 31) & ~31ll; }   // tables on 128-byte lines
+
+// A warp makes unit u's table and length.
+__device__ __forceinline__ void list_table(const skv_pool_sparse_args& s, int u, int units) {
+    const skv_pool_attention_args& a = s.attention;
+    const int lane = threadIdx.x & 31, P = a.pool.page_size;
+    const int h = u % a.pool.heads, bi = u / a.pool.heads, i = bi % a.S_q, b = bi / a.S_q;
+    const int32_t* list = s.pages + b * s.pages_stride_b + h * s.pages_stride_h + i * s.pages_stride_s;
+    int e = lane < s.keep ? list[lane] : -1;
+    const int tokens = seq_tokens(a, b), n_new = a.new_lengths ? __ldg(a.new_lengths + b) : a.S_q;
+    const int seen = i >= n_new ? 0 : a.causal ? max(0, tokens - n_new + 1 + i) : tokens, pages = seen > 0 ? (seen - 1) / P + 1 : 0;
+    int32_t* table = static_cast<int32_t*>(s.tables) + u * list_stride(s.keep);
+    int top = -1, count = 0, last = -1;   // the largest entry so far, those that count and the last of them
+    bool bad = a.lengths[b] != tokens;
+#pragma unroll 1
+    for (int k0 = 0; k0 < s.keep; k0 += 32) {
+        if (k0 > 0) e = k0 + lane < s.keep ? list[k0 + lane] : -1;
+        int upto = e;   // the largest of the lanes up to this one
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto = max(upto, x);
+        }
+        upto = max(top, upto);
+        int before = __shfl_up_sync(0xffffffffu, upto, 1);
+        if (lane == 0) before = top;
+        const bool counts = e > before && e < pages;
+        bad |= e < -1 || e >= a.pool.table_width || (e >= 0 && e <= before);
+        const unsigned these = __ballot_sync(0xffffffffu, counts);
+        if (counts) {
+            const int page = __ldg(a.pool.block_table + b * a.pool.table_stride + e);
+            table[count + __popc(these & ((1u << lane) - 1))] = page >= 0 && page < a.pool.num_pages ? page * a.pool.heads + h : -1;
+        }
+        if (these) last = __shfl_sync(0xffffffffu, e, 31 - __clz(these));
+        count += __popc(these);
+        top = __shfl_sync(0xffffffffu, upto, 31);
+    }
+    if (bad && a.error_flag) atomicExch(a.error_flag, 1);
+    if (lane == 0)
+        static_cast<int32_t*>(s.tables)[units * list_stride(s.keep) + u] =
+            count == 0 ? 0 : last == pages - 1 ? (count - 1) * P + (seen - last * P) : count * P;
+}
+int launch_tables(const skv_pool_sparse_args& s, cudaStream_t st);   // of all units
 
 // Instead of an even share of everything: the tiles of one unit (a sequence of one head, a row tile) over `splits` CTAs.  Tiles are
 // numbered as if every CTA of a unit had `each`, so that a tile's CTA is found as in a share.

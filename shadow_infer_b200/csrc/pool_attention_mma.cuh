@@ -139,7 +139,7 @@ struct PageDivide {
 struct PageRows {
     const int32_t* table;
     int width, base, cur, next, lane;
-    __device__ __forceinline__ int entry(int i) const { return i < width ? __ldg(table + i) : -1; }
+    __device__ __forceinline__ int entry(int i) const { return i < width ? table[i] : -1; }   // (may have been written by this kernel)
     __device__ __forceinline__ void start(const skv_pool& p, int b, int first) {
         table = p.block_table + b * p.table_stride;
         width = p.table_width;
@@ -281,8 +281,8 @@ __host__ __device__ constexpr size_t mma_smem() {
 // left out, which costs a call of one token 3 %.
 template <int PREC, int DP, int NT, int NQ, int NP, bool LIMIT>
 __global__ void __launch_bounds__(32 * MmaShape<PREC, DP, NT>::W, MmaShape<PREC, DP, NT>::CTAS)
-pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int row_tiles, PageDivide magic, bool exact, bool q_vec,
-                          bool out_vec) {
+pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, const __grid_constant__ skv_pool_sparse_args lists,
+                          int row_tiles, PageDivide magic, bool exact, bool q_vec, bool out_vec) {
     using L = Slot<PREC, DP>;
     constexpr int M = DP / 16, MQ = MmaShape<PREC, DP, NT>::MQ, ROWS = 8 * NT, W = MmaShape<PREC, DP, NT>::W, S = MmaShape<PREC, DP, NT>::SLOTS;
     constexpr int THREADS = 32 * W, TILE = 16 * W;
@@ -304,9 +304,12 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
     const int rep = a.q.heads / a.pool.heads, R = rep * a.S_q;
     const bool p16 = P % 16 == 0;   // a tile lies in one page
     auto page_of = [&](int t) { return (int)(((uint64_t)(uint32_t)t * magic.mul) >> magic.shift); };
-    wait_for_dependency();
-    if (a.reserved > 0) take_split<THREADS>(a, TILE, row_tiles, a.reserved, &s);
-    else take_share<THREADS>(a, TILE, a.pool.heads * row_tiles, kMmaPad, kMinTiles, &s);
+    if (a.reserved > 0) {
+        wait_for_dependency();
+        if (warp == 0) list_table(lists, blockIdx.x / a.reserved / row_tiles, a.pool.batch);
+        __syncthreads();
+        take_split<THREADS>(a, TILE, row_tiles, a.reserved, &s);
+    } else take_share<THREADS>(a, TILE, a.pool.heads * row_tiles, kMmaPad, kMinTiles, &s);
     if (s.lo >= s.hi) return;
     char* ring = s_ring + warp * S * L::BYTES;
     if (!exact) {   // chunks that the head does not have are never copied: they count as zero
@@ -357,7 +360,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, int
                 atomicExch(a.error_flag, 1);
             }
         } else if (t < f.tokens) {
-            const int j = page_of(t), page = __ldg(pages.table + j);   // t is below the table's width
+            const int j = page_of(t), page = pages.table[j];   // t is below the table's width
             if (page >= 0 && page < a.pool.num_pages) row = (page * a.pool.heads + f.hk) * P + (t - j * P);
             else if (a.error_flag) atomicExch(a.error_flag, 1);
         }
@@ -1082,7 +1085,8 @@ int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
                        (PREC != 3 || (a.pool.int4_group == 16 && ((reinterpret_cast<uintptr_t>(a.pool.scale_k) |
                                                                    reinterpret_cast<uintptr_t>(a.pool.scale_v)) & 15) == 0));
     const bool q_vec = rows_aligned(a.q), out_vec = rows_aligned(a.out);
-    if (a.reserved) {
+    if (a.reserved < 0) {
+        const skv_pool_sparse_args& lists = *static_cast<const AttentionCall&>(a).lists;
         // Sequences of one head and of known length at most (lists of pages).  Where there are fewer units than CTAs, a unit's tiles are split
         // over those that would be idle; else units stay whole, unless too many CTAs would idle in the last round, where even shares of
         // all tiles are the better cut (512 units of 1024 fp16 tokens on 444 CTAs 57 against 52 us, of 512 int8 tokens on 296 28 against 37).
@@ -1093,13 +1097,15 @@ int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
         if (units * (most > splits ? most : splits) < (1ll << 30) && (rounds == 1 || 4 * units >= 3 * rounds * resident)) {
             skv_pool_attention_args part = a;
             part.reserved = (int32_t)splits;
-            launch_after(kernel, dim3((unsigned)(units * splits)), 32 * Shape::W, smem, st, part, row_tiles, magic, exact, q_vec, out_vec);
+            launch_after(kernel, dim3((unsigned)(units * splits)), 32 * Shape::W, smem, st, part, lists, row_tiles, magic, exact, q_vec, out_vec);
             return check_launch("pool_attention");
         }
+        if (const int rc = launch_tables(lists, st)) return rc;
     }
+    const skv_pool_sparse_args none = {};
     return by_sequences(a, step, [&](skv_pool_attention_args part) {
         part.reserved = 0;
-        kernel<<<sm_count() * Shape::CTAS, 32 * Shape::W, smem, st>>>(part, row_tiles, magic, exact, q_vec, out_vec);
+        kernel<<<sm_count() * Shape::CTAS, 32 * Shape::W, smem, st>>>(part, none, row_tiles, magic, exact, q_vec, out_vec);
         return check_launch("pool_attention");
     });
 }

@@ -315,7 +315,7 @@ def paged_attention(
     ``pages`` (int32 or int64, broadcast to ``[B, heads, S_q, keep]``; ``page_select`` finds them) leaves each query, of those
     tokens, the ones in the listed pages, which are all that is read: an entry counts if it is one of the pages
     that the query sees and larger than every entry before it, so lists are ascending and anything else in them, -1 among it, stands
-    for no page.  One launch more.
+    for no page.  One launch, or two.
 
     The result has ``q``'s dimension order in memory (as torch's own operators keep it), so that the output of a
     ``[B, S, H, D]`` projection goes back to one without a copy.  (With ``pages``, several new tokens of another order are
@@ -359,7 +359,7 @@ def paged_attention(
         else:
             sb, sh, ss, _ = listed.stride()
             keep = listed.shape[3]
-            tables = _workspace("tables", dev, stream, B * S_q * pool[9] * (keep + 1) * 4)
+            tables = _workspace("tables", dev, stream, B * S_q * pool[9] * (keep + 32) * 4)
             st = lib.skv_pool_sparse_attention(_SPARSE.pack(*fields, listed.data_ptr(), sb, sh, ss, tables.data_ptr(), tables.numel(),
                                                             keep, 0), stream)
     if st:

@@ -78,13 +78,13 @@ def test_sparse_attention_refuses_before_a_launch():
     lib = _lib.load()
     bad = _lib.SKV_ERR_INVALID_ARGUMENT
 
-    def attend(pool=None, q=(16, 16, 8, 16, 0, 2), out=(16, 16, 8, 16, 0, 2), lengths=16, S=1, pages=16, tables=16, room=1 << 20, keep=4):
+    def attend(pool=None, q=(16, 16, 8, 16, 0, 2), out=(16, 16, 8, 16, 0, 2), lengths=16, S=1, pages=16, tables=128, room=1 << 20, keep=4):
         return lib.skv_pool_sparse_attention(
             paged_pool._SPARSE.pack(*(pool or _pool()), *q, *out, lengths, 0, 16, 1 << 40, 0, S, 0, 1.0, 0, pages, 8, 4, 8, tables, room,
                                     keep, 0), None)
 
     assert lib.skv_pool_sparse_attention(None, None) == bad
-    assert attend(pages=0) == bad and attend(tables=0) == bad and attend(keep=0) == bad and attend(lengths=0) == bad
+    assert attend(pages=0) == bad and attend(tables=0) == bad and attend(tables=192) == bad and attend(keep=0) == bad and attend(lengths=0) == bad
     assert attend(q=(0, 16, 8, 16, 0, 2)) == bad and attend(_pool(P=0)) == bad
     assert attend(room=4) == _lib.SKV_ERR_SCRATCH
     assert attend(_pool(N=1 << 30, H=4), q=(16, 32, 8, 32, 0, 4), out=(16, 32, 8, 32, 0, 4)) == _lib.SKV_ERR_TOO_LARGE
