@@ -17,7 +17,7 @@
 namespace skv {
 
 constexpr int kBeamKeep = 128, kBeamMost = 4096;      // most continuations; most beams of a search
-constexpr int kMergeEntries = 16384;                  // entries of lists whose scores a merge holds; half of it is aimed at
+constexpr int kMergeEntries = 8192;                   // entries of lists that a merge holds
 constexpr int kBeamWarps = 4, kBeamHeld = 256;        // warps of a block, candidates that a warp holds
 constexpr int kManyLoads = 8, kFewLoads = 4;          // 16-byte loads a lane, of a block
 constexpr int kBeamBatch = 16;                        // blocks between two looks for candidates
@@ -45,7 +45,7 @@ inline BeamShape beam_shape(int B, int beams, int V, int keep, int bytes, bool a
     };
     cut(kManyLoads);
     if (rows * s.blocks < sm_count() * 8) cut(kFewLoads);          // too few warps to fill the GPU: more and smaller blocks
-    int64_t most = kMergeEntries / 2 / keep / beams, resident = sm_count() * 16 / rows;   // 16 warps an SM at a time
+    int64_t most = kMergeEntries / keep / beams, resident = sm_count() * 16 / rows;   // 16 warps an SM at a time
     if (most > resident) most = resident;
     if (most < 1) most = 1;
     s.parts = (int)(s.blocks < most ? s.blocks : most);
@@ -123,14 +123,15 @@ __device__ __forceinline__ float high_of(uint64_t x) { return __uint_as_float((u
 __device__ __forceinline__ bool ahead(float x, int i, float y, int j) { return x > y || (x == y && i < j); }
 
 // The value of rank `rank` (0: the largest) among the lanes' values, none a NaN: sorted by compare and exchange.
-__device__ __forceinline__ float warp_ranked(float x, int rank) {
+template <class V>
+__device__ __forceinline__ V warp_ranked(V x, int rank) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
         for (int o = size >> 1; o > 0; o >>= 1) {
-            const float y = __shfl_xor_sync(0xffffffffu, x, o);
-            x = ((lane & o) == 0) == ((lane & size) == 0) ? fmaxf(x, y) : fminf(x, y);
+            const V y = __shfl_xor_sync(0xffffffffu, x, o);
+            x = ((lane & o) == 0) == ((lane & size) == 0) ? max(x, y) : min(x, y);
         }
     return __shfl_sync(0xffffffffu, x, rank);
 }
@@ -371,43 +372,69 @@ __global__ void __launch_bounds__(32 * kBeamWarps, LOADS == kManyLoads ? 4 : 6) 
 }
 
 // ------------------------------------------------------------------------------------------ the merge
-constexpr int kMergeThreads = 256, kMergeHeld = 768;
+constexpr int kMergeThreads = 256, kMergeHeld = 512;
 
+// A continuation as it is compared: the order-preserving image of its score in 64 bits (0: none), then its place, beam * 2^32 + token.
 struct BeamBest {
-    double score;
-    uint64_t place;    // beam * 2^32 + token; the largest number for none
+    uint64_t score, place;
     __device__ __forceinline__ bool before(const BeamBest& o) const { return score > o.score || (score == o.score && place < o.place); }
 };
+__device__ __forceinline__ uint64_t score_image(double x) {
+    if (x == 0.0) x = 0.0;   // (-0 ties with 0)
+    const uint64_t u = (uint64_t)__double_as_longlong(x);
+    return u >> 63 ? ~u : u | 1ull << 63;
+}
+__device__ __forceinline__ double score_of_image(uint64_t u) { return __longlong_as_double((long long)(u >> 63 ? u ^ 1ull << 63 : ~u)); }
 
-// A block a search.
+// ln x for a normal x > 0: x = 2^e m with m in [sqrt(1/2), sqrt(2)), ln m = 2 atanh(s) with s = (m - 1) / (m + 1), |s| < 0.172, by its series
+// up to s^17 (what is left out is below 2e-15).
+__device__ __forceinline__ double logarithm(double x) {
+    const int high = __double2hiint(x), e = ((high >> 20) - 1022) - ((high & 0xfffff) < 0x6a09e);
+    const double m = x * __hiloint2double((1023 - e) << 20, 0), d = m + 1.0;
+    double r = (double)(1.0f / (float)d);   // two steps of Newton's method: 24, 48, 53 bits
+    r = r * (2.0 - d * r);
+    r = r * (2.0 - d * r);
+    const double s = (m - 1.0) * r, q = s * s;
+    double sum = 1.0 / 17;
+#pragma unroll
+    for (int k = 15; k > 0; k -= 2) sum = fma(sum, q, 1.0 / k);
+    return fma((double)e, 0.69314718055994531, 2.0 * s * sum);
+}
+
+// by_parts, by_keep: 1 / parts, 1 / keep (numbers below 2^20 are divided by a product: half of a unit is more than its error).
+// A block a search.  It runs once, so its time is the latency of one step after another, instructions fetched included: loops are not
+// unrolled where that gains no overlap.
 template <class T>
-__global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_constant__ skv_beam_args a, int parts) {
+__global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_constant__ skv_beam_args a, int parts, bool staged, float by_parts, float by_keep) {
     extern __shared__ __align__(16) unsigned char s_raw[];
     __shared__ BeamBest s_held[kMergeHeld];
     __shared__ BeamBest s_best[2][kMergeThreads / 32];
-    __shared__ float s_front[2][kMergeThreads / 32];
+    __shared__ uint32_t s_front[kMergeThreads / 32], s_top[kMergeThreads / 32];
     __shared__ int s_part[2][kMergeThreads / 32], s_n, s_owner[2][kMergeThreads / 32];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, keep = a.keep, beams = a.beams, lists = beams * parts;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, keep = a.keep, beams = a.beams, lists = beams * parts, all = lists * keep;
     const int64_t row0 = (int64_t)blockIdx.x * beams;
     double* s_from = reinterpret_cast<double*>(s_raw);              // [beams] what a logit less the largest is added to
-    float* s_most = reinterpret_cast<float*>(s_from + beams);       // [beams] the largest logit
-    int* s_count = reinterpret_cast<int*>(s_most + beams);          // [lists] entries
+    float2* s_entry = reinterpret_cast<float2*>(s_from + beams);    // staged: [lists][keep]
+    uint64_t* s_score = reinterpret_cast<uint64_t*>(s_entry + (staged ? all : 0));   // staged: [lists][keep] images
+    float* s_most = reinterpret_cast<float*>(s_score + (staged ? all : 0));          // [beams] the largest logit
+    int* s_count = reinterpret_cast<int*>(s_most + beams);          // [lists] entries; -1: a finished beam's one continuation
+    int* s_at = s_count + lists;                                    // [lists] places of the fronts
+    uint32_t* s_upper = reinterpret_cast<uint32_t*>(s_at + lists);  // staged: [lists][keep] the images' upper halves
     const BeamPart* part = static_cast<const BeamPart*>(a.scratch) + row0 * parts;
     const float2* entries = reinterpret_cast<const float2*>(static_cast<const BeamPart*>(a.scratch) + (int64_t)a.B * lists) +
                             row0 * parts * keep;
     if (tid == 0) s_n = 0;
-    // what the scores need is on its way before the sums are looked at
-    const int entries_all = lists * keep;
-    constexpr int FLY = 6;
-    float2 early[FLY];
     wait_for_dependency();
-#pragma unroll
-    for (int k = 0; k < FLY; ++k) early[k] = tid + k * kMergeThreads < entries_all ? __ldcg(entries + tid + k * kMergeThreads) : make_float2(0.0f, 0.0f);
+    if (staged)
+#pragma unroll 4
+        for (int i = tid; i < all; i += kMergeThreads) s_entry[i] = __ldcg(entries + i);
+#pragma unroll 1
     for (int r = warp; r < beams; r += kMergeThreads / 32) {        // a warp a beam
         const float cum = __ldg(a.scores + row0 + r);
         const bool done = beam_done(a, row0 + r), dead = !(fabsf(cum) < INFINITY);
         float most = -INFINITY;
         double sum = 0.0;
+#pragma unroll 1
         for (int p0 = 0; p0 < parts; p0 += 32) {
             BeamPart y{0.0, -INFINITY, 0};
             if (p0 + lane < parts && !done && !dead) y = part[r * parts + p0 + lane];
@@ -422,101 +449,104 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
             most = now;
         }
         if (lane == 0) {
-            s_from[r] = done || dead ? (double)cum : cum - log(sum);   // (without a logit above -inf: not used)
+            s_from[r] = done || dead ? (double)cum : cum - logarithm(sum);   // (without a logit above -inf: not used)
             s_most[r] = done || dead ? -INFINITY : most;
             if (done && !dead) s_count[r * parts] = -1;
         }
     }
     __syncthreads();
-    // entry `at` of list l, x as it was left; false: there is none, or it scores -inf
-    const float by_parts = 1.0f / (float)parts, by_keep = 1.0f / (float)keep;   // (numbers below 2^20: half of a unit is more than the error)
-    auto entry_of = [&](int l, int at, float2 x, BeamBest& e) {
+    // entry `at` of list l; its score's image is 0 where there is none, or it scores -inf
+    auto entry = [&](int l, int at) {
         const int r = (int)(((float)l + 0.5f) * by_parts), count = s_count[l];
-        if (at >= count) {                                          // (-1: a finished beam's one continuation)
-            e = BeamBest{s_from[r], (uint64_t)r << 32 | (uint32_t)a.pad_token};
-            return count < 0 && at == 0;
-        }
+        if (at >= count)
+            return BeamBest{count < 0 && at == 0 ? score_image(s_from[r]) : 0, (uint64_t)r << 32 | (uint32_t)a.pad_token};
+        const float2 x = staged ? s_entry[l * keep + at] : __ldcg(entries + (int64_t)l * keep + at);
         const float most = s_most[r];
-        e.score = x.x == most ? s_from[r] : s_from[r] + ((double)x.x - (double)most);
-        e.place = (uint64_t)r << 32 | (uint32_t)__float_as_int(x.y);
-        return x.x == most || most < INFINITY;
+        const double score = x.x == most ? s_from[r] : s_from[r] + ((double)x.x - (double)most);
+        return BeamBest{x.x == most || most < INFINITY ? score_image(score) : 0, (uint64_t)r << 32 | (uint32_t)__float_as_int(x.y)};
     };
-    auto entry = [&](int l, int at, BeamBest& e) { return entry_of(l, at, at < s_count[l] ? __ldcg(entries + (int64_t)l * keep + at) : make_float2(0.0f, 0.0f), e); };
-    // ---- candidates: scores as 32-bit numbers, from one on that keep of them, and not many more, reach
-    BeamBest e;
-    int round = 0, n = kMergeHeld + 1;
-    if (entries_all <= kMergeEntries) {
-        float* s_score = reinterpret_cast<float*>(s_count + lists);   // [lists][keep]
-        float best = -INFINITY, front = -INFINITY;                  // of a thread's entries, of a thread's lists' fronts
-        auto put_score = [&](int i, float2 y) {
-            const int l = (int)(((float)i + 0.5f) * by_keep);
-            const float x = entry_of(l, i - l * keep, y, e) ? fmaxf((float)e.score, -FLT_MAX) : -INFINITY;
+    // ---- candidates: by the images' upper halves.  The keep-th best of 32 lists' fronts is no better than the keep-th best of all; from there
+    // on the range is halved until not many more than keep are left.
+    int n = kMergeHeld + 1, found = 0, round = 0;
+    if (staged) {
+        uint32_t best = 0, front = 0;                               // of a thread's entries, of its lists' fronts
+        // (entry() without its branches)
+#pragma unroll 1
+        for (int i = tid; i < all; i += kMergeThreads) {
+            const int l = (int)(((float)i + 0.5f) * by_keep), r = (int)(((float)l + 0.5f) * by_parts), at = i - l * keep;
+            const int count = s_count[l];
+            const float logit = s_entry[i].x, most = s_most[r];
+            const double from = s_from[r], score = logit == most || count < 0 ? from : from + ((double)logit - (double)most);
+            const bool is = count < 0 ? at == 0 : at < count && (logit == most || most < INFINITY);
+            const uint64_t x = is ? score_image(score) : 0;
             s_score[i] = x;
-            best = fmaxf(best, x);
-        };
-#pragma unroll
-        for (int k = 0; k < FLY; ++k)
-            if (tid + k * kMergeThreads < entries_all) put_score(tid + k * kMergeThreads, early[k]);
-        for (int i = tid + FLY * kMergeThreads; i < entries_all; i += kMergeThreads) put_score(i, __ldcg(entries + i));
+            s_upper[i] = (uint32_t)(x >> 32);
+            best = max(best, (uint32_t)(x >> 32));
+        }
         __syncthreads();
-        for (int l = tid; l < lists; l += kMergeThreads) front = fmaxf(front, s_score[l * keep]);
-        front = keep <= 32 ? warp_ranked(front, keep - 1) : -INFINITY;
-        best = warp_max(best);
-        if (lane == 0) { s_front[0][warp] = front; s_front[1][warp] = best; }
+#pragma unroll 1
+        for (int l = tid; l < lists; l += kMergeThreads) front = max(front, s_upper[l * keep]);
+        front = keep <= 32 && lists >= keep ? warp_ranked(front, keep - 1) : 0;
+        best = __reduce_max_sync(0xffffffffu, best);
+        if (lane == 0) { s_front[warp] = front; s_top[warp] = best; }
         __syncthreads();
-        for (int w = 0; w < kMergeThreads / 32; ++w) { front = fmaxf(front, s_front[0][w]); best = fmaxf(best, s_front[1][w]); }
-        auto count_from = [&](float x) {
+        uint32_t lo = max(__reduce_max_sync(0xffffffffu, s_front[lane % (kMergeThreads / 32)]), 1u);
+        uint32_t hi = __reduce_max_sync(0xffffffffu, s_top[lane % (kMergeThreads / 32)]), x = lo;
+#pragma unroll 1
+        for (bool first = true; first || (lo < hi && n > keep + 32); first = false) {
             int m = 0;
-            for (int i = tid; i < entries_all; i += kMergeThreads) m += s_score[i] >= x;
+#pragma unroll 2
+            for (int i = tid; i < all; i += kMergeThreads) m += s_upper[i] >= x;
             m = __reduce_add_sync(0xffffffffu, m);
             if (lane == 0) s_part[round & 1][warp] = m;
             __syncthreads();
-            m = 0;
-            for (int w = 0; w < kMergeThreads / 32; ++w) m += s_part[round & 1][w];
+            m = __reduce_add_sync(0xffffffffu, lane < kMergeThreads / 32 ? s_part[round & 1][lane] : 0);
             ++round;
-            return m;
-        };
-        auto value_of = [](uint32_t image) { return __uint_as_float(image & 0x80000000u ? image ^ 0x80000000u : ~image); };
-        uint32_t lo = score_bits(fmaxf(front, -FLT_MAX)), hi = score_bits(fmaxf(best, -FLT_MAX));
-        n = count_from(value_of(lo));
-        while (lo < hi && n > keep + 64) {
-            const uint32_t mid = lo + (hi - lo + 1) / 2;
-            const int m = count_from(value_of(mid));
-            if (m >= keep) { lo = mid; n = m; } else hi = mid - 1;
+            if (first || m >= keep) { lo = x; n = m; } else hi = x - 1;
+            x = lo + (hi - lo + 1) / 2;
         }
         if (n <= kMergeHeld) {
-            const float least = value_of(lo);
-            for (int i = tid; i < entries_all; i += kMergeThreads)
-                if (s_score[i] >= least && entry((int)(((float)i + 0.5f) * by_keep), i % keep, e)) s_held[atomicAdd(&s_n, 1)] = e;
+#pragma unroll 2
+            for (int i = tid; i < all; i += kMergeThreads) {
+                if (s_upper[i] < lo) continue;
+                const int l = (int)(((float)i + 0.5f) * by_keep), r = (int)(((float)l + 0.5f) * by_parts);
+                const int token = s_count[l] < 0 ? a.pad_token : __float_as_int(s_entry[i].y);
+                s_held[atomicAdd(&s_n, 1)] = BeamBest{s_score[i], (uint64_t)r << 32 | (uint32_t)token};
+            }
             __syncthreads();
-            n = s_n;
         }
     }
-    int found = 0;
     auto put = [&](int rank, const BeamBest& x) {
         const int64_t to = (int64_t)blockIdx.x * keep + rank;
-        a.values[to] = (float)x.score;
+        a.values[to] = (float)score_of_image(x.score);
         a.parents[to] = (int64_t)(x.place >> 32);
         a.tokens[to] = (int64_t)(x.place & 0xffffffffu);
     };
     if (n <= kMergeHeld) {
-        for (int i = tid; i < n; i += kMergeThreads) {
+        // a warp an entry: how many are before it
+#pragma unroll 1
+        for (int i = warp; i < n; i += kMergeThreads / 32) {
             const BeamBest x = s_held[i];
             int rank = 0;
-            for (int j = 0; j < n; ++j) rank += s_held[j].before(x);
-            if (rank < keep) put(rank, x);
+#pragma unroll 1
+            for (int j = lane; j < n; j += 32) rank += s_held[j].before(x);
+            rank = __reduce_add_sync(0xffffffffu, rank);
+            if (lane == 0 && rank < keep) put(rank, x);
         }
         found = min(n, keep);
     } else {
         // more candidates than are held (many equal ones): the best of the lists' fronts, `keep` times
         __syncthreads();
-        int* s_at = s_count + lists;                                // [lists] places of the fronts
         for (int l = tid; l < lists; l += kMergeThreads) s_at[l] = 0;
+#pragma unroll 1
         for (; found < keep; ++found) {
-            BeamBest best{-(double)INFINITY, ~0ull};
+            BeamBest best{0, ~0ull};
             int owner = -1;
-            for (int l = tid; l < lists; l += kMergeThreads)        // (each thread reads and advances its own lists only)
-                if (entry(l, s_at[l], e) && e.before(best)) { best = e; owner = l; }
+#pragma unroll 1
+            for (int l = tid; l < lists; l += kMergeThreads) {      // (each thread reads and advances its own lists only)
+                const BeamBest e = entry(l, s_at[l]);
+                if (e.score && e.before(best)) { best = e; owner = l; }
+            }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) {
                 const BeamBest y{__shfl_xor_sync(0xffffffffu, best.score, o), __shfl_xor_sync(0xffffffffu, best.place, o)};
@@ -527,6 +557,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
             __syncthreads();
             best = s_best[found & 1][0];
             owner = s_owner[found & 1][0];
+#pragma unroll 1
             for (int w = 1; w < kMergeThreads / 32; ++w)
                 if (s_best[found & 1][w].before(best)) { best = s_best[found & 1][w]; owner = s_owner[found & 1][w]; }
             if (owner < 0) break;
@@ -535,6 +566,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
         }
     }
     // ---- too few: continuations of -inf, from the first on
+#pragma unroll 1
     for (int64_t i0 = 0; found < keep && i0 < (int64_t)beams * a.V; i0 += kMergeThreads, ++round) {
         const int64_t i = i0 + tid;
         bool none = false;
@@ -553,6 +585,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
         if (lane == 0) s_part[round & 1][warp] = __popc(these);
         __syncthreads();
         int before = 0, total = 0;
+#pragma unroll 1
         for (int w = 0; w < kMergeThreads / 32; ++w) {
             if (w < warp) before += s_part[round & 1][w];
             total += s_part[round & 1][w];
@@ -574,55 +607,85 @@ int launch_beam(const skv_beam_args& a, cudaStream_t st) {
     const BeamShape s = beam_shape(a.B, a.beams, a.V, a.keep, sizeof(T), aligned);
     const int64_t jobs = (int64_t)a.B * a.beams * s.parts;
     const unsigned grid = (unsigned)((jobs + kBeamWarps - 1) / kBeamWarps);
+    prefer_shared<beam_lists_kernel<T, kManyLoads>>(50);   // (32 searches of 8 beams 32.5 -> 27.7 us)
+    prefer_shared<beam_lists_kernel<T, kFewLoads>>(50);
+    prefer_shared<beam_merge_kernel<T>>(50);
     static std::mutex launches;   // a call's two launches stay together: host threads may share a stream and its scratch
     const std::lock_guard<std::mutex> both(launches);
     if (s.loads == kManyLoads) beam_lists_kernel<T, kManyLoads><<<grid, 32 * kBeamWarps, 0, st>>>(a, s.parts, s.blocks);
     else beam_lists_kernel<T, kFewLoads><<<grid, 32 * kBeamWarps, 0, st>>>(a, s.parts, s.blocks);
     if (const int rc = check_launch("beam_select")) return rc;
     const int64_t lists = (int64_t)a.beams * s.parts, entries = lists * a.keep;
-    const size_t smem = (size_t)a.beams * 12 + (lists + (entries <= kMergeEntries ? entries : lists)) * 4;   // at most 48 + 32 + 64 KB
+    const bool staged = entries <= kMergeEntries;
+    const size_t smem = (size_t)a.beams * 12 + lists * 8 + (staged ? entries * 20 : 0);   // at most 16 + 16 + 160 KB (more beams than lists are not staged)
     if (smem > 24 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(beam_merge_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 144 * 1024);
+        const cudaError_t e = cudaFuncSetAttribute(beam_merge_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 208 * 1024);
         if (e != cudaSuccess) return fail(SKV_ERR_CUDA, "beam_select: %s", cudaGetErrorString(e));
     }
-    launch_after(beam_merge_kernel<T>, dim3(a.B), kMergeThreads, smem, st, a, s.parts);
+    launch_after(beam_merge_kernel<T>, dim3(a.B), kMergeThreads, smem, st, a, s.parts, staged, 1.0f / (float)s.parts, 1.0f / (float)a.keep);
     return check_launch("beam_select");
 }
 
 // ------------------------------------------------------------------------------------------ reordering
 constexpr int kReorderThreads = 256, kReorderBeams = 1024;
+constexpr int kReorderBytes = 16 * 1024;   // that a block copies at least, where there are as many
 
-// A block a (beam, key head, K or V).  Every block finds out by itself where its beam comes from: a beam is the keeper of its
-// parent's last page if it is the parent, or the first child of a parent that does not go on from itself; the n-th beam that
-// is no keeper takes the last page of the n-th beam without children.  Pages are copied from keepers' parents, which have
+// Copies `bytes` bytes with a block, four 16-byte loads a thread on the way where both ends are on 16-byte boundaries.
+__device__ __noinline__ void move_block(char* to, const char* from, int bytes) {
+    constexpr int FLY = 4;
+    const int n = ((reinterpret_cast<uintptr_t>(to) | reinterpret_cast<uintptr_t>(from)) & 15) == 0 ? bytes / 16 : 0;
+    uint4* d = reinterpret_cast<uint4*>(to);
+    const uint4* s = reinterpret_cast<const uint4*>(from);
+#pragma unroll 1
+    for (int i = threadIdx.x; i < n; i += FLY * kReorderThreads) {
+        uint4 x[FLY];
+#pragma unroll
+        for (int f = 0; f < FLY; ++f) x[f] = s[min(i + f * kReorderThreads, n - 1)];
+#pragma unroll
+        for (int f = 0; f < FLY; ++f)
+            if (i + f * kReorderThreads < n) d[i + f * kReorderThreads] = x[f];
+    }
+#pragma unroll 1
+    for (int i = 16 * n + threadIdx.x; i < bytes; i += kReorderThreads) to[i] = from[i];
+}
+
+// A block a beam and a share of its last page's (key head, K or V) blocks.  Every block finds out by itself where its beam comes from: a
+// beam is the keeper of its parent's last page if it is the parent, or the first child of a parent that does not go on from itself; the
+// n-th beam that is no keeper takes the last page of the n-th beam without children.  Pages are copied from keepers' parents, which have
 // children, to pages of beams that have none, so no block reads what another writes; the old table is only read.
-__global__ void __launch_bounds__(kReorderThreads) pool_reorder_kernel(const __grid_constant__ skv_pool_reorder_args a) {
+__global__ void __launch_bounds__(kReorderThreads, 5) pool_reorder_kernel(const __grid_constant__ skv_pool_reorder_args a) {
     __shared__ int s_parent[kReorderBeams];
     __shared__ bool s_extra[kReorderBeams], s_childless[kReorderBeams];
     __shared__ int s_donor;
     const int tid = threadIdx.x, lane = tid & 31, R = a.beams, P = a.pool.page_size, width = a.pool.table_width;
     const int64_t row = blockIdx.x, row0 = row / R * R;
     const int c = (int)(row - row0);
-    for (int r = tid; r < R; r += kReorderThreads) {
+    auto parent = [&](int r) {
         const int64_t p = a.parents_bytes == 8 ? __ldg(static_cast<const long long*>(a.parents) + row0 + r)
                                                : (long long)__ldg(static_cast<const int32_t*>(a.parents) + row0 + r);
-        s_parent[r] = p >= 0 && p < R ? (int)p : -1;
-    }
-    __syncthreads();
-    const int p = s_parent[c];
-    const int64_t tokens = p < 0 ? 0 : max(0, __ldg(a.lengths + row0 + p)), j = tokens / P;
-    const int rows = j < width ? (int)(tokens - j * P) : 0;      // of the last page, if it is partly filled
-    const int32_t* old = a.pool.block_table + (row0 + max(p, 0)) * a.pool.table_stride;
-    bool copy = rows > 0 && p != c;
-    if (copy) {                                                  // an own page is needed, unless this is the first child of a parent that ends
-        if (s_parent[p] != p) {
-            int before = 0;
-            for (int r = tid; r < c; r += kReorderThreads) before |= s_parent[r] == p;
-            copy = __syncthreads_or(before);
+        return p >= 0 && p < R ? (int)p : -1;
+    };
+    int p, donor = -1;                                           // donor: -1 where the beam keeps its parent's last page
+    bool extra;
+    if (R <= 32) {                                               // a warp by itself, a lane a beam
+        const int mine = lane < R ? parent(lane) : -1;
+        const unsigned some = __reduce_or_sync(0xffffffffu, mine >= 0 ? 1u << mine : 0u), alike = __match_any_sync(0xffffffffu, mine);
+        const unsigned self = __ballot_sync(0xffffffffu, mine == lane);
+        const bool keeps = mine == lane || (mine >= 0 && !(self >> mine & 1) && __ffs(alike) - 1 == lane);
+        const unsigned extras = __ballot_sync(0xffffffffu, mine >= 0 && !keeps);
+        p = __shfl_sync(0xffffffffu, mine, c);
+        extra = extras >> c & 1;
+        if (!extra && blockIdx.y) return;
+        unsigned childless = ~some & (R == 32 ? 0xffffffffu : (1u << R) - 1);
+        if (extra) {
+            for (int n = __popc(extras & ((1u << c) - 1)); n > 0; --n) childless &= childless - 1;
+            donor = __ffs(childless) - 1;
         }
-    }
-    int target = -1;
-    if (copy) {                                                  // (the same for the whole block)
+    } else {
+        for (int r = tid; r < R; r += kReorderThreads) s_parent[r] = parent(r);
+        if (tid == 0) s_donor = -1;
+        __syncthreads();
+        p = s_parent[c];
         for (int r = tid; r < R; r += kReorderThreads) {
             bool childless = true, first = true;
             const int q = s_parent[r];
@@ -633,9 +696,10 @@ __global__ void __launch_bounds__(kReorderThreads) pool_reorder_kernel(const __g
             s_childless[r] = childless;
             s_extra[r] = q >= 0 && q != r && !(first && s_parent[q] != q);
         }
-        if (tid == 0) s_donor = -1;
         __syncthreads();
-        if (tid < 32) {
+        extra = s_extra[c];
+        if (!extra && blockIdx.y) return;
+        if (extra && tid < 32) {
             int rank = 0, seen = 0;
             for (int r0 = 0; r0 < c; r0 += 32) rank += __popc(__ballot_sync(0xffffffffu, r0 + lane < c && s_extra[r0 + lane]));
             for (int r0 = 0; r0 < R; r0 += 32) {
@@ -646,40 +710,37 @@ __global__ void __launch_bounds__(kReorderThreads) pool_reorder_kernel(const __g
             }
         }
         __syncthreads();
+        donor = s_donor;
+    }
+    const int length = p < 0 ? 0 : __ldg(a.lengths + row0 + p), tokens = max(0, length), j = tokens / P;
+    const int rows = j < width ? tokens - j * P : 0;             // of the last page, if it is partly filled
+    const int32_t* old = a.pool.block_table + (row0 + max(p, 0)) * a.pool.table_stride;
+    const bool copy = extra && rows > 0;
+    int target = -1;
+    if (copy) {
         const int source = __ldg(old + j);
-        if (s_donor >= 0) target = __ldg(a.pool.block_table + (row0 + s_donor) * a.pool.table_stride + j);
+        if (donor >= 0) target = __ldg(a.pool.block_table + (row0 + donor) * a.pool.table_stride + j);
         if (target < 0 || target >= a.pool.num_pages || source < 0 || source >= a.pool.num_pages || source == target) {
             target = -1;
             if (a.error_flag && tid == 0) atomicExch(a.error_flag, 1);
         } else {
-            const int head = blockIdx.y >> 1;
-            const bool is_v = blockIdx.y & 1;
-            const int64_t from = ((int64_t)source * a.pool.heads + head) * P, to = ((int64_t)target * a.pool.heads + head) * P;
             const int64_t bytes = pool_row_bytes(a.pool.precision, a.pool.head_dim);
-            auto move = [&](char* base, int64_t row_bytes, int n) {   // n rows of row_bytes
-                char* d = base + to * row_bytes;
-                const char* s = base + from * row_bytes;
-                const int64_t all = n * row_bytes;
-                const uintptr_t odd = reinterpret_cast<uintptr_t>(d) | reinterpret_cast<uintptr_t>(s) | (uintptr_t)all;
-                if ((odd & 15) == 0) {
-                    for (int64_t i = tid; i < all / 16; i += kReorderThreads)
-                        reinterpret_cast<uint4*>(d)[i] = reinterpret_cast<const uint4*>(s)[i];
-                } else if ((odd & 3) == 0) {
-                    for (int64_t i = tid; i < all / 4; i += kReorderThreads)
-                        reinterpret_cast<uint32_t*>(d)[i] = reinterpret_cast<const uint32_t*>(s)[i];
-                } else {
-                    for (int64_t i = tid; i < all; i += kReorderThreads) d[i] = s[i];
+            const int64_t scales = a.pool.precision < 2 ? 0 : a.pool.precision == 2 ? 4 : 4ll * (a.pool.head_dim / a.pool.int4_group);
+            for (int part = blockIdx.y; part < 2 * a.pool.heads; part += gridDim.y) {
+                const int head = part >> 1;
+                const bool is_v = part & 1;
+                const int64_t s = (int64_t)source * a.pool.heads + head, d = (int64_t)target * a.pool.heads + head;
+                char* values = static_cast<char*>(is_v ? a.pool.v : a.pool.k);
+                move_block(values + d * P * bytes, values + s * P * bytes, (int)(rows * bytes));
+                if (scales) {
+                    char* base = reinterpret_cast<char*>(is_v ? a.pool.scale_v : a.pool.scale_k);
+                    move_block(base + d * P * scales, base + s * P * scales, (int)(rows * scales));
                 }
-            };
-            move(static_cast<char*>(is_v ? a.pool.v : a.pool.k), bytes, rows);
-            if (a.pool.precision >= 2)
-                move(reinterpret_cast<char*>(is_v ? a.pool.scale_v : a.pool.scale_k),
-                     a.pool.precision == 2 ? 4 : 4ll * (a.pool.head_dim / a.pool.int4_group), rows);
-            if (a.bounds && !is_v) {
-                const int64_t d = (int64_t)target * a.pool.heads + head, s = (int64_t)source * a.pool.heads + head;
-                const int64_t n = 2ll * a.pool.head_dim;
-                for (int64_t i = tid; i < n; i += kReorderThreads) a.bounds[d * n + i] = a.bounds[s * n + i];
-                if (tid == 0) a.steps[d] = a.steps[s];
+                if (a.bounds && !is_v) {
+                    const int64_t n = 2ll * a.pool.head_dim;
+                    move_block(reinterpret_cast<char*>(a.bounds) + d * n, reinterpret_cast<const char*>(a.bounds) + s * n, (int)n);
+                    if (tid == 0) a.steps[d] = a.steps[s];
+                }
             }
         }
     }
@@ -689,8 +750,8 @@ __global__ void __launch_bounds__(kReorderThreads) pool_reorder_kernel(const __g
     for (int i = tid; i < width; i += kReorderThreads)
         table[i] = p < 0 ? -1 : copy && i == j ? target : __ldg((i < j + (rows > 0) ? old : own) + i);
     if (tid == 0) {
-        a.new_lengths[row] = p < 0 ? 0 : __ldg(a.lengths + row0 + p);
-        if (a.error_flag && (p < 0 || __ldg(a.lengths + row0 + p) < 0 || tokens > (int64_t)width * P)) atomicExch(a.error_flag, 1);
+        a.new_lengths[row] = length;
+        if (a.error_flag && (p < 0 || length < 0 || tokens > (int64_t)width * P)) atomicExch(a.error_flag, 1);
     }
 }
 
@@ -743,8 +804,13 @@ int skv_pool_reorder(const skv_pool_reorder_args* args, void* stream) {
         return fail(SKV_ERR_INVALID_ARGUMENT, "pool_reorder: null pointer");
     if (a.beams > kReorderBeams || a.pool.heads > 32767)
         return fail(SKV_ERR_TOO_LARGE, "pool_reorder: %d beams (at most %d), %d heads", a.beams, kReorderBeams, a.pool.heads);
-    const dim3 grid((unsigned)a.pool.batch, 2 * a.pool.heads);
-    pool_reorder_kernel<<<grid, kReorderThreads, 0, as_stream(stream)>>>(a);
+    const int64_t scales = a.pool.precision < 2 ? 0 : a.pool.precision == 2 ? 4 : 4ll * (a.pool.head_dim / a.pool.int4_group);
+    const int64_t part = a.pool.page_size * (pool_row_bytes(a.pool.precision, a.pool.head_dim) + scales), most = 2ll * a.pool.heads * part;
+    if (part > 0x7fffffff || a.pool.head_dim > 1 << 28)
+        return fail(SKV_ERR_TOO_LARGE, "pool_reorder: pages of %d rows of %d values", a.pool.page_size, a.pool.head_dim);
+    int64_t blocks = (most + kReorderBytes - 1) / kReorderBytes;
+    if (blocks > 2 * a.pool.heads) blocks = 2 * a.pool.heads;
+    pool_reorder_kernel<<<dim3((unsigned)a.pool.batch, (unsigned)blocks), kReorderThreads, 0, as_stream(stream)>>>(a);
     return check_launch("pool_reorder");
 }
 

@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "shadowkv_b200.h"
 
 namespace skv {
@@ -147,6 +149,17 @@ inline void launch_after(void (*kernel)(Params...), dim3 grid, unsigned threads,
 }
 __device__ __forceinline__ void start_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_dependency() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Asks once a device for an SM's division between shared memory and L1 cache.  Kernels that follow each other closely should ask for the same:
+// an SM changes it only while it is empty, which keeps the second from starting beside the first.
+template <auto KERNEL>
+inline void prefer_shared(int percent) {
+    static std::atomic<uint64_t> asked{0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || (dev < 64 && asked.load(std::memory_order_relaxed) >> dev & 1)) return;
+    if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributePreferredSharedMemoryCarveout, percent) == cudaSuccess && dev < 64)
+        asked.fetch_or(1ull << dev, std::memory_order_relaxed);
+}
 
 // Copies `bytes` bytes with a warp, using 16-byte vectors when both ends allow.
 __device__ __forceinline__ void warp_copy(void* dst, const void* src, int64_t bytes, int lane) {
