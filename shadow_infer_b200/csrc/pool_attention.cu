@@ -316,6 +316,7 @@ constexpr int kTableWarps = 8;
 
 // A warp a unit.
 __global__ void __launch_bounds__(32 * kTableWarps) sparse_tables_kernel(const __grid_constant__ skv_pool_sparse_args s, int units) {
+    start_dependents();
     wait_for_dependency();
     const int u = blockIdx.x * kTableWarps + (threadIdx.x >> 5);
     if (u < units) list_table(s, u, units);

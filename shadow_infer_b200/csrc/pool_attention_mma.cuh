@@ -304,8 +304,8 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, con
     const int rep = a.q.heads / a.pool.heads, R = rep * a.S_q;
     const bool p16 = P % 16 == 0;   // a tile lies in one page
     auto page_of = [&](int t) { return (int)(((uint64_t)(uint32_t)t * magic.mul) >> magic.shift); };
+    wait_for_dependency();
     if (a.reserved > 0) {
-        wait_for_dependency();
         if (warp == 0) list_table(lists, blockIdx.x / a.reserved / row_tiles, a.pool.batch);
         __syncthreads();
         take_split<THREADS>(a, TILE, row_tiles, a.reserved, &s);
@@ -1103,9 +1103,11 @@ int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
         if (const int rc = launch_tables(lists, st)) return rc;
     }
     const skv_pool_sparse_args none = {};
+    const bool listed = a.reserved < 0;   // (behind the launch that makes the tables)
     return by_sequences(a, step, [&](skv_pool_attention_args part) {
         part.reserved = 0;
-        kernel<<<sm_count() * Shape::CTAS, 32 * Shape::W, smem, st>>>(part, none, row_tiles, magic, exact, q_vec, out_vec);
+        if (listed) launch_after(kernel, dim3(sm_count() * Shape::CTAS), 32 * Shape::W, smem, st, part, none, row_tiles, magic, exact, q_vec, out_vec);
+        else kernel<<<sm_count() * Shape::CTAS, 32 * Shape::W, smem, st>>>(part, none, row_tiles, magic, exact, q_vec, out_vec);
         return check_launch("pool_attention");
     });
 }

@@ -282,15 +282,25 @@ int launch_bounds(const skv_pool_bounds_args& a, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------------------------------------- scores
+// What the kernel is told besides the call's arguments: query heads a key head, tokens a block takes, blocks that share them, and a
+// division by the page size as a product (mul = ceil(2^shift / page_size), shift = 31 + ceil(log2 page_size), exact below 2^31).
+struct SelectShape {
+    int rep, log_span, block_tokens, blocks;
+    uint32_t mul;
+    int shift;
+    __device__ __forceinline__ int pages_of(int tokens) const {   // that tokens > 0 reach
+        return tokens > 0 ? (int)(((uint64_t)(uint32_t)(tokens - 1) * mul) >> shift) + 1 : 0;
+    }
+};
+
 // What query i of sequence b sees (as in pool_attention.cuh).
 __device__ __forceinline__ int select_tokens(const skv_pool_select_args& a, int b) {
     const int64_t n = __ldg(a.lengths + b), cap = (int64_t)a.table_width * a.page_size;
     return (int)max((int64_t)0, min(n, min(cap, (int64_t)0x7fffff00)));
 }
-__device__ __forceinline__ int select_pages(const skv_pool_select_args& a, int b, int i) {
-    const int tokens = select_tokens(a, b), fresh = a.new_lengths ? __ldg(a.new_lengths + b) : a.S_q;
-    const int seen = i >= fresh ? 0 : a.causal ? max(0, tokens - fresh + 1 + i) : tokens;
-    return seen > 0 ? (seen - 1) / a.page_size + 1 : 0;
+__device__ __forceinline__ int select_pages(const skv_pool_select_args& a, const SelectShape& shape, int b, int i, int tokens) {
+    const int fresh = a.new_lengths ? __ldg(a.new_lengths + b) : a.S_q;
+    return shape.pages_of(i >= fresh ? 0 : a.causal ? max(0, tokens - fresh + 1 + i) : tokens);
 }
 
 // Order-preserving image of a score; a page whose step is not finite is above all, one without a number below.
@@ -353,18 +363,19 @@ constexpr int kSelectKeys = 4096;        // keys that a block keeps in shared me
 // where their bodies follow one another anyway, and the pages' loads stand in one place, an iteration ahead of their use, the first
 // ones on their way while the queries are laid out.
 template <class T, int SEGS>
-__device__ __forceinline__ void score_pages(const skv_pool_select_args& a, int log_span, int b, int h, int pages, int i0, int block_tokens,
+__device__ __forceinline__ void score_pages(const skv_pool_select_args& a, const SelectShape& shape, int rank, int b, int h, int pages, int i0,
                                             __half* s_q, float* s_t, float* s_start, uint32_t* keys, int pitch) {
     constexpr int BYTES = 64 * SEGS, PITCH = BYTES + 8;
-    const int D = a.head_dim, H = a.heads, rep = a.q.heads / H, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, span = 1 << log_span;
+    const int D = a.head_dim, H = a.heads, rep = shape.rep, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int log_span = shape.log_span, span = 1 << log_span;
     const int head_tiles = (rep + span - 1) >> log_span;          // tiles of a token (1 unless rep > 8)
     const int g = lane >> 2, c = lane & 3;
     const int32_t* table = a.block_table + b * a.table_stride;
-    const int p_first = (blockIdx.x * kSelectWarps + warp) * 16, p_step = gridDim.x * kSelectWarps * 16;
+    const int p_first = (rank * kSelectWarps + warp) * 16, p_step = shape.blocks * kSelectWarps * 16;
     for (int first = 0; first < head_tiles; first += kScoreTiles) {
         // (further rounds are for more than 8 * kScoreTiles heads only: their largest joins what is written already)
         const int tiles = head_tiles > 1 ? min(kScoreTiles, head_tiles - first)
-                                         : ((min(block_tokens, a.S_q - i0) << log_span) + 7) / 8;
+                                         : ((min(shape.block_tokens, a.S_q - i0) << log_span) + 7) / 8;
         int ahead[2];                                             // numbers of the pages that are loaded next
 #pragma unroll
         for (int r = 0; r < 2; ++r) ahead[r] = p_first + g + 8 * r < pages ? __ldg(table + p_first + g + 8 * r) : -1;
@@ -464,9 +475,10 @@ __device__ __forceinline__ void score_pages(const skv_pool_select_args& a, int l
 
 // Heads that are not whole 16-byte rows of bounds, or above 256 values: a warp a page, a column at a time.
 template <class T>
-__device__ __forceinline__ void score_pages_any(const skv_pool_select_args& a, int b, int h, int pages, int i, int8_t* s_q, float* s_t,
+__device__ __forceinline__ void score_pages_any(const skv_pool_select_args& a, const SelectShape& shape, int rank, int b, int h, int pages, int i,
+                                                int8_t* s_q, float* s_t,
                                                 uint32_t* keys, int pitch) {
-    const int D = a.head_dim, H = a.heads, rep = a.q.heads / H, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int D = a.head_dim, H = a.heads, rep = shape.rep, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int head = 0; head < rep; ++head) {
         __syncthreads();
         if (warp == 0) {
@@ -475,7 +487,7 @@ __device__ __forceinline__ void score_pages_any(const skv_pool_select_args& a, i
             whole_query(x, D, largest_of(x), [&](int p, int n) { s_q[p] = (int8_t)n; }, s_t);
         }
         __syncthreads();
-        for (int j = blockIdx.x * kSelectWarps + warp; j < pages; j += gridDim.x * kSelectWarps) {
+        for (int j = rank * kSelectWarps + warp; j < pages; j += shape.blocks * kSelectWarps) {
             const int page = __ldg(a.block_table + b * a.table_stride + j);
             const bool named = page >= 0 && page < a.num_pages;
             if (!named && lane == 0 && a.error_flag) atomicExch(a.error_flag, 1);
@@ -676,43 +688,47 @@ __device__ __forceinline__ void choose_pages(SelectShared& s, const uint32_t* gl
 // A block scores a share of a (sequence, key head)'s pages for up to 32 columns of queries.  The blocks that share them are a cluster:
 // once all of its scores are there, each chooses for some of the queries.
 template <class T, int SEGS>
-__global__ void __launch_bounds__(kSelectThreads, SEGS == 8 ? 1 : 2) page_select_kernel(const __grid_constant__ skv_pool_select_args a, int log_span, int block_tokens) {
+__global__ void __launch_bounds__(kSelectThreads, SEGS == 8 ? 1 : 2) page_select_kernel(const __grid_constant__ skv_pool_select_args a, const __grid_constant__ SelectShape shape) {
     extern __shared__ __align__(16) __half s_raw[];               // SEGS: [columns][64 SEGS + 8], the bytes 0, 2, 1, 3 of each word; else [2 D] bytes
     __shared__ float s_t[8 * kScoreTiles], s_start[8 * kScoreTiles];
     SelectShared& s_choice = *reinterpret_cast<SelectShared*>(s_raw);   // (the queries are not needed any more then)
     start_dependents();
     wait_for_dependency();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, H = a.heads;
-    const int b = blockIdx.z / H, h = blockIdx.z % H, i0 = blockIdx.y * block_tokens, i1 = min(a.S_q, i0 + block_tokens);
-    const int tokens = select_tokens(a, b), pages = (tokens + a.page_size - 1) / a.page_size, want = a.keep - a.first - a.recent;
-    const int pitch = a.table_width;
-    uint32_t* keys = static_cast<uint32_t*>(a.scratch) + (int64_t)blockIdx.z * a.S_q * pitch;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.z, h = blockIdx.y;
+    int rank = 0, group = blockIdx.x;                             // of the cluster, of the new tokens
+    if (shape.blocks > 1) {
+        asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+        asm("mov.u32 %0, %%clusterid.x;" : "=r"(group));
+    }
+    const int i0 = group * shape.block_tokens, i1 = min(a.S_q, i0 + shape.block_tokens);
+    const int tokens = select_tokens(a, b), pages = shape.pages_of(tokens), want = a.keep - a.first - a.recent, pitch = a.table_width;
+    const int64_t unit0 = ((int64_t)b * a.heads + h) * a.S_q;
+    uint32_t* keys = static_cast<uint32_t*>(a.scratch) + unit0 * pitch;
     if (pages > a.keep && want > 0) {
         if (a.num_pages == 0) {                                   // no table can name a page
             for (int i = i0; i < i1; ++i)
-                for (int j = blockIdx.x * kSelectThreads + tid; j < pages; j += gridDim.x * kSelectThreads) keys[(int64_t)i * pitch + j] = 1;
+                for (int j = rank * kSelectThreads + tid; j < pages; j += shape.blocks * kSelectThreads) keys[(int64_t)i * pitch + j] = 1;
             if (a.error_flag) atomicExch(a.error_flag, 1);
-        } else if constexpr (SEGS > 0) score_pages<T, SEGS>(a, log_span, b, h, pages, i0, block_tokens, s_raw, s_t, s_start, keys, pitch);
-        else score_pages_any<T>(a, b, h, pages, i0, reinterpret_cast<int8_t*>(s_raw), s_t, keys, pitch);
-        if (gridDim.x > 1) {
+        } else if constexpr (SEGS > 0) score_pages<T, SEGS>(a, shape, rank, b, h, pages, i0, s_raw, s_t, s_start, keys, pitch);
+        else score_pages_any<T>(a, shape, rank, b, h, pages, i0, reinterpret_cast<int8_t*>(s_raw), s_t, keys, pitch);
+        if (shape.blocks > 1) {
             asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
             asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         } else {
             __syncthreads();
         }
     }
-    if (tid == 0 && a.error_flag && __ldg(a.lengths + b) != select_tokens(a, b)) atomicExch(a.error_flag, 1);
-    const bool by_warp = i1 - i0 > 2 * (int)gridDim.x && pages <= kSelectKeys / kSelectWarps;
-    const int one_of = by_warp ? gridDim.x * kSelectWarps : gridDim.x, first_of = by_warp ? blockIdx.x * kSelectWarps + warp : blockIdx.x;
+    if (tid == 0 && a.error_flag && __ldg(a.lengths + b) != tokens) atomicExch(a.error_flag, 1);
+    const bool by_warp = i1 - i0 > 2 * shape.blocks && pages <= kSelectKeys / kSelectWarps;
+    const int one_of = by_warp ? shape.blocks * kSelectWarps : shape.blocks, first_of = by_warp ? rank * kSelectWarps + warp : rank;
     for (int i = i0 + first_of; i < i1; i += one_of) {
-        const int n = select_pages(a, b, i), step = by_warp ? 32 : kSelectThreads, me = by_warp ? lane : tid;
-        int32_t* out = a.pages + ((int64_t)blockIdx.z * a.S_q + i) * a.keep;
+        const int n = select_pages(a, shape, b, i, tokens), step = by_warp ? 32 : kSelectThreads, me = by_warp ? lane : tid;
+        int32_t* out = a.pages + (unit0 + i) * a.keep;
         if (n <= a.keep) {
             for (int k = me; k < a.keep; k += step) out[k] = k < n ? k : -1;
             continue;
         }
-        for (int k = me; k < a.first; k += step) out[k] = k;
-        for (int k = me; k < a.recent; k += step) out[a.keep - a.recent + k] = n - a.recent + k;
+        for (int k = me; k < a.first + a.recent; k += step) out[k < a.first ? k : want + k] = k < a.first ? k : n - a.recent - a.first + k;
         if (want == 0) continue;
         if (by_warp) choose_pages<1>(s_choice, keys + (int64_t)i * pitch, a.first, n - a.recent, want, out + a.first, lane);
         else choose_pages<kSelectWarps>(s_choice, keys + (int64_t)i * pitch, a.first, n - a.recent, want, out + a.first, tid);
@@ -720,31 +736,36 @@ __global__ void __launch_bounds__(kSelectThreads, SEGS == 8 ? 1 : 2) page_select
 }
 
 template <class T, int SEGS>
-int launch_select_kernel(const skv_pool_select_args& a, int log_span, int block_tokens, size_t smem, cudaStream_t st) {
-    const int groups = a.batch * a.heads, y = (a.S_q + block_tokens - 1) / block_tokens;
+int launch_select_kernel(const skv_pool_select_args& a, SelectShape shape, size_t smem, cudaStream_t st) {
+    shape.shift = 31;
+    while ((1ll << (shape.shift - 31)) < a.page_size) ++shape.shift;
+    shape.mul = (uint32_t)(((1ull << shape.shift) + a.page_size - 1) / a.page_size);
     // as many blocks as fill the GPU, no more than there are shares and a cluster has
-    const int share = SEGS > 0 ? 16 * kSelectWarps : 8 * kSelectWarps;
-    const int64_t all = (int64_t)groups * y, fill = (2ll * sm_count() + all - 1) / all;
+    const int share = SEGS > 0 ? 16 * kSelectWarps : 8 * kSelectWarps, groups = (a.S_q + shape.block_tokens - 1) / shape.block_tokens;
+    const int64_t all = (int64_t)a.batch * a.heads * groups, fill = (2ll * sm_count() + all - 1) / all;
     if (smem < sizeof(SelectShared)) smem = sizeof(SelectShared);
     int x = (a.table_width + share - 1) / share;
     if (x > fill) x = (int)fill;
     if (x > kSelectCluster) x = kSelectCluster;
     if (x < 1) x = 1;
-    launch_cluster_after(page_select_kernel<T, SEGS>, dim3(x, y, groups), dim3(x), kSelectThreads, smem, st, a, log_span, block_tokens);
+    shape.blocks = x;
+    launch_cluster_after(page_select_kernel<T, SEGS>, dim3((unsigned)groups * x, a.heads, a.batch), dim3(x), kSelectThreads, smem, st, a, shape);
     return check_launch("pool_select");
 }
 
 template <class T>
 int launch_select(const skv_pool_select_args& a, cudaStream_t st) {
-    const int D = a.head_dim, rep = a.q.heads / a.heads;
-    if (D % 8 || D > 256 || (reinterpret_cast<uintptr_t>(a.bounds) & 15)) return launch_select_kernel<T, 0>(a, 0, 1, 2 * (size_t)D, st);
-    int log_span = 0;
-    while (1 << log_span < rep && log_span < 3) ++log_span;
-    const int block_tokens = rep > 8 ? 1 : 8 * kScoreTiles >> log_span;
+    const int D = a.head_dim;
+    SelectShape shape = {};
+    shape.rep = a.q.heads / a.heads;
+    shape.block_tokens = 1;
+    if (D % 8 || D > 256 || (reinterpret_cast<uintptr_t>(a.bounds) & 15)) return launch_select_kernel<T, 0>(a, shape, 2 * (size_t)D, st);
+    while (1 << shape.log_span < shape.rep && shape.log_span < 3) ++shape.log_span;
+    if (shape.rep <= 8) shape.block_tokens = 8 * kScoreTiles >> shape.log_span;
     const auto smem = [](int segs) { return (size_t)8 * kScoreTiles * (64 * segs + 8) * sizeof(__half); };
-    if (D <= 64) return launch_select_kernel<T, 2>(a, log_span, block_tokens, smem(2), st);
-    if (D <= 128) return launch_select_kernel<T, 4>(a, log_span, block_tokens, smem(4), st);
-    return launch_select_kernel<T, 8>(a, log_span, block_tokens, smem(8), st);
+    if (D <= 64) return launch_select_kernel<T, 2>(a, shape, smem(2), st);
+    if (D <= 128) return launch_select_kernel<T, 4>(a, shape, smem(4), st);
+    return launch_select_kernel<T, 8>(a, shape, smem(8), st);
 }
 
 }  // namespace skv
@@ -789,7 +810,7 @@ int skv_pool_select(const skv_pool_select_args* args, void* stream) {
         return fail(SKV_ERR_INVALID_ARGUMENT, "pool_select: null pointer");
     if (reinterpret_cast<uintptr_t>(a.scratch) & 15) return fail(SKV_ERR_INVALID_ARGUMENT, "pool_select: scratch is not on a 16-byte boundary");
     if (a.head_dim > 1024) return fail(SKV_ERR_UNSUPPORTED, "pool_select: head_dim %d above 1024", a.head_dim);
-    if ((int64_t)a.batch * a.heads > 65535 || a.S_q > 65535 || (int64_t)a.batch * a.heads * a.S_q > 0x7fffffff)
+    if (a.batch > 65535 || a.heads > 65535 || a.S_q > 0x7fffffff / kSelectCluster || (int64_t)a.batch * a.heads * a.S_q > 0x7fffffff)
         return fail(SKV_ERR_TOO_LARGE, "pool_select: %d sequences of %d heads and %d queries", a.batch, a.heads, a.S_q);
     if (a.scratch_bytes < (int64_t)skv_pool_select_scratch_bytes(a.batch, a.heads, a.S_q, a.table_width))
         return fail(SKV_ERR_SCRATCH, "pool_select: scratch of %lld bytes", (long long)a.scratch_bytes);

@@ -22,6 +22,7 @@ from .rotary import _DTYPE_CODE, _launch
 _BEAM = struct.Struct("<QqqQQQQQQqiiiiii")
 _REORDER = struct.Struct("<" + _POOL + "QQQQQQQii")
 assert (_BEAM.size, _REORDER.size) == (104, 144)
+_SCRATCH_BYTES = {}   # (device, B, beams, V, keep) -> the selection's scratch
 
 
 def beam_select(
@@ -71,12 +72,18 @@ def beam_select(
     done = finished
     if done is not None and (done.get_device() != dev.index or not done.is_contiguous()):
         done = done.to(dev).contiguous()
-    values = torch.empty((B, keep), dtype=torch.float32, device=dev)
-    parents, tokens = torch.empty((2, B, keep), dtype=torch.int64, device=dev).unbind()
+    values = torch.empty(B, keep, dtype=torch.float32, device=dev)
+    parents = torch.empty(B, keep, dtype=torch.int64, device=dev)
+    tokens = torch.empty(B, keep, dtype=torch.int64, device=dev)
     lib = _lib.load()
     with device_ctx(dev):   # (the size depends on the device's SMs)
         stream = _lib.stream_of(dev)
-        scratch = _workspace("beam", dev, stream, max(16, lib.skv_beam_scratch_bytes(B, beams, V, keep)))
+        need = _SCRATCH_BYTES.get((dev.index, B, beams, V, keep))
+        if need is None:
+            if len(_SCRATCH_BYTES) > 4096:   # (sizes that a server has met: not more than some)
+                _SCRATCH_BYTES.clear()
+            need = _SCRATCH_BYTES[dev.index, B, beams, V, keep] = max(16, lib.skv_beam_scratch_bytes(B, beams, V, keep))
+        scratch = _workspace("beam", dev, stream, need)
         st = lib.skv_beam_select(_BEAM.pack(
             x.data_ptr(), sb, sr, cum.data_ptr(), 0 if done is None else done.data_ptr(), values.data_ptr(), parents.data_ptr(),
             tokens.data_ptr(), scratch.data_ptr(), scratch.numel(), code, B, beams, V, keep, pad_token if finished is not None else 0),

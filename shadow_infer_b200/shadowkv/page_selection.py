@@ -133,7 +133,7 @@ def page_select(
     lens = _index(lengths, (B,), dev, "lengths")
     new = None if new_lengths is None else _index(new_lengths, (B,), dev, "new_lengths")
     qd, q_rows = _rows(q, dev)
-    pages = torch.empty((B, H, S_q, keep), dtype=torch.int32, device=dev)
+    pages = torch.empty(B, H, S_q, keep, dtype=torch.int32, device=dev)
     flag = _flag(check, dev)
     lib = _lib.load()
     with device_ctx(dev):
