@@ -616,8 +616,9 @@ int launch_beam(const skv_beam_args& a, cudaStream_t st) {
     else beam_lists_kernel<T, kFewLoads><<<grid, 32 * kBeamWarps, 0, st>>>(a, s.parts, s.blocks);
     if (const int rc = check_launch("beam_select")) return rc;
     const int64_t lists = (int64_t)a.beams * s.parts, entries = lists * a.keep;
-    const bool staged = entries <= kMergeEntries;
-    const size_t smem = (size_t)a.beams * 12 + lists * 8 + (staged ? entries * 20 : 0);   // at most 16 + 16 + 160 KB (more beams than lists are not staged)
+    const size_t fixed = (size_t)a.beams * 12 + lists * 8;   // at most 80 KB
+    const bool staged = entries <= kMergeEntries && fixed + entries * 20 <= 200 * 1024;
+    const size_t smem = fixed + (staged ? entries * 20 : 0);
     if (smem > 24 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(beam_merge_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 208 * 1024);
         if (e != cudaSuccess) return fail(SKV_ERR_CUDA, "beam_select: %s", cudaGetErrorString(e));
@@ -763,8 +764,12 @@ extern "C" {
 
 size_t skv_beam_scratch_bytes(int B, int beams, int V, int keep) {
     if (B <= 0 || beams <= 0 || beams > kBeamMost || V <= 0 || keep <= 0) return 0;
-    const int wide = beam_shape(B, beams, V, keep, 4, false).parts, narrow = beam_shape(B, beams, V, keep, 2, false).parts;
-    return (size_t)B * beams * (wide > narrow ? wide : narrow) * (sizeof(BeamPart) + (size_t)keep * 8);
+    int parts = 1;   // of whichever type and alignment has most
+    for (int i = 0; i < 4; ++i) {
+        const int some = beam_shape(B, beams, V, keep, i & 1 ? 2 : 4, i & 2).parts;
+        if (some > parts) parts = some;
+    }
+    return (size_t)B * beams * parts * (sizeof(BeamPart) + (size_t)keep * 8);
 }
 
 int skv_beam_select(const skv_beam_args* args, void* stream) {

@@ -170,6 +170,66 @@ def test_selection_in_a_graph_on_streams_and_for_host_tensors(skv):
         assert all(torch.equal(a, b) for a, b in zip(got, skv.beam_select(logits, scores, 7)))
 
 
+@pytest.mark.parametrize("B,beams,V,keep", [(125, 4, 4096, 5), (125, 4, 2048, 5), (148, 4, 1024, 8), (1, 1, 100000, 3), (2, 16, 33000, 32),
+                                            (74, 8, 6144, 16), (1, 4, 512, 4)])
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("shift", [0, 1])
+def test_scratch_is_as_large_as_said(skv, B, beams, V, keep, dtype, shift):
+    """Nothing is written behind the scratch's stated size, whatever the rows' type and alignment (which decide how rows are cut)."""
+    from shadow_infer_b200 import _lib
+    from shadow_infer_b200.shadowkv import beam
+    from shadow_infer_b200.shadowkv.rotary import _DTYPE_CODE
+    lib = _lib.load()
+    pitch = V + 8 if shift == 0 else V + 1
+    flat = torch.randn(B * beams * pitch + 1, generator=_gen(V), device="cuda").to(dtype)
+    x = flat[shift:shift + B * beams * pitch].view(B, beams, pitch)[..., :V]
+    scores = torch.zeros(B, beams, device="cuda")
+    need = lib.skv_beam_scratch_bytes(B, beams, V, keep)
+    scratch = torch.full((need + (1 << 16),), 77, dtype=torch.uint8, device="cuda")
+    values, parents, tokens = torch.empty(B, keep, device="cuda"), *torch.empty(2, B, keep, dtype=torch.int64, device="cuda")
+    args = beam._BEAM.pack(x.data_ptr(), x.stride(0), x.stride(1), scores.data_ptr(), 0, values.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
+                           scratch.data_ptr(), need, _DTYPE_CODE[dtype], B, beams, V, keep, 0)
+    assert lib.skv_beam_select(args, torch.cuda.current_stream().cuda_stream) == 0
+    assert (scratch[need:] == 77).all()
+    want = skv.beam_select(x, scores, keep)
+    assert all(torch.equal(a, b) for a, b in zip((values, parents, tokens), want))
+
+
+def test_more_beams_than_a_merge_holds_entries_for(skv):
+    """Searches whose lists do not fit the merge's shared memory: all beams alike, and all different."""
+    gen = _gen(5)
+    for beams, V, keep in ((4096, 9, 2), (4096, 3, 128), (2000, 40, 5), (64, 300, 128)):
+        logits = torch.randn(1, beams, V, generator=gen, device="cuda")
+        _check(skv, logits, -30 * torch.rand(1, beams, generator=gen, device="cuda"), keep)
+        _check(skv, torch.zeros_like(logits), torch.linspace(0, -1, beams, device="cuda")[None], keep)
+
+
+def test_selection_from_two_threads_on_one_stream(skv):
+    """A call's launches share a scratch that the stream's other calls use too."""
+    import threading
+
+    calls = []
+    for seed, (B, beams, V, keep) in enumerate(((4, 4, 30000, 8), (2, 7, 50001, 12))):
+        x = torch.randn(B, beams, V, generator=_gen(seed), device="cuda")
+        calls.append(lambda x=x, keep=keep: skv.beam_select(x, torch.zeros(x.shape[:2], device="cuda"), keep))
+    want = [call() for call in calls]
+    torch.cuda.synchronize()
+    wrong, go = [], threading.Barrier(2)
+
+    def work(i):
+        go.wait()
+        for _ in range(200):
+            if not all(torch.equal(a, b) for a, b in zip(calls[i](), want[i])):
+                wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 def test_empty_batch(skv):
     assert [tuple(t.shape) for t in skv.beam_select(torch.zeros(0, 2, 9, device="cuda"), torch.zeros(0, 2, device="cuda"))] == [(0, 2)] * 3
 

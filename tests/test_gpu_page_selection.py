@@ -302,6 +302,8 @@ SPARSE = [  # counts, H, rep, Sq, D, P, G, causal, keep
     ([40], 1, 1, 1, 300, 8, 16, False, 3),
     ([333, 700], 1, 12, 2, 128, 32, 64, False, 33),
     ([300], 1, 50, 2, 64, 16, 32, False, 7),                # enough rows a key head for the kernel of prompts
+    ([170] * 40, 4, 3, 3, 64, 16, 16, True, 8),             # more units than CTAs: whole ones, one after the other
+    ([300, 20] * 30, 8, 2, 1, 64, 16, 16, False, 15),       # in even shares
 ]
 
 
@@ -405,6 +407,72 @@ def test_selection_in_a_graph_and_on_another_stream(skv):
         lens.copy_(_lens([400 + seed, 299]))
         graph.replay()
         assert all(torch.equal(x, y) for x, y in zip(got, step()))
+
+
+def test_sparse_calls_from_two_threads_on_one_stream(skv):
+    """Selection and attention of both kinds (units split by number, and in even shares) from two host threads that share workspaces."""
+    import threading
+
+    calls = []
+    for seed, (counts, H, rep, Sq, keep) in enumerate((([3000, 16], 2, 4, 1, 30), ([2000] * 64, 8, 3, 1, 20))):
+        pages_kv, scales, table, lens = _filled(skv, "fp16", counts, H, 32, 128, 16, seed)
+        bounds, steps = skv.page_bounds(pages_kv[0], table, lens)
+        q = _rows(_gen(seed), len(counts), H * rep, Sq, 128, torch.bfloat16)
+
+        def call(q=q, pages_kv=pages_kv, table=table, lens=lens, bounds=bounds, steps=steps, keep=keep):
+            pages = skv.page_select(q, bounds, steps, table, lens, 32, keep)
+            return pages, skv.paged_attention(q, *pages_kv, table, lens, pages=pages)
+        calls.append(call)
+    want = [call() for call in calls]
+    torch.cuda.synchronize()
+    wrong, go = [], threading.Barrier(2)
+
+    def work(i):
+        go.wait()
+        for _ in range(200):
+            if not all(torch.equal(a, b) for a, b in zip(calls[i](), want[i])):
+                wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_two_graphs_do_not_share_workspaces(skv):
+    """Graphs captured on one stream and replayed on two."""
+    made = []
+    for seed, counts in enumerate(([2000, 1500], [900, 3000])):
+        pages_kv, scales, table, lens = _filled(skv, "int8", counts, 2, 16, 128, 16, seed)
+        bounds, steps = skv.page_bounds(pages_kv[0], table, lens, scales[0])
+        q = _rows(_gen(seed), 2, 8, 4, 128, torch.float16, "projection")
+        logits, scores = torch.randn(2, 4, 20000, generator=_gen(seed), device="cuda"), torch.zeros(2, 4, device="cuda")
+
+        def step(q=q, pages_kv=pages_kv, scales=scales, table=table, lens=lens, bounds=bounds, steps=steps, logits=logits, scores=scores):
+            pages = skv.page_select(q, bounds, steps, table, lens, 16, 12, causal=True)
+            return (pages, skv.paged_attention(q, *pages_kv, table, lens, *scales, causal=True, pages=pages),
+                    *skv.beam_select(logits, scores, 9))
+
+        want = step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step()
+        made.append((graph, got, want, step))   # (a graph does not keep what it reads)
+    streams = [torch.cuda.Stream() for _ in made]
+    for _ in range(20):
+        for _, got, _, _ in made:
+            for x in got:
+                x.zero_()
+        torch.cuda.synchronize()
+        for (graph, *_), s in zip(made, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, got, want, _ in made:
+            assert all(torch.equal(x, y) for x, y in zip(got, want))
 
 
 @pytest.mark.parametrize("precision", ["fp32", "fp16", "int8", "int4"])
