@@ -158,23 +158,43 @@ __device__ __forceinline__ void list_table(const skv_pool_sparse_args& s, int u,
 }
 int launch_tables(const skv_pool_sparse_args& s, cudaStream_t st);   // of all units
 
-// Instead of an even share of everything: the tiles of one unit (a sequence of one head, a row tile) over `splits` CTAs.  Tiles are
-// numbered as if every CTA of a unit had `each`, so that a tile's CTA is found as in a share.
+// Instead of an even share of everything (the sequences have one head, and their tables and lengths are made here, too):
+// the tiles of one unit (sequence and row tile) over `splits` CTAs, tiles numbered as if every CTA of a unit had `each`, so that a
+// tile's CTA is found as in a share;  or, where there are fewer CTAs than sequences, a run of whole sequences a CTA.
 template <int THREADS>
-__device__ __forceinline__ void take_split(const skv_pool_attention_args& a, int tile, int row_tiles, int splits, Share* s) {
+__device__ __forceinline__ void take_listed(const skv_pool_attention_args& a, const skv_pool_sparse_args& lists, int tile, int row_tiles, Share* s) {
+    const int splits = a.reserved, warp = threadIdx.x >> 5, B = a.pool.batch;
+    const bool run = gridDim.x < (unsigned)B;
+    int unit = 0, b0, b1;
+    if (run) {
+        const int each = (unsigned)B / gridDim.x, more = B - each * gridDim.x, c = blockIdx.x;
+        b0 = c * each + min(c, more);
+        b1 = b0 + each + (c < more);
+    } else {
+        unit = splits > 1 ? blockIdx.x / splits : blockIdx.x;
+        b0 = row_tiles > 1 ? unit / row_tiles : unit;
+        b1 = b0 + 1;
+    }
+#pragma unroll 1
+    for (int b = b0 + warp; b < b1; b += THREADS / 32) list_table(lists, b, B);
+    __syncthreads();
     if (threadIdx.x == 0) {
-        const int unit = blockIdx.x / splits, b = unit / row_tiles, rt = unit - b * row_tiles;
-        const int tiles = seq_tiles(seq_tokens(a, b), tile);
         Share t;
-        t.each = (tiles + splits - 1) / splits;
-        t.more = 0;
-        t.pad = 0;
-        const int first = unit * splits * t.each;
-        t.lo = (int)blockIdx.x * t.each;
-        t.hi = min(t.lo + t.each, first + tiles);
+        t.more = t.pad = 0;
         t.total = 0x7fffffff;
-        t.b = b;
-        t.base = first - rt * tiles;
+        t.b = b0;
+        if (run) {
+            t.each = 0x7fffffff;
+            t.lo = t.hi = t.base = 0;
+            for (int b = b0; b < b1; ++b) t.hi += seq_tiles(seq_tokens(a, b), tile) * row_tiles;
+        } else {
+            const int rt = unit - b0 * row_tiles, tiles = seq_tiles(seq_tokens(a, b0), tile);
+            t.each = (tiles + splits - 1) / splits;
+            const int first = unit * splits * t.each;
+            t.lo = (int)blockIdx.x * t.each;
+            t.hi = min(t.lo + t.each, first + tiles);
+            t.base = first - rt * tiles;
+        }
         *s = t;
     }
     __syncthreads();

@@ -305,11 +305,8 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, con
     const bool p16 = P % 16 == 0;   // a tile lies in one page
     auto page_of = [&](int t) { return (int)(((uint64_t)(uint32_t)t * magic.mul) >> magic.shift); };
     wait_for_dependency();
-    if (a.reserved > 0) {
-        if (warp == 0) list_table(lists, blockIdx.x / a.reserved / row_tiles, a.pool.batch);
-        __syncthreads();
-        take_split<THREADS>(a, TILE, row_tiles, a.reserved, &s);
-    } else take_share<THREADS>(a, TILE, a.pool.heads * row_tiles, kMmaPad, kMinTiles, &s);
+    if (a.reserved > 0) take_listed<THREADS>(a, lists, TILE, row_tiles, &s);
+    else take_share<THREADS>(a, TILE, a.pool.heads * row_tiles, kMmaPad, kMinTiles, &s);
     if (s.lo >= s.hi) return;
     char* ring = s_ring + warp * S * L::BYTES;
     if (!exact) {   // chunks that the head does not have are never copied: they count as zero
@@ -1097,7 +1094,8 @@ int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
         if (units * (most > splits ? most : splits) < (1ll << 30) && (rounds == 1 || 4 * units >= 3 * rounds * resident)) {
             skv_pool_attention_args part = a;
             part.reserved = (int32_t)splits;
-            launch_after(kernel, dim3((unsigned)(units * splits)), 32 * Shape::W, smem, st, part, lists, row_tiles, magic, exact, q_vec, out_vec);
+            const int64_t ctas = rounds > 1 && a.pool.batch > resident ? resident : units * splits;   // (runs of whole sequences)
+            launch_after(kernel, dim3((unsigned)ctas), 32 * Shape::W, smem, st, part, lists, row_tiles, magic, exact, q_vec, out_vec);
             return check_launch("pool_attention");
         }
         if (const int rc = launch_tables(lists, st)) return rc;
