@@ -2,11 +2,19 @@
 // follow them.
 //
 // Selection.  A continuation's score is  s_r + x_rv - m_r - ln sum_v e^(x_rv - m_r),  m_r the row's largest logit.  Within a row
-// scores are ordered as logits are, so one pass over the logits is enough.  A warp takes a block of a row into its registers,
-// up to 128 logits a lane, and leaves the block's maximum, its sum and its `keep` best logits: the keep-th largest of the lanes'
-// maxima is no more than the keep-th largest logit, so the few logits that are not below it are all that have to be ranked.  A
-// second launch, a block a search, joins the sums, turns the lists' logits into scores in 64 bits, and finds the best of all
-// in the same way from the lists' fronts.
+// scores are ordered as logits are, so the logits are read once (and a few pieces of them again).  A warp takes a part of a row, as
+// many parts as there are warps on the GPU at a time, and leaves the part's maximum, its sum and its `keep` best logits.  A second
+// launch, a block a search, joins the sums, turns the lists' logits into scores in 64 bits and merges the lists; it is set
+// up while the first still runs.
+//
+// What bounds it.  256 rows of 131072 16-bit logits (205 of them not finished, 54 MB): 27.4 us, of which the lists take about 20 (2.7 TB/s:
+// a warp has one block of 4 KB ahead of the one at work, and 16 warps fit an SM's registers; 24 without the block ahead were no faster, nor
+// were more parts than warps) and the merge 7, one step's latency after the other.  4 rows of 32000 fp32 logits: 8.9 us, two launches and
+// the same steps; from Python such a call costs 16.
+//
+// Reordering moves what a step has to copy, about a third of the beams' last pages: 256 beams with 63 int8 tokens of 10 heads of 128 values
+// in theirs, 28 MB read and written in 11.3 us (2.6 TB/s; blocks that copy 16 KB each wait for parents, lengths, tables and rows in turn);
+// a step of 8 searches of 4 beams takes 3.8 us.
 #include <float.h>
 
 #include <mutex>
@@ -201,7 +209,7 @@ __global__ void __launch_bounds__(32 * kBeamWarps, LOADS == kManyLoads ? 4 : 6) 
     const int shift = (int)((reinterpret_cast<uintptr_t>(x0) & 15) / sizeof(T));
     float2* list = s_list[warp];
     const int b0 = (int)(blocks * part / parts), b1 = (int)(blocks * (part + 1) / parts);
-    float top = -INFINITY;                                // of the warp
+    float top = -INFINITY;                                // of the lane
     double sum = 0.0;
     int held = 0;
     float low = -INFINITY;                                // the keep-th best so far
@@ -269,38 +277,32 @@ __global__ void __launch_bounds__(32 * kBeamWarps, LOADS == kManyLoads ? 4 : 6) 
             }
             s_best[warp][i][lane] = best;
             mine = fmaxf(mine, best);
-            const float most = warp_max(best);
-            if (most == -INFINITY) continue;
-            // ---- the sum, relative to the block's largest logit
+            // ---- the lane's sum, relative to its own largest logit so far
+            if (best == -INFINITY) continue;
             float more;
-            if (most == INFINITY) {
-                int n = 0;                                // (seldom: the logits are read again)
-                for (int j = max(block * BLOCK - shift, 0) + lane; j < min(a.V, (block + 1) * BLOCK - shift); j += 32)
-                    n += to_float(x0[j]) == INFINITY;
-                more = (float)__reduce_add_sync(0xffffffffu, n);
+            if (best == INFINITY) {
+                more = 0.0f;                              // (seldom)
+#pragma unroll
+                for (int k = 0; k < WORDS; ++k)
+#pragma unroll
+                    for (int j = 0; j < W::N; ++j) more += W::at(w[k], j) == INFINITY ? 1.0f : 0.0f;
             } else {
-                // (sums of 32 or 16 terms in 32 bits each, two apart, so that their rounding stays below the exponentials')
-                const uint64_t less = pack2(-most, -most), by = pack2(kLog2e, kLog2e);
-                uint64_t total = 0;
-                more = 0.0f;
+                const uint64_t less = pack2(-best, -best), by = pack2(kLog2e, kLog2e);
+                uint64_t total[2] = {0, 0};
 #pragma unroll
                 for (int k = 0; k < WORDS; k += W::N == 2 ? 1 : 2) {
                     const float x = W::at(w[k], 0), y = W::N == 2 ? W::at(w[k], 1) : W::at(w[k + 1], 0);
                     const uint64_t d = mul2(add2(pack2(x, y), less), by);
-                    total = add2(total, pack2(exp2_fast(low_of(d)), exp2_fast(high_of(d))));
-                    if (k % 16 >= (W::N == 2 ? 15 : 14)) {
-                        more += low_of(total) + high_of(total);
-                        total = 0;
-                    }
+                    total[k / 2 % 2] = add2(total[k / 2 % 2], pack2(exp2_fast(low_of(d)), exp2_fast(high_of(d))));
                 }
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
+                total[0] = add2(total[0], total[1]);
+                more = low_of(total[0]) + high_of(total[0]);
             }
-            if (most > top) {
-                sum = sum * exp2_fast((top - most) * kLog2e) + more;     // (of -inf: 0)
-                top = most;
-            } else if (top < INFINITY || most == INFINITY) {
-                sum += most == top ? more : more * exp2_fast((most - top) * kLog2e);
+            if (best > top) {
+                sum = sum * exp2_fast((top - best) * kLog2e) + more;     // (of -inf: 0)
+                top = best;
+            } else if (top < INFINITY || best == INFINITY) {
+                sum += best == top ? more : more * exp2_fast((best - top) * kLog2e);
             }
         }
         // ---- candidates: larger than the keep-th best so far (equal ones come behind it), not below the bound
@@ -366,7 +368,11 @@ __global__ void __launch_bounds__(32 * kBeamWarps, LOADS == kManyLoads ? 4 : 6) 
         if (many || n > kBeamHeld) n = beam_many(x0, batch * BLOCK - shift, count * BLOCK, a.V, from, most, keep, held, list, s_held + warp);
         rank(n);
     }
-    if (lane == 0) static_cast<BeamPart*>(a.scratch)[job] = BeamPart{sum, top, held};
+    const float most = warp_max(top);
+    if (top < most) sum = most < INFINITY ? sum * exp2_fast((top - most) * kLog2e) : 0.0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) static_cast<BeamPart*>(a.scratch)[job] = BeamPart{sum, most, held};
     float2* out = reinterpret_cast<float2*>(static_cast<BeamPart*>(a.scratch) + (int64_t)a.B * a.beams * parts) + job * keep;
     for (int i = lane; i < held; i += 32) out[i] = list[i];
 }

@@ -8,6 +8,13 @@
 //     max(n, 0) . highs + min(n, 0) . lows,
 // a product of whole numbers with the 2 D bytes that a page's bounds are: at most 127 * 127 * D < 2^24, so that 32-bit floats
 // hold every partial sum exactly.  The choice does not depend on any order of additions, and ties go to the lowest page.
+//
+// What bounds it.  Bounds of a prompt: HBM, 32768 fp16 tokens of 32 heads of 128 values in 48.4 us, 5.7 TB/s (85 % of the copy
+// rate; values compared one by one in 32 bits took 76); of 8 sequences' newest pages: 6.9 us of latency.  A choice: latency, one step after
+// the other in one kernel (lengths, table, bounds, queries, products, a cluster's barrier, keys, bins, the list): 1024 pages of 32 heads
+// 11.4 us, 2049 pages of 8 heads for 4 query heads each 11.7, 64 sequences of 2 to 256 pages with 8 key heads 16.4, 64 queries of 128 pages
+// with 8 key heads 13.7.  Two launches, with the want-th key found bit by bit, took 14 to 27; loads a round ahead of their use
+// 0.8 to 2.6 more.
 #include "pool.cuh"
 
 namespace skv {
@@ -359,9 +366,7 @@ constexpr int kSelectKeys = 4096;        // keys that a block keeps in shared me
 // of pages g and g + 8.  A byte x becomes an fp16 operand by its place alone: the bits of x + 128 are those of the subnormal
 // (x + 128) 2^-24, so an MMA over a word of 4 bytes a lane gives 2^-24 (n . x + 128 sum n), exactly (at most 255 * 127 * 256 < 2^23 of
 // these units); the accumulators start at what is too much.  (Integer MMAs are not native here.)
-// A call of one token runs through this once, so the time is latency, that of fetching the instructions too: loops are left rolled
-// where their bodies follow one another anyway, and the pages' loads stand in one place, an iteration ahead of their use, the first
-// ones on their way while the queries are laid out.
+// The first pages' loads are on their way while the queries are laid out.
 template <class T, int SEGS>
 __device__ __forceinline__ void score_pages(const skv_pool_select_args& a, const SelectShape& shape, int rank, int b, int h, int pages, int i0,
                                             __half* s_q, float* s_t, float* s_start, uint32_t* keys, int pitch) {
@@ -379,37 +384,30 @@ __device__ __forceinline__ void score_pages(const skv_pool_select_args& a, const
         int ahead[2];                                             // numbers of the pages that are loaded next
 #pragma unroll
         for (int r = 0; r < 2; ++r) ahead[r] = p_first + g + 8 * r < pages ? __ldg(table + p_first + g + 8 * r) : -1;
-        uint4 next[2][SEGS];
-        float next_step[2] = {1.0f, 1.0f};
-        bool next_named[2] = {false, false};
         if (first > 0) __syncthreads();
+        bool laid_out = false;
 #pragma unroll 1
-        for (int p0 = p_first - p_step; p0 < pages; p0 += p_step) {
-            uint32_t y[2][4 * SEGS];
+        for (int p0 = p_first; p0 < pages || !laid_out; p0 += p_step) {
+            uint4 y[2][SEGS];
             float step[2];
             bool named[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-#pragma unroll
-                for (int s = 0; s < SEGS; ++s) {
-                    y[r][4 * s] = next[r][s].x; y[r][4 * s + 1] = next[r][s].y; y[r][4 * s + 2] = next[r][s].z; y[r][4 * s + 3] = next[r][s].w;
-                }
-                step[r] = next_step[r];
-                named[r] = next_named[r];
-                const int j = p0 + p_step + g + 8 * r, page = ahead[r];
-                next_named[r] = j < pages && page >= 0 && page < a.num_pages;
-                if (j < pages && !next_named[r] && a.error_flag) atomicExch(a.error_flag, 1);
+                const int j = p0 + g + 8 * r, page = ahead[r];
+                named[r] = j < pages && page >= 0 && page < a.num_pages;
+                if (j < pages && !named[r] && a.error_flag) atomicExch(a.error_flag, 1);
                 ahead[r] = j + p_step < pages ? __ldg(table + j + p_step) : -1;
                 // (page 0 in place of none, the row's first bytes in place of those behind it: loads without a branch that waits for
                 // them; their scores are not used, the queries are zero there)
-                const int64_t at = next_named[r] ? (int64_t)page * H + h : 0;
+                const int64_t at = named[r] ? (int64_t)page * H + h : 0;
                 const int8_t* row = a.bounds + at * (2 * D);
-                next_step[r] = __ldg(a.steps + at);
+                step[r] = __ldg(a.steps + at);
 #pragma unroll
                 for (int s = 0; s < SEGS; ++s)
-                    next[r][s] = __ldg(reinterpret_cast<const uint4*>(row + (64 * s + 16 * c < 2 * D ? 64 * s + 16 * c : 0)));
+                    y[r][s] = __ldg(reinterpret_cast<const uint4*>(row + (64 * s + 16 * c < 2 * D ? 64 * s + 16 * c : 0)));
             }
-            if (p0 < p_first) {                                   // nothing to score yet
+            if (!laid_out) {
+                laid_out = true;
 #pragma unroll 1
                 for (int col = warp; col < 8 * tiles; col += kSelectWarps) {
                     const int i = head_tiles > 1 ? i0 : min(a.S_q - 1, i0 + (col >> log_span));
@@ -424,7 +422,6 @@ __device__ __forceinline__ void score_pages(const skv_pool_select_args& a, const
                     if (lane == 0) s_start[col] = -128.0f * (float)sum * 0x1p-24f;
                 }
                 __syncthreads();
-                continue;
             }
             float best[2] = {-INFINITY, -INFINITY};               // more than 8 heads
 #pragma unroll 1
@@ -438,7 +435,7 @@ __device__ __forceinline__ void score_pages(const skv_pool_select_args& a, const
                     const uint32_t z[8] = {z0.x, z0.y, z0.z, z0.w, z1.x, z1.y, z1.z, z1.w};
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
-                        const uint32_t u = y[0][4 * s + w], v = y[1][4 * s + w];
+                        const uint32_t u = (&y[0][s].x)[w], v = (&y[1][s].x)[w];
                         mma_f16(acc[w & 1], (u & 0x00FF00FFu) ^ 0x00800080u, (v & 0x00FF00FFu) ^ 0x00800080u,
                                 ((u >> 8) & 0x00FF00FFu) ^ 0x00800080u, ((v >> 8) & 0x00FF00FFu) ^ 0x00800080u, z[2 * w], z[2 * w + 1]);
                     }
