@@ -9,7 +9,7 @@
 //
 // What bounds it.  256 rows of 131072 16-bit logits (205 of them not finished, 54 MB): 27.4 us, of which the lists take about 20 (2.7 TB/s:
 // a warp has one block of 4 KB ahead of the one at work, and 16 warps fit an SM's registers; 24 without the block ahead were no faster, nor
-// were more parts than warps) and the merge 7, one step's latency after the other.  4 rows of 32000 fp32 logits: 8.9 us, two launches and
+// were more parts than warps) and the merge 7, one step's latency after the other.  4 rows of 32000 fp32 logits: 9.2 us, two launches and
 // the same steps; from Python such a call costs 16.
 //
 // Reordering moves what a step has to copy, about a third of the beams' last pages: 256 beams with 63 int8 tokens of 10 heads of 128 values

@@ -18,6 +18,8 @@
 // tokens: 131071 int8 tokens with fp32 queries in 76 us (57 % of the copy rate), 32768 int4 tokens of 32 heads in 82 us (38 %).
 // fp32: 16 KB a tile leave room for 4 warps an SM, 16384 tokens in 36 us (57 %).  Small calls: 4 to 5 us until the first rows
 // are there, 1.7 us a unit and 3 to 6 us for a join; 512 tokens of 32 heads in 12 us, 8 int8 sequences of up to 2048 tokens in 18.
+// Lists of pages: a unit's table is made first, 2 to 4 us; 32 units of 2048 int4 tokens in 19 us, 8 of 4096 int8 tokens in 19, 512 of 512 int8
+// tokens in 26 (from L2: the rounds' instructions), 512 of up to 1024 fp16 tokens in 52 with its tables' launch (256 MB, 5 TB/s).
 //
 // Exactness.  Page values enter the MMAs exactly: fp16 as it is, int8 and int4 as small integers, fp32 as two terms of 11 bits
 // (of the products of small parts only that of both is left out, 2^-24 of a value).  For the scores they stay
@@ -1086,7 +1088,7 @@ int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
         const skv_pool_sparse_args& lists = *static_cast<const AttentionCall&>(a).lists;
         // Sequences of one head and of known length at most (lists of pages).  Where there are fewer units than CTAs, a unit's tiles are split
         // over those that would be idle; else units stay whole, unless too many CTAs would idle in the last round, where even shares of
-        // all tiles are the better cut (512 units of 1024 fp16 tokens on 444 CTAs 57 against 52 us, of 512 int8 tokens on 296 28 against 37).
+        // all tiles are the better cut (512 units of 1024 fp16 tokens on 444 CTAs 57 against 52 us, of 512 int8 tokens on 296 26 against 37).
         const int64_t units = (int64_t)a.pool.batch * row_tiles, resident = (int64_t)sm_count() * Shape::CTAS;
         const int64_t most = (token_cap(a) + 16 * Shape::W - 1) / (16 * Shape::W), rounds = (units + resident - 1) / resident;
         int64_t splits = resident / units < most ? resident / units : most;
