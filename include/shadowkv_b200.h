@@ -533,7 +533,8 @@ typedef struct skv_pool_select_args {
  * sees, where they are no more than keep; else the first `first`, the last `recent` (first + recent <=
  * keep, recent >= 1), and those of the largest score, ties to the lowest page.  score = the largest, over the
  * query heads that share the key head, of t * step * sum_d n_d (n_d > 0 ? highs_d : lows_d) with n = rint(q / t) and
- * t the least power of two of which 127 reach max |q| (a query row that is not finite scores 0).  The sum is exact.  A page
+ * t the least power of two of which 127 reach max |q| (a query row that is not finite scores 0).  The sum is exact, the
+ * products with t, then step, are 32-bit floats.  table_width <= 2^30.  A page
  * whose step is not finite comes before all others, one that the table does not name behind.
  * scratch: skv_pool_select_scratch_bytes bytes, 16-byte aligned; calls that may overlap on the GPU use scratch of their own. */
 size_t skv_pool_select_scratch_bytes(int batch, int heads, int S_q, int table_width);
@@ -598,7 +599,8 @@ typedef struct skv_pool_reorder_args {
  * first child; the n-th of the other children takes the page that the n-th beam without children has in
  * that place of its table, and the tokens (and bounds) are copied there.  The beams of a group are equally long (else that
  * place may be empty: its table entry is -1 then and error_flag set, as by a parent outside the group, whose child is empty).
- * Table entries behind the tokens (pages taken ahead) stay where they are.  beams <= 1024. */
+ * Table entries behind the tokens (pages taken ahead) stay where they are.  The new table and lengths share no memory with the old.
+ * beams <= 1024. */
 int skv_pool_reorder(const skv_pool_reorder_args* args, void* stream);
 
 #ifdef __cplusplus

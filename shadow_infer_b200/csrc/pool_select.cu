@@ -441,10 +441,11 @@ __device__ __forceinline__ void score_pages(const skv_pool_select_args& a, const
                     }
                 }
                 // columns 2 c and 2 c + 1 of pages g (acc 0, 1) and g + 8
-                const float t0 = s_t[8 * t + 2 * c] * 0x1p24f, t1 = s_t[8 * t + 2 * c + 1] * 0x1p24f;
+                const float t0 = s_t[8 * t + 2 * c], t1 = s_t[8 * t + 2 * c + 1];
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    float u = __fmul_rn(acc[0][2 * r] + acc[1][2 * r], t0), v = __fmul_rn(acc[0][2 * r + 1] + acc[1][2 * r + 1], t1);
+                    float u = __fmul_rn(__fmul_rn(acc[0][2 * r] + acc[1][2 * r], 0x1p24f), t0);   // (not 2^24 t: it may pass the largest float)
+                    float v = __fmul_rn(__fmul_rn(acc[0][2 * r + 1] + acc[1][2 * r + 1], 0x1p24f), t1);
                     if (span > 1) u = fmaxf(u, v);
                     if (span > 2) u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, 1));
                     if (span > 4) u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, 2));
@@ -807,6 +808,7 @@ int skv_pool_select(const skv_pool_select_args* args, void* stream) {
         return fail(SKV_ERR_INVALID_ARGUMENT, "pool_select: null pointer");
     if (reinterpret_cast<uintptr_t>(a.scratch) & 15) return fail(SKV_ERR_INVALID_ARGUMENT, "pool_select: scratch is not on a 16-byte boundary");
     if (a.head_dim > 1024) return fail(SKV_ERR_UNSUPPORTED, "pool_select: head_dim %d above 1024", a.head_dim);
+    if (a.table_width > 1 << 30) return fail(SKV_ERR_TOO_LARGE, "pool_select: tables of %d pages", a.table_width);
     if (a.batch > 65535 || a.heads > 65535 || a.S_q > 0x7fffffff / kSelectCluster || (int64_t)a.batch * a.heads * a.S_q > 0x7fffffff)
         return fail(SKV_ERR_TOO_LARGE, "pool_select: %d sequences of %d heads and %d queries", a.batch, a.heads, a.S_q);
     if (a.scratch_bytes < (int64_t)skv_pool_select_scratch_bytes(a.batch, a.heads, a.S_q, a.table_width))

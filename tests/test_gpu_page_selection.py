@@ -191,6 +191,20 @@ def test_selection_is_the_definitions(skv, counts, H, rep, Sq, D, P, keep, first
         assert torch.equal(got, _select64(q, bounds, steps, table, counts, P, keep, first, recent, False, [Sq] * len(counts)))
 
 
+@pytest.mark.parametrize("rep", [1, 4, 9])
+@pytest.mark.parametrize("size", [5e33, 1e30, 1e-30, 4e-36])
+def test_selection_of_very_large_and_small_queries(skv, size, rep):
+    """Scores are whole numbers below 2^24 times powers of two: exact as long as the score itself fits a float."""
+    gen = _gen(rep)
+    kp = torch.randn(90, 2, 8, 64, generator=gen, device="cuda")
+    table = torch.randperm(90, generator=gen, device="cuda").int()[None, :88]
+    lens = _lens([700])
+    bounds, steps = skv.page_bounds(kp, table, lens)
+    q = torch.randn(1, 2 * rep, 3, 64, generator=gen, device="cuda") * size
+    want = _select64(q, bounds, steps, table, [700], 8, 11, 1, 2, False, [3])
+    assert torch.equal(skv.page_select(q, bounds, steps, table, lens, 8, 11, 1, 2, check=True), want)
+
+
 def test_selection_ties_and_pages_that_nothing_bounds(skv):
     """Equal scores go to the lowest page, pages without a finite step come first, unnamed ones last."""
     H, D, P, n = 2, 64, 4, 400
