@@ -7,10 +7,12 @@
 // launch, a block a search, joins the sums, turns the lists' logits into scores in 64 bits and merges the lists; it is set
 // up while the first still runs.
 //
+// Small searches are a launch of clusters, whose first block merges what the others found.
+//
 // What bounds it.  256 rows of 131072 16-bit logits (205 of them not finished, 54 MB): 27.4 us, of which the lists take about 20 (2.7 TB/s:
 // a warp has one block of 4 KB ahead of the one at work, and 16 warps fit an SM's registers; 24 without the block ahead were no faster, nor
-// were more parts than warps) and the merge 7, one step's latency after the other.  4 rows of 32000 fp32 logits: 9.2 us, two launches and
-// the same steps; from Python such a call costs 16.
+// were more parts than warps) and the merge 7, one step's latency after the other.  4 rows of 32000 fp32 logits: 8.5 us, the same steps and a
+// cluster's barrier; from Python such a call costs 14.
 //
 // Reordering moves what a step has to copy, about a third of the beams' last pages: 256 beams with 63 int8 tokens of 10 heads of 128 values
 // in theirs, 28 MB read and written in 11.3 us (2.6 TB/s; blocks that copy 16 KB each wait for parents, lengths, tables and rows in turn);
@@ -25,7 +27,7 @@
 namespace skv {
 
 constexpr int kBeamKeep = 128, kBeamMost = 4096;      // most continuations; most beams of a search
-constexpr int kMergeEntries = 8192;                   // entries of lists that a merge holds
+constexpr int kMergeEntries = 8192, kMergeFew = 2048;  // entries of lists that a merge holds, and is given if it can
 constexpr int kBeamWarps = 4, kBeamHeld = 256;        // warps of a block, candidates that a warp holds
 constexpr int kManyLoads = 8, kFewLoads = 4;          // 16-byte loads a lane, of a block
 constexpr int kBeamBatch = 16;                        // blocks between two looks for candidates
@@ -53,10 +55,29 @@ inline BeamShape beam_shape(int B, int beams, int V, int keep, int bytes, bool a
     };
     cut(kManyLoads);
     if (rows * s.blocks < sm_count() * 8) cut(kFewLoads);          // too few warps to fill the GPU: more and smaller blocks
-    int64_t most = kMergeEntries / keep / beams, resident = sm_count() * 16 / rows;   // 16 warps an SM at a time
+    // 16 warps an SM at a time; but a merge's time grows with its entries: 2048, or 4096 where that leaves few warps (a search of 8 beams of
+    // 131072 fp32 logits, 16 kept: 8192 entries 21.2 us, 4096 15.7, 2048 15.6, 1024 19.3; of 32 beams of 32000, 32 kept: 27, 26, 34, 51)
+    int64_t most = kMergeFew / keep / beams, resident = sm_count() * 16 / rows;
+    if (rows * most < 128) most = 2 * kMergeFew / keep / beams;
     if (most > resident) most = resident;
     if (most < 1) most = 1;
     s.parts = (int)(s.blocks < most ? s.blocks : most);
+    return s;
+}
+
+// The same for searches that a cluster of blocks takes in one launch; parts 0 where it does not: a warp would have more than 8 blocks, the clusters would
+// not be resident together, or the merge would hold more than its share.  (One launch against two, device time: a search of 4 beams of 32000
+// fp32 logits 8.1 against 8.9 us, 8 searches 9.4 and 11.4, 32 searches 10.4 and 11.5; 16 blocks a warp 13.9 and 11.0, 64 searches of 8000
+// logits 15 and 8.9.  From Python a call costs 3 us less.)
+constexpr int kCluster = 8, kClusterWarps = 8;        // blocks of a search, warps of a block
+inline BeamShape small_shape(int B, int beams, int V, int keep, int bytes, bool aligned) {
+    BeamShape s;
+    s.loads = kFewLoads;
+    s.block = 32ll * kFewLoads * (16 / bytes);
+    s.blocks = (V + (aligned ? 0 : 16 / bytes - 1) + s.block - 1) / s.block;
+    const int most = kCluster * kClusterWarps / beams;
+    s.parts = (int)(s.blocks < most ? s.blocks : most);
+    if (s.parts > 0 && (s.blocks > 8 * s.parts || (int64_t)B * kCluster > 2 * sm_count() || (int64_t)s.parts * beams * keep > kMergeFew)) s.parts = 0;
     return s;
 }
 
@@ -127,6 +148,9 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 __device__ __forceinline__ float low_of(uint64_t x) { return __uint_as_float((uint32_t)x); }
 __device__ __forceinline__ float high_of(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
 
+// The number that score_bits gives an image of.
+__device__ __forceinline__ float of_score_bits(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u); }
+
 // Whether (x, i) comes before (y, j).
 __device__ __forceinline__ bool ahead(float x, int i, float y, int j) { return x > y || (x == y && i < j); }
 
@@ -164,7 +188,7 @@ __device__ __noinline__ int beam_many(const T* x0, int first, int count, int V, 
         const int m = count_from(mid);
         if (m >= keep) { lo = mid; from_lo = m; } else hi = mid - 1;
     }
-    const float cut = __uint_as_float(lo & 0x80000000u ? lo ^ 0x80000000u : ~lo);
+    const float cut = of_score_bits(lo);
     int last = end - 1;                                       // equal ones up to here are taken
     if (from_lo > room) {                                     // (then fewer than `keep` are larger)
         int lower = begin - 1;                                // there is room for those up to here
@@ -191,23 +215,24 @@ __device__ __noinline__ int beam_many(const T* x0, int first, int count, int V, 
 // every lane and block; the keep-th largest of the lanes' largest is a bound that few (lane, block) pieces reach, about `keep` and a
 // half, and only these are read again (they are in L2 still) for their candidates.  (Candidates looked for block by block, as they
 // come, took as many instructions again as all else: 34 us for 33.5 M 16-bit logits, 20 without them.)
+struct ListShared {                                       // of a warp
+    float2 list[kBeamHeld], ranked[kBeamKeep];
+    float best[kBeamBatch][32];
+    int piece[kBeamPieces], held;
+};
 template <class T, int LOADS>
-__global__ void __launch_bounds__(32 * kBeamWarps, LOADS == kManyLoads ? 4 : 6) beam_lists_kernel(const __grid_constant__ skv_beam_args a, int parts, int64_t blocks) {
+__device__ __forceinline__ void beam_list(const skv_beam_args& a, int parts, int64_t blocks, int64_t job, ListShared& s) {
     using W = Word<T>;
     constexpr int PER = 16 / (int)sizeof(T), WORDS = 4 * LOADS, BLOCK = 32 * LOADS * PER;
-    __shared__ float2 s_list[kBeamWarps][kBeamHeld], s_ranked[kBeamWarps][kBeamKeep];
-    __shared__ float s_best[kBeamWarps][kBeamBatch][32];
-    __shared__ int s_piece[kBeamWarps][kBeamPieces], s_held[kBeamWarps];
-    start_dependents();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, keep = a.keep;
-    const int64_t job = (int64_t)blockIdx.x * kBeamWarps + warp, row = job / parts;
+    const int lane = threadIdx.x & 31, keep = a.keep;
+    const int64_t row = job / parts;
     if (row >= (int64_t)a.B * a.beams) return;
     const int part = (int)(job - row * parts);
     if (beam_dead(a, row) || beam_done(a, row)) return;   // the merge does not look at their lists
     const T* x0 = static_cast<const T*>(a.logits) + row / a.beams * a.stride_b + row % a.beams * a.stride_r;
     // 16-byte pieces on their boundaries: piece i holds logits i * PER - shift and on, the first and the last piece not all of theirs
     const int shift = (int)((reinterpret_cast<uintptr_t>(x0) & 15) / sizeof(T));
-    float2* list = s_list[warp];
+    float2* list = s.list;
     const int b0 = (int)(blocks * part / parts), b1 = (int)(blocks * (part + 1) / parts);
     float top = -INFINITY;                                // of the lane
     double sum = 0.0;
@@ -222,11 +247,11 @@ __global__ void __launch_bounds__(32 * kBeamWarps, LOADS == kManyLoads ? 4 : 6) 
                 const float2 f = list[j];
                 before += ahead(f.x, __float_as_int(f.y), e.x, __float_as_int(e.y));
             }
-            if (before < keep) s_ranked[warp][before] = e;
+            if (before < keep) s.ranked[before] = e;
         }
         __syncwarp();
         held = min(n, keep);
-        for (int i = lane; i < held; i += 32) list[i] = s_ranked[warp][i];
+        for (int i = lane; i < held; i += 32) list[i] = s.ranked[i];
         __syncwarp();
         if (held == keep) low = list[keep - 1].x;
     };
@@ -255,7 +280,6 @@ __global__ void __launch_bounds__(32 * kBeamWarps, LOADS == kManyLoads ? 4 : 6) 
     load(b0);
     for (int batch = b0; batch < b1; batch += kBeamBatch) {
         const int count = min(kBeamBatch, b1 - batch);
-        float mine = -INFINITY;                           // the lane's largest of the batch
         for (int i = 0; i < count; ++i) {
             const int block = batch + i;
             uint32_t w[WORDS];
@@ -275,8 +299,7 @@ __global__ void __launch_bounds__(32 * kBeamWarps, LOADS == kManyLoads ? 4 : 6) 
                 for (int k = 0; k < WORDS; ++k) w[k] = W::larger(w[k], none);
                 best = find_best();
             }
-            s_best[warp][i][lane] = best;
-            mine = fmaxf(mine, best);
+            s.best[i][lane] = best;
             // ---- the lane's sum, relative to its own largest logit so far
             if (best == -INFINITY) continue;
             float more;
@@ -306,7 +329,12 @@ __global__ void __launch_bounds__(32 * kBeamWarps, LOADS == kManyLoads ? 4 : 6) 
             }
         }
         // ---- candidates: larger than the keep-th best so far (equal ones come behind it), not below the bound
-        const float most = warp_max(mine);
+        float mine[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};   // the lane's largest of every fourth block
+#pragma unroll
+        for (int i = 0; i < kBeamBatch; ++i)
+            if (i < count) mine[i & 3] = fmaxf(mine[i & 3], s.best[i][lane]);
+        const uint32_t largest = score_bits(fmaxf(fmaxf(mine[0], mine[1]), fmaxf(mine[2], mine[3])));
+        const float most = of_score_bits(__reduce_max_sync(0xffffffffu, largest));
         if (most <= low || most == -INFINITY) continue;
         float from = W::kLowest;
         if (low > -INFINITY) {                            // the next number of the type
@@ -315,23 +343,40 @@ __global__ void __launch_bounds__(32 * kBeamWarps, LOADS == kManyLoads ? 4 : 6) 
             u = u & (W::N == 2 ? 0x8000u : 0x80000000u) ? u - 1 : u + 1;
             from = W::at(u, 0);
         }
-        if (keep <= 32) {
-            from = fmaxf(from, warp_ranked(mine, keep - 1));
-        } else if (count * 32 >= keep) {                  // of all that was kept: the range of their images is halved
+        // Where `keep` is near 32 the least of the lanes' largest would let many through: the keep-th largest of up to 128, which a range of
+        // images that holds it is halved to, until not many more are above its lower end.
+        if (keep <= 16) {
+            from = fmaxf(from, of_score_bits(warp_ranked(largest, keep - 1)));
+        } else if (keep <= 32 || 32 * min(count, 4) >= keep) {
             uint32_t lo = score_bits(from), hi = score_bits(most);
-            while (lo < hi) {
+            if (keep <= 32) lo = max(lo, __reduce_min_sync(0xffffffffu, largest));
+            int above = 2 * kBeamKeep;
+            while (lo < hi && above > keep + 4) {
                 const uint32_t mid = lo + (hi - lo + 1) / 2;
                 int m = 0;
-                for (int i = 0; i < count; ++i) m += score_bits(s_best[warp][i][lane]) >= mid;
-                if (__reduce_add_sync(0xffffffffu, m) >= keep) lo = mid; else hi = mid - 1;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) m += score_bits(mine[j]) >= mid;
+                m = __reduce_add_sync(0xffffffffu, m);
+                if (m >= keep) { lo = mid; above = m; } else hi = mid - 1;
             }
-            from = fmaxf(from, __uint_as_float(lo & 0x80000000u ? lo ^ 0x80000000u : ~lo));
+            from = fmaxf(from, of_score_bits(lo));
+        } else if (count * 32 >= keep) {                  // of all that was kept
+            uint32_t lo = score_bits(from), hi = score_bits(most);
+            int above = 2 * kBeamKeep;
+            while (lo < hi && above > keep + 4) {
+                const uint32_t mid = lo + (hi - lo + 1) / 2;
+                int m = 0;
+                for (int i = 0; i < count; ++i) m += score_bits(s.best[i][lane]) >= mid;
+                m = __reduce_add_sync(0xffffffffu, m);
+                if (m >= keep) { lo = mid; above = m; } else hi = mid - 1;
+            }
+            from = fmaxf(from, of_score_bits(lo));
         }
         int n = held, pieces = 0;
         for (int i = 0; i < count; ++i) {
-            const unsigned these = __ballot_sync(0xffffffffu, s_best[warp][i][lane] >= from);
+            const unsigned these = __ballot_sync(0xffffffffu, s.best[i][lane] >= from);
             const int to = pieces + __popc(these & ((1u << lane) - 1));
-            if (these >> lane & 1 && to < kBeamPieces) s_piece[warp][to] = ((batch + i) * 32 * LOADS + lane) * PER - shift;
+            if (these >> lane & 1 && to < kBeamPieces) s.piece[to] = ((batch + i) * 32 * LOADS + lane) * PER - shift;
             pieces += __popc(these);
         }
         __syncwarp();
@@ -344,7 +389,7 @@ __global__ void __launch_bounds__(32 * kBeamWarps, LOADS == kManyLoads ? 4 : 6) 
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const bool is = i + h * AT_ONCE < pieces;
-                first[h] = (is ? s_piece[warp][i + h * AT_ONCE] : 0) + lane % LOADS * 32 * PER;
+                first[h] = (is ? s.piece[i + h * AT_ONCE] : 0) + lane % LOADS * 32 * PER;
                 if (is && first[h] >= 0 && first[h] + PER <= a.V) {
                     const uint4 u = __ldg(reinterpret_cast<const uint4*>(x0 + first[h]));
                     y[h][0] = u.x; y[h][1] = u.y; y[h][2] = u.z; y[h][3] = u.w;
@@ -365,7 +410,7 @@ __global__ void __launch_bounds__(32 * kBeamWarps, LOADS == kManyLoads ? 4 : 6) 
                 }
         }
         __syncwarp();
-        if (many || n > kBeamHeld) n = beam_many(x0, batch * BLOCK - shift, count * BLOCK, a.V, from, most, keep, held, list, s_held + warp);
+        if (many || n > kBeamHeld) n = beam_many(x0, batch * BLOCK - shift, count * BLOCK, a.V, from, most, keep, held, list, &s.held);
         rank(n);
     }
     const float most = warp_max(top);
@@ -375,6 +420,13 @@ __global__ void __launch_bounds__(32 * kBeamWarps, LOADS == kManyLoads ? 4 : 6) 
     if (lane == 0) static_cast<BeamPart*>(a.scratch)[job] = BeamPart{sum, most, held};
     float2* out = reinterpret_cast<float2*>(static_cast<BeamPart*>(a.scratch) + (int64_t)a.B * a.beams * parts) + job * keep;
     for (int i = lane; i < held; i += 32) out[i] = list[i];
+}
+template <class T, int LOADS>
+__global__ void __launch_bounds__(32 * kBeamWarps, LOADS == kManyLoads ? 4 : 6) beam_lists_kernel(const __grid_constant__ skv_beam_args a, int parts, int64_t blocks) {
+    __shared__ ListShared s[kBeamWarps];
+    start_dependents();
+    const int warp = threadIdx.x >> 5;
+    beam_list<T, LOADS>(a, parts, blocks, (int64_t)blockIdx.x * kBeamWarps + warp, s[warp]);
 }
 
 // ------------------------------------------------------------------------------------------ the merge
@@ -410,15 +462,16 @@ __device__ __forceinline__ double logarithm(double x) {
 // by_parts, by_keep: 1 / parts, 1 / keep (numbers below 2^20 are divided by a product: half of a unit is more than its error).
 // A block a search.  It runs once, so its time is the latency of one step after another, instructions fetched included: loops are not
 // unrolled where that gains no overlap.
+struct MergeShared {
+    BeamBest held[kMergeHeld], best[2][kMergeThreads / 32];
+    uint32_t front[kMergeThreads / 32], top[kMergeThreads / 32];
+    int part[2][kMergeThreads / 32], n, owner[2][kMergeThreads / 32];
+};
 template <class T>
-__global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_constant__ skv_beam_args a, int parts, bool staged, float by_parts, float by_keep) {
-    extern __shared__ __align__(16) unsigned char s_raw[];
-    __shared__ BeamBest s_held[kMergeHeld];
-    __shared__ BeamBest s_best[2][kMergeThreads / 32];
-    __shared__ uint32_t s_front[kMergeThreads / 32], s_top[kMergeThreads / 32];
-    __shared__ int s_part[2][kMergeThreads / 32], s_n, s_owner[2][kMergeThreads / 32];
+__device__ __forceinline__ void beam_merge(const skv_beam_args& a, int parts, bool staged, float by_parts, float by_keep, int search,
+                                           MergeShared& s, unsigned char* s_raw) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, keep = a.keep, beams = a.beams, lists = beams * parts, all = lists * keep;
-    const int64_t row0 = (int64_t)blockIdx.x * beams;
+    const int64_t row0 = (int64_t)search * beams;
     double* s_from = reinterpret_cast<double*>(s_raw);              // [beams] what a logit less the largest is added to
     float2* s_entry = reinterpret_cast<float2*>(s_from + beams);    // staged: [lists][keep]
     uint64_t* s_score = reinterpret_cast<uint64_t*>(s_entry + (staged ? all : 0));   // staged: [lists][keep] images
@@ -429,8 +482,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
     const BeamPart* part = static_cast<const BeamPart*>(a.scratch) + row0 * parts;
     const float2* entries = reinterpret_cast<const float2*>(static_cast<const BeamPart*>(a.scratch) + (int64_t)a.B * lists) +
                             row0 * parts * keep;
-    if (tid == 0) s_n = 0;
-    wait_for_dependency();
+    if (tid == 0) s.n = 0;
     if (staged)
 #pragma unroll 4
         for (int i = tid; i < all; i += kMergeThreads) s_entry[i] = __ldcg(entries + i);
@@ -494,19 +546,19 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
         for (int l = tid; l < lists; l += kMergeThreads) front = max(front, s_upper[l * keep]);
         front = keep <= 32 && lists >= keep ? warp_ranked(front, keep - 1) : 0;
         best = __reduce_max_sync(0xffffffffu, best);
-        if (lane == 0) { s_front[warp] = front; s_top[warp] = best; }
+        if (lane == 0) { s.front[warp] = front; s.top[warp] = best; }
         __syncthreads();
-        uint32_t lo = max(__reduce_max_sync(0xffffffffu, s_front[lane % (kMergeThreads / 32)]), 1u);
-        uint32_t hi = __reduce_max_sync(0xffffffffu, s_top[lane % (kMergeThreads / 32)]), x = lo;
+        uint32_t lo = max(__reduce_max_sync(0xffffffffu, s.front[lane % (kMergeThreads / 32)]), 1u);
+        uint32_t hi = __reduce_max_sync(0xffffffffu, s.top[lane % (kMergeThreads / 32)]), x = lo;
 #pragma unroll 1
         for (bool first = true; first || (lo < hi && n > keep + 32); first = false) {
             int m = 0;
 #pragma unroll 2
             for (int i = tid; i < all; i += kMergeThreads) m += s_upper[i] >= x;
             m = __reduce_add_sync(0xffffffffu, m);
-            if (lane == 0) s_part[round & 1][warp] = m;
+            if (lane == 0) s.part[round & 1][warp] = m;
             __syncthreads();
-            m = __reduce_add_sync(0xffffffffu, lane < kMergeThreads / 32 ? s_part[round & 1][lane] : 0);
+            m = __reduce_add_sync(0xffffffffu, lane < kMergeThreads / 32 ? s.part[round & 1][lane] : 0);
             ++round;
             if (first || m >= keep) { lo = x; n = m; } else hi = x - 1;
             x = lo + (hi - lo + 1) / 2;
@@ -517,13 +569,13 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
                 if (s_upper[i] < lo) continue;
                 const int l = (int)(((float)i + 0.5f) * by_keep), r = (int)(((float)l + 0.5f) * by_parts);
                 const int token = s_count[l] < 0 ? a.pad_token : __float_as_int(s_entry[i].y);
-                s_held[atomicAdd(&s_n, 1)] = BeamBest{s_score[i], (uint64_t)r << 32 | (uint32_t)token};
+                s.held[atomicAdd(&s.n, 1)] = BeamBest{s_score[i], (uint64_t)r << 32 | (uint32_t)token};
             }
             __syncthreads();
         }
     }
     auto put = [&](int rank, const BeamBest& x) {
-        const int64_t to = (int64_t)blockIdx.x * keep + rank;
+        const int64_t to = (int64_t)search * keep + rank;
         a.values[to] = (float)score_of_image(x.score);
         a.parents[to] = (int64_t)(x.place >> 32);
         a.tokens[to] = (int64_t)(x.place & 0xffffffffu);
@@ -532,10 +584,10 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
         // a warp an entry: how many are before it
 #pragma unroll 1
         for (int i = warp; i < n; i += kMergeThreads / 32) {
-            const BeamBest x = s_held[i];
+            const BeamBest x = s.held[i];
             int rank = 0;
 #pragma unroll 1
-            for (int j = lane; j < n; j += 32) rank += s_held[j].before(x);
+            for (int j = lane; j < n; j += 32) rank += s.held[j].before(x);
             rank = __reduce_add_sync(0xffffffffu, rank);
             if (lane == 0 && rank < keep) put(rank, x);
         }
@@ -559,13 +611,13 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
                 const int y_owner = __shfl_xor_sync(0xffffffffu, owner, o);
                 if (y.before(best)) { best = y; owner = y_owner; }
             }
-            if (lane == 0) { s_best[found & 1][warp] = best; s_owner[found & 1][warp] = owner; }
+            if (lane == 0) { s.best[found & 1][warp] = best; s.owner[found & 1][warp] = owner; }
             __syncthreads();
-            best = s_best[found & 1][0];
-            owner = s_owner[found & 1][0];
+            best = s.best[found & 1][0];
+            owner = s.owner[found & 1][0];
 #pragma unroll 1
             for (int w = 1; w < kMergeThreads / 32; ++w)
-                if (s_best[found & 1][w].before(best)) { best = s_best[found & 1][w]; owner = s_owner[found & 1][w]; }
+                if (s.best[found & 1][w].before(best)) { best = s.best[found & 1][w]; owner = s.owner[found & 1][w]; }
             if (owner < 0) break;
             if (tid == 0) put(found, best);
             if (owner % kMergeThreads == tid) ++s_at[owner];
@@ -583,41 +635,72 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
             if (beam_dead(a, row0 + r)) none = true;
             else if (beam_done(a, row0 + r)) none = t != a.pad_token;
             else {
-                const float x = to_float(static_cast<const T*>(a.logits)[blockIdx.x * a.stride_b + r * a.stride_r + t]);
+                const float x = to_float(static_cast<const T*>(a.logits)[search * a.stride_b + r * a.stride_r + t]);
                 none = !(x > -INFINITY) || (s_most[r] == INFINITY && x < INFINITY);
             }
         }
         const unsigned these = __ballot_sync(0xffffffffu, none);
-        if (lane == 0) s_part[round & 1][warp] = __popc(these);
+        if (lane == 0) s.part[round & 1][warp] = __popc(these);
         __syncthreads();
         int before = 0, total = 0;
 #pragma unroll 1
         for (int w = 0; w < kMergeThreads / 32; ++w) {
-            if (w < warp) before += s_part[round & 1][w];
-            total += s_part[round & 1][w];
+            if (w < warp) before += s.part[round & 1][w];
+            total += s.part[round & 1][w];
         }
         const int to = found + before + __popc(these & ((1u << lane) - 1));
         if (none && to < keep) {
-            a.values[(int64_t)blockIdx.x * keep + to] = -INFINITY;
-            a.parents[(int64_t)blockIdx.x * keep + to] = r;
-            a.tokens[(int64_t)blockIdx.x * keep + to] = t;
+            a.values[(int64_t)search * keep + to] = -INFINITY;
+            a.parents[(int64_t)search * keep + to] = r;
+            a.tokens[(int64_t)search * keep + to] = t;
         }
         found += total;
     }
 }
 
 template <class T>
+__global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_constant__ skv_beam_args a, int parts, bool staged, float by_parts, float by_keep) {
+    extern __shared__ __align__(16) unsigned char s_raw[];
+    __shared__ MergeShared s;
+    wait_for_dependency();
+    beam_merge<T>(a, parts, staged, by_parts, by_keep, blockIdx.x, s, s_raw);
+}
+
+// Small searches in one launch: a cluster of blocks makes a search's lists, and its first block merges them.
+static_assert(kMergeThreads == 32 * kClusterWarps);
+template <class T>
+__global__ void __launch_bounds__(kMergeThreads, 2) beam_small_kernel(const __grid_constant__ skv_beam_args a, int parts, int64_t blocks, float by_parts, float by_keep) {
+    extern __shared__ __align__(16) unsigned char s_raw[];       // the warps' lists, then the merge's
+    int rank;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    const int warp = threadIdx.x >> 5, search = blockIdx.x / kCluster, job = rank + kCluster * warp, lists = a.beams * parts;
+    wait_for_dependency();
+    if (job < lists) beam_list<T, kFewLoads>(a, parts, blocks, (int64_t)search * lists + job, reinterpret_cast<ListShared*>(s_raw)[warp]);
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    if (rank == 0) beam_merge<T>(a, parts, true, by_parts, by_keep, search, *reinterpret_cast<MergeShared*>(s_raw), s_raw + sizeof(MergeShared));
+}
+
+template <class T>
 int launch_beam(const skv_beam_args& a, cudaStream_t st) {
     const bool aligned = (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 && a.stride_b % (16 / (int)sizeof(T)) == 0 &&
                          a.stride_r % (16 / (int)sizeof(T)) == 0;
+    const BeamShape small = small_shape(a.B, a.beams, a.V, a.keep, sizeof(T), aligned);
+    if (small.parts > 0) {
+        const size_t entries = (size_t)a.beams * small.parts * a.keep, merge = sizeof(MergeShared) + a.beams * 12 + a.beams * small.parts * 8 + entries * 20;
+        const size_t smem = merge > kClusterWarps * sizeof(ListShared) ? merge : kClusterWarps * sizeof(ListShared);   // 45 to 65 KB
+        const cudaError_t e = cudaFuncSetAttribute(beam_small_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
+        if (e != cudaSuccess) return fail(SKV_ERR_CUDA, "beam_select: %s", cudaGetErrorString(e));
+        launch_cluster_after(beam_small_kernel<T>, dim3((unsigned)a.B * kCluster), dim3(kCluster), kMergeThreads, smem, st, a, small.parts, small.blocks,
+                             1.0f / (float)small.parts, 1.0f / (float)a.keep);
+        return check_launch("beam_select");
+    }
     const BeamShape s = beam_shape(a.B, a.beams, a.V, a.keep, sizeof(T), aligned);
     const int64_t jobs = (int64_t)a.B * a.beams * s.parts;
     const unsigned grid = (unsigned)((jobs + kBeamWarps - 1) / kBeamWarps);
     prefer_shared<beam_lists_kernel<T, kManyLoads>>(50);   // (32 searches of 8 beams 32.5 -> 27.7 us)
     prefer_shared<beam_lists_kernel<T, kFewLoads>>(50);
     prefer_shared<beam_merge_kernel<T>>(50);
-    static std::mutex launches;   // a call's two launches stay together: host threads may share a stream and its scratch
-    const std::lock_guard<std::mutex> both(launches);
     if (s.loads == kManyLoads) beam_lists_kernel<T, kManyLoads><<<grid, 32 * kBeamWarps, 0, st>>>(a, s.parts, s.blocks);
     else beam_lists_kernel<T, kFewLoads><<<grid, 32 * kBeamWarps, 0, st>>>(a, s.parts, s.blocks);
     if (const int rc = check_launch("beam_select")) return rc;
@@ -773,7 +856,9 @@ size_t skv_beam_scratch_bytes(int B, int beams, int V, int keep) {
     int parts = 1;   // of whichever type and alignment has most
     for (int i = 0; i < 4; ++i) {
         const int some = beam_shape(B, beams, V, keep, i & 1 ? 2 : 4, i & 2).parts;
+        const int few = small_shape(B, beams, V, keep, i & 1 ? 2 : 4, i & 2).parts;
         if (some > parts) parts = some;
+        if (few > parts) parts = few;
     }
     return (size_t)B * beams * parts * (sizeof(BeamPart) + (size_t)keep * 8);
 }
@@ -799,6 +884,8 @@ int skv_beam_select(const skv_beam_args* args, void* stream) {
     if (a.scratch_bytes < (int64_t)skv_beam_scratch_bytes(a.B, a.beams, a.V, a.keep))
         return fail(SKV_ERR_SCRATCH, "beam_select: scratch of %lld bytes", (long long)a.scratch_bytes);
     cudaStream_t st = as_stream(stream);
+    static std::mutex launches;   // a call's two launches stay together: host threads may share a stream and its scratch
+    const std::lock_guard<std::mutex> both(launches);
     if (a.dtype == kF32) return launch_beam<float>(a, st);
     if (a.dtype == kF16) return launch_beam<__half>(a, st);
     return launch_beam<__nv_bfloat16>(a, st);

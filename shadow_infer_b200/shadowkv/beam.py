@@ -43,7 +43,7 @@ def beam_select(
     A ``finished`` beam (bool ``[B, beams]``) has a single continuation: ``pad_token``, at the score that it has.
     Tokens that are not allowed have logits of -inf; a NaN counts as one, and logits of +inf share their beam's whole probability.
     A beam whose score is not finite (a search that starts from one beam gives the others -inf), or to which no token is allowed,
-    has continuations of -inf only.  Where fewer than ``keep`` are better, the first of those fill up the result.  Two launches.
+    has continuations of -inf only.  Where fewer than ``keep`` are better, the first of those fill up the result.  One launch, or two.
     """
     if logits.dim() != 3:
         raise ValueError(f"logits must be [batch, beams, vocabulary], got {tuple(logits.shape)}")

@@ -67,6 +67,7 @@ def _check(skv, logits, scores, keep, finished=None, pad=0):
 BEAM = [  # B, beams, V, keep
     (1, 1, 1, 1), (1, 1, 7, 7), (2, 3, 5, 15), (1, 4, 32000, 4), (3, 2, 4096, 9), (2, 5, 4097, 10), (2, 3, 8191, 128), (5, 3, 40009, 7),
     (1, 1, 300000, 128), (7, 16, 1000, 32), (2, 64, 5000, 64), (1, 1500, 64, 100), (300, 2, 333, 4),
+    (37, 2, 4500, 17), (38, 2, 4500, 17), (1, 2, 9000, 32), (3, 2, 70000, 24), (40, 1, 60000, 33), (1, 64, 700, 8), (1, 65, 700, 8), (2, 8, 131072, 16),
 ]
 
 
@@ -83,7 +84,8 @@ def test_selection_is_the_definitions(skv, B, beams, V, keep, dtype):
 
 
 @pytest.mark.parametrize("dtype", FLOATS)
-def test_equal_logits_go_to_the_lowest(skv, dtype):
+@pytest.mark.parametrize("copies", [1, 20])                  # searches of one launch, of two
+def test_equal_logits_go_to_the_lowest(skv, dtype, copies):
     """Everything alike, alike but for a few, alike in steps: more candidates than a block's list holds."""
     B, beams, V = 2, 2, 20000
     for case in range(5):
@@ -98,15 +100,16 @@ def test_equal_logits_go_to_the_lowest(skv, dtype):
             logits[:, 1:] = -0.0
         for keep in (1, 5, 33, 128):
             scores = torch.tensor([[-1.0, -1.0], [-2.0, -5.0]], device="cuda")
-            values, parents, tokens = skv.beam_select(logits, scores, keep)
+            values, parents, tokens = skv.beam_select(logits.repeat(copies, 1, 1), scores.repeat(copies, 1), keep)
             every = _continuations(logits, scores, None, 0)
             at = torch.sort((every * 2 ** 30).round(), dim=1, descending=True, stable=True).indices[:, :keep]
-            assert torch.equal(parents * V + tokens, at), (case, keep)
+            assert torch.equal(parents * V + tokens, at.repeat(copies, 1)), (case, keep)
 
 
 @pytest.mark.parametrize("dtype", FLOATS)
 @pytest.mark.parametrize("V", [50, 9001])
-def test_masked_logits_and_beams_that_end(skv, dtype, V):
+@pytest.mark.parametrize("copies", [1, 7])                   # searches of one launch, of two
+def test_masked_logits_and_beams_that_end(skv, dtype, V, copies):
     """Masks of -inf and of the type's lowest value, rows that nothing is left of, infinities, NaN, scores that are not finite."""
     B, beams = 6, 4
     gen = _gen(V)
@@ -122,6 +125,7 @@ def test_masked_logits_and_beams_that_end(skv, dtype, V):
     scores[5] = -math.inf
     done = torch.zeros(B, beams, dtype=torch.bool, device="cuda")
     done[1, 2] = done[4, 0] = done[5, 1] = done[3, 1] = True
+    logits, scores, done = logits.repeat(copies, 1, 1), scores.repeat(copies, 1), done.repeat(copies, 1)
     for keep in (1, 4, 13, 40, 128):
         _check(skv, logits, scores, keep)
         _check(skv, logits, scores, keep, done, 2)
@@ -204,17 +208,17 @@ def test_more_beams_than_a_merge_holds_entries_for(skv):
         _check(skv, torch.zeros_like(logits), torch.linspace(0, -1, beams, device="cuda")[None], keep)
 
 
-def test_selection_from_two_threads_on_one_stream(skv):
+def test_selection_from_threads_on_one_stream(skv):
     """A call's launches share a scratch that the stream's other calls use too."""
     import threading
 
     calls = []
-    for seed, (B, beams, V, keep) in enumerate(((4, 4, 30000, 8), (2, 7, 50001, 12))):
-        x = torch.randn(B, beams, V, generator=_gen(seed), device="cuda")
+    for seed, (B, beams, V, keep) in enumerate(((4, 4, 30000, 8), (2, 7, 50001, 12), (40, 3, 20001, 12))):   # one launch, two, two of another type
+        x = torch.randn(B, beams, V, generator=_gen(seed), device="cuda").to(torch.float16 if seed == 2 else torch.float32)
         calls.append(lambda x=x, keep=keep: skv.beam_select(x, torch.zeros(x.shape[:2], device="cuda"), keep))
     want = [call() for call in calls]
     torch.cuda.synchronize()
-    wrong, go = [], threading.Barrier(2)
+    wrong, go = [], threading.Barrier(3)
 
     def work(i):
         go.wait()
@@ -222,7 +226,7 @@ def test_selection_from_two_threads_on_one_stream(skv):
             if not all(torch.equal(a, b) for a, b in zip(calls[i](), want[i])):
                 wrong.append(i)
 
-    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
     for t in threads:
         t.start()
     for t in threads:

@@ -67,6 +67,7 @@ def test_select_refuses_before_a_launch():
     assert select(q=(16, 8, 8, 8, 0, 3)) == _lib.SKV_ERR_SHAPE
     assert select(D=1032) == _lib.SKV_ERR_UNSUPPORTED
     assert select(B=1 << 20) == large and select(S=1 << 30) == large and select(H=1 << 17, q=(16, 8, 8, 8, 0, 1 << 17)) == large
+    assert select(width=(1 << 30) + 1) == large
     assert select(room=15) == _lib.SKV_ERR_SCRATCH
     assert select(B=0) == _lib.SKV_OK and select(S=0) == _lib.SKV_OK
     assert lib.skv_pool_select_scratch_bytes(3, 2, 5, 7) >= 3 * 2 * 5 * 7 * 4 and lib.skv_pool_select_scratch_bytes(-1, 2, 5, 7) == 0
