@@ -18,7 +18,7 @@
 // tokens: 131071 int8 tokens with fp32 queries in 76 us (57 % of the copy rate), 32768 int4 tokens of 32 heads in 82 us (38 %).
 // fp32: 16 KB a tile leave room for 4 warps an SM, 16384 tokens in 36 us (57 %).  Small calls: 4 to 5 us until the first rows
 // are there, 1.7 us a unit and 3 to 6 us for a join; 512 tokens of 32 heads in 12 us, 8 int8 sequences of up to 2048 tokens in 18.
-// Lists of pages: a unit's table is made first, 2 to 4 us; 32 units of 2048 int4 tokens in 19 us, 8 of 4096 int8 tokens in 16, 512 of 512 int8
+// Lists of pages: a unit's table is made first, 2 to 4 us; 32 units of 2048 int4 tokens in 19 us, 8 of 4096 int8 tokens in 16, of 512 in 11, 512 of 512 int8
 // tokens in 26 (from L2: the rounds' instructions), 512 of up to 1024 fp16 tokens in 52 with its tables' launch (256 MB, 5 TB/s).
 //
 // Exactness.  Page values enter the MMAs exactly: fp16 as it is, int8 and int4 as small integers, fp32 as two terms of 11 bits
@@ -1092,11 +1092,14 @@ int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
         const int64_t units = (int64_t)a.pool.batch * row_tiles, resident = (int64_t)sm_count() * Shape::CTAS;
         const int64_t most = (token_cap(a) + 16 * Shape::W - 1) / (16 * Shape::W), rounds = (units + resident - 1) / resident;
         int64_t splits = resident / units < most ? resident / units : most;
-        // One CTA an SM where it has 4 tiles at most, or 8 and nothing to join: two on an SM would have fewer, slower ones, and a longer join (8 units
-        // of 4096 int8 tokens 18.5 -> 16.4 us, 16 of 2048 fp16 tokens 17.2 -> 14.8, 128 of 512 int8 tokens 15.8 -> 11.6; 8 tiles and a join: 32 of
-        // 2048 fp16 tokens 15.8 -> 17.5).
-        const int64_t single = sm_count() / units, each = single > 0 ? (most + single - 1) / single : 0;
-        if (single > 0 && single < splits && each <= (single == 1 ? 8 : 4)) splits = single;
+        // Units of 4 tiles stay whole, of 8 where two CTAs would be the cut: there is nothing to join then.  Else one CTA an SM where it has 256 tokens
+        // at most: two on an SM would have fewer, slower ones, and a longer join.  (With the choice of pages before it: 8 units of 512 int8 tokens
+        // 21.3 -> 17.9 us, 128 of 512 28.0 -> 23.3, 64 of 512 fp16 tokens 22.6 -> 20.2; 8 of 4096 int8 tokens 26.1 -> 24.7, 16 of 2048 fp16 tokens
+        // 24.7 -> 23.3.  With twice the tokens 32 of 2048 fp16 or int8 tokens 24.2 -> 26.0, 24.0 -> 25.3.  int4, whose tiles are
+        // more instructions: 32 of 1024 tokens 23.3 -> 24.3, 64 whole ones 26.3 -> 27.1.)
+        const int64_t single = sm_count() / units;
+        if (most <= 4 || (most <= 8 && (single == 1 || (single == 2 && PREC != 3)))) splits = 1;
+        else if (PREC != 3 && single > 0 && single < splits && (most + single - 1) / single * 16 * Shape::W <= 256) splits = single;
         if (splits < 1) splits = 1;
         if (units * (most > splits ? most : splits) < (1ll << 30) && (rounds == 1 || 4 * units >= 3 * rounds * resident)) {
             skv_pool_attention_args part = a;
