@@ -151,9 +151,10 @@ def test_rows_of_any_alignment_and_stride(skv, dtype):
                        skv.beam_select(x, torch.zeros(beams, B, device="cuda"))[2])
 
 
-def test_selection_in_a_graph_on_streams_and_for_host_tensors(skv):
+@pytest.mark.parametrize("B", [3, 40])                       # one launch, two
+def test_selection_in_a_graph_on_streams_and_for_host_tensors(skv, B):
     gen = _gen(12)
-    logits, scores = torch.randn(3, 4, 9000, generator=gen, device="cuda"), torch.zeros(3, 4, device="cuda")
+    logits, scores = torch.randn(B, 4, 9000, generator=gen, device="cuda"), torch.zeros(B, 4, device="cuda")
     logits.requires_grad_(True)
     want = skv.beam_select(logits, scores)
     assert not want[0].requires_grad
@@ -169,7 +170,7 @@ def test_selection_in_a_graph_on_streams_and_for_host_tensors(skv):
     with torch.cuda.graph(graph):
         got = skv.beam_select(logits, scores, 7)
     for _ in range(2):
-        logits.copy_(torch.randn(3, 4, 9000, generator=gen, device="cuda"))
+        logits.copy_(torch.randn(B, 4, 9000, generator=gen, device="cuda"))
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(got, skv.beam_select(logits, scores, 7)))
 
