@@ -344,6 +344,27 @@ def test_attention_of_listed_pages(skv, counts, H, rep, Sq, D, P, G, causal, kee
         assert (got[want == 0] == 0).all() or (want == 0).sum() < D
 
 
+CUTS = [  # counts, H, rep, keep: units of 1 to 150, of few and of many tokens, whole or over some CTAs
+    ([4096], 8, 4, 128), ([2048, 40], 8, 4, 64), ([2048, 2000], 8, 1, 63), ([3000, 3000, 10], 20, 1, 90), ([1100] * 2, 32, 2, 32),
+    ([600] * 4, 37, 1, 16), ([1000] * 5, 30, 1, 20), ([512], 1, 8, 16), ([5000], 1, 1, 157), ([250] * 10, 10, 1, 8), ([1024] * 8, 16, 1, 31),
+]
+
+
+@pytest.mark.parametrize("counts,H,rep,keep", CUTS)
+@pytest.mark.parametrize("kv", ["fp32", "fp16", "int8", "int4"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_attention_of_listed_pages_however_units_are_cut(skv, counts, H, rep, keep, kv, dtype):
+    pages_kv, scales, table, lens = _filled(skv, kv, counts, H, 32, 128, 16, sum(counts))
+    gen = _gen(keep)
+    B = len(counts)
+    q = _rows(gen, B, H * rep, 1, 128, dtype, "bhsd")
+    pages = torch.rand(B, H, 1, max(keep, table.shape[1]), generator=gen, device="cuda").argsort(-1)[..., :keep].sort(-1).values.int()
+    got = skv.paged_attention(q, *pages_kv, table, lens, *scales, pages=pages)
+    want, bound = _sparse64(q, pages_kv, scales, table, counts, [1] * B, False, pages)
+    assert ((got.double() - want).abs() <= bound).all()
+    assert torch.equal(skv.paged_attention(q, *pages_kv, table, lens, *scales, pages=pages), got)
+
+
 def test_listed_pages_broadcast_and_tell_nothing_else(skv):
     """Lists are broadcast, 64-bit lists are not cut, and what is in a list besides its pages changes nothing."""
     counts, H, P, D = [200, 90], 2, 16, 64
