@@ -7,12 +7,12 @@
 // launch, a block a search, joins the sums, turns the lists' logits into scores in 64 bits and merges the lists; it is set
 // up while the first still runs.
 //
-// Small searches are a launch of clusters, whose first block merges what the others found.
+// Few searches, or small ones, are one launch of clusters, whose first block merges what the others found.
 //
-// What bounds it.  256 rows of 131072 16-bit logits (205 of them not finished, 54 MB): 27.4 us, of which the lists take about 20 (2.7 TB/s:
+// What bounds it.  256 rows of 131072 16-bit logits (205 of them not finished, 54 MB): 26.4 us, of which the lists take about 20 (2.7 TB/s:
 // a warp has one block of 4 KB ahead of the one at work, and 16 warps fit an SM's registers; 24 without the block ahead were no faster, nor
-// were more parts than warps) and the merge 7, one step's latency after the other.  4 rows of 32000 fp32 logits: 8.5 us, the same steps and a
-// cluster's barrier; from Python such a call costs 14.
+// were more parts than warps) and the merge 6, one step's latency after the other (in two launches 27.4).  4 rows of 32000 fp32 logits: 8.5 us,
+// the same steps; from Python such a call costs 14.
 //
 // Reordering moves what a step has to copy, about a third of the beams' last pages: 256 beams with 63 int8 tokens of 10 heads of 128 values
 // in theirs, 28 MB read and written in 11.3 us (2.6 TB/s; blocks that copy 16 KB each wait for parents, lengths, tables and rows in turn);
@@ -65,19 +65,26 @@ inline BeamShape beam_shape(int B, int beams, int V, int keep, int bytes, bool a
     return s;
 }
 
-// The same for searches that a cluster of blocks takes in one launch; parts 0 where it does not: a warp would have more than 8 blocks, the clusters would
-// not be resident together, or the merge would hold more than its share.  (One launch against two, device time: a search of 4 beams of 32000
-// fp32 logits 8.1 against 8.9 us, 8 searches 9.4 and 11.4, 32 searches 10.4 and 11.5; 16 blocks a warp 13.9 and 11.0, 64 searches of 8000
-// logits 15 and 8.9.  From Python a call costs 3 us less.)
+// The same for searches that a cluster of blocks takes in one launch; parts 0 where it does not: the clusters would not be resident together, or would
+// leave SMs idle while a warp has more than 8 blocks, or the merge would hold more than its share.  (One launch against two, device time: a
+// search of 4 beams of 32000 fp32 logits 8.1 against 8.9 us, 8 searches 9.4 and 11.4, 32 searches 10.4 and 11.5, 64 searches 20.9 and 15.7;
+// 16 blocks a warp: one search 13.9 and 11.0.  8 beams of 131072 bf16 logits: 16 searches 24.1 and 21.2, 24 25.5 and 25.1, 32 25.8 and
+// 26.9, 37 37.6 and 27.9.  From Python a call costs 3 us less.)
 constexpr int kCluster = 8, kClusterWarps = 8;        // blocks of a search, warps of a block
 inline BeamShape small_shape(int B, int beams, int V, int keep, int bytes, bool aligned) {
     BeamShape s;
-    s.loads = kFewLoads;
-    s.block = 32ll * kFewLoads * (16 / bytes);
-    s.blocks = (V + (aligned ? 0 : 16 / bytes - 1) + s.block - 1) / s.block;
     const int most = kCluster * kClusterWarps / beams;
-    s.parts = (int)(s.blocks < most ? s.blocks : most);
-    if (s.parts > 0 && (s.blocks > 8 * s.parts || (int64_t)B * kCluster > 2 * sm_count() || (int64_t)s.parts * beams * keep > kMergeFew)) s.parts = 0;
+    auto cut = [&](int loads) {
+        s.loads = loads;
+        s.block = 32ll * loads * (16 / bytes);
+        s.blocks = (V + (aligned ? 0 : 16 / bytes - 1) + s.block - 1) / s.block;
+        s.parts = (int)(s.blocks < most ? s.blocks : most);
+    };
+    cut(kFewLoads);
+    const bool short_rows = s.blocks <= 8 * s.parts, fill = 4ll * B * kCluster >= 5 * sm_count();
+    const bool resident = 4ll * B * kCluster <= 7 * sm_count();   // (not all SMs of a GPC make up clusters)
+    if (!short_rows && s.parts > 0) cut(kManyLoads);
+    if (!(short_rows || fill) || !resident || (int64_t)s.parts * beams * keep > kMergeFew) s.parts = 0;
     return s;
 }
 
@@ -666,16 +673,16 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
     beam_merge<T>(a, parts, staged, by_parts, by_keep, blockIdx.x, s, s_raw);
 }
 
-// Small searches in one launch: a cluster of blocks makes a search's lists, and its first block merges them.
+// The same in one launch: a cluster of blocks makes a search's lists, and its first block merges them.
 static_assert(kMergeThreads == 32 * kClusterWarps);
-template <class T>
+template <class T, int LOADS>
 __global__ void __launch_bounds__(kMergeThreads, 2) beam_small_kernel(const __grid_constant__ skv_beam_args a, int parts, int64_t blocks, float by_parts, float by_keep) {
     extern __shared__ __align__(16) unsigned char s_raw[];       // the warps' lists, then the merge's
     int rank;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     const int warp = threadIdx.x >> 5, search = blockIdx.x / kCluster, job = rank + kCluster * warp, lists = a.beams * parts;
     wait_for_dependency();
-    if (job < lists) beam_list<T, kFewLoads>(a, parts, blocks, (int64_t)search * lists + job, reinterpret_cast<ListShared*>(s_raw)[warp]);
+    if (job < lists) beam_list<T, LOADS>(a, parts, blocks, (int64_t)search * lists + job, reinterpret_cast<ListShared*>(s_raw)[warp]);
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
     if (rank == 0) beam_merge<T>(a, parts, true, by_parts, by_keep, search, *reinterpret_cast<MergeShared*>(s_raw), s_raw + sizeof(MergeShared));
@@ -689,9 +696,10 @@ int launch_beam(const skv_beam_args& a, cudaStream_t st) {
     if (small.parts > 0) {
         const size_t entries = (size_t)a.beams * small.parts * a.keep, merge = sizeof(MergeShared) + a.beams * 12 + a.beams * small.parts * 8 + entries * 20;
         const size_t smem = merge > kClusterWarps * sizeof(ListShared) ? merge : kClusterWarps * sizeof(ListShared);   // 45 to 65 KB
-        const cudaError_t e = cudaFuncSetAttribute(beam_small_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
+        const auto kernel = small.loads == kManyLoads ? beam_small_kernel<T, kManyLoads> : beam_small_kernel<T, kFewLoads>;
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
         if (e != cudaSuccess) return fail(SKV_ERR_CUDA, "beam_select: %s", cudaGetErrorString(e));
-        launch_cluster_after(beam_small_kernel<T>, dim3((unsigned)a.B * kCluster), dim3(kCluster), kMergeThreads, smem, st, a, small.parts, small.blocks,
+        launch_cluster_after(kernel, dim3((unsigned)a.B * kCluster), dim3(kCluster), kMergeThreads, smem, st, a, small.parts, small.blocks,
                              1.0f / (float)small.parts, 1.0f / (float)a.keep);
         return check_launch("beam_select");
     }

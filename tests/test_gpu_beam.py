@@ -67,7 +67,7 @@ def _check(skv, logits, scores, keep, finished=None, pad=0):
 BEAM = [  # B, beams, V, keep
     (1, 1, 1, 1), (1, 1, 7, 7), (2, 3, 5, 15), (1, 4, 32000, 4), (3, 2, 4096, 9), (2, 5, 4097, 10), (2, 3, 8191, 128), (5, 3, 40009, 7),
     (1, 1, 300000, 128), (7, 16, 1000, 32), (2, 64, 5000, 64), (1, 1500, 64, 100), (300, 2, 333, 4),
-    (37, 2, 4500, 17), (38, 2, 4500, 17), (1, 2, 9000, 32), (3, 2, 70000, 24), (40, 1, 60000, 33), (1, 64, 700, 8), (1, 65, 700, 8), (2, 8, 131072, 16),
+    (37, 2, 4500, 17), (38, 2, 4500, 17), (1, 2, 9000, 32), (3, 2, 70000, 24), (40, 1, 60000, 33), (1, 64, 700, 8), (1, 65, 700, 8), (2, 8, 131072, 16), (25, 8, 70001, 16),
 ]
 
 
@@ -176,7 +176,7 @@ def test_selection_in_a_graph_on_streams_and_for_host_tensors(skv, B):
 
 
 @pytest.mark.parametrize("B,beams,V,keep", [(125, 4, 4096, 5), (125, 4, 2048, 5), (148, 4, 1024, 8), (1, 1, 100000, 3), (2, 16, 33000, 32),
-                                            (74, 8, 6144, 16), (1, 4, 512, 4)])
+                                            (74, 8, 6144, 16), (1, 4, 512, 4), (32, 8, 70000, 16)])
 @pytest.mark.parametrize("dtype", FLOATS)
 @pytest.mark.parametrize("shift", [0, 1])
 def test_scratch_is_as_large_as_said(skv, B, beams, V, keep, dtype, shift):
