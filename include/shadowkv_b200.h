@@ -598,8 +598,10 @@ typedef struct skv_pool_reorder_args {
  * last page that is partly filled must be its sequence's own: it goes to the parent itself, if it goes on from itself, else to the
  * first child; the n-th of the other children takes the page that the n-th beam without children has in
  * that place of its table, and the tokens (and bounds) are copied there.  The beams of a group are equally long (else that
- * place may be empty: its table entry is -1 then and error_flag set, as by a parent outside the group, whose child is empty).
- * Table entries behind the tokens (pages taken ahead) stay where they are.  The new table and lengths share no memory with the old.
+ * place may be empty, or a full page, which others may share and which is not taken: the table entry is -1 then and error_flag set, as by
+ * a parent outside the group, whose child is empty).
+ * Table entries behind the tokens (pages taken ahead) stay where they are; where a beam was longer, those of its former tokens are -1, and
+ * error_flag is set.  The new table and lengths share no memory with the old.
  * beams <= 1024. */
 int skv_pool_reorder(const skv_pool_reorder_args* args, void* stream);
 

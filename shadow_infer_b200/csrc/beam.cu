@@ -750,7 +750,9 @@ __device__ __noinline__ void move_block(char* to, const char* from, int bytes) {
 // A block a beam and a share of its last page's (key head, K or V) blocks.  Every block finds out by itself where its beam comes from: a
 // beam is the keeper of its parent's last page if it is the parent, or the first child of a parent that does not go on from itself; the
 // n-th beam that is no keeper takes the last page of the n-th beam without children.  Pages are copied from keepers' parents, which have
-// children, to pages of beams that have none, so no block reads what another writes; the old table is only read.
+// children, to pages of beams that have none, so no block reads what another writes; the old table is only read.  A full page may be
+// shared, so one is neither taken from a beam without children nor left behind the tokens of a beam that was longer (beams of a group
+// that are not equally long).
 __global__ void __launch_bounds__(kReorderThreads, 5) pool_reorder_kernel(const __grid_constant__ skv_pool_reorder_args a) {
     __shared__ int s_parent[kReorderBeams];
     __shared__ bool s_extra[kReorderBeams], s_childless[kReorderBeams];
@@ -817,7 +819,8 @@ __global__ void __launch_bounds__(kReorderThreads, 5) pool_reorder_kernel(const 
     int target = -1;
     if (copy) {
         const int source = __ldg(old + j);
-        if (donor >= 0) target = __ldg(a.pool.block_table + (row0 + donor) * a.pool.table_stride + j);
+        if (donor >= 0 && max(0, __ldg(a.lengths + row0 + donor)) / P <= j)   // (else its page there is full)
+            target = __ldg(a.pool.block_table + (row0 + donor) * a.pool.table_stride + j);
         if (target < 0 || target >= a.pool.num_pages || source < 0 || source >= a.pool.num_pages || source == target) {
             target = -1;
             if (a.error_flag && tid == 0) atomicExch(a.error_flag, 1);
@@ -845,11 +848,12 @@ __global__ void __launch_bounds__(kReorderThreads, 5) pool_reorder_kernel(const 
     if (blockIdx.y) return;
     int32_t* table = a.new_table + row * width;
     const int32_t* own = a.pool.block_table + row * a.pool.table_stride;
+    const int behind = j + (rows > 0), had = max(0, __ldg(a.lengths + row)), held = had > 0 ? (had - 1) / P + 1 : 0;   // pages; of its own
     for (int i = tid; i < width; i += kReorderThreads)
-        table[i] = p < 0 ? -1 : copy && i == j ? target : __ldg((i < j + (rows > 0) ? old : own) + i);
+        table[i] = p < 0 || (i >= behind && i < held) ? -1 : copy && i == j ? target : __ldg((i < behind ? old : own) + i);
     if (tid == 0) {
         a.new_lengths[row] = length;
-        if (a.error_flag && (p < 0 || length < 0 || tokens > (int64_t)width * P)) atomicExch(a.error_flag, 1);
+        if (a.error_flag && (p < 0 || length < 0 || tokens > (int64_t)width * P || held > behind)) atomicExch(a.error_flag, 1);
     }
 }
 

@@ -121,7 +121,8 @@ def paged_reorder(
     it ends.
 
     Pages are changed in place, the tables are new tensors.  A parent outside its group leaves an empty sequence, a last page
-    that cannot be had a table entry of -1; ``check=True`` waits and raises ``ValueError`` for them.  One launch.
+    that cannot be had a table entry of -1 (beams that are not equally long: a full page may be shared and is never given away, and entries
+    that held a longer beam's own tokens are -1); ``check=True`` waits and raises ``ValueError`` for them.  One launch.
     """
     if parents.dim() != 2:
         raise ValueError(f"parents must be [groups, beams], got {tuple(parents.shape)}")

@@ -551,7 +551,8 @@ class PagedKVPool:
         table = self._with_pages(places, taken) if taken else self.block_table
         at = _staged(torch.tensor(rows, dtype=torch.int64), self.lengths.device)
         parents = torch.zeros(1, len(rows), dtype=torch.int64, device=self.lengths.device)
-        new_table, new_lengths = paged_reorder(self.k_pages, self.v_pages, table[at], self.lengths[at], parents, self.scale_k, self.scale_v,
+        lengths = self.lengths[at[:1]].expand(len(rows)).contiguous()
+        new_table, new_lengths = paged_reorder(self.k_pages, self.v_pages, table[at], lengths, parents, self.scale_k, self.scale_v,
                                                self.bounds, self.steps, self.head_dim)
         self.block_table.index_copy_(0, at, new_table)
         self.lengths.index_copy_(0, at, new_lengths)

@@ -349,6 +349,40 @@ def test_reordering_names_bad_parents_and_pages(skv):
         skv.paged_reorder(kp, kp.clone(), table, lens, torch.zeros(3, 2, dtype=torch.int64, device="cuda"))
 
 
+@pytest.mark.parametrize("beams", [3, 40])                   # a warp's beams, a block's
+def test_reordering_leaves_full_pages_of_longer_beams_alone(skv, beams):
+    """A beam without children that is longer than a child has a full page, which others share, where the child wants one."""
+    kp = torch.randn(2 * beams + 3, 1, 4, 8, generator=_gen(1), device="cuda")
+    vp, bounds = kp + 1, torch.randint(-9, 9, (2 * beams + 3, 1, 2, 8), dtype=torch.int8, device="cuda")
+    steps = torch.rand(2 * beams + 3, 1, device="cuda")
+    # beam 0: 6 tokens in pages 0 and 1; beams 1 and 2: 11 tokens in pages 2 and 3, which they share, and one of their own; the others: 6 tokens
+    table = torch.full((beams, 3), -1, dtype=torch.int32)
+    lens = torch.full((beams,), 6, dtype=torch.int32)
+    table[0, :2] = torch.tensor([0, 1])
+    table[1], table[2] = torch.tensor([2, 3, 4]), torch.tensor([2, 3, 5])
+    lens[1:3] = 11
+    for r in range(3, beams):
+        table[r, :2] = torch.tensor([2 * r, 2 * r + 1])
+    table, lens = table.cuda(), lens.cuda()
+    parents = torch.arange(beams, device="cuda")[None].clone()
+    parents[0, 1] = 0                                        # beam 1 goes on from beam 0, beam 2 from itself
+    was = [t.clone() for t in (kp, vp, bounds, steps)]
+    for check in (False, True):
+        if check:
+            with pytest.raises(ValueError, match="outside"):
+                skv.paged_reorder(kp, vp, table, lens, parents, bounds=bounds, steps=steps, check=True)
+        else:
+            got, n = skv.paged_reorder(kp, vp, table, lens, parents, bounds=bounds, steps=steps)
+            assert got[:3].tolist() == [[0, 1, -1], [0, -1, -1], [2, 3, 5]] and n[:3].tolist() == [6, 6, 11]
+            assert torch.equal(got[3:], table[3:])
+        assert all(torch.equal(a, b) for a, b in zip(was, (kp, vp, bounds, steps)))
+    # a shorter one has its own page there, or one taken ahead
+    lens[1] = 5
+    got, n = skv.paged_reorder(kp, vp, table, lens, parents, bounds=bounds, steps=steps, check=True)
+    assert got[:3].tolist() == [[0, 1, -1], [0, 3, 4], [2, 3, 5]] and n[:3].tolist() == [6, 6, 11]
+    assert torch.equal(kp[3, :, :2], was[0][1, :, :2]) and torch.equal(bounds[3], was[2][1])
+
+
 @pytest.mark.parametrize("precision", ["fp16", "int8", "int4"])
 def test_pool_forks_and_reorders(skv, precision):
     """A pool's sequences against one dense copy each: forks, steps of a search, ends, and new sequences in the pages that became free."""
