@@ -51,7 +51,7 @@ inline BeamShape beam_shape(int B, int beams, int V, int keep, int bytes, bool a
     auto cut = [&](int loads) {
         s.loads = loads;
         s.block = 32ll * loads * (16 / bytes);
-        s.blocks = (V + (aligned ? 0 : 16 / bytes - 1) + s.block - 1) / s.block;   // (a row may begin inside of 16 bytes)
+        s.blocks = (V + (aligned ? 0 : 16 / bytes) + s.block - 1) / s.block;   // (else the first piece is empty: see realign)
     };
     cut(kManyLoads);
     if (rows * s.blocks < sm_count() * 8) cut(kFewLoads);          // too few warps to fill the GPU: more and smaller blocks
@@ -77,7 +77,7 @@ inline BeamShape small_shape(int B, int beams, int V, int keep, int bytes, bool 
     auto cut = [&](int loads) {
         s.loads = loads;
         s.block = 32ll * loads * (16 / bytes);
-        s.blocks = (V + (aligned ? 0 : 16 / bytes - 1) + s.block - 1) / s.block;
+        s.blocks = (V + (aligned ? 0 : 16 / bytes) + s.block - 1) / s.block;
         s.parts = (int)(s.blocks < most ? s.blocks : most);
     };
     cut(kFewLoads);
@@ -218,6 +218,28 @@ __device__ __noinline__ int beam_many(const T* x0, int first, int count, int V, 
     return *s_count;
 }
 
+// Rows that do not all begin on 16 bytes are read in pieces on such boundaries all the same, and then moved: a row's pieces are its logits
+// 0 to 7, 8 to 15 (or 0 to 3, 4 to 7) and so on wherever it begins, so that equal rows add up to equal sums, bit by bit, and
+// their continuations tie.  A piece as it was read, which begins Q words and `bits` bits before the row's own, gives way to what it
+// completes: the row's piece that begins in the one before it, which is the lane's below or, for lane 0, lane 31's of the load
+// before (`carry`: of the block before).  (8 searches of 4 beams of 50257 bf16 logits take 12.8 us, with sums by the places of pieces in memory
+// 11.5; 32 searches of 8 beams of 131071 36.5 and 33.2; rows on 16 bytes do without.)
+template <class T, int LOADS, int Q>
+__device__ __forceinline__ void realign(uint32_t (&w)[4 * LOADS], const uint32_t (&carry)[4], int bits) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int l = LOADS - 1; l >= 0; --l) {
+        uint32_t z[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (k >= Q) z[k] = __shfl_sync(0xffffffffu, lane < 31 ? w[4 * l + k] : l > 0 ? w[4 * (l > 0 ? l - 1 : 0) + k] : carry[k], (lane + 31) & 31);
+            z[4 + k] = w[4 * l + k];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[4 * l + k] = sizeof(T) == 4 ? z[Q + k] : __funnelshift_r(z[Q + k], z[Q + k + 1], bits);
+    }
+}
+
 // A row's part in batches of up to kBeamBatch blocks.  The first look at a batch adds up its exponentials and keeps the largest logit of
 // every lane and block; the keep-th largest of the lanes' largest is a bound that few (lane, block) pieces reach, about `keep` and a
 // half, and only these are read again (they are in L2 still) for their candidates.  (Candidates looked for block by block, as they
@@ -227,7 +249,7 @@ struct ListShared {                                       // of a warp
     float best[kBeamBatch][32];
     int piece[kBeamPieces], held;
 };
-template <class T, int LOADS>
+template <class T, int LOADS, bool ALIGNED>
 __device__ __forceinline__ void beam_list(const skv_beam_args& a, int parts, int64_t blocks, int64_t job, ListShared& s) {
     using W = Word<T>;
     constexpr int PER = 16 / (int)sizeof(T), WORDS = 4 * LOADS, BLOCK = 32 * LOADS * PER;
@@ -237,8 +259,9 @@ __device__ __forceinline__ void beam_list(const skv_beam_args& a, int parts, int
     const int part = (int)(job - row * parts);
     if (beam_dead(a, row) || beam_done(a, row)) return;   // the merge does not look at their lists
     const T* x0 = static_cast<const T*>(a.logits) + row / a.beams * a.stride_b + row % a.beams * a.stride_r;
-    // 16-byte pieces on their boundaries: piece i holds logits i * PER - shift and on, the first and the last piece not all of theirs
-    const int shift = (int)((reinterpret_cast<uintptr_t>(x0) & 15) / sizeof(T));
+    // piece i holds logits i * PER - LEAD and on, as it is read (on 16 bytes) i * PER - shift and on
+    constexpr int LEAD = ALIGNED ? 0 : PER;
+    const int shift = ALIGNED ? 0 : (int)((reinterpret_cast<uintptr_t>(x0) & 15) / sizeof(T));
     float2* list = s.list;
     const int b0 = (int)(blocks * part / parts), b1 = (int)(blocks * (part + 1) / parts);
     float top = -INFINITY;                                // of the lane
@@ -284,6 +307,11 @@ __device__ __forceinline__ void beam_list(const skv_beam_args& a, int parts, int
 #pragma unroll
             for (int k = 0; k < 4; ++k) next[4 * l + k] = word(first0 + 32 * PER * l + k * W::N);
     };
+    uint32_t carry[4];
+    if constexpr (!ALIGNED) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) carry[k] = word((b0 * 32 * LOADS - 1) * PER - shift + k * W::N);
+    }
     load(b0);
     for (int batch = b0; batch < b1; batch += kBeamBatch) {
         const int count = min(kBeamBatch, b1 - batch);
@@ -293,6 +321,18 @@ __device__ __forceinline__ void beam_list(const skv_beam_args& a, int parts, int
 #pragma unroll
             for (int k = 0; k < WORDS; ++k) w[k] = next[k];
             if (block + 1 < b1) load(block + 1);
+            if constexpr (!ALIGNED) {
+                const uint32_t last[4] = {w[WORDS - 4], w[WORDS - 3], w[WORDS - 2], w[WORDS - 1]};
+                const int bytes = shift * (int)sizeof(T), bits = 8 * (bytes & 3);
+                switch (bytes >> 2) {
+                    case 0: realign<T, LOADS, 0>(w, carry, bits); break;
+                    case 1: realign<T, LOADS, 1>(w, carry, bits); break;
+                    case 2: realign<T, LOADS, 2>(w, carry, bits); break;
+                    default: realign<T, LOADS, 3>(w, carry, bits);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) carry[k] = last[k];
+            }
             auto find_best = [&]() {
                 uint32_t best[4];
 #pragma unroll
@@ -383,7 +423,7 @@ __device__ __forceinline__ void beam_list(const skv_beam_args& a, int parts, int
         for (int i = 0; i < count; ++i) {
             const unsigned these = __ballot_sync(0xffffffffu, s.best[i][lane] >= from);
             const int to = pieces + __popc(these & ((1u << lane) - 1));
-            if (these >> lane & 1 && to < kBeamPieces) s.piece[to] = ((batch + i) * 32 * LOADS + lane) * PER - shift;
+            if (these >> lane & 1 && to < kBeamPieces) s.piece[to] = ((batch + i) * 32 * LOADS + lane) * PER - LEAD;
             pieces += __popc(these);
         }
         __syncwarp();
@@ -397,9 +437,17 @@ __device__ __forceinline__ void beam_list(const skv_beam_args& a, int parts, int
             for (int h = 0; h < 2; ++h) {
                 const bool is = i + h * AT_ONCE < pieces;
                 first[h] = (is ? s.piece[i + h * AT_ONCE] : 0) + lane % LOADS * 32 * PER;
-                if (is && first[h] >= 0 && first[h] + PER <= a.V) {
+                if (ALIGNED && is && first[h] >= 0 && first[h] + PER <= a.V) {
                     const uint4 u = __ldg(reinterpret_cast<const uint4*>(x0 + first[h]));
                     y[h][0] = u.x; y[h][1] = u.y; y[h][2] = u.z; y[h][3] = u.w;
+                } else if (!ALIGNED && is && first[h] > 0 && first[h] + PER + 2 <= a.V) {   // (the words may hold a neighbour)
+                    const uintptr_t at = reinterpret_cast<uintptr_t>(x0 + first[h]);
+                    const uint32_t* z = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
+                    uint32_t u[5];
+#pragma unroll
+                    for (int k = 0; k < 3 + W::N; ++k) u[k] = __ldg(z + k);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) y[h][k] = W::N == 1 ? u[k] : __funnelshift_r(u[k], u[k + 1], 8 * (int)(at & 3));
                 } else {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) y[h][k] = is ? word(first[h] + k * W::N) : W::both(-INFINITY);
@@ -417,7 +465,7 @@ __device__ __forceinline__ void beam_list(const skv_beam_args& a, int parts, int
                 }
         }
         __syncwarp();
-        if (many || n > kBeamHeld) n = beam_many(x0, batch * BLOCK - shift, count * BLOCK, a.V, from, most, keep, held, list, &s.held);
+        if (many || n > kBeamHeld) n = beam_many(x0, batch * BLOCK - LEAD, count * BLOCK, a.V, from, most, keep, held, list, &s.held);
         rank(n);
     }
     const float most = warp_max(top);
@@ -428,12 +476,12 @@ __device__ __forceinline__ void beam_list(const skv_beam_args& a, int parts, int
     float2* out = reinterpret_cast<float2*>(static_cast<BeamPart*>(a.scratch) + (int64_t)a.B * a.beams * parts) + job * keep;
     for (int i = lane; i < held; i += 32) out[i] = list[i];
 }
-template <class T, int LOADS>
+template <class T, int LOADS, bool ALIGNED>
 __global__ void __launch_bounds__(32 * kBeamWarps, LOADS == kManyLoads ? 4 : 6) beam_lists_kernel(const __grid_constant__ skv_beam_args a, int parts, int64_t blocks) {
     __shared__ ListShared s[kBeamWarps];
     start_dependents();
     const int warp = threadIdx.x >> 5;
-    beam_list<T, LOADS>(a, parts, blocks, (int64_t)blockIdx.x * kBeamWarps + warp, s[warp]);
+    beam_list<T, LOADS, ALIGNED>(a, parts, blocks, (int64_t)blockIdx.x * kBeamWarps + warp, s[warp]);
 }
 
 // ------------------------------------------------------------------------------------------ the merge
@@ -675,42 +723,40 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
 
 // The same in one launch: a cluster of blocks makes a search's lists, and its first block merges them.
 static_assert(kMergeThreads == 32 * kClusterWarps);
-template <class T, int LOADS>
+template <class T, int LOADS, bool ALIGNED>
 __global__ void __launch_bounds__(kMergeThreads, 2) beam_small_kernel(const __grid_constant__ skv_beam_args a, int parts, int64_t blocks, float by_parts, float by_keep) {
     extern __shared__ __align__(16) unsigned char s_raw[];       // the warps' lists, then the merge's
     int rank;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     const int warp = threadIdx.x >> 5, search = blockIdx.x / kCluster, job = rank + kCluster * warp, lists = a.beams * parts;
     wait_for_dependency();
-    if (job < lists) beam_list<T, LOADS>(a, parts, blocks, (int64_t)search * lists + job, reinterpret_cast<ListShared*>(s_raw)[warp]);
+    if (job < lists) beam_list<T, LOADS, ALIGNED>(a, parts, blocks, (int64_t)search * lists + job, reinterpret_cast<ListShared*>(s_raw)[warp]);
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
     if (rank == 0) beam_merge<T>(a, parts, true, by_parts, by_keep, search, *reinterpret_cast<MergeShared*>(s_raw), s_raw + sizeof(MergeShared));
 }
 
-template <class T>
+template <class T, bool ALIGNED>
 int launch_beam(const skv_beam_args& a, cudaStream_t st) {
-    const bool aligned = (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 && a.stride_b % (16 / (int)sizeof(T)) == 0 &&
-                         a.stride_r % (16 / (int)sizeof(T)) == 0;
-    const BeamShape small = small_shape(a.B, a.beams, a.V, a.keep, sizeof(T), aligned);
+    const BeamShape small = small_shape(a.B, a.beams, a.V, a.keep, sizeof(T), ALIGNED);
     if (small.parts > 0) {
         const size_t entries = (size_t)a.beams * small.parts * a.keep, merge = sizeof(MergeShared) + a.beams * 12 + a.beams * small.parts * 8 + entries * 20;
         const size_t smem = merge > kClusterWarps * sizeof(ListShared) ? merge : kClusterWarps * sizeof(ListShared);   // 45 to 65 KB
-        const auto kernel = small.loads == kManyLoads ? beam_small_kernel<T, kManyLoads> : beam_small_kernel<T, kFewLoads>;
+        const auto kernel = small.loads == kManyLoads ? beam_small_kernel<T, kManyLoads, ALIGNED> : beam_small_kernel<T, kFewLoads, ALIGNED>;
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
         if (e != cudaSuccess) return fail(SKV_ERR_CUDA, "beam_select: %s", cudaGetErrorString(e));
         launch_cluster_after(kernel, dim3((unsigned)a.B * kCluster), dim3(kCluster), kMergeThreads, smem, st, a, small.parts, small.blocks,
                              1.0f / (float)small.parts, 1.0f / (float)a.keep);
         return check_launch("beam_select");
     }
-    const BeamShape s = beam_shape(a.B, a.beams, a.V, a.keep, sizeof(T), aligned);
+    const BeamShape s = beam_shape(a.B, a.beams, a.V, a.keep, sizeof(T), ALIGNED);
     const int64_t jobs = (int64_t)a.B * a.beams * s.parts;
     const unsigned grid = (unsigned)((jobs + kBeamWarps - 1) / kBeamWarps);
-    prefer_shared<beam_lists_kernel<T, kManyLoads>>(50);   // (32 searches of 8 beams 32.5 -> 27.7 us)
-    prefer_shared<beam_lists_kernel<T, kFewLoads>>(50);
+    prefer_shared<beam_lists_kernel<T, kManyLoads, ALIGNED>>(50);   // (32 searches of 8 beams 32.5 -> 27.7 us)
+    prefer_shared<beam_lists_kernel<T, kFewLoads, ALIGNED>>(50);
     prefer_shared<beam_merge_kernel<T>>(50);
-    if (s.loads == kManyLoads) beam_lists_kernel<T, kManyLoads><<<grid, 32 * kBeamWarps, 0, st>>>(a, s.parts, s.blocks);
-    else beam_lists_kernel<T, kFewLoads><<<grid, 32 * kBeamWarps, 0, st>>>(a, s.parts, s.blocks);
+    if (s.loads == kManyLoads) beam_lists_kernel<T, kManyLoads, ALIGNED><<<grid, 32 * kBeamWarps, 0, st>>>(a, s.parts, s.blocks);
+    else beam_lists_kernel<T, kFewLoads, ALIGNED><<<grid, 32 * kBeamWarps, 0, st>>>(a, s.parts, s.blocks);
     if (const int rc = check_launch("beam_select")) return rc;
     const int64_t lists = (int64_t)a.beams * s.parts, entries = lists * a.keep;
     const size_t fixed = (size_t)a.beams * 12 + lists * 8;   // at most 80 KB
@@ -722,6 +768,13 @@ int launch_beam(const skv_beam_args& a, cudaStream_t st) {
     }
     launch_after(beam_merge_kernel<T>, dim3(a.B), kMergeThreads, smem, st, a, s.parts, staged, 1.0f / (float)s.parts, 1.0f / (float)a.keep);
     return check_launch("beam_select");
+}
+
+template <class T>
+int launch_beam(const skv_beam_args& a, cudaStream_t st) {
+    constexpr int PER = 16 / (int)sizeof(T);
+    const bool aligned = (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 && a.stride_b % PER == 0 && a.stride_r % PER == 0;
+    return aligned ? launch_beam<T, true>(a, st) : launch_beam<T, false>(a, st);
 }
 
 // ------------------------------------------------------------------------------------------ reordering

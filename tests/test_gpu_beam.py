@@ -151,6 +151,28 @@ def test_rows_of_any_alignment_and_stride(skv, dtype):
                        skv.beam_select(x, torch.zeros(beams, B, device="cuda"))[2])
 
 
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("B,beams,V,keep", [(1, 4, 50257, 13), (3, 8, 20001, 24), (2, 5, 333, 40), (40, 4, 20001, 9), (64, 8, 5003, 17), (24, 8, 50257, 16),
+                                            (1, 2, 300007, 5), (2, 40, 1003, 128)])
+def test_equal_beams_tie_wherever_their_rows_begin(skv, dtype, B, beams, V, keep):
+    """Copies of one row with equal scores: the order is that of the logits, then of the beams, exactly."""
+    gen = _gen(V)
+    for at, pitch in ((0, V), (1, V), (3, V + 2), (0, V + 7), (5, (V + 15) // 8 * 8)):
+        row = (3 * torch.randn(B, 1, V, generator=gen, device="cuda")).to(dtype)
+        row[:, :, ::7] = -math.inf
+        row[0, 0, 5], row[0, 0, 11] = math.nan, -1e-6
+        x = torch.full((at + B * beams * pitch,), 1000.0, device="cuda", dtype=dtype)[at:].view(B, beams, pitch)[..., :V]
+        x.copy_(row.expand(B, beams, V))
+        scores = -torch.rand(B, 1, generator=gen, device="cuda").expand(B, beams)
+        values, parents, tokens = skv.beam_select(x, scores, keep)
+        every = torch.where(x.isnan(), -math.inf, x.double()).flatten(1)
+        assert torch.equal(parents * V + tokens, torch.sort(every, dim=1, descending=True, stable=True).indices[:, :keep])
+        # beams that tie have one score, whichever group of lanes added it up
+        same = every.gather(1, parents * V + tokens)
+        assert ((values[:, 1:] == values[:, :-1]) | (same[:, 1:] < same[:, :-1])).all()
+        _check(skv, x, -3 * torch.rand(B, beams, generator=gen, device="cuda"), keep)
+
+
 @pytest.mark.parametrize("B", [3, 40])                       # one launch, two
 def test_selection_in_a_graph_on_streams_and_for_host_tensors(skv, B):
     gen = _gen(12)
