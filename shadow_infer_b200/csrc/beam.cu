@@ -487,10 +487,16 @@ __global__ void __launch_bounds__(32 * kBeamWarps, LOADS == kManyLoads ? 4 : 6) 
 // ------------------------------------------------------------------------------------------ the merge
 constexpr int kMergeThreads = 256, kMergeHeld = 512;
 
-// A continuation as it is compared: the order-preserving image of its score in 64 bits (0: none), then its place, beam * 2^32 + token.
+// A continuation as it is compared: the order-preserving image of its score in 64 bits (0: none), then its beam; within a beam its logit, which
+// tells apart what 64 bits do not (and orders the lists, whose ends are cut by it), then its token.
 struct BeamBest {
-    uint64_t score, place;
-    __device__ __forceinline__ bool before(const BeamBest& o) const { return score > o.score || (score == o.score && place < o.place); }
+    uint64_t score, place;   // place: beam * 2^32 + token
+    float logit;
+    __device__ __forceinline__ bool before(const BeamBest& o) const {
+        if (score != o.score) return score > o.score;
+        if ((place ^ o.place) >> 32 || logit == o.logit) return place < o.place;
+        return logit > o.logit;
+    }
 };
 __device__ __forceinline__ uint64_t score_image(double x) {
     if (x == 0.0) x = 0.0;   // (-0 ties with 0)
@@ -572,11 +578,11 @@ __device__ __forceinline__ void beam_merge(const skv_beam_args& a, int parts, bo
     auto entry = [&](int l, int at) {
         const int r = (int)(((float)l + 0.5f) * by_parts), count = s_count[l];
         if (at >= count)
-            return BeamBest{count < 0 && at == 0 ? score_image(s_from[r]) : 0, (uint64_t)r << 32 | (uint32_t)a.pad_token};
+            return BeamBest{count < 0 && at == 0 ? score_image(s_from[r]) : 0, (uint64_t)r << 32 | (uint32_t)a.pad_token, 0.0f};
         const float2 x = staged ? s_entry[l * keep + at] : __ldcg(entries + (int64_t)l * keep + at);
         const float most = s_most[r];
         const double score = x.x == most ? s_from[r] : s_from[r] + ((double)x.x - (double)most);
-        return BeamBest{x.x == most || most < INFINITY ? score_image(score) : 0, (uint64_t)r << 32 | (uint32_t)__float_as_int(x.y)};
+        return BeamBest{x.x == most || most < INFINITY ? score_image(score) : 0, (uint64_t)r << 32 | (uint32_t)__float_as_int(x.y), x.x};
     };
     // ---- candidates: by the images' upper halves.  The keep-th best of 32 lists' fronts is no better than the keep-th best of all; from there
     // on the range is halved until not many more than keep are left.
@@ -624,7 +630,7 @@ __device__ __forceinline__ void beam_merge(const skv_beam_args& a, int parts, bo
                 if (s_upper[i] < lo) continue;
                 const int l = (int)(((float)i + 0.5f) * by_keep), r = (int)(((float)l + 0.5f) * by_parts);
                 const int token = s_count[l] < 0 ? a.pad_token : __float_as_int(s_entry[i].y);
-                s.held[atomicAdd(&s.n, 1)] = BeamBest{s_score[i], (uint64_t)r << 32 | (uint32_t)token};
+                s.held[atomicAdd(&s.n, 1)] = BeamBest{s_score[i], (uint64_t)r << 32 | (uint32_t)token, s_entry[i].x};
             }
             __syncthreads();
         }
@@ -653,7 +659,7 @@ __device__ __forceinline__ void beam_merge(const skv_beam_args& a, int parts, bo
         for (int l = tid; l < lists; l += kMergeThreads) s_at[l] = 0;
 #pragma unroll 1
         for (; found < keep; ++found) {
-            BeamBest best{0, ~0ull};
+            BeamBest best{0, ~0ull, 0.0f};
             int owner = -1;
 #pragma unroll 1
             for (int l = tid; l < lists; l += kMergeThreads) {      // (each thread reads and advances its own lists only)
@@ -662,7 +668,8 @@ __device__ __forceinline__ void beam_merge(const skv_beam_args& a, int parts, bo
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) {
-                const BeamBest y{__shfl_xor_sync(0xffffffffu, best.score, o), __shfl_xor_sync(0xffffffffu, best.place, o)};
+                const BeamBest y{__shfl_xor_sync(0xffffffffu, best.score, o), __shfl_xor_sync(0xffffffffu, best.place, o),
+                                 __shfl_xor_sync(0xffffffffu, best.logit, o)};
                 const int y_owner = __shfl_xor_sync(0xffffffffu, owner, o);
                 if (y.before(best)) { best = y; owner = y_owner; }
             }

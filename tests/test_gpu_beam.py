@@ -173,6 +173,26 @@ def test_equal_beams_tie_wherever_their_rows_begin(skv, dtype, B, beams, V, keep
         _check(skv, x, -3 * torch.rand(B, beams, generator=gen, device="cuda"), keep)
 
 
+@pytest.mark.parametrize("B,V", [(1, 300), (2, 20001), (40, 20001), (40, 20000)])      # searches of one launch, of two
+@pytest.mark.parametrize("near", [40, 700])
+def test_logits_that_64_bits_do_not_tell_apart(skv, B, V, near):
+    """Scores that are equal in 64 bits: a beam's own continuations by their logits, as the lists that are cut have them, behind lower beams'."""
+    near = min(near, V)
+    gen = _gen(V + near)
+    logits = torch.full((B, 2, V), -9.0, device="cuda")
+    for b in range(B):
+        at = torch.randperm(V, generator=gen, device="cuda")[:near]
+        logits[b, :, at] = -1e-20 * torch.rand(2, near, generator=gen, device="cuda")
+    for keep in (1, 2, 13, 60, 128):
+        order = torch.sort(logits, dim=2, descending=True, stable=True).indices[:, :, :near]   # equal beams: all of the first one's
+        want = torch.cat((order[:, 0], order[:, 1] + V), 1)[:, :keep]
+        _, parents, tokens = skv.beam_select(logits, torch.zeros(B, 2, device="cuda"), keep)
+        n = min(keep, 2 * near)
+        assert torch.equal((parents * V + tokens)[:, :n], want[:, :n])
+        _, parents, tokens = skv.beam_select(logits, torch.tensor([-50.0, 0.0], device="cuda").expand(B, 2), min(keep, near))
+        assert (parents == 1).all() and torch.equal(tokens, order[:, 1, :keep])
+
+
 @pytest.mark.parametrize("B", [3, 40])                       # one launch, two
 def test_selection_in_a_graph_on_streams_and_for_host_tensors(skv, B):
     gen = _gen(12)
