@@ -371,10 +371,11 @@ def paged_attention(
 
 
 class _Family:
-    """Sequences that may share pages, and the pages taken for those of them that have ended."""
+    """Sequences that reordered beams' pages are among (which of them holds which, the device alone knows), and the pages named by those
+    of them that have ended."""
 
-    def __init__(self, b: int) -> None:
-        self.rows = {b}
+    def __init__(self) -> None:
+        self.rows = set()
         self.pages: List[int] = []
 
 
@@ -385,8 +386,9 @@ class PagedKVPool:
     ``read`` use what is held; ``release`` ends a sequence and returns its pages.  ``block_table`` and ``lengths``
     are device tensors (for graphs and for the functions above); ``token_counts`` are the lengths on the host.
 
-    ``fork`` lets empty sequences go on from a sequence, and ``reorder`` lets the beams of a search go on from one another; sequences that
-    share pages in these ways return them when the last of them is released.  With ``bounds``, ``append`` keeps the
+    ``fork`` lets empty sequences go on from a sequence, and ``reorder`` lets the beams of a search go on from one another.  A page is free
+    again when the last sequence that it is shared by is released; sequences that were reordered return theirs together, when
+    the last of them (and of those that were forked from them since) is.  With ``bounds``, ``append`` keeps the
     pages' bounds (``page_bounds``) and ``attention`` can be told to read the pages that they rank highest only.
     """
 
@@ -427,13 +429,14 @@ class PagedKVPool:
         if bounds:
             self.bounds = torch.zeros(num_pages, num_heads, 2, head_dim, dtype=torch.int8, device=dev)
             self.steps = torch.ones(num_pages, num_heads, device=dev)
-        # the pages taken for each sequence; which of them it holds is known to the device alone once beams were reordered
+        # each sequence's pages; of reordered sequences those that were taken for it, wherever they are now
         self._table = torch.full((batch_size, -(-max_tokens // page_size)), -1, dtype=torch.int32)
         self.block_table = self._table.to(dev)
         self.lengths = torch.zeros(batch_size, dtype=torch.int32, device=dev)
         self.token_counts: List[int] = [0] * batch_size
         self._free = list(range(num_pages - 1, -1, -1))
-        self._family = [_Family(b) for b in range(batch_size)]
+        self._names = [0] * num_pages       # how many sequences (or families, for those that have ended) name a page
+        self._family: List[Optional[_Family]] = [None] * batch_size
 
     @property
     def free_pages(self) -> int:
@@ -499,6 +502,8 @@ class PagedKVPool:
         rows, columns = zip(*places)
         del self._free[len(self._free) - len(pages):]
         self._table[list(rows), list(columns)] = torch.tensor(pages, dtype=torch.int32)
+        for p in pages:
+            self._names[p] = 1
 
     def _with_pages(self, places: List[Tuple[int, int]], pages: List[int]) -> torch.Tensor:
         """The block table with ``pages`` at ``places`` (sequence, number), without waiting for the GPU."""
@@ -556,9 +561,15 @@ class PagedKVPool:
                                                self.bounds, self.steps, self.head_dim)
         self.block_table.index_copy_(0, at, new_table)
         self.lengths.index_copy_(0, at, new_lengths)
+        if self._family[rows[0]] is None:
+            shared = self._table[rows[0], :j]
+            self._table[rows[1:], :j] = shared
+            for p in shared.tolist():
+                self._names[p] += len(rows) - 1
+        else:
+            self._join(rows)
         if taken:
             self._take(places, taken)
-        self._join(rows)
         for r in rows[1:]:
             self.token_counts[r] = self.token_counts[rows[0]]
 
@@ -582,37 +593,44 @@ class PagedKVPool:
         self.block_table.copy_(table)
         self.lengths.copy_(lengths)
         for g in range(groups):
-            if self.token_counts[g * beams]:
+            if beams > 1 and self.token_counts[g * beams]:
                 self._join(range(g * beams, (g + 1) * beams))
 
     def _join(self, rows: Sequence[int]) -> None:
-        """Sequences ``rows``, and those that they share pages with, return their pages together from now on."""
-        family = self._family[rows[0]]
-        for r in rows[1:]:
+        """Sequences ``rows``, and those that their pages are among already, return their pages together from now on."""
+        family = self._family[rows[0]] or _Family()
+        for r in rows:
             other = self._family[r]
-            if other is not family:
-                family.rows |= other.rows
+            if other is family and r in family.rows:
+                continue
+            mine = {r} if other is None else other.rows
+            if other is not None and other is not family:
                 family.pages.extend(other.pages)
-                for o in other.rows:
-                    self._family[o] = family
+            family.rows |= mine
+            for o in mine:
+                self._family[o] = family
 
     def release(self, b: int) -> int:
-        """End sequence ``b``: its pages are free again, once no sequence is left that it shared pages with.  Returns how many
-        became free."""
+        """End sequence ``b``: its pages are free again, but for those that other sequences share and, if it was reordered, until the
+        others of its family have ended.  Returns how many became free."""
         b = range(self.batch_size)[b]
-        family = self._family[b]
-        family.rows.discard(b)
-        family.pages.extend(p for p in self._table[b].tolist() if p >= 0)
+        pages = [p for p in self._table[b].tolist() if p >= 0]
         self._table[b] = -1
-        self._family[b] = _Family(b)
-        n = 0
-        if not family.rows:
-            n = len(family.pages)
-            self._free.extend(reversed(family.pages))
+        family, self._family[b] = self._family[b], None
+        if family is not None:
+            family.rows.discard(b)
+            family.pages.extend(pages)
+            pages = [] if family.rows else family.pages
+        free = []
+        for p in pages:
+            self._names[p] -= 1
+            if self._names[p] == 0:
+                free.append(p)
+        self._free.extend(reversed(free))
         self.block_table[b].fill_(-1)
         self.lengths[b:b + 1].zero_()   # (an assignment to one element waits for the GPU)
         self.token_counts[b] = 0
-        return n
+        return len(free)
 
     def __repr__(self) -> str:
         return (f"PagedKVPool(precision={self.precision}, heads={self.num_heads}, head_dim={self.head_dim}, "

@@ -483,6 +483,93 @@ def test_pool_forks_and_reorders(skv, precision):
         check()
 
 
+def _same_as_dense(pool, dense):
+    counts = [x.shape[1] for x in dense]
+    assert pool.token_counts == counts == pool.lengths.tolist()
+    k, _ = pool.read()
+    assert all(torch.equal(k[b, :, :n], x) for b, (n, x) in enumerate(zip(counts, dense)))
+
+
+def test_forks_that_end_return_their_pages(skv):
+    """A prefix that stays, forked for one request after another: what a request took is free again when it ends."""
+    H, D, P, B = 2, 16, 4, 4
+    for prefix in (7, 8):                                    # a last page that is partly filled, or none
+        pool = skv.PagedKVPool(12, B, H, D, max_tokens=32, page_size=P, precision="fp32", bounds=True)
+        gen = _gen(prefix)
+        dense = [torch.zeros(H, 0, D, device="cuda") for _ in range(B)]
+
+        def append(new):
+            k = torch.randn(B, H, max(new), D, generator=gen, device="cuda")
+            pool.append(k, -k, new_lengths=new)
+            for b, n in enumerate(new):
+                dense[b] = torch.cat((dense[b], k[b, :, :n]), 1)
+            _same_as_dense(pool, dense)
+
+        append([prefix, 0, 0, 0])
+        free = pool.free_pages
+        for _ in range(8):
+            pool.fork(0, [1, 2])
+            dense[1] = dense[2] = dense[0]
+            append([0, 5, 1, 0])
+            pool.fork(1, [3])                                # a request's own fork, which outlives it
+            dense[3] = dense[1]
+            _same_as_dense(pool, dense)
+            held = {p for b in (0, 2, 3) for p in pool.block_table[b].tolist() if p >= 0}
+            own = [p for p in pool.block_table[1].tolist() if p >= 0 and p not in held]
+            was = pool.free_pages
+            assert pool.release(1) == len(own) == pool.free_pages - was
+            dense[1] = dense[1][:, :0]
+            append([0, 4, 0, 3])                             # in the pages that became free
+            for b in (3, 1, 2):
+                pool.release(b)
+                dense[b] = dense[b][:, :0]
+            assert pool.free_pages == free
+            _same_as_dense(pool, dense)
+        pool.fork(0, [1])
+        assert pool.release(0) == prefix % P // 3 and pool.release(1) == 2 and pool.free_pages == 12
+
+
+@pytest.mark.parametrize("order", [(0, 1, 2, 3, 4, 5), (5, 4, 3, 2, 1, 0), (3, 0, 4, 2, 5, 1)])
+def test_searches_that_share_a_prompt_end_one_by_one(skv, order):
+    """Two searches of one prompt (rows 0 and 1, rows 2 and 3) and a fork of a beam of each (4, 5): no page is free that a sequence reads."""
+    H, D, P, B = 1, 16, 4, 6
+    gen = _gen(8)
+    pool = skv.PagedKVPool(40, B, H, D, max_tokens=48, page_size=P, precision="fp32")
+    dense = [torch.zeros(H, 0, D, device="cuda") for _ in range(B)]
+
+    def append(new):
+        k = torch.randn(B, H, max(new), D, generator=gen, device="cuda")
+        pool.append(k, -k, new_lengths=new)
+        for b, n in enumerate(new):
+            dense[b] = torch.cat((dense[b], k[b, :, :n]), 1)
+        check()
+
+    def check():
+        for p in pool._free:
+            pool.k_pages[p] = math.nan
+        _same_as_dense(pool, dense)
+
+    append([9, 0, 0, 0, 0, 0])
+    pool.fork(0, [1, 2, 3])
+    dense[1] = dense[2] = dense[3] = dense[0]
+    for parents in ([[1, 1], [0, 1], [0, 0]], [[0, 0], [1, 0], [1, 1]], [[1, 0], [1, 1], [0, 1]]):
+        append([3, 3, 3, 3, 0, 0])
+        pool.reorder(torch.tensor(parents, device="cuda"))
+        dense = [dense[2 * g + p] for g, ps in enumerate(parents) for p in ps]
+        check()
+    pool.fork(1, [4])
+    pool.fork(3, [5])
+    dense[4], dense[5] = dense[1], dense[3]
+    append([1, 0, 2, 0, 3, 6])
+    for b in order:
+        pool.release(b)
+        dense[b] = dense[b][:, :0]
+        check()
+    assert sorted(pool._free) == list(range(40))
+    append([5, 1, 0, 9, 4, 4])
+    assert pool.release(4) == 1 and pool.release(3) == 3
+
+
 def test_pool_fork_refusals(skv):
     pool = skv.PagedKVPool(4, 4, 1, 8, max_tokens=16, page_size=4)
     x = torch.randn(4, 1, 6, 8, device="cuda")
