@@ -481,12 +481,12 @@ class PagedKVPool:
         taken = self._free[len(self._free) - sum(wanted):][::-1]
         places = [(b, g - n + i) for b, (g, n) in enumerate(zip(grown, wanted)) for i in range(n)]
         if taken:
-            block_table = self._with_pages(places, taken)
+            host, block_table = self._with_pages(places, taken)
         fresh = None if new_lengths is None else _staged(torch.tensor(new, dtype=torch.int32), self.lengths.device)
         out = paged_append(k, v, self.k_pages, self.v_pages, block_table, self.lengths, self.scale_k, self.scale_v, fresh,
                            q, cos, sin, positions, interleaved, check)
         if taken:
-            self._take(places, taken)
+            self._take(host, taken)
             self.block_table.copy_(block_table)
         start = None if self.bounds is None else self.lengths.clone()
         self.lengths += S if fresh is None else fresh
@@ -497,21 +497,25 @@ class PagedKVPool:
             page_bounds(self.k_pages, self.block_table, self.lengths, self.scale_k, start, self.bounds, self.steps, self.head_dim)
         return out
 
-    def _take(self, places: List[Tuple[int, int]], pages: List[int]) -> None:
-        """``pages``, the last of the free ones, are taken for ``places``."""
+    def _with_pages(self, places: List[Tuple[int, int]], pages: List[int]) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The host's and the device's table with ``pages`` at ``places`` (sequence, number), without waiting for the GPU: one copy of
+        the host's, unless a sequence has been reordered."""
         rows, columns = zip(*places)
-        del self._free[len(self._free) - len(pages):]
-        self._table[list(rows), list(columns)] = torch.tensor(pages, dtype=torch.int32)
-        for p in pages:
-            self._names[p] = 1
-
-    def _with_pages(self, places: List[Tuple[int, int]], pages: List[int]) -> torch.Tensor:
-        """The block table with ``pages`` at ``places`` (sequence, number), without waiting for the GPU."""
-        rows, columns = zip(*places)
+        host = self._table.clone()
+        host.numpy()[rows, columns] = pages
+        if not any(self._family):
+            return host, _staged(host, self.lengths.device)
         at = _staged(torch.tensor([rows, columns, pages], dtype=torch.int64), self.lengths.device)
         table = self.block_table.clone()
         table[at[0], at[1]] = at[2].to(torch.int32)
-        return table
+        return host, table
+
+    def _take(self, host: torch.Tensor, pages: List[int]) -> None:
+        """``pages``, the last of the free ones, are taken as the table ``host`` has them."""
+        self._table = host
+        del self._free[len(self._free) - len(pages):]
+        for p in pages:
+            self._names[p] = 1
 
     def attention(self, q: torch.Tensor, scale: Optional[float] = None, causal: bool = False,
                   new_lengths: Optional[torch.Tensor] = None, keep: Optional[int] = None, first: int = 1,
@@ -552,8 +556,7 @@ class PagedKVPool:
             raise ValueError(f"{len(rows) - 1} sequences go on from one, 1023 at most")
         from .beam import paged_reorder
 
-        places = [(r, j) for r in rows[1:]]
-        table = self._with_pages(places, taken) if taken else self.block_table
+        host, table = self._with_pages([(r, j) for r in rows[1:]], taken) if taken else (self._table, self.block_table)
         at = _staged(torch.tensor(rows, dtype=torch.int64), self.lengths.device)
         parents = torch.zeros(1, len(rows), dtype=torch.int64, device=self.lengths.device)
         lengths = self.lengths[at[:1]].expand(len(rows)).contiguous()
@@ -561,6 +564,8 @@ class PagedKVPool:
                                                self.bounds, self.steps, self.head_dim)
         self.block_table.index_copy_(0, at, new_table)
         self.lengths.index_copy_(0, at, new_lengths)
+        if taken:
+            self._take(host, taken)
         if self._family[rows[0]] is None:
             shared = self._table[rows[0], :j]
             self._table[rows[1:], :j] = shared
@@ -568,8 +573,6 @@ class PagedKVPool:
                 self._names[p] += len(rows) - 1
         else:
             self._join(rows)
-        if taken:
-            self._take(places, taken)
         for r in rows[1:]:
             self.token_counts[r] = self.token_counts[rows[0]]
 

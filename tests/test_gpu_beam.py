@@ -525,6 +525,7 @@ def test_forks_that_end_return_their_pages(skv):
                 dense[b] = dense[b][:, :0]
             assert pool.free_pages == free
             _same_as_dense(pool, dense)
+            assert torch.equal(pool.block_table.cpu(), pool._table)   # (which appends copy as long as nothing was reordered)
         pool.fork(0, [1])
         assert pool.release(0) == prefix % P // 3 and pool.release(1) == 2 and pool.free_pages == 12
 
