@@ -310,9 +310,10 @@ __device__ __forceinline__ int select_pages(const skv_pool_select_args& a, const
     return shape.pages_of(i >= fresh ? 0 : a.causal ? max(0, tokens - fresh + 1 + i) : tokens);
 }
 
-// Order-preserving image of a score; a page whose step is not finite is above all, one without a number below.
+// Order-preserving image of a score; a page whose step is not finite is above all (+inf, where a product is too large, among them), one
+// without a number below.
 __device__ __forceinline__ uint32_t score_key(float dot, float t, float step) {
-    return score_bits(step < INFINITY ? __fmul_rn(__fmul_rn(dot, t), step) : INFINITY);
+    return step < INFINITY ? score_bits(__fmul_rn(__fmul_rn(dot, t), step)) : 0xffffffffu;
 }
 
 // A query row n = rint(q / t) as [min(n, 0) (D), max(n, 0) (D)], put(place, n) for each place, and t; a warp a row, N values a lane

@@ -234,6 +234,18 @@ def test_selection_ties_and_pages_that_nothing_bounds(skv):
         assert torch.equal(got, _select64(q, bounds, steps, table, counts, P, keep, 1, 1, False, [3, 3]))
 
 
+@pytest.mark.parametrize("D,rep", [(16, 1), (128, 4), (64, 12), (33, 2)])
+def test_pages_that_are_not_finite_go_before_scores_that_overflow(skv, D, rep):
+    k = torch.ones(1, 1, 24, D, device="cuda")
+    k[:, :, 4:8], k[:, :, 17, 3] = 2.0 ** 60, math.nan       # pages 1 and 4 of 6
+    table = torch.arange(6, dtype=torch.int32, device="cuda")[None]
+    bounds, steps = skv.page_bounds(k.view(6, 4, 1, D).transpose(1, 2).contiguous(), table, _lens([24]))
+    assert steps[4] == math.inf
+    q = torch.full((1, rep, 1, D), 2.0 ** 90, device="cuda")
+    for keep, want in ((1, [5]), (2, [4, 5]), (3, [1, 4, 5]), (4, [0, 1, 4, 5])):
+        assert skv.page_select(q, bounds, steps, table, _lens([24]), 4, keep, first=0)[0, 0, 0].tolist() == want
+
+
 @pytest.mark.parametrize("n", [-3, 41])
 def test_selection_names_bad_lengths(skv, n):
     bounds, steps = torch.zeros(4, 1, 2, 16, dtype=torch.int8, device="cuda"), torch.ones(4, 1, device="cuda")
