@@ -739,9 +739,10 @@ int launch_select_kernel(const skv_pool_select_args& a, SelectShape shape, size_
     shape.shift = 31;
     while ((1ll << (shape.shift - 31)) < a.page_size) ++shape.shift;
     shape.mul = (uint32_t)(((1ull << shape.shift) + a.page_size - 1) / a.page_size);
-    // as many blocks as fill the GPU, no more than there are shares and a cluster has
+    // as many blocks as fill the GPU, no more than there are shares and a cluster has (heads above 128 values: one block an SM, by its registers; 32
+    // sequences of 256 pages with 8 such heads 32.2 us with shares for two, 20.9 with one, other batches the same)
     const int share = SEGS > 0 ? 16 * kSelectWarps : 8 * kSelectWarps, groups = (a.S_q + shape.block_tokens - 1) / shape.block_tokens;
-    const int64_t all = (int64_t)a.batch * a.heads * groups, fill = (2ll * sm_count() + all - 1) / all;
+    const int64_t all = (int64_t)a.batch * a.heads * groups, fill = ((SEGS == 8 ? 1ll : 2ll) * sm_count() + all - 1) / all;
     if (smem < sizeof(SelectShared)) smem = sizeof(SelectShared);
     int x = (a.table_width + share - 1) / share;
     if (x > fill) x = (int)fill;

@@ -191,6 +191,13 @@ def test_selection_is_the_definitions(skv, counts, H, rep, Sq, D, P, keep, first
         assert torch.equal(got, _select64(q, bounds, steps, table, counts, P, keep, first, recent, False, [Sq] * len(counts)))
 
 
+@pytest.mark.parametrize("B", [1, 5, 20, 40])
+def test_selection_of_heads_above_128_values(skv, B):
+    """However many blocks share a sequence's pages."""
+    counts = [16 * (1 + 37 * b % 190) for b in range(B - 1)] + [16 * 300]
+    test_selection_is_the_definitions(skv, counts, 8, 2, 1, 256, 16, 20, 1, 1, False, torch.bfloat16, "bhsd")
+
+
 @pytest.mark.parametrize("rep", [1, 4, 9])
 @pytest.mark.parametrize("size", [5e33, 1e30, 1e-30, 4e-36])
 def test_selection_of_very_large_and_small_queries(skv, size, rep):
