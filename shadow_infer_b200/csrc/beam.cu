@@ -68,8 +68,9 @@ inline BeamShape beam_shape(int B, int beams, int V, int keep, int bytes, bool a
 // The same for searches that a cluster of blocks takes in one launch; parts 0 where it does not: the clusters would not be resident together, or would
 // leave SMs idle while a warp has more than 8 blocks, or the merge would hold more than its share.  (One launch against two, device time: a
 // search of 4 beams of 32000 fp32 logits 8.1 against 8.9 us, 8 searches 9.4 and 11.4, 32 searches 10.4 and 11.5, 64 searches 20.9 and 15.7;
-// 16 blocks a warp: one search 13.9 and 11.0.  8 beams of 131072 bf16 logits: 16 searches 24.1 and 21.2, 24 25.5 and 25.1, 32 25.8 and
-// 26.9, 37 37.6 and 27.9.  From Python a call costs 3 us less.)
+// 16 blocks a warp: one search 13.9 and 11.0.  8 beams of 131072 bf16 logits: 16 searches 24.3 and 22.0, 20 25.5 and 24.9, 22 26.2 and 25.3, 24 25.9 and 25.5, 26 26.7 and 27.3,
+// 28 25.7 and 26.9, 32 27.0 and 28.2, 37 37.6 and 27.9; of 65536 fp32 logits 16 19.3 and 20.0, 24 21.9 and 22.8, 32 24.4 and 25.2; 4 beams of 131072 fp32
+// logits 16 15.0 and 13.3, 20 15.7 and 15.2, 24 16.3 and 16.8, 32 18.1 and 19.2.  From Python a call costs 3 us less.)
 constexpr int kCluster = 8, kClusterWarps = 8;        // blocks of a search, warps of a block
 inline BeamShape small_shape(int B, int beams, int V, int keep, int bytes, bool aligned) {
     BeamShape s;
@@ -122,7 +123,6 @@ template <class T> struct Word {
     static __device__ __forceinline__ uint32_t bits(__nv_bfloat16 x) { return __bfloat16_as_ushort(x); }
     static __device__ __forceinline__ uint32_t from(T x, T y) { return bits(x) | bits(y) << 16; }
     static __device__ __forceinline__ uint32_t both(float x) { return from(from_float<T>(x), from_float<T>(x)); }
-    static __device__ __forceinline__ bool any_from(uint32_t w, uint32_t low) { return __hge2_mask(pair(w), pair(low)) != 0; }
     static __device__ __forceinline__ float at(uint32_t w, int i) {
         if constexpr (std::is_same_v<T, __half>) return __half2float(__ushort_as_half((unsigned short)(i ? w >> 16 : w & 0xffff)));
         else return __uint_as_float(i ? w & 0xffff0000u : w << 16);
@@ -135,7 +135,6 @@ template <> struct Word<float> {
     static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
     static __device__ __forceinline__ uint32_t larger_nan(uint32_t a, uint32_t b) { return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b))); }
     static __device__ __forceinline__ uint32_t both(float x) { return __float_as_uint(x); }
-    static __device__ __forceinline__ bool any_from(uint32_t w, uint32_t low) { return __uint_as_float(w) >= __uint_as_float(low); }
     static __device__ __forceinline__ float at(uint32_t w, int) { return __uint_as_float(w); }
     static __device__ __forceinline__ float largest(uint32_t w) { return __uint_as_float(w); }
     static constexpr float kLowest = -FLT_MAX;
@@ -729,7 +728,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
 }
 
 // The same in one launch: a cluster of blocks makes a search's lists, and its first block merges them.
-static_assert(kMergeThreads == 32 * kClusterWarps);
+static_assert(kMergeThreads == 32 * kClusterWarps);   // (a warp a part of a beam: at most kCluster * kClusterWarps beams and lists)
 template <class T, int LOADS, bool ALIGNED>
 __global__ void __launch_bounds__(kMergeThreads, 2) beam_small_kernel(const __grid_constant__ skv_beam_args a, int parts, int64_t blocks, float by_parts, float by_keep) {
     extern __shared__ __align__(16) unsigned char s_raw[];       // the warps' lists, then the merge's
@@ -748,9 +747,10 @@ int launch_beam(const skv_beam_args& a, cudaStream_t st) {
     const BeamShape small = small_shape(a.B, a.beams, a.V, a.keep, sizeof(T), ALIGNED);
     if (small.parts > 0) {
         const size_t entries = (size_t)a.beams * small.parts * a.keep, merge = sizeof(MergeShared) + a.beams * 12 + a.beams * small.parts * 8 + entries * 20;
-        const size_t smem = merge > kClusterWarps * sizeof(ListShared) ? merge : kClusterWarps * sizeof(ListShared);   // 45 to 65 KB
+        constexpr size_t some = kClusterWarps * sizeof(ListShared), most = sizeof(MergeShared) + kCluster * kClusterWarps * 20 + kMergeFew * 20;   // 45, 55 KB
+        const size_t smem = merge > some ? merge : some;
         const auto kernel = small.loads == kManyLoads ? beam_small_kernel<T, kManyLoads, ALIGNED> : beam_small_kernel<T, kFewLoads, ALIGNED>;
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(most > some ? most : some));
         if (e != cudaSuccess) return fail(SKV_ERR_CUDA, "beam_select: %s", cudaGetErrorString(e));
         launch_cluster_after(kernel, dim3((unsigned)a.B * kCluster), dim3(kCluster), kMergeThreads, smem, st, a, small.parts, small.blocks,
                              1.0f / (float)small.parts, 1.0f / (float)a.keep);

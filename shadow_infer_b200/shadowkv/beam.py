@@ -34,7 +34,7 @@ def beam_select(
 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The ``keep`` best continuations of each search: ``(scores, parents, tokens)``, each ``[B, keep]``, best first.
 
-    ``logits`` ``[B, beams, V]`` (fp32, fp16 or bf16, any strides over the first two dimensions) are those of each beam's next
+    ``logits`` ``[B, beams, V]`` (fp32, fp16 or bf16, other types as fp32; any strides over the first two dimensions) are those of each beam's next
     token, ``scores`` ``[B, beams]`` the beams' log-probabilities so far.  A continuation scores
     ``scores[b, r] + log_softmax(logits[b, r])[token]``; scores are compared in 64 bits, a beam's own continuations by their logits, and
     ties go to the lowest beam, then to the lowest token.  A row's exponentials are 32-bit numbers, so the logarithm of their sum is up to 2^-20 off,

@@ -104,7 +104,8 @@ def page_select(
     with the query in 8 bits: ``n = rint(q / t)``, ``t`` the least power of two of which 127 reach the row's largest
     magnitude.  The products and sums are whole numbers and exact, so equal inputs give equal pages on any device.  A page whose step is
     not finite goes before all others, one that the table does not name behind them; a query row that is not finite scores 0.
-    Rows that require a gradient are read as constants.  One launch.
+    Rows that require a gradient are read as constants.  The scores are kept meanwhile, 4 bytes for each of the table's pages, key heads and new
+    tokens (4 GB for 8192 tokens, 32 heads and 4096 pages): a long prompt chooses in parts.  One launch.
     """
     shape = q.shape
     if len(shape) != 4:
@@ -138,7 +139,7 @@ def page_select(
     lib = _lib.load()
     with device_ctx(dev):
         stream = _lib.stream_of(dev)
-        scratch = _workspace("select", dev, stream, B * H * S_q * (width + 3) * 4 + 16)   # (no less than the library asks for)
+        scratch = _workspace("select", dev, stream, max(16, lib.skv_pool_select_scratch_bytes(B, H, S_q, width)))
         st = lib.skv_pool_select(_SELECT.pack(
             *q_rows, bounds.data_ptr(), steps.data_ptr(), table.data_ptr(), lens.data_ptr(), 0 if new is None else new.data_ptr(),
             pages.data_ptr(), scratch.data_ptr(), 0 if flag is None else flag.data_ptr(), table.stride(0), scratch.numel(), width, N,
