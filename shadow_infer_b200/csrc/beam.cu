@@ -10,7 +10,8 @@
 // Few searches, or small ones, are one launch of clusters, whose first block merges what the others found.
 //
 // What bounds it.  256 rows of 131072 16-bit logits (205 of them not finished, 54 MB): 26.4 us, of which the lists take about 20 (2.7 TB/s:
-// a warp has one block of 4 KB ahead of the one at work, and 16 warps fit an SM's registers; 24 without the block ahead were no faster, nor
+// a warp has one block of 4 KB ahead of the one at work, and 16 warps fit an SM's registers, of which about 11 are at work: a warp's part is of one
+// beam, finished or not, and 256 blocks are two on some SMs; 24 without the block ahead were no faster, nor
 // were more parts than warps) and the merge 6, one step's latency after the other (in two launches 27.4).  4 rows of 32000 fp32 logits: 8.5 us,
 // the same steps; from Python such a call costs 14.
 //

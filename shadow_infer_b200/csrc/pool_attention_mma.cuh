@@ -19,7 +19,7 @@
 // fp32: 16 KB a tile leave room for 4 warps an SM, 16384 tokens in 36 us (57 %).  Small calls: 4 to 5 us until the first rows
 // are there, 1.7 us a unit and 3 to 6 us for a join; 512 tokens of 32 heads in 12 us, 8 int8 sequences of up to 2048 tokens in 18.
 // Lists of pages: a unit's table is made first, 2 to 4 us; 32 units of 2048 int4 tokens in 19 us, 8 of 4096 int8 tokens in 16, of 512 in 11, 512 of 512 int8
-// tokens in 26 (from L2: the rounds' instructions), 512 of up to 1024 fp16 tokens in 52 with its tables' launch (256 MB, 5 TB/s).
+// tokens in 26 (from L2; instructions fill 47 % of the issue slots, their waits and the units' barriers the rest), 512 of up to 1024 fp16 tokens in 52 with its tables' launch (256 MB, 5 TB/s).
 //
 // Exactness.  Page values enter the MMAs exactly: fp16 as it is, int8 and int4 as small integers, fp32 as two terms of 11 bits
 // (of the products of small parts only that of both is left out, 2^-24 of a value).  For the scores they stay
