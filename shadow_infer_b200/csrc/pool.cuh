@@ -92,12 +92,21 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8]) {
     *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// A number that the kernel only reads.  FRESH: one that it may have written itself, or has waited for after it had started
+// (wait_for_dependency): a read-only load could be moved before that.
+template <bool FRESH, class T>
+__device__ __forceinline__ T number_at(const T* p) {
+    if constexpr (FRESH) return *p;
+    else return __ldg(p);
+}
+
 // The pool row (all heads of a page counted, head 0's block) that holds token t of sequence b, or
 // -1 where the table names no page for it.  + head * page_size gives the head's row.
+template <bool FRESH = false>
 __device__ __forceinline__ int64_t pool_row(const skv_pool& p, int b, int64_t t) {
     if (t < 0 || t >= (int64_t)p.table_width * p.page_size) return -1;
     const int64_t j = t <= 0xffffffffll ? (int64_t)((uint32_t)t / (uint32_t)p.page_size) : t / p.page_size;
-    const int page = p.block_table[b * p.table_stride + j];   // (may have been written by this kernel: no read-only load)
+    const int page = number_at<FRESH>(p.block_table + b * p.table_stride + j);
     if (page < 0 || page >= p.num_pages) return -1;
     return (int64_t)page * p.heads * p.page_size + (t - j * p.page_size);
 }
@@ -107,18 +116,18 @@ __host__ __device__ inline int64_t pool_row_bytes(int precision, int D) {
 }
 
 // Value col of pool rows, any D and group; block: col / int4_group.
-template <int PREC>
+template <int PREC, bool FRESH = false>
 __device__ __forceinline__ float pool_value(const skv_pool& p, bool is_v, int64_t row, int col, int block) {
     const uint8_t* base = static_cast<const uint8_t*>(is_v ? p.v : p.k);
     const float* sc = is_v ? p.scale_v : p.scale_k;
     const int D = p.head_dim;
-    if constexpr (PREC == 0) return __ldg(reinterpret_cast<const float*>(base) + row * D + col);
-    else if constexpr (PREC == 1) return __half2float(__ldg(reinterpret_cast<const __half*>(base) + row * D + col));
-    else if constexpr (PREC == 2) return __fmul_rn((float)__ldg(reinterpret_cast<const signed char*>(base) + row * D + col), __ldg(sc + row));
+    if constexpr (PREC == 0) return number_at<FRESH>(reinterpret_cast<const float*>(base) + row * D + col);
+    else if constexpr (PREC == 1) return __half2float(number_at<FRESH>(reinterpret_cast<const __half*>(base) + row * D + col));
+    else if constexpr (PREC == 2) return __fmul_rn((float)number_at<FRESH>(reinterpret_cast<const signed char*>(base) + row * D + col), number_at<FRESH>(sc + row));
     else {
-        const uint8_t byte = __ldg(base + row * ((D + 1) / 2) + col / 2);
+        const uint8_t byte = number_at<FRESH>(base + row * ((D + 1) / 2) + col / 2);
         const int q = (col & 1) ? (byte & 15) : (byte >> 4);
-        return __fmul_rn((float)(q - 8), __ldg(sc + row * (D / p.int4_group) + block));
+        return __fmul_rn((float)(q - 8), number_at<FRESH>(sc + row * (D / p.int4_group) + block));
     }
 }
 

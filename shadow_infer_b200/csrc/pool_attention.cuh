@@ -40,8 +40,9 @@ __host__ __device__ inline int64_t token_cap(const skv_pool_attention_args& a) {
     const int64_t cap = (int64_t)a.pool.table_width * a.pool.page_size;
     return cap < 0x7fffff00 ? cap : 0x7fffff00;
 }
+template <bool FRESH = false>
 __device__ __forceinline__ int seq_tokens(const skv_pool_attention_args& a, int b) {
-    const int64_t n = a.lengths[b], cap = token_cap(a);   // (may have been written by this kernel)
+    const int64_t n = number_at<FRESH>(a.lengths + b), cap = token_cap(a);
     return (int)(n < 0 ? 0 : n > cap ? cap : n);
 }
 // Tiles of a sequence for one row tile of one head; an empty sequence keeps one, to write its zeros.
@@ -97,12 +98,12 @@ __device__ __forceinline__ void take_share(const skv_pool_attention_args& a, Cos
 }
 
 // The same for units that all see their whole sequence.
-template <int THREADS>
+template <int THREADS, bool FRESH = false>
 __device__ __forceinline__ void take_share(const skv_pool_attention_args& a, int tile, int units, int pad, int min_tiles,
                                            Share* s) {
     // a single short sequence: a CTA a unit and nothing to join (128 tokens of 32 fp16 heads 11.3 -> 7.8 us)
-    const bool whole = a.pool.batch == 1 && seq_tiles(seq_tokens(a, 0), tile) <= min_tiles;
-    take_share<THREADS>(a, [&](int b) { return (seq_tiles(seq_tokens(a, b), tile) + pad) * units; }, pad, min_tiles, s, whole ? units : 0);
+    const bool whole = a.pool.batch == 1 && seq_tiles(seq_tokens<FRESH>(a, 0), tile) <= min_tiles;
+    take_share<THREADS>(a, [&](int b) { return (seq_tiles(seq_tokens<FRESH>(a, b), tile) + pad) * units; }, pad, min_tiles, s, whole ? units : 0);
 }
 
 // ------------------------------------------------------------------------------- listed pages only
@@ -116,14 +117,15 @@ struct AttentionCall : skv_pool_attention_args {
 };
 __host__ __device__ inline int64_t list_stride(int keep) { return ((int64_t)keep + 31) & ~31ll; }   // tables on 128-byte lines
 
-// A warp makes unit u's table and length.
+// A warp makes unit u's table and length.  (Its kernel may have started before the choice of pages had ended: nothing here, nor behind it, is
+// read by a read-only load.)
 __device__ __forceinline__ void list_table(const skv_pool_sparse_args& s, int u, int units) {
     const skv_pool_attention_args& a = s.attention;
     const int lane = threadIdx.x & 31, P = a.pool.page_size;
     const int h = u % a.pool.heads, bi = u / a.pool.heads, i = bi % a.S_q, b = bi / a.S_q;
     const int32_t* list = s.pages + b * s.pages_stride_b + h * s.pages_stride_h + i * s.pages_stride_s;
     int e = lane < s.keep ? list[lane] : -1;
-    const int tokens = seq_tokens(a, b), n_new = a.new_lengths ? __ldg(a.new_lengths + b) : a.S_q;
+    const int tokens = seq_tokens<true>(a, b), n_new = a.new_lengths ? a.new_lengths[b] : a.S_q;
     const int seen = i >= n_new ? 0 : a.causal ? max(0, tokens - n_new + 1 + i) : tokens, pages = seen > 0 ? (seen - 1) / P + 1 : 0;
     int32_t* table = static_cast<int32_t*>(s.tables) + u * list_stride(s.keep);
     int top = -1, count = 0, last = -1;   // the largest entry so far, those that count and the last of them
@@ -144,7 +146,7 @@ __device__ __forceinline__ void list_table(const skv_pool_sparse_args& s, int u,
         bad |= e < -1 || e >= a.pool.table_width || (e >= 0 && e <= before);
         const unsigned these = __ballot_sync(0xffffffffu, counts);
         if (counts) {
-            const int page = __ldg(a.pool.block_table + b * a.pool.table_stride + e);
+            const int page = a.pool.block_table[b * a.pool.table_stride + e];
             table[count + __popc(these & ((1u << lane) - 1))] = page >= 0 && page < a.pool.num_pages ? page * a.pool.heads + h : -1;
         }
         if (these) last = __shfl_sync(0xffffffffu, e, 31 - __clz(these));
@@ -186,9 +188,9 @@ __device__ __forceinline__ void take_listed(const skv_pool_attention_args& a, co
         if (run) {
             t.each = 0x7fffffff;
             t.lo = t.hi = t.base = 0;
-            for (int b = b0; b < b1; ++b) t.hi += seq_tiles(seq_tokens(a, b), tile) * row_tiles;
+            for (int b = b0; b < b1; ++b) t.hi += seq_tiles(seq_tokens<true>(a, b), tile) * row_tiles;
         } else {
-            const int rt = unit - b0 * row_tiles, tiles = seq_tiles(seq_tokens(a, b0), tile);
+            const int rt = unit - b0 * row_tiles, tiles = seq_tiles(seq_tokens<true>(a, b0), tile);
             t.each = (tiles + splits - 1) / splits;
             const int first = unit * splits * t.each;
             t.lo = (int)blockIdx.x * t.each;
@@ -217,12 +219,13 @@ struct Segment {
 };
 
 // The segment that starts at tile `at` of the share.
+template <bool FRESH = false>
 __device__ __forceinline__ Segment segment_at(const skv_pool_attention_args& a, const Share& s, int at, int tile,
                                               int row_tiles, int& b, int& base) {
     Segment g;
     const int units = a.pool.heads * row_tiles;
     for (;;) {
-        g.tokens = seq_tokens(a, b);
+        g.tokens = seq_tokens<FRESH>(a, b);
         const int nt = seq_tiles(g.tokens, tile), all = nt + s.pad;
         if (at < base + all * units) {
             const int u = (at - base) / all;
@@ -478,7 +481,7 @@ __device__ __forceinline__ uint4 finite_halves(uint4 w) {
 // Adds what is not finite among the values of tokens [from, to) to rows r0 .. r0 + rows - 1 of a unit, in its part or, where that is
 // null, in the output.  Rare, so it reads the pages again; thread tid of `threads`, which has every threads-th value of a row,
 // between barriers of them.
-template <int PREC>
+template <int PREC, bool FRESH = false>
 __device__ __noinline__ void add_not_finite(const skv_pool_attention_args& a, int b, int hk, int tokens, int r0, int rows, int from, int to,
                                             float* part, int tid, int threads) {
     const int D = a.pool.head_dim, rep = a.q.heads / a.pool.heads;
@@ -486,8 +489,8 @@ __device__ __noinline__ void add_not_finite(const skv_pool_attention_args& a, in
         const int block = PREC == 3 ? d / a.pool.int4_group : 0;
 #pragma unroll 4
         for (int t = from; t < to; ++t) {
-            const int64_t row = pool_row(a.pool, b, t);
-            const float v = row < 0 ? 0.0f : pool_value<PREC>(a.pool, true, row + (int64_t)hk * a.pool.page_size, d, block);
+            const int64_t row = pool_row<FRESH>(a.pool, b, t);
+            const float v = row < 0 ? 0.0f : pool_value<PREC, FRESH>(a.pool, true, row + (int64_t)hk * a.pool.page_size, d, block);
             if (finite(v)) continue;
             for (int j = 0; j < rows; ++j) {
                 const int r = r0 + j;

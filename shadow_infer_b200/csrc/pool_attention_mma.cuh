@@ -138,10 +138,11 @@ struct PageDivide {
 
 // The page rows of a sequence's tokens for one key head.  A warp keeps the next 64 entries of the
 // block table in its lanes and asks them by shuffle: tiles need no dependent load.
+template <bool FRESH>
 struct PageRows {
     const int32_t* table;
     int width, base, cur, next, lane;
-    __device__ __forceinline__ int entry(int i) const { return i < width ? table[i] : -1; }   // (may have been written by this kernel)
+    __device__ __forceinline__ int entry(int i) const { return i < width ? number_at<FRESH>(table + i) : -1; }
     __device__ __forceinline__ void start(const skv_pool& p, int b, int first) {
         table = p.block_table + b * p.table_stride;
         width = p.table_width;
@@ -281,7 +282,9 @@ __host__ __device__ constexpr size_t mma_smem() {
 // exact: the head has DP values (and, for int4, groups of 16): rows and scales are copied whole, in steps known here.
 // LIMIT: rows may see different tokens (several new ones under a causal limit).  Without it the look at fp16 and fp32 values is
 // left out, which costs a call of one token 3 %.
-template <int PREC, int DP, int NT, int NQ, int NP, bool LIMIT>
+// LISTED: lists of pages, whose tables and lengths the CTAs make (a.reserved > 0) or a launch before this one.  A kernel of its own, as their
+// plain loads and the second way to a share cost calls of whole sequences 2 to 5 % (one of 32768 int4 tokens 82.6 -> 84.6 us, 128 fp16 tokens 12.7 -> 13.1).
+template <int PREC, int DP, int NT, int NQ, int NP, bool LIMIT, bool LISTED>
 __global__ void __launch_bounds__(32 * MmaShape<PREC, DP, NT>::W, MmaShape<PREC, DP, NT>::CTAS)
 pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, const __grid_constant__ skv_pool_sparse_args lists,
                           int row_tiles, PageDivide magic, bool exact, bool q_vec, bool out_vec) {
@@ -306,9 +309,9 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, con
     const int rep = a.q.heads / a.pool.heads, R = rep * a.S_q;
     const bool p16 = P % 16 == 0;   // a tile lies in one page
     auto page_of = [&](int t) { return (int)(((uint64_t)(uint32_t)t * magic.mul) >> magic.shift); };
-    wait_for_dependency();
-    if (a.reserved > 0) take_listed<THREADS>(a, lists, TILE, row_tiles, &s);
-    else take_share<THREADS>(a, TILE, a.pool.heads * row_tiles, kMmaPad, kMinTiles, &s);
+    if constexpr (LISTED) wait_for_dependency();
+    if (LISTED && a.reserved > 0) take_listed<THREADS>(a, lists, TILE, row_tiles, &s);
+    else take_share<THREADS, LISTED>(a, TILE, a.pool.heads * row_tiles, kMmaPad, kMinTiles, &s);
     if (s.lo >= s.hi) return;
     char* ring = s_ring + warp * S * L::BYTES;
     if (!exact) {   // chunks that the head does not have are never copied: they count as zero
@@ -325,7 +328,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, con
     f.b = s.b;
     f.base = s.base;
     f.st = f.end = f.hk = f.tokens = 0;
-    PageRows pages;
+    PageRows<LISTED> pages;
     const int row_bytes = PREC == 0 ? 4 * D : PREC == 1 ? 2 * D : PREC == 2 ? D : D / 2;
     constexpr int WIDE = L::CHUNKS > 32 ? L::CHUNKS / 32 : 1;   // copies a row takes
     constexpr int STEP = 32 * WIDE / L::CHUNKS, COPIES = 16 / STEP;   // rows a warp's copy takes, copies a tile takes
@@ -339,7 +342,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, con
                 copy_commit();   // an empty group keeps the count
                 return;
             }
-            const Segment g = segment_at(a, s, f.at, TILE, row_tiles, f.b, f.base);
+            const Segment g = segment_at<LISTED>(a, s, f.at, TILE, row_tiles, f.b, f.base);
             f.at = g.next;
             f.hk = g.hk;
             f.tokens = g.tokens;
@@ -359,7 +362,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, con
                 atomicExch(a.error_flag, 1);
             }
         } else if (t < f.tokens) {
-            const int j = page_of(t), page = pages.table[j];   // t is below the table's width
+            const int j = page_of(t), page = number_at<LISTED>(pages.table + j);   // t is below the table's width
             if (page >= 0 && page < a.pool.num_pages) row = (page * a.pool.heads + f.hk) * P + (t - j * P);
             else if (a.error_flag) atomicExch(a.error_flag, 1);
         }
@@ -438,7 +441,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, con
 
     int at = s.lo, b = s.b, base = s.base;
     while (at < s.hi) {
-        const Segment g = segment_at(a, s, at, TILE, row_tiles, b, base);
+        const Segment g = segment_at<LISTED>(a, s, at, TILE, row_tiles, b, base);
         at = g.next;
         if (g.t0 >= g.t1) continue;
         const int n = g.tokens, r0 = g.rt * ROWS;
@@ -1045,7 +1048,7 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, con
         if ((PREC == 3 || (PREC <= 1 && LIMIT)) && s_odd) {   // (set before the barriers above)
             const int first = g.t0 * TILE;
             __syncthreads();
-            add_not_finite<PREC>(a, g.b, g.hk, n, r0, min(ROWS, R - r0), PREC == 3 ? first : max(first, not_all), min(n, g.t1 * TILE),
+            add_not_finite<PREC, LISTED>(a, g.b, g.hk, n, r0, min(ROWS, R - r0), PREC == 3 ? first : max(first, not_all), min(n, g.t1 * TILE),
                                  g.whole ? nullptr : part, tid, THREADS);
         }
         if (!g.whole) {
@@ -1058,6 +1061,19 @@ pool_attention_mma_kernel(const __grid_constant__ skv_pool_attention_args a, con
     }
 }
 
+// Raises the kernel's limit on shared memory, once a device.
+template <auto KERNEL>
+int allow_shared(size_t bytes) {
+    static std::atomic<uint64_t> allowed{0};   // devices where that was done
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev >= 64 || !(allowed.load(std::memory_order_relaxed) >> dev & 1))) {
+        e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e == cudaSuccess && dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
+    return e == cudaSuccess ? SKV_OK : fail(SKV_ERR_CUDA, "pool_attention: %s", cudaGetErrorString(e));
+}
+
 template <int PREC, int DP, int NT, int NQ, int NP, bool LIMIT>
 int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
     using Shape = MmaShape<PREC, DP, NT>;
@@ -1067,15 +1083,6 @@ int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
     const int R = a.q.heads / a.pool.heads * a.S_q, row_tiles = (R + 8 * NT - 1) / (8 * NT);
     const int64_t step = sequences_a_launch(a, row_tiles, 16 * Shape::W, kMmaPad);
     if (step == 0) return SKV_ERR_TOO_LARGE;
-    const auto kernel = pool_attention_mma_kernel<PREC, DP, NT, NQ, NP, LIMIT>;
-    static std::atomic<uint64_t> allowed{0};   // devices whose limit on the kernel's shared memory was raised
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess && (dev >= 64 || !(allowed.load(std::memory_order_relaxed) >> dev & 1))) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e == cudaSuccess && dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
-    }
-    if (e != cudaSuccess) return fail(SKV_ERR_CUDA, "pool_attention: %s", cudaGetErrorString(e));
     PageDivide magic;
     magic.shift = 31;
     while ((1ll << (magic.shift - 31)) < a.pool.page_size) ++magic.shift;
@@ -1084,7 +1091,11 @@ int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
                        (PREC != 3 || (a.pool.int4_group == 16 && ((reinterpret_cast<uintptr_t>(a.pool.scale_k) |
                                                                    reinterpret_cast<uintptr_t>(a.pool.scale_v)) & 15) == 0));
     const bool q_vec = rows_aligned(a.q), out_vec = rows_aligned(a.out);
-    if (a.reserved < 0) {
+    const unsigned all = sm_count() * Shape::CTAS, threads = 32 * Shape::W;
+    const skv_pool_sparse_args none = {};
+    if constexpr (!LIMIT) if (a.reserved < 0) {   // (a unit is one token)
+        constexpr auto kernel = pool_attention_mma_kernel<PREC, DP, NT, NQ, NP, false, true>;
+        if (const int rc = allow_shared<kernel>(smem)) return rc;
         const skv_pool_sparse_args& lists = *static_cast<const AttentionCall&>(a).lists;
         // Sequences of one head and of known length at most (lists of pages).  Where there are fewer units than CTAs, a unit's tiles are split
         // over those that would be idle; else units stay whole, unless too many CTAs would idle in the last round, where even shares of
@@ -1105,17 +1116,20 @@ int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
             skv_pool_attention_args part = a;
             part.reserved = (int32_t)splits;
             const int64_t ctas = rounds > 1 && a.pool.batch > resident ? resident : units * splits;   // (runs of whole sequences)
-            launch_after(kernel, dim3((unsigned)ctas), 32 * Shape::W, smem, st, part, lists, row_tiles, magic, exact, q_vec, out_vec);
+            launch_after(kernel, dim3((unsigned)ctas), threads, smem, st, part, lists, row_tiles, magic, exact, q_vec, out_vec);
             return check_launch("pool_attention");
         }
         if (const int rc = launch_tables(lists, st)) return rc;
+        return by_sequences(a, step, [&](skv_pool_attention_args part) {
+            part.reserved = 0;
+            launch_after(kernel, dim3(all), threads, smem, st, part, none, row_tiles, magic, exact, q_vec, out_vec);
+            return check_launch("pool_attention");
+        });
     }
-    const skv_pool_sparse_args none = {};
-    const bool listed = a.reserved < 0;   // (behind the launch that makes the tables)
-    return by_sequences(a, step, [&](skv_pool_attention_args part) {
-        part.reserved = 0;
-        if (listed) launch_after(kernel, dim3(sm_count() * Shape::CTAS), 32 * Shape::W, smem, st, part, none, row_tiles, magic, exact, q_vec, out_vec);
-        else kernel<<<sm_count() * Shape::CTAS, 32 * Shape::W, smem, st>>>(part, none, row_tiles, magic, exact, q_vec, out_vec);
+    constexpr auto kernel = pool_attention_mma_kernel<PREC, DP, NT, NQ, NP, LIMIT, false>;
+    if (const int rc = allow_shared<kernel>(smem)) return rc;
+    return by_sequences(a, step, [&](const skv_pool_attention_args& part) {
+        kernel<<<all, threads, smem, st>>>(part, none, row_tiles, magic, exact, q_vec, out_vec);
         return check_launch("pool_attention");
     });
 }
