@@ -90,9 +90,10 @@ inline BeamShape small_shape(int B, int beams, int V, int keep, int bytes, bool 
     return s;
 }
 
-// Whether beam r of search b has continuations of its own, and whether it has but one.
-__device__ __forceinline__ bool beam_dead(const skv_beam_args& a, int64_t row) { return !(fabsf(__ldg(a.scores + row)) < INFINITY); }
-__device__ __forceinline__ bool beam_done(const skv_beam_args& a, int64_t row) { return a.finished && __ldg(a.finished + row); }
+// Whether beam r of search b has continuations of its own, and whether it has but one.  (The kernels of the selection wait for those before them by
+// themselves: no read-only loads in them, which could be moved before that.)
+__device__ __forceinline__ bool beam_dead(const skv_beam_args& a, int64_t row) { return !(fabsf(a.scores[row]) < INFINITY); }
+__device__ __forceinline__ bool beam_done(const skv_beam_args& a, int64_t row) { return a.finished && a.finished[row]; }
 
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
@@ -297,7 +298,7 @@ __device__ __forceinline__ void beam_list(const skv_beam_args& a, int parts, int
             const uint4* y = reinterpret_cast<const uint4*>(x0 + first0);
 #pragma unroll
             for (int l = 0; l < LOADS; ++l) {
-                const uint4 u = __ldg(y + 32 * l);
+                const uint4 u = y[32 * l];
                 next[4 * l] = u.x; next[4 * l + 1] = u.y; next[4 * l + 2] = u.z; next[4 * l + 3] = u.w;
             }
             return;
@@ -438,14 +439,14 @@ __device__ __forceinline__ void beam_list(const skv_beam_args& a, int parts, int
                 const bool is = i + h * AT_ONCE < pieces;
                 first[h] = (is ? s.piece[i + h * AT_ONCE] : 0) + lane % LOADS * 32 * PER;
                 if (ALIGNED && is && first[h] >= 0 && first[h] + PER <= a.V) {
-                    const uint4 u = __ldg(reinterpret_cast<const uint4*>(x0 + first[h]));
+                    const uint4 u = *reinterpret_cast<const uint4*>(x0 + first[h]);
                     y[h][0] = u.x; y[h][1] = u.y; y[h][2] = u.z; y[h][3] = u.w;
                 } else if (!ALIGNED && is && first[h] > 0 && first[h] + PER + 2 <= a.V) {   // (the words may hold a neighbour)
                     const uintptr_t at = reinterpret_cast<uintptr_t>(x0 + first[h]);
                     const uint32_t* z = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
                     uint32_t u[5];
 #pragma unroll
-                    for (int k = 0; k < 3 + W::N; ++k) u[k] = __ldg(z + k);
+                    for (int k = 0; k < 3 + W::N; ++k) u[k] = z[k];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) y[h][k] = W::N == 1 ? u[k] : __funnelshift_r(u[k], u[k + 1], 8 * (int)(at & 3));
                 } else {
@@ -546,10 +547,10 @@ __device__ __forceinline__ void beam_merge(const skv_beam_args& a, int parts, bo
     if (tid == 0) s.n = 0;
     if (staged)
 #pragma unroll 4
-        for (int i = tid; i < all; i += kMergeThreads) s_entry[i] = __ldcg(entries + i);
+        for (int i = tid; i < all; i += kMergeThreads) s_entry[i] = entries[i];
 #pragma unroll 1
     for (int r = warp; r < beams; r += kMergeThreads / 32) {        // a warp a beam
-        const float cum = __ldg(a.scores + row0 + r);
+        const float cum = a.scores[row0 + r];
         const bool done = beam_done(a, row0 + r), dead = !(fabsf(cum) < INFINITY);
         float most = -INFINITY;
         double sum = 0.0;
@@ -579,7 +580,7 @@ __device__ __forceinline__ void beam_merge(const skv_beam_args& a, int parts, bo
         const int r = (int)(((float)l + 0.5f) * by_parts), count = s_count[l];
         if (at >= count)
             return BeamBest{count < 0 && at == 0 ? score_image(s_from[r]) : 0, (uint64_t)r << 32 | (uint32_t)a.pad_token, 0.0f};
-        const float2 x = staged ? s_entry[l * keep + at] : __ldcg(entries + (int64_t)l * keep + at);
+        const float2 x = staged ? s_entry[l * keep + at] : entries[(int64_t)l * keep + at];
         const float most = s_most[r];
         const double score = x.x == most ? s_from[r] : s_from[r] + ((double)x.x - (double)most);
         return BeamBest{x.x == most || most < INFINITY ? score_image(score) : 0, (uint64_t)r << 32 | (uint32_t)__float_as_int(x.y), x.x};

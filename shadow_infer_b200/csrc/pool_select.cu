@@ -300,13 +300,13 @@ struct SelectShape {
     }
 };
 
-// What query i of sequence b sees (as in pool_attention.cuh).
+// What query i of sequence b sees (as in pool_attention.cuh).  (The kernel waits for those before it by itself: no read-only loads here and below.)
 __device__ __forceinline__ int select_tokens(const skv_pool_select_args& a, int b) {
-    const int64_t n = __ldg(a.lengths + b), cap = (int64_t)a.table_width * a.page_size;
+    const int64_t n = a.lengths[b], cap = (int64_t)a.table_width * a.page_size;
     return (int)max((int64_t)0, min(n, min(cap, (int64_t)0x7fffff00)));
 }
 __device__ __forceinline__ int select_pages(const skv_pool_select_args& a, const SelectShape& shape, int b, int i, int tokens) {
-    const int fresh = a.new_lengths ? __ldg(a.new_lengths + b) : a.S_q;
+    const int fresh = a.new_lengths ? a.new_lengths[b] : a.S_q;
     return shape.pages_of(i >= fresh ? 0 : a.causal ? max(0, tokens - fresh + 1 + i) : tokens);
 }
 
@@ -384,7 +384,7 @@ __device__ __forceinline__ void score_pages(const skv_pool_select_args& a, const
                                          : ((min(shape.block_tokens, a.S_q - i0) << log_span) + 7) / 8;
         int ahead[2];                                             // numbers of the pages that are loaded next
 #pragma unroll
-        for (int r = 0; r < 2; ++r) ahead[r] = p_first + g + 8 * r < pages ? __ldg(table + p_first + g + 8 * r) : -1;
+        for (int r = 0; r < 2; ++r) ahead[r] = p_first + g + 8 * r < pages ? table[p_first + g + 8 * r] : -1;
         if (first > 0) __syncthreads();
         bool laid_out = false;
 #pragma unroll 1
@@ -397,15 +397,15 @@ __device__ __forceinline__ void score_pages(const skv_pool_select_args& a, const
                 const int j = p0 + g + 8 * r, page = ahead[r];
                 named[r] = j < pages && page >= 0 && page < a.num_pages;
                 if (j < pages && !named[r] && a.error_flag) atomicExch(a.error_flag, 1);
-                ahead[r] = j + p_step < pages ? __ldg(table + j + p_step) : -1;
+                ahead[r] = j + p_step < pages ? table[j + p_step] : -1;
                 // (page 0 in place of none, the row's first bytes in place of those behind it: loads without a branch that waits for
                 // them; their scores are not used, the queries are zero there)
                 const int64_t at = named[r] ? (int64_t)page * H + h : 0;
                 const int8_t* row = a.bounds + at * (2 * D);
-                step[r] = __ldg(a.steps + at);
+                step[r] = a.steps[at];
 #pragma unroll
                 for (int s = 0; s < SEGS; ++s)
-                    y[r][s] = __ldg(reinterpret_cast<const uint4*>(row + (64 * s + 16 * c < 2 * D ? 64 * s + 16 * c : 0)));
+                    y[r][s] = *reinterpret_cast<const uint4*>(row + (64 * s + 16 * c < 2 * D ? 64 * s + 16 * c : 0));
             }
             if (!laid_out) {
                 laid_out = true;
@@ -487,16 +487,16 @@ __device__ __forceinline__ void score_pages_any(const skv_pool_select_args& a, c
         }
         __syncthreads();
         for (int j = rank * kSelectWarps + warp; j < pages; j += shape.blocks * kSelectWarps) {
-            const int page = __ldg(a.block_table + b * a.table_stride + j);
+            const int page = a.block_table[b * a.table_stride + j];
             const bool named = page >= 0 && page < a.num_pages;
             if (!named && lane == 0 && a.error_flag) atomicExch(a.error_flag, 1);
             const int64_t at = named ? (int64_t)page * H + h : 0;
             int sum = 0;
             if (named)
-                for (int d = lane; d < 2 * D; d += 32) sum += (int)s_q[d] * (int)__ldg(a.bounds + at * 2 * D + d);
+                for (int d = lane; d < 2 * D; d += 32) sum += (int)s_q[d] * (int)a.bounds[at * 2 * D + d];
             sum = __reduce_add_sync(0xffffffffu, sum);
             if (lane == 0) {
-                const uint32_t key = named ? score_key((float)sum, *s_t, __ldg(a.steps + at)) : 1;
+                const uint32_t key = named ? score_key((float)sum, *s_t, a.steps[at]) : 1;
                 keys[(int64_t)i * pitch + j] = head == 0 ? key : max(key, keys[(int64_t)i * pitch + j]);
             }
         }
@@ -541,7 +541,7 @@ __device__ __forceinline__ void choose_pages(SelectShared& s, const uint32_t* gl
     uint32_t least = 0xffffffffu, most = 0;
 #pragma unroll 4
     for (int j = lo + tid; j < hi; j += THREADS) {
-        const uint32_t x = __ldcg(global + j);
+        const uint32_t x = global[j];
         if (kept) s.keys[w0 * KEYS + j - lo] = x;
         least = min(least, x);
         most = max(most, x);
@@ -717,7 +717,7 @@ __global__ void __launch_bounds__(kSelectThreads, SEGS == 8 ? 1 : 2) page_select
             __syncthreads();
         }
     }
-    if (tid == 0 && a.error_flag && __ldg(a.lengths + b) != tokens) atomicExch(a.error_flag, 1);
+    if (tid == 0 && a.error_flag && a.lengths[b] != tokens) atomicExch(a.error_flag, 1);
     const bool by_warp = i1 - i0 > 2 * shape.blocks && pages <= kSelectKeys / kSelectWarps;
     const int one_of = by_warp ? shape.blocks * kSelectWarps : shape.blocks, first_of = by_warp ? rank * kSelectWarps + warp : rank;
     for (int i = i0 + first_of; i < i1; i += one_of) {

@@ -124,7 +124,8 @@ __device__ __forceinline__ int quant_value_fast(float x, float scale, float rcp,
 }
 
 // A launch whose blocks may be set up while the kernel before it on the stream still runs (which allows it by start_dependents); it
-// reads what that kernel writes only after wait_for_dependency.  (A launch's latency of 2 to 3 us is mostly hidden.)
+// reads what that kernel, or one before it, writes only after wait_for_dependency, and not by read-only loads (__ldg), which the compiler may
+// move before it.  (A launch's latency of 2 to 3 us is mostly hidden.)
 template <class... Params, class... Args>
 inline void launch_cluster_after(void (*kernel)(Params...), dim3 grid, dim3 cluster, unsigned threads, size_t smem, cudaStream_t st, const Args&... args) {
     cudaLaunchConfig_t config = {};

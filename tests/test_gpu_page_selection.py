@@ -495,6 +495,35 @@ def test_sparse_calls_from_two_threads_on_one_stream(skv):
     assert not wrong
 
 
+def test_calls_that_start_early_read_what_was_written_last(skv):
+    """Inputs change in place behind a slow kernel, and a choice of pages, behind which the next calls are set up early, stands between."""
+    gen = _gen(30)
+    counts, H, D, P, keep = [700, 333, 512], 2, 64, 16, 9
+    pages_kv, scales, table, lens = _filled(skv, "fp16", counts, H, P, D, 16, 7)
+    bounds, steps = skv.page_bounds(pages_kv[0], table, lens)
+    q, other = torch.randn(2, 3, 2 * H, 1, D, generator=gen, device="cuda")
+    logits, scores, lengths = torch.zeros(2, 4, 5003, device="cuda"), torch.zeros(2, 4, device="cuda"), lens.clone()
+    slow = torch.randn(4096, 4096, generator=gen, device="cuda")
+
+    def calls():
+        skv.page_select(other, bounds, steps, table, lens, P, keep)
+        beams = skv.beam_select(logits, scores, 7)
+        skv.page_select(other, bounds, steps, table, lens, P, keep)
+        chosen = skv.page_select(q, bounds, steps, table, lengths, P, keep)
+        return [*beams, chosen, skv.paged_attention(q, *pages_kv, table, lengths, pages=chosen)]
+
+    for _ in range(20):
+        new = torch.randn(2, 4, 5003, generator=gen, device="cuda"), torch.randn(2, 4, generator=gen, device="cuda"), \
+            lens - torch.randint(300, (3,), generator=gen, device="cuda", dtype=torch.int32), torch.randn(q.shape, generator=gen, device="cuda")
+        torch.cuda.synchronize()
+        slow @ slow
+        for to, x in zip((logits, scores, lengths, q), new):
+            to.copy_(x)
+        got = calls()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, calls()))
+
+
 def test_two_graphs_do_not_share_workspaces(skv):
     """Graphs captured on one stream and replayed on two."""
     made = []
