@@ -574,8 +574,8 @@ typedef struct skv_beam_args {
 } skv_beam_args;                 /* 104 bytes */
 
 /* The keep <= 128 best of the beams * V continuations of each of B searches, best first, ties to the lowest beam, then
- * token: scores[b, r] + log softmax(logits[b, r])[token], compared in 64 bits.  The exponentials are 32-bit numbers: a row's log sum is up to
- * 2^-20 off, by the same for equal rows of a call wherever they begin.  A finished beam
+ * token: scores[b, r] + log softmax(logits[b, r])[token], compared in 64 bits, and a beam's own continuations by their logits.  The
+ * exponentials are 32-bit numbers: a row's log sum is up to 2^-19 off, by the same for equal rows of a call wherever they begin.  A finished beam
  * has one continuation, pad_token, at its score.  A NaN logit counts as -inf; logits of +inf share their beam's whole
  * probability.  A beam whose score is -inf, NaN or +inf, or whose logits are all -inf, has continuations of -inf only.
  * keep <= beams * V; beams <= 4096.  scratch: skv_beam_scratch_bytes bytes, 16-byte aligned. */

@@ -37,7 +37,7 @@ def beam_select(
     ``logits`` ``[B, beams, V]`` (fp32, fp16 or bf16, other types as fp32; any strides over the first two dimensions) are those of each beam's next
     token, ``scores`` ``[B, beams]`` the beams' log-probabilities so far.  A continuation scores
     ``scores[b, r] + log_softmax(logits[b, r])[token]``; scores are compared in 64 bits, a beam's own continuations by their logits, and
-    ties go to the lowest beam, then to the lowest token.  A row's exponentials are 32-bit numbers, so the logarithm of their sum is up to 2^-20 off,
+    ties go to the lowest beam, then to the lowest token.  A row's exponentials are 32-bit numbers, so the logarithm of their sum is up to 2^-19 off,
     by the same for equal rows of a call: their continuations tie, others of different beams that are nearer than that may change places.
     ``parents`` and ``tokens`` are int64, the new scores float32.  ``keep`` (at most 128)
     defaults to the number of beams; a search that sets beams aside as they end wants twice as many.
