@@ -220,11 +220,15 @@ int launch_any(const skv_pool_attention_args& a, cudaStream_t st) {
     }
 }
 
-// The tensor-core kernels (pool_attention_mma.cuh), one translation unit a precision.
+// The tensor-core kernels (pool_attention_mma.cuh), one translation unit a precision, of whole sequences and of lists of pages.
 int attend_fp32(const skv_pool_attention_args& a, cudaStream_t st);
 int attend_fp16(const skv_pool_attention_args& a, cudaStream_t st);
 int attend_int8(const skv_pool_attention_args& a, cudaStream_t st);
 int attend_int4(const skv_pool_attention_args& a, cudaStream_t st);
+int attend_listed_fp32(const skv_pool_attention_args& a, cudaStream_t st);
+int attend_listed_fp16(const skv_pool_attention_args& a, cudaStream_t st);
+int attend_listed_int8(const skv_pool_attention_args& a, cudaStream_t st);
+int attend_listed_int4(const skv_pool_attention_args& a, cudaStream_t st);
 
 // The tcgen05 kernel (pool_attention_tc.cuh), and the query rows a key head from which it is taken.  The lengths are on the device,
 // so the rule cannot look at them; it is set by long sequences, and short ones lose a few us by it.  8 key heads of 128
@@ -304,8 +308,15 @@ int attend(const skv_pool_attention_args& a, cudaStream_t st) {
     if (a.reserved < 0 && (!mma || many))
         if (const int rc = launch_tables(*static_cast<const AttentionCall&>(a).lists, st)) return rc;
     if (many) return attend_many(a, st);
-    if (mma)
-        return a.pool.precision == 0 ? attend_fp32(a, st) : a.pool.precision == 1 ? attend_fp16(a, st) : a.pool.precision == 2 ? attend_int8(a, st) : attend_int4(a, st);
+    if (mma) {
+        const bool listed = a.reserved < 0;
+        switch (a.pool.precision) {
+            case 0: return listed ? attend_listed_fp32(a, st) : attend_fp32(a, st);
+            case 1: return listed ? attend_listed_fp16(a, st) : attend_fp16(a, st);
+            case 2: return listed ? attend_listed_int8(a, st) : attend_int8(a, st);
+            default: return listed ? attend_listed_int4(a, st) : attend_int4(a, st);
+        }
+    }
     if (a.q.dtype == kF32) return launch_any<float>(a, st);
     if (a.q.dtype == kF16) return launch_any<__half>(a, st);
     return launch_any<__nv_bfloat16>(a, st);

@@ -1074,7 +1074,7 @@ int allow_shared(size_t bytes) {
     return e == cudaSuccess ? SKV_OK : fail(SKV_ERR_CUDA, "pool_attention: %s", cudaGetErrorString(e));
 }
 
-template <int PREC, int DP, int NT, int NQ, int NP, bool LIMIT>
+template <int PREC, int DP, int NT, int NQ, int NP, bool LIMIT, bool LISTED>
 int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
     using Shape = MmaShape<PREC, DP, NT>;
     static_assert(Shape::CTAS * 2 * 8 * NT <= kRowsPerSm, "the scratch holds every CTA's slots");
@@ -1093,9 +1093,9 @@ int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
     const bool q_vec = rows_aligned(a.q), out_vec = rows_aligned(a.out);
     const unsigned all = sm_count() * Shape::CTAS, threads = 32 * Shape::W;
     const skv_pool_sparse_args none = {};
-    if constexpr (!LIMIT) if (a.reserved < 0) {   // (a unit is one token)
-        constexpr auto kernel = pool_attention_mma_kernel<PREC, DP, NT, NQ, NP, false, true>;
-        if (const int rc = allow_shared<kernel>(smem)) return rc;
+    constexpr auto kernel = pool_attention_mma_kernel<PREC, DP, NT, NQ, NP, LIMIT, LISTED>;
+    if (const int rc = allow_shared<kernel>(smem)) return rc;
+    if constexpr (LISTED) {
         const skv_pool_sparse_args& lists = *static_cast<const AttentionCall&>(a).lists;
         // Sequences of one head and of known length at most (lists of pages).  Where there are fewer units than CTAs, a unit's tiles are split
         // over those that would be idle; else units stay whole, unless too many CTAs would idle in the last round, where even shares of
@@ -1125,38 +1125,37 @@ int launch_mma(const skv_pool_attention_args& a, cudaStream_t st) {
             launch_after(kernel, dim3(all), threads, smem, st, part, none, row_tiles, magic, exact, q_vec, out_vec);
             return check_launch("pool_attention");
         });
+    } else {
+        return by_sequences(a, step, [&](const skv_pool_attention_args& part) {
+            kernel<<<all, threads, smem, st>>>(part, none, row_tiles, magic, exact, q_vec, out_vec);
+            return check_launch("pool_attention");
+        });
     }
-    constexpr auto kernel = pool_attention_mma_kernel<PREC, DP, NT, NQ, NP, LIMIT, false>;
-    if (const int rc = allow_shared<kernel>(smem)) return rc;
-    return by_sequences(a, step, [&](const skv_pool_attention_args& part) {
-        kernel<<<all, threads, smem, st>>>(part, none, row_tiles, magic, exact, q_vec, out_vec);
-        return check_launch("pool_attention");
-    });
 }
 
-template <int PREC, int DP, int NT, int NQ, int NP>
+template <int PREC, int DP, int NT, int NQ, int NP, bool LISTED>
 int launch_mma_limit(const skv_pool_attention_args& a, cudaStream_t st) {
-    if constexpr (PREC <= 1)
-        if (a.causal && a.S_q > 1) return launch_mma<PREC, DP, NT, NQ, NP, true>(a, st);
-    return launch_mma<PREC, DP, NT, NQ, NP, false>(a, st);
+    if constexpr (PREC <= 1 && !LISTED)   // (a unit of lists is one token)
+        if (a.causal && a.S_q > 1) return launch_mma<PREC, DP, NT, NQ, NP, true, false>(a, st);
+    return launch_mma<PREC, DP, NT, NQ, NP, false, LISTED>(a, st);
 }
 
-template <int PREC, int DP, int NT>
+template <int PREC, int DP, int NT, bool LISTED>
 int launch_mma_type(const skv_pool_attention_args& a, cudaStream_t st) {
-    if (a.q.dtype == kF32) return launch_mma_limit<PREC, DP, NT, 2, 2>(a, st);
-    if (a.q.dtype == kF16) return launch_mma_limit<PREC, DP, NT, 1, 2>(a, st);
-    return launch_mma_limit<PREC, DP, NT, 1, 1>(a, st);
+    if (a.q.dtype == kF32) return launch_mma_limit<PREC, DP, NT, 2, 2, LISTED>(a, st);
+    if (a.q.dtype == kF16) return launch_mma_limit<PREC, DP, NT, 1, 2, LISTED>(a, st);
+    return launch_mma_limit<PREC, DP, NT, 1, 1, LISTED>(a, st);
 }
 
 // Row tiles of 8 or 16 rows.  (32 rows a tile were 10 to 20 % faster where hundreds of rows meet 8 K tokens or more,
 // 212 against 255 us for 1024 rows of 8 key heads, and 1.5 times slower below: 50 against 33 us for 32 rows.)
-template <int PREC>
+template <int PREC, bool LISTED>
 int launch_mma_prec(const skv_pool_attention_args& a, cudaStream_t st) {
     const int R = a.q.heads / a.pool.heads * a.S_q, D = a.pool.head_dim;
-    if (D <= 64) return R <= 8 ? launch_mma_type<PREC, 64, 1>(a, st) : launch_mma_type<PREC, 64, 2>(a, st);
-    if (D <= 128) return R <= 8 ? launch_mma_type<PREC, 128, 1>(a, st) : launch_mma_type<PREC, 128, 2>(a, st);
-    if constexpr (PREC == 0) return launch_mma_type<0, 256, 1>(a, st);   // slots of 32 KB leave no room for more rows
-    else return R <= 8 ? launch_mma_type<PREC, 256, 1>(a, st) : launch_mma_type<PREC, 256, 2>(a, st);
+    if (D <= 64) return R <= 8 ? launch_mma_type<PREC, 64, 1, LISTED>(a, st) : launch_mma_type<PREC, 64, 2, LISTED>(a, st);
+    if (D <= 128) return R <= 8 ? launch_mma_type<PREC, 128, 1, LISTED>(a, st) : launch_mma_type<PREC, 128, 2, LISTED>(a, st);
+    if constexpr (PREC == 0) return launch_mma_type<0, 256, 1, LISTED>(a, st);   // slots of 32 KB leave no room for more rows
+    else return R <= 8 ? launch_mma_type<PREC, 256, 1, LISTED>(a, st) : launch_mma_type<PREC, 256, 2, LISTED>(a, st);
 }
 
 }  // namespace skv
